@@ -42,6 +42,8 @@
  *                       v11/fused_ce.py:98-141  linear_ce_per_token /
  *                                               linear_ce_stats
  *   qpam_ce_bwd         v11/fused_ce.py:56-82   _FusedLinearCE.backward
+ *   qpam_embed_fwd/_bwd v11/complex_ops.py:223-235 ComplexEmbed.forward and its
+ *                       autograd backward (two nn.Embedding gradients)
  *   qpam_prologue_fwd   the elementwise steps of V11PAMLayer between the
  *                       projections and the scan: _project's RoPE / qk-norm
  *                       (v11/model.py:290-305), _gamma_all_and_vprime /
@@ -801,6 +803,39 @@ typedef struct {
 
 size_t qpam_ce_bwd_workspace_size(const qpam_ce_bwd_args *a);
 int qpam_ce_bwd(const qpam_ce_bwd_args *a, void *stream);
+
+/* The complex embedding lookup (ComplexEmbed.forward, v11/complex_ops.py:223-235)
+ * with a scale, and its gradient.
+ *
+ * qpam_embed_fwd: out[i][j] = scale * (re[ids[i]][j], im[ids[i]][j]), out
+ * [n][dim][2] contiguous, in dtype; an id outside [0, V) reads nothing and gives
+ * a row of zeros.  Tables of row strides ld_re, ld_im (elements), unit column
+ * stride, any alignment.
+ * qpam_embed_bwd: d_re[v][j] = scale * sum of dz[i][j][0] over ids[i] == v, d_im
+ * from dz[i][j][1]: fp32 sums in the order of i, rounded once to dtype.  Writes
+ * both contiguous [V][dim] tables (zeros for tokens that do not occur); ids
+ * outside [0, V) or equal to padding_idx give nothing.  dz [n][dim][2]
+ * contiguous.  dz, d_re, d_im and workspace 16-byte aligned. */
+typedef struct {
+    int64_t n;
+    int32_t V, dim;
+    int32_t dtype;
+    int32_t ids_i64;               /* ids are int64 (1) or int32 (0) */
+    const void *ids;
+    int64_t padding_idx;           /* backward; negative: none */
+    float scale;
+    const void *re; int64_t ld_re; /* forward */
+    const void *im; int64_t ld_im;
+    void *out;
+    const void *dz;                /* backward */
+    void *d_re, *d_im;
+    void *workspace;
+    size_t workspace_bytes;
+} qpam_embed_args;
+
+int qpam_embed_fwd(const qpam_embed_args *a, void *stream);
+size_t qpam_embed_bwd_workspace_size(const qpam_embed_args *a);
+int qpam_embed_bwd(const qpam_embed_args *a, void *stream);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ import os
 import torch  # noqa: F401  (must be loaded before the HIP library)
 
 LIB_NAME = "libqpam.so"
-ABI_VERSION = 15
+ABI_VERSION = 16
 _HERE = os.path.dirname(os.path.abspath(__file__))
 
 QPAM_F32 = 0
@@ -255,6 +255,15 @@ class PlanesArgs(ctypes.Structure):
     _fields_ = [("count", c_i32), ("merge", c_i32), ("item", PlanesItem * QPAM_PLANES_MAX)]
 
 
+class EmbedArgs(ctypes.Structure):
+    _fields_ = [
+        ("n", c_i64), ("V", c_i32), ("dim", c_i32), ("dtype", c_i32), ("ids_i64", c_i32), ("ids", c_ptr),
+        ("padding_idx", c_i64), ("scale", c_f32), ("re", c_ptr), ("ld_re", c_i64), ("im", c_ptr), ("ld_im", c_i64),
+        ("out", c_ptr), ("dz", c_ptr), ("d_re", c_ptr), ("d_im", c_ptr), ("workspace", c_ptr),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 SIGNATURES = {
     "qpam_version": (ctypes.c_int, []),
     "qpam_last_error": (ctypes.c_char_p, []),
@@ -278,6 +287,9 @@ SIGNATURES = {
     "qpam_cplx_bwd": (ctypes.c_int, [ctypes.POINTER(CplxArgs), c_ptr]),
     "qpam_resid_norm": (ctypes.c_int, [ctypes.POINTER(ResidNormArgs), c_ptr]),
     "qpam_cgu_mix": (ctypes.c_int, [ctypes.POINTER(CguMixArgs), c_ptr]),
+    "qpam_embed_fwd": (ctypes.c_int, [ctypes.POINTER(EmbedArgs), c_ptr]),
+    "qpam_embed_bwd_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(EmbedArgs)]),
+    "qpam_embed_bwd": (ctypes.c_int, [ctypes.POINTER(EmbedArgs), c_ptr]),
     "qpam_prologue_fwd": (ctypes.c_int, [ctypes.POINTER(PrologueArgs), c_ptr]),
     "qpam_prologue_bwd": (ctypes.c_int, [ctypes.POINTER(PrologueBwdArgs), c_ptr]),
     "qpam_cabs_fwd": (ctypes.c_int, [c_i32, c_i64, c_ptr, c_ptr, c_ptr]),
