@@ -42,6 +42,9 @@
  *                       v11/fused_ce.py:98-141  linear_ce_per_token /
  *                                               linear_ce_stats
  *   qpam_ce_bwd         v11/fused_ce.py:56-82   _FusedLinearCE.backward
+ *   qpam_logprobs_fwd   log-softmax rows, their token entries, entropy and top
+ *   qpam_logprobs_bwd   entries: what V11LM.generate (v11/model.py:1207-1245) has
+ *                       in its softmax and top-k and does not return
  *   qpam_embed_fwd/_bwd v11/complex_ops.py:223-235 ComplexEmbed.forward and its
  *                       autograd backward (two nn.Embedding gradients)
  *   qpam_prologue_fwd   the elementwise steps of V11PAMLayer between the
@@ -836,6 +839,42 @@ typedef struct {
 int qpam_embed_fwd(const qpam_embed_args *a, void *stream);
 size_t qpam_embed_bwd_workspace_size(const qpam_embed_args *a);
 int qpam_embed_bwd(const qpam_embed_args *a, void *stream);
+
+/* Log probabilities of given tokens, entropy and top alternatives of n rows of
+ * logits (dtype, row stride ld elements, unit column stride, any alignment of the
+ * type), and the gradient.  With p = softmax(x / temperature):
+ *   logprobs[i] = ln p[ids[i]]   (0 where ids[i] is ignore_index or outside [0, V))
+ *   entropy[i]  = -sum p ln p
+ *   top_ids[i][0 .. top_k), top_logprobs: the largest entries in descending order,
+ *     equal values by the lower index (NaN above +inf, -0 equal to +0); top_k at
+ *     most 64 and at most V.
+ *   stats[i] = (max x, sum exp((x - max) / temperature)): what the gradient needs
+ *     (optional in the forward).
+ * Entries of -inf have probability 0.  A row of nothing else: log probabilities
+ * -inf, entropy 0, gradient 0.  A row with NaN or +inf: NaN.
+ * qpam_logprobs_bwd: d_logits [n][V] (dtype, row stride ldd) from g_logprobs [n],
+ * g_entropy [n], g_top [n][top_k] (fp32, each optional) and the forward's entropy,
+ * stats and (with g_top) top_ids.  The token's entry gets its term where it is
+ * masked, too; rows without a token get the other terms. */
+typedef struct {
+    int64_t n;
+    int32_t V;
+    int32_t dtype;
+    int32_t top_k;
+    float temperature;
+    const void *logits; int64_t ld;
+    const int64_t *ids;
+    int64_t ignore_index;
+    float *logprobs, *entropy;     /* entropy: read by the backward */
+    float *stats;                  /* [n][2] */
+    float *top_logprobs;           /* [n][top_k] */
+    int64_t *top_ids;              /* [n][top_k] */
+    const float *g_logprobs, *g_entropy, *g_top;
+    void *d_logits; int64_t ldd;
+} qpam_logprobs_args;
+
+int qpam_logprobs_fwd(const qpam_logprobs_args *a, void *stream);
+int qpam_logprobs_bwd(const qpam_logprobs_args *a, void *stream);
 
 #ifdef __cplusplus
 }

@@ -264,6 +264,15 @@ class EmbedArgs(ctypes.Structure):
     ]
 
 
+class LogprobsArgs(ctypes.Structure):
+    _fields_ = [
+        ("n", c_i64), ("V", c_i32), ("dtype", c_i32), ("top_k", c_i32), ("temperature", c_f32), ("logits", c_ptr),
+        ("ld", c_i64), ("ids", c_ptr), ("ignore_index", c_i64), ("logprobs", c_ptr), ("entropy", c_ptr), ("stats", c_ptr),
+        ("top_logprobs", c_ptr), ("top_ids", c_ptr), ("g_logprobs", c_ptr), ("g_entropy", c_ptr), ("g_top", c_ptr),
+        ("d_logits", c_ptr), ("ldd", c_i64),
+    ]
+
+
 SIGNATURES = {
     "qpam_version": (ctypes.c_int, []),
     "qpam_last_error": (ctypes.c_char_p, []),
@@ -287,6 +296,8 @@ SIGNATURES = {
     "qpam_cplx_bwd": (ctypes.c_int, [ctypes.POINTER(CplxArgs), c_ptr]),
     "qpam_resid_norm": (ctypes.c_int, [ctypes.POINTER(ResidNormArgs), c_ptr]),
     "qpam_cgu_mix": (ctypes.c_int, [ctypes.POINTER(CguMixArgs), c_ptr]),
+    "qpam_logprobs_fwd": (ctypes.c_int, [ctypes.POINTER(LogprobsArgs), c_ptr]),
+    "qpam_logprobs_bwd": (ctypes.c_int, [ctypes.POINTER(LogprobsArgs), c_ptr]),
     "qpam_embed_fwd": (ctypes.c_int, [ctypes.POINTER(EmbedArgs), c_ptr]),
     "qpam_embed_bwd_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(EmbedArgs)]),
     "qpam_embed_bwd": (ctypes.c_int, [ctypes.POINTER(EmbedArgs), c_ptr]),

@@ -1,0 +1,155 @@
+"""Log probabilities of given tokens, with entropy and top alternatives.
+
+token_logprobs reads rows of logits (qpam_logprobs_fwd / _bwd): what a serving
+loop reports beside the tokens of ModelDecoder.step, and what policy gradients and
+distillation differentiate.  The reference's V11LM.generate (v11/model.py:1207-1245)
+forms these softmax rows to draw from them and returns none of it.
+"""
+
+import ctypes
+import math
+from typing import List, NamedTuple, Optional
+
+import torch
+from torch import Tensor
+
+from . import _lib, _ops
+
+__all__ = ["TokenLogprobs", "token_logprobs"]
+
+MAX_TOP_K = 64
+
+_CODE = {torch.float32: _lib.QPAM_F32, torch.bfloat16: _lib.QPAM_BF16}
+
+
+class TokenLogprobs(NamedTuple):
+    """logprobs and entropy fp32 in the shape of ids; top_logprobs (fp32) and top_ids
+    (int64) with a last axis of top_k, or None without top_k."""
+    logprobs: Tensor
+    entropy: Tensor
+    top_logprobs: Optional[Tensor] = None
+    top_ids: Optional[Tensor] = None
+
+
+def _check_temperature(temperature, name):
+    if not (0.0 < temperature < math.inf):
+        raise ValueError(f"qpam {name}: temperature {temperature} must be positive and finite")
+
+
+def _check(logits, ids, temperature, top_k):
+    if not (logits.is_cuda and ids.is_cuda and logits.device == ids.device):
+        raise ValueError("qpam token_logprobs: logits and ids must be on one GPU (no CPU path in this library)")
+    if logits.dtype not in _CODE:
+        raise ValueError(f"qpam token_logprobs: logits must be float32 or bfloat16, got {logits.dtype}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"qpam token_logprobs: ids must be int64 or int32, got {ids.dtype}")
+    if logits.dim() < 1 or logits.shape[:-1] != ids.shape or logits.shape[-1] < 1:
+        raise ValueError(f"qpam token_logprobs: logits [..., V] and ids [...] expected, got {tuple(logits.shape)} and "
+                         f"{tuple(ids.shape)}")
+    if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
+        raise ValueError(f"qpam token_logprobs: top_k {top_k} outside 0 .. {min(MAX_TOP_K, logits.shape[-1])}")
+    _check_temperature(temperature, "token_logprobs")
+
+
+def _args(logits, ids, temperature, top_k, ignore_index):
+    a = _lib.LogprobsArgs()
+    a.n, a.V, a.dtype, a.top_k, a.temperature = logits.shape[0], logits.shape[1], _CODE[logits.dtype], top_k, temperature
+    a.logits, a.ld = logits.data_ptr(), max(logits.stride(0), logits.shape[1])
+    a.ids, a.ignore_index = ids.data_ptr(), ignore_index
+    return a
+
+
+def _rows(logits):
+    """[n, V] rows as the kernels read them: unit column stride, rows apart (one row: any stride)."""
+    return logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous()
+
+
+def _forward(logits: Tensor, ids: Tensor, temperature: float, top_k: int, ignore_index: int) -> List[Tensor]:
+    """logits [n, V], ids [n] int64 -> [logprobs, entropy, stats [n, 2], top_logprobs [n, k], top_ids [n, k]]."""
+    x, ids = _rows(logits), ids.contiguous()
+    n, dev = x.shape[0], x.device
+    lp, ent, stats = (torch.empty(s, device=dev, dtype=torch.float32) for s in ((n,), (n,), (n, 2)))
+    top = torch.empty(n, top_k, device=dev, dtype=torch.float32)
+    top_ids = torch.empty(n, top_k, device=dev, dtype=torch.int64)
+    a = _args(x, ids, temperature, top_k, ignore_index)
+    a.logprobs, a.entropy, a.stats = lp.data_ptr(), ent.data_ptr(), stats.data_ptr()
+    a.top_logprobs, a.top_ids = top.data_ptr(), top_ids.data_ptr()
+    with _lib.device(dev):
+        _lib.check(_lib.lib().qpam_logprobs_fwd(ctypes.byref(a), _lib.stream_ptr(dev)), "qpam_logprobs_fwd")
+    return [lp, ent, stats, top, top_ids]
+
+
+logprobs_fwd_op = _ops.op("qpam::logprobs_fwd")(_forward)
+
+
+@logprobs_fwd_op.register_fake
+def _(logits, ids, temperature, top_k, ignore_index):
+    n = logits.shape[0]
+    f = lambda *s: logits.new_empty(s, dtype=torch.float32)  # noqa: E731
+    return [f(n), f(n), f(n, 2), f(n, top_k), logits.new_empty((n, top_k), dtype=torch.int64)]
+
+
+def _gradient(logits: Tensor, ids: Tensor, entropy: Tensor, stats: Tensor, top_ids: Tensor, g_logprobs: Optional[Tensor],
+              g_entropy: Optional[Tensor], g_top: Optional[Tensor], temperature: float, ignore_index: int) -> Tensor:
+    """d logits [n, V] in the logits' dtype."""
+    x, ids = _rows(logits), ids.contiguous()
+    n, V = x.shape
+    out = torch.empty(n, V, device=x.device, dtype=x.dtype)
+    gs = [g if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy, g_top)]
+    a = _args(x, ids, temperature, top_ids.shape[1], ignore_index)
+    a.entropy, a.stats, a.top_ids = entropy.data_ptr(), stats.data_ptr(), top_ids.data_ptr()
+    a.g_logprobs, a.g_entropy, a.g_top = (g if g is None else g.data_ptr() for g in gs)
+    a.d_logits, a.ldd = out.data_ptr(), V
+    with _lib.device(x.device):
+        _lib.check(_lib.lib().qpam_logprobs_bwd(ctypes.byref(a), _lib.stream_ptr(x.device)), "qpam_logprobs_bwd")
+    return out
+
+
+logprobs_bwd_op = _ops.op("qpam::logprobs_bwd")(_gradient)
+
+
+@logprobs_bwd_op.register_fake
+def _(logits, ids, entropy, stats, top_ids, g_logprobs, g_entropy, g_top, temperature, ignore_index):
+    return logits.new_empty(logits.shape)
+
+
+def _setup(ctx, inputs, output):
+    logits, ids, ctx.temperature, ctx.top_k, ctx.ignore_index = inputs
+    ctx.mark_non_differentiable(output[2], output[4])
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(logits, ids, output[1], output[2], output[4])
+
+
+def _backward(ctx, grads):
+    g_lp, g_ent, _, g_top, _ = grads
+    if g_lp is None and g_ent is None and g_top is None:
+        return None, None, None, None, None
+    if not ctx.top_k:
+        g_top = None
+    return logprobs_bwd_op(*ctx.saved_tensors, g_lp, g_ent, g_top, ctx.temperature, ctx.ignore_index), None, None, None, None
+
+
+logprobs_fwd_op.register_autograd(_backward, setup_context=_setup)
+
+
+def token_logprobs(logits: Tensor, ids: Tensor, temperature: float = 1.0, top_k: int = 0,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """Of p = softmax(logits / temperature) in each row: ln p of the given token, the
+    entropy -sum p ln p, and the top_k (0 to 64) largest entries with their ids,
+    equal logits by the lower id.
+
+    logits [..., V] float32 or bfloat16 (rows of any stride), ids [...] int64 or
+    int32.  A row whose id is ignore_index or outside [0, V) has log probability 0
+    and its entropy and alternatives.  Logits of -inf are masked: probability 0; a
+    row of nothing else has log probabilities -inf, entropy 0 and no gradient.  A
+    row with NaN or +inf gives NaN.  Statistics are fp32.  Differentiable in
+    logits through logprobs, entropy and top_logprobs (once: a second derivative
+    raises); the gradient has the logits' dtype."""
+    _check(logits, ids, temperature, top_k)
+    V = logits.shape[-1]
+    lp, ent, _, top, top_ids = logprobs_fwd_op(logits.reshape(-1, V), ids.reshape(-1).long(), float(temperature), top_k,
+                                               ignore_index)
+    shape = ids.shape
+    if not top_k:
+        return TokenLogprobs(lp.view(shape), ent.view(shape))
+    return TokenLogprobs(lp.view(shape), ent.view(shape), top.view(*shape, top_k), top_ids.view(*shape, top_k))

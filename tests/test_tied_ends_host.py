@@ -11,7 +11,7 @@ from qllm2_amd import _lib
 from test_abi import _header_struct_fields
 
 
-@pytest.mark.parametrize("cname,pyname", [("qpam_embed_args", "EmbedArgs")])
+@pytest.mark.parametrize("cname,pyname", [("qpam_embed_args", "EmbedArgs"), ("qpam_logprobs_args", "LogprobsArgs")])
 def test_ctypes_structs_match_header(cname, pyname):
     assert [f[0] for f in getattr(_lib, pyname)._fields_] == _header_struct_fields(cname)
 
@@ -83,3 +83,65 @@ def test_embedding_fake_kernels():
         assert z.shape == (2, 5, 6, 2) and z.dtype == torch.bfloat16 and z.device.type == "cuda"
         for g in embed_bwd_op(ids, torch.empty_like(z), 9, 2.0, 0):
             assert g.shape == (9, 6) and g.dtype == torch.bfloat16
+
+
+def test_token_logprobs_refusals():
+    from qllm2_amd.token_logprobs import _check, token_logprobs
+    with pytest.raises(ValueError, match="GPU"):
+        token_logprobs(torch.zeros(2, 5), torch.zeros(2, dtype=torch.long))
+    with FakeTensorMode():
+        c = lambda *s, **k: torch.empty(*s, device="cuda", **k)  # noqa: E731
+        x, ids = c(4, 9), c(4, dtype=torch.long)
+        for args, what in [
+            ((c(4, 9, dtype=torch.float16), ids, 1.0, 0), "float32 or bfloat16"),
+            ((c(4, 9, dtype=torch.float64), ids, 1.0, 0), "float32 or bfloat16"),
+            ((x, c(4), 1.0, 0), "int64 or int32"),
+            ((x, c(5, dtype=torch.long), 1.0, 0), "ids"),
+            ((x, c(4, 1, dtype=torch.long), 1.0, 0), "ids"),
+            ((c(4, 0), ids, 1.0, 0), "ids"),
+            ((x, ids, 1.0, 10), "top_k"), ((x, ids, 1.0, -1), "top_k"), ((c(4, 100), ids, 1.0, 65), "top_k"),
+            ((x, ids, 0.0, 0), "temperature"), ((x, ids, -1.0, 0), "temperature"),
+            ((x, ids, float("inf"), 0), "temperature"), ((x, ids, float("nan"), 0), "temperature"),
+        ]:
+            with pytest.raises(ValueError, match=what):
+                _check(*args)
+
+
+def test_token_logprobs_entry_errors_without_gpu():
+    lib = _lib.lib()
+
+    def err(fn, **kw):
+        a = _lib.LogprobsArgs()
+        a.n, a.V, a.dtype, a.top_k, a.temperature, a.ld, a.ldd = 4, 10, _lib.QPAM_F32, 0, 1.0, 10, 10
+        a.logits = a.ids = a.logprobs = a.entropy = a.stats = a.d_logits = 4096
+        for k, v in kw.items():
+            setattr(a, k, v)
+        assert getattr(lib, fn)(ctypes.byref(a), None) == _lib.QPAM_ERR_ARG
+        return lib.qpam_last_error().decode()
+
+    for fn in ("qpam_logprobs_fwd", "qpam_logprobs_bwd"):
+        assert "dtype" in err(fn, dtype=3)
+        assert "sizes" in err(fn, V=0) and "sizes" in err(fn, n=-1)
+        for t in (0.0, -1.0, float("inf"), float("nan")):
+            assert "temperature" in err(fn, temperature=t)
+        assert "top_k" in err(fn, top_k=11) and "top_k" in err(fn, top_k=65, V=100)
+        assert "stride" in err(fn, ld=9) and "null" in err(fn, ids=None)
+        assert "aligned" in err(fn, logits=4098)
+    assert "null output" in err("qpam_logprobs_fwd", top_k=3)
+    assert "stats" in err("qpam_logprobs_bwd", stats=None) and "stride" in err("qpam_logprobs_bwd", ldd=5)
+    assert "g_top" in err("qpam_logprobs_bwd", g_top=4096)
+    assert "aligned" in err("qpam_logprobs_bwd", d_logits=4097)
+
+
+def test_token_logprobs_fake_kernels():
+    from qllm2_amd.token_logprobs import logprobs_bwd_op, token_logprobs
+    with FakeTensorMode():
+        x = torch.empty(3, 4, 50, device="cuda", dtype=torch.bfloat16)
+        ids = torch.empty(3, 4, device="cuda", dtype=torch.int32)
+        r = token_logprobs(x, ids, top_k=6)
+        assert [tuple(t.shape) for t in r] == [(3, 4), (3, 4), (3, 4, 6), (3, 4, 6)]
+        assert r.top_ids.dtype == torch.int64 and r.top_logprobs.dtype == torch.float32
+        f = torch.empty(12, device="cuda")
+        d = logprobs_bwd_op(x.view(12, 50), ids.view(12).long(), f, torch.empty(12, 2, device="cuda"),
+                            r.top_ids.view(12, 6), f, None, None, 1.0, -100)
+        assert d.shape == (12, 50) and d.dtype == torch.bfloat16
