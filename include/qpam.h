@@ -876,6 +876,36 @@ typedef struct {
 int qpam_logprobs_fwd(const qpam_logprobs_args *a, void *stream);
 int qpam_logprobs_bwd(const qpam_logprobs_args *a, void *stream);
 
+/* qpam_logprobs_fwd's logprobs, entropy and stats of the rows x = h w^T / temperature
+ * (h [N][D], w [V][D] as qpam_ce_fwd's) without logits in memory, and the gradient:
+ * the tied LM head's token scores (logits of V11LM.ce_from_lm, v11/model.py:1175-1190).
+ * bf16 operands: fp32 sums of exact products; the gradient's dx is rounded to bf16
+ * between the tiles and the two products dh = dx w, dw = dx^T h.  D a multiple of 32;
+ * h and w as qpam_ce_fwd takes them.  chunk bounds the backward's memory as
+ * qpam_ce_bwd's does; dw_out 1: dw in dtype, 2: dw in fp32 (both written). */
+typedef struct {
+    int32_t N, V, D;
+    int32_t dtype;
+    const void *h; int64_t ldh;
+    const void *w; int64_t ldw;
+    const int64_t *ids;
+    int64_t ignore_index;
+    float temperature;
+    float *logprobs;               /* forward */
+    float *entropy, *stats;        /* written by the forward, read by the backward */
+    const float *g_logprobs, *g_entropy; /* each optional */
+    void *dh; int64_t lddh;
+    void *dw; int64_t lddw;
+    int32_t chunk, dw_out;
+    void *workspace;
+    size_t workspace_bytes;
+} qpam_linear_logprobs_args;
+
+size_t qpam_linear_logprobs_fwd_workspace_size(const qpam_linear_logprobs_args *a);
+int qpam_linear_logprobs_fwd(const qpam_linear_logprobs_args *a, void *stream);
+size_t qpam_linear_logprobs_bwd_workspace_size(const qpam_linear_logprobs_args *a);
+int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -273,6 +273,16 @@ class LogprobsArgs(ctypes.Structure):
     ]
 
 
+class LinearLogprobsArgs(ctypes.Structure):
+    _fields_ = [
+        ("N", c_i32), ("V", c_i32), ("D", c_i32), ("dtype", c_i32),
+        ("h", c_ptr), ("ldh", c_i64), ("w", c_ptr), ("ldw", c_i64), ("ids", c_ptr), ("ignore_index", c_i64),
+        ("temperature", c_f32), ("logprobs", c_ptr), ("entropy", c_ptr), ("stats", c_ptr),
+        ("g_logprobs", c_ptr), ("g_entropy", c_ptr), ("dh", c_ptr), ("lddh", c_i64), ("dw", c_ptr), ("lddw", c_i64),
+        ("chunk", c_i32), ("dw_out", c_i32), ("workspace", c_ptr), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 SIGNATURES = {
     "qpam_version": (ctypes.c_int, []),
     "qpam_last_error": (ctypes.c_char_p, []),
@@ -298,6 +308,10 @@ SIGNATURES = {
     "qpam_cgu_mix": (ctypes.c_int, [ctypes.POINTER(CguMixArgs), c_ptr]),
     "qpam_logprobs_fwd": (ctypes.c_int, [ctypes.POINTER(LogprobsArgs), c_ptr]),
     "qpam_logprobs_bwd": (ctypes.c_int, [ctypes.POINTER(LogprobsArgs), c_ptr]),
+    "qpam_linear_logprobs_fwd_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LinearLogprobsArgs)]),
+    "qpam_linear_logprobs_fwd": (ctypes.c_int, [ctypes.POINTER(LinearLogprobsArgs), c_ptr]),
+    "qpam_linear_logprobs_bwd_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(LinearLogprobsArgs)]),
+    "qpam_linear_logprobs_bwd": (ctypes.c_int, [ctypes.POINTER(LinearLogprobsArgs), c_ptr]),
     "qpam_embed_fwd": (ctypes.c_int, [ctypes.POINTER(EmbedArgs), c_ptr]),
     "qpam_embed_bwd_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(EmbedArgs)]),
     "qpam_embed_bwd": (ctypes.c_int, [ctypes.POINTER(EmbedArgs), c_ptr]),

@@ -19,6 +19,13 @@
 // and H^T transposed once into the workspace).  The G buffers hold `chunk`
 // rows, the reference's own memory bound (it keeps chunk x V fp32 logits and
 // softmax alive).
+//
+// Token scores (SCORES variants of the same kernels; qpam_linear_logprobs_*): the
+// log probability of each row's token and the entropy of the row.  With u = (x -
+// max) / T in units of log2 the tiles also reduce t = sum 2^u u, so that
+//   log prob = (x_token - max) / T - ln s,   entropy = ln s - ln2 t / s,
+// and the gradient tiles write
+//   G_v = -p_v / T (g_lp + g_ent (ln p_v + entropy)) + [v = token] g_lp / T.
 #include <algorithm>
 
 #include "blas.h"
@@ -135,19 +142,37 @@ __device__ __forceinline__ void gemm_tile(const T *A, int64_t lda, int a_rows, c
 }
 
 // ------------------------------------------------------------ forward -----
+constexpr float LN2 = 0.6931471805599453f, LOG2 = 1.4426950408889634f;
+// u of a logit that is -inf or far below the maximum: 2^u is 0 and 2^u u is -0, not NaN
+constexpr float U_FLOOR = -1e4f;
+
 struct FwdParams {
     qpam_ce_fwd_args a;
     int n_vt;
     float *part_m, *part_s;  // [N][n_vt]
     int *part_i;             // [N][n_vt] argmax
     float *red;              // [2] loss sum, denominator
+    // token scores
+    float *part_t;           // [N][n_vt] sum of 2^u u, in part_i's place
+    float inv_t, c;          // 1 / T, log2(e) / T
+    float *logprobs, *entropy, *stats;
 };
 
-template <typename T>
+// (m, s, t) of two parts of a row's logits as one
+__device__ __forceinline__ void join_scores(float &m, float &s, float &t, float om, float os, float ot, float c) {
+    const float nm = fmaxf(m, om), lo = fmaxf(nm, -3.402823466e38f);
+    const float g = fmaxf((m - lo) * c, U_FLOOR), og = fmaxf((om - lo) * c, U_FLOOR);
+    const float f = __builtin_amdgcn_exp2f(g), of = __builtin_amdgcn_exp2f(og);
+    t = f * (t + s * g) + of * (ot + os * og);
+    s = f * s + of * os;
+    m = nm;
+}
+
+template <typename T, bool SCORES>
 __global__ void __launch_bounds__(THREADS) ce_fwd_tile_kernel(FwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     T *smem = reinterpret_cast<T *>(smem_raw);
-    __shared__ float sM[2][BM], sS[2][BM];
+    __shared__ float sM[2][BM], sS[2][BM], sT[2][SCORES ? BM : 1];
     __shared__ int sI[2][BM];
     const qpam_ce_fwd_args &a = p.a;
     const int vt = blockIdx.x, rt = blockIdx.y;
@@ -176,23 +201,43 @@ __global__ void __launch_bounds__(THREADS) ce_fwd_tile_kernel(FwdParams p) {
                 const int oi = __shfl_xor(ix, off);
                 if (om > mx || (om == mx && oi < ix)) { mx = om; ix = oi; }
             }
-            float s = 0.f;
+            float s = 0.f, t = 0.f;
+            const float lo = fmaxf(mx, -3.402823466e38f);
 #pragma unroll
             for (int ni = 0; ni < 4; ++ni) {
                 const int v = v0 + 64 * wn + 16 * ni + l16;
-                if (v < a.V) s += __expf(acc[mi][ni][r] - mx);
+                if (!SCORES) {
+                    if (v < a.V) s += __expf(acc[mi][ni][r] - mx);
+                } else if (v < a.V) {
+                    const float u = (acc[mi][ni][r] - lo) * p.c, e = __builtin_amdgcn_exp2f(u);
+                    s += e;
+                    t += e * fmaxf(u, U_FLOOR);
+                }
             }
 #pragma unroll
             for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off);
+            if (SCORES) t = row16_sum(t);
             if (l16 == 0) {
                 const int row = 64 * wm + 16 * mi + 4 * g + r;
                 sM[wn][row] = mx;
                 sS[wn][row] = s;
-                sI[wn][row] = ix;
+                if (SCORES) sT[wn][row] = t;
+                else sI[wn][row] = ix;
             }
         }
     }
     __syncthreads();
+    if (SCORES) {
+        if (tid < BM && r0 + tid < a.N) {
+            float m = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
+            join_scores(m, s, t, sM[1][tid], sS[1][tid], sT[1][tid], p.c);
+            const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
+            p.part_m[o] = m;
+            p.part_s[o] = s;
+            p.part_t[o] = t;
+        }
+        return;
+    }
     if (tid < BM && r0 + tid < a.N) {
         const float m0 = sM[0][tid], m1 = sM[1][tid];
         const float m = fmaxf(m0, m1);
@@ -255,6 +300,40 @@ __global__ void __launch_bounds__(THREADS) ce_fwd_finalize_kernel(FwdParams p) {
     }
 }
 
+// one wave per row: merge the vocab tiles into (max, s, t), add the token's logit
+template <typename T>
+__global__ void __launch_bounds__(THREADS) scores_finalize_kernel(FwdParams p) {
+    const qpam_ce_fwd_args &a = p.a;
+    const int lane = threadIdx.x & 63;
+    const int row = blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6);
+    if (row >= a.N) return;
+    const int64_t id = a.targets[row];
+    const bool valid = id != a.ignore_index && id >= 0 && id < a.V;
+    float m = -INFINITY, s = 0.f, t = 0.f;
+    for (int vt = lane; vt < p.n_vt; vt += 64) {
+        const int64_t o = (int64_t)row * p.n_vt + vt;
+        join_scores(m, s, t, p.part_m[o], p.part_s[o], p.part_t[o], p.c);
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1)
+        join_scores(m, s, t, __shfl_xor(m, off), __shfl_xor(s, off), __shfl_xor(t, off), p.c);
+    float dot = 0.f;
+    if (valid) {
+        const T *hr = (const T *)a.h + (int64_t)row * a.ldh;
+        const T *wr = (const T *)a.w + id * a.ldw;
+        for (int k = lane; k < a.D; k += 64) dot += Elem<T>::load(hr + k) * Elem<T>::load(wr + k);
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) dot += __shfl_xor(dot, off);
+    if (lane == 0) {
+        const float ln_s = logf(s);
+        p.logprobs[row] = valid ? (dot - m) * p.inv_t - ln_s : 0.f;
+        p.entropy[row] = ln_s - LN2 * (t / s);
+        p.stats[2 * row] = m;
+        p.stats[2 * row + 1] = s;
+    }
+}
+
 // deterministic single-block sum: red[0] = sum loss, red[1] = denominator
 __global__ void __launch_bounds__(1024) ce_reduce_kernel(FwdParams p) {
     const qpam_ce_fwd_args &a = p.a;
@@ -302,7 +381,26 @@ struct BwdParams {
     void *gtbuf;     // [Vp][Rp]
     void *ht;        // [D][Rp]
     int write_g;     // bf16 path: also write G (only the hand-written dH GEMM reads it)
+    // token scores
+    float inv_t, c;  // 1 / T, log2(e) / T
+    const float *stats, *entropy, *g_logprobs, *g_entropy;
 };
+
+// A row's part of G_v = k 2^u (base + slope u) + [v = tgt] extra, u = (x - m) c
+struct RowScore {
+    float m, k, base, slope, extra;
+    int tgt;
+};
+
+__device__ __forceinline__ RowScore row_score(const BwdParams &p, int row) {
+    const qpam_ce_bwd_args &a = p.a;
+    const int64_t id = a.targets[row];
+    const bool valid = id != a.ignore_index && id >= 0 && id < a.V;
+    const float s = p.stats[2 * row + 1];
+    const float g_lp = valid && p.g_logprobs ? p.g_logprobs[row] : 0.f, g_ent = p.g_entropy ? p.g_entropy[row] : 0.f;
+    return {p.stats[2 * row], -p.inv_t / s, g_lp + g_ent * (p.entropy[row] - logf(s)), g_ent * LN2, g_lp * p.inv_t,
+            valid ? (int)id : -1};
+}
 
 // out[c][r] = in[r][c] for an R x Cc tile grid (64 x 64 LDS tiles); rows >= R
 // and cols >= Cc of the (padded) output are written as zero.
@@ -329,11 +427,12 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ unsigned short from_f32<unsigned short>(float x) { return f32_to_bf16(x); }
 
 // G tile: recompute logits, G = (exp(x - lse) - [v == t]) * scale; write G and G^T
-template <typename T>
+template <typename T, bool SCORES>
 __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     T *smem = reinterpret_cast<T *>(smem_raw);
     __shared__ float sLse[BM], sScale[BM];
+    __shared__ float sBase[SCORES ? BM : 1], sSlope[SCORES ? BM : 1], sExtra[SCORES ? BM : 1];
     __shared__ int sTgt[BM];
     const qpam_ce_bwd_args &a = p.a;
     const int vt = blockIdx.x, rt = blockIdx.y;
@@ -343,7 +442,15 @@ __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
         const int lr = lr0 + tid, row = p.row0 + lr;
         float lse = 0.f, sc = 0.f;
         int tg = -1;
-        if (lr < p.rows) {
+        if (SCORES) {
+            const RowScore q = lr < p.rows ? row_score(p, row) : RowScore{};
+            lse = q.m;
+            sc = q.k;
+            tg = lr < p.rows ? q.tgt : -1;
+            sBase[tid] = q.base;
+            sSlope[tid] = q.slope;
+            sExtra[tid] = q.extra;
+        } else if (lr < p.rows) {
             const int64_t t = a.targets[row];
             const bool valid = (t != a.ignore_index) && t >= 0 && t < a.V;
             lse = a.lse[row];
@@ -371,7 +478,13 @@ __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
             for (int r = 0; r < 4; ++r) {
                 const int rl = 64 * wm + 16 * mi + 4 * g + r;
                 float x = 0.f;
-                if (v < a.V && sScale[rl] != 0.f) {
+                if (SCORES) {
+                    if (v < a.V && lr0 + rl < p.rows) {
+                        const float u = (acc[mi][ni][r] - sLse[rl]) * p.c;
+                        x = sScale[rl] * __builtin_amdgcn_exp2f(u) * (sBase[rl] + sSlope[rl] * fmaxf(u, U_FLOOR));
+                        if (v == sTgt[rl]) x += sExtra[rl];
+                    }
+                } else if (v < a.V && sScale[rl] != 0.f) {
                     x = __expf(acc[mi][ni][r] - sLse[rl]);
                     if (v == sTgt[rl]) x -= 1.f;
                     x *= sScale[rl];
@@ -968,10 +1081,10 @@ __device__ __forceinline__ void wave_lds_sync() {
 // Row statistics over a wave's 128 columns: per lane over its 8 columns, then
 // across the 16 lanes that hold the row (DPP); the argmax (first column at the
 // maximum) only when accuracy counts are requested.
-template <bool ARGMAX>
+template <bool ARGMAX, bool SCORES>
 __global__ void __launch_bounds__(WTHREADS) fwd_tile_kernel(FwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    __shared__ float sM[2][TM], sS[2][TM];
+    __shared__ float sM[2][TM], sS[2][TM], sT[2][SCORES ? TM : 1];
     __shared__ int sI[2][TM];
     const qpam_ce_fwd_args &a = p.a;
     const int n_rt = (a.N + TM - 1) / TM;
@@ -1001,9 +1114,19 @@ __global__ void __launch_bounds__(WTHREADS) fwd_tile_kernel(FwdParams p) {
             for (int ni = 0; ni < 8; ++ni)
                 if (full || vl + 16 * ni < a.V) lm = fmaxf(lm, acc[mi][ni][r]);
             const float mx = row16_max(lm);
-            float s = 0.f;
+            float s = 0.f, t = 0.f;
             int ix = 0x7fffffff;
-            if (mx > -INFINITY) {
+            if (SCORES) {
+                const float lo = fmaxf(mx, -3.402823466e38f);
+#pragma unroll
+                for (int ni = 0; ni < 8; ++ni)
+                    if (full || vl + 16 * ni < a.V) {
+                        const float u = (acc[mi][ni][r] - lo) * p.c, e = __builtin_amdgcn_exp2f(u);
+                        s += e;
+                        t += e * fmaxf(u, U_FLOOR);
+                    }
+                t = row16_sum(t);
+            } else if (mx > -INFINITY) {
                 const float mx2 = mx * LOG2E;  // exp(x - mx) = exp2(x log2e - mx log2e)
 #pragma unroll
                 for (int ni = 0; ni < 8; ++ni)
@@ -1019,11 +1142,23 @@ __global__ void __launch_bounds__(WTHREADS) fwd_tile_kernel(FwdParams p) {
                 const int row = 64 * wm + 16 * mi + 4 * g + r;
                 sM[wn][row] = mx;
                 sS[wn][row] = s;
+                if (SCORES) sT[wn][row] = t;
                 if (ARGMAX) sI[wn][row] = ix;
             }
         }
     }
     __syncthreads();
+    if (SCORES) {
+        if (tid < TM && r0 + tid < a.N) {
+            float m = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
+            join_scores(m, s, t, sM[1][tid], sS[1][tid], sT[1][tid], p.c);
+            const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
+            p.part_m[o] = m;
+            p.part_s[o] = s;
+            p.part_t[o] = t;
+        }
+        return;
+    }
     if (tid < TM && r0 + tid < a.N) {
         const float m0 = sM[0][tid], m1 = sM[1][tid];
         const float m = fmaxf(m0, m1);
@@ -1039,9 +1174,11 @@ __global__ void __launch_bounds__(WTHREADS) fwd_tile_kernel(FwdParams p) {
 
 // backward G tile (256 rows x 256 vocab): recompute logits, write G^T [Vp][Rp]
 // (and G [rows][Vp] when write_g)
+template <bool SCORES>
 __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ float sLse[TM], sScale[TM];
+    __shared__ float sBase[SCORES ? TM : 1], sSlope[SCORES ? TM : 1], sExtra[SCORES ? TM : 1];
     __shared__ int sTgt[TM];
     const qpam_ce_bwd_args &a = p.a;
     const int n_rt = p.Rp / TM, n_vt = p.Vp / TN;
@@ -1055,7 +1192,15 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
         const int lr = lr0 + tid, row = p.row0 + lr;
         float lse = 0.f, sc = 0.f;
         int tg = -1;
-        if (lr < p.rows) {
+        if (SCORES) {
+            const RowScore q = lr < p.rows ? row_score(p, row) : RowScore{};
+            lse = q.m;
+            sc = q.k;
+            tg = lr < p.rows ? q.tgt : -1;
+            sBase[tid] = q.base;
+            sSlope[tid] = q.slope;
+            sExtra[tid] = q.extra;
+        } else if (lr < p.rows) {
             const int64_t t = a.targets[row];
             const bool valid = (t != a.ignore_index) && t >= 0 && t < a.V;
             lse = a.lse[row];
@@ -1090,6 +1235,7 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
     // +inf for rows without a gradient (their G is exp2(-inf) = 0), the scale and
     // the target column
     float hl[4][4], hs[4][4];
+    float hb[SCORES ? 4 : 1][4], hd[SCORES ? 4 : 1][4];
     int ht[4][4];
 #pragma unroll
     for (int mi = 0; mi < 4; ++mi)
@@ -1097,10 +1243,17 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
         for (int r = 0; r < 4; ++r) {
             const int rl = 64 * wm + 16 * mi + 4 * g + r;
             hs[mi][r] = sScale[rl];
-            hl[mi][r] = hs[mi][r] != 0.f ? sLse[rl] * LOG2E : INFINITY;
+            if constexpr (SCORES) {
+                hl[mi][r] = sLse[rl];
+                hb[mi][r] = sBase[rl];
+                hd[mi][r] = sSlope[rl];
+            } else {
+                hl[mi][r] = hs[mi][r] != 0.f ? sLse[rl] * LOG2E : INFINITY;
+            }
             ht[mi][r] = sTgt[rl];
         }
     const bool full = v0 + TN <= a.V;  // every column of the tile is a vocabulary entry
+    const bool fullr = lr0 + TM <= p.rows;
 #pragma unroll
     for (int ni = 0; ni < 8; ++ni) {
         const int vb = v0 + 128 * wn + 16 * ni, v = vb + l16;
@@ -1111,8 +1264,15 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
             float x[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][ni][r], LOG2E, -hl[mi][r]));
-                x[r] = vok ? (e - (v == ht[mi][r] ? 1.f : 0.f)) * hs[mi][r] : 0.f;
+                if constexpr (SCORES) {
+                    const float u = (acc[mi][ni][r] - hl[mi][r]) * p.c;
+                    float y = hs[mi][r] * __builtin_amdgcn_exp2f(u) * (hb[mi][r] + hd[mi][r] * fmaxf(u, U_FLOOR));
+                    if (v == ht[mi][r]) y += sExtra[rl0 + r];
+                    x[r] = vok && (fullr || lr0 + rl0 + r < p.rows) ? y : 0.f;
+                } else {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][ni][r], LOG2E, -hl[mi][r]));
+                    x[r] = vok ? (e - (v == ht[mi][r] ? 1.f : 0.f)) * hs[mi][r] : 0.f;
+                }
             }
             const unsigned lo = pack_bf16x2(x[0], x[1]), hi = pack_bf16x2(x[2], x[3]);
             if (p.write_g) {
@@ -1217,28 +1377,35 @@ __global__ void __launch_bounds__(THREADS) dw_cast_kernel(const float *src, int6
     }
 }
 
+// scores: a FwdParams with the token scores' fields set, or NULL for the loss
 template <typename T>
-int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream) {
+int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scores = nullptr) {
     FwdParams p;
+    if (scores) p = *scores;
     p.a = a;
-    const bool wide_tiles = is_bf<T>() && use_wide(a.D);
+    const bool wide_tiles = is_bf<T>() && (scores || use_wide(a.D));  // the direct-load loop takes any multiple of 32
     p.n_vt = wide_tiles ? (a.V + wide::TN - 1) / wide::TN : (a.V + vocab_tile<T>() - 1) / vocab_tile<T>();
     char *ws = (char *)a.workspace;
     const int64_t cnt = (int64_t)a.N * p.n_vt;
     p.part_m = (float *)ws;
     p.part_s = p.part_m + cnt;
     p.part_i = (int *)(p.part_s + cnt);
+    p.part_t = (float *)p.part_i;
     p.red = nullptr;
     int st;
     if (wide_tiles) {
         // the argmax (accuracy counts) only when requested
-        const void *kern = a.correct ? (const void *)wide::fwd_tile_kernel<true> : (const void *)wide::fwd_tile_kernel<false>;
+        const void *kern = scores      ? (const void *)wide::fwd_tile_kernel<false, true>
+                           : a.correct ? (const void *)wide::fwd_tile_kernel<true, false>
+                                       : (const void *)wide::fwd_tile_kernel<false, false>;
         QPAM_CHECK_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)wide::KSMEM));
         dim3 grid(big::xcd_grid(p.n_vt * ((a.N + wide::TM - 1) / wide::TM)));
-        if (a.correct)
-            hipLaunchKernelGGL(wide::fwd_tile_kernel<true>, grid, dim3(wide::WTHREADS), wide::KSMEM, stream, p);
+        if (scores)
+            hipLaunchKernelGGL((wide::fwd_tile_kernel<false, true>), grid, dim3(wide::WTHREADS), wide::KSMEM, stream, p);
+        else if (a.correct)
+            hipLaunchKernelGGL((wide::fwd_tile_kernel<true, false>), grid, dim3(wide::WTHREADS), wide::KSMEM, stream, p);
         else
-            hipLaunchKernelGGL(wide::fwd_tile_kernel<false>, grid, dim3(wide::WTHREADS), wide::KSMEM, stream, p);
+            hipLaunchKernelGGL((wide::fwd_tile_kernel<false, false>), grid, dim3(wide::WTHREADS), wide::KSMEM, stream, p);
         st = launch_status("ce fwd_tile_kernel (bf16, 256 x 256)");
     } else if (is_bf<T>()) {
         QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)big::fwd_tile_kernel,
@@ -1248,13 +1415,20 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream) {
         st = launch_status("ce fwd_tile_kernel (bf16)");
     } else {
         const size_t smem = gemm_smem<T>();
-        QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_fwd_tile_kernel<T>,
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        const void *kern = scores ? (const void *)ce_fwd_tile_kernel<T, true> : (const void *)ce_fwd_tile_kernel<T, false>;
+        QPAM_CHECK_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         dim3 grid(p.n_vt, (a.N + BM - 1) / BM);
-        hipLaunchKernelGGL(ce_fwd_tile_kernel<T>, grid, dim3(THREADS), smem, stream, p);
+        if (scores)
+            hipLaunchKernelGGL((ce_fwd_tile_kernel<T, true>), grid, dim3(THREADS), smem, stream, p);
+        else
+            hipLaunchKernelGGL((ce_fwd_tile_kernel<T, false>), grid, dim3(THREADS), smem, stream, p);
         st = launch_status("ce_fwd_tile_kernel");
     }
     if (st) return st;
+    if (scores) {
+        hipLaunchKernelGGL(scores_finalize_kernel<T>, dim3((a.N + 3) / 4), dim3(THREADS), 0, stream, p);
+        return launch_status("scores_finalize_kernel");
+    }
     hipLaunchKernelGGL(ce_fwd_finalize_kernel<T>, dim3((a.N + 3) / 4), dim3(THREADS), 0, stream, p);
     st = launch_status("ce_fwd_finalize_kernel");
     if (st) return st;
@@ -1267,23 +1441,28 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream) {
 
 // dw_write: dW written (beta 0; one pass over the rows) by the library GEMM, in
 // bf16 (dw_out 1) or fp32 (dw_out 2); otherwise added into the fp32 dW
-int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, bool dw_write = false) {
+int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams *scores, bool dw_write = false) {
     using U = unsigned short;
     big::GroupParams q;
     BwdParams &p = q.p;
+    if (scores) p = *scores;
     p.a = a;
     p.Vp = round_up(a.V, vocab_pad<U>());
     const int chunk = pass_rows(a);
     const int Rmax = round_up(chunk, big::BTM);
-    const bool wide_tiles = use_wide(a.D);
+    const bool wide_tiles = scores || use_wide(a.D);
     // the G-tile kernel: 256 x 256 tiles, or 256 x 128 for hidden sizes that are not
     // a multiple of 64 (Vp and Rp are multiples of both)
-    const void *gkern = wide_tiles ? (const void *)wide::grad_tile_kernel : (const void *)big::grad_tile_kernel;
+    const void *gkern = scores       ? (const void *)wide::grad_tile_kernel<true>
+                        : wide_tiles ? (const void *)wide::grad_tile_kernel<false>
+                                     : (const void *)big::grad_tile_kernel;
     const size_t gsmem = wide_tiles ? wide::KSMEM : big::SMEM;
     auto launch_grad = [&]() {
         const int tiles = (p.Vp / (wide_tiles ? wide::TN : big::BTN)) * (p.Rp / big::BTM);
-        if (wide_tiles)
-            hipLaunchKernelGGL(wide::grad_tile_kernel, dim3(big::xcd_grid(tiles)), dim3(wide::WTHREADS), gsmem, stream, p);
+        if (scores)
+            hipLaunchKernelGGL(wide::grad_tile_kernel<true>, dim3(big::xcd_grid(tiles)), dim3(wide::WTHREADS), gsmem, stream, p);
+        else if (wide_tiles)
+            hipLaunchKernelGGL(wide::grad_tile_kernel<false>, dim3(big::xcd_grid(tiles)), dim3(wide::WTHREADS), gsmem, stream, p);
         else
             hipLaunchKernelGGL(big::grad_tile_kernel, dim3(big::xcd_grid(tiles)), dim3(THREADS), gsmem, stream, p);
         return launch_status(wide_tiles ? "ce grad_tile_kernel (bf16, 256 x 256)" : "ce grad_tile_kernel (bf16)");
@@ -1363,9 +1542,10 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, bool dw_write = 
 }
 
 template <typename T>
-int run_bwd(const qpam_ce_bwd_args &a, hipStream_t stream) {
-    if (is_bf<T>()) return run_bwd_bf16(a, stream);
+int run_bwd(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams *scores) {
+    if (is_bf<T>()) return run_bwd_bf16(a, stream, scores);
     BwdParams p;
+    if (scores) p = *scores;
     p.a = a;
     p.write_g = 1;
     p.Vp = round_up(a.V, VT);
@@ -1377,7 +1557,8 @@ int run_bwd(const qpam_ce_bwd_args &a, hipStream_t stream) {
     p.gtbuf = (T *)p.gbuf + (int64_t)chunk * p.Vp;
     p.ht = (T *)p.gtbuf + (int64_t)p.Vp * Rmax;
     const size_t smem = gemm_smem<T>();
-    QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_grad_tile_kernel<T>,
+    QPAM_CHECK_HIP(hipFuncSetAttribute(scores ? (const void *)ce_grad_tile_kernel<T, true>
+                                              : (const void *)ce_grad_tile_kernel<T, false>,
                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_gemm_kernel<T, false>,
                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -1398,7 +1579,10 @@ int run_bwd(const qpam_ce_bwd_args &a, hipStream_t stream) {
                            p.Rp);
         st = launch_status("transpose_kernel(H)");
         if (st) return st;
-        hipLaunchKernelGGL(ce_grad_tile_kernel<T>, dim3(p.Vp / VT, p.Rp / BM), dim3(THREADS), smem, stream, p);
+        if (scores)
+            hipLaunchKernelGGL((ce_grad_tile_kernel<T, true>), dim3(p.Vp / VT, p.Rp / BM), dim3(THREADS), smem, stream, p);
+        else
+            hipLaunchKernelGGL((ce_grad_tile_kernel<T, false>), dim3(p.Vp / VT, p.Rp / BM), dim3(THREADS), smem, stream, p);
         st = launch_status("ce_grad_tile_kernel");
         if (st) return st;
         // dH[r0 .. r0+rows] = G [rows][Vp] * (W^T [D][Vp])^T
@@ -1427,6 +1611,65 @@ int validate_common(int N, int V, int D, int dtype, const void *h, int64_t ldh, 
     QPAM_REQUIRE(((uintptr_t)h % 16) == 0 && ((uintptr_t)w % 16) == 0 && ldh % vec == 0 && ldw % vec == 0 &&
                      ldh >= D && ldw >= D,
                  "%s: H and W must be 16-byte aligned with leading dims multiple of %d and >= D", who, vec);
+    return QPAM_OK;
+}
+
+// The backward passes with dW as a.dw_out asks for it.
+int run_backward(const qpam_ce_bwd_args &a, hipStream_t s, const BwdParams *scores) {
+    if (a.dw_out == 0) return a.dtype == QPAM_BF16 ? run_bwd<unsigned short>(a, s, scores) : run_bwd<float>(a, s, scores);
+    if (dw_direct(a)) return run_bwd_bf16(a, s, scores, true);
+    // dW accumulated in fp32 -- dw itself when it is fp32, else the workspace's tail -- from zero
+    qpam_ce_bwd_args b = a;
+    b.dw_out = 0;
+    float *acc = static_cast<float *>(a.dw);
+    int64_t ld = a.lddw;
+    const bool convert = a.dw_out == 1 && a.dtype == QPAM_BF16;
+    if (convert) {
+        acc = (float *)(((uintptr_t)a.workspace + bwd_ws_base<unsigned short>(b) + 255) & ~(uintptr_t)255);
+        ld = a.D;
+    }
+    const int64_t n = (int64_t)a.V * a.D;
+    const dim3 grid((unsigned)std::min<int64_t>((n + THREADS - 1) / THREADS, 65536));
+    hipLaunchKernelGGL(dw_fill_kernel, grid, dim3(THREADS), 0, s, acc, (int64_t)a.V, a.D, ld);
+    int st = launch_status("ce dw_fill_kernel");
+    if (st) return st;
+    b.dw = acc;
+    b.lddw = ld;
+    st = a.dtype == QPAM_BF16 ? run_bwd<unsigned short>(b, s, scores) : run_bwd<float>(b, s, scores);
+    if (st || !convert) return st;
+    hipLaunchKernelGGL(dw_cast_kernel, grid, dim3(THREADS), 0, s, (const float *)acc, ld, (unsigned short *)a.dw, a.lddw,
+                       (int64_t)a.V, a.D);
+    return launch_status("ce dw_cast_kernel");
+}
+
+// qpam_linear_logprobs_args as the loss's arguments (what they share)
+qpam_ce_fwd_args fwd_args(const qpam_linear_logprobs_args &a) {
+    qpam_ce_fwd_args f = {};
+    f.N = a.N, f.V = a.V, f.D = a.D, f.dtype = a.dtype;
+    f.h = a.h, f.ldh = a.ldh, f.w = a.w, f.ldw = a.ldw;
+    f.targets = a.ids, f.ignore_index = a.ignore_index;
+    f.workspace = a.workspace, f.workspace_bytes = a.workspace_bytes;
+    return f;
+}
+
+qpam_ce_bwd_args bwd_args(const qpam_linear_logprobs_args &a) {
+    qpam_ce_bwd_args b = {};
+    b.N = a.N, b.V = a.V, b.D = a.D, b.dtype = a.dtype;
+    b.h = a.h, b.ldh = a.ldh, b.w = a.w, b.ldw = a.ldw;
+    b.targets = a.ids, b.ignore_index = a.ignore_index;
+    b.dh = a.dh, b.lddh = a.lddh, b.dw = a.dw, b.lddw = a.lddw, b.dw_out = a.dw_out;
+    b.chunk = a.chunk;
+    b.workspace = a.workspace, b.workspace_bytes = a.workspace_bytes;
+    return b;
+}
+
+int validate_scores(const qpam_linear_logprobs_args &a, const char *who) {
+    int st = validate_common(a.N, a.V, a.D, a.dtype, a.h, a.ldh, a.w, a.ldw, a.ids, who);
+    if (st) return st;
+    QPAM_REQUIRE(a.temperature > 0.f && a.temperature < INFINITY, "%s: temperature %g must be positive and finite", who,
+                 a.temperature);
+    QPAM_REQUIRE(a.entropy && a.stats, "%s: null entropy or stats", who);
+    QPAM_REQUIRE((a.N + BM - 1) / BM <= 65535, "%s: too many rows", who);
     return QPAM_OK;
 }
 
@@ -1474,29 +1717,62 @@ extern "C" int qpam_ce_bwd(const qpam_ce_bwd_args *a, void *stream) {
     const size_t need = qpam_ce_bwd_workspace_size(a);
     QPAM_REQUIRE(a->workspace && a->workspace_bytes >= need && ((uintptr_t)a->workspace % 16) == 0,
                  "qpam_ce_bwd: workspace needs %zu bytes (got %zu)", need, a->workspace_bytes);
-    hipStream_t s = (hipStream_t)stream;
-    if (a->dw_out == 0) return a->dtype == QPAM_BF16 ? run_bwd<unsigned short>(*a, s) : run_bwd<float>(*a, s);
-    if (dw_direct(*a)) return run_bwd_bf16(*a, s, true);
-    // dW accumulated in fp32 -- dw itself when it is fp32, else the workspace's tail -- from zero
-    qpam_ce_bwd_args b = *a;
-    b.dw_out = 0;
-    float *acc = static_cast<float *>(a->dw);
-    int64_t ld = a->lddw;
-    const bool convert = a->dw_out == 1 && a->dtype == QPAM_BF16;
-    if (convert) {
-        acc = (float *)(((uintptr_t)a->workspace + bwd_ws_base<unsigned short>(b) + 255) & ~(uintptr_t)255);
-        ld = a->D;
-    }
-    const int64_t n = (int64_t)a->V * a->D;
-    const dim3 grid((unsigned)std::min<int64_t>((n + THREADS - 1) / THREADS, 65536));
-    hipLaunchKernelGGL(dw_fill_kernel, grid, dim3(THREADS), 0, s, acc, (int64_t)a->V, a->D, ld);
-    st = launch_status("ce dw_fill_kernel");
+    return run_backward(*a, (hipStream_t)stream, nullptr);
+}
+
+extern "C" size_t qpam_linear_logprobs_fwd_workspace_size(const qpam_linear_logprobs_args *a) {
+    using namespace qpam::ce;
+    if (!a || a->N < 1 || a->V < 1) return 0;
+    const qpam_ce_fwd_args f = fwd_args(*a);
+    return qpam_ce_fwd_workspace_size(&f);
+}
+
+extern "C" int qpam_linear_logprobs_fwd(const qpam_linear_logprobs_args *a, void *stream) {
+    using namespace qpam;
+    using namespace qpam::ce;
+    QPAM_REQUIRE(a != nullptr, "qpam_linear_logprobs_fwd: null args");
+    int st = validate_scores(*a, "qpam_linear_logprobs_fwd");
     if (st) return st;
-    b.dw = acc;
-    b.lddw = ld;
-    st = a->dtype == QPAM_BF16 ? run_bwd<unsigned short>(b, s) : run_bwd<float>(b, s);
-    if (st || !convert) return st;
-    hipLaunchKernelGGL(dw_cast_kernel, grid, dim3(THREADS), 0, s, (const float *)acc, ld, (unsigned short *)a->dw,
-                       a->lddw, (int64_t)a->V, a->D);
-    return launch_status("ce dw_cast_kernel");
+    QPAM_REQUIRE(a->logprobs, "qpam_linear_logprobs_fwd: null logprobs");
+    const size_t need = qpam_linear_logprobs_fwd_workspace_size(a);
+    QPAM_REQUIRE(a->workspace && a->workspace_bytes >= need && ((uintptr_t)a->workspace % 16) == 0,
+                 "qpam_linear_logprobs_fwd: workspace needs %zu bytes (got %zu)", need, a->workspace_bytes);
+    FwdParams p = {};
+    p.inv_t = 1.f / a->temperature;
+    p.c = p.inv_t * LOG2;
+    p.logprobs = a->logprobs;
+    p.entropy = a->entropy;
+    p.stats = a->stats;
+    return a->dtype == QPAM_BF16 ? run_fwd<unsigned short>(fwd_args(*a), (hipStream_t)stream, &p)
+                                 : run_fwd<float>(fwd_args(*a), (hipStream_t)stream, &p);
+}
+
+extern "C" size_t qpam_linear_logprobs_bwd_workspace_size(const qpam_linear_logprobs_args *a) {
+    using namespace qpam::ce;
+    if (!a || a->N < 1 || a->V < 1 || a->chunk < 1) return 0;
+    const qpam_ce_bwd_args b = bwd_args(*a);
+    return qpam_ce_bwd_workspace_size(&b);
+}
+
+extern "C" int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void *stream) {
+    using namespace qpam;
+    using namespace qpam::ce;
+    QPAM_REQUIRE(a != nullptr, "qpam_linear_logprobs_bwd: null args");
+    int st = validate_scores(*a, "qpam_linear_logprobs_bwd");
+    if (st) return st;
+    QPAM_REQUIRE(a->dh && a->dw, "qpam_linear_logprobs_bwd: null dh or dw");
+    QPAM_REQUIRE(a->chunk >= 1, "qpam_linear_logprobs_bwd: chunk must be >= 1");
+    QPAM_REQUIRE(a->lddh >= a->D && a->lddw >= a->D, "qpam_linear_logprobs_bwd: output leading dims must be >= D");
+    QPAM_REQUIRE(a->dw_out == 1 || a->dw_out == 2, "qpam_linear_logprobs_bwd: dw_out must be 1 or 2");
+    const size_t need = qpam_linear_logprobs_bwd_workspace_size(a);
+    QPAM_REQUIRE(a->workspace && a->workspace_bytes >= need && ((uintptr_t)a->workspace % 16) == 0,
+                 "qpam_linear_logprobs_bwd: workspace needs %zu bytes (got %zu)", need, a->workspace_bytes);
+    BwdParams p = {};
+    p.inv_t = 1.f / a->temperature;
+    p.c = p.inv_t * LOG2;
+    p.stats = a->stats;
+    p.entropy = a->entropy;
+    p.g_logprobs = a->g_logprobs;
+    p.g_entropy = a->g_entropy;
+    return run_backward(bwd_args(*a), (hipStream_t)stream, &p);
 }

@@ -4,6 +4,11 @@ token_logprobs reads rows of logits (qpam_logprobs_fwd / _bwd): what a serving
 loop reports beside the tokens of ModelDecoder.step, and what policy gradients and
 distillation differentiate.  The reference's V11LM.generate (v11/model.py:1207-1245)
 forms these softmax rows to draw from them and returns none of it.
+
+linear_token_logprobs gives the same values from the hidden rows and the tied table
+(qpam_linear_logprobs_fwd / _bwd), with the operands of
+fused_ce.fused_linear_cross_entropy and no logits in memory: scoring of whole
+sequences, and policy-gradient steps with an entropy term.
 """
 
 import ctypes
@@ -11,11 +16,13 @@ import math
 from typing import List, NamedTuple, Optional
 
 import torch
+import torch.nn.functional as F
 from torch import Tensor
 
 from . import _lib, _ops
+from .fused_ce import _operands
 
-__all__ = ["TokenLogprobs", "token_logprobs"]
+__all__ = ["TokenLogprobs", "token_logprobs", "linear_token_logprobs"]
 
 MAX_TOP_K = 64
 
@@ -153,3 +160,143 @@ def token_logprobs(logits: Tensor, ids: Tensor, temperature: float = 1.0, top_k:
     if not top_k:
         return TokenLogprobs(lp.view(shape), ent.view(shape))
     return TokenLogprobs(lp.view(shape), ent.view(shape), top.view(*shape, top_k), top_ids.view(*shape, top_k))
+
+
+# ------------------------------------------------------------ from hidden rows
+
+def _check_linear(hidden_rows, weight_matrix, ids, temperature, chunk):
+    name = "linear_token_logprobs"
+    if not (hidden_rows.is_cuda and hidden_rows.device == weight_matrix.device == ids.device):
+        raise ValueError(f"qpam {name}: tensors must be on one GPU (no CPU path in this library)")
+    if hidden_rows.dtype not in _CODE or weight_matrix.dtype not in _CODE:
+        raise ValueError(f"qpam {name}: float32 or bfloat16 expected, got {hidden_rows.dtype} and {weight_matrix.dtype}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"qpam {name}: ids must be int64 or int32, got {ids.dtype}")
+    if (hidden_rows.dim() < 1 or weight_matrix.dim() != 2 or hidden_rows.shape[-1] != weight_matrix.shape[1]
+            or hidden_rows.shape[:-1] != ids.shape or not weight_matrix.numel()):
+        raise ValueError(f"qpam {name}: hidden_rows [..., D], weight_matrix [V, D] and ids [...] expected, got "
+                         f"{tuple(hidden_rows.shape)}, {tuple(weight_matrix.shape)} and {tuple(ids.shape)}")
+    if chunk < 1:
+        raise ValueError(f"qpam {name}: chunk {chunk} must be at least 1")
+    _check_temperature(temperature, name)
+
+
+def _linear_args(h, w, dtype, ids, entropy, stats, temperature, ignore_index):
+    a = _lib.LinearLogprobsArgs()
+    a.N, a.V, a.D, a.dtype, a.temperature = h.shape[0], w.shape[0], h.shape[1], dtype, temperature
+    a.h, a.ldh, a.w, a.ldw = h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0)
+    a.ids, a.ignore_index = ids.data_ptr(), ignore_index
+    a.entropy, a.stats = entropy.data_ptr(), stats.data_ptr()
+    return a
+
+
+def _workspace(a, nbytes, device):
+    ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    return ws
+
+
+def _linear_forward(hidden_rows: Tensor, weight_matrix: Tensor, weight_copy: Optional[Tensor], ids: Tensor,
+                    temperature: float, chunk: int, ignore_index: int) -> List[Tensor]:
+    """hidden_rows [n, D], ids [n] int64 -> [logprobs, entropy, stats [n, 2]]; weight_copy:
+    an fp32 weight_matrix in the rows' bf16."""
+    h, w, dtype = _operands(hidden_rows, weight_matrix if weight_copy is None else weight_copy)
+    n, dev = h.shape[0], h.device
+    lp, ent, stats = (torch.empty(s, device=dev, dtype=torch.float32) for s in ((n,), (n,), (n, 2)))
+    if n:
+        ids = ids.contiguous()
+        a = _linear_args(h, w, dtype, ids, ent, stats, temperature, ignore_index)
+        a.logprobs = lp.data_ptr()
+        L = _lib.lib()
+        ws = _workspace(a, L.qpam_linear_logprobs_fwd_workspace_size(ctypes.byref(a)), dev)  # noqa: F841
+        with _lib.device(dev):
+            _lib.check(L.qpam_linear_logprobs_fwd(ctypes.byref(a), _lib.stream_ptr(dev)), "qpam_linear_logprobs_fwd")
+    return [lp, ent, stats]
+
+
+linear_logprobs_fwd_op = _ops.op("qpam::linear_logprobs_fwd")(_linear_forward)
+
+
+@linear_logprobs_fwd_op.register_fake
+def _(hidden_rows, weight_matrix, weight_copy, ids, temperature, chunk, ignore_index):
+    n = hidden_rows.shape[0]
+    f = lambda *s: hidden_rows.new_empty(s, dtype=torch.float32)  # noqa: E731
+    return [f(n), f(n), f(n, 2)]
+
+
+def _linear_gradient(hidden_rows: Tensor, weight_matrix: Tensor, ids: Tensor, entropy: Tensor, stats: Tensor,
+                     g_logprobs: Optional[Tensor], g_entropy: Optional[Tensor], temperature: float, chunk: int,
+                     ignore_index: int, dw_fp32: bool) -> List[Tensor]:
+    """[d hidden_rows, d weight_matrix] in the inputs' dtypes (d weight_matrix in fp32
+    with dw_fp32)."""
+    h, w, dtype = _operands(hidden_rows, weight_matrix)
+    n, dev = h.shape[0], h.device
+    dw_fp32 = dw_fp32 or weight_matrix.dtype != w.dtype
+    dh = torch.empty(h.shape, device=dev, dtype=h.dtype)
+    dw = torch.empty(w.shape, device=dev, dtype=torch.float32 if dw_fp32 else w.dtype)
+    if not n:
+        return [dh.to(hidden_rows.dtype), dw.zero_()]
+    ids = ids.contiguous()
+    gs = [g if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy)]
+    a = _linear_args(h, w, dtype, ids, entropy, stats, temperature, ignore_index)
+    a.g_logprobs, a.g_entropy = (g if g is None else g.data_ptr() for g in gs)
+    a.dh, a.lddh, a.dw, a.lddw = dh.data_ptr(), dh.stride(0), dw.data_ptr(), dw.stride(0)
+    a.chunk, a.dw_out = min(chunk, n), 2 if dw_fp32 else 1
+    L = _lib.lib()
+    ws = _workspace(a, L.qpam_linear_logprobs_bwd_workspace_size(ctypes.byref(a)), dev)  # noqa: F841
+    with _lib.device(dev):
+        _lib.check(L.qpam_linear_logprobs_bwd(ctypes.byref(a), _lib.stream_ptr(dev)), "qpam_linear_logprobs_bwd")
+    return [dh.to(hidden_rows.dtype), dw]
+
+
+linear_logprobs_bwd_op = _ops.op("qpam::linear_logprobs_bwd")(_linear_gradient)
+
+
+@linear_logprobs_bwd_op.register_fake
+def _(hidden_rows, weight_matrix, ids, entropy, stats, g_logprobs, g_entropy, temperature, chunk, ignore_index, dw_fp32):
+    return [hidden_rows.new_empty(hidden_rows.shape),
+            weight_matrix.new_empty(weight_matrix.shape, dtype=torch.float32 if dw_fp32 else weight_matrix.dtype)]
+
+
+def _linear_setup(ctx, inputs, output):
+    hidden_rows, weight_matrix, weight_copy, ids, ctx.temperature, ctx.chunk, ctx.ignore_index = inputs
+    ctx.mark_non_differentiable(output[2])
+    ctx.set_materialize_grads(False)
+    ctx.master = weight_copy is not None
+    ctx.save_for_backward(hidden_rows, weight_copy if ctx.master else weight_matrix, ids, output[1], output[2])
+
+
+def _linear_backward(ctx, grads):
+    g_lp, g_ent, _ = grads
+    if g_lp is None and g_ent is None:
+        return (None,) * 7
+    dh, dw = linear_logprobs_bwd_op(*ctx.saved_tensors, g_lp, g_ent, ctx.temperature, ctx.chunk, ctx.ignore_index,
+                                    ctx.master)
+    return dh, dw, None, None, None, None, None
+
+
+linear_logprobs_fwd_op.register_autograd(_linear_backward, setup_context=_linear_setup)
+
+
+def linear_token_logprobs(hidden_rows: Tensor, weight_matrix: Tensor, ids: Tensor, temperature: float = 1.0,
+                          chunk: int = 4096, ignore_index: int = -100) -> TokenLogprobs:
+    """token_logprobs(hidden_rows @ weight_matrix.T, ids, temperature) without the
+    logits in memory: log probabilities and entropies of rows [..., D] against a table
+    [V, D], float32 or bfloat16, ids [...] int64 or int32.
+
+    Differentiable in hidden_rows and weight_matrix (once: a second derivative
+    raises).  If either operand is bf16, both enter the products as bf16, with fp32
+    sums; the logits' gradient is rounded to bf16 before the two products that give
+    the operands' gradients.  The gradients have the operands' dtypes; that of an fp32
+    weight_matrix with bf16 rows (a master table) leaves from the fp32 sums.  chunk
+    bounds the backward's memory as in fused_ce.fused_linear_cross_entropy.  D off the
+    multiples of 32 pads both operands by copies.  Alternatives need the logits:
+    token_logprobs gives them."""
+    _check_linear(hidden_rows, weight_matrix, ids, temperature, chunk)
+    D = hidden_rows.shape[-1]
+    h, w = hidden_rows.reshape(-1, D), weight_matrix
+    if D % 32:
+        h, w = F.pad(h, (0, -D % 32)), F.pad(w, (0, -D % 32))
+    copy = w.detach().to(torch.bfloat16) if w.dtype == torch.float32 and h.dtype == torch.bfloat16 else None
+    lp, ent, _ = linear_logprobs_fwd_op(h, w, copy, ids.reshape(-1).long(), float(temperature), chunk, ignore_index)
+    return TokenLogprobs(lp.view(ids.shape), ent.view(ids.shape))

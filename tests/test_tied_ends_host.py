@@ -11,7 +11,8 @@ from qllm2_amd import _lib
 from test_abi import _header_struct_fields
 
 
-@pytest.mark.parametrize("cname,pyname", [("qpam_embed_args", "EmbedArgs"), ("qpam_logprobs_args", "LogprobsArgs")])
+@pytest.mark.parametrize("cname,pyname", [("qpam_embed_args", "EmbedArgs"), ("qpam_logprobs_args", "LogprobsArgs"),
+                                          ("qpam_linear_logprobs_args", "LinearLogprobsArgs")])
 def test_ctypes_structs_match_header(cname, pyname):
     assert [f[0] for f in getattr(_lib, pyname)._fields_] == _header_struct_fields(cname)
 
@@ -145,3 +146,61 @@ def test_token_logprobs_fake_kernels():
         d = logprobs_bwd_op(x.view(12, 50), ids.view(12).long(), f, torch.empty(12, 2, device="cuda"),
                             r.top_ids.view(12, 6), f, None, None, 1.0, -100)
         assert d.shape == (12, 50) and d.dtype == torch.bfloat16
+
+
+def test_linear_token_logprobs_refusals():
+    from qllm2_amd.token_logprobs import _check_linear, linear_token_logprobs
+    with pytest.raises(ValueError, match="GPU"):
+        linear_token_logprobs(torch.zeros(2, 32), torch.zeros(5, 32), torch.zeros(2, dtype=torch.long))
+    with FakeTensorMode():
+        c = lambda *s, **k: torch.empty(*s, device="cuda", **k)  # noqa: E731
+        h, w, ids = c(4, 32), c(9, 32), c(4, dtype=torch.long)
+        for args, what in [
+            ((h.half(), w, ids, 1.0, 1), "float32 or bfloat16"), ((h, w.double(), ids, 1.0, 1), "float32 or bfloat16"),
+            ((h, w, c(4), 1.0, 1), "int64 or int32"), ((h, w, c(5, dtype=torch.long), 1.0, 1), "hidden_rows"),
+            ((h, c(9, 31), ids, 1.0, 1), "hidden_rows"), ((h, c(0, 32), ids, 1.0, 1), "hidden_rows"),
+            ((h, c(1, 9, 32), ids, 1.0, 1), "hidden_rows"), ((h, w, ids, 1.0, 0), "chunk"),
+            ((h, w, ids, 0.0, 1), "temperature"), ((h, w, ids, float("nan"), 1), "temperature"),
+        ]:
+            with pytest.raises(ValueError, match=what):
+                _check_linear(*args)
+
+
+def test_linear_token_logprobs_entry_errors_without_gpu():
+    lib = _lib.lib()
+
+    def err(fn, **kw):
+        a = _lib.LinearLogprobsArgs()
+        a.N, a.V, a.D, a.dtype, a.temperature, a.chunk, a.dw_out = 4, 10, 64, _lib.QPAM_F32, 1.0, 4, 1
+        a.ldh = a.ldw = a.lddh = a.lddw = 64
+        a.h = a.w = a.ids = a.logprobs = a.entropy = a.stats = a.dh = a.dw = a.workspace = 4096
+        a.workspace_bytes = 1 << 30
+        for k, v in kw.items():
+            setattr(a, k, v)
+        assert getattr(lib, fn)(ctypes.byref(a), None) == _lib.QPAM_ERR_ARG
+        return lib.qpam_last_error().decode()
+
+    for fn in ("qpam_linear_logprobs_fwd", "qpam_linear_logprobs_bwd"):
+        assert "sizes" in err(fn, N=0) and "sizes" in err(fn, V=0) and "dtype" in err(fn, dtype=5)
+        assert "multiple" in err(fn, D=63) and "null" in err(fn, ids=None) and "aligned" in err(fn, h=4100)
+        assert "temperature" in err(fn, temperature=0.0) and "temperature" in err(fn, temperature=float("nan"))
+        assert "stats" in err(fn, stats=None) and "workspace" in err(fn, workspace_bytes=64)
+    assert "logprobs" in err("qpam_linear_logprobs_fwd", logprobs=None)
+    assert "dh" in err("qpam_linear_logprobs_bwd", dh=None) and "dw_out" in err("qpam_linear_logprobs_bwd", dw_out=0)
+    assert "chunk" in err("qpam_linear_logprobs_bwd", chunk=0)
+    assert "leading" in err("qpam_linear_logprobs_bwd", lddw=60)
+
+
+def test_linear_token_logprobs_fake_kernels():
+    from qllm2_amd.token_logprobs import linear_logprobs_bwd_op, linear_token_logprobs
+    with FakeTensorMode():
+        h = torch.empty(3, 4, 40, device="cuda", dtype=torch.bfloat16)
+        w = torch.empty(70, 40, device="cuda")
+        r = linear_token_logprobs(h, w, torch.empty(3, 4, device="cuda", dtype=torch.int32))
+        assert r.logprobs.shape == r.entropy.shape == (3, 4) and r.top_ids is None
+        f = torch.empty(12, device="cuda")
+        for fp32 in (False, True):
+            dh, dw = linear_logprobs_bwd_op(h.view(12, 40), w.bfloat16(), f.long(), f, torch.empty(12, 2, device="cuda"),
+                                            f, None, 1.0, 8, -100, fp32)
+            assert dh.shape == (12, 40) and dw.shape == (70, 40)
+            assert dh.dtype == torch.bfloat16 and dw.dtype == (torch.float32 if fp32 else torch.bfloat16)
