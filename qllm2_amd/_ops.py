@@ -12,6 +12,12 @@ and backward 315 against 110 us, one host core), which was most of a small
 training step.  Here the Autograd kernel applies one torch.autograd.Function
 that redispatches below autograd and keeps the saved tensors.  It needs a few
 names of torch._C; where one is missing, op() is torch.library.custom_op.
+
+op(name, direct=True) takes small calls out of the dispatcher as well: where nothing
+listens there (no compilation, tracing, dispatch or function mode, functorch level,
+forward-mode level or tensor subclass), the operator's function is called as it is,
+or under one torch.autograd.Function if a gradient is wanted.  Measured on a lookup of
+8 rows: 9.6 us against 14.5 without a gradient, 13.5 against 39.8 with one.
 """
 
 import sys
@@ -20,6 +26,7 @@ import threading
 import torch
 
 _LIB = torch.library.Library("qpam", "FRAGMENT")
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 _CALL = threading.local()  # the dispatch keys of the call that is entering its autograd function
 
 
@@ -41,10 +48,22 @@ def _kernel(name, fn):
     return kernel
 
 
+def _nothing_listens(args):
+    """No part of torch that reads calls at the dispatcher would see this one."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack():
+        return False
+    if torch._C._functorch.peek_interpreter_stack() is not None or torch._C._get_tracing_state() is not None:
+        return False
+    if torch.autograd.forward_ad._current_level >= 0:
+        return False
+    return all(type(a) in _PLAIN or not isinstance(a, torch.Tensor) for a in args)
+
+
 class Op:
     """One qpam:: operator, callable as the function it was made from."""
 
-    def __init__(self, name, fn):
+    def __init__(self, name, fn, direct=False):
+        self._plain_fn = fn if direct else None
         ns, self._name = name.split("::")
         if ns != "qpam":
             raise ValueError(f"operator {name}: the namespace must be qpam")
@@ -61,6 +80,11 @@ class Op:
         self._autograd(None, None)
 
     def __call__(self, *args, **kwargs):
+        if self._plain_fn is not None and not kwargs and len(args) == len(self._defaults) and _nothing_listens(args):
+            if torch.is_grad_enabled() and torch._C._any_requires_grad(*args):
+                out = self._direct_fn.apply(*args)
+                return list(out) if self._list else out
+            return self._plain_fn(*args)
         return self._op(*args, **kwargs)
 
     def register_fake(self, fn):
@@ -76,6 +100,8 @@ class Op:
     def _autograd(self, backward, setup_context):
         op, is_list, name, first = self._op, self._list, self._name, not hasattr(self, "_fn")
         defaults = self._defaults
+
+        plain_fn = self._plain_fn
 
         class Fn(torch.autograd.Function):
             @staticmethod
@@ -93,8 +119,17 @@ class Op:
                     raise RuntimeError(f"qpam::{name} has no backward")
                 return backward(ctx, list(grads) if is_list else grads[0])
 
-        Fn.__name__ = Fn.__qualname__ = f"qpam_{name}"
-        self._fn = Fn
+        class Direct(Fn):
+            @staticmethod
+            def forward(ctx, *args):
+                out = plain_fn(*args)
+                if setup_context is not None:
+                    setup_context(ctx, args, out)
+                return tuple(out) if is_list else out
+
+        for f in (Fn, Direct):
+            f.__name__ = f.__qualname__ = f"qpam_{name}"
+        self._fn, self._direct_fn = Fn, Direct
         if first:
             def autograd_kernel(keyset, *args):
                 if torch.is_grad_enabled() and torch._C._any_requires_grad(*args):
@@ -110,11 +145,12 @@ class Op:
             _LIB.impl(name, autograd_kernel, "Autograd", with_keyset=True)
 
 
+_DIRECT_NAMES = ("_len_torch_dispatch_stack", "_len_torch_function_stack", "_functorch", "_get_tracing_state")
 _NAMES = ("_AutoDispatchBelowAutograd", "_after_autograd_keyset", "_any_requires_grad")
 
 
-def op(name):
+def op(name, direct=False):
     """Decorator: the qpam:: operator made from an annotated function."""
     if all(hasattr(torch._C, n) for n in _NAMES) and hasattr(torch, "_disable_dynamo"):
-        return lambda fn: Op(name, fn)
+        return lambda fn: Op(name, fn, direct and all(hasattr(torch._C, n) for n in _DIRECT_NAMES))
     return lambda fn: torch.library.custom_op(name, fn, mutates_args=())

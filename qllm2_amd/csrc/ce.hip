@@ -27,6 +27,7 @@
 // and the gradient tiles write
 //   G_v = -p_v / T (g_lp + g_ent (ln p_v + entropy)) + [v = token] g_lp / T.
 #include <algorithm>
+#include <type_traits>
 
 #include "blas.h"
 #include "common.h"
@@ -87,18 +88,65 @@ template <> struct Mma<float> {
     }
 };
 
+// fp32 inputs on the bf16 matrix units (token scores): every value is split into three
+// bf16 parts, x = hi + mid + lo with |mid| <= 2^-9 |x|, |lo| <= 2^-18 |x| and nothing
+// left above 2^-27 |x|, and a product is the six part products down to 2^-18; the three
+// left out are below 2^-26 of it, less than one fp32 rounding.  The parts are made in
+// registers from the fp32 tiles.  Per 64 x 64 x 32 step a wave spends 96 MFMAs of 16
+// cycles and some 320 VALU instructions of 4 beside them, against 128 MFMAs of 32
+// cycles with v_mfma_f32_16x16x4_f32.  Infinite operands give NaN.
+struct SplitF32 {};
+template <> struct Mma<SplitF32> {
+    static constexpr int PITCH = Mma<float>::PITCH;
+
+    // 8 values (k = 4 g .. and 16 + 4 g ..) -> the parts of one fragment
+    __device__ __forceinline__ static void parts(const float *row, bf16x8 (&x)[3]) {
+        const float4 a = *reinterpret_cast<const float4 *>(row), b = *reinterpret_cast<const float4 *>(row + 16);
+        float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+            unsigned q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                q[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+                if (part < 2) {
+                    v[2 * i] -= __uint_as_float(q[i] << 16);
+                    v[2 * i + 1] -= __uint_as_float(q[i] & 0xFFFF0000u);
+                }
+            }
+            x[part] = __builtin_bit_cast(bf16x8, uintx4{q[0], q[1], q[2], q[3]});
+        }
+    }
+    __device__ __forceinline__ static void step(const float *sA, const float *sB, int arow0, int brow0,
+                                                floatx4 (&acc)[4][4], int l16, int g) {
+        bf16x8 a[4][3];
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi) parts(sA + (arow0 + 16 * mi + l16) * PITCH + 4 * g, a[mi]);
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni) {
+            bf16x8 b[3];
+            parts(sB + (brow0 + 16 * ni + l16) * PITCH + 4 * g, b);
+            constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};  // small products first
+#pragma unroll
+            for (int j = 0; j < 6; ++j)
+#pragma unroll
+                for (int mi = 0; mi < 4; ++mi)
+                    acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mi][PA[j]], b[PB[j]], acc[mi][ni], 0, 0, 0);
+        }
+    }
+};
+
 template <typename T>
 constexpr size_t gemm_smem() { return (size_t)2 * (BM + BN) * Mma<T>::PITCH * sizeof(T); }
 
 // C[m][n] = sum_k A[m][k] B[n][k] for one BM x BN tile; A and B point at the
 // tile's first row; rows beyond a_rows / b_rows read as zero; K % BK == 0.
 // Wave w owns rows 64*(w>>1).., cols 64*(w&1)..; acc[mi][ni] lane holds
-// C[64*(w>>1) + 16mi + 4g + r][64*(w&1) + 16ni + l16].
-template <typename T>
+// C[64*(w>>1) + 16mi + 4g + r][64*(w&1) + 16ni + l16].  MM: how a k-step is multiplied.
+template <typename T, typename MM = Mma<T>>
 __device__ __forceinline__ void gemm_tile(const T *A, int64_t lda, int a_rows, const T *B, int64_t ldb, int b_rows,
                                           int K, floatx4 (&acc)[4][4], T *smem) {
-    using MM = Mma<T>;
-    constexpr int PITCH = MM::PITCH, R16 = MM::ROW16, EPC = 16 / sizeof(T);
+    constexpr int PITCH = MM::PITCH, R16 = Mma<T>::ROW16, EPC = 16 / sizeof(T);
     constexpr int LOADS = BM * R16 / THREADS;  // 16-byte loads per thread per operand
     T *sA[2] = {smem, smem + (BM + BN) * PITCH};
     T *sB[2] = {smem + BM * PITCH, smem + (BM + BN) * PITCH + BM * PITCH};
@@ -168,6 +216,10 @@ __device__ __forceinline__ void join_scores(float &m, float &s, float &t, float 
     m = nm;
 }
 
+// the product of the token scores' fp32 tiles
+template <typename T, bool SCORES>
+using TileMma = Mma<std::conditional_t<SCORES && std::is_same_v<T, float>, SplitF32, T>>;
+
 template <typename T, bool SCORES>
 __global__ void __launch_bounds__(THREADS) ce_fwd_tile_kernel(FwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -178,8 +230,8 @@ __global__ void __launch_bounds__(THREADS) ce_fwd_tile_kernel(FwdParams p) {
     const int vt = blockIdx.x, rt = blockIdx.y;
     const int r0 = rt * BM, v0 = vt * VT;
     floatx4 acc[4][4];
-    gemm_tile<T>((const T *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(BM, a.N - r0), (const T *)a.w + (int64_t)v0 * a.ldw,
-                 a.ldw, min(BN, a.V - v0), a.D, acc, smem);
+    gemm_tile<T, TileMma<T, SCORES>>((const T *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(BM, a.N - r0),
+                                     (const T *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(BN, a.V - v0), a.D, acc, smem);
 
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
@@ -319,9 +371,15 @@ __global__ void __launch_bounds__(THREADS) scores_finalize_kernel(FwdParams p) {
         join_scores(m, s, t, __shfl_xor(m, off), __shfl_xor(s, off), __shfl_xor(t, off), p.c);
     float dot = 0.f;
     if (valid) {
-        const T *hr = (const T *)a.h + (int64_t)row * a.ldh;
-        const T *wr = (const T *)a.w + id * a.ldw;
-        for (int k = lane; k < a.D; k += 64) dot += Elem<T>::load(hr + k) * Elem<T>::load(wr + k);
+        constexpr int E = 16 / sizeof(T);  // rows are 16-byte aligned and whole vectors long
+        const uintx4 *hr = reinterpret_cast<const uintx4 *>((const T *)a.h + (int64_t)row * a.ldh);
+        const uintx4 *wr = reinterpret_cast<const uintx4 *>((const T *)a.w + id * a.ldw);
+        for (int k = lane; k < a.D / E; k += 64) {
+            const uintx4 hv = hr[k], wv = wr[k];
+            const T *he = reinterpret_cast<const T *>(&hv), *we = reinterpret_cast<const T *>(&wv);
+#pragma unroll
+            for (int i = 0; i < E; ++i) dot += Elem<T>::load(he + i) * Elem<T>::load(we + i);
+        }
     }
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) dot += __shfl_xor(dot, off);
@@ -462,8 +520,8 @@ __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
         sTgt[tid] = tg;
     }
     floatx4 acc[4][4];
-    gemm_tile<T>((const T *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(BM, p.rows - lr0),
-                 (const T *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(BN, a.V - v0), a.D, acc, smem);
+    gemm_tile<T, TileMma<T, SCORES>>((const T *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(BM, p.rows - lr0),
+                                     (const T *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(BN, a.V - v0), a.D, acc, smem);
     const int w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
     T *G = (T *)p.gbuf;
@@ -531,6 +589,45 @@ __global__ void __launch_bounds__(THREADS) ce_gemm_kernel(const T *A, int64_t ld
                     }
                 }
             }
+}
+
+// C = A B^T of fp32 operands in parts (token scores' dH and dW), the K axis in
+// gridDim.z ranges of kper: one range writes C (or adds to it), several write C + z
+// split_stride, summed by split_sum_kernel in their order.
+__global__ void __launch_bounds__(THREADS) split_gemm_kernel(const float *A, int64_t lda, int M, const float *B, int64_t ldb,
+                                                            int N, int K, int kper, float *C, int64_t ldc,
+                                                            int64_t split_stride, int accumulate) {
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN, k0 = blockIdx.z * kper;
+    floatx4 acc[4][4];
+    gemm_tile<float, Mma<SplitF32>>(A + (int64_t)m0 * lda + k0, lda, min(BM, M - m0), B + (int64_t)n0 * ldb + k0, ldb,
+                                    min(BN, N - n0), min(kper, K - k0), acc, reinterpret_cast<float *>(smem_raw));
+    C += blockIdx.z * split_stride;
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wm = w >> 1, wn = w & 1;
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int m = m0 + 64 * wm + 16 * mi + 4 * g + r, n = n0 + 64 * wn + 16 * ni + l16;
+                if (m < M && n < N) {
+                    float *c = C + (int64_t)m * ldc + n;
+                    *c = accumulate ? *c + acc[mi][ni][r] : acc[mi][ni][r];
+                }
+            }
+}
+
+__global__ void __launch_bounds__(THREADS) split_sum_kernel(const float *part, int splits, int64_t rows, int cols, float *out,
+                                                           int64_t ldo) {
+    const int64_t n = rows * cols;
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * THREADS) {
+        float x = 0.f;
+        for (int z = 0; z < splits; ++z) x += part[z * n + i];
+        const int64_t r = i / cols;
+        out[r * ldo + (i - r * cols)] = x;
+    }
 }
 
 // ------------------------------------------------------ bf16 big tiles ----
@@ -1300,6 +1397,137 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
 }
 }  // namespace wide
 
+// Token scores of few rows (a decode step's), bound by reading the table once: a wave
+// takes 16 table rows and every hidden row, 16 MI of them.  The table goes from memory
+// straight to the MFMA's A registers, 8 steps of 64 bytes a row ahead (8 KiB a wave in
+// flight); the hidden rows' next 512 bytes a row go through LDS, shared by the block's
+// four waves, its 16-byte chunks XOR-swizzled by the row so that the 16 lanes of a
+// fragment read distinct banks.  Both operands take a lane's 16 bytes as consecutive k.
+namespace thin {
+constexpr int ROWS = 64;              // at most this many hidden rows
+constexpr int VB = 64;                // table rows of a block
+constexpr int STEPS = 8, CHUNKS = 4 * STEPS;  // 64-byte steps, 16-byte chunks of a stage
+
+__device__ __forceinline__ void mma(uintx4 w, uintx4 h, floatx4 &acc, unsigned short) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, h), acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(uintx4 w, uintx4 h, floatx4 &acc, float) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[i]), __uint_as_float(h[i]), acc, 0, 0, 0);
+}
+
+template <typename T, int MI>
+__global__ void __launch_bounds__(THREADS) scores_kernel(FwdParams p) {
+    __shared__ uintx4 sH[2][16 * MI * CHUNKS];
+    __shared__ float sM[4][16 * MI], sS[4][16 * MI], sT[4][16 * MI];
+    const qpam_ce_fwd_args &a = p.a;
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int v0 = blockIdx.x * VB + 16 * w;
+    const int steps = a.D * (int)sizeof(T) / 64, stages = (steps + STEPS - 1) / STEPS;
+    // rows past the end of an operand re-read its last row, steps past the end the last step
+    const uintx4 *wrow = reinterpret_cast<const uintx4 *>((const T *)a.w + (int64_t)min(v0 + l16, a.V - 1) * a.ldw) + g;
+    uintx4 hr[2 * MI];
+    auto load_h = [&](int stage) {
+#pragma unroll
+        for (int i = 0; i < 2 * MI; ++i) {
+            const int e = tid + i * THREADS, row = e / CHUNKS, c = e % CHUNKS;
+            const int at = min(stage * CHUNKS + (c ^ (row & 15)), 4 * steps - 1);
+            hr[i] = reinterpret_cast<const uintx4 *>((const T *)a.h + (int64_t)min(row, a.N - 1) * a.ldh)[at];
+        }
+    };
+    auto store_h = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < 2 * MI; ++i) sH[buf][tid + i * THREADS] = hr[i];
+    };
+    auto load_w = [&](uintx4 (&x)[STEPS], int stage) {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) x[i] = __builtin_nontemporal_load(wrow + 4 * min(stage * STEPS + i, steps - 1));
+    };
+    floatx4 acc[MI];
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) acc[mi] = floatx4{0.f, 0.f, 0.f, 0.f};
+    auto step = [&](const uintx4 (&x)[STEPS], int buf, int stage) {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            if (stage * STEPS + i >= steps) break;
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi)
+                mma(x[i], sH[buf][(16 * mi + l16) * CHUNKS + ((4 * i + g) ^ l16)], acc[mi], T());
+        }
+    };
+    uintx4 x0[STEPS], x1[STEPS];
+    load_h(0);
+    load_w(x0, 0);
+    store_h(0);
+    __syncthreads();
+    for (int st = 0; st < stages; st += 2) {
+        load_h(min(st + 1, stages - 1));
+        load_w(x1, min(st + 1, stages - 1));
+        __builtin_amdgcn_sched_barrier(0);
+        step(x0, 0, st);
+        store_h(1);
+        __syncthreads();
+        if (st + 1 >= stages) break;
+        load_h(min(st + 2, stages - 1));
+        load_w(x0, min(st + 2, stages - 1));
+        __builtin_amdgcn_sched_barrier(0);
+        step(x1, 1, st + 1);
+        store_h(0);
+        __syncthreads();
+    }
+    // acc[mi][r]: table row v0 + 4 g + r, hidden row 16 mi + l16
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (v0 + 4 * g + r < a.V) m = fmaxf(m, acc[mi][r]);
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const float lo = fmaxf(m, -3.402823466e38f);
+        float s = 0.f, t = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (v0 + 4 * g + r < a.V) {
+                const float u = (acc[mi][r] - lo) * p.c, e = __builtin_amdgcn_exp2f(u);
+                s += e;
+                t += e * fmaxf(u, U_FLOOR);
+            }
+        s += __shfl_xor(s, 16);
+        t += __shfl_xor(t, 16);
+        s += __shfl_xor(s, 32);
+        t += __shfl_xor(t, 32);
+        if (g == 0) {
+            sM[w][16 * mi + l16] = m;
+            sS[w][16 * mi + l16] = s;
+            sT[w][16 * mi + l16] = t;
+        }
+    }
+    __syncthreads();
+    if (tid < 16 * MI && tid < a.N) {
+        float m = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
+        for (int v = 1; v < 4; ++v) join_scores(m, s, t, sM[v][tid], sS[v][tid], sT[v][tid], p.c);
+        const int64_t o = (int64_t)tid * p.n_vt + blockIdx.x;
+        p.part_m[o] = m;
+        p.part_s[o] = s;
+        p.part_t[o] = t;
+    }
+}
+
+template <typename T>
+int launch(const FwdParams &p, hipStream_t stream) {
+    const dim3 grid(p.n_vt);
+    if (p.a.N <= 16)
+        hipLaunchKernelGGL((scores_kernel<T, 1>), grid, dim3(THREADS), 0, stream, p);
+    else if (p.a.N <= 32)
+        hipLaunchKernelGGL((scores_kernel<T, 2>), grid, dim3(THREADS), 0, stream, p);
+    else
+        hipLaunchKernelGGL((scores_kernel<T, 4>), grid, dim3(THREADS), 0, stream, p);
+    return launch_status("thin scores_kernel");
+}
+}  // namespace thin
+
 int round_up(int x, int m) { return (x + m - 1) / m * m; }
 
 template <typename T> constexpr bool is_bf() { return sizeof(T) == 2; }
@@ -1383,8 +1611,9 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     FwdParams p;
     if (scores) p = *scores;
     p.a = a;
+    const bool few = scores && a.N <= thin::ROWS;
     const bool wide_tiles = is_bf<T>() && (scores || use_wide(a.D));  // the direct-load loop takes any multiple of 32
-    p.n_vt = wide_tiles ? (a.V + wide::TN - 1) / wide::TN : (a.V + vocab_tile<T>() - 1) / vocab_tile<T>();
+    p.n_vt = few ? (a.V + thin::VB - 1) / thin::VB : wide_tiles ? (a.V + wide::TN - 1) / wide::TN : (a.V + vocab_tile<T>() - 1) / vocab_tile<T>();
     char *ws = (char *)a.workspace;
     const int64_t cnt = (int64_t)a.N * p.n_vt;
     p.part_m = (float *)ws;
@@ -1393,7 +1622,9 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     p.part_t = (float *)p.part_i;
     p.red = nullptr;
     int st;
-    if (wide_tiles) {
+    if (few) {
+        st = thin::launch<T>(p, stream);
+    } else if (wide_tiles) {
         // the argmax (accuracy counts) only when requested
         const void *kern = scores      ? (const void *)wide::fwd_tile_kernel<false, true>
                            : a.correct ? (const void *)wide::fwd_tile_kernel<true, false>
@@ -1545,7 +1776,6 @@ template <typename T>
 int run_bwd(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams *scores) {
     if (is_bf<T>()) return run_bwd_bf16(a, stream, scores);
     BwdParams p;
-    if (scores) p = *scores;
     p.a = a;
     p.write_g = 1;
     p.Vp = round_up(a.V, VT);
@@ -1557,8 +1787,7 @@ int run_bwd(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams *scor
     p.gtbuf = (T *)p.gbuf + (int64_t)chunk * p.Vp;
     p.ht = (T *)p.gtbuf + (int64_t)p.Vp * Rmax;
     const size_t smem = gemm_smem<T>();
-    QPAM_CHECK_HIP(hipFuncSetAttribute(scores ? (const void *)ce_grad_tile_kernel<T, true>
-                                              : (const void *)ce_grad_tile_kernel<T, false>,
+    QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_grad_tile_kernel<T, false>,
                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_gemm_kernel<T, false>,
                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -1579,10 +1808,7 @@ int run_bwd(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams *scor
                            p.Rp);
         st = launch_status("transpose_kernel(H)");
         if (st) return st;
-        if (scores)
-            hipLaunchKernelGGL((ce_grad_tile_kernel<T, true>), dim3(p.Vp / VT, p.Rp / BM), dim3(THREADS), smem, stream, p);
-        else
-            hipLaunchKernelGGL((ce_grad_tile_kernel<T, false>), dim3(p.Vp / VT, p.Rp / BM), dim3(THREADS), smem, stream, p);
+        hipLaunchKernelGGL((ce_grad_tile_kernel<T, false>), dim3(p.Vp / VT, p.Rp / BM), dim3(THREADS), smem, stream, p);
         st = launch_status("ce_grad_tile_kernel");
         if (st) return st;
         // dH[r0 .. r0+rows] = G [rows][Vp] * (W^T [D][Vp])^T
@@ -1614,8 +1840,79 @@ int validate_common(int N, int V, int D, int dtype, const void *h, int64_t ldh, 
     return QPAM_OK;
 }
 
+// Ranges of the vocabulary that share the token scores' fp32 dH of `rows` rows: two
+// blocks for each of the 256 CUs, at most 16 ranges and none below 512 entries.
+int dh_splits(int rows, int D, int Vp) {
+    const int tiles = ((rows + BM - 1) / BM) * ((D + BN - 1) / BN);
+    return std::max(1, std::min({512 / std::max(tiles, 1), Vp / 512, 16}));
+}
+
+// ... and their partial sums: splits * rows <= 16 rows, and <= 512 BM as splits * tiles <= 512
+size_t scores_f32_ws(const qpam_ce_bwd_args &a) {
+    const int64_t rows = std::min<int64_t>(16ll * pass_rows(a), 512ll * BM);
+    return bwd_ws_base<float>(a) + 256 + (size_t)rows * a.D * 4;
+}
+
+// Token scores in fp32: G tiles, then dH and dW, all in bf16 parts.  dW is written by the
+// first pass and added to by the others.
+int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams &scores) {
+    using T = float;
+    BwdParams p = scores;
+    p.a = a;
+    p.write_g = 1;
+    p.Vp = round_up(a.V, VT);
+    const int chunk = pass_rows(a);
+    const int Rmax = round_up(chunk, BM);
+    T *ws = (T *)a.workspace;
+    p.wt = ws;
+    p.gbuf = ws + (int64_t)a.D * p.Vp;
+    p.gtbuf = (T *)p.gbuf + (int64_t)chunk * p.Vp;
+    p.ht = (T *)p.gtbuf + (int64_t)p.Vp * Rmax;
+    float *part = (float *)(((uintptr_t)a.workspace + bwd_ws_base<T>(a) + 255) & ~(uintptr_t)255);
+    const size_t smem = gemm_smem<T>();
+    QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_grad_tile_kernel<T, true>,
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)split_gemm_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    hipLaunchKernelGGL(transpose_kernel<T>, dim3((a.D + 63) / 64, (p.Vp + 63) / 64), dim3(THREADS), 0, stream,
+                       (const T *)a.w, a.ldw, a.V, a.D, (T *)p.wt, (int64_t)p.Vp, a.D, p.Vp);
+    int st = launch_status("transpose_kernel(W)");
+    if (st) return st;
+    for (int r0 = 0; r0 < a.N; r0 += chunk) {
+        p.row0 = r0;
+        p.rows = std::min(chunk, a.N - r0);
+        p.Rp = round_up(p.rows, BM);
+        hipLaunchKernelGGL(transpose_kernel<T>, dim3((a.D + 63) / 64, (p.Rp + 63) / 64), dim3(THREADS), 0, stream,
+                           (const T *)a.h + (int64_t)r0 * a.ldh, a.ldh, p.rows, a.D, (T *)p.ht, (int64_t)p.Rp, a.D, p.Rp);
+        if ((st = launch_status("transpose_kernel(H)"))) return st;
+        hipLaunchKernelGGL((ce_grad_tile_kernel<T, true>), dim3(p.Vp / VT, p.Rp / BM), dim3(THREADS), smem, stream, p);
+        if ((st = launch_status("ce_grad_tile_kernel"))) return st;
+        // dH[r0 .. r0 + rows] = G [rows][Vp] (W^T [D][Vp])^T
+        const int splits = dh_splits(p.rows, a.D, p.Vp), kper = round_up((p.Vp + splits - 1) / splits, BK);
+        float *dh = (float *)a.dh + (int64_t)r0 * a.lddh;
+        hipLaunchKernelGGL(split_gemm_kernel, dim3((a.D + BN - 1) / BN, (p.rows + BM - 1) / BM, (p.Vp + kper - 1) / kper),
+                           dim3(THREADS), smem, stream, (const T *)p.gbuf, (int64_t)p.Vp, p.rows, (const T *)p.wt,
+                           (int64_t)p.Vp, a.D, p.Vp, kper, splits > 1 ? part : dh, splits > 1 ? (int64_t)a.D : a.lddh,
+                           (int64_t)p.rows * a.D, 0);
+        if ((st = launch_status("split_gemm_kernel(dH)"))) return st;
+        if (splits > 1) {
+            const int64_t n = (int64_t)p.rows * a.D;
+            hipLaunchKernelGGL(split_sum_kernel, dim3((unsigned)std::min<int64_t>((n + THREADS - 1) / THREADS, 4096)),
+                               dim3(THREADS), 0, stream, (const float *)part, (p.Vp + kper - 1) / kper, (int64_t)p.rows, a.D,
+                               dh, a.lddh);
+            if ((st = launch_status("split_sum_kernel"))) return st;
+        }
+        // dW [V][D] (+)= G^T [Vp][Rp] (H^T [D][Rp])^T
+        hipLaunchKernelGGL(split_gemm_kernel, dim3((a.D + BN - 1) / BN, (a.V + BM - 1) / BM, 1), dim3(THREADS), smem, stream,
+                           (const T *)p.gtbuf, (int64_t)p.Rp, a.V, (const T *)p.ht, (int64_t)p.Rp, a.D, p.Rp, p.Rp,
+                           (float *)a.dw, a.lddw, (int64_t)0, r0 > 0 ? 1 : 0);
+        if ((st = launch_status("split_gemm_kernel(dW)"))) return st;
+    }
+    return QPAM_OK;
+}
+
 // The backward passes with dW as a.dw_out asks for it.
 int run_backward(const qpam_ce_bwd_args &a, hipStream_t s, const BwdParams *scores) {
+    if (scores && a.dtype == QPAM_F32) return run_scores_f32(a, s, *scores);
     if (a.dw_out == 0) return a.dtype == QPAM_BF16 ? run_bwd<unsigned short>(a, s, scores) : run_bwd<float>(a, s, scores);
     if (dw_direct(a)) return run_bwd_bf16(a, s, scores, true);
     // dW accumulated in fp32 -- dw itself when it is fp32, else the workspace's tail -- from zero
@@ -1724,6 +2021,7 @@ extern "C" size_t qpam_linear_logprobs_fwd_workspace_size(const qpam_linear_logp
     using namespace qpam::ce;
     if (!a || a->N < 1 || a->V < 1) return 0;
     const qpam_ce_fwd_args f = fwd_args(*a);
+    if (a->N <= thin::ROWS) return (size_t)a->N * ((a->V + thin::VB - 1) / thin::VB) * 12 + 256;
     return qpam_ce_fwd_workspace_size(&f);
 }
 
@@ -1751,7 +2049,7 @@ extern "C" size_t qpam_linear_logprobs_bwd_workspace_size(const qpam_linear_logp
     using namespace qpam::ce;
     if (!a || a->N < 1 || a->V < 1 || a->chunk < 1) return 0;
     const qpam_ce_bwd_args b = bwd_args(*a);
-    return qpam_ce_bwd_workspace_size(&b);
+    return a->dtype == QPAM_F32 ? scores_f32_ws(b) : qpam_ce_bwd_workspace_size(&b);
 }
 
 extern "C" int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void *stream) {

@@ -36,11 +36,10 @@ def _check(ids, weight_real, weight_imag):
         raise ValueError(f"qpam complex_embedding: ids must be int64 or int32, got {ids.dtype}")
 
 
-def _args(ids, V, dim, dtype, scale):
-    a = _lib.EmbedArgs()
-    a.n, a.V, a.dim, a.dtype, a.scale = ids.numel(), V, dim, _CODE[dtype], scale
-    a.ids_i64, a.ids = ids.dtype == torch.int64, ids.data_ptr()
-    return a
+def _args(ids, V, dim, dtype, padding_idx, scale, *more):
+    """EmbedArgs, `more` being the fields from `re` on."""
+    return _lib.EmbedArgs(ids.numel(), V, dim, _CODE[dtype], ids.dtype == torch.int64, ids.data_ptr(), padding_idx, scale,
+                          *more)
 
 
 def _rows(w):
@@ -52,15 +51,16 @@ def _lookup(ids: Tensor, weight_real: Tensor, weight_imag: Tensor, scale: float,
     _check(ids, weight_real, weight_imag)
     V, dim = weight_real.shape
     ids, re, im = ids.contiguous(), _rows(weight_real), _rows(weight_imag)
-    out = torch.empty(*ids.shape, dim, 2, device=re.device, dtype=re.dtype)
-    a = _args(ids, V, dim, re.dtype, scale)
-    a.re, a.ld_re, a.im, a.ld_im, a.out = re.data_ptr(), re.stride(0), im.data_ptr(), im.stride(0), out.data_ptr()
-    with _lib.device(re.device):
-        _lib.check(_lib.lib().qpam_embed_fwd(ctypes.byref(a), _lib.stream_ptr(re.device)), "qpam_embed_fwd")
+    dev = re.device
+    out = torch.empty(*ids.shape, dim, 2, device=dev, dtype=re.dtype)
+    a = _args(ids, V, dim, re.dtype, padding_idx, scale, re.data_ptr(), re.stride(0), im.data_ptr(), im.stride(0),
+              out.data_ptr())
+    with _lib.device(dev):
+        _lib.check(_lib.lib().qpam_embed_fwd(ctypes.byref(a), _lib.stream_ptr(dev)), "qpam_embed_fwd")
     return out
 
 
-embed_fwd_op = _ops.op("qpam::embed_fwd")(_lookup)
+embed_fwd_op = _ops.op("qpam::embed_fwd", direct=True)(_lookup)
 
 
 @embed_fwd_op.register_fake
@@ -75,8 +75,8 @@ def _gradient(ids: Tensor, dz: Tensor, num_embeddings: int, scale: float, paddin
     if dz.data_ptr() % 16:
         dz = dz.clone()
     grads = [torch.empty(num_embeddings, dim, device=dz.device, dtype=dz.dtype) for _ in range(2)]
-    a = _args(ids, num_embeddings, dim, dz.dtype, scale)
-    a.padding_idx, a.dz, a.d_re, a.d_im = padding_idx, dz.data_ptr(), grads[0].data_ptr(), grads[1].data_ptr()
+    a = _args(ids, num_embeddings, dim, dz.dtype, padding_idx, scale, None, 0, None, 0, None, dz.data_ptr(),
+              grads[0].data_ptr(), grads[1].data_ptr())
     L = _lib.lib()
     nbytes = L.qpam_embed_bwd_workspace_size(ctypes.byref(a))
     ws = torch.empty(nbytes, device=dz.device, dtype=torch.uint8)
@@ -86,7 +86,7 @@ def _gradient(ids: Tensor, dz: Tensor, num_embeddings: int, scale: float, paddin
     return grads
 
 
-embed_bwd_op = _ops.op("qpam::embed_bwd")(_gradient)
+embed_bwd_op = _ops.op("qpam::embed_bwd", direct=True)(_gradient)
 
 
 @embed_bwd_op.register_fake

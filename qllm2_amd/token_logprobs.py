@@ -58,12 +58,11 @@ def _check(logits, ids, temperature, top_k):
     _check_temperature(temperature, "token_logprobs")
 
 
-def _args(logits, ids, temperature, top_k, ignore_index):
-    a = _lib.LogprobsArgs()
-    a.n, a.V, a.dtype, a.top_k, a.temperature = logits.shape[0], logits.shape[1], _CODE[logits.dtype], top_k, temperature
-    a.logits, a.ld = logits.data_ptr(), max(logits.stride(0), logits.shape[1])
-    a.ids, a.ignore_index = ids.data_ptr(), ignore_index
-    return a
+def _args(logits, ids, temperature, top_k, ignore_index, *more):
+    """LogprobsArgs, `more` being the fields from `logprobs` on."""
+    n, V = logits.shape
+    return _lib.LogprobsArgs(n, V, _CODE[logits.dtype], top_k, temperature, logits.data_ptr(), max(logits.stride(0), V),
+                             ids.data_ptr(), ignore_index, *more)
 
 
 def _rows(logits):
@@ -78,15 +77,14 @@ def _forward(logits: Tensor, ids: Tensor, temperature: float, top_k: int, ignore
     lp, ent, stats = (torch.empty(s, device=dev, dtype=torch.float32) for s in ((n,), (n,), (n, 2)))
     top = torch.empty(n, top_k, device=dev, dtype=torch.float32)
     top_ids = torch.empty(n, top_k, device=dev, dtype=torch.int64)
-    a = _args(x, ids, temperature, top_k, ignore_index)
-    a.logprobs, a.entropy, a.stats = lp.data_ptr(), ent.data_ptr(), stats.data_ptr()
-    a.top_logprobs, a.top_ids = top.data_ptr(), top_ids.data_ptr()
+    a = _args(x, ids, temperature, top_k, ignore_index, lp.data_ptr(), ent.data_ptr(), stats.data_ptr(), top.data_ptr(),
+              top_ids.data_ptr())
     with _lib.device(dev):
         _lib.check(_lib.lib().qpam_logprobs_fwd(ctypes.byref(a), _lib.stream_ptr(dev)), "qpam_logprobs_fwd")
     return [lp, ent, stats, top, top_ids]
 
 
-logprobs_fwd_op = _ops.op("qpam::logprobs_fwd")(_forward)
+logprobs_fwd_op = _ops.op("qpam::logprobs_fwd", direct=True)(_forward)
 
 
 @logprobs_fwd_op.register_fake
@@ -103,16 +101,14 @@ def _gradient(logits: Tensor, ids: Tensor, entropy: Tensor, stats: Tensor, top_i
     n, V = x.shape
     out = torch.empty(n, V, device=x.device, dtype=x.dtype)
     gs = [g if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy, g_top)]
-    a = _args(x, ids, temperature, top_ids.shape[1], ignore_index)
-    a.entropy, a.stats, a.top_ids = entropy.data_ptr(), stats.data_ptr(), top_ids.data_ptr()
-    a.g_logprobs, a.g_entropy, a.g_top = (g if g is None else g.data_ptr() for g in gs)
-    a.d_logits, a.ldd = out.data_ptr(), V
+    a = _args(x, ids, temperature, top_ids.shape[1], ignore_index, None, entropy.data_ptr(), stats.data_ptr(), None,
+              top_ids.data_ptr(), *(g if g is None else g.data_ptr() for g in gs), out.data_ptr(), V)
     with _lib.device(x.device):
         _lib.check(_lib.lib().qpam_logprobs_bwd(ctypes.byref(a), _lib.stream_ptr(x.device)), "qpam_logprobs_bwd")
     return out
 
 
-logprobs_bwd_op = _ops.op("qpam::logprobs_bwd")(_gradient)
+logprobs_bwd_op = _ops.op("qpam::logprobs_bwd", direct=True)(_gradient)
 
 
 @logprobs_bwd_op.register_fake
@@ -153,10 +149,14 @@ def token_logprobs(logits: Tensor, ids: Tensor, temperature: float = 1.0, top_k:
     logits through logprobs, entropy and top_logprobs (once: a second derivative
     raises); the gradient has the logits' dtype."""
     _check(logits, ids, temperature, top_k)
-    V = logits.shape[-1]
-    lp, ent, _, top, top_ids = logprobs_fwd_op(logits.reshape(-1, V), ids.reshape(-1).long(), float(temperature), top_k,
-                                               ignore_index)
     shape = ids.shape
+    flat = len(shape) == 1
+    if not flat:
+        logits, ids = logits.reshape(-1, logits.shape[-1]), ids.reshape(-1)
+    lp, ent, _, top, top_ids = logprobs_fwd_op(logits, ids if ids.dtype == torch.int64 else ids.long(), float(temperature),
+                                               top_k, ignore_index)
+    if flat:
+        return TokenLogprobs(lp, ent, top, top_ids) if top_k else TokenLogprobs(lp, ent)
     if not top_k:
         return TokenLogprobs(lp.view(shape), ent.view(shape))
     return TokenLogprobs(lp.view(shape), ent.view(shape), top.view(*shape, top_k), top_ids.view(*shape, top_k))
@@ -214,7 +214,7 @@ def _linear_forward(hidden_rows: Tensor, weight_matrix: Tensor, weight_copy: Opt
     return [lp, ent, stats]
 
 
-linear_logprobs_fwd_op = _ops.op("qpam::linear_logprobs_fwd")(_linear_forward)
+linear_logprobs_fwd_op = _ops.op("qpam::linear_logprobs_fwd", direct=True)(_linear_forward)
 
 
 @linear_logprobs_fwd_op.register_fake
@@ -249,7 +249,7 @@ def _linear_gradient(hidden_rows: Tensor, weight_matrix: Tensor, ids: Tensor, en
     return [dh.to(hidden_rows.dtype), dw]
 
 
-linear_logprobs_bwd_op = _ops.op("qpam::linear_logprobs_bwd")(_linear_gradient)
+linear_logprobs_bwd_op = _ops.op("qpam::linear_logprobs_bwd", direct=True)(_linear_gradient)
 
 
 @linear_logprobs_bwd_op.register_fake

@@ -2,12 +2,13 @@
 probabilities): refusals, argument structures, fake kernels."""
 
 import ctypes
+from typing import List
 
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-from qllm2_amd import _lib
+from qllm2_amd import _lib, _ops
 from test_abi import _header_struct_fields
 
 
@@ -204,3 +205,71 @@ def test_linear_token_logprobs_fake_kernels():
                                             f, None, 1.0, 8, -100, fp32)
             assert dh.shape == (12, 40) and dw.shape == (70, 40)
             assert dh.dtype == torch.bfloat16 and dw.dtype == (torch.float32 if fp32 else torch.bfloat16)
+
+
+def _toy(a: torch.Tensor, b: torch.Tensor, s: float) -> List[torch.Tensor]:
+    return [a * s + b, a * a]
+
+
+def _wired(name, direct):
+    f = _ops.op(name, direct=direct)(_toy)
+    f.register_fake(lambda a, b, s: [torch.empty_like(a), torch.empty_like(a)])
+
+    def setup(ctx, inputs, output):
+        ctx.save_for_backward(inputs[0])
+        ctx.s = inputs[2]
+        ctx.set_materialize_grads(False)
+
+    def back(ctx, grads):
+        a, = ctx.saved_tensors
+        with torch.no_grad():
+            da = (grads[0] * ctx.s if grads[0] is not None else 0) + (2 * a * grads[1] if grads[1] is not None else 0)
+        return da, grads[0], None
+
+    f.register_autograd(back, setup_context=setup)
+    return f
+
+
+def test_direct_operators_equal_the_dispatched_ones():
+    """op(direct=True): same values and gradients outside the dispatcher; every listener
+    of the dispatcher still sees the operator."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+    direct, plain = _wired("qpam::t_direct", True), _wired("qpam::t_dispatched", False)
+    g = torch.Generator().manual_seed(1)
+    res = []
+    for f in (direct, plain):
+        g.manual_seed(1)
+        a, b = (torch.randn(4, 3, generator=g, requires_grad=True) for _ in range(2))
+        y = f(a, b, 1.5)
+        assert [t.requires_grad for t in y] == [True, True] and type(y) is list
+        gs = torch.autograd.grad(y, [a, b], [torch.ones(4, 3), torch.full((4, 3), 2.0)], retain_graph=True)
+        first, = torch.autograd.grad(y[0].sum(), [a])
+        with torch.no_grad():
+            assert not f(a, b, 1.5)[0].requires_grad
+        with torch.inference_mode():
+            assert f(a, b, 1.5)[0].is_inference()
+        res.append([*y, *gs, first])
+    for x, z in zip(*res):
+        assert torch.equal(x, z)
+
+    class Watch(TorchDispatchMode):
+        seen = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen += func.namespace == "qpam"
+            return func(*args, **(kwargs or {}))
+
+    a = torch.ones(2)
+    with Watch() as w:
+        direct(a, a, 2.0)
+    assert w.seen == 1
+    with FakeTensorMode():
+        assert direct(torch.empty(3), torch.empty(3), 2.0)[0].shape == (3,)
+    assert "t_direct" in str(make_fx(lambda x: direct(x, x, 2.0)[0])(a).graph)
+    with pytest.raises(Exception):
+        torch.func.vmap(lambda x: direct(x, x, 2.0)[0])(torch.ones(3, 2))
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(Exception):
+        d = torch.autograd.forward_ad.make_dual(a.clone().requires_grad_(), a)
+        direct(d, a, 2.0)
+    assert torch.equal(torch.compile(lambda x: direct(x, x, 2.0)[0], backend="eager", fullgraph=True)(a), a * 3)
