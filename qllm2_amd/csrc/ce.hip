@@ -1397,16 +1397,19 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
 }
 }  // namespace wide
 
-// Token scores of few rows (a decode step's), bound by reading the table once: a wave
-// takes 16 table rows and every hidden row, 16 MI of them.  The table goes from memory
-// straight to the MFMA's A registers, 8 steps of 64 bytes a row ahead (8 KiB a wave in
-// flight); the hidden rows' next 512 bytes a row go through LDS, shared by the block's
-// four waves, its 16-byte chunks XOR-swizzled by the row so that the 16 lanes of a
-// fragment read distinct banks.  Both operands take a lane's 16 bytes as consecutive k.
+// Token scores of few rows (a decode step's), bound by reading the table once.  A wave
+// takes 16 table rows and every hidden row, 16 MI of them.  The table streams global ->
+// LDS by direct loads in stages of 128 bytes a row, three stages deep, each wave its own
+// rows (no barrier); the hidden rows in stages of 256 bytes a row, two deep, shared by
+// the block.  Both are XOR-swizzled by 16-byte chunks so that the 16 rows of a fragment
+// read distinct banks, and both operands take a lane's 16 bytes as consecutive k.
+// Measured on 50261 x 1536 bf16 (154 MB): a load instruction has to cover whole 128-byte
+// lines (16 rows x 64 bytes straight to registers: 45 us), and 197 blocks of 16 waves
+// balance the CUs better than 786 of 4 (35 us).
 namespace thin {
-constexpr int ROWS = 64;              // at most this many hidden rows
-constexpr int VB = 64;                // table rows of a block
-constexpr int STEPS = 8, CHUNKS = 4 * STEPS;  // 64-byte steps, 16-byte chunks of a stage
+constexpr int ROWS = 64;                     // at most this many hidden rows
+constexpr int WB = 128, HB = 256;            // bytes a row of a table / hidden stage
+__host__ __device__ constexpr int waves(int V) { return V > 64 * 512 ? 16 : 4; }  // two blocks of 4 waves a CU, then 16
 
 __device__ __forceinline__ void mma(uintx4 w, uintx4 h, floatx4 &acc, unsigned short) {
     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, h), acc, 0, 0, 0);
@@ -1416,66 +1419,97 @@ __device__ __forceinline__ void mma(uintx4 w, uintx4 h, floatx4 &acc, float) {
     for (int i = 0; i < 4; ++i)
         acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[i]), __uint_as_float(h[i]), acc, 0, 0, 0);
 }
+__device__ __forceinline__ void to_lds(const char *from, char *lds) {
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const unsigned *>(from), reinterpret_cast<unsigned *>(lds), 16, 0, 0);
+}
+// direct loads still in flight at most `n`, and LDS reads stay behind the wait
+template <int N> __device__ __forceinline__ void landed() {
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(N));
+    wave_lds_order();
+}
 
-template <typename T, int MI>
-__global__ void __launch_bounds__(THREADS) scores_kernel(FwdParams p) {
-    __shared__ uintx4 sH[2][16 * MI * CHUNKS];
-    __shared__ float sM[4][16 * MI], sS[4][16 * MI], sT[4][16 * MI];
+template <typename T, int MI, int NW>
+__global__ void __launch_bounds__(64 * NW) scores_kernel(FwdParams p) {
+    __shared__ __align__(16) char sW0[NW * 16 * WB], sW1[NW * 16 * WB], sW2[NW * 16 * WB];
+    __shared__ __align__(16) char sH0[16 * MI * HB], sH1[16 * MI * HB];
+    __shared__ float sM[NW][16 * MI], sS[NW][16 * MI], sT[NW][16 * MI];
+    constexpr int HI = MI * 4 / NW > 0 ? MI * 4 / NW : 1;  // hidden-stage loads of a wave (spare waves repeat one)
     const qpam_ce_fwd_args &a = p.a;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
-    const int v0 = blockIdx.x * VB + 16 * w;
-    const int steps = a.D * (int)sizeof(T) / 64, stages = (steps + STEPS - 1) / STEPS;
-    // rows past the end of an operand re-read its last row, steps past the end the last step
-    const uintx4 *wrow = reinterpret_cast<const uintx4 *>((const T *)a.w + (int64_t)min(v0 + l16, a.V - 1) * a.ldw) + g;
-    uintx4 hr[2 * MI];
-    auto load_h = [&](int stage) {
+    const int v0 = (blockIdx.x * NW + w) * 16;
+    const int bytes = a.D * (int)sizeof(T), steps = bytes / 64, chunks = (bytes + HB - 1) / HB;
+    // Rows past the end of an operand re-read its last row, chunks past a row's end its last
+    // chunk.  A table load covers 8 rows, a hidden load 4; lane -> (row, chunk ^ row).
+    const char *wrow[2], *hrow[HI];
+    int hc[HI];
+    const int wc = 16 * ((lane & 7) ^ (lane >> 3));
 #pragma unroll
-        for (int i = 0; i < 2 * MI; ++i) {
-            const int e = tid + i * THREADS, row = e / CHUNKS, c = e % CHUNKS;
-            const int at = min(stage * CHUNKS + (c ^ (row & 15)), 4 * steps - 1);
-            hr[i] = reinterpret_cast<const uintx4 *>((const T *)a.h + (int64_t)min(row, a.N - 1) * a.ldh)[at];
-        }
+    for (int i = 0; i < 2; ++i)
+        wrow[i] = reinterpret_cast<const char *>((const T *)a.w + (int64_t)min(v0 + 8 * i + (lane >> 3), a.V - 1) * a.ldw);
+#pragma unroll
+    for (int i = 0; i < HI; ++i) {
+        const int row = ((w * HI + i) % (4 * MI)) * 4 + (lane >> 4);
+        hrow[i] = reinterpret_cast<const char *>((const T *)a.h + (int64_t)min(row, a.N - 1) * a.ldh);
+        hc[i] = 16 * ((lane & 15) ^ (row & 15));
+    }
+    auto load_w = [&](char *lds, int stage) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) to_lds(wrow[i] + min(stage * WB + wc, bytes - 16), lds + (w * 16 + 8 * i) * WB);
     };
-    auto store_h = [&](int buf) {
+    auto load_h = [&](char *lds, int chunk) {
 #pragma unroll
-        for (int i = 0; i < 2 * MI; ++i) sH[buf][tid + i * THREADS] = hr[i];
-    };
-    auto load_w = [&](uintx4 (&x)[STEPS], int stage) {
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) x[i] = __builtin_nontemporal_load(wrow + 4 * min(stage * STEPS + i, steps - 1));
+        for (int i = 0; i < HI; ++i)
+            to_lds(hrow[i] + min(chunk * HB + hc[i], bytes - 16), lds + ((w * HI + i) % (4 * MI)) * 4 * HB);
     };
     floatx4 acc[MI];
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) acc[mi] = floatx4{0.f, 0.f, 0.f, 0.f};
-    auto step = [&](const uintx4 (&x)[STEPS], int buf, int stage) {
+    // one table stage (two 64-byte steps) against half a hidden stage
+    auto multiply = [&](const char *sw, const char *sh, int stage) {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            if (stage * STEPS + i >= steps) break;
+        for (int q = 0; q < 2; ++q) {
+            if (2 * stage + q < steps) {
+                const uintx4 x = *reinterpret_cast<const uintx4 *>(sw + (w * 16 + l16) * WB + 16 * ((4 * q + g) ^ (l16 & 7)));
 #pragma unroll
-            for (int mi = 0; mi < MI; ++mi)
-                mma(x[i], sH[buf][(16 * mi + l16) * CHUNKS + ((4 * i + g) ^ l16)], acc[mi], T());
+                for (int mi = 0; mi < MI; ++mi)
+                    mma(x, *reinterpret_cast<const uintx4 *>(sh + (16 * mi + l16) * HB + 16 * ((8 * (stage & 1) + 4 * q + g) ^ l16)),
+                        acc[mi], T());
+            }
         }
     };
-    uintx4 x0[STEPS], x1[STEPS];
-    load_h(0);
-    load_w(x0, 0);
-    store_h(0);
-    __syncthreads();
-    for (int st = 0; st < stages; st += 2) {
-        load_h(min(st + 1, stages - 1));
-        load_w(x1, min(st + 1, stages - 1));
-        __builtin_amdgcn_sched_barrier(0);
-        step(x0, 0, st);
-        store_h(1);
-        __syncthreads();
-        if (st + 1 >= stages) break;
-        load_h(min(st + 2, stages - 1));
-        load_w(x0, min(st + 2, stages - 1));
-        __builtin_amdgcn_sched_barrier(0);
-        step(x1, 1, st + 1);
-        store_h(0);
-        __syncthreads();
+    // Loads leave in the order W(0) W(1) h(0) | h(j+1) W(2j+2) .. W(2j+3) .. of chunk j, two a
+    // table stage; every wave issues the same number, past the end too.
+    load_w(sW0, 0);
+    load_w(sW1, 1);
+    load_h(sH0, 0);
+    landed<0>();
+    __builtin_amdgcn_s_barrier();
+#define QPAM_THIN_CHUNK(J, WA, WB_, WC, H, HN)                                                  \
+    load_h(HN, (J) + 1);                                                                        \
+    load_w(WC, 2 * (J) + 2);                                                                    \
+    landed<4 + HI>();                                                                           \
+    multiply(WA, H, 2 * (J));                                                                   \
+    wave_lds_order();                                                                           \
+    load_w(WA, 2 * (J) + 3);                                                                    \
+    landed<4 + HI>();                                                                           \
+    multiply(WB_, H, 2 * (J) + 1);                                                              \
+    landed<4>();                                                                                \
+    __builtin_amdgcn_s_barrier();
+    for (int j = 0; j < chunks; j += 6) {  // table stages repeat after 3, hidden ones after 2 chunks
+        QPAM_THIN_CHUNK(j, sW0, sW1, sW2, sH0, sH1)
+        if (j + 1 >= chunks) break;
+        QPAM_THIN_CHUNK(j + 1, sW2, sW0, sW1, sH1, sH0)
+        if (j + 2 >= chunks) break;
+        QPAM_THIN_CHUNK(j + 2, sW1, sW2, sW0, sH0, sH1)
+        if (j + 3 >= chunks) break;
+        QPAM_THIN_CHUNK(j + 3, sW0, sW1, sW2, sH1, sH0)
+        if (j + 4 >= chunks) break;
+        QPAM_THIN_CHUNK(j + 4, sW2, sW0, sW1, sH0, sH1)
+        if (j + 5 >= chunks) break;
+        QPAM_THIN_CHUNK(j + 5, sW1, sW2, sW0, sH1, sH0)
     }
+#undef QPAM_THIN_CHUNK
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // no direct load outlives the wave
     // acc[mi][r]: table row v0 + 4 g + r, hidden row 16 mi + l16
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
@@ -1507,7 +1541,7 @@ __global__ void __launch_bounds__(THREADS) scores_kernel(FwdParams p) {
     __syncthreads();
     if (tid < 16 * MI && tid < a.N) {
         float m = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
-        for (int v = 1; v < 4; ++v) join_scores(m, s, t, sM[v][tid], sS[v][tid], sT[v][tid], p.c);
+        for (int v = 1; v < NW; ++v) join_scores(m, s, t, sM[v][tid], sS[v][tid], sT[v][tid], p.c);
         const int64_t o = (int64_t)tid * p.n_vt + blockIdx.x;
         p.part_m[o] = m;
         p.part_s[o] = s;
@@ -1515,17 +1549,18 @@ __global__ void __launch_bounds__(THREADS) scores_kernel(FwdParams p) {
     }
 }
 
-template <typename T>
+template <typename T, int NW>
 int launch(const FwdParams &p, hipStream_t stream) {
-    const dim3 grid(p.n_vt);
+    const dim3 grid(p.n_vt), block(64 * NW);
     if (p.a.N <= 16)
-        hipLaunchKernelGGL((scores_kernel<T, 1>), grid, dim3(THREADS), 0, stream, p);
+        hipLaunchKernelGGL((scores_kernel<T, 1, NW>), grid, block, 0, stream, p);
     else if (p.a.N <= 32)
-        hipLaunchKernelGGL((scores_kernel<T, 2>), grid, dim3(THREADS), 0, stream, p);
+        hipLaunchKernelGGL((scores_kernel<T, 2, NW>), grid, block, 0, stream, p);
     else
-        hipLaunchKernelGGL((scores_kernel<T, 4>), grid, dim3(THREADS), 0, stream, p);
+        hipLaunchKernelGGL((scores_kernel<T, 4, NW>), grid, block, 0, stream, p);
     return launch_status("thin scores_kernel");
 }
+int blocks(int V) { return (V + 16 * waves(V) - 1) / (16 * waves(V)); }
 }  // namespace thin
 
 int round_up(int x, int m) { return (x + m - 1) / m * m; }
@@ -1613,7 +1648,7 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     p.a = a;
     const bool few = scores && a.N <= thin::ROWS;
     const bool wide_tiles = is_bf<T>() && (scores || use_wide(a.D));  // the direct-load loop takes any multiple of 32
-    p.n_vt = few ? (a.V + thin::VB - 1) / thin::VB : wide_tiles ? (a.V + wide::TN - 1) / wide::TN : (a.V + vocab_tile<T>() - 1) / vocab_tile<T>();
+    p.n_vt = few ? thin::blocks(a.V) : wide_tiles ? (a.V + wide::TN - 1) / wide::TN : (a.V + vocab_tile<T>() - 1) / vocab_tile<T>();
     char *ws = (char *)a.workspace;
     const int64_t cnt = (int64_t)a.N * p.n_vt;
     p.part_m = (float *)ws;
@@ -1623,7 +1658,7 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     p.red = nullptr;
     int st;
     if (few) {
-        st = thin::launch<T>(p, stream);
+        st = thin::waves(a.V) == 16 ? thin::launch<T, 16>(p, stream) : thin::launch<T, 4>(p, stream);
     } else if (wide_tiles) {
         // the argmax (accuracy counts) only when requested
         const void *kern = scores      ? (const void *)wide::fwd_tile_kernel<false, true>
@@ -2021,7 +2056,7 @@ extern "C" size_t qpam_linear_logprobs_fwd_workspace_size(const qpam_linear_logp
     using namespace qpam::ce;
     if (!a || a->N < 1 || a->V < 1) return 0;
     const qpam_ce_fwd_args f = fwd_args(*a);
-    if (a->N <= thin::ROWS) return (size_t)a->N * ((a->V + thin::VB - 1) / thin::VB) * 12 + 256;
+    if (a->N <= thin::ROWS) return (size_t)a->N * thin::blocks(a->V) * 12 + 256;
     return qpam_ce_fwd_workspace_size(&f);
 }
 
