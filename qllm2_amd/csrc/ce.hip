@@ -148,8 +148,10 @@ __device__ __forceinline__ void gemm_tile(const T *A, int64_t lda, int a_rows, c
                                           int K, floatx4 (&acc)[4][4], T *smem) {
     constexpr int PITCH = MM::PITCH, R16 = Mma<T>::ROW16, EPC = 16 / sizeof(T);
     constexpr int LOADS = BM * R16 / THREADS;  // 16-byte loads per thread per operand
-    T *sA[2] = {smem, smem + (BM + BN) * PITCH};
-    T *sB[2] = {smem + BM * PITCH, smem + (BM + BN) * PITCH + BM * PITCH};
+    // buffers by offset: a table of pointers loses their address space, and flat loads
+    // from LDS wait for the global loads in flight as well
+    auto sA = [&](int buf) { return smem + buf * (BM + BN) * PITCH; };
+    auto sB = [&](int buf) { return smem + (buf * (BM + BN) + BM) * PITCH; };
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int arow0 = 64 * (w >> 1), brow0 = 64 * (w & 1);
 #pragma unroll
@@ -172,8 +174,8 @@ __device__ __forceinline__ void gemm_tile(const T *A, int64_t lda, int a_rows, c
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int ci = tid + i * THREADS, row = ci / R16, c = ci % R16;
-            *reinterpret_cast<uint4 *>(sA[buf] + row * PITCH + c * EPC) = ra[i];
-            *reinterpret_cast<uint4 *>(sB[buf] + row * PITCH + c * EPC) = rb[i];
+            *reinterpret_cast<uint4 *>(sA(buf) + row * PITCH + c * EPC) = ra[i];
+            *reinterpret_cast<uint4 *>(sB(buf) + row * PITCH + c * EPC) = rb[i];
         }
     };
     const int KT = K / BK;
@@ -183,7 +185,7 @@ __device__ __forceinline__ void gemm_tile(const T *A, int64_t lda, int a_rows, c
     for (int kt = 0; kt < KT; ++kt) {
         const int buf = kt & 1;
         if (kt + 1 < KT) gload((kt + 1) * BK);
-        MM::step(sA[buf], sB[buf], arow0, brow0, acc, l16, g);
+        MM::step(sA(buf), sB(buf), arow0, brow0, acc, l16, g);
         if (kt + 1 < KT) lstore(buf ^ 1);
         __syncthreads();
     }
