@@ -88,65 +88,18 @@ template <> struct Mma<float> {
     }
 };
 
-// fp32 inputs on the bf16 matrix units (token scores): every value is split into three
-// bf16 parts, x = hi + mid + lo with |mid| <= 2^-9 |x|, |lo| <= 2^-18 |x| and nothing
-// left above 2^-27 |x|, and a product is the six part products down to 2^-18; the three
-// left out are below 2^-26 of it, less than one fp32 rounding.  The parts are made in
-// registers from the fp32 tiles.  Per 64 x 64 x 32 step a wave spends 96 MFMAs of 16
-// cycles and some 320 VALU instructions of 4 beside them, against 128 MFMAs of 32
-// cycles with v_mfma_f32_16x16x4_f32.  Infinite operands give NaN.
-struct SplitF32 {};
-template <> struct Mma<SplitF32> {
-    static constexpr int PITCH = Mma<float>::PITCH;
-
-    // 8 values (k = 4 g .. and 16 + 4 g ..) -> the parts of one fragment
-    __device__ __forceinline__ static void parts(const float *row, bf16x8 (&x)[3]) {
-        const float4 a = *reinterpret_cast<const float4 *>(row), b = *reinterpret_cast<const float4 *>(row + 16);
-        float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int part = 0; part < 3; ++part) {
-            unsigned q[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                q[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-                if (part < 2) {
-                    v[2 * i] -= __uint_as_float(q[i] << 16);
-                    v[2 * i + 1] -= __uint_as_float(q[i] & 0xFFFF0000u);
-                }
-            }
-            x[part] = __builtin_bit_cast(bf16x8, uintx4{q[0], q[1], q[2], q[3]});
-        }
-    }
-    __device__ __forceinline__ static void step(const float *sA, const float *sB, int arow0, int brow0,
-                                                floatx4 (&acc)[4][4], int l16, int g) {
-        bf16x8 a[4][3];
-#pragma unroll
-        for (int mi = 0; mi < 4; ++mi) parts(sA + (arow0 + 16 * mi + l16) * PITCH + 4 * g, a[mi]);
-#pragma unroll
-        for (int ni = 0; ni < 4; ++ni) {
-            bf16x8 b[3];
-            parts(sB + (brow0 + 16 * ni + l16) * PITCH + 4 * g, b);
-            constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};  // small products first
-#pragma unroll
-            for (int j = 0; j < 6; ++j)
-#pragma unroll
-                for (int mi = 0; mi < 4; ++mi)
-                    acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mi][PA[j]], b[PB[j]], acc[mi][ni], 0, 0, 0);
-        }
-    }
-};
-
 template <typename T>
 constexpr size_t gemm_smem() { return (size_t)2 * (BM + BN) * Mma<T>::PITCH * sizeof(T); }
 
 // C[m][n] = sum_k A[m][k] B[n][k] for one BM x BN tile; A and B point at the
 // tile's first row; rows beyond a_rows / b_rows read as zero; K % BK == 0.
 // Wave w owns rows 64*(w>>1).., cols 64*(w&1)..; acc[mi][ni] lane holds
-// C[64*(w>>1) + 16mi + 4g + r][64*(w&1) + 16ni + l16].  MM: how a k-step is multiplied.
-template <typename T, typename MM = Mma<T>>
+// C[64*(w>>1) + 16mi + 4g + r][64*(w&1) + 16ni + l16].
+template <typename T>
 __device__ __forceinline__ void gemm_tile(const T *A, int64_t lda, int a_rows, const T *B, int64_t ldb, int b_rows,
                                           int K, floatx4 (&acc)[4][4], T *smem) {
-    constexpr int PITCH = MM::PITCH, R16 = Mma<T>::ROW16, EPC = 16 / sizeof(T);
+    using MM = Mma<T>;
+    constexpr int PITCH = MM::PITCH, R16 = MM::ROW16, EPC = 16 / sizeof(T);
     constexpr int LOADS = BM * R16 / THREADS;  // 16-byte loads per thread per operand
     // buffers by offset: a table of pointers loses their address space, and flat loads
     // from LDS wait for the global loads in flight as well
@@ -191,6 +144,92 @@ __device__ __forceinline__ void gemm_tile(const T *A, int64_t lda, int a_rows, c
     }
 }
 
+// The same tile of fp32 operands on the bf16 matrix units (token scores): every value is
+// split into three bf16 parts, x = hi + mid + lo with |mid| <= 2^-9 |x|, |lo| <= 2^-18
+// |x| and nothing left above 2^-27 |x|, and a product is the six part products down to
+// 2^-18; the three left out are below 2^-26 of it, less than one fp32 rounding.  Values
+// are split on their way from registers to LDS, once a block: 160 VALU instructions a
+// thread and k-step beside 96 MFMAs of 16 cycles, against 128 MFMAs of 32 cycles with
+// v_mfma_f32_16x16x4_f32.  LDS holds one k-step as three planes of 16-byte chunks,
+// XOR-swizzled like the bf16 tiles (48 KiB, so that two blocks share a CU and one
+// multiplies while the other splits); the next k-step's loads are in flight meanwhile.
+// Rows past the end of an operand re-read its last row.  Infinite operands give NaN.
+constexpr size_t SPLIT_SMEM = 3 * (BM + BN) * BK * sizeof(unsigned short);
+
+__device__ __forceinline__ void split_store(uint4 raw, unsigned short *lds) {
+    float v[4] = {__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w)};
+#pragma unroll
+    for (int part = 0; part < 3; ++part) {
+        const uint2 q = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        *reinterpret_cast<uint2 *>(lds + part * (BM + BN) * BK) = q;
+        v[0] -= __uint_as_float(q.x << 16);
+        v[1] -= __uint_as_float(q.x & 0xFFFF0000u);
+        v[2] -= __uint_as_float(q.y << 16);
+        v[3] -= __uint_as_float(q.y & 0xFFFF0000u);
+    }
+}
+
+__device__ __forceinline__ void split_tile(const float *A, int64_t lda, int a_rows, const float *B, int64_t ldb, int b_rows,
+                                           int K, floatx4 (&acc)[4][4], unsigned short *smem) {
+    constexpr int LOADS = BM * BK / 4 / THREADS;  // 16-byte loads a thread, operand and k-step
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int arow0 = 64 * (w >> 1), brow0 = BM + 64 * (w & 1);
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
+    const float *pa[LOADS], *pb[LOADS];
+    int to[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int row = (tid >> 3) + 32 * i, c = tid & 7;  // four values, half a chunk of eight
+        pa[i] = A + min(row, a_rows - 1) * lda + 4 * c;
+        pb[i] = B + min(row, b_rows - 1) * ldb + 4 * c;
+        to[i] = row * BK + 8 * ((c >> 1) ^ ((row >> 1) & 3)) + 4 * (c & 1);
+    }
+    uint4 ra[LOADS], rb[LOADS];
+    auto gload = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            ra[i] = *reinterpret_cast<const uint4 *>(pa[i] + k0);
+            rb[i] = *reinterpret_cast<const uint4 *>(pb[i] + k0);
+        }
+    };
+    auto fragment = [&](int row, int part) {
+        return *reinterpret_cast<const bf16x8 *>(smem + (part * (BM + BN) + row) * BK + 8 * (g ^ ((row >> 1) & 3)));
+    };
+    const int KT = K / BK;
+    gload(0);
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            split_store(ra[i], smem + to[i]);
+            split_store(rb[i], smem + BM * BK + to[i]);
+        }
+        __syncthreads();
+        gload(min(kt + 1, KT - 1) * BK);
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8 a[4][3];
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+            for (int part = 0; part < 3; ++part) a[mi][part] = fragment(arow0 + 16 * mi + l16, part);
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni) {
+            bf16x8 b[3];
+#pragma unroll
+            for (int part = 0; part < 3; ++part) b[part] = fragment(brow0 + 16 * ni + l16, part);
+            constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};  // small products first
+#pragma unroll
+            for (int j = 0; j < 6; ++j)
+#pragma unroll
+                for (int mi = 0; mi < 4; ++mi)
+                    acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mi][PA[j]], b[PB[j]], acc[mi][ni], 0, 0, 0);
+        }
+        __syncthreads();
+    }
+}
+
 // ------------------------------------------------------------ forward -----
 constexpr float LN2 = 0.6931471805599453f, LOG2 = 1.4426950408889634f;
 // u of a logit that is -inf or far below the maximum: 2^u is 0 and 2^u u is -0, not NaN
@@ -218,22 +257,29 @@ __device__ __forceinline__ void join_scores(float &m, float &s, float &t, float 
     m = nm;
 }
 
-// the product of the token scores' fp32 tiles
+template <typename T, bool SCORES> constexpr bool SPLIT = SCORES && std::is_same_v<T, float>;
+template <typename T, bool SCORES> constexpr size_t tile_smem() { return SPLIT<T, SCORES> ? SPLIT_SMEM : gemm_smem<T>(); }
+
 template <typename T, bool SCORES>
-using TileMma = Mma<std::conditional_t<SCORES && std::is_same_v<T, float>, SplitF32, T>>;
+__device__ __forceinline__ void logits_tile(const T *A, int64_t lda, int a_rows, const T *B, int64_t ldb, int b_rows, int K,
+                                            floatx4 (&acc)[4][4], unsigned char *smem) {
+    if constexpr (SPLIT<T, SCORES>)
+        split_tile(A, lda, a_rows, B, ldb, b_rows, K, acc, reinterpret_cast<unsigned short *>(smem));
+    else
+        gemm_tile<T>(A, lda, a_rows, B, ldb, b_rows, K, acc, reinterpret_cast<T *>(smem));
+}
 
 template <typename T, bool SCORES>
 __global__ void __launch_bounds__(THREADS) ce_fwd_tile_kernel(FwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    T *smem = reinterpret_cast<T *>(smem_raw);
     __shared__ float sM[2][BM], sS[2][BM], sT[2][SCORES ? BM : 1];
     __shared__ int sI[2][BM];
     const qpam_ce_fwd_args &a = p.a;
     const int vt = blockIdx.x, rt = blockIdx.y;
     const int r0 = rt * BM, v0 = vt * VT;
     floatx4 acc[4][4];
-    gemm_tile<T, TileMma<T, SCORES>>((const T *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(BM, a.N - r0),
-                                     (const T *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(BN, a.V - v0), a.D, acc, smem);
+    logits_tile<T, SCORES>((const T *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(BM, a.N - r0),
+                           (const T *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(BN, a.V - v0), a.D, acc, smem_raw);
 
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
@@ -490,7 +536,6 @@ template <> __device__ __forceinline__ unsigned short from_f32<unsigned short>(f
 template <typename T, bool SCORES>
 __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    T *smem = reinterpret_cast<T *>(smem_raw);
     __shared__ float sLse[BM], sScale[BM];
     __shared__ float sBase[SCORES ? BM : 1], sSlope[SCORES ? BM : 1], sExtra[SCORES ? BM : 1];
     __shared__ int sTgt[BM];
@@ -522,8 +567,8 @@ __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
         sTgt[tid] = tg;
     }
     floatx4 acc[4][4];
-    gemm_tile<T, TileMma<T, SCORES>>((const T *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(BM, p.rows - lr0),
-                                     (const T *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(BN, a.V - v0), a.D, acc, smem);
+    logits_tile<T, SCORES>((const T *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(BM, p.rows - lr0),
+                           (const T *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(BN, a.V - v0), a.D, acc, smem_raw);
     const int w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
     T *G = (T *)p.gbuf;
@@ -602,8 +647,8 @@ __global__ void __launch_bounds__(THREADS) split_gemm_kernel(const float *A, int
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN, k0 = blockIdx.z * kper;
     floatx4 acc[4][4];
-    gemm_tile<float, Mma<SplitF32>>(A + (int64_t)m0 * lda + k0, lda, min(BM, M - m0), B + (int64_t)n0 * ldb + k0, ldb,
-                                    min(BN, N - n0), min(kper, K - k0), acc, reinterpret_cast<float *>(smem_raw));
+    split_tile(A + (int64_t)m0 * lda + k0, lda, min(BM, M - m0), B + (int64_t)n0 * ldb + k0, ldb, min(BN, N - n0),
+               min(kper, K - k0), acc, reinterpret_cast<unsigned short *>(smem_raw));
     C += blockIdx.z * split_stride;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
@@ -1682,7 +1727,7 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
         hipLaunchKernelGGL(big::fwd_tile_kernel, grid, dim3(THREADS), big::SMEM, stream, p);
         st = launch_status("ce fwd_tile_kernel (bf16)");
     } else {
-        const size_t smem = gemm_smem<T>();
+        const size_t smem = scores ? tile_smem<T, true>() : tile_smem<T, false>();
         const void *kern = scores ? (const void *)ce_fwd_tile_kernel<T, true> : (const void *)ce_fwd_tile_kernel<T, false>;
         QPAM_CHECK_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         dim3 grid(p.n_vt, (a.N + BM - 1) / BM);
@@ -1906,7 +1951,7 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
     p.gtbuf = (T *)p.gbuf + (int64_t)chunk * p.Vp;
     p.ht = (T *)p.gtbuf + (int64_t)p.Vp * Rmax;
     float *part = (float *)(((uintptr_t)a.workspace + bwd_ws_base<T>(a) + 255) & ~(uintptr_t)255);
-    const size_t smem = gemm_smem<T>();
+    const size_t smem = SPLIT_SMEM;
     QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_grad_tile_kernel<T, true>,
                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)split_gemm_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
