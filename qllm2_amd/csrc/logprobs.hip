@@ -16,9 +16,9 @@
 //
 // Top alternatives without a sort or a second pass: the row's entries fall into 64
 // groups (one per lane), the k-th largest of the groups' maxima bounds the k-th
-// largest entry from below, and only threads whose own maximum reaches that bound
-// read their entries again (from the cache) and list those at or above it.  The
-// list, about k long, is ranked by counting.  Entries order by value, equal values
+// largest entry from below, and only the entries of threads whose own maximum reaches
+// that bound, about k threads, are read again (from the cache, by the whole block) and
+// those at or above it listed.  The list, about k long, is ranked by counting.  Entries order by value, equal values
 // by the lower index, through one 64-bit key.
 #include <algorithm>
 
@@ -136,15 +136,18 @@ __device__ __forceinline__ void top_by_passes(const Row<T> &row, int k, uint64_t
 template <typename T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
     constexpr int E = Vec<T>::E, WAVES = THREADS / 64;
-    constexpr int U = 16 / E;  // vectors of a batch: 16 entries
+    constexpr int U = 32 / E;  // vectors of a batch: 32 entries, 64 or 128 bytes a thread in flight
     __shared__ float sM[WAVES], sS[WAVES], sT[WAVES];
     __shared__ uint64_t sKey[TOP ? WAVES * 64 : 1], sCand[TOP ? CAP : 1], sTop[TOP ? MAX_K : 1];
     __shared__ uint64_t sBound;
-    __shared__ int sCount;
+    __shared__ int sCount, sOwners, sOwner[TOP ? THREADS : 1];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int64_t n = blockIdx.x;
     const Row<T> row(static_cast<const T *>(a.logits) + n * a.ld, a.V);
     const float inv_t = 1.f / a.temperature, c = inv_t * LOG2E;
+    const int64_t id = a.ids[n];
+    const bool valid = id != a.ignore_index && id >= 0 && id < a.V;
+    const float x_id = row.at(valid ? (int)id : 0);
 
     float m = -INFINITY, s = 0.f, t = 0.f;
     int batch_end = 0;  // the last entry of the batch that holds this thread's maximum
@@ -170,12 +173,12 @@ __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
     int v0 = row.lo + tid;
     for (; v0 + (U - 1) * THREADS < row.hi; v0 += U * THREADS) {
         uintx4 r[U];
-        float x[16];
+        float x[U * E];
 #pragma unroll
         for (int i = 0; i < U; ++i) r[i] = row.load(v0 + i * THREADS);
 #pragma unroll
         for (int i = 0; i < U; ++i) Vec<T>::unpack(r[i], x + i * E);
-        add(x, 16, row.first(v0 + (U - 1) * THREADS) + E - 1);
+        add(x, U * E, row.first(v0 + (U - 1) * THREADS) + E - 1);
     }
     for (; v0 < row.hi; v0 += THREADS) {
         float x[E];
@@ -205,7 +208,7 @@ __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
     }
     if (TOP) {
         sKey[w * 64 + lane] = m > -INFINITY ? make_key(m, batch_end) : 0ull;
-        if (tid == 0) sCount = 0;
+        if (tid == 0) sCount = sOwners = 0;
     }
     __syncthreads();
     s = t = 0.f;
@@ -217,9 +220,7 @@ __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
     const float ln_s = logf(s);
     auto logprob = [&](float x) { return empty ? -INFINITY : (x - M) * inv_t - ln_s; };
     if (tid == 0) {
-        const int64_t id = a.ids[n];
-        const bool valid = id != a.ignore_index && id >= 0 && id < a.V;
-        a.logprobs[n] = valid ? logprob(row.at((int)id)) : 0.f;
+        a.logprobs[n] = valid ? logprob(x_id) : 0.f;
         a.entropy[n] = empty ? 0.f : ln_s - LN2 * (t / s);
         if (a.stats) {
             a.stats[2 * n] = M;
@@ -252,13 +253,19 @@ __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
                 }
             };
             if (m > -INFINITY && order(m) >= (uint32_t)(bound >> 32)) {
-                for (int v = row.lo + tid; v < row.hi; v += THREADS) {
-                    float x[E];
-                    Vec<T>::unpack(row.load(v), x);
-#pragma unroll
-                    for (int i = 0; i < E; ++i) list(x[i], row.first(v) + i);
-                }
+                sOwner[atomicAdd(&sOwners, 1)] = tid;
                 if (edge >= 0) list(row.at(edge), edge);
+            }
+            __syncthreads();
+            // (owner, its j-th vector) over the block's threads
+            const int per = (row.hi - row.lo + THREADS - 1) / THREADS, total = sOwners * per;
+            for (int i = tid; i < total; i += THREADS) {
+                const int o = i / per, v = row.lo + sOwner[o] + (i - o * per) * THREADS;
+                if (v >= row.hi) continue;
+                float x[E];
+                Vec<T>::unpack(row.load(v), x);
+#pragma unroll
+                for (int j = 0; j < E; ++j) list(x[j], row.first(v) + j);
             }
             __syncthreads();
             count = sCount;
@@ -390,7 +397,7 @@ int launch_rows(const Args &a, hipStream_t stream) {
 
 template <typename T>
 int run_rows(const Args &a, hipStream_t stream) {
-    return a.n < 512 && a.V >= 16384 ? launch_rows<T, 1024>(a, stream) : launch_rows<T, 256>(a, stream);
+    return a.n <= 256 && a.V >= 16384 ? launch_rows<T, 1024>(a, stream) : launch_rows<T, 256>(a, stream);
 }
 
 template <typename T>
