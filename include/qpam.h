@@ -876,7 +876,7 @@ typedef struct {
 int qpam_logprobs_fwd(const qpam_logprobs_args *a, void *stream);
 int qpam_logprobs_bwd(const qpam_logprobs_args *a, void *stream);
 
-/* qpam_logprobs_fwd's logprobs, entropy and stats of the rows x = h w^T / temperature
+/* qpam_logprobs_fwd's logprobs and entropy of the rows x = h w^T / temperature
  * (h [N][D], w [V][D] as qpam_ce_fwd's) without logits in memory, and the gradient:
  * the tied LM head's token scores (logits of V11LM.ce_from_lm, v11/model.py:1175-1190).
  * bf16 operands: fp32 sums of exact products; the gradient's dx is rounded to bf16
@@ -891,8 +891,8 @@ typedef struct {
     const int64_t *ids;
     int64_t ignore_index;
     float temperature;
-    float *logprobs;               /* forward */
-    float *entropy, *stats;        /* written by the forward, read by the backward */
+    float *logprobs, *entropy;     /* written by the forward, read by the backward, */
+    float *stats;                  /* [N][2]: as are the rows' reference and sum */
     const float *g_logprobs, *g_entropy; /* each optional */
     void *dh; int64_t lddh;
     void *dw; int64_t lddw;

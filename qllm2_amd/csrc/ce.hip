@@ -21,11 +21,13 @@
 // softmax alive).
 //
 // Token scores (SCORES variants of the same kernels; qpam_linear_logprobs_*): the
-// log probability of each row's token and the entropy of the row.  With u = (x -
-// max) / T in units of log2 the tiles also reduce t = sum 2^u u, so that
-//   log prob = (x_token - max) / T - ln s,   entropy = ln s - ln2 t / s,
+// log probability of each row's token and the entropy of the row.  With c = log2(e) / T,
+// b = c max x rounded and u = c x - b (one fma, so b's rounding shifts every u alike and
+// cancels), the tiles reduce s = sum 2^u and t = sum 2^u u, so that
+//   log prob = ln2 (u_token - log2 s),   entropy = ln2 (log2 s - t / s),
 // and the gradient tiles write
 //   G_v = -p_v / T (g_lp + g_ent (ln p_v + entropy)) + [v = token] g_lp / T.
+// Logits with |c x| past fp32's range give NaN.
 #include <algorithm>
 #include <type_traits>
 
@@ -232,8 +234,7 @@ __device__ __forceinline__ void split_tile(const float *A, int64_t lda, int a_ro
 
 // ------------------------------------------------------------ forward -----
 constexpr float LN2 = 0.6931471805599453f, LOG2 = 1.4426950408889634f;
-// u of a logit that is -inf or far below the maximum: 2^u is 0 and 2^u u is -0, not NaN
-constexpr float U_FLOOR = -1e4f;
+constexpr float U_FLOOR = -1e4f;  // 2^u is 0 and 2^u u is -0, not NaN
 
 struct FwdParams {
     qpam_ce_fwd_args a;
@@ -243,18 +244,18 @@ struct FwdParams {
     float *red;              // [2] loss sum, denominator
     // token scores
     float *part_t;           // [N][n_vt] sum of 2^u u, in part_i's place
-    float inv_t, c;          // 1 / T, log2(e) / T
+    float c;                 // log2(e) / T
     float *logprobs, *entropy, *stats;
 };
 
-// (m, s, t) of two parts of a row's logits as one
-__device__ __forceinline__ void join_scores(float &m, float &s, float &t, float om, float os, float ot, float c) {
-    const float nm = fmaxf(m, om), lo = fmaxf(nm, -3.402823466e38f);
-    const float g = fmaxf((m - lo) * c, U_FLOOR), og = fmaxf((om - lo) * c, U_FLOOR);
+// (b, s, t) of two parts of a row's logits as one (b = -inf: a part of nothing)
+__device__ __forceinline__ void join_scores(float &b, float &s, float &t, float ob, float os, float ot) {
+    const float nb = fmaxf(b, ob), lo = fmaxf(nb, -3.402823466e38f);
+    const float g = fmaxf(b - lo, U_FLOOR), og = fmaxf(ob - lo, U_FLOOR);
     const float f = __builtin_amdgcn_exp2f(g), of = __builtin_amdgcn_exp2f(og);
     t = f * (t + s * g) + of * (ot + os * og);
     s = f * s + of * os;
-    m = nm;
+    b = nb;
 }
 
 template <typename T, bool SCORES> constexpr bool SPLIT = SCORES && std::is_same_v<T, float>;
@@ -302,16 +303,16 @@ __global__ void __launch_bounds__(THREADS) ce_fwd_tile_kernel(FwdParams p) {
                 if (om > mx || (om == mx && oi < ix)) { mx = om; ix = oi; }
             }
             float s = 0.f, t = 0.f;
-            const float lo = fmaxf(mx, -3.402823466e38f);
+            const float b = mx * p.c;
 #pragma unroll
             for (int ni = 0; ni < 4; ++ni) {
                 const int v = v0 + 64 * wn + 16 * ni + l16;
                 if (!SCORES) {
                     if (v < a.V) s += __expf(acc[mi][ni][r] - mx);
                 } else if (v < a.V) {
-                    const float u = (acc[mi][ni][r] - lo) * p.c, e = __builtin_amdgcn_exp2f(u);
+                    const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
                     s += e;
-                    t += e * fmaxf(u, U_FLOOR);
+                    t += e * u;
                 }
             }
 #pragma unroll
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(THREADS) ce_fwd_tile_kernel(FwdParams p) {
             if (SCORES) t = row16_sum(t);
             if (l16 == 0) {
                 const int row = 64 * wm + 16 * mi + 4 * g + r;
-                sM[wn][row] = mx;
+                sM[wn][row] = SCORES ? b : mx;
                 sS[wn][row] = s;
                 if (SCORES) sT[wn][row] = t;
                 else sI[wn][row] = ix;
@@ -329,10 +330,10 @@ __global__ void __launch_bounds__(THREADS) ce_fwd_tile_kernel(FwdParams p) {
     __syncthreads();
     if (SCORES) {
         if (tid < BM && r0 + tid < a.N) {
-            float m = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
-            join_scores(m, s, t, sM[1][tid], sS[1][tid], sT[1][tid], p.c);
+            float b = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
+            join_scores(b, s, t, sM[1][tid], sS[1][tid], sT[1][tid]);
             const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
-            p.part_m[o] = m;
+            p.part_m[o] = b;
             p.part_s[o] = s;
             p.part_t[o] = t;
         }
@@ -400,7 +401,7 @@ __global__ void __launch_bounds__(THREADS) ce_fwd_finalize_kernel(FwdParams p) {
     }
 }
 
-// one wave per row: merge the vocab tiles into (max, s, t), add the token's logit
+// one wave per row: merge the vocab tiles into (b, s, t), add the token's logit
 template <typename T>
 __global__ void __launch_bounds__(THREADS) scores_finalize_kernel(FwdParams p) {
     const qpam_ce_fwd_args &a = p.a;
@@ -409,14 +410,14 @@ __global__ void __launch_bounds__(THREADS) scores_finalize_kernel(FwdParams p) {
     if (row >= a.N) return;
     const int64_t id = a.targets[row];
     const bool valid = id != a.ignore_index && id >= 0 && id < a.V;
-    float m = -INFINITY, s = 0.f, t = 0.f;
+    float b = -INFINITY, s = 0.f, t = 0.f;
     for (int vt = lane; vt < p.n_vt; vt += 64) {
         const int64_t o = (int64_t)row * p.n_vt + vt;
-        join_scores(m, s, t, p.part_m[o], p.part_s[o], p.part_t[o], p.c);
+        join_scores(b, s, t, p.part_m[o], p.part_s[o], p.part_t[o]);
     }
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1)
-        join_scores(m, s, t, __shfl_xor(m, off), __shfl_xor(s, off), __shfl_xor(t, off), p.c);
+        join_scores(b, s, t, __shfl_xor(b, off), __shfl_xor(s, off), __shfl_xor(t, off));
     float dot = 0.f;
     if (valid) {
         constexpr int E = 16 / sizeof(T);  // rows are 16-byte aligned and whole vectors long
@@ -432,10 +433,10 @@ __global__ void __launch_bounds__(THREADS) scores_finalize_kernel(FwdParams p) {
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) dot += __shfl_xor(dot, off);
     if (lane == 0) {
-        const float ln_s = logf(s);
-        p.logprobs[row] = valid ? (dot - m) * p.inv_t - ln_s : 0.f;
-        p.entropy[row] = ln_s - LN2 * (t / s);
-        p.stats[2 * row] = m;
+        const float log_s = log2f(s);
+        p.logprobs[row] = valid ? LN2 * (__builtin_fmaf(dot, p.c, -b) - log_s) : 0.f;
+        p.entropy[row] = LN2 * (log_s - t / s);
+        p.stats[2 * row] = b;
         p.stats[2 * row + 1] = s;
     }
 }
@@ -489,23 +490,42 @@ struct BwdParams {
     int write_g;     // bf16 path: also write G (only the hand-written dH GEMM reads it)
     // token scores
     float inv_t, c;  // 1 / T, log2(e) / T
-    const float *stats, *entropy, *g_logprobs, *g_entropy;
+    const float *stats, *logprobs, *entropy, *g_logprobs, *g_entropy;
 };
 
-// A row's part of G_v = k 2^u (base + slope u) + [v = tgt] extra, u = (x - m) c
+// A row's part of G_v = 2^u (base + slope u), u = c x - b.  Zero for a row past the end.
 struct RowScore {
-    float m, k, base, slope, extra;
-    int tgt;
+    float b, base, slope;
 };
 
-__device__ __forceinline__ RowScore row_score(const BwdParams &p, int row) {
+__device__ __forceinline__ RowScore row_score(const BwdParams &p, int lr) {
+    if (lr >= p.rows) return {0.f, 0.f, 0.f};
     const qpam_ce_bwd_args &a = p.a;
+    const int row = p.row0 + lr;
     const int64_t id = a.targets[row];
     const bool valid = id != a.ignore_index && id >= 0 && id < a.V;
-    const float s = p.stats[2 * row + 1];
+    const float s = p.stats[2 * row + 1], k = -p.inv_t / s;
     const float g_lp = valid && p.g_logprobs ? p.g_logprobs[row] : 0.f, g_ent = p.g_entropy ? p.g_entropy[row] : 0.f;
-    return {p.stats[2 * row], -p.inv_t / s, g_lp + g_ent * (p.entropy[row] - logf(s)), g_ent * LN2, g_lp * p.inv_t,
-            valid ? (int)id : -1};
+    return {p.stats[2 * row], k * (g_lp + g_ent * (p.entropy[row] - LN2 * log2f(s))), k * g_ent * LN2};
+}
+
+// G at the rows' tokens, where the tiles left out the one-hot term: with p = e^logprob
+//   G = (g_lp (1 - p) - g_ent p (logprob + entropy)) / T.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) scores_token_kernel(BwdParams p) {
+    const qpam_ce_bwd_args &a = p.a;
+    const int lr = blockIdx.x * THREADS + threadIdx.x, row = p.row0 + lr;
+    if (lr >= p.rows) return;
+    const int64_t id = a.targets[row];
+    if (id == a.ignore_index || id < 0 || id >= a.V) return;
+    const float g_lp = p.g_logprobs ? p.g_logprobs[row] : 0.f, g_ent = p.g_entropy ? p.g_entropy[row] : 0.f;
+    const float lp = p.logprobs[row], q = expf(lp);
+    const float x = p.inv_t * (g_lp * (1.f - q) - g_ent * q * (lp + p.entropy[row]));
+    T v;
+    if constexpr (sizeof(T) == 2) v = __builtin_bit_cast(unsigned short, (__bf16)x);
+    else v = x;
+    static_cast<T *>(p.gtbuf)[id * p.Rp + lr] = v;
+    if (p.write_g) static_cast<T *>(p.gbuf)[(int64_t)lr * p.Vp + id] = v;
 }
 
 // out[c][r] = in[r][c] for an R x Cc tile grid (64 x 64 LDS tiles); rows >= R
@@ -537,7 +557,7 @@ template <typename T, bool SCORES>
 __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ float sLse[BM], sScale[BM];
-    __shared__ float sBase[SCORES ? BM : 1], sSlope[SCORES ? BM : 1], sExtra[SCORES ? BM : 1];
+    __shared__ float sSlope[SCORES ? BM : 1];
     __shared__ int sTgt[BM];
     const qpam_ce_bwd_args &a = p.a;
     const int vt = blockIdx.x, rt = blockIdx.y;
@@ -548,13 +568,10 @@ __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
         float lse = 0.f, sc = 0.f;
         int tg = -1;
         if (SCORES) {
-            const RowScore q = lr < p.rows ? row_score(p, row) : RowScore{};
-            lse = q.m;
-            sc = q.k;
-            tg = lr < p.rows ? q.tgt : -1;
-            sBase[tid] = q.base;
+            const RowScore q = row_score(p, lr);
+            lse = q.b;
+            sc = q.base;
             sSlope[tid] = q.slope;
-            sExtra[tid] = q.extra;
         } else if (lr < p.rows) {
             const int64_t t = a.targets[row];
             const bool valid = (t != a.ignore_index) && t >= 0 && t < a.V;
@@ -585,9 +602,8 @@ __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
                 float x = 0.f;
                 if (SCORES) {
                     if (v < a.V && lr0 + rl < p.rows) {
-                        const float u = (acc[mi][ni][r] - sLse[rl]) * p.c;
-                        x = sScale[rl] * __builtin_amdgcn_exp2f(u) * (sBase[rl] + sSlope[rl] * fmaxf(u, U_FLOOR));
-                        if (v == sTgt[rl]) x += sExtra[rl];
+                        const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -sLse[rl]);
+                        x = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(sSlope[rl], u, sScale[rl]);
                     }
                 } else if (v < a.V && sScale[rl] != 0.f) {
                     x = __expf(acc[mi][ni][r] - sLse[rl]);
@@ -1225,10 +1241,10 @@ __device__ __forceinline__ void wave_lds_sync() {
 // Row statistics over a wave's 128 columns: per lane over its 8 columns, then
 // across the 16 lanes that hold the row (DPP); the argmax (first column at the
 // maximum) only when accuracy counts are requested.
-template <bool ARGMAX, bool SCORES>
+template <bool ARGMAX>
 __global__ void __launch_bounds__(WTHREADS) fwd_tile_kernel(FwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    __shared__ float sM[2][TM], sS[2][TM], sT[2][SCORES ? TM : 1];
+    __shared__ float sM[2][TM], sS[2][TM];
     __shared__ int sI[2][TM];
     const qpam_ce_fwd_args &a = p.a;
     const int n_rt = (a.N + TM - 1) / TM;
@@ -1258,19 +1274,9 @@ __global__ void __launch_bounds__(WTHREADS) fwd_tile_kernel(FwdParams p) {
             for (int ni = 0; ni < 8; ++ni)
                 if (full || vl + 16 * ni < a.V) lm = fmaxf(lm, acc[mi][ni][r]);
             const float mx = row16_max(lm);
-            float s = 0.f, t = 0.f;
+            float s = 0.f;
             int ix = 0x7fffffff;
-            if (SCORES) {
-                const float lo = fmaxf(mx, -3.402823466e38f);
-#pragma unroll
-                for (int ni = 0; ni < 8; ++ni)
-                    if (full || vl + 16 * ni < a.V) {
-                        const float u = (acc[mi][ni][r] - lo) * p.c, e = __builtin_amdgcn_exp2f(u);
-                        s += e;
-                        t += e * fmaxf(u, U_FLOOR);
-                    }
-                t = row16_sum(t);
-            } else if (mx > -INFINITY) {
+            if (mx > -INFINITY) {
                 const float mx2 = mx * LOG2E;  // exp(x - mx) = exp2(x log2e - mx log2e)
 #pragma unroll
                 for (int ni = 0; ni < 8; ++ni)
@@ -1286,23 +1292,11 @@ __global__ void __launch_bounds__(WTHREADS) fwd_tile_kernel(FwdParams p) {
                 const int row = 64 * wm + 16 * mi + 4 * g + r;
                 sM[wn][row] = mx;
                 sS[wn][row] = s;
-                if (SCORES) sT[wn][row] = t;
                 if (ARGMAX) sI[wn][row] = ix;
             }
         }
     }
     __syncthreads();
-    if (SCORES) {
-        if (tid < TM && r0 + tid < a.N) {
-            float m = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
-            join_scores(m, s, t, sM[1][tid], sS[1][tid], sT[1][tid], p.c);
-            const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
-            p.part_m[o] = m;
-            p.part_s[o] = s;
-            p.part_t[o] = t;
-        }
-        return;
-    }
     if (tid < TM && r0 + tid < a.N) {
         const float m0 = sM[0][tid], m1 = sM[1][tid];
         const float m = fmaxf(m0, m1);
@@ -1318,11 +1312,9 @@ __global__ void __launch_bounds__(WTHREADS) fwd_tile_kernel(FwdParams p) {
 
 // backward G tile (256 rows x 256 vocab): recompute logits, write G^T [Vp][Rp]
 // (and G [rows][Vp] when write_g)
-template <bool SCORES>
 __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ float sLse[TM], sScale[TM];
-    __shared__ float sBase[SCORES ? TM : 1], sSlope[SCORES ? TM : 1], sExtra[SCORES ? TM : 1];
     __shared__ int sTgt[TM];
     const qpam_ce_bwd_args &a = p.a;
     const int n_rt = p.Rp / TM, n_vt = p.Vp / TN;
@@ -1336,15 +1328,7 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
         const int lr = lr0 + tid, row = p.row0 + lr;
         float lse = 0.f, sc = 0.f;
         int tg = -1;
-        if (SCORES) {
-            const RowScore q = lr < p.rows ? row_score(p, row) : RowScore{};
-            lse = q.m;
-            sc = q.k;
-            tg = lr < p.rows ? q.tgt : -1;
-            sBase[tid] = q.base;
-            sSlope[tid] = q.slope;
-            sExtra[tid] = q.extra;
-        } else if (lr < p.rows) {
+        if (lr < p.rows) {
             const int64_t t = a.targets[row];
             const bool valid = (t != a.ignore_index) && t >= 0 && t < a.V;
             lse = a.lse[row];
@@ -1379,7 +1363,6 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
     // +inf for rows without a gradient (their G is exp2(-inf) = 0), the scale and
     // the target column
     float hl[4][4], hs[4][4];
-    float hb[SCORES ? 4 : 1][4], hd[SCORES ? 4 : 1][4];
     int ht[4][4];
 #pragma unroll
     for (int mi = 0; mi < 4; ++mi)
@@ -1387,17 +1370,10 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
         for (int r = 0; r < 4; ++r) {
             const int rl = 64 * wm + 16 * mi + 4 * g + r;
             hs[mi][r] = sScale[rl];
-            if constexpr (SCORES) {
-                hl[mi][r] = sLse[rl];
-                hb[mi][r] = sBase[rl];
-                hd[mi][r] = sSlope[rl];
-            } else {
-                hl[mi][r] = hs[mi][r] != 0.f ? sLse[rl] * LOG2E : INFINITY;
-            }
+            hl[mi][r] = hs[mi][r] != 0.f ? sLse[rl] * LOG2E : INFINITY;
             ht[mi][r] = sTgt[rl];
         }
     const bool full = v0 + TN <= a.V;  // every column of the tile is a vocabulary entry
-    const bool fullr = lr0 + TM <= p.rows;
 #pragma unroll
     for (int ni = 0; ni < 8; ++ni) {
         const int vb = v0 + 128 * wn + 16 * ni, v = vb + l16;
@@ -1408,15 +1384,8 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
             float x[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                if constexpr (SCORES) {
-                    const float u = (acc[mi][ni][r] - hl[mi][r]) * p.c;
-                    float y = hs[mi][r] * __builtin_amdgcn_exp2f(u) * (hb[mi][r] + hd[mi][r] * fmaxf(u, U_FLOOR));
-                    if (v == ht[mi][r]) y += sExtra[rl0 + r];
-                    x[r] = vok && (fullr || lr0 + rl0 + r < p.rows) ? y : 0.f;
-                } else {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][ni][r], LOG2E, -hl[mi][r]));
-                    x[r] = vok ? (e - (v == ht[mi][r] ? 1.f : 0.f)) * hs[mi][r] : 0.f;
-                }
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][ni][r], LOG2E, -hl[mi][r]));
+                x[r] = vok ? (e - (v == ht[mi][r] ? 1.f : 0.f)) * hs[mi][r] : 0.f;
             }
             const unsigned lo = pack_bf16x2(x[0], x[1]), hi = pack_bf16x2(x[2], x[3]);
             if (p.write_g) {
@@ -1443,6 +1412,261 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
     }
 }
 }  // namespace wide
+
+// Token scores' bf16 tiles, 256 x 256: loads, swizzle and wave layout as in `wide`, with a
+// k-step's first fragments read from LDS between the MFMAs of the step before, so that no
+// wave waits for LDS at the head of a step.
+namespace tiles {
+constexpr int TM = wide::TM, TN = wide::TN, DK = wide::DK, TT = wide::WTHREADS;
+using U16 = unsigned short;
+
+struct Stage {
+    U16 a[TM * DK], b[TN * DK];
+};
+struct Frags {
+    bf16x8 a[4], b[4];  // the step's A fragments and the first half of its B fragments
+};
+// A wave's four loads of a stage (16 rows of 64 bytes each, two of A and two of B): a
+// uniform base that advances and 32-bit offsets that stay (row strides below 2^22).
+struct Loads {
+    const char *a, *b;
+    unsigned ao[2], bo[2];
+};
+
+__device__ __forceinline__ void to_lds(const char *from, U16 *lds) {
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const unsigned *>(from), reinterpret_cast<unsigned *>(lds), 16, 0, 0);
+}
+__device__ __forceinline__ void load(Stage &s, const Loads &q, int step) {
+    const int w = threadIdx.x >> 6;
+    const char *a = q.a + (int64_t)step * (2 * DK), *b = q.b + (int64_t)step * (2 * DK);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        to_lds(a + q.ao[j], &s.a[(32 * w + 16 * j) * DK]);
+        to_lds(b + q.bo[j], &s.b[(32 * w + 16 * j) * DK]);
+    }
+}
+
+__device__ __forceinline__ bf16x8 fragment(const U16 *at, int i) {
+    return *reinterpret_cast<const bf16x8 *>(at + 16 * i * DK);
+}
+
+// The products of a step: the second half of its B fragments is read in front of the
+// products of the first, the next step's first fragments (stage s) between those of the second.
+__device__ __forceinline__ void step(const Frags &cur, const Stage &c, Frags &next, const Stage &s, floatx4 (&acc)[4][8], int aat,
+                                     int bat) {
+    bf16x8 late[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) late[i] = fragment(c.b + bat, 4 + i);
+#pragma unroll
+    for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi)
+            acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur.a[mi], cur.b[ni], acc[mi][ni], 0, 0, 0);
+#pragma unroll
+    for (int ni = 0; ni < 4; ++ni) {
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi)
+            acc[mi][4 + ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur.a[mi], late[ni], acc[mi][4 + ni], 0, 0, 0);
+        next.a[ni] = fragment(s.a + aat, ni);
+        next.b[ni] = fragment(s.b + bat, ni);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);   // LDS reads
+    __builtin_amdgcn_sched_group_barrier(0x008, 16, 0);  // MFMAs
+#pragma unroll
+    for (int ni = 0; ni < 4; ++ni) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+}
+
+// acc[mi][ni] lane holds C[64*(w>>1) + 16mi + 4g + r][128*(w&1) + 16ni + l16]; K % 32 == 0.
+// Step kt multiplies stage kt, reads the first fragments of stage kt + 1 and starts the
+// loads of stage kt + 3, four a wave (past the end they re-read the last step): at its end
+// "stage kt + 2 landed" is vmcnt <= 4.  Rows past the end of an operand re-read its last
+// row.  The stages are free and no load is in flight when it returns.
+__device__ __forceinline__ void product(const U16 *A, int64_t lda, int a_rows, const U16 *B, int64_t ldb, int b_rows, int K,
+                                        floatx4 (&acc)[4][8], Stage &s0, Stage &s1, Stage &s2, Stage &s3) {
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 8; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
+    Loads q{reinterpret_cast<const char *>(A), reinterpret_cast<const char *>(B), {}, {}};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int row = 32 * w + 16 * j + (lane >> 2), c = 16 * wide::swz(row, lane & 3);
+        q.ao[j] = 2u * (unsigned)min(row, a_rows - 1) * (unsigned)lda + c;
+        q.bo[j] = 2u * (unsigned)min(row, b_rows - 1) * (unsigned)ldb + c;
+    }
+    // fragment (row, chunk g); the swizzle repeats every eight rows
+    const int aat = (64 * (w >> 1) + l16) * DK + 8 * wide::swz(l16, g), bat = (128 * (w & 1) + l16) * DK + 8 * wide::swz(l16, g);
+    const int KT = K / DK;
+    load(s0, q, 0);
+    load(s1, q, min(1, KT - 1));
+    load(s2, q, min(2, KT - 1));
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(4));
+    __builtin_amdgcn_s_barrier();
+    Frags f0, f1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f0.a[i] = fragment(s0.a + aat, i);
+        f0.b[i] = fragment(s0.b + bat, i);
+    }
+#define QPAM_STEP(KT_, CUR, STAGE, NEXT, NEXT_STAGE, FREE)                                     \
+    load(FREE, q, min((KT_) + 3, KT - 1));                                                     \
+    step(CUR, STAGE, NEXT, NEXT_STAGE, acc, aat, bat);                                         \
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(4));                                                 \
+    __builtin_amdgcn_s_barrier();
+    int kt = 0;
+    for (; kt + 3 < KT; kt += 4) {
+        QPAM_STEP(kt, f0, s0, f1, s1, s3)
+        QPAM_STEP(kt + 1, f1, s1, f0, s2, s0)
+        QPAM_STEP(kt + 2, f0, s2, f1, s3, s1)
+        QPAM_STEP(kt + 3, f1, s3, f0, s0, s2)
+    }
+    if (kt < KT) { QPAM_STEP(kt, f0, s0, f1, s1, s3) }
+    if (kt + 1 < KT) { QPAM_STEP(kt + 1, f1, s1, f0, s2, s0) }
+    if (kt + 2 < KT) { QPAM_STEP(kt + 2, f0, s2, f1, s3, s1) }
+#undef QPAM_STEP
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    __builtin_amdgcn_s_barrier();
+}
+
+__global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
+    __shared__ __align__(16) Stage s0, s1, s2, s3;
+    __shared__ float sB[2][TM], sS[2][TM], sT[2][TM];
+    const qpam_ce_fwd_args &a = p.a;
+    const int n_rt = (a.N + TM - 1) / TM;
+    const int item = big::xcd_item(blockIdx.x, n_rt * p.n_vt);
+    if (item >= n_rt * p.n_vt) return;
+    int rt, vt;
+    big::grouped_tile(item, n_rt, p.n_vt, rt, vt);
+    const int r0 = rt * TM, v0 = vt * TN;
+    floatx4 acc[4][8];
+    product((const U16 *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0), (const U16 *)a.w + (int64_t)v0 * a.ldw, a.ldw,
+            min(TN, a.V - v0), a.D, acc, s0, s1, s2, s3);
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wm = w >> 1, wn = w & 1;
+    const int vl = v0 + 128 * wn + l16;  // this lane's column in tile ni: vl + 16 ni
+    auto rows = [&](auto whole) {        // whole: no column past the vocabulary
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int ni = 0; ni < 8; ++ni)
+                    if (whole || vl + 16 * ni < a.V) mx = fmaxf(mx, acc[mi][ni][r]);
+                const float b = row16_max(mx) * p.c;
+                float s = 0.f, t = 0.f;
+#pragma unroll
+                for (int ni = 0; ni < 8; ++ni)
+                    if (whole || vl + 16 * ni < a.V) {
+                        const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
+                        s += e;
+                        t = __builtin_fmaf(e, u, t);
+                    }
+                s = row16_sum(s);
+                t = row16_sum(t);
+                if (l16 == 0) {
+                    const int row = 64 * wm + 16 * mi + 4 * g + r;
+                    sB[wn][row] = b;
+                    sS[wn][row] = s;
+                    sT[wn][row] = t;
+                }
+            }
+        }
+    };
+    if (v0 + TN <= a.V) rows(std::true_type{});
+    else rows(std::false_type{});
+    __syncthreads();
+    if (tid < TM && r0 + tid < a.N) {
+        float b = sB[0][tid], s = sS[0][tid], t = sT[0][tid];
+        join_scores(b, s, t, sB[1][tid], sS[1][tid], sT[1][tid]);
+        const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
+        p.part_m[o] = b;
+        p.part_s[o] = s;
+        p.part_t[o] = t;
+    }
+}
+
+// G^T [Vp][Rp] (and G [rows][Vp] when write_g) without the tokens' one-hot terms; zero past
+// the vocabulary and past the rows.  A 16-wide vocab slab of a wave goes through LDS (the
+// stages' space) and leaves as 128-byte runs of G^T.
+__global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
+    __shared__ __align__(16) Stage s0, s1, s2, s3;
+    __shared__ float sB[TM], sBase[TM], sSlope[TM];
+    const qpam_ce_bwd_args &a = p.a;
+    const int n_rt = p.Rp / TM, n_vt = p.Vp / TN;
+    const int item = big::xcd_item(blockIdx.x, n_rt * n_vt);
+    if (item >= n_rt * n_vt) return;
+    int rt, vt;
+    big::grouped_tile(item, n_rt, n_vt, rt, vt);
+    const int lr0 = rt * TM, v0 = vt * TN, tid = threadIdx.x;
+    if (tid < TM) {
+        const RowScore q = row_score(p, lr0 + tid);
+        sB[tid] = q.b;
+        sBase[tid] = q.base;
+        sSlope[tid] = q.slope;
+    }
+    floatx4 acc[4][8];
+    product((const U16 *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(TM, p.rows - lr0),
+            (const U16 *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(TN, a.V - v0), a.D, acc, s0, s1, s2, s3);
+    const int w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wm = w >> 1, wn = w & 1;
+    U16 *G = (U16 *)p.gbuf;
+    U16 *GT = (U16 *)p.gtbuf;
+    constexpr int LD = 72;  // bf16 per staged vocab row: 64 tile rows + padding against bank conflicts
+    static_assert(8 * 16 * LD <= TM * DK + TN * DK, "the slabs of eight waves fit one stage");
+    U16 *slab = reinterpret_cast<U16 *>(&s0) + w * 16 * LD;
+    // the 16 rows of this lane (rows 64 wm + 16 mi + 4 g + r)
+    float hb[4][4], h0[4][4], h1[4][4];
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int rl = 64 * wm + 16 * mi + 4 * g + r;
+            hb[mi][r] = sB[rl];
+            h0[mi][r] = sBase[rl];
+            h1[mi][r] = sSlope[rl];
+        }
+    auto slabs = [&](auto whole) {  // whole: every column is a vocabulary entry, every row a row
+#pragma unroll
+        for (int ni = 0; ni < 8; ++ni) {
+            const int vb = v0 + 128 * wn + 16 * ni, v = vb + l16;
+#pragma unroll
+            for (int mi = 0; mi < 4; ++mi) {
+                const int rl0 = 64 * wm + 16 * mi + 4 * g;
+                float x[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -hb[mi][r]);
+                    x[r] = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(h1[mi][r], u, h0[mi][r]);
+                    if (!whole && (v >= a.V || lr0 + rl0 + r >= p.rows)) x[r] = 0.f;
+                }
+                const unsigned lo = pack_bf16x2(x[0], x[1]), hi = pack_bf16x2(x[2], x[3]);
+                if (p.write_g) {
+                    const U16 gb[4] = {(U16)(lo & 0xFFFFu), (U16)(lo >> 16), (U16)(hi & 0xFFFFu), (U16)(hi >> 16)};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (lr0 + rl0 + r < p.rows) G[(int64_t)(lr0 + rl0 + r) * p.Vp + v] = gb[r];
+                }
+                *reinterpret_cast<uint2 *>(slab + l16 * LD + 16 * mi + 4 * g) = make_uint2(lo, hi);
+            }
+            wide::wave_lds_sync();  // the slab is this wave's own
+            const int vl = lane >> 2, part = lane & 3;  // vocab row, 16 tile rows: 32 bytes a lane
+            const uint4 *src = reinterpret_cast<const uint4 *>(slab + vl * LD + 16 * part);
+            const uint4 d0 = src[0], d1 = src[1];
+            uint4 *dst = reinterpret_cast<uint4 *>(GT + (int64_t)(vb + vl) * p.Rp + lr0 + 64 * wm + 16 * part);
+            dst[0] = d0;
+            dst[1] = d1;
+            wide::wave_lds_sync();
+        }
+    };
+    if (v0 + TN <= a.V && lr0 + TM <= p.rows) slabs(std::true_type{});
+    else slabs(std::false_type{});
+}
+}  // namespace tiles
 
 // Token scores of few rows (a decode step's), bound by reading the table once.  A wave
 // takes 16 table rows and every hidden row, 16 MI of them.  The table streams global ->
@@ -1566,31 +1790,31 @@ __global__ void __launch_bounds__(64 * NW) scores_kernel(FwdParams p) {
             if (v0 + 4 * g + r < a.V) m = fmaxf(m, acc[mi][r]);
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
-        const float lo = fmaxf(m, -3.402823466e38f);
+        const float b = m * p.c;
         float s = 0.f, t = 0.f;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (v0 + 4 * g + r < a.V) {
-                const float u = (acc[mi][r] - lo) * p.c, e = __builtin_amdgcn_exp2f(u);
+                const float u = __builtin_fmaf(acc[mi][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
                 s += e;
-                t += e * fmaxf(u, U_FLOOR);
+                t += e * u;
             }
         s += __shfl_xor(s, 16);
         t += __shfl_xor(t, 16);
         s += __shfl_xor(s, 32);
         t += __shfl_xor(t, 32);
         if (g == 0) {
-            sM[w][16 * mi + l16] = m;
+            sM[w][16 * mi + l16] = b;
             sS[w][16 * mi + l16] = s;
             sT[w][16 * mi + l16] = t;
         }
     }
     __syncthreads();
     if (tid < 16 * MI && tid < a.N) {
-        float m = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
-        for (int v = 1; v < NW; ++v) join_scores(m, s, t, sM[v][tid], sS[v][tid], sT[v][tid], p.c);
+        float b = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
+        for (int v = 1; v < NW; ++v) join_scores(b, s, t, sM[v][tid], sS[v][tid], sT[v][tid]);
         const int64_t o = (int64_t)tid * p.n_vt + blockIdx.x;
-        p.part_m[o] = m;
+        p.part_m[o] = b;
         p.part_s[o] = s;
         p.part_t[o] = t;
     }
@@ -1706,19 +1930,19 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     int st;
     if (few) {
         st = thin::waves(a.V) == 16 ? thin::launch<T, 16>(p, stream) : thin::launch<T, 4>(p, stream);
+    } else if (scores && is_bf<T>()) {
+        const dim3 grid(big::xcd_grid(p.n_vt * ((a.N + tiles::TM - 1) / tiles::TM)));
+        hipLaunchKernelGGL(tiles::scores_tile_kernel, grid, dim3(tiles::TT), 0, stream, p);
+        st = launch_status("scores_tile_kernel");
     } else if (wide_tiles) {
         // the argmax (accuracy counts) only when requested
-        const void *kern = scores      ? (const void *)wide::fwd_tile_kernel<false, true>
-                           : a.correct ? (const void *)wide::fwd_tile_kernel<true, false>
-                                       : (const void *)wide::fwd_tile_kernel<false, false>;
+        const void *kern = a.correct ? (const void *)wide::fwd_tile_kernel<true> : (const void *)wide::fwd_tile_kernel<false>;
         QPAM_CHECK_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)wide::KSMEM));
         dim3 grid(big::xcd_grid(p.n_vt * ((a.N + wide::TM - 1) / wide::TM)));
-        if (scores)
-            hipLaunchKernelGGL((wide::fwd_tile_kernel<false, true>), grid, dim3(wide::WTHREADS), wide::KSMEM, stream, p);
-        else if (a.correct)
-            hipLaunchKernelGGL((wide::fwd_tile_kernel<true, false>), grid, dim3(wide::WTHREADS), wide::KSMEM, stream, p);
+        if (a.correct)
+            hipLaunchKernelGGL(wide::fwd_tile_kernel<true>, grid, dim3(wide::WTHREADS), wide::KSMEM, stream, p);
         else
-            hipLaunchKernelGGL((wide::fwd_tile_kernel<false, false>), grid, dim3(wide::WTHREADS), wide::KSMEM, stream, p);
+            hipLaunchKernelGGL(wide::fwd_tile_kernel<false>, grid, dim3(wide::WTHREADS), wide::KSMEM, stream, p);
         st = launch_status("ce fwd_tile_kernel (bf16, 256 x 256)");
     } else if (is_bf<T>()) {
         QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)big::fwd_tile_kernel,
@@ -1766,16 +1990,20 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
     const bool wide_tiles = scores || use_wide(a.D);
     // the G-tile kernel: 256 x 256 tiles, or 256 x 128 for hidden sizes that are not
     // a multiple of 64 (Vp and Rp are multiples of both)
-    const void *gkern = scores       ? (const void *)wide::grad_tile_kernel<true>
-                        : wide_tiles ? (const void *)wide::grad_tile_kernel<false>
-                                     : (const void *)big::grad_tile_kernel;
+    const void *gkern = wide_tiles ? (const void *)wide::grad_tile_kernel : (const void *)big::grad_tile_kernel;
     const size_t gsmem = wide_tiles ? wide::KSMEM : big::SMEM;
     auto launch_grad = [&]() {
+        if (scores) {
+            hipLaunchKernelGGL(tiles::scores_grad_kernel, dim3(big::xcd_grid((p.Vp / tiles::TN) * (p.Rp / tiles::TM))),
+                               dim3(tiles::TT), 0, stream, p);
+            const int st = launch_status("scores_grad_kernel");
+            if (st) return st;
+            hipLaunchKernelGGL(scores_token_kernel<U>, dim3((p.rows + THREADS - 1) / THREADS), dim3(THREADS), 0, stream, p);
+            return launch_status("scores_token_kernel");
+        }
         const int tiles = (p.Vp / (wide_tiles ? wide::TN : big::BTN)) * (p.Rp / big::BTM);
-        if (scores)
-            hipLaunchKernelGGL(wide::grad_tile_kernel<true>, dim3(big::xcd_grid(tiles)), dim3(wide::WTHREADS), gsmem, stream, p);
-        else if (wide_tiles)
-            hipLaunchKernelGGL(wide::grad_tile_kernel<false>, dim3(big::xcd_grid(tiles)), dim3(wide::WTHREADS), gsmem, stream, p);
+        if (wide_tiles)
+            hipLaunchKernelGGL(wide::grad_tile_kernel, dim3(big::xcd_grid(tiles)), dim3(wide::WTHREADS), gsmem, stream, p);
         else
             hipLaunchKernelGGL(big::grad_tile_kernel, dim3(big::xcd_grid(tiles)), dim3(THREADS), gsmem, stream, p);
         return launch_status(wide_tiles ? "ce grad_tile_kernel (bf16, 256 x 256)" : "ce grad_tile_kernel (bf16)");
@@ -1968,6 +2196,8 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
         if ((st = launch_status("transpose_kernel(H)"))) return st;
         hipLaunchKernelGGL((ce_grad_tile_kernel<T, true>), dim3(p.Vp / VT, p.Rp / BM), dim3(THREADS), smem, stream, p);
         if ((st = launch_status("ce_grad_tile_kernel"))) return st;
+        hipLaunchKernelGGL(scores_token_kernel<T>, dim3((p.rows + THREADS - 1) / THREADS), dim3(THREADS), 0, stream, p);
+        if ((st = launch_status("scores_token_kernel"))) return st;
         // dH[r0 .. r0 + rows] = G [rows][Vp] (W^T [D][Vp])^T
         const int splits = dh_splits(p.rows, a.D, p.Vp), kper = round_up((p.Vp + splits - 1) / splits, BK);
         float *dh = (float *)a.dh + (int64_t)r0 * a.lddh;
@@ -2049,6 +2279,7 @@ int validate_scores(const qpam_linear_logprobs_args &a, const char *who) {
                  a.temperature);
     QPAM_REQUIRE(a.entropy && a.stats, "%s: null entropy or stats", who);
     QPAM_REQUIRE((a.N + BM - 1) / BM <= 65535, "%s: too many rows", who);
+    QPAM_REQUIRE(a.ldh < (1 << 22) && a.ldw < (1 << 22), "%s: row strides of 2^22 elements or more", who);
     return QPAM_OK;
 }
 
@@ -2118,8 +2349,7 @@ extern "C" int qpam_linear_logprobs_fwd(const qpam_linear_logprobs_args *a, void
     QPAM_REQUIRE(a->workspace && a->workspace_bytes >= need && ((uintptr_t)a->workspace % 16) == 0,
                  "qpam_linear_logprobs_fwd: workspace needs %zu bytes (got %zu)", need, a->workspace_bytes);
     FwdParams p = {};
-    p.inv_t = 1.f / a->temperature;
-    p.c = p.inv_t * LOG2;
+    p.c = LOG2 / a->temperature;
     p.logprobs = a->logprobs;
     p.entropy = a->entropy;
     p.stats = a->stats;
@@ -2140,7 +2370,7 @@ extern "C" int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void
     QPAM_REQUIRE(a != nullptr, "qpam_linear_logprobs_bwd: null args");
     int st = validate_scores(*a, "qpam_linear_logprobs_bwd");
     if (st) return st;
-    QPAM_REQUIRE(a->dh && a->dw, "qpam_linear_logprobs_bwd: null dh or dw");
+    QPAM_REQUIRE(a->logprobs && a->dh && a->dw, "qpam_linear_logprobs_bwd: null logprobs, dh or dw");
     QPAM_REQUIRE(a->chunk >= 1, "qpam_linear_logprobs_bwd: chunk must be >= 1");
     QPAM_REQUIRE(a->lddh >= a->D && a->lddw >= a->D, "qpam_linear_logprobs_bwd: output leading dims must be >= D");
     QPAM_REQUIRE(a->dw_out == 1 || a->dw_out == 2, "qpam_linear_logprobs_bwd: dw_out must be 1 or 2");
@@ -2149,8 +2379,9 @@ extern "C" int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void
                  "qpam_linear_logprobs_bwd: workspace needs %zu bytes (got %zu)", need, a->workspace_bytes);
     BwdParams p = {};
     p.inv_t = 1.f / a->temperature;
-    p.c = p.inv_t * LOG2;
+    p.c = LOG2 / a->temperature;
     p.stats = a->stats;
+    p.logprobs = a->logprobs;
     p.entropy = a->entropy;
     p.g_logprobs = a->g_logprobs;
     p.g_entropy = a->g_entropy;

@@ -181,12 +181,12 @@ def _check_linear(hidden_rows, weight_matrix, ids, temperature, chunk):
     _check_temperature(temperature, name)
 
 
-def _linear_args(h, w, dtype, ids, entropy, stats, temperature, ignore_index):
+def _linear_args(h, w, dtype, ids, logprobs, entropy, stats, temperature, ignore_index):
     a = _lib.LinearLogprobsArgs()
     a.N, a.V, a.D, a.dtype, a.temperature = h.shape[0], w.shape[0], h.shape[1], dtype, temperature
     a.h, a.ldh, a.w, a.ldw = h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0)
     a.ids, a.ignore_index = ids.data_ptr(), ignore_index
-    a.entropy, a.stats = entropy.data_ptr(), stats.data_ptr()
+    a.logprobs, a.entropy, a.stats = logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr()
     return a
 
 
@@ -205,8 +205,7 @@ def _linear_forward(hidden_rows: Tensor, weight_matrix: Tensor, weight_copy: Opt
     lp, ent, stats = (torch.empty(s, device=dev, dtype=torch.float32) for s in ((n,), (n,), (n, 2)))
     if n:
         ids = ids.contiguous()
-        a = _linear_args(h, w, dtype, ids, ent, stats, temperature, ignore_index)
-        a.logprobs = lp.data_ptr()
+        a = _linear_args(h, w, dtype, ids, lp, ent, stats, temperature, ignore_index)
         L = _lib.lib()
         ws = _workspace(a, L.qpam_linear_logprobs_fwd_workspace_size(ctypes.byref(a)), dev)  # noqa: F841
         with _lib.device(dev):
@@ -224,8 +223,8 @@ def _(hidden_rows, weight_matrix, weight_copy, ids, temperature, chunk, ignore_i
     return [f(n), f(n), f(n, 2)]
 
 
-def _linear_gradient(hidden_rows: Tensor, weight_matrix: Tensor, ids: Tensor, entropy: Tensor, stats: Tensor,
-                     g_logprobs: Optional[Tensor], g_entropy: Optional[Tensor], temperature: float, chunk: int,
+def _linear_gradient(hidden_rows: Tensor, weight_matrix: Tensor, ids: Tensor, logprobs: Tensor, entropy: Tensor,
+                     stats: Tensor, g_logprobs: Optional[Tensor], g_entropy: Optional[Tensor], temperature: float, chunk: int,
                      ignore_index: int, dw_fp32: bool) -> List[Tensor]:
     """[d hidden_rows, d weight_matrix] in the inputs' dtypes (d weight_matrix in fp32
     with dw_fp32)."""
@@ -238,7 +237,7 @@ def _linear_gradient(hidden_rows: Tensor, weight_matrix: Tensor, ids: Tensor, en
         return [dh.to(hidden_rows.dtype), dw.zero_()]
     ids = ids.contiguous()
     gs = [g if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy)]
-    a = _linear_args(h, w, dtype, ids, entropy, stats, temperature, ignore_index)
+    a = _linear_args(h, w, dtype, ids, logprobs, entropy, stats, temperature, ignore_index)
     a.g_logprobs, a.g_entropy = (g if g is None else g.data_ptr() for g in gs)
     a.dh, a.lddh, a.dw, a.lddw = dh.data_ptr(), dh.stride(0), dw.data_ptr(), dw.stride(0)
     a.chunk, a.dw_out = min(chunk, n), 2 if dw_fp32 else 1
@@ -253,7 +252,8 @@ linear_logprobs_bwd_op = _ops.op("qpam::linear_logprobs_bwd", direct=True)(_line
 
 
 @linear_logprobs_bwd_op.register_fake
-def _(hidden_rows, weight_matrix, ids, entropy, stats, g_logprobs, g_entropy, temperature, chunk, ignore_index, dw_fp32):
+def _(hidden_rows, weight_matrix, ids, logprobs, entropy, stats, g_logprobs, g_entropy, temperature, chunk, ignore_index,
+      dw_fp32):
     return [hidden_rows.new_empty(hidden_rows.shape),
             weight_matrix.new_empty(weight_matrix.shape, dtype=torch.float32 if dw_fp32 else weight_matrix.dtype)]
 
@@ -263,7 +263,7 @@ def _linear_setup(ctx, inputs, output):
     ctx.mark_non_differentiable(output[2])
     ctx.set_materialize_grads(False)
     ctx.master = weight_copy is not None
-    ctx.save_for_backward(hidden_rows, weight_copy if ctx.master else weight_matrix, ids, output[1], output[2])
+    ctx.save_for_backward(hidden_rows, weight_copy if ctx.master else weight_matrix, ids, *output)
 
 
 def _linear_backward(ctx, grads):

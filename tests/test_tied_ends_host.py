@@ -186,7 +186,7 @@ def test_linear_token_logprobs_entry_errors_without_gpu():
         assert "multiple" in err(fn, D=63) and "null" in err(fn, ids=None) and "aligned" in err(fn, h=4100)
         assert "temperature" in err(fn, temperature=0.0) and "temperature" in err(fn, temperature=float("nan"))
         assert "stats" in err(fn, stats=None) and "workspace" in err(fn, workspace_bytes=64)
-    assert "logprobs" in err("qpam_linear_logprobs_fwd", logprobs=None)
+        assert "logprobs" in err(fn, logprobs=None)
     assert "dh" in err("qpam_linear_logprobs_bwd", dh=None) and "dw_out" in err("qpam_linear_logprobs_bwd", dw_out=0)
     assert "chunk" in err("qpam_linear_logprobs_bwd", chunk=0)
     assert "leading" in err("qpam_linear_logprobs_bwd", lddw=60)
@@ -201,7 +201,7 @@ def test_linear_token_logprobs_fake_kernels():
         assert r.logprobs.shape == r.entropy.shape == (3, 4) and r.top_ids is None
         f = torch.empty(12, device="cuda")
         for fp32 in (False, True):
-            dh, dw = linear_logprobs_bwd_op(h.view(12, 40), w.bfloat16(), f.long(), f, torch.empty(12, 2, device="cuda"),
+            dh, dw = linear_logprobs_bwd_op(h.view(12, 40), w.bfloat16(), f.long(), f, f, torch.empty(12, 2, device="cuda"),
                                             f, None, 1.0, 8, -100, fp32)
             assert dh.shape == (12, 40) and dw.shape == (70, 40)
             assert dh.dtype == torch.bfloat16 and dw.dtype == (torch.float32 if fp32 else torch.bfloat16)
