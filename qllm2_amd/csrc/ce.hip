@@ -1436,8 +1436,10 @@ struct Loads {
 __device__ __forceinline__ void to_lds(const char *from, U16 *lds) {
     __builtin_amdgcn_global_load_lds(reinterpret_cast<const unsigned *>(from), reinterpret_cast<unsigned *>(lds), 16, 0, 0);
 }
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 __device__ __forceinline__ void load(Stage &s, const Loads &q, int step) {
-    const int w = threadIdx.x >> 6;
+    const int w = wave_id();
     const char *a = q.a + (int64_t)step * (2 * DK), *b = q.b + (int64_t)step * (2 * DK);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -1479,18 +1481,36 @@ __device__ __forceinline__ void step(const Frags &cur, const Stage &c, Frags &ne
     }
 }
 
-// acc[mi][ni] lane holds C[64*(w>>1) + 16mi + 4g + r][128*(w&1) + 16ni + l16]; K % 32 == 0.
-// Step kt multiplies stage kt, reads the first fragments of stage kt + 1 and starts the
-// loads of stage kt + 3, four a wave (past the end they re-read the last step): at its end
-// "stage kt + 2 landed" is vmcnt <= 4.  Rows past the end of an operand re-read its last
-// row.  The stages are free and no load is in flight when it returns.
-__device__ __forceinline__ void product(const U16 *A, int64_t lda, int a_rows, const U16 *B, int64_t ldb, int b_rows, int K,
-                                        floatx4 (&acc)[4][8], Stage &s0, Stage &s1, Stage &s2, Stage &s3) {
-    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int mi = 0; mi < 4; ++mi)
-#pragma unroll
-        for (int ni = 0; ni < 8; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
+// A block takes tile after tile (one block a CU): the first three stages of the next tile
+// are loaded while this one is in its epilogue.  Tiles in the order and by the XCD ranges
+// of big::xcd_item / grouped_tile.
+struct Walk {
+    int item, end, n_rt, n_vt, rt, vt;
+    __device__ __forceinline__ Walk(int rts, int vts) : n_rt(rts), n_vt(vts) {
+        const int total = n_rt * n_vt, per = (total + big::XCDS - 1) / big::XCDS, x = blockIdx.x % big::XCDS;
+        item = x * per + blockIdx.x / big::XCDS;
+        end = min(total, (x + 1) * per);
+        place();
+    }
+    __device__ __forceinline__ bool more() const { return item < end; }
+    __device__ __forceinline__ void place() {
+        if (more()) big::grouped_tile(item, n_rt, n_vt, rt, vt);
+    }
+    __device__ __forceinline__ void next() {
+        item += gridDim.x / big::XCDS;
+        place();
+    }
+};
+// blocks of a launch: every XCD's 32 CUs, or one block a tile if there are fewer
+inline int grid(int tiles) { return big::XCDS * std::min(32, (tiles + big::XCDS - 1) / big::XCDS); }
+
+struct Stages {
+    Stage &s0, &s1, &s2, &s3;
+};
+
+// Rows past the end of an operand re-read its last row.
+__device__ __forceinline__ Loads loads(const U16 *A, int64_t lda, int a_rows, const U16 *B, int64_t ldb, int b_rows) {
+    const int w = wave_id(), lane = threadIdx.x & 63;
     Loads q{reinterpret_cast<const char *>(A), reinterpret_cast<const char *>(B), {}, {}};
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -1498,12 +1518,28 @@ __device__ __forceinline__ void product(const U16 *A, int64_t lda, int a_rows, c
         q.ao[j] = 2u * (unsigned)min(row, a_rows - 1) * (unsigned)lda + c;
         q.bo[j] = 2u * (unsigned)min(row, b_rows - 1) * (unsigned)ldb + c;
     }
+    return q;
+}
+__device__ __forceinline__ void start(const Stages &s, const Loads &q, int KT) {
+    load(s.s0, q, 0);
+    load(s.s1, q, min(1, KT - 1));
+    load(s.s2, q, min(2, KT - 1));
+}
+
+// The product whose first stages start() has under way: acc[mi][ni] lane holds
+// C[64*(w>>1) + 16mi + 4g + r][128*(w&1) + 16ni + l16].  Step kt multiplies stage kt, reads
+// the first fragments of stage kt + 1 and starts the loads of stage kt + 3, four a wave
+// (past the end they re-read the last step): at its end "stage kt + 2 landed" is vmcnt
+// <= 4.  The stages are free and no load is in flight when it returns.
+__device__ __forceinline__ void product(const Stages &st, const Loads &q, int KT, floatx4 (&acc)[4][8]) {
+    Stage &s0 = st.s0, &s1 = st.s1, &s2 = st.s2, &s3 = st.s3;
+    const int tid = threadIdx.x, w = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 8; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
     // fragment (row, chunk g); the swizzle repeats every eight rows
     const int aat = (64 * (w >> 1) + l16) * DK + 8 * wide::swz(l16, g), bat = (128 * (w & 1) + l16) * DK + 8 * wide::swz(l16, g);
-    const int KT = K / DK;
-    load(s0, q, 0);
-    load(s1, q, min(1, KT - 1));
-    load(s2, q, min(2, KT - 1));
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(4));
     __builtin_amdgcn_s_barrier();
     Frags f0, f1;
@@ -1532,139 +1568,172 @@ __device__ __forceinline__ void product(const U16 *A, int64_t lda, int a_rows, c
     __builtin_amdgcn_s_barrier();
 }
 
+// The block's LDS writes before it are read after it; loads and stores stay in flight.
+__device__ __forceinline__ void block_lds_sync() {
+    wide::wave_lds_sync();
+    __builtin_amdgcn_s_barrier();
+    wave_lds_order();
+}
+
 __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
     __shared__ __align__(16) Stage s0, s1, s2, s3;
     __shared__ float sB[2][TM], sS[2][TM], sT[2][TM];
     const qpam_ce_fwd_args &a = p.a;
-    const int n_rt = (a.N + TM - 1) / TM;
-    const int item = big::xcd_item(blockIdx.x, n_rt * p.n_vt);
-    if (item >= n_rt * p.n_vt) return;
-    int rt, vt;
-    big::grouped_tile(item, n_rt, p.n_vt, rt, vt);
-    const int r0 = rt * TM, v0 = vt * TN;
-    floatx4 acc[4][8];
-    product((const U16 *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0), (const U16 *)a.w + (int64_t)v0 * a.ldw, a.ldw,
-            min(TN, a.V - v0), a.D, acc, s0, s1, s2, s3);
-    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const Stages stages{s0, s1, s2, s3};
+    const int KT = a.D / DK;
+    const int tid = threadIdx.x, w = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
-    const int vl = v0 + 128 * wn + l16;  // this lane's column in tile ni: vl + 16 ni
-    auto rows = [&](auto whole) {        // whole: no column past the vocabulary
+    Walk at((a.N + TM - 1) / TM, p.n_vt);
+    if (!at.more()) return;
+    auto operands = [&]() {
+        const int r0 = at.rt * TM, v0 = at.vt * TN;
+        return loads((const U16 *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0), (const U16 *)a.w + (int64_t)v0 * a.ldw,
+                     a.ldw, min(TN, a.V - v0));
+    };
+    Loads q = operands();
+    start(stages, q, KT);
+    for (;;) {
+        floatx4 acc[4][8];
+        product(stages, q, KT, acc);
+        const int r0 = at.rt * TM, v0 = at.vt * TN, vt = at.vt;
+        at.next();
+        if (at.more()) {
+            q = operands();
+            start(stages, q, KT);
+        }
+        const int vl = v0 + 128 * wn + l16;  // this lane's column in tile ni: vl + 16 ni
+        auto rows = [&](auto whole) {        // whole: no column past the vocabulary
 #pragma unroll
-        for (int mi = 0; mi < 4; ++mi) {
+            for (int mi = 0; mi < 4; ++mi) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float mx = -INFINITY;
+                for (int r = 0; r < 4; ++r) {
+                    float mx = -INFINITY;
 #pragma unroll
-                for (int ni = 0; ni < 8; ++ni)
-                    if (whole || vl + 16 * ni < a.V) mx = fmaxf(mx, acc[mi][ni][r]);
-                const float b = row16_max(mx) * p.c;
-                float s = 0.f, t = 0.f;
+                    for (int ni = 0; ni < 8; ++ni)
+                        if (whole || vl + 16 * ni < a.V) mx = fmaxf(mx, acc[mi][ni][r]);
+                    const float b = row16_max(mx) * p.c;
+                    float s = 0.f, t = 0.f;
 #pragma unroll
-                for (int ni = 0; ni < 8; ++ni)
-                    if (whole || vl + 16 * ni < a.V) {
-                        const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
-                        s += e;
-                        t = __builtin_fmaf(e, u, t);
+                    for (int ni = 0; ni < 8; ++ni)
+                        if (whole || vl + 16 * ni < a.V) {
+                            const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
+                            s += e;
+                            t = __builtin_fmaf(e, u, t);
+                        }
+                    s = row16_sum(s);
+                    t = row16_sum(t);
+                    if (l16 == 0) {
+                        const int row = 64 * wm + 16 * mi + 4 * g + r;
+                        sB[wn][row] = b;
+                        sS[wn][row] = s;
+                        sT[wn][row] = t;
                     }
-                s = row16_sum(s);
-                t = row16_sum(t);
-                if (l16 == 0) {
-                    const int row = 64 * wm + 16 * mi + 4 * g + r;
-                    sB[wn][row] = b;
-                    sS[wn][row] = s;
-                    sT[wn][row] = t;
                 }
             }
+        };
+        if (v0 + TN <= a.V) rows(std::true_type{});
+        else rows(std::false_type{});
+        block_lds_sync();
+        if (tid < TM && r0 + tid < a.N) {
+            float b = sB[0][tid], s = sS[0][tid], t = sT[0][tid];
+            join_scores(b, s, t, sB[1][tid], sS[1][tid], sT[1][tid]);
+            const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
+            p.part_m[o] = b;
+            p.part_s[o] = s;
+            p.part_t[o] = t;
         }
-    };
-    if (v0 + TN <= a.V) rows(std::true_type{});
-    else rows(std::false_type{});
-    __syncthreads();
-    if (tid < TM && r0 + tid < a.N) {
-        float b = sB[0][tid], s = sS[0][tid], t = sT[0][tid];
-        join_scores(b, s, t, sB[1][tid], sS[1][tid], sT[1][tid]);
-        const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
-        p.part_m[o] = b;
-        p.part_s[o] = s;
-        p.part_t[o] = t;
+        if (!at.more()) return;
     }
 }
 
-// G^T [Vp][Rp] (and G [rows][Vp] when write_g) without the tokens' one-hot terms; zero past
-// the vocabulary and past the rows.  A 16-wide vocab slab of a wave goes through LDS (the
-// stages' space) and leaves as 128-byte runs of G^T.
+// G^T [Vp][Rp] (and G [rows][Vp] with WRITE_G) without the tokens' one-hot terms; zero past
+// the vocabulary and past the rows.  A 16-wide vocab slab of a wave goes through LDS and
+// leaves as 128-byte runs of G^T.
+template <bool WRITE_G>
 __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
-    __shared__ __align__(16) Stage s0, s1, s2, s3;
-    __shared__ float sB[TM], sBase[TM], sSlope[TM];
-    const qpam_ce_bwd_args &a = p.a;
-    const int n_rt = p.Rp / TM, n_vt = p.Vp / TN;
-    const int item = big::xcd_item(blockIdx.x, n_rt * n_vt);
-    if (item >= n_rt * n_vt) return;
-    int rt, vt;
-    big::grouped_tile(item, n_rt, n_vt, rt, vt);
-    const int lr0 = rt * TM, v0 = vt * TN, tid = threadIdx.x;
-    if (tid < TM) {
-        const RowScore q = row_score(p, lr0 + tid);
-        sB[tid] = q.b;
-        sBase[tid] = q.base;
-        sSlope[tid] = q.slope;
-    }
-    floatx4 acc[4][8];
-    product((const U16 *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(TM, p.rows - lr0),
-            (const U16 *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(TN, a.V - v0), a.D, acc, s0, s1, s2, s3);
-    const int w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
-    const int wm = w >> 1, wn = w & 1;
-    U16 *G = (U16 *)p.gbuf;
-    U16 *GT = (U16 *)p.gtbuf;
     constexpr int LD = 72;  // bf16 per staged vocab row: 64 tile rows + padding against bank conflicts
-    static_assert(8 * 16 * LD <= TM * DK + TN * DK, "the slabs of eight waves fit one stage");
-    U16 *slab = reinterpret_cast<U16 *>(&s0) + w * 16 * LD;
-    // the 16 rows of this lane (rows 64 wm + 16 mi + 4 g + r)
-    float hb[4][4], h0[4][4], h1[4][4];
-#pragma unroll
-    for (int mi = 0; mi < 4; ++mi)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int rl = 64 * wm + 16 * mi + 4 * g + r;
-            hb[mi][r] = sB[rl];
-            h0[mi][r] = sBase[rl];
-            h1[mi][r] = sSlope[rl];
-        }
-    auto slabs = [&](auto whole) {  // whole: every column is a vocabulary entry, every row a row
-#pragma unroll
-        for (int ni = 0; ni < 8; ++ni) {
-            const int vb = v0 + 128 * wn + 16 * ni, v = vb + l16;
-#pragma unroll
-            for (int mi = 0; mi < 4; ++mi) {
-                const int rl0 = 64 * wm + 16 * mi + 4 * g;
-                float x[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -hb[mi][r]);
-                    x[r] = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(h1[mi][r], u, h0[mi][r]);
-                    if (!whole && (v >= a.V || lr0 + rl0 + r >= p.rows)) x[r] = 0.f;
-                }
-                const unsigned lo = pack_bf16x2(x[0], x[1]), hi = pack_bf16x2(x[2], x[3]);
-                if (p.write_g) {
-                    const U16 gb[4] = {(U16)(lo & 0xFFFFu), (U16)(lo >> 16), (U16)(hi & 0xFFFFu), (U16)(hi >> 16)};
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (lr0 + rl0 + r < p.rows) G[(int64_t)(lr0 + rl0 + r) * p.Vp + v] = gb[r];
-                }
-                *reinterpret_cast<uint2 *>(slab + l16 * LD + 16 * mi + 4 * g) = make_uint2(lo, hi);
-            }
-            wide::wave_lds_sync();  // the slab is this wave's own
-            const int vl = lane >> 2, part = lane & 3;  // vocab row, 16 tile rows: 32 bytes a lane
-            const uint4 *src = reinterpret_cast<const uint4 *>(slab + vl * LD + 16 * part);
-            const uint4 d0 = src[0], d1 = src[1];
-            uint4 *dst = reinterpret_cast<uint4 *>(GT + (int64_t)(vb + vl) * p.Rp + lr0 + 64 * wm + 16 * part);
-            dst[0] = d0;
-            dst[1] = d1;
-            wide::wave_lds_sync();
+    __shared__ __align__(16) Stage s0, s1, s2, s3;
+    __shared__ __align__(16) U16 sSlab[8 * 16 * LD];
+    __shared__ __align__(16) float sRow[2][3][TM];  // the rows' scores, of this tile and the next
+    const qpam_ce_bwd_args &a = p.a;
+    const Stages stages{s0, s1, s2, s3};
+    const int KT = a.D / DK;
+    const int tid = threadIdx.x, w = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wm = w >> 1, wn = w & 1;
+    Walk at(p.Rp / TM, p.Vp / TN);
+    if (!at.more()) return;
+    auto operands = [&]() {
+        const int lr0 = at.rt * TM, v0 = at.vt * TN;
+        return loads((const U16 *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(TM, p.rows - lr0),
+                     (const U16 *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(TN, a.V - v0));
+    };
+    auto keep_rows = [&](const RowScore &q, int buf) {
+        if (tid < TM) {
+            sRow[buf][0][tid] = q.b;
+            sRow[buf][1][tid] = q.base;
+            sRow[buf][2][tid] = q.slope;
         }
     };
-    if (v0 + TN <= a.V && lr0 + TM <= p.rows) slabs(std::true_type{});
-    else slabs(std::false_type{});
+    U16 *G = (U16 *)p.gbuf;
+    U16 *GT = (U16 *)p.gtbuf;
+    U16 *slab = sSlab + w * 16 * LD;
+    // a slab's way out: vocab row lane / 4, 16 tile rows lane % 4, 32 bytes a lane
+    const U16 *from = slab + (lane >> 2) * LD + 16 * (lane & 3);
+    const unsigned to = 2u * ((lane >> 2) * (unsigned)p.Rp + 16 * (lane & 3));
+    keep_rows(row_score(p, at.rt * TM + (tid & (TM - 1))), 0);
+    Loads q = operands();
+    start(stages, q, KT);
+    for (int buf = 0;; buf ^= 1) {
+        floatx4 acc[4][8];
+        product(stages, q, KT, acc);
+        const int lr0 = at.rt * TM, v0 = at.vt * TN;
+        at.next();
+        if (at.more()) {
+            keep_rows(row_score(p, at.rt * TM + (tid & (TM - 1))), buf ^ 1);
+            q = operands();
+            start(stages, q, KT);
+        }
+        // this lane's rows are 64 wm + 16 mi + 4 g + r; their scores are read again for every
+        // slab, as 48 registers of them beside the accumulators spill
+        const float *mine = &sRow[buf][0][64 * wm + 4 * g];
+        auto slabs = [&](auto whole) {  // whole: every column is a vocabulary entry, every row a row
+#pragma unroll
+            for (int ni = 0; ni < 8; ++ni) {
+                const int vb = v0 + 128 * wn + 16 * ni, v = vb + l16;
+#pragma unroll
+                for (int mi = 0; mi < 4; ++mi) {
+                    const int rl0 = 64 * wm + 16 * mi + 4 * g;
+                    const floatx4 hb = *reinterpret_cast<const floatx4 *>(mine + 16 * mi);
+                    const floatx4 h0 = *reinterpret_cast<const floatx4 *>(mine + TM + 16 * mi);
+                    const floatx4 h1 = *reinterpret_cast<const floatx4 *>(mine + 2 * TM + 16 * mi);
+                    float x[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -hb[r]);
+                        x[r] = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(h1[r], u, h0[r]);
+                        if (!whole && (v >= a.V || lr0 + rl0 + r >= p.rows)) x[r] = 0.f;
+                    }
+                    const unsigned lo = pack_bf16x2(x[0], x[1]), hi = pack_bf16x2(x[2], x[3]);
+                    if constexpr (WRITE_G) {
+                        const U16 gb[4] = {(U16)(lo & 0xFFFFu), (U16)(lo >> 16), (U16)(hi & 0xFFFFu), (U16)(hi >> 16)};
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (lr0 + rl0 + r < p.rows) G[(int64_t)(lr0 + rl0 + r) * p.Vp + v] = gb[r];
+                    }
+                    *reinterpret_cast<uint2 *>(slab + l16 * LD + 16 * mi + 4 * g) = make_uint2(lo, hi);
+                }
+                wide::wave_lds_sync();  // the slab is this wave's own
+                const uint4 d0 = reinterpret_cast<const uint4 *>(from)[0], d1 = reinterpret_cast<const uint4 *>(from)[1];
+                char *out = reinterpret_cast<char *>(GT + (int64_t)vb * p.Rp + lr0 + 64 * wm);
+                *reinterpret_cast<uint4 *>(out + to) = d0;
+                *reinterpret_cast<uint4 *>(out + to + 16) = d1;
+                wide::wave_lds_sync();
+            }
+        };
+        if (v0 + TN <= a.V && lr0 + TM <= p.rows) slabs(std::true_type{});
+        else slabs(std::false_type{});
+        if (!at.more()) return;
+    }
 }
 }  // namespace tiles
 
@@ -1931,7 +2000,7 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     if (few) {
         st = thin::waves(a.V) == 16 ? thin::launch<T, 16>(p, stream) : thin::launch<T, 4>(p, stream);
     } else if (scores && is_bf<T>()) {
-        const dim3 grid(big::xcd_grid(p.n_vt * ((a.N + tiles::TM - 1) / tiles::TM)));
+        const dim3 grid(tiles::grid(p.n_vt * ((a.N + tiles::TM - 1) / tiles::TM)));
         hipLaunchKernelGGL(tiles::scores_tile_kernel, grid, dim3(tiles::TT), 0, stream, p);
         st = launch_status("scores_tile_kernel");
     } else if (wide_tiles) {
@@ -1994,8 +2063,11 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
     const size_t gsmem = wide_tiles ? wide::KSMEM : big::SMEM;
     auto launch_grad = [&]() {
         if (scores) {
-            hipLaunchKernelGGL(tiles::scores_grad_kernel, dim3(big::xcd_grid((p.Vp / tiles::TN) * (p.Rp / tiles::TM))),
-                               dim3(tiles::TT), 0, stream, p);
+            const dim3 grid(tiles::grid((p.Vp / tiles::TN) * (p.Rp / tiles::TM)));
+            if (p.write_g)
+                hipLaunchKernelGGL(tiles::scores_grad_kernel<true>, grid, dim3(tiles::TT), 0, stream, p);
+            else
+                hipLaunchKernelGGL(tiles::scores_grad_kernel<false>, grid, dim3(tiles::TT), 0, stream, p);
             const int st = launch_status("scores_grad_kernel");
             if (st) return st;
             hipLaunchKernelGGL(scores_token_kernel<U>, dim3((p.rows + THREADS - 1) / THREADS), dim3(THREADS), 0, stream, p);
