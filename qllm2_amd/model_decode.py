@@ -7,7 +7,7 @@ batch that shares one step_offset; here sequences join (admit: their prompt's
 prefill) and leave (release) between steps, each keeps its own position, and a
 step runs only the live rows:
 
-  embedding rows of the tokens (the tied table, interleaved [V, dim, 2])
+  embedding rows of the tokens, both tables' in one launch (qpam_embed_fwd)
   -> ComplexNorm                                     (qpam_cplx_fwd)
   -> per block (v11/model.py:1038-1049), h = norm1(x) from the step before:
        x += cgu_scale * down(cgu_gate(gate(h), act(up(h))))
@@ -28,6 +28,10 @@ accumulation; the residual stream, the norms' statistics and the PAM states
 stay fp32).  With graphs=True a whole step (every layer and the head) is
 captured once per live-count bucket and replayed.
 
+What the answers are worth: logprobs gives the log probabilities of chosen tokens,
+entropies and top alternatives of a step's logits, score the log probabilities of
+a whole given sequence without its logits.
+
 Prefill (admit) runs the same blocks over the prompt with the fused PAM layer
 forward (pam_layer.forward) and hands each layer's state to the slot pool.
 The model is any module with V11LM's attribute names (embed.embed_real /
@@ -44,7 +48,9 @@ import torch.nn.functional as F
 from . import _lib
 from . import pam_layer
 from . import triton_kernels as tk
+from .embedding import complex_embedding
 from .engine import DecodeEngine
+from .token_logprobs import linear_token_logprobs, token_logprobs
 
 MAX_DIM = 2048  # qpam_resid_norm: a thread per four complex columns, 512 per row
 
@@ -161,9 +167,10 @@ class ModelDecoder:
         self._wver += 1
         self.engine.refresh_weights()
         with torch.no_grad():
-            e = torch.stack([m.embed.embed_real.weight, m.embed.embed_imag.weight], -1).float()  # [V, dim, 2]
+            tables = (m.embed.embed_real.weight, m.embed.embed_imag.weight)
+            e = torch.stack(tables, -1).float()                                                  # [V, dim, 2]
             self.vocab, self.dim = e.shape[0], e.shape[1]
-            self._embed = e.contiguous()
+            self._embed = [t.detach().float().contiguous().clone() for t in tables]              # fp32, lookups
             self._embed_w = e.reshape(self.vocab, 2 * self.dim).to(dt).contiguous()           # logits GEMM
             self._blk = []
             if self.dim % 4 or self.dim > MAX_DIM:
@@ -213,12 +220,19 @@ class ModelDecoder:
         g = cgu_mix(gu, blk["hid"], blk["act_bias"], blk["act_beta"], blk["act_pa"], blk["act_pb"])
         return F.linear(g.view(n, -1), blk["w_down"]).view(n, self.dim, 2)
 
-    def _head(self, h):
-        """Logits [n, V] (fp32) from output-normed rows h [n, dim, 2] (GEMM dtype)."""
+    def _embedded(self, ids):
+        """Normed embedding rows [n, dim, 2] of ids [n]: the fp32 residual stream."""
+        return self._norm(complex_embedding(ids, *self._embed), self._norm_e)
+
+    def _lm_rows(self, h):
+        """The LM head's rows [n, 2 dim] (GEMM dtype) from output-normed rows h [n, dim, 2]."""
         n = h.shape[0]
         lm = F.linear(h.reshape(n, -1), self._w_head, self._b_head).view(n, self.dim, 2)
-        lm = self._norm(lm, self._norm_h)                                      # in the GEMM dtype
-        logits = F.linear(lm.reshape(n, -1), self._embed_w)                     # [n, V]
+        return self._norm(lm, self._norm_h).reshape(n, -1)
+
+    def _head(self, h):
+        """Logits [n, V] (fp32) from output-normed rows h [n, dim, 2] (GEMM dtype)."""
+        logits = F.linear(self._lm_rows(h), self._embed_w)                      # [n, V]
         return logits if logits.dtype == torch.float32 else logits.float()
 
     def _next_norm(self, li):
@@ -228,7 +242,7 @@ class ModelDecoder:
     def _tokens(self, ids, slots):
         """Every layer and the head for the listed rows: ids [n] int64, slots [n] int32."""
         dt = self.dtype
-        x = self._norm(self._embed[ids], self._norm_e)                          # fp32 residual stream
+        x = self._embedded(ids)
         h = resid_norm(x, *self._next_norm(-1), out_dtype=dt)
         for li, blk in enumerate(self._blk):
             h = resid_norm(x, *blk["norm2"], y=self._cgu(h, blk), y_scale=blk["cgu_scale"], out_dtype=dt)
@@ -237,13 +251,11 @@ class ModelDecoder:
         return self._head(h)
 
     # ------------------------------------------------------------ slots
-    @torch.no_grad()
-    def prefill(self, prompt_ids):
-        """The model over one prompt (ids [T]) with the fused PAM prefill:
-        (logits of its last token [V], the per-layer states)."""
-        ids = prompt_ids.to(self._embed.device).long().view(1, -1)
-        t, dt = ids.shape[1], self.dtype
-        x = self._norm(self._embed[ids[0]], self._norm_e)                       # [t, dim, 2] fp32
+    def _prompt_rows(self, ids):
+        """Output-normed rows [t, dim, 2] (GEMM dtype) of one sequence's tokens ids [t]
+        through the blocks with the fused PAM prefill, and the per-layer states."""
+        t, dt = ids.shape[0], self.dtype
+        x = self._embedded(ids)                                                 # [t, dim, 2] fp32
         h = resid_norm(x, *self._next_norm(-1), out_dtype=dt)
         states = []
         for li, (blk, b) in enumerate(zip(self._blk, self.blocks)):
@@ -252,7 +264,28 @@ class ModelDecoder:
             states.append(s)
             h = resid_norm(x, *self._next_norm(li), y=y.reshape(t, self.dim, 2).contiguous(),
                            y_scale=blk["pam_scale"], out_dtype=dt)
+        return h, states
+
+    def _prompt_ids(self, prompt_ids):
+        return prompt_ids.to(self._embed[0].device).long().view(-1)
+
+    @torch.no_grad()
+    def prefill(self, prompt_ids):
+        """The model over one prompt (ids [T]) with the fused PAM prefill:
+        (logits of its last token [V], the per-layer states)."""
+        h, states = self._prompt_rows(self._prompt_ids(prompt_ids))
         return self._head(h[-1:])[0], states
+
+    @torch.no_grad()
+    def score(self, ids, temperature=1.0):
+        """Of one sequence ids [T], T >= 2: for each token after the first, the log
+        probability the model gives it after those before it, and the entropy of that
+        choice, fp32 [T - 1] each; no logits in memory."""
+        ids = self._prompt_ids(ids)
+        if ids.numel() < 2:
+            raise ValueError("ModelDecoder.score: at least two tokens")
+        h, _ = self._prompt_rows(ids)
+        return linear_token_logprobs(self._lm_rows(h[:-1]), self._embed_w, ids[1:], temperature=temperature)
 
     def admit(self, prompt_ids):
         """A sequence with this prompt joins: its prefill's states enter a
@@ -333,3 +366,9 @@ class ModelDecoder:
             v, _ = x.topk(min(top_k, x.shape[-1]))
             x = x.masked_fill(x < v[:, -1:], float("-inf"))
         return torch.multinomial(x.softmax(-1), 1, generator=generator).squeeze(1)
+
+    @staticmethod
+    def logprobs(logits, ids, temperature=1.0, top_k=0):
+        """TokenLogprobs of a step's logits [n, V] for the tokens ids [n] drawn from them:
+        log probabilities, entropies and top_k alternatives at the temperature."""
+        return token_logprobs(logits, ids, temperature=temperature, top_k=top_k)
