@@ -146,92 +146,6 @@ __device__ __forceinline__ void gemm_tile(const T *A, int64_t lda, int a_rows, c
     }
 }
 
-// The same tile of fp32 operands on the bf16 matrix units (token scores): every value is
-// split into three bf16 parts, x = hi + mid + lo with |mid| <= 2^-9 |x|, |lo| <= 2^-18
-// |x| and nothing left above 2^-27 |x|, and a product is the six part products down to
-// 2^-18; the three left out are below 2^-26 of it, less than one fp32 rounding.  Values
-// are split on their way from registers to LDS, once a block: 160 VALU instructions a
-// thread and k-step beside 96 MFMAs of 16 cycles, against 128 MFMAs of 32 cycles with
-// v_mfma_f32_16x16x4_f32.  LDS holds one k-step as three planes of 16-byte chunks,
-// XOR-swizzled like the bf16 tiles (48 KiB, so that two blocks share a CU and one
-// multiplies while the other splits); the next k-step's loads are in flight meanwhile.
-// Rows past the end of an operand re-read its last row.  Infinite operands give NaN.
-constexpr size_t SPLIT_SMEM = 3 * (BM + BN) * BK * sizeof(unsigned short);
-
-__device__ __forceinline__ void split_store(uint4 raw, unsigned short *lds) {
-    float v[4] = {__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w)};
-#pragma unroll
-    for (int part = 0; part < 3; ++part) {
-        const uint2 q = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-        *reinterpret_cast<uint2 *>(lds + part * (BM + BN) * BK) = q;
-        v[0] -= __uint_as_float(q.x << 16);
-        v[1] -= __uint_as_float(q.x & 0xFFFF0000u);
-        v[2] -= __uint_as_float(q.y << 16);
-        v[3] -= __uint_as_float(q.y & 0xFFFF0000u);
-    }
-}
-
-__device__ __forceinline__ void split_tile(const float *A, int64_t lda, int a_rows, const float *B, int64_t ldb, int b_rows,
-                                           int K, floatx4 (&acc)[4][4], unsigned short *smem) {
-    constexpr int LOADS = BM * BK / 4 / THREADS;  // 16-byte loads a thread, operand and k-step
-    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
-    const int arow0 = 64 * (w >> 1), brow0 = BM + 64 * (w & 1);
-#pragma unroll
-    for (int mi = 0; mi < 4; ++mi)
-#pragma unroll
-        for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
-    const float *pa[LOADS], *pb[LOADS];
-    int to[LOADS];
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const int row = (tid >> 3) + 32 * i, c = tid & 7;  // four values, half a chunk of eight
-        pa[i] = A + min(row, a_rows - 1) * lda + 4 * c;
-        pb[i] = B + min(row, b_rows - 1) * ldb + 4 * c;
-        to[i] = row * BK + 8 * ((c >> 1) ^ ((row >> 1) & 3)) + 4 * (c & 1);
-    }
-    uint4 ra[LOADS], rb[LOADS];
-    auto gload = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            ra[i] = *reinterpret_cast<const uint4 *>(pa[i] + k0);
-            rb[i] = *reinterpret_cast<const uint4 *>(pb[i] + k0);
-        }
-    };
-    auto fragment = [&](int row, int part) {
-        return *reinterpret_cast<const bf16x8 *>(smem + (part * (BM + BN) + row) * BK + 8 * (g ^ ((row >> 1) & 3)));
-    };
-    const int KT = K / BK;
-    gload(0);
-    for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            split_store(ra[i], smem + to[i]);
-            split_store(rb[i], smem + BM * BK + to[i]);
-        }
-        __syncthreads();
-        gload(min(kt + 1, KT - 1) * BK);
-        __builtin_amdgcn_sched_barrier(0);
-        bf16x8 a[4][3];
-#pragma unroll
-        for (int mi = 0; mi < 4; ++mi)
-#pragma unroll
-            for (int part = 0; part < 3; ++part) a[mi][part] = fragment(arow0 + 16 * mi + l16, part);
-#pragma unroll
-        for (int ni = 0; ni < 4; ++ni) {
-            bf16x8 b[3];
-#pragma unroll
-            for (int part = 0; part < 3; ++part) b[part] = fragment(brow0 + 16 * ni + l16, part);
-            constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};  // small products first
-#pragma unroll
-            for (int j = 0; j < 6; ++j)
-#pragma unroll
-                for (int mi = 0; mi < 4; ++mi)
-                    acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mi][PA[j]], b[PB[j]], acc[mi][ni], 0, 0, 0);
-        }
-        __syncthreads();
-    }
-}
-
 // ------------------------------------------------------------ forward -----
 constexpr float LN2 = 0.6931471805599453f, LOG2 = 1.4426950408889634f;
 constexpr float U_FLOOR = -1e4f;  // 2^u is 0 and 2^u u is -0, not NaN
@@ -258,29 +172,18 @@ __device__ __forceinline__ void join_scores(float &b, float &s, float &t, float 
     b = nb;
 }
 
-template <typename T, bool SCORES> constexpr bool SPLIT = SCORES && std::is_same_v<T, float>;
-template <typename T, bool SCORES> constexpr size_t tile_smem() { return SPLIT<T, SCORES> ? SPLIT_SMEM : gemm_smem<T>(); }
-
-template <typename T, bool SCORES>
-__device__ __forceinline__ void logits_tile(const T *A, int64_t lda, int a_rows, const T *B, int64_t ldb, int b_rows, int K,
-                                            floatx4 (&acc)[4][4], unsigned char *smem) {
-    if constexpr (SPLIT<T, SCORES>)
-        split_tile(A, lda, a_rows, B, ldb, b_rows, K, acc, reinterpret_cast<unsigned short *>(smem));
-    else
-        gemm_tile<T>(A, lda, a_rows, B, ldb, b_rows, K, acc, reinterpret_cast<T *>(smem));
-}
-
-template <typename T, bool SCORES>
+template <typename T>
 __global__ void __launch_bounds__(THREADS) ce_fwd_tile_kernel(FwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    __shared__ float sM[2][BM], sS[2][BM], sT[2][SCORES ? BM : 1];
+    T *smem = reinterpret_cast<T *>(smem_raw);
+    __shared__ float sM[2][BM], sS[2][BM];
     __shared__ int sI[2][BM];
     const qpam_ce_fwd_args &a = p.a;
     const int vt = blockIdx.x, rt = blockIdx.y;
     const int r0 = rt * BM, v0 = vt * VT;
     floatx4 acc[4][4];
-    logits_tile<T, SCORES>((const T *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(BM, a.N - r0),
-                           (const T *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(BN, a.V - v0), a.D, acc, smem_raw);
+    gemm_tile<T>((const T *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(BM, a.N - r0), (const T *)a.w + (int64_t)v0 * a.ldw,
+                 a.ldw, min(BN, a.V - v0), a.D, acc, smem);
 
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
@@ -302,43 +205,23 @@ __global__ void __launch_bounds__(THREADS) ce_fwd_tile_kernel(FwdParams p) {
                 const int oi = __shfl_xor(ix, off);
                 if (om > mx || (om == mx && oi < ix)) { mx = om; ix = oi; }
             }
-            float s = 0.f, t = 0.f;
-            const float b = mx * p.c;
+            float s = 0.f;
 #pragma unroll
             for (int ni = 0; ni < 4; ++ni) {
                 const int v = v0 + 64 * wn + 16 * ni + l16;
-                if (!SCORES) {
-                    if (v < a.V) s += __expf(acc[mi][ni][r] - mx);
-                } else if (v < a.V) {
-                    const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
-                    s += e;
-                    t += e * u;
-                }
+                if (v < a.V) s += __expf(acc[mi][ni][r] - mx);
             }
 #pragma unroll
             for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off);
-            if (SCORES) t = row16_sum(t);
             if (l16 == 0) {
                 const int row = 64 * wm + 16 * mi + 4 * g + r;
-                sM[wn][row] = SCORES ? b : mx;
+                sM[wn][row] = mx;
                 sS[wn][row] = s;
-                if (SCORES) sT[wn][row] = t;
-                else sI[wn][row] = ix;
+                sI[wn][row] = ix;
             }
         }
     }
     __syncthreads();
-    if (SCORES) {
-        if (tid < BM && r0 + tid < a.N) {
-            float b = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
-            join_scores(b, s, t, sM[1][tid], sS[1][tid], sT[1][tid]);
-            const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
-            p.part_m[o] = b;
-            p.part_s[o] = s;
-            p.part_t[o] = t;
-        }
-        return;
-    }
     if (tid < BM && r0 + tid < a.N) {
         const float m0 = sM[0][tid], m1 = sM[1][tid];
         const float m = fmaxf(m0, m1);
@@ -553,11 +436,11 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ unsigned short from_f32<unsigned short>(float x) { return f32_to_bf16(x); }
 
 // G tile: recompute logits, G = (exp(x - lse) - [v == t]) * scale; write G and G^T
-template <typename T, bool SCORES>
+template <typename T>
 __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
+    T *smem = reinterpret_cast<T *>(smem_raw);
     __shared__ float sLse[BM], sScale[BM];
-    __shared__ float sSlope[SCORES ? BM : 1];
     __shared__ int sTgt[BM];
     const qpam_ce_bwd_args &a = p.a;
     const int vt = blockIdx.x, rt = blockIdx.y;
@@ -567,12 +450,7 @@ __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
         const int lr = lr0 + tid, row = p.row0 + lr;
         float lse = 0.f, sc = 0.f;
         int tg = -1;
-        if (SCORES) {
-            const RowScore q = row_score(p, lr);
-            lse = q.b;
-            sc = q.base;
-            sSlope[tid] = q.slope;
-        } else if (lr < p.rows) {
+        if (lr < p.rows) {
             const int64_t t = a.targets[row];
             const bool valid = (t != a.ignore_index) && t >= 0 && t < a.V;
             lse = a.lse[row];
@@ -584,8 +462,8 @@ __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
         sTgt[tid] = tg;
     }
     floatx4 acc[4][4];
-    logits_tile<T, SCORES>((const T *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(BM, p.rows - lr0),
-                           (const T *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(BN, a.V - v0), a.D, acc, smem_raw);
+    gemm_tile<T>((const T *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(BM, p.rows - lr0),
+                 (const T *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(BN, a.V - v0), a.D, acc, smem);
     const int w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
     T *G = (T *)p.gbuf;
@@ -600,12 +478,7 @@ __global__ void __launch_bounds__(THREADS) ce_grad_tile_kernel(BwdParams p) {
             for (int r = 0; r < 4; ++r) {
                 const int rl = 64 * wm + 16 * mi + 4 * g + r;
                 float x = 0.f;
-                if (SCORES) {
-                    if (v < a.V && lr0 + rl < p.rows) {
-                        const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -sLse[rl]);
-                        x = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(sSlope[rl], u, sScale[rl]);
-                    }
-                } else if (v < a.V && sScale[rl] != 0.f) {
+                if (v < a.V && sScale[rl] != 0.f) {
                     x = __expf(acc[mi][ni][r] - sLse[rl]);
                     if (v == sTgt[rl]) x -= 1.f;
                     x *= sScale[rl];
@@ -654,17 +527,210 @@ __global__ void __launch_bounds__(THREADS) ce_gemm_kernel(const T *A, int64_t ld
             }
 }
 
-// C = A B^T of fp32 operands in parts (token scores' dH and dW), the K axis in
-// gridDim.z ranges of kper: one range writes C (or adds to it), several write C + z
-// split_stride, summed by split_sum_kernel in their order.
-__global__ void __launch_bounds__(THREADS) split_gemm_kernel(const float *A, int64_t lda, int M, const float *B, int64_t ldb,
-                                                            int N, int K, int kper, float *C, int64_t ldc,
-                                                            int64_t split_stride, int accumulate) {
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN, k0 = blockIdx.z * kper;
+// Token scores in fp32, 256 x 128 tiles on the bf16 matrix units: every value is split into
+// three bf16 parts, x = hi + mid + lo with |mid| <= 2^-9 |x|, |lo| <= 2^-18 |x| and nothing
+// left above 2^-27 |x|, and a product is the six part products down to 2^-18; the three
+// left out are below 2^-26 of it, less than one fp32 rounding.  A k-step of 32 takes a
+// wave (64 x 64) 96 MFMAs of 16 cycles, against 128 of 32 cycles with
+// v_mfma_f32_16x16x4_f32.  Values are split on their way from registers to LDS, once a
+// block, in the shadow of the MFMAs: 8 waves, two LDS buffers of three planes (72 KiB
+// each) of 16-byte chunks, swizzled like the bf16 tiles; the loads run two steps ahead.
+// Rows past the end of an operand re-read its last row.  Infinite operands give NaN.
+namespace split {
+constexpr int TM = 256, TN = 128, TT = 512;
+constexpr int PLANE = (TM + TN) * BK;  // bf16 elements of a plane: A's rows, then B's
+using U16 = unsigned short;
+
+struct Raw {
+    uint4 a[TM * BK / 4 / TT], b[TN * BK / 4 / TT];  // 4 and 2 loads a thread and step
+};
+
+__device__ __forceinline__ int swz(int row, int c) { return c ^ ((row >> 1) & 3); }
+
+__device__ __forceinline__ void store(uint4 raw, U16 *lds) {
+    float v[4] = {__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w)};
+#pragma unroll
+    for (int part = 0; part < 3; ++part) {
+        const uint2 q = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        *reinterpret_cast<uint2 *>(lds + part * PLANE) = q;
+        v[0] -= __uint_as_float(q.x << 16);
+        v[1] -= __uint_as_float(q.x & 0xFFFF0000u);
+        v[2] -= __uint_as_float(q.y << 16);
+        v[3] -= __uint_as_float(q.y & 0xFFFF0000u);
+    }
+}
+
+// acc[mi][ni] lane holds C[64*(w>>1) + 16mi + 4g + r][64*(w&1) + 16ni + l16]; K % 32 == 0.
+// Row strides below 2^22 (32-bit byte offsets in a tile).
+__device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, const float *B, int64_t ldb, int b_rows, int K,
+                                     floatx4 (&acc)[4][4], U16 *s0, U16 *s1) {
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int arow0 = 64 * (w >> 1), brow0 = TM + 64 * (w & 1);
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
+    // thread -> rows tid / 8 + 64 i, values 4 (tid % 8) ..: half a chunk of eight
+    const int r8 = tid >> 3, c8 = tid & 7;
+    unsigned ao[4], bo[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ao[i] = 4u * ((unsigned)min(r8 + 64 * i, a_rows - 1) * (unsigned)lda + 4 * c8);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) bo[i] = 4u * ((unsigned)min(r8 + 64 * i, b_rows - 1) * (unsigned)ldb + 4 * c8);
+    const int to = r8 * BK + 8 * swz(r8, c8 >> 1) + 4 * (c8 & 1);  // the swizzle repeats every eight rows
+    auto gload = [&](Raw &x, int step) {
+        const char *a = reinterpret_cast<const char *>(A + (int64_t)step * BK);
+        const char *b = reinterpret_cast<const char *>(B + (int64_t)step * BK);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.a[i] = *reinterpret_cast<const uint4 *>(a + ao[i]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x.b[i] = *reinterpret_cast<const uint4 *>(b + bo[i]);
+    };
+    auto put = [&](const Raw &x, U16 *s, int i) {  // the i-th of the six pieces
+        store(i < 4 ? x.a[i < 4 ? i : 0] : x.b[i < 4 ? 0 : i - 4], s + to + 64 * (i < 4 ? i : TM / 64 + i - 4) * BK);
+    };
+    auto fragment = [&](const U16 *s, int row, int part) {
+        return *reinterpret_cast<const bf16x8 *>(s + part * PLANE + (row + l16) * BK + 8 * swz(l16, g));
+    };
+    // the products of the step in `cur`; the next step's values go from x to `next`
+    auto step = [&](const U16 *cur, U16 *next, const Raw &x) {
+        bf16x8 a[4][3];
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+            for (int part = 0; part < 3; ++part) a[mi][part] = fragment(cur, arow0 + 16 * mi, part);
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni) {
+            bf16x8 b[3];
+#pragma unroll
+            for (int part = 0; part < 3; ++part) b[part] = fragment(cur, brow0 + 16 * ni, part);
+            constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};  // small products first
+#pragma unroll
+            for (int j = 0; j < 6; ++j)
+#pragma unroll
+                for (int mi = 0; mi < 4; ++mi)
+                    acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mi][PA[j]], b[PB[j]], acc[mi][ni], 0, 0, 0);
+            if (ni < 3) {
+                put(x, next, 2 * ni);
+                put(x, next, 2 * ni + 1);
+            }
+        }
+    };
+    const int KT = K / BK;
+    Raw x0, x1;
+    gload(x0, 0);
+    gload(x1, min(1, KT - 1));
+#pragma unroll
+    for (int i = 0; i < 6; ++i) put(x0, s0, i);
+    __syncthreads();
+    for (int kt = 0; kt < KT; kt += 2) {
+        gload(x0, min(kt + 2, KT - 1));
+        step(s0, s1, x1);
+        __syncthreads();
+        if (kt + 1 >= KT) break;
+        gload(x1, min(kt + 3, KT - 1));
+        step(s1, s0, x0);
+        __syncthreads();
+    }
+}
+
+__global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
+    __shared__ __align__(16) U16 s0[3 * PLANE], s1[3 * PLANE];
+    __shared__ float sB[2][TM], sS[2][TM], sT[2][TM];
+    const qpam_ce_fwd_args &a = p.a;
+    const int vt = blockIdx.x, r0 = blockIdx.y * TM, v0 = vt * TN;
     floatx4 acc[4][4];
-    split_tile(A + (int64_t)m0 * lda + k0, lda, min(BM, M - m0), B + (int64_t)n0 * ldb + k0, ldb, min(BN, N - n0),
-               min(kper, K - k0), acc, reinterpret_cast<unsigned short *>(smem_raw));
+    tile((const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0), (const float *)a.w + (int64_t)v0 * a.ldw, a.ldw,
+         min(TN, a.V - v0), a.D, acc, s0, s1);
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wm = w >> 1, wn = w & 1, vl = v0 + 64 * wn + l16;
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int ni = 0; ni < 4; ++ni)
+                if (vl + 16 * ni < a.V) mx = fmaxf(mx, acc[mi][ni][r]);
+            const float b = row16_max(mx) * p.c;
+            float s = 0.f, t = 0.f;
+#pragma unroll
+            for (int ni = 0; ni < 4; ++ni)
+                if (vl + 16 * ni < a.V) {
+                    const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
+                    s += e;
+                    t = __builtin_fmaf(e, u, t);
+                }
+            s = row16_sum(s);
+            t = row16_sum(t);
+            if (l16 == 0) {
+                const int row = 64 * wm + 16 * mi + 4 * g + r;
+                sB[wn][row] = b;
+                sS[wn][row] = s;
+                sT[wn][row] = t;
+            }
+        }
+    __syncthreads();
+    if (tid < TM && r0 + tid < a.N) {
+        float b = sB[0][tid], s = sS[0][tid], t = sT[0][tid];
+        join_scores(b, s, t, sB[1][tid], sS[1][tid], sT[1][tid]);
+        const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
+        p.part_m[o] = b;
+        p.part_s[o] = s;
+        p.part_t[o] = t;
+    }
+}
+
+// G [rows][Vp] and G^T [Vp][Rp] without the tokens' one-hot terms; zero past the
+// vocabulary and past the rows (Rp: a multiple of 256)
+__global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
+    __shared__ __align__(16) U16 s0[3 * PLANE], s1[3 * PLANE];
+    __shared__ __align__(16) float sRow[3][TM];
+    const qpam_ce_bwd_args &a = p.a;
+    const int lr0 = blockIdx.y * TM, v0 = blockIdx.x * TN, tid = threadIdx.x;
+    if (tid < TM) {
+        const RowScore q = row_score(p, lr0 + tid);
+        sRow[0][tid] = q.b;
+        sRow[1][tid] = q.base;
+        sRow[2][tid] = q.slope;
+    }
+    floatx4 acc[4][4];
+    tile((const float *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(TM, p.rows - lr0),
+         (const float *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(TN, a.V - v0), a.D, acc, s0, s1);
+    const int w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wm = w >> 1, wn = w & 1;
+    float *G = (float *)p.gbuf, *GT = (float *)p.gtbuf;
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi) {
+        const int rl = 64 * wm + 16 * mi + 4 * g;
+        const floatx4 hb = *reinterpret_cast<const floatx4 *>(&sRow[0][rl]);
+        const floatx4 h0 = *reinterpret_cast<const floatx4 *>(&sRow[1][rl]);
+        const floatx4 h1 = *reinterpret_cast<const floatx4 *>(&sRow[2][rl]);
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni) {
+            const int v = v0 + 64 * wn + 16 * ni + l16;
+            floatx4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -hb[r]);
+                const bool in = v < a.V && lr0 + rl + r < p.rows;
+                x[r] = in ? __builtin_amdgcn_exp2f(u) * __builtin_fmaf(h1[r], u, h0[r]) : 0.f;
+                if (lr0 + rl + r < p.rows) G[(int64_t)(lr0 + rl + r) * p.Vp + v] = x[r];
+            }
+            *reinterpret_cast<floatx4 *>(GT + (int64_t)v * p.Rp + lr0 + rl) = x;
+        }
+    }
+}
+
+// C = A B^T (dH and dW), the K axis in gridDim.z ranges of kper: one range writes C (or
+// adds to it), several write C + z split_stride, summed by sum_kernel in their order.
+__global__ void __launch_bounds__(TT) gemm_kernel(const float *A, int64_t lda, int M, const float *B, int64_t ldb, int N, int K,
+                                                  int kper, float *C, int64_t ldc, int64_t split_stride, int accumulate) {
+    __shared__ __align__(16) U16 s0[3 * PLANE], s1[3 * PLANE];
+    const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN, k0 = blockIdx.z * kper;
+    floatx4 acc[4][4];
+    tile(A + (int64_t)m0 * lda + k0, lda, min(TM, M - m0), B + (int64_t)n0 * ldb + k0, ldb, min(TN, N - n0), min(kper, K - k0),
+         acc, s0, s1);
     C += blockIdx.z * split_stride;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
@@ -682,8 +748,7 @@ __global__ void __launch_bounds__(THREADS) split_gemm_kernel(const float *A, int
             }
 }
 
-__global__ void __launch_bounds__(THREADS) split_sum_kernel(const float *part, int splits, int64_t rows, int cols, float *out,
-                                                           int64_t ldo) {
+__global__ void __launch_bounds__(THREADS) sum_kernel(const float *part, int splits, int64_t rows, int cols, float *out, int64_t ldo) {
     const int64_t n = rows * cols;
     for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * THREADS) {
         float x = 0.f;
@@ -692,6 +757,7 @@ __global__ void __launch_bounds__(THREADS) split_sum_kernel(const float *part, i
         out[r * ldo + (i - r * cols)] = x;
     }
 }
+}  // namespace split
 
 // ------------------------------------------------------ bf16 big tiles ----
 // bf16 operands use 256 x 256 block tiles: 4 waves of 128 x 128, 8 x 8
@@ -1999,7 +2065,10 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     int st;
     if (few) {
         st = thin::waves(a.V) == 16 ? thin::launch<T, 16>(p, stream) : thin::launch<T, 4>(p, stream);
-    } else if (scores && is_bf<T>()) {
+    } else if (scores && !is_bf<T>()) {
+        hipLaunchKernelGGL(split::scores_tile_kernel, dim3(p.n_vt, (a.N + split::TM - 1) / split::TM), dim3(split::TT), 0, stream, p);
+        st = launch_status("split scores_tile_kernel");
+    } else if (scores) {
         const dim3 grid(tiles::grid(p.n_vt * ((a.N + tiles::TM - 1) / tiles::TM)));
         hipLaunchKernelGGL(tiles::scores_tile_kernel, grid, dim3(tiles::TT), 0, stream, p);
         st = launch_status("scores_tile_kernel");
@@ -2020,14 +2089,11 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
         hipLaunchKernelGGL(big::fwd_tile_kernel, grid, dim3(THREADS), big::SMEM, stream, p);
         st = launch_status("ce fwd_tile_kernel (bf16)");
     } else {
-        const size_t smem = scores ? tile_smem<T, true>() : tile_smem<T, false>();
-        const void *kern = scores ? (const void *)ce_fwd_tile_kernel<T, true> : (const void *)ce_fwd_tile_kernel<T, false>;
-        QPAM_CHECK_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        const size_t smem = gemm_smem<T>();
+        QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_fwd_tile_kernel<T>,
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         dim3 grid(p.n_vt, (a.N + BM - 1) / BM);
-        if (scores)
-            hipLaunchKernelGGL((ce_fwd_tile_kernel<T, true>), grid, dim3(THREADS), smem, stream, p);
-        else
-            hipLaunchKernelGGL((ce_fwd_tile_kernel<T, false>), grid, dim3(THREADS), smem, stream, p);
+        hipLaunchKernelGGL(ce_fwd_tile_kernel<T>, grid, dim3(THREADS), smem, stream, p);
         st = launch_status("ce_fwd_tile_kernel");
     }
     if (st) return st;
@@ -2169,7 +2235,7 @@ int run_bwd(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams *scor
     p.gtbuf = (T *)p.gbuf + (int64_t)chunk * p.Vp;
     p.ht = (T *)p.gtbuf + (int64_t)p.Vp * Rmax;
     const size_t smem = gemm_smem<T>();
-    QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_grad_tile_kernel<T, false>,
+    QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_grad_tile_kernel<T>,
                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_gemm_kernel<T, false>,
                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -2190,7 +2256,7 @@ int run_bwd(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams *scor
                            p.Rp);
         st = launch_status("transpose_kernel(H)");
         if (st) return st;
-        hipLaunchKernelGGL((ce_grad_tile_kernel<T, false>), dim3(p.Vp / VT, p.Rp / BM), dim3(THREADS), smem, stream, p);
+        hipLaunchKernelGGL(ce_grad_tile_kernel<T>, dim3(p.Vp / VT, p.Rp / BM), dim3(THREADS), smem, stream, p);
         st = launch_status("ce_grad_tile_kernel");
         if (st) return st;
         // dH[r0 .. r0+rows] = G [rows][Vp] * (W^T [D][Vp])^T
@@ -2222,74 +2288,71 @@ int validate_common(int N, int V, int D, int dtype, const void *h, int64_t ldh, 
     return QPAM_OK;
 }
 
-// Ranges of the vocabulary that share the token scores' fp32 dH of `rows` rows: two
-// blocks for each of the 256 CUs, at most 16 ranges and none below 512 entries.
+// Ranges of the vocabulary that share the token scores' fp32 dH of `rows` rows: a block for
+// each of the 256 CUs, at most 16 ranges and none below 512 entries.
 int dh_splits(int rows, int D, int Vp) {
-    const int tiles = ((rows + BM - 1) / BM) * ((D + BN - 1) / BN);
-    return std::max(1, std::min({512 / std::max(tiles, 1), Vp / 512, 16}));
+    const int tiles = ((rows + split::TM - 1) / split::TM) * ((D + split::TN - 1) / split::TN);
+    return std::max(1, std::min({256 / std::max(tiles, 1), Vp / 512, 16}));
 }
 
-// ... and their partial sums: splits * rows <= 16 rows, and <= 512 BM as splits * tiles <= 512
+// W^T, G, G^T and H^T as the loss's fp32 passes have them, the rows padded to 256, and
+// dH's partial sums: splits * rows <= 16 rows, and <= 256 TM as splits * tiles <= 256
 size_t scores_f32_ws(const qpam_ce_bwd_args &a) {
-    const int64_t rows = std::min<int64_t>(16ll * pass_rows(a), 512ll * BM);
-    return bwd_ws_base<float>(a) + 256 + (size_t)rows * a.D * 4;
+    const int64_t Vp = round_up(a.V, split::TN), chunk = pass_rows(a), Rp = round_up((int)chunk, split::TM);
+    const int64_t part = std::min<int64_t>(16 * chunk, 256ll * split::TM) * a.D;
+    return (size_t)((int64_t)a.D * Vp + chunk * Vp + Vp * Rp + (int64_t)a.D * Rp + part) * sizeof(float) + 256;
 }
 
 // Token scores in fp32: G tiles, then dH and dW, all in bf16 parts.  dW is written by the
 // first pass and added to by the others.
 int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams &scores) {
-    using T = float;
     BwdParams p = scores;
     p.a = a;
     p.write_g = 1;
-    p.Vp = round_up(a.V, VT);
+    p.Vp = round_up(a.V, split::TN);
     const int chunk = pass_rows(a);
-    const int Rmax = round_up(chunk, BM);
-    T *ws = (T *)a.workspace;
-    p.wt = ws;
-    p.gbuf = ws + (int64_t)a.D * p.Vp;
-    p.gtbuf = (T *)p.gbuf + (int64_t)chunk * p.Vp;
-    p.ht = (T *)p.gtbuf + (int64_t)p.Vp * Rmax;
-    float *part = (float *)(((uintptr_t)a.workspace + bwd_ws_base<T>(a) + 255) & ~(uintptr_t)255);
-    const size_t smem = SPLIT_SMEM;
-    QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)ce_grad_tile_kernel<T, true>,
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    QPAM_CHECK_HIP(hipFuncSetAttribute((const void *)split_gemm_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    hipLaunchKernelGGL(transpose_kernel<T>, dim3((a.D + 63) / 64, (p.Vp + 63) / 64), dim3(THREADS), 0, stream,
-                       (const T *)a.w, a.ldw, a.V, a.D, (T *)p.wt, (int64_t)p.Vp, a.D, p.Vp);
+    float *wt = (float *)a.workspace, *gb = wt + (int64_t)a.D * p.Vp, *gt = gb + (int64_t)chunk * p.Vp;
+    float *ht = gt + (int64_t)p.Vp * round_up(chunk, split::TM), *part = ht + (int64_t)a.D * round_up(chunk, split::TM);
+    p.gbuf = gb;
+    p.gtbuf = gt;
+    auto gemm = [&](const char *what, const float *A, int64_t lda, int M, const float *B, int64_t ldb, int K, int kper, float *C,
+                    int64_t ldc, int64_t stride, int accumulate) {
+        hipLaunchKernelGGL(split::gemm_kernel,
+                           dim3((a.D + split::TN - 1) / split::TN, (M + split::TM - 1) / split::TM, (K + kper - 1) / kper),
+                           dim3(split::TT), 0, stream, A, lda, M, B, ldb, a.D, K, kper, C, ldc, stride, accumulate);
+        return launch_status(what);
+    };
+    hipLaunchKernelGGL(transpose_kernel<float>, dim3((a.D + 63) / 64, (p.Vp + 63) / 64), dim3(THREADS), 0, stream,
+                       (const float *)a.w, a.ldw, a.V, a.D, wt, (int64_t)p.Vp, a.D, p.Vp);
     int st = launch_status("transpose_kernel(W)");
     if (st) return st;
     for (int r0 = 0; r0 < a.N; r0 += chunk) {
         p.row0 = r0;
         p.rows = std::min(chunk, a.N - r0);
-        p.Rp = round_up(p.rows, BM);
-        hipLaunchKernelGGL(transpose_kernel<T>, dim3((a.D + 63) / 64, (p.Rp + 63) / 64), dim3(THREADS), 0, stream,
-                           (const T *)a.h + (int64_t)r0 * a.ldh, a.ldh, p.rows, a.D, (T *)p.ht, (int64_t)p.Rp, a.D, p.Rp);
+        p.Rp = round_up(p.rows, split::TM);
+        hipLaunchKernelGGL(transpose_kernel<float>, dim3((a.D + 63) / 64, (p.Rp + 63) / 64), dim3(THREADS), 0, stream,
+                           (const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, p.rows, a.D, ht, (int64_t)p.Rp, a.D, p.Rp);
         if ((st = launch_status("transpose_kernel(H)"))) return st;
-        hipLaunchKernelGGL((ce_grad_tile_kernel<T, true>), dim3(p.Vp / VT, p.Rp / BM), dim3(THREADS), smem, stream, p);
-        if ((st = launch_status("ce_grad_tile_kernel"))) return st;
-        hipLaunchKernelGGL(scores_token_kernel<T>, dim3((p.rows + THREADS - 1) / THREADS), dim3(THREADS), 0, stream, p);
+        hipLaunchKernelGGL(split::scores_grad_kernel, dim3(p.Vp / split::TN, p.Rp / split::TM), dim3(split::TT), 0, stream, p);
+        if ((st = launch_status("split scores_grad_kernel"))) return st;
+        hipLaunchKernelGGL(scores_token_kernel<float>, dim3((p.rows + THREADS - 1) / THREADS), dim3(THREADS), 0, stream, p);
         if ((st = launch_status("scores_token_kernel"))) return st;
         // dH[r0 .. r0 + rows] = G [rows][Vp] (W^T [D][Vp])^T
         const int splits = dh_splits(p.rows, a.D, p.Vp), kper = round_up((p.Vp + splits - 1) / splits, BK);
         float *dh = (float *)a.dh + (int64_t)r0 * a.lddh;
-        hipLaunchKernelGGL(split_gemm_kernel, dim3((a.D + BN - 1) / BN, (p.rows + BM - 1) / BM, (p.Vp + kper - 1) / kper),
-                           dim3(THREADS), smem, stream, (const T *)p.gbuf, (int64_t)p.Vp, p.rows, (const T *)p.wt,
-                           (int64_t)p.Vp, a.D, p.Vp, kper, splits > 1 ? part : dh, splits > 1 ? (int64_t)a.D : a.lddh,
-                           (int64_t)p.rows * a.D, 0);
-        if ((st = launch_status("split_gemm_kernel(dH)"))) return st;
+        st = gemm("split gemm_kernel(dH)", gb, p.Vp, p.rows, wt, p.Vp, p.Vp, kper, splits > 1 ? part : dh,
+                  splits > 1 ? a.D : a.lddh, (int64_t)p.rows * a.D, 0);
+        if (st) return st;
         if (splits > 1) {
             const int64_t n = (int64_t)p.rows * a.D;
-            hipLaunchKernelGGL(split_sum_kernel, dim3((unsigned)std::min<int64_t>((n + THREADS - 1) / THREADS, 4096)),
+            hipLaunchKernelGGL(split::sum_kernel, dim3((unsigned)std::min<int64_t>((n + THREADS - 1) / THREADS, 4096)),
                                dim3(THREADS), 0, stream, (const float *)part, (p.Vp + kper - 1) / kper, (int64_t)p.rows, a.D,
                                dh, a.lddh);
-            if ((st = launch_status("split_sum_kernel"))) return st;
+            if ((st = launch_status("split sum_kernel"))) return st;
         }
         // dW [V][D] (+)= G^T [Vp][Rp] (H^T [D][Rp])^T
-        hipLaunchKernelGGL(split_gemm_kernel, dim3((a.D + BN - 1) / BN, (a.V + BM - 1) / BM, 1), dim3(THREADS), smem, stream,
-                           (const T *)p.gtbuf, (int64_t)p.Rp, a.V, (const T *)p.ht, (int64_t)p.Rp, a.D, p.Rp, p.Rp,
-                           (float *)a.dw, a.lddw, (int64_t)0, r0 > 0 ? 1 : 0);
-        if ((st = launch_status("split_gemm_kernel(dW)"))) return st;
+        st = gemm("split gemm_kernel(dW)", gt, p.Rp, a.V, ht, p.Rp, p.Rp, p.Rp, (float *)a.dw, a.lddw, 0, r0 > 0 ? 1 : 0);
+        if (st) return st;
     }
     return QPAM_OK;
 }
@@ -2446,6 +2509,8 @@ extern "C" int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void
     QPAM_REQUIRE(a->chunk >= 1, "qpam_linear_logprobs_bwd: chunk must be >= 1");
     QPAM_REQUIRE(a->lddh >= a->D && a->lddw >= a->D, "qpam_linear_logprobs_bwd: output leading dims must be >= D");
     QPAM_REQUIRE(a->dw_out == 1 || a->dw_out == 2, "qpam_linear_logprobs_bwd: dw_out must be 1 or 2");
+    QPAM_REQUIRE(a->dtype == QPAM_BF16 || (a->V < (1 << 22) - 256 && std::min(a->chunk, a->N) < (1 << 22) - 256),
+                 "qpam_linear_logprobs_bwd: fp32 takes V and chunk below 2^22 - 256");
     const size_t need = qpam_linear_logprobs_bwd_workspace_size(a);
     QPAM_REQUIRE(a->workspace && a->workspace_bytes >= need && ((uintptr_t)a->workspace % 16) == 0,
                  "qpam_linear_logprobs_bwd: workspace needs %zu bytes (got %zu)", need, a->workspace_bytes);
