@@ -2410,7 +2410,7 @@ qpam_ce_bwd_args bwd_args(const qpam_linear_logprobs_args &a) {
 int validate_scores(const qpam_linear_logprobs_args &a, const char *who) {
     int st = validate_common(a.N, a.V, a.D, a.dtype, a.h, a.ldh, a.w, a.ldw, a.ids, who);
     if (st) return st;
-    QPAM_REQUIRE(a.temperature > 0.f && a.temperature < INFINITY, "%s: temperature %g must be positive and finite", who,
+    QPAM_REQUIRE(a.temperature >= 1e-30f && a.temperature <= 1e30f, "%s: temperature %g outside 1e-30 .. 1e30", who,
                  a.temperature);
     QPAM_REQUIRE(a.entropy && a.stats, "%s: null entropy or stats", who);
     QPAM_REQUIRE((a.N + BM - 1) / BM <= 65535, "%s: too many rows", who);

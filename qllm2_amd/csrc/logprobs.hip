@@ -377,7 +377,7 @@ int check(const Args &a, const char *who) {
     QPAM_REQUIRE(a.dtype == QPAM_F32 || a.dtype == QPAM_BF16, "%s: dtype %d", who, a.dtype);
     QPAM_REQUIRE(a.n >= 0 && a.n < (1ll << 31) && a.V >= 1 && a.V <= (1 << 30), "%s: bad sizes n=%lld V=%d", who,
                  (long long)a.n, a.V);
-    QPAM_REQUIRE(a.temperature > 0.f && a.temperature < INFINITY, "%s: temperature %g must be positive and finite", who,
+    QPAM_REQUIRE(a.temperature >= 1e-30f && a.temperature <= 1e30f, "%s: temperature %g outside 1e-30 .. 1e30", who,
                  a.temperature);
     QPAM_REQUIRE(a.top_k >= 0 && a.top_k <= MAX_K && a.top_k <= a.V, "%s: top_k %d (0 to %d, at most V=%d)", who, a.top_k,
                  MAX_K, a.V);

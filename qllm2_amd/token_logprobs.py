@@ -12,7 +12,6 @@ sequences, and policy-gradient steps with an entropy term.
 """
 
 import ctypes
-import math
 from typing import List, NamedTuple, Optional
 
 import torch
@@ -39,8 +38,8 @@ class TokenLogprobs(NamedTuple):
 
 
 def _check_temperature(temperature, name):
-    if not (0.0 < temperature < math.inf):
-        raise ValueError(f"qpam {name}: temperature {temperature} must be positive and finite")
+    if not 1e-30 <= temperature <= 1e30:  # its reciprocal and what it scales stay in fp32's range
+        raise ValueError(f"qpam {name}: temperature {temperature} outside 1e-30 .. 1e30")
 
 
 def _check(logits, ids, temperature, top_k):

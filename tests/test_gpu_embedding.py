@@ -214,3 +214,25 @@ def test_two_streams_at_once(gpu_lib):
     for (ids, _, _, dz), got in zip(data, outs):
         for part in (0, 1):
             _check_grad(got[part].cpu(), ids, dz, 500, 1.0, part=part)
+
+
+def test_offsets_past_31_bits(gpu_lib):
+    """1.1 million ids of 1024 columns: the rows' elements pass 2^31.  Gradients of small
+    whole numbers, so that every sum is exact: token v gets the sum over its positions i
+    of (i % 7) - 3 in every column."""
+    from qllm2_amd.embedding import complex_embedding
+    n, V, dim = 1100000, 1000, 1024
+    ids = torch.randint(0, V, (n,), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    re, im = (torch.randn(V, dim, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    with torch.no_grad():
+        z = complex_embedding(ids, re, im)
+    assert z.numel() > 2 ** 31
+    for rows in (slice(0, 3), slice(n // 2, n // 2 + 3), slice(n - 3, n)):
+        assert torch.equal(z[rows], torch.stack([re[ids[rows]], im[ids[rows]]], -1))
+    del z
+    step = (torch.arange(n, device="cuda") % 7 - 3).bfloat16()
+    from qllm2_amd.embedding import embed_bwd_op
+    d_re, d_im = embed_bwd_op(ids, step[:, None, None].expand(n, dim, 2).contiguous(), V, 1.0, -1)
+    want = torch.zeros(V, device="cuda", dtype=torch.float64).index_add_(0, ids, step.double()).bfloat16()
+    for d in (d_re, d_im):
+        assert torch.equal(d, want[:, None].expand(V, dim))

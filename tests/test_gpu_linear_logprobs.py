@@ -210,3 +210,46 @@ def test_captured_training_step_replays(gpu_lib):
             torch.cuda.synchronize()
             for a, b in zip(outs, step()):
                 assert torch.equal(a, b)
+
+
+def test_full_vocabulary_batch(gpu_lib):
+    """16384 rows against 50261 x 512 in bf16 (a G of 823 million entries), float64 on the
+    GPU beside it; norms: a value is off by 2^-20 or so, dh and dw by the roundings of dx
+    and of themselves (2^-8 each)."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    g = torch.Generator("cuda").manual_seed(2)
+    n, V, D = 16384, 50261, 512
+    h = torch.randn(n, D, device="cuda", generator=g).bfloat16().requires_grad_()
+    w = (torch.randn(V, D, device="cuda", generator=g) * 2.5 / D ** 0.5).bfloat16().requires_grad_()
+    ids = torch.randint(0, V, (n,), device="cuda", generator=g)
+    ids[::9] = -100
+    gs = [torch.randn(n, device="cuda", generator=g) / n, torch.randn(n, device="cuda", generator=g) / n]
+    r = linear_token_logprobs(h, w, ids)
+    dh, dw = torch.autograd.grad([r.logprobs, r.entropy], [h, w], gs)
+    hd, wd = h.detach().double(), w.detach().double()
+    logp = torch.log_softmax(hd @ wd.T, -1)
+    p = logp.exp()
+    ent = -(p * logp).sum(-1)
+    valid = ids >= 0
+    lp = torch.where(valid, logp.gather(1, ids.clamp(min=0)[:, None])[:, 0], 0.0)
+    g_lp = torch.where(valid, gs[0].double(), 0.0)
+    dx = -p * (g_lp[:, None] + gs[1].double()[:, None] * (logp + ent[:, None]))
+    dx.scatter_add_(1, ids.clamp(min=0)[:, None], g_lp[:, None])
+    for got, want, tol in ((r.logprobs, lp, 2.0 ** -20), (r.entropy, ent, 2.0 ** -20), (dh, dx @ wd, 2.0 ** -7),
+                           (dw, dx.T @ hd, 2.0 ** -7)):
+        assert ((got.double() - want).norm() / want.norm()).item() < tol
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_one_operand_frozen(gpu_lib, dtype):
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, gs = _data(150, 300, 64, dtype, dtype, 8)
+    both = [h.cuda().requires_grad_(), w.cuda().requires_grad_()]
+    r = linear_token_logprobs(*both, ids.cuda())
+    want = torch.autograd.grad([r.logprobs, r.entropy], both, [g.cuda() for g in gs])
+    for i in (0, 1):
+        ops = [h.cuda(), w.cuda()]
+        ops[i].requires_grad_()
+        r = linear_token_logprobs(*ops, ids.cuda())
+        got, = torch.autograd.grad([r.logprobs, r.entropy], [ops[i]], [g.cuda() for g in gs])
+        assert torch.equal(got, want[i])

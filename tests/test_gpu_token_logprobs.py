@@ -316,3 +316,26 @@ def test_captured_pass_replays(gpu_lib):
         for a, b in zip(outs, step()):
             assert torch.equal(a.nan_to_num(7.0) if a.is_floating_point() else a,
                                b.nan_to_num(7.0) if b.is_floating_point() else b)
+
+
+def test_offsets_past_31_bits(gpu_lib):
+    """43000 bf16 rows of 50300: the last rows' elements lie past 2^31, forward and in
+    the gradient."""
+    from qllm2_amd.token_logprobs import token_logprobs
+    n, V = 43000, 50300
+    buf = torch.zeros(n, V, device="cuda", dtype=torch.bfloat16)
+    assert buf.numel() > 2 ** 31
+    x, ids = _rows("normal", 4, V, torch.bfloat16, 9)
+    buf[-4:] = x.cuda()
+    all_ids = torch.full((n,), 7, device="cuda")
+    all_ids[-4:] = ids.cuda()
+    buf.requires_grad_()
+    r = token_logprobs(buf, all_ids, top_k=3)
+    _check(x, ids, 3, 1.0, type(r)(*(t[-4:] for t in r)))
+    _check(torch.zeros(1, V), torch.tensor([7]), 3, 1.0, type(r)(*(t[:1] for t in r)))
+    g = torch.zeros(n, device="cuda")
+    g[-4:] = torch.tensor([1.0, -2.0, 0.5, 3.0], device="cuda")
+    got, = torch.autograd.grad([r.logprobs, r.entropy], [buf], [g, 0.1 * g])
+    g4 = g[-4:].cpu()
+    _grad_check(x, ids, 0, 1.0, [g4.double(), (0.1 * g4).double(), None], got[-4:], None)
+    assert (got[:-4] == 0).all()
