@@ -2412,6 +2412,7 @@ int validate_scores(const qpam_linear_logprobs_args &a, const char *who) {
     if (st) return st;
     QPAM_REQUIRE(a.temperature >= 1e-30f && a.temperature <= 1e30f, "%s: temperature %g outside 1e-30 .. 1e30", who,
                  a.temperature);
+    QPAM_REQUIRE(a.V <= (1 << 30), "%s: V=%d (at most 2^30)", who, a.V);
     QPAM_REQUIRE(a.entropy && a.stats, "%s: null entropy or stats", who);
     QPAM_REQUIRE((a.N + BM - 1) / BM <= 65535, "%s: too many rows", who);
     QPAM_REQUIRE(a.ldh < (1 << 22) && a.ldw < (1 << 22), "%s: row strides of 2^22 elements or more", who);

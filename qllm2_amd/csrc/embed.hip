@@ -442,6 +442,7 @@ __global__ void __launch_bounds__(THREADS) grad_runs_kernel(GradParams p) {
 
 // ------------------------------------------------------------------ host ---
 constexpr int64_t MAX_N = (int64_t)1 << 30;
+constexpr int64_t MAX_THREADS = (int64_t)1 << 31;  // of a launch, which holds less than 2^32
 
 struct Layout {
     size_t list[2], hist, part, bytes;
@@ -482,19 +483,26 @@ int run_lookup(const qpam_embed_args &a, hipStream_t stream) {
     const int steps = wide ? a.dim / W : a.dim;
     int lg = 0;
     while (lg < 6 && (1 << lg) < steps) ++lg;
-    const int64_t blocks = ((a.n << lg) + THREADS - 1) / THREADS;
-    QPAM_REQUIRE(blocks < (1ll << 31), "qpam_embed_fwd: too many rows");
-    if (wide)
-        hipLaunchKernelGGL((lookup_kernel<T, W>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, a, lg);
-    else
-        hipLaunchKernelGGL((lookup_kernel<T, 1>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, a, lg);
-    return launch_status("embed lookup_kernel");
+    const int64_t per = MAX_THREADS >> lg;  // rows of a launch
+    for (int64_t n0 = 0; n0 < a.n; n0 += per) {
+        qpam_embed_args s = a;
+        s.n = std::min(per, a.n - n0);
+        s.ids = static_cast<const char *>(a.ids) + n0 * (a.ids_i64 ? 8 : 4);
+        s.out = static_cast<T *>(a.out) + n0 * 2 * a.dim;
+        const unsigned blocks = (unsigned)(((s.n << lg) + THREADS - 1) / THREADS);
+        if (wide)
+            hipLaunchKernelGGL((lookup_kernel<T, W>), dim3(blocks), dim3(THREADS), 0, stream, s, lg);
+        else
+            hipLaunchKernelGGL((lookup_kernel<T, 1>), dim3(blocks), dim3(THREADS), 0, stream, s, lg);
+        const int st = launch_status("embed lookup_kernel");
+        if (st) return st;
+    }
+    return QPAM_OK;
 }
 
 template <typename T, int W>
 int launch_grad(const GradParams &g, hipStream_t stream) {
     const int64_t items = (int64_t)g.chunks * g.segs;
-    QPAM_REQUIRE(items < (1ll << 31), "qpam_embed_bwd: too many rows");
     hipLaunchKernelGGL((grad_chunk_kernel<T, W>), dim3((unsigned)((items + 3) / 4)), dim3(THREADS), 0, stream, g);
     int st = launch_status("embed grad_chunk_kernel");
     if (st || g.chunks < 2) return st;
@@ -504,7 +512,12 @@ int launch_grad(const GradParams &g, hipStream_t stream) {
 
 template <typename T>
 int run_grad(const qpam_embed_args &a, hipStream_t stream) {
+    constexpr int W = 8 / sizeof(T);
+    const bool wide = a.dim % W == 0;
     const Layout l = layout(a.n, a.dim);
+    GradParams g;
+    g.segs = (a.dim + 64 * (wide ? W : 1) - 1) / (64 * (wide ? W : 1));
+    QPAM_REQUIRE((int64_t)l.chunks * g.segs * THREADS <= MAX_THREADS, "qpam_embed_bwd: too many ids for this dim");
     char *ws = static_cast<char *>(a.workspace);
     SortParams s;
     s.a = a;
@@ -549,16 +562,12 @@ int run_grad(const qpam_embed_args &a, hipStream_t stream) {
             s.pos = s.pos2;
         }
     }
-    GradParams g;
     g.a = a;
     g.n = (int)a.n;
     g.chunks = l.chunks;
     g.key = list[at];
     g.pos = list[at] + a.n;
     g.part = reinterpret_cast<float *>(ws + l.part);
-    constexpr int W = 8 / sizeof(T);
-    const bool wide = a.dim % W == 0;
-    g.segs = (a.dim + 64 * (wide ? W : 1) - 1) / (64 * (wide ? W : 1));
     return wide ? launch_grad<T, W>(g, stream) : launch_grad<T, 1>(g, stream);
 }
 

@@ -29,6 +29,8 @@ def _check(ids, weight_real, weight_imag):
     if weight_real.dim() != 2 or weight_real.shape != weight_imag.shape or not weight_real.numel():
         raise ValueError(f"qpam complex_embedding: two tables [V, dim] expected, got {tuple(weight_real.shape)} and "
                          f"{tuple(weight_imag.shape)}")
+    if weight_real.shape[0] >= 2 ** 30 or weight_real.shape[1] > 2 ** 20:  # 32-bit sizes below
+        raise ValueError(f"qpam complex_embedding: table {tuple(weight_real.shape)} too large (below 2^30 rows of at most 2^20)")
     if weight_real.dtype not in _CODE or weight_real.dtype != weight_imag.dtype:
         raise ValueError("qpam complex_embedding: both tables must be float32 or both bfloat16, got "
                          f"{weight_real.dtype} and {weight_imag.dtype}")

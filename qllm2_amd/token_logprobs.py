@@ -24,6 +24,8 @@ from .fused_ce import _operands
 __all__ = ["TokenLogprobs", "token_logprobs", "linear_token_logprobs"]
 
 MAX_TOP_K = 64
+MAX_VOCAB = 2 ** 30  # 32-bit sizes below
+MAX_ROWS = 65535 * 128  # hidden rows: a launch's second axis
 
 _CODE = {torch.float32: _lib.QPAM_F32, torch.bfloat16: _lib.QPAM_BF16}
 
@@ -52,6 +54,8 @@ def _check(logits, ids, temperature, top_k):
     if logits.dim() < 1 or logits.shape[:-1] != ids.shape or logits.shape[-1] < 1:
         raise ValueError(f"qpam token_logprobs: logits [..., V] and ids [...] expected, got {tuple(logits.shape)} and "
                          f"{tuple(ids.shape)}")
+    if logits.shape[-1] > MAX_VOCAB:
+        raise ValueError(f"qpam token_logprobs: rows of {logits.shape[-1]} logits (at most 2^30)")
     if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
         raise ValueError(f"qpam token_logprobs: top_k {top_k} outside 0 .. {min(MAX_TOP_K, logits.shape[-1])}")
     _check_temperature(temperature, "token_logprobs")
@@ -175,6 +179,9 @@ def _check_linear(hidden_rows, weight_matrix, ids, temperature, chunk):
             or hidden_rows.shape[:-1] != ids.shape or not weight_matrix.numel()):
         raise ValueError(f"qpam {name}: hidden_rows [..., D], weight_matrix [V, D] and ids [...] expected, got "
                          f"{tuple(hidden_rows.shape)}, {tuple(weight_matrix.shape)} and {tuple(ids.shape)}")
+    if weight_matrix.shape[0] > MAX_VOCAB or weight_matrix.shape[1] >= 2 ** 22 or ids.numel() > MAX_ROWS:
+        raise ValueError(f"qpam {name}: at most 2^30 table rows, {MAX_ROWS} hidden rows, below 2^22 columns, got "
+                         f"{tuple(weight_matrix.shape)} and {ids.numel()}")
     if chunk < 1:
         raise ValueError(f"qpam {name}: chunk {chunk} must be at least 1")
     _check_temperature(temperature, name)

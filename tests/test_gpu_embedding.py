@@ -236,3 +236,16 @@ def test_offsets_past_31_bits(gpu_lib):
     want = torch.zeros(V, device="cuda", dtype=torch.float64).index_add_(0, ids, step.double()).bfloat16()
     for d in (d_re, d_im):
         assert torch.equal(d, want[:, None].expand(V, dim))
+
+
+def test_more_rows_than_one_launch_holds(gpu_lib):
+    """2^25 rows of 64 lanes are a launch; rows behind it go in a second one."""
+    from qllm2_amd.embedding import complex_embedding
+    n, V, dim = 2 ** 25 + 5, 50, 33
+    g = torch.Generator(device="cuda").manual_seed(5)
+    re, im = (torch.randn(V, dim, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(2))
+    ids = torch.randint(0, V, (n,), device="cuda", dtype=torch.int32, generator=g)
+    z = complex_embedding(ids, re, im)
+    for rows in (slice(0, 3), slice(2 ** 25 - 4, n)):
+        t = ids[rows].long()
+        assert torch.equal(z[rows], torch.stack([re[t], im[t]], -1))

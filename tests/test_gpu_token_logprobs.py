@@ -339,3 +339,22 @@ def test_offsets_past_31_bits(gpu_lib):
     g4 = g[-4:].cpu()
     _grad_check(x, ids, 0, 1.0, [g4.double(), (0.1 * g4).double(), None], got[-4:], None)
     assert (got[:-4] == 0).all()
+
+
+def test_more_rows_than_one_launch_holds(gpu_lib):
+    """2^23 blocks of 256 threads are a launch; rows behind it go in a second one."""
+    from qllm2_amd.token_logprobs import token_logprobs
+    n, V = 2 ** 23 + 5, 8
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(n, V, device="cuda", dtype=torch.bfloat16, generator=g).requires_grad_()
+    ids = torch.randint(0, V, (n,), device="cuda", generator=g)
+    r = token_logprobs(x, ids, top_k=1)
+    (r.logprobs.sum() + r.entropy.sum() + r.top_logprobs.sum()).backward()
+    rows = torch.cat([torch.arange(3), torch.arange(2 ** 23 - 4, n)]).cuda()
+    y = x.detach()[rows].requires_grad_()
+    q = token_logprobs(y, ids[rows], top_k=1)
+    (q.logprobs.sum() + q.entropy.sum() + q.top_logprobs.sum()).backward()
+    for a, b in zip(r, q):
+        assert torch.equal(a[rows], b)
+    assert torch.equal(x.grad[rows], y.grad)
+    assert (r.logprobs.detach() < 0).all()

@@ -38,6 +38,9 @@ def test_embedding_refusals():
             (c(3, dtype=torch.long), c(0, 4), c(0, 4), "two tables"),
             (c(3, dtype=torch.long), c(5, 4), c(5, 4, dtype=torch.bfloat16), "float32"),
             (c(3, dtype=torch.long), c(5, 4, dtype=torch.float16), c(5, 4, dtype=torch.float16), "float32"),
+            # sizes that 32 bits would wrap to small ones
+            (c(3, dtype=torch.long), c(2 ** 32 + 5, 4), c(2 ** 32 + 5, 4), "too large"),
+            (c(3, dtype=torch.long), c(5, 2 ** 32 + 4), c(5, 2 ** 32 + 4), "too large"),
         ]
         for ids, re, im, what in bad:
             with pytest.raises(ValueError, match=what):
@@ -68,6 +71,7 @@ def test_embedding_entry_errors_without_gpu():
     assert "null" in err("qpam_embed_fwd", out=None)
     assert "null" in err("qpam_embed_bwd", dz=None)
     assert "aligned" in err("qpam_embed_bwd", d_im=4104)
+    assert "too many ids" in err("qpam_embed_bwd", n=1 << 28, dim=65, workspace_bytes=1 << 50)
     assert "workspace" in err("qpam_embed_bwd", workspace_bytes=16)
     a = _lib.EmbedArgs()
     a.n, a.dim = 0, 8
@@ -102,6 +106,7 @@ def test_token_logprobs_refusals():
             ((x, c(4, 1, dtype=torch.long), 1.0, 0), "ids"),
             ((c(4, 0), ids, 1.0, 0), "ids"),
             ((x, ids, 1.0, 10), "top_k"), ((x, ids, 1.0, -1), "top_k"), ((c(4, 100), ids, 1.0, 65), "top_k"),
+            ((c(4, 2 ** 32 + 9), ids, 1.0, 0), "at most 2\\^30"),
             ((x, ids, 0.0, 0), "temperature"), ((x, ids, -1.0, 0), "temperature"),
             ((x, ids, float("inf"), 0), "temperature"), ((x, ids, float("nan"), 0), "temperature"),
         ]:
@@ -162,6 +167,8 @@ def test_linear_token_logprobs_refusals():
             ((h, c(9, 31), ids, 1.0, 1), "hidden_rows"), ((h, c(0, 32), ids, 1.0, 1), "hidden_rows"),
             ((h, c(1, 9, 32), ids, 1.0, 1), "hidden_rows"), ((h, w, ids, 1.0, 0), "chunk"),
             ((h, w, ids, 0.0, 1), "temperature"), ((h, w, ids, float("nan"), 1), "temperature"),
+            ((h, c(2 ** 32 + 9, 32), ids, 1.0, 1), "at most 2\\^30"),
+            ((c(2 ** 32 + 4, 32), w, c(2 ** 32 + 4, dtype=torch.long), 1.0, 1), "hidden rows"),
         ]:
             with pytest.raises(ValueError, match=what):
                 _check_linear(*args)
@@ -186,7 +193,7 @@ def test_linear_token_logprobs_entry_errors_without_gpu():
         assert "multiple" in err(fn, D=63) and "null" in err(fn, ids=None) and "aligned" in err(fn, h=4100)
         assert "temperature" in err(fn, temperature=0.0) and "temperature" in err(fn, temperature=float("nan"))
         assert "stats" in err(fn, stats=None) and "workspace" in err(fn, workspace_bytes=64)
-        assert "logprobs" in err(fn, logprobs=None)
+        assert "logprobs" in err(fn, logprobs=None) and "2^30" in err(fn, V=(1 << 30) + 1)
     assert "dh" in err("qpam_linear_logprobs_bwd", dh=None) and "dw_out" in err("qpam_linear_logprobs_bwd", dw_out=0)
     assert "chunk" in err("qpam_linear_logprobs_bwd", chunk=0)
     assert "leading" in err("qpam_linear_logprobs_bwd", lddw=60)
