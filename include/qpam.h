@@ -45,6 +45,8 @@
  *   qpam_logprobs_fwd   log-softmax rows, their token entries, entropy and top
  *   qpam_logprobs_bwd   entries: what V11LM.generate (v11/model.py:1207-1245) has
  *                       in its softmax and top-k and does not return
+ *   qpam_linear_logprobs_fwd/_bwd  the same of hidden rows and the tied table: the
+ *                       logits of V11LM.ce_from_lm (v11/model.py:1175-1190)
  *   qpam_embed_fwd/_bwd v11/complex_ops.py:223-235 ComplexEmbed.forward and its
  *                       autograd backward (two nn.Embedding gradients)
  *   qpam_prologue_fwd   the elementwise steps of V11PAMLayer between the
@@ -847,7 +849,7 @@ int qpam_embed_bwd(const qpam_embed_args *a, void *stream);
  *   entropy[i]  = -sum p ln p
  *   top_ids[i][0 .. top_k), top_logprobs: the largest entries in descending order,
  *     equal values by the lower index (NaN above +inf, -0 equal to +0); top_k at
- *     most 64 and at most V.
+ *     most 64 and at most V.  Temperature 1e-30 to 1e30.
  *   stats[i] = (max x, sum exp((x - max) / temperature)): what the gradient needs
  *     (optional in the forward).
  * Entries of -inf have probability 0.  A row of nothing else: log probabilities
@@ -880,9 +882,12 @@ int qpam_logprobs_bwd(const qpam_logprobs_args *a, void *stream);
  * (h [N][D], w [V][D] as qpam_ce_fwd's) without logits in memory, and the gradient:
  * the tied LM head's token scores (logits of V11LM.ce_from_lm, v11/model.py:1175-1190).
  * bf16 operands: fp32 sums of exact products; the gradient's dx is rounded to bf16
- * between the tiles and the two products dh = dx w, dw = dx^T h.  D a multiple of 32;
- * h and w as qpam_ce_fwd takes them.  chunk bounds the backward's memory as
- * qpam_ce_bwd's does; dw_out 1: dw in dtype, 2: dw in fp32 (both written). */
+ * between the tiles and the two products dh = dx w, dw = dx^T h.  fp32
+ * operands: each value as the sum of three bf16 parts, products to about 2^-24.  D a
+ * multiple of 32; h and w as qpam_ce_fwd takes them, with row strides below 2^22.  V at
+ * most 2^30 (backward in fp32: V and chunk below 2^22 - 256).  Temperature 1e-30 to 1e30.
+ * chunk bounds the backward's memory as qpam_ce_bwd's does; dw_out 1: dw in dtype, 2: dw
+ * in fp32.  dh or dw may be NULL: its product is left out; the other is written. */
 typedef struct {
     int32_t N, V, D;
     int32_t dtype;

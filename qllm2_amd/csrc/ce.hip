@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(THREADS) scores_token_kernel(BwdParams p) {
     T v;
     if constexpr (sizeof(T) == 2) v = __builtin_bit_cast(unsigned short, (__bf16)x);
     else v = x;
-    static_cast<T *>(p.gtbuf)[id * p.Rp + lr] = v;
+    if (p.gtbuf) static_cast<T *>(p.gtbuf)[id * p.Rp + lr] = v;
     if (p.write_g) static_cast<T *>(p.gbuf)[(int64_t)lr * p.Vp + id] = v;
 }
 
@@ -681,8 +681,8 @@ __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
     }
 }
 
-// G [rows][Vp] and G^T [Vp][Rp] without the tokens' one-hot terms; zero past the
-// vocabulary and past the rows (Rp: a multiple of 256)
+// G [rows][Vp] and G^T [Vp][Rp] (each if there is a buffer for it) without the tokens'
+// one-hot terms; zero past the vocabulary and past the rows (Rp: a multiple of 256)
 __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
     __shared__ __align__(16) U16 s0[3 * PLANE], s1[3 * PLANE];
     __shared__ __align__(16) float sRow[3][TM];
@@ -715,9 +715,9 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
                 const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -hb[r]);
                 const bool in = v < a.V && lr0 + rl + r < p.rows;
                 x[r] = in ? __builtin_amdgcn_exp2f(u) * __builtin_fmaf(h1[r], u, h0[r]) : 0.f;
-                if (lr0 + rl + r < p.rows) G[(int64_t)(lr0 + rl + r) * p.Vp + v] = x[r];
+                if (G && lr0 + rl + r < p.rows) G[(int64_t)(lr0 + rl + r) * p.Vp + v] = x[r];
             }
-            *reinterpret_cast<floatx4 *>(GT + (int64_t)v * p.Rp + lr0 + rl) = x;
+            if (GT) *reinterpret_cast<floatx4 *>(GT + (int64_t)v * p.Rp + lr0 + rl) = x;
         }
     }
 }
@@ -2164,10 +2164,12 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
             p.Rp = round_up(p.rows, big::BTM);
             int st = launch_grad();
             if (st) return st;
-            st = blas::gemm_bf16(false, false, a.D, a.V, p.rows, (const U *)a.h + (int64_t)r0 * a.ldh, a.ldh,
-                                 p.gtbuf, p.Rp, dw_write ? 0.f : 1.f, a.dw, a.lddw, !(dw_write && a.dw_out == 1),
-                                 q.dh_part, blas_ws, stream);
+            if (a.dw)
+                st = blas::gemm_bf16(false, false, a.D, a.V, p.rows, (const U *)a.h + (int64_t)r0 * a.ldh, a.ldh,
+                                     p.gtbuf, p.Rp, dw_write ? 0.f : 1.f, a.dw, a.lddw, !(dw_write && a.dw_out == 1),
+                                     q.dh_part, blas_ws, stream);
             if (st) return st;
+            if (!a.dh) continue;
             st = blas::gemm_bf16(false, true, a.D, p.rows, a.V, a.w, a.ldw, p.gtbuf, p.Rp, 0.f,
                                  (U *)a.dh + (int64_t)r0 * a.lddh, a.lddh, false, q.dh_part, blas_ws, stream);
             if (st) return st;
@@ -2206,9 +2208,12 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
         st = launch_grad();
         if (st) return st;
         q.dh_ntiles_m = (p.rows + big::BTM - 1) / big::BTM;
-        hipLaunchKernelGGL(big::dw_gemm_kernel, dim3(big::xcd_grid(q.n_dw)), dim3(THREADS), smem, stream, q);
-        st = launch_status("ce dw_gemm_kernel (bf16)");
-        if (st) return st;
+        if (a.dw) {
+            hipLaunchKernelGGL(big::dw_gemm_kernel, dim3(big::xcd_grid(q.n_dw)), dim3(THREADS), smem, stream, q);
+            st = launch_status("ce dw_gemm_kernel (bf16)");
+            if (st) return st;
+        }
+        if (!a.dh) continue;
         hipLaunchKernelGGL(big::dh_gemm_kernel, dim3(big::xcd_grid(q.splits * q.dh_ntiles_m * q.dh_ntiles_n)),
                            dim3(THREADS), smem, stream, q);
         st = launch_status("ce dh_gemm_kernel (bf16)");
@@ -2303,18 +2308,18 @@ size_t scores_f32_ws(const qpam_ce_bwd_args &a) {
     return (size_t)((int64_t)a.D * Vp + chunk * Vp + Vp * Rp + (int64_t)a.D * Rp + part) * sizeof(float) + 256;
 }
 
-// Token scores in fp32: G tiles, then dH and dW, all in bf16 parts.  dW is written by the
-// first pass and added to by the others.
+// Token scores in fp32: G tiles, then dH and dW (those that are asked for), all in bf16
+// parts.  dW is written by the first pass and added to by the others.
 int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams &scores) {
     BwdParams p = scores;
     p.a = a;
-    p.write_g = 1;
+    p.write_g = a.dh != nullptr;
     p.Vp = round_up(a.V, split::TN);
     const int chunk = pass_rows(a);
     float *wt = (float *)a.workspace, *gb = wt + (int64_t)a.D * p.Vp, *gt = gb + (int64_t)chunk * p.Vp;
     float *ht = gt + (int64_t)p.Vp * round_up(chunk, split::TM), *part = ht + (int64_t)a.D * round_up(chunk, split::TM);
-    p.gbuf = gb;
-    p.gtbuf = gt;
+    p.gbuf = a.dh ? gb : nullptr;
+    p.gtbuf = a.dw ? gt : nullptr;
     auto gemm = [&](const char *what, const float *A, int64_t lda, int M, const float *B, int64_t ldb, int K, int kper, float *C,
                     int64_t ldc, int64_t stride, int accumulate) {
         hipLaunchKernelGGL(split::gemm_kernel,
@@ -2322,17 +2327,21 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
                            dim3(split::TT), 0, stream, A, lda, M, B, ldb, a.D, K, kper, C, ldc, stride, accumulate);
         return launch_status(what);
     };
-    hipLaunchKernelGGL(transpose_kernel<float>, dim3((a.D + 63) / 64, (p.Vp + 63) / 64), dim3(THREADS), 0, stream,
-                       (const float *)a.w, a.ldw, a.V, a.D, wt, (int64_t)p.Vp, a.D, p.Vp);
-    int st = launch_status("transpose_kernel(W)");
-    if (st) return st;
+    int st = QPAM_OK;
+    if (a.dh) {
+        hipLaunchKernelGGL(transpose_kernel<float>, dim3((a.D + 63) / 64, (p.Vp + 63) / 64), dim3(THREADS), 0, stream,
+                           (const float *)a.w, a.ldw, a.V, a.D, wt, (int64_t)p.Vp, a.D, p.Vp);
+        if ((st = launch_status("transpose_kernel(W)"))) return st;
+    }
     for (int r0 = 0; r0 < a.N; r0 += chunk) {
         p.row0 = r0;
         p.rows = std::min(chunk, a.N - r0);
         p.Rp = round_up(p.rows, split::TM);
-        hipLaunchKernelGGL(transpose_kernel<float>, dim3((a.D + 63) / 64, (p.Rp + 63) / 64), dim3(THREADS), 0, stream,
-                           (const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, p.rows, a.D, ht, (int64_t)p.Rp, a.D, p.Rp);
-        if ((st = launch_status("transpose_kernel(H)"))) return st;
+        if (a.dw) {
+            hipLaunchKernelGGL(transpose_kernel<float>, dim3((a.D + 63) / 64, (p.Rp + 63) / 64), dim3(THREADS), 0, stream,
+                               (const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, p.rows, a.D, ht, (int64_t)p.Rp, a.D, p.Rp);
+            if ((st = launch_status("transpose_kernel(H)"))) return st;
+        }
         hipLaunchKernelGGL(split::scores_grad_kernel, dim3(p.Vp / split::TN, p.Rp / split::TM), dim3(split::TT), 0, stream, p);
         if ((st = launch_status("split scores_grad_kernel"))) return st;
         hipLaunchKernelGGL(scores_token_kernel<float>, dim3((p.rows + THREADS - 1) / THREADS), dim3(THREADS), 0, stream, p);
@@ -2340,16 +2349,19 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
         // dH[r0 .. r0 + rows] = G [rows][Vp] (W^T [D][Vp])^T
         const int splits = dh_splits(p.rows, a.D, p.Vp), kper = round_up((p.Vp + splits - 1) / splits, BK);
         float *dh = (float *)a.dh + (int64_t)r0 * a.lddh;
-        st = gemm("split gemm_kernel(dH)", gb, p.Vp, p.rows, wt, p.Vp, p.Vp, kper, splits > 1 ? part : dh,
-                  splits > 1 ? a.D : a.lddh, (int64_t)p.rows * a.D, 0);
-        if (st) return st;
-        if (splits > 1) {
+        if (a.dh) {
+            st = gemm("split gemm_kernel(dH)", gb, p.Vp, p.rows, wt, p.Vp, p.Vp, kper, splits > 1 ? part : dh,
+                      splits > 1 ? a.D : a.lddh, (int64_t)p.rows * a.D, 0);
+            if (st) return st;
+        }
+        if (a.dh && splits > 1) {
             const int64_t n = (int64_t)p.rows * a.D;
             hipLaunchKernelGGL(split::sum_kernel, dim3((unsigned)std::min<int64_t>((n + THREADS - 1) / THREADS, 4096)),
                                dim3(THREADS), 0, stream, (const float *)part, (p.Vp + kper - 1) / kper, (int64_t)p.rows, a.D,
                                dh, a.lddh);
             if ((st = launch_status("split sum_kernel"))) return st;
         }
+        if (!a.dw) continue;
         // dW [V][D] (+)= G^T [Vp][Rp] (H^T [D][Rp])^T
         st = gemm("split gemm_kernel(dW)", gt, p.Rp, a.V, ht, p.Rp, p.Rp, p.Rp, (float *)a.dw, a.lddw, 0, r0 > 0 ? 1 : 0);
         if (st) return st;
@@ -2361,7 +2373,7 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
 int run_backward(const qpam_ce_bwd_args &a, hipStream_t s, const BwdParams *scores) {
     if (scores && a.dtype == QPAM_F32) return run_scores_f32(a, s, *scores);
     if (a.dw_out == 0) return a.dtype == QPAM_BF16 ? run_bwd<unsigned short>(a, s, scores) : run_bwd<float>(a, s, scores);
-    if (dw_direct(a)) return run_bwd_bf16(a, s, scores, true);
+    if (dw_direct(a) || !a.dw) return run_bwd_bf16(a, s, scores, true);
     // dW accumulated in fp32 -- dw itself when it is fp32, else the workspace's tail -- from zero
     qpam_ce_bwd_args b = a;
     b.dw_out = 0;
@@ -2506,9 +2518,9 @@ extern "C" int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void
     QPAM_REQUIRE(a != nullptr, "qpam_linear_logprobs_bwd: null args");
     int st = validate_scores(*a, "qpam_linear_logprobs_bwd");
     if (st) return st;
-    QPAM_REQUIRE(a->logprobs && a->dh && a->dw, "qpam_linear_logprobs_bwd: null logprobs, dh or dw");
+    QPAM_REQUIRE(a->logprobs && (a->dh || a->dw), "qpam_linear_logprobs_bwd: null logprobs, or neither dh nor dw");
     QPAM_REQUIRE(a->chunk >= 1, "qpam_linear_logprobs_bwd: chunk must be >= 1");
-    QPAM_REQUIRE(a->lddh >= a->D && a->lddw >= a->D, "qpam_linear_logprobs_bwd: output leading dims must be >= D");
+    QPAM_REQUIRE((!a->dh || a->lddh >= a->D) && (!a->dw || a->lddw >= a->D), "qpam_linear_logprobs_bwd: output leading dims must be >= D");
     QPAM_REQUIRE(a->dw_out == 1 || a->dw_out == 2, "qpam_linear_logprobs_bwd: dw_out must be 1 or 2");
     QPAM_REQUIRE(a->dtype == QPAM_BF16 || (a->V < (1 << 22) - 256 && std::min(a->chunk, a->N) < (1 << 22) - 256),
                  "qpam_linear_logprobs_bwd: fp32 takes V and chunk below 2^22 - 256");

@@ -231,21 +231,24 @@ def _(hidden_rows, weight_matrix, weight_copy, ids, temperature, chunk, ignore_i
 
 def _linear_gradient(hidden_rows: Tensor, weight_matrix: Tensor, ids: Tensor, logprobs: Tensor, entropy: Tensor,
                      stats: Tensor, g_logprobs: Optional[Tensor], g_entropy: Optional[Tensor], temperature: float, chunk: int,
-                     ignore_index: int, dw_fp32: bool) -> List[Tensor]:
+                     ignore_index: int, dw_fp32: bool, need_dh: bool = True, need_dw: bool = True) -> List[Tensor]:
     """[d hidden_rows, d weight_matrix] in the inputs' dtypes (d weight_matrix in fp32
-    with dw_fp32)."""
+    with dw_fp32); one that is not needed is an empty tensor."""
     h, w, dtype = _operands(hidden_rows, weight_matrix)
     n, dev = h.shape[0], h.device
     dw_fp32 = dw_fp32 or weight_matrix.dtype != w.dtype
-    dh = torch.empty(h.shape, device=dev, dtype=h.dtype)
-    dw = torch.empty(w.shape, device=dev, dtype=torch.float32 if dw_fp32 else w.dtype)
-    if not n:
+    dh = torch.empty(h.shape if need_dh else 0, device=dev, dtype=h.dtype)
+    dw = torch.empty(w.shape if need_dw else 0, device=dev, dtype=torch.float32 if dw_fp32 else w.dtype)
+    if not n or not (need_dh or need_dw):
         return [dh.to(hidden_rows.dtype), dw.zero_()]
     ids = ids.contiguous()
     gs = [g if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy)]
     a = _linear_args(h, w, dtype, ids, logprobs, entropy, stats, temperature, ignore_index)
     a.g_logprobs, a.g_entropy = (g if g is None else g.data_ptr() for g in gs)
-    a.dh, a.lddh, a.dw, a.lddw = dh.data_ptr(), dh.stride(0), dw.data_ptr(), dw.stride(0)
+    if need_dh:
+        a.dh, a.lddh = dh.data_ptr(), dh.stride(0)
+    if need_dw:
+        a.dw, a.lddw = dw.data_ptr(), dw.stride(0)
     a.chunk, a.dw_out = min(chunk, n), 2 if dw_fp32 else 1
     L = _lib.lib()
     ws = _workspace(a, L.qpam_linear_logprobs_bwd_workspace_size(ctypes.byref(a)), dev)  # noqa: F841
@@ -259,9 +262,10 @@ linear_logprobs_bwd_op = _ops.op("qpam::linear_logprobs_bwd", direct=True)(_line
 
 @linear_logprobs_bwd_op.register_fake
 def _(hidden_rows, weight_matrix, ids, logprobs, entropy, stats, g_logprobs, g_entropy, temperature, chunk, ignore_index,
-      dw_fp32):
-    return [hidden_rows.new_empty(hidden_rows.shape),
-            weight_matrix.new_empty(weight_matrix.shape, dtype=torch.float32 if dw_fp32 else weight_matrix.dtype)]
+      dw_fp32, need_dh=True, need_dw=True):
+    return [hidden_rows.new_empty(hidden_rows.shape if need_dh else 0),
+            weight_matrix.new_empty(weight_matrix.shape if need_dw else 0,
+                                    dtype=torch.float32 if dw_fp32 else weight_matrix.dtype)]
 
 
 def _linear_setup(ctx, inputs, output):
@@ -276,9 +280,10 @@ def _linear_backward(ctx, grads):
     g_lp, g_ent, _ = grads
     if g_lp is None and g_ent is None:
         return (None,) * 7
+    need_dh, need_dw = ctx.needs_input_grad[:2]
     dh, dw = linear_logprobs_bwd_op(*ctx.saved_tensors, g_lp, g_ent, ctx.temperature, ctx.chunk, ctx.ignore_index,
-                                    ctx.master)
-    return dh, dw, None, None, None, None, None
+                                    ctx.master, need_dh, need_dw)
+    return dh if need_dh else None, dw if need_dw else None, None, None, None, None, None
 
 
 linear_logprobs_fwd_op.register_autograd(_linear_backward, setup_context=_linear_setup)

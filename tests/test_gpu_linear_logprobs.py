@@ -253,3 +253,20 @@ def test_one_operand_frozen(gpu_lib, dtype):
         r = linear_token_logprobs(*ops, ids.cuda())
         got, = torch.autograd.grad([r.logprobs, r.entropy], [ops[i]], [g.cuda() for g in gs])
         assert torch.equal(got, want[i])
+
+
+@pytest.mark.parametrize("dtype,wdtype", [(F32, F32), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("n,V,D,chunk", [(900, 500, 96, 70), (300, 700, 64, 4096), (5, 40, 32, 1)])
+def test_one_operand_frozen_over_several_passes(gpu_lib, n, V, D, chunk, dtype, wdtype):
+    """The product of an operand without a gradient is left out; the other's stays the same bits."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, gs = _data(n, V, D, dtype, wdtype, 9)
+    both = [h.cuda().requires_grad_(), w.cuda().requires_grad_()]
+    r = linear_token_logprobs(*both, ids.cuda(), temperature=0.8, chunk=chunk)
+    want = torch.autograd.grad([r.logprobs, r.entropy], both, [g.cuda() for g in gs])
+    for i in (0, 1):
+        ops = [h.cuda(), w.cuda()]
+        ops[i].requires_grad_()
+        r = linear_token_logprobs(*ops, ids.cuda(), temperature=0.8, chunk=chunk)
+        got, = torch.autograd.grad([r.logprobs, r.entropy], [ops[i]], [g.cuda() for g in gs])
+        assert torch.equal(got, want[i])

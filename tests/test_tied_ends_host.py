@@ -194,7 +194,7 @@ def test_linear_token_logprobs_entry_errors_without_gpu():
         assert "temperature" in err(fn, temperature=0.0) and "temperature" in err(fn, temperature=float("nan"))
         assert "stats" in err(fn, stats=None) and "workspace" in err(fn, workspace_bytes=64)
         assert "logprobs" in err(fn, logprobs=None) and "2^30" in err(fn, V=(1 << 30) + 1)
-    assert "dh" in err("qpam_linear_logprobs_bwd", dh=None) and "dw_out" in err("qpam_linear_logprobs_bwd", dw_out=0)
+    assert "dh" in err("qpam_linear_logprobs_bwd", dh=None, dw=None) and "dw_out" in err("qpam_linear_logprobs_bwd", dw_out=0)
     assert "chunk" in err("qpam_linear_logprobs_bwd", chunk=0)
     assert "leading" in err("qpam_linear_logprobs_bwd", lddw=60)
 
@@ -211,6 +211,9 @@ def test_linear_token_logprobs_fake_kernels():
             dh, dw = linear_logprobs_bwd_op(h.view(12, 40), w.bfloat16(), f.long(), f, f, torch.empty(12, 2, device="cuda"),
                                             f, None, 1.0, 8, -100, fp32)
             assert dh.shape == (12, 40) and dw.shape == (70, 40)
+            dh1, dw0 = linear_logprobs_bwd_op(h.view(12, 40), w.bfloat16(), f.long(), f, f, torch.empty(12, 2, device="cuda"),
+                                              f, None, 1.0, 8, -100, fp32, True, False)
+            assert dh1.shape == (12, 40) and dw0.shape == (0,) and dw0.dtype == dw.dtype
             assert dh.dtype == torch.bfloat16 and dw.dtype == (torch.float32 if fp32 else torch.bfloat16)
 
 
