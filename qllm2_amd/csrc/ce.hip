@@ -158,6 +158,7 @@ struct FwdParams {
     float *red;              // [2] loss sum, denominator
     // token scores
     float *part_t;           // [N][n_vt] sum of 2^u u, in part_i's place
+    int full_vt;             // vocab tiles of 256 columns in front of the narrow ones (tiles::Columns)
     float c;                 // log2(e) / T
     float *logprobs, *entropy, *stats;
 };
@@ -1489,8 +1490,9 @@ using U16 = unsigned short;
 struct Stage {
     U16 a[TM * DK], b[TN * DK];
 };
-struct Frags {
-    bf16x8 a[4], b[4];  // the step's A fragments and the first half of its B fragments
+// The wave's share of a tile is 64 rows x 16 NI columns; NI = 8 is the whole tile.
+template <int NI> struct Frags {
+    bf16x8 a[4], b[NI / 2];  // the step's A fragments and the first half of its B fragments
 };
 // A wave's four loads of a stage (16 rows of 64 bytes each, two of A and two of B): a
 // uniform base that advances and 32-bit offsets that stay (row strides below 2^22).
@@ -1520,24 +1522,29 @@ __device__ __forceinline__ bf16x8 fragment(const U16 *at, int i) {
 
 // The products of a step: the second half of its B fragments is read in front of the
 // products of the first, the next step's first fragments (stage s) between those of the second.
-__device__ __forceinline__ void step(const Frags &cur, const Stage &c, Frags &next, const Stage &s, floatx4 (&acc)[4][8], int aat,
-                                     int bat) {
-    bf16x8 late[4];
+template <int NI>
+__device__ __forceinline__ void step(const Frags<NI> &cur, const Stage &c, Frags<NI> &next, const Stage &s,
+                                     floatx4 (&acc)[4][NI], int aat, int bat) {
+    constexpr int H = NI / 2;
+    bf16x8 late[H];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) late[i] = fragment(c.b + bat, 4 + i);
+    for (int i = 0; i < H; ++i) late[i] = fragment(c.b + bat, H + i);
 #pragma unroll
-    for (int ni = 0; ni < 4; ++ni)
+    for (int ni = 0; ni < H; ++ni)
 #pragma unroll
         for (int mi = 0; mi < 4; ++mi)
             acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur.a[mi], cur.b[ni], acc[mi][ni], 0, 0, 0);
 #pragma unroll
-    for (int ni = 0; ni < 4; ++ni) {
+    for (int ni = 0; ni < H; ++ni)
 #pragma unroll
         for (int mi = 0; mi < 4; ++mi)
-            acc[mi][4 + ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur.a[mi], late[ni], acc[mi][4 + ni], 0, 0, 0);
-        next.a[ni] = fragment(s.a + aat, ni);
-        next.b[ni] = fragment(s.b + bat, ni);
+            acc[mi][H + ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur.a[mi], late[ni], acc[mi][H + ni], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        next.a[i] = fragment(s.a + aat, i);
+        if (i < H) next.b[i < H ? i : 0] = fragment(s.b + bat, i);
     }
+    if constexpr (NI < 8) return;
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);   // LDS reads
     __builtin_amdgcn_sched_group_barrier(0x008, 16, 0);  // MFMAs
 #pragma unroll
@@ -1593,26 +1600,28 @@ __device__ __forceinline__ void start(const Stages &s, const Loads &q, int KT) {
 }
 
 // The product whose first stages start() has under way: acc[mi][ni] lane holds
-// C[64*(w>>1) + 16mi + 4g + r][128*(w&1) + 16ni + l16].  Step kt multiplies stage kt, reads
+// C[64*(w>>1) + 16mi + 4g + r][16*NI*(w&1) + 16ni + l16].  Step kt multiplies stage kt, reads
 // the first fragments of stage kt + 1 and starts the loads of stage kt + 3, four a wave
 // (past the end they re-read the last step): at its end "stage kt + 2 landed" is vmcnt
 // <= 4.  The stages are free and no load is in flight when it returns.
-__device__ __forceinline__ void product(const Stages &st, const Loads &q, int KT, floatx4 (&acc)[4][8]) {
+template <int NI>
+__device__ __forceinline__ void product(const Stages &st, const Loads &q, int KT, floatx4 (&acc)[4][NI]) {
     Stage &s0 = st.s0, &s1 = st.s1, &s2 = st.s2, &s3 = st.s3;
     const int tid = threadIdx.x, w = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int mi = 0; mi < 4; ++mi)
 #pragma unroll
-        for (int ni = 0; ni < 8; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
     // fragment (row, chunk g); the swizzle repeats every eight rows
-    const int aat = (64 * (w >> 1) + l16) * DK + 8 * wide::swz(l16, g), bat = (128 * (w & 1) + l16) * DK + 8 * wide::swz(l16, g);
+    const int aat = (64 * (w >> 1) + l16) * DK + 8 * wide::swz(l16, g);
+    const int bat = (16 * NI * (w & 1) + l16) * DK + 8 * wide::swz(l16, g);
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(4));
     __builtin_amdgcn_s_barrier();
-    Frags f0, f1;
+    Frags<NI> f0, f1;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         f0.a[i] = fragment(s0.a + aat, i);
-        f0.b[i] = fragment(s0.b + bat, i);
+        if (i < NI / 2) f0.b[i < NI / 2 ? i : 0] = fragment(s0.b + bat, i);
     }
 #define QPAM_STEP(KT_, CUR, STAGE, NEXT, NEXT_STAGE, FREE)                                     \
     load(FREE, q, min((KT_) + 3, KT - 1));                                                     \
@@ -1641,75 +1650,109 @@ __device__ __forceinline__ void block_lds_sync() {
     wave_lds_order();
 }
 
+// A tile's (b, s, t) per row: over each wave's columns from v0 on, then the two waves of a row.
+template <int NI>
+__device__ __forceinline__ void reduce_rows(const FwdParams &p, const floatx4 (&acc)[4][NI], int r0, int v0, int vt,
+                                            float (&sB)[2][TM], float (&sS)[2][TM], float (&sT)[2][TM]) {
+    const qpam_ce_fwd_args &a = p.a;
+    const int tid = threadIdx.x, w = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wm = w >> 1, wn = w & 1;
+    const int vl = v0 + 16 * NI * wn + l16;  // this lane's column in tile ni: vl + 16 ni
+    auto rows = [&](auto whole) {            // whole: no column past the vocabulary
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni)
+                    if (whole || vl + 16 * ni < a.V) mx = fmaxf(mx, acc[mi][ni][r]);
+                const float b = row16_max(mx) * p.c;
+                float s = 0.f, t = 0.f;
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni)
+                    if (whole || vl + 16 * ni < a.V) {
+                        const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
+                        s += e;
+                        t = __builtin_fmaf(e, u, t);
+                    }
+                s = row16_sum(s);
+                t = row16_sum(t);
+                if (l16 == 0) {
+                    const int row = 64 * wm + 16 * mi + 4 * g + r;
+                    sB[wn][row] = b;
+                    sS[wn][row] = s;
+                    sT[wn][row] = t;
+                }
+            }
+        }
+    };
+    if (v0 + 32 * NI <= a.V) rows(std::true_type{});
+    else rows(std::false_type{});
+    block_lds_sync();
+    if (tid < TM && r0 + tid < a.N) {
+        float b = sB[0][tid], s = sS[0][tid], t = sT[0][tid];
+        join_scores(b, s, t, sB[1][tid], sS[1][tid], sT[1][tid]);
+        const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
+        p.part_m[o] = b;
+        p.part_s[o] = s;
+        p.part_t[o] = t;
+    }
+}
+
+// The vocabulary's columns: `full` tiles of 256 that fill whole rounds of the 256 CUs, the
+// rest (what would be a last round with few blocks) in tiles of 32 NARROW columns, one a
+// block, if they fit one round.
+struct Columns {
+    int full, narrow, n_vt;  // narrow: 2 (64 columns) or 4 (128)
+};
+inline Columns columns(int N, int V) {
+    const int64_t n_rt = (N + TM - 1) / TM, n_ct = (V + TN - 1) / TN;
+    const int64_t full = n_rt * n_ct / 256 * 256 / n_rt, rest = V - full * TN;
+    if (rest > 0)
+        for (int ni = 2; ni <= 4; ni *= 2) {
+            const int64_t more = (rest + 32 * ni - 1) / (32 * ni);
+            if (n_rt * more <= 256) return {(int)full, ni, (int)(full + more)};
+        }
+    return {(int)n_ct, 2, (int)n_ct};
+}
+
+template <int NARROW>
 __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
     __shared__ __align__(16) Stage s0, s1, s2, s3;
     __shared__ float sB[2][TM], sS[2][TM], sT[2][TM];
     const qpam_ce_fwd_args &a = p.a;
     const Stages stages{s0, s1, s2, s3};
-    const int KT = a.D / DK;
-    const int tid = threadIdx.x, w = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
-    const int wm = w >> 1, wn = w & 1;
-    Walk at((a.N + TM - 1) / TM, p.n_vt);
-    if (!at.more()) return;
-    auto operands = [&]() {
-        const int r0 = at.rt * TM, v0 = at.vt * TN;
+    const int KT = a.D / DK, n_rt = (a.N + TM - 1) / TM;
+    Walk at(n_rt, p.full_vt);
+    const bool last = (int)blockIdx.x < n_rt * (p.n_vt - p.full_vt);
+    const int last_rt = blockIdx.x % n_rt, last_ct = blockIdx.x / n_rt;
+    const int last_v0 = p.full_vt * TN + 32 * NARROW * last_ct;
+    auto operands = [&](int rt, int v0, int cols) {
+        const int r0 = rt * TM;
         return loads((const U16 *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0), (const U16 *)a.w + (int64_t)v0 * a.ldw,
-                     a.ldw, min(TN, a.V - v0));
+                     a.ldw, min(cols, a.V - v0));
     };
-    Loads q = operands();
-    start(stages, q, KT);
-    for (;;) {
+    Loads q;
+    auto load_next = [&]() {
+        if (at.more()) q = operands(at.rt, at.vt * TN, TN);
+        else if (last) q = operands(last_rt, last_v0, 32 * NARROW);
+        else return;
+        start(stages, q, KT);
+    };
+    load_next();
+    while (at.more()) {
         floatx4 acc[4][8];
         product(stages, q, KT, acc);
-        const int r0 = at.rt * TM, v0 = at.vt * TN, vt = at.vt;
+        const int rt = at.rt, vt = at.vt;
         at.next();
-        if (at.more()) {
-            q = operands();
-            start(stages, q, KT);
-        }
-        const int vl = v0 + 128 * wn + l16;  // this lane's column in tile ni: vl + 16 ni
-        auto rows = [&](auto whole) {        // whole: no column past the vocabulary
-#pragma unroll
-            for (int mi = 0; mi < 4; ++mi) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int ni = 0; ni < 8; ++ni)
-                        if (whole || vl + 16 * ni < a.V) mx = fmaxf(mx, acc[mi][ni][r]);
-                    const float b = row16_max(mx) * p.c;
-                    float s = 0.f, t = 0.f;
-#pragma unroll
-                    for (int ni = 0; ni < 8; ++ni)
-                        if (whole || vl + 16 * ni < a.V) {
-                            const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
-                            s += e;
-                            t = __builtin_fmaf(e, u, t);
-                        }
-                    s = row16_sum(s);
-                    t = row16_sum(t);
-                    if (l16 == 0) {
-                        const int row = 64 * wm + 16 * mi + 4 * g + r;
-                        sB[wn][row] = b;
-                        sS[wn][row] = s;
-                        sT[wn][row] = t;
-                    }
-                }
-            }
-        };
-        if (v0 + TN <= a.V) rows(std::true_type{});
-        else rows(std::false_type{});
-        block_lds_sync();
-        if (tid < TM && r0 + tid < a.N) {
-            float b = sB[0][tid], s = sS[0][tid], t = sT[0][tid];
-            join_scores(b, s, t, sB[1][tid], sS[1][tid], sT[1][tid]);
-            const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
-            p.part_m[o] = b;
-            p.part_s[o] = s;
-            p.part_t[o] = t;
-        }
-        if (!at.more()) return;
+        load_next();
+        reduce_rows(p, acc, rt * TM, vt * TN, vt, sB, sS, sT);
     }
+    if (!last) return;
+    floatx4 acc[4][NARROW];
+    product(stages, q, KT, acc);
+    reduce_rows(p, acc, last_rt * TM, last_v0, p.full_vt + last_ct, sB, sS, sT);
 }
 
 // G^T [Vp][Rp] (and G [rows][Vp] with WRITE_G) without the tokens' one-hot terms; zero past
@@ -2054,7 +2097,10 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     p.a = a;
     const bool few = scores && a.N <= thin::ROWS;
     const bool wide_tiles = is_bf<T>() && (scores || use_wide(a.D));  // the direct-load loop takes any multiple of 32
-    p.n_vt = few ? thin::blocks(a.V) : wide_tiles ? (a.V + wide::TN - 1) / wide::TN : (a.V + vocab_tile<T>() - 1) / vocab_tile<T>();
+    const tiles::Columns cols = tiles::columns(a.N, a.V);
+    const bool score_tiles = scores && is_bf<T>() && !few;
+    p.full_vt = cols.full;
+    p.n_vt = few ? thin::blocks(a.V) : score_tiles ? cols.n_vt : wide_tiles ? (a.V + wide::TN - 1) / wide::TN : (a.V + vocab_tile<T>() - 1) / vocab_tile<T>();
     char *ws = (char *)a.workspace;
     const int64_t cnt = (int64_t)a.N * p.n_vt;
     p.part_m = (float *)ws;
@@ -2068,9 +2114,12 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     } else if (scores && !is_bf<T>()) {
         hipLaunchKernelGGL(split::scores_tile_kernel, dim3(p.n_vt, (a.N + split::TM - 1) / split::TM), dim3(split::TT), 0, stream, p);
         st = launch_status("split scores_tile_kernel");
-    } else if (scores) {
+    } else if (score_tiles) {
         const dim3 grid(tiles::grid(p.n_vt * ((a.N + tiles::TM - 1) / tiles::TM)));
-        hipLaunchKernelGGL(tiles::scores_tile_kernel, grid, dim3(tiles::TT), 0, stream, p);
+        if (cols.narrow == 2)
+            hipLaunchKernelGGL(tiles::scores_tile_kernel<2>, grid, dim3(tiles::TT), 0, stream, p);
+        else
+            hipLaunchKernelGGL(tiles::scores_tile_kernel<4>, grid, dim3(tiles::TT), 0, stream, p);
         st = launch_status("scores_tile_kernel");
     } else if (wide_tiles) {
         // the argmax (accuracy counts) only when requested
@@ -2483,6 +2532,7 @@ extern "C" size_t qpam_linear_logprobs_fwd_workspace_size(const qpam_linear_logp
     if (!a || a->N < 1 || a->V < 1) return 0;
     const qpam_ce_fwd_args f = fwd_args(*a);
     if (a->N <= thin::ROWS) return (size_t)a->N * thin::blocks(a->V) * 12 + 256;
+    if (a->dtype == QPAM_BF16) return (size_t)a->N * tiles::columns(a->N, a->V).n_vt * 12 + 256;
     return qpam_ce_fwd_workspace_size(&f);
 }
 

@@ -270,3 +270,14 @@ def test_one_operand_frozen_over_several_passes(gpu_lib, n, V, D, chunk, dtype, 
         r = linear_token_logprobs(*ops, ids.cuda(), temperature=0.8, chunk=chunk)
         got, = torch.autograd.grad([r.logprobs, r.entropy], [ops[i]], [g.cuda() for g in gs])
         assert torch.equal(got, want[i])
+
+
+@pytest.mark.parametrize("n,V,D", [(2047, 50261, 32), (4096, 50261, 96), (4100, 50261, 64), (300, 5000, 96), (300, 10000, 32)])
+def test_tiles_that_do_not_fill_their_last_round(gpu_lib, n, V, D):
+    """bf16 rows against vocabularies whose tiles leave a part of a round over, beside float64 on the GPU."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, _ = (x if isinstance(x, list) else x.cuda() for x in _data(n, V, D, BF16, BF16, 11))
+    r = linear_token_logprobs(h, w, ids, temperature=0.9)
+    want = _reference(h, w, ids, 0.9, None, 0.0)
+    _close(r.logprobs, want["lp"].cpu(), want["t_lp"].cpu())
+    _close(r.entropy, want["H"].cpu(), want["t_H"].cpu())
