@@ -16,10 +16,10 @@
 //
 // Top alternatives without a sort or a second pass: the row's entries fall into 64
 // groups (one per lane), the k-th largest of the groups' maxima bounds the k-th
-// largest entry from below, and only the entries of threads whose own maximum reaches
-// that bound, about k threads, are read again (from the cache, by the whole block) and
-// those at or above it listed.  The list, about k long, is ranked by counting.  Entries order by value, equal values
-// by the lower index, through one 64-bit key.
+// largest entry from below, and only the batches of 32 entries whose own maximum reaches
+// that bound, about k, are read again (by the whole block) and the entries at or above it
+// listed.  The list, about k long, is ranked by counting.  Entries order by value, equal
+// values by the lower index, through one 64-bit key.
 #include <algorithm>
 
 #include "common.h"
@@ -138,9 +138,14 @@ __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
     constexpr int E = Vec<T>::E, WAVES = THREADS / 64;
     constexpr int U = 32 / E;  // vectors of a batch: 32 entries, 64 or 128 bytes a thread in flight
     __shared__ float sM[WAVES], sS[WAVES], sT[WAVES];
+    // the maxima of a thread's batches, SLOTS of them (batch i in slot i % SLOTS); the
+    // listed candidates follow in the same memory
+    constexpr int SLOTS = CAP * 2 / THREADS;
     __shared__ uint64_t sKey[TOP ? WAVES * 64 : 1], sCand[TOP ? CAP : 1], sTop[TOP ? MAX_K : 1];
     __shared__ uint64_t sBound;
-    __shared__ int sCount, sOwners, sOwner[TOP ? THREADS : 1];
+    __shared__ int sCount, sOwners;
+    __shared__ unsigned short sOwner[TOP ? SLOTS * THREADS : 1];  // slot * THREADS + thread
+    float *sMax = reinterpret_cast<float *>(sCand);
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int64_t n = blockIdx.x;
     const Row<T> row(static_cast<const T *>(a.logits) + n * a.ld, a.V);
@@ -151,10 +156,11 @@ __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
 
     float m = -INFINITY, s = 0.f, t = 0.f;
     int batch_end = 0;  // the last entry of the batch that holds this thread's maximum
-    auto add = [&](const float *x, int cnt, int last) {
+    auto add = [&](const float *x, int cnt, int last, int slot) {
         float bm = x[0];
 #pragma unroll
         for (int i = 1; i < cnt; ++i) bm = fmaxf(bm, x[i]);
+        if (TOP && slot >= 0) sMax[slot * THREADS + tid] = fmaxf(sMax[slot * THREADS + tid], bm);
         if (bm > m) {
             const float g = fmaxf((m - bm) * c, FLOOR), f = __builtin_amdgcn_exp2f(g);
             t = f * (t + s * g);
@@ -170,7 +176,9 @@ __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
             t += e * fmaxf(u, FLOOR);
         }
     };
-    int v0 = row.lo + tid;
+    if constexpr (TOP)
+        for (int i = 0; i < SLOTS; ++i) sMax[i * THREADS + tid] = -INFINITY;
+    int v0 = row.lo + tid, slot = 0;
     for (; v0 + (U - 1) * THREADS < row.hi; v0 += U * THREADS) {
         uintx4 r[U];
         float x[U * E];
@@ -178,17 +186,18 @@ __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
         for (int i = 0; i < U; ++i) r[i] = row.load(v0 + i * THREADS);
 #pragma unroll
         for (int i = 0; i < U; ++i) Vec<T>::unpack(r[i], x + i * E);
-        add(x, U * E, row.first(v0 + (U - 1) * THREADS) + E - 1);
+        add(x, U * E, row.first(v0 + (U - 1) * THREADS) + E - 1, slot);
+        slot = (slot + 1) % SLOTS;
     }
     for (; v0 < row.hi; v0 += THREADS) {
         float x[E];
         Vec<T>::unpack(row.load(v0), x);
-        add(x, E, row.first(v0) + E - 1);
+        add(x, E, row.first(v0) + E - 1, slot);
     }
     const int edge = row.edge(tid);
     if (edge >= 0) {
         const float x = row.at(edge);
-        add(&x, 1, edge);
+        add(&x, 1, edge, -1);
     }
 
     // the block's maximum, s and t
@@ -252,20 +261,27 @@ __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
                     if (at < CAP) sCand[at] = key;
                 }
             };
-            if (m > -INFINITY && order(m) >= (uint32_t)(bound >> 32)) {
-                sOwner[atomicAdd(&sOwners, 1)] = tid;
-                if (edge >= 0) list(row.at(edge), edge);
-            }
+            const bool owner = m > -INFINITY && order(m) >= (uint32_t)(bound >> 32);
+            if (owner)
+                for (int i = 0; i < SLOTS; ++i) {
+                    const float x = sMax[i * THREADS + tid];
+                    if (x > -INFINITY && order(x) >= (uint32_t)(bound >> 32))
+                        sOwner[atomicAdd(&sOwners, 1)] = (unsigned short)(i * THREADS + tid);
+                }
             __syncthreads();
-            // (owner, its j-th vector) over the block's threads
-            const int per = (row.hi - row.lo + THREADS - 1) / THREADS, total = sOwners * per;
+            if (owner && edge >= 0) list(row.at(edge), edge);
+            // (owner's slot, its j-th vector) over the block's threads
+            const int batches = (row.hi - row.lo + U * THREADS - 1) / (U * THREADS);
+            const int per = (batches + SLOTS - 1) / SLOTS * U, total = sOwners * per;
             for (int i = tid; i < total; i += THREADS) {
-                const int o = i / per, v = row.lo + sOwner[o] + (i - o * per) * THREADS;
+                const int o = i / per, j = i - o * per, code = sOwner[o];
+                const int vec = (j / U * SLOTS + code / THREADS) * U + j % U;
+                const int64_t v = row.lo + code % THREADS + (int64_t)vec * THREADS;
                 if (v >= row.hi) continue;
                 float x[E];
-                Vec<T>::unpack(row.load(v), x);
+                Vec<T>::unpack(row.load((int)v), x);
 #pragma unroll
-                for (int j = 0; j < E; ++j) list(x[j], row.first(v) + j);
+                for (int e = 0; e < E; ++e) list(x[e], row.first((int)v) + e);
             }
             __syncthreads();
             count = sCount;

@@ -358,3 +358,25 @@ def test_more_rows_than_one_launch_holds(gpu_lib):
         assert torch.equal(a[rows], b)
     assert torch.equal(x.grad[rows], y.grad)
     assert (r.logprobs.detach() < 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V,k", [(3, 200001, 64), (300, 200001, 64), (260, 131072, 7), (5, 65536 + 13, 33), (700, 3, 2)])
+def test_alternatives_of_long_rows(gpu_lib, n, V, k, dtype):
+    """Vocabularies of many batches a thread: the order of a stable sort, and its log softmax."""
+    from qllm2_amd.token_logprobs import token_logprobs
+    g = torch.Generator(device="cuda").manual_seed(V + n)
+    x = (torch.randn(n, V, device="cuda", generator=g) * 3).to(dtype)
+    x[1::3, V // 2:] = float("-inf")
+    x[2::3] = x[2::3].sort(-1).values  # the largest entries side by side at the end
+    ids = torch.randint(0, V, (n,), device="cuda", generator=g)
+    r = token_logprobs(x, ids, top_k=k)
+    _, order = torch.sort(x, dim=-1, descending=True, stable=True)
+    assert torch.equal(r.top_ids, order[:, :k])
+    # a log probability of at most 40 (or -inf): V additions in 1024 or 256 chains and their joining, the
+    # maximum's rescalings and two roundings of the result, below (V / 256 + 100) 2^-24 of s in all
+    want = torch.log_softmax(x.double(), -1).gather(1, order[:, :k])
+    assert torch.equal(r.top_logprobs.isinf(), want.isinf())
+    live = ~want.isinf()
+    err = (r.top_logprobs.double() - want)[live].abs().max().item()
+    assert err <= (V / 256 + 100) * 2.0 ** -24 + 40 * 2.0 ** -22
