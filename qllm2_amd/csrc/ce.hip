@@ -536,6 +536,9 @@ __global__ void __launch_bounds__(THREADS) ce_gemm_kernel(const T *A, int64_t ld
 // v_mfma_f32_16x16x4_f32.  Values are split on their way from registers to LDS, once a
 // block, in the shadow of the MFMAs: 8 waves, two LDS buffers of three planes (72 KiB
 // each) of 16-byte chunks, swizzled like the bf16 tiles; the loads run two steps ahead.
+// 1000 x 8191 x 768 (12.6 GFLOP, one tile a CU): scores 65 us, G 72, dH and dW 71 to 79;
+// the MFMAs run 48 % of the time, the rest is the first loads, the step's barrier and the
+// epilogue.  The fp32 MFMAs took 172 us, parts made in front of the products 80.
 // Rows past the end of an operand re-read its last row.  Infinite operands give NaN.
 namespace split {
 constexpr int TM = 256, TN = 128, TT = 512;
@@ -1482,7 +1485,9 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
 
 // Token scores' bf16 tiles, 256 x 256: loads, swizzle and wave layout as in `wide`, with a
 // k-step's first fragments read from LDS between the MFMAs of the step before, so that no
-// wave waits for LDS at the head of a step.
+// wave waits for LDS at the head of a step.  16384 x 50261 x 1024: scores 1.48 ms (1.14
+// PFLOP/s, the MFMA pipes 57 % busy at the 1.9 GHz that the card holds under this load, LDS
+// 23 %), G^T 1.80 ms with 1.65 GB of stores; two blocks of 128 x 256 a CU took 1.85 and 2.11.
 namespace tiles {
 constexpr int TM = wide::TM, TN = wide::TN, DK = wide::DK, TT = wide::WTHREADS;
 using U16 = unsigned short;
@@ -1786,9 +1791,10 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
     U16 *G = (U16 *)p.gbuf;
     U16 *GT = (U16 *)p.gtbuf;
     U16 *slab = sSlab + w * 16 * LD;
-    // a slab's way out: vocab row lane / 4, 16 tile rows lane % 4, 32 bytes a lane
-    const U16 *from = slab + (lane >> 2) * LD + 16 * (lane & 3);
-    const unsigned to = 2u * ((lane >> 2) * (unsigned)p.Rp + 16 * (lane & 3));
+    // a slab's way out in two stores of eight whole 128-byte lines: vocab rows lane / 8 and
+    // lane / 8 + 8, 16 bytes a lane
+    const U16 *from = slab + (lane >> 3) * LD + 8 * (lane & 7);
+    const unsigned to = 2u * ((lane >> 3) * (unsigned)p.Rp + 8 * (lane & 7));
     keep_rows(row_score(p, at.rt * TM + (tid & (TM - 1))), 0);
     Loads q = operands();
     start(stages, q, KT);
@@ -1831,12 +1837,12 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
                     }
                     *reinterpret_cast<uint2 *>(slab + l16 * LD + 16 * mi + 4 * g) = make_uint2(lo, hi);
                 }
-                wide::wave_lds_sync();  // the slab is this wave's own
-                const uint4 d0 = reinterpret_cast<const uint4 *>(from)[0], d1 = reinterpret_cast<const uint4 *>(from)[1];
+                wave_lds_order();  // the slab is this wave's own, and a wave's LDS accesses stay in order
+                const uint4 d0 = *reinterpret_cast<const uint4 *>(from), d1 = *reinterpret_cast<const uint4 *>(from + 8 * LD);
                 char *out = reinterpret_cast<char *>(GT + (int64_t)vb * p.Rp + lr0 + 64 * wm);
                 *reinterpret_cast<uint4 *>(out + to) = d0;
-                *reinterpret_cast<uint4 *>(out + to + 16) = d1;
-                wide::wave_lds_sync();
+                *reinterpret_cast<uint4 *>(out + 16ll * p.Rp + to) = d1;
+                wave_lds_order();
             }
         };
         if (v0 + TN <= a.V && lr0 + TM <= p.rows) slabs(std::true_type{});

@@ -35,8 +35,10 @@ __device__ __forceinline__ int64_t load_id(const void *ids, int is64, int64_t i)
 }
 
 // ---------------------------------------------------------------- lookup ---
-// W complex values of one table row per lane and step: 2 W elements leave as one
-// or two 16-byte stores.
+// W complex values of one table row per lane and step: 16 bytes of each table in, two
+// 16-byte stores out.  Lanes to a row: the least power of two that covers it, at most a
+// wave, so that short rows share waves.  Bound by the launch (192 rows of 768 fp32: 3.3
+// us) or by HBM (16384 rows of 512 bf16, 33 MB written and as much read: 12.9 us).
 template <typename T, int W>
 __global__ void __launch_bounds__(THREADS) lookup_kernel(qpam_embed_args a, int lanes_log2) {
     typedef T VecT __attribute__((ext_vector_type(W)));
@@ -120,6 +122,9 @@ __device__ __forceinline__ void zero_tables(const SortParams &p) {
 // Up to SMALL ids sorted by one block: the list lives in LDS between the passes,
 // each wave ranks a contiguous part of it (stable: rounds of 64 in order, lanes of
 // a round in order), and the counts of [wave][digit] give every wave its places.
+// One launch instead of the six of the longer lists' two passes, and the other blocks
+// zero the tables beside it: 27 us for 16384 ids and 103 MB (the sort's own time; the
+// fill alone takes 15), 37 us for 3001 ids and 197 MB (the fill's).
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
 constexpr int ROUNDS = 16, SMALL = SORT_THREADS * ROUNDS;
 constexpr size_t SORT_SMEM = SMALL * 6 + SORT_WAVES * RADIX * 4;
@@ -331,7 +336,10 @@ __device__ __forceinline__ void write_row(const GradParams &p, uint32_t key, int
     *reinterpret_cast<VecT *>(static_cast<T *>(p.a.d_im) + o) = *reinterpret_cast<const VecT *>(m);
 }
 
-// One wave: a chunk's entries over 64 W complex columns.
+// One wave: a chunk's entries over 64 W complex columns, 8 bytes of a table's row a lane.
+// Bound by the latency of its gathered rows, so all CH are in flight at once; a longer
+// chunk has fewer waves, a shorter one more partial sums.  16384 rows of 512 bf16 (33 MB
+// read): 12.0 us, and 4.3 us for the runs that cross chunks.
 template <typename T, int W>
 __global__ void __launch_bounds__(THREADS) grad_chunk_kernel(GradParams p) {
     typedef T VecT __attribute__((ext_vector_type(2 * W)));

@@ -133,6 +133,10 @@ __device__ __forceinline__ void top_by_passes(const Row<T> &row, int k, uint64_t
     __syncthreads();
 }
 
+// Bound by HBM and, in bf16, nearly as much by the VALU (an exp, a maximum and five more
+// operations an entry: 50 us of the 75).  4000 rows of 50261 bf16 (402 MB): 75 us without
+// alternatives (5.3 TB/s), 82 with five, 86 with 32; 2048 rows fp32 (412 MB): 72 us.  One
+// row of 50261 fp32 with five alternatives: 10.5 us, the block's own latency.
 template <typename T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
     constexpr int E = Vec<T>::E, WAVES = THREADS / 64;
@@ -329,6 +333,7 @@ __device__ __forceinline__ void put(unsigned short *p, float x) { *p = __builtin
 // A block writes a stretch of one row's gradient without the terms of the given and
 // top tokens, then overwrites those entries that fall into its stretch.  VECTORS: the
 // row of logits and the row of the gradient start at the same offset from 16 bytes.
+// Bound by HBM: 2048 rows of 50261 fp32, 412 MB read and as much written, 141 us (5.8 TB/s).
 template <typename T, bool VECTORS>
 __global__ void __launch_bounds__(GT) grad_kernel(Args a, int segs) {
     constexpr int E = Vec<T>::E;
