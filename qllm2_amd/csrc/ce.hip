@@ -542,7 +542,9 @@ __global__ void __launch_bounds__(THREADS) ce_gemm_kernel(const T *A, int64_t ld
 // Rows past the end of an operand re-read its last row.  Infinite operands give NaN.
 namespace split {
 constexpr int TM = 256, TN = 128, TT = 512;
-constexpr int PLANE = (TM + TN) * BK;  // bf16 elements of a plane: A's rows, then B's
+constexpr int PT = TN + 16;  // pitch of a [32][128] tile of B
+// bf16 elements of a plane: A's rows, then B's (BT: B's tile as it stands in memory)
+template <bool BT> constexpr int plane() { return TM * BK + (BT ? BK * PT : TN * BK); }
 using U16 = unsigned short;
 
 struct Raw {
@@ -550,13 +552,16 @@ struct Raw {
 };
 
 __device__ __forceinline__ int swz(int row, int c) { return c ^ ((row >> 1) & 3); }
+// place of a row of a [32][PT] tile: bits 2 and 3 swapped, so that the 32-byte pieces that
+// half a wave reads (rows 0 .. 3 and 8 .. 11, or four or sixteen behind them) share no bank
+__device__ __forceinline__ int place(int row) { return (row & 19) | (row & 4) << 1 | (row & 8) >> 1; }
 
-__device__ __forceinline__ void store(uint4 raw, U16 *lds) {
+template <bool BT> __device__ __forceinline__ void store(uint4 raw, U16 *lds) {
     float v[4] = {__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w)};
 #pragma unroll
     for (int part = 0; part < 3; ++part) {
         const uint2 q = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-        *reinterpret_cast<uint2 *>(lds + part * PLANE) = q;
+        *reinterpret_cast<uint2 *>(lds + part * plane<BT>()) = q;
         v[0] -= __uint_as_float(q.x << 16);
         v[1] -= __uint_as_float(q.x & 0xFFFF0000u);
         v[2] -= __uint_as_float(q.y << 16);
@@ -566,9 +571,13 @@ __device__ __forceinline__ void store(uint4 raw, U16 *lds) {
 
 // acc[mi][ni] lane holds C[64*(w>>1) + 16mi + 4g + r][64*(w&1) + 16ni + l16]; K % 32 == 0.
 // Row strides below 2^22 (32-bit byte offsets in a tile).
-__device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, const float *B, int64_t ldb, int b_rows, int K,
-                                     floatx4 (&acc)[4][4], U16 *s0, U16 *s1) {
-    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+// BT: B is [K][N] as it stands in memory, b_rows of its K rows there (past them A is zero)
+// and b_cols columns (a multiple of four).  Its tile stays [32][128] in LDS, and the
+// fragments come out by transpose reads.
+template <bool BT>
+__device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, const float *B, int64_t ldb, int b_rows, int b_cols,
+                                     int K, floatx4 (&acc)[4][4], U16 *s0, U16 *s1) {
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int arow0 = 64 * (w >> 1), brow0 = TM + 64 * (w & 1);
 #pragma unroll
     for (int mi = 0; mi < 4; ++mi)
@@ -582,19 +591,34 @@ __device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, co
 #pragma unroll
     for (int i = 0; i < 2; ++i) bo[i] = 4u * ((unsigned)min(r8 + 64 * i, b_rows - 1) * (unsigned)ldb + 4 * c8);
     const int to = r8 * BK + 8 * swz(r8, c8 >> 1) + 4 * (c8 & 1);  // the swizzle repeats every eight rows
+    // BT: thread -> B's row tid / 16, columns 4 (tid % 16) + 64 i
+    const int r16 = tid >> 4, c16 = tid & 15, bt_to = TM * BK + place(r16) * PT + 4 * c16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (BT) bo[i] = 4u * min(64 * i + 4 * c16, b_cols - 4);
     auto gload = [&](Raw &x, int step) {
         const char *a = reinterpret_cast<const char *>(A + (int64_t)step * BK);
-        const char *b = reinterpret_cast<const char *>(B + (int64_t)step * BK);
+        const int row0 = BT ? min(step * BK, b_rows - 1) : 0;
+        const char *b = reinterpret_cast<const char *>(BT ? B + row0 * ldb : B + (int64_t)step * BK);
+        const unsigned row = BT ? 4u * (unsigned)min(r16, b_rows - 1 - row0) * (unsigned)ldb : 0u;
 #pragma unroll
         for (int i = 0; i < 4; ++i) x.a[i] = *reinterpret_cast<const uint4 *>(a + ao[i]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) x.b[i] = *reinterpret_cast<const uint4 *>(b + bo[i]);
+        for (int i = 0; i < 2; ++i) x.b[i] = *reinterpret_cast<const uint4 *>(b + (row + bo[i]));
     };
     auto put = [&](const Raw &x, U16 *s, int i) {  // the i-th of the six pieces
-        store(i < 4 ? x.a[i < 4 ? i : 0] : x.b[i < 4 ? 0 : i - 4], s + to + 64 * (i < 4 ? i : TM / 64 + i - 4) * BK);
+        if (BT && i >= 4) store<BT>(x.b[i < 4 ? 0 : i - 4], s + bt_to + 64 * (i - 4));
+        else store<BT>(i < 4 ? x.a[i < 4 ? i : 0] : x.b[i < 4 ? 0 : i - 4], s + to + 64 * (i < 4 ? i : TM / 64 + i - 4) * BK);
+    };
+    // BT: the lane's column l16 of a 16-column chunk, k = 8 g ..: rows 8 g + l16 / 4 and four behind it
+    const int bt_at = TM * BK + place(8 * g + (l16 >> 2)) * PT + 64 * (w & 1) + 4 * (l16 & 3);
+    auto fragment_t = [&](const U16 *s, int ni, int part) {
+        const U16 *at = s + part * plane<BT>() + bt_at + 16 * ni;
+        const shortx4 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * PT);
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     auto fragment = [&](const U16 *s, int row, int part) {
-        return *reinterpret_cast<const bf16x8 *>(s + part * PLANE + (row + l16) * BK + 8 * swz(l16, g));
+        return *reinterpret_cast<const bf16x8 *>(s + part * plane<BT>() + (row + l16) * BK + 8 * swz(l16, g));
     };
     // the products of the step in `cur`; the next step's values go from x to `next`
     auto step = [&](const U16 *cur, U16 *next, const Raw &x) {
@@ -607,7 +631,8 @@ __device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, co
         for (int ni = 0; ni < 4; ++ni) {
             bf16x8 b[3];
 #pragma unroll
-            for (int part = 0; part < 3; ++part) b[part] = fragment(cur, brow0 + 16 * ni, part);
+            for (int part = 0; part < 3; ++part)
+                b[part] = BT ? fragment_t(cur, ni, part) : fragment(cur, brow0 + 16 * ni, part);
             constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};  // small products first
 #pragma unroll
             for (int j = 0; j < 6; ++j)
@@ -639,13 +664,13 @@ __device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, co
 }
 
 __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
-    __shared__ __align__(16) U16 s0[3 * PLANE], s1[3 * PLANE];
+    __shared__ __align__(16) U16 s0[3 * plane<false>()], s1[3 * plane<false>()];
     __shared__ float sB[2][TM], sS[2][TM], sT[2][TM];
     const qpam_ce_fwd_args &a = p.a;
     const int vt = blockIdx.x, r0 = blockIdx.y * TM, v0 = vt * TN;
     floatx4 acc[4][4];
-    tile((const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0), (const float *)a.w + (int64_t)v0 * a.ldw, a.ldw,
-         min(TN, a.V - v0), a.D, acc, s0, s1);
+    tile<false>((const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0), (const float *)a.w + (int64_t)v0 * a.ldw,
+                a.ldw, min(TN, a.V - v0), 0, a.D, acc, s0, s1);
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1, vl = v0 + 64 * wn + l16;
 #pragma unroll
@@ -688,7 +713,7 @@ __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
 // G [rows][Vp] and G^T [Vp][Rp] (each if there is a buffer for it) without the tokens'
 // one-hot terms; zero past the vocabulary and past the rows (Rp: a multiple of 256)
 __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
-    __shared__ __align__(16) U16 s0[3 * PLANE], s1[3 * PLANE];
+    __shared__ __align__(16) U16 s0[3 * plane<false>()], s1[3 * plane<false>()];
     __shared__ __align__(16) float sRow[3][TM];
     const qpam_ce_bwd_args &a = p.a;
     const int lr0 = blockIdx.y * TM, v0 = blockIdx.x * TN, tid = threadIdx.x;
@@ -699,8 +724,8 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
         sRow[2][tid] = q.slope;
     }
     floatx4 acc[4][4];
-    tile((const float *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(TM, p.rows - lr0),
-         (const float *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(TN, a.V - v0), a.D, acc, s0, s1);
+    tile<false>((const float *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(TM, p.rows - lr0),
+                (const float *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(TN, a.V - v0), 0, a.D, acc, s0, s1);
     const int w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
     float *G = (float *)p.gbuf, *GT = (float *)p.gtbuf;
@@ -726,15 +751,17 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
     }
 }
 
-// C = A B^T (dH and dW), the K axis in gridDim.z ranges of kper: one range writes C (or
-// adds to it), several write C + z split_stride, summed by sum_kernel in their order.
-__global__ void __launch_bounds__(TT) gemm_kernel(const float *A, int64_t lda, int M, const float *B, int64_t ldb, int N, int K,
-                                                  int kper, float *C, int64_t ldc, int64_t split_stride, int accumulate) {
-    __shared__ __align__(16) U16 s0[3 * PLANE], s1[3 * PLANE];
+// C = A B (dH and dW), A [M][K], B [b_rows][N] with b_rows <= K and zeros in A past them, the
+// K axis in gridDim.z ranges of kper: one range writes C (or adds to it), several write
+// C + z split_stride, summed by sum_kernel in their order.
+__global__ void __launch_bounds__(TT) gemm_kernel(const float *A, int64_t lda, int M, const float *B, int64_t ldb, int b_rows,
+                                                  int N, int K, int kper, float *C, int64_t ldc, int64_t split_stride, int accumulate) {
+    __shared__ __align__(16) U16 s0[3 * plane<true>()], s1[3 * plane<true>()];
     const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN, k0 = blockIdx.z * kper;
     floatx4 acc[4][4];
-    tile(A + (int64_t)m0 * lda + k0, lda, min(TM, M - m0), B + (int64_t)n0 * ldb + k0, ldb, min(TN, N - n0), min(kper, K - k0),
-         acc, s0, s1);
+    const int kb = min(k0, b_rows - 1);  // a range past B's rows: A is zero there
+    tile<true>(A + (int64_t)m0 * lda + k0, lda, min(TM, M - m0), B + (int64_t)kb * ldb + n0, ldb, b_rows - kb, min(TN, N - n0),
+               min(kper, K - k0), acc, s0, s1);
     C += blockIdx.z * split_stride;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
@@ -2355,12 +2382,12 @@ int dh_splits(int rows, int D, int Vp) {
     return std::max(1, std::min({256 / std::max(tiles, 1), Vp / 512, 16}));
 }
 
-// W^T, G, G^T and H^T as the loss's fp32 passes have them, the rows padded to 256, and
-// dH's partial sums: splits * rows <= 16 rows, and <= 256 TM as splits * tiles <= 256
+// G, G^T (the rows padded to 256) and dH's partial sums: splits * rows <= 16 rows, and <=
+// 256 TM as splits * tiles <= 256
 size_t scores_f32_ws(const qpam_ce_bwd_args &a) {
     const int64_t Vp = round_up(a.V, split::TN), chunk = pass_rows(a), Rp = round_up((int)chunk, split::TM);
     const int64_t part = std::min<int64_t>(16 * chunk, 256ll * split::TM) * a.D;
-    return (size_t)((int64_t)a.D * Vp + chunk * Vp + Vp * Rp + (int64_t)a.D * Rp + part) * sizeof(float) + 256;
+    return (size_t)(chunk * Vp + Vp * Rp + part) * sizeof(float) + 256;
 }
 
 // Token scores in fp32: G tiles, then dH and dW (those that are asked for), all in bf16
@@ -2371,41 +2398,30 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
     p.write_g = a.dh != nullptr;
     p.Vp = round_up(a.V, split::TN);
     const int chunk = pass_rows(a);
-    float *wt = (float *)a.workspace, *gb = wt + (int64_t)a.D * p.Vp, *gt = gb + (int64_t)chunk * p.Vp;
-    float *ht = gt + (int64_t)p.Vp * round_up(chunk, split::TM), *part = ht + (int64_t)a.D * round_up(chunk, split::TM);
+    float *gb = (float *)a.workspace, *gt = gb + (int64_t)chunk * p.Vp, *part = gt + (int64_t)p.Vp * round_up(chunk, split::TM);
     p.gbuf = a.dh ? gb : nullptr;
     p.gtbuf = a.dw ? gt : nullptr;
-    auto gemm = [&](const char *what, const float *A, int64_t lda, int M, const float *B, int64_t ldb, int K, int kper, float *C,
-                    int64_t ldc, int64_t stride, int accumulate) {
+    auto gemm = [&](const char *what, const float *A, int64_t lda, int M, const float *B, int64_t ldb, int b_rows, int K, int kper,
+                    float *C, int64_t ldc, int64_t stride, int accumulate) {
         hipLaunchKernelGGL(split::gemm_kernel,
                            dim3((a.D + split::TN - 1) / split::TN, (M + split::TM - 1) / split::TM, (K + kper - 1) / kper),
-                           dim3(split::TT), 0, stream, A, lda, M, B, ldb, a.D, K, kper, C, ldc, stride, accumulate);
+                           dim3(split::TT), 0, stream, A, lda, M, B, ldb, b_rows, a.D, K, kper, C, ldc, stride, accumulate);
         return launch_status(what);
     };
     int st = QPAM_OK;
-    if (a.dh) {
-        hipLaunchKernelGGL(transpose_kernel<float>, dim3((a.D + 63) / 64, (p.Vp + 63) / 64), dim3(THREADS), 0, stream,
-                           (const float *)a.w, a.ldw, a.V, a.D, wt, (int64_t)p.Vp, a.D, p.Vp);
-        if ((st = launch_status("transpose_kernel(W)"))) return st;
-    }
     for (int r0 = 0; r0 < a.N; r0 += chunk) {
         p.row0 = r0;
         p.rows = std::min(chunk, a.N - r0);
         p.Rp = round_up(p.rows, split::TM);
-        if (a.dw) {
-            hipLaunchKernelGGL(transpose_kernel<float>, dim3((a.D + 63) / 64, (p.Rp + 63) / 64), dim3(THREADS), 0, stream,
-                               (const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, p.rows, a.D, ht, (int64_t)p.Rp, a.D, p.Rp);
-            if ((st = launch_status("transpose_kernel(H)"))) return st;
-        }
         hipLaunchKernelGGL(split::scores_grad_kernel, dim3(p.Vp / split::TN, p.Rp / split::TM), dim3(split::TT), 0, stream, p);
         if ((st = launch_status("split scores_grad_kernel"))) return st;
         hipLaunchKernelGGL(scores_token_kernel<float>, dim3((p.rows + THREADS - 1) / THREADS), dim3(THREADS), 0, stream, p);
         if ((st = launch_status("scores_token_kernel"))) return st;
-        // dH[r0 .. r0 + rows] = G [rows][Vp] (W^T [D][Vp])^T
+        // dH[r0 .. r0 + rows] = G [rows][Vp] W
         const int splits = dh_splits(p.rows, a.D, p.Vp), kper = round_up((p.Vp + splits - 1) / splits, BK);
         float *dh = (float *)a.dh + (int64_t)r0 * a.lddh;
         if (a.dh) {
-            st = gemm("split gemm_kernel(dH)", gb, p.Vp, p.rows, wt, p.Vp, p.Vp, kper, splits > 1 ? part : dh,
+            st = gemm("split gemm_kernel(dH)", gb, p.Vp, p.rows, (const float *)a.w, a.ldw, a.V, p.Vp, kper, splits > 1 ? part : dh,
                       splits > 1 ? a.D : a.lddh, (int64_t)p.rows * a.D, 0);
             if (st) return st;
         }
@@ -2417,8 +2433,8 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
             if ((st = launch_status("split sum_kernel"))) return st;
         }
         if (!a.dw) continue;
-        // dW [V][D] (+)= G^T [Vp][Rp] (H^T [D][Rp])^T
-        st = gemm("split gemm_kernel(dW)", gt, p.Rp, a.V, ht, p.Rp, p.Rp, p.Rp, (float *)a.dw, a.lddw, 0, r0 > 0 ? 1 : 0);
+        // dW [V][D] (+)= G^T [Vp][Rp] H
+        st = gemm("split gemm_kernel(dW)", gt, p.Rp, a.V, (const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, p.rows, p.Rp, p.Rp, (float *)a.dw, a.lddw, 0, r0 > 0 ? 1 : 0);
         if (st) return st;
     }
     return QPAM_OK;

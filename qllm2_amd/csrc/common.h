@@ -111,6 +111,15 @@ __device__ __forceinline__ void wave_lds_order() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// gfx950 LDS transpose read (ds_read_b64_tr_b16).  Within each group of 16
+// lanes, lane 4a+b receives element b of the 8-byte chunks addressed by lanes
+// 4e+a (e = 0..3), so 16 lanes addressing a 4 x 16 block of a row-major bf16
+// tile receive its columns.
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ shortx4 lds_read_tr(const unsigned short *p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)p);
+}
+
 // DPP lane permutations (quad_perm [1,0,3,2], [2,3,0,1], row_half_mirror,
 // row_mirror) and reductions over the 16 lanes of a DPP row: every lane of the
 // row ends with the result.  Four steps: pairs, quads, halves, rows.

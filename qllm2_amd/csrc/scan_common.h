@@ -231,15 +231,6 @@ __device__ __forceinline__ ushortx4 to_bf16x4(float4 v) {
     return ushortx4{f32_to_bf16(v.x), f32_to_bf16(v.y), f32_to_bf16(v.z), f32_to_bf16(v.w)};
 }
 
-// gfx950 LDS transpose read (ds_read_b64_tr_b16).  Within each group of 16
-// lanes, lane 4a+b receives element b of the 8-byte chunks addressed by lanes
-// 4e+a (e = 0..3), so 16 lanes addressing a 4 x 16 block of a row-major bf16
-// tile receive its columns.
-typedef short shortx4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ shortx4 lds_read_tr(const unsigned short *p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)p);
-}
-
 // MFMA operand fragment (8 k values per lane) of a natural row-major [k][n]
 // bf16 LDS tile (pitch PB) for a contraction over its rows: lane l16 of each
 // 16-lane group receives rows r0..r0+3 then r1..r1+3 of column col0 + l16.  The
