@@ -885,7 +885,7 @@ int qpam_logprobs_bwd(const qpam_logprobs_args *a, void *stream);
  * between the tiles and the two products dh = dx w, dw = dx^T h.  fp32
  * operands: each value as the sum of three bf16 parts, products to about 2^-24.  D a
  * multiple of 32; h and w as qpam_ce_fwd takes them, with row strides below 2^22.  V at
- * most 2^30 (backward in fp32: V and chunk below 2^22 - 256).  Temperature 1e-30 to 1e30.
+ * most 2^30 (backward in fp32: V, and 2 chunk or N, below 2^22 - 256).  Temperature 1e-30 to 1e30.
  * chunk bounds the backward's memory as qpam_ce_bwd's does; dw_out 1: dw in dtype, 2: dw
  * in fp32.  dh or dw may be NULL: its product is left out; the other is written. */
 typedef struct {

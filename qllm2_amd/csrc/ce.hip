@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(THREADS) scores_token_kernel(BwdParams p) {
     T v;
     if constexpr (sizeof(T) == 2) v = __builtin_bit_cast(unsigned short, (__bf16)x);
     else v = x;
-    if (p.gtbuf) static_cast<T *>(p.gtbuf)[id * p.Rp + lr] = v;
+    static_cast<T *>(p.gtbuf)[id * p.Rp + lr] = v;
     if (p.write_g) static_cast<T *>(p.gbuf)[(int64_t)lr * p.Vp + id] = v;
 }
 
@@ -536,15 +536,17 @@ __global__ void __launch_bounds__(THREADS) ce_gemm_kernel(const T *A, int64_t ld
 // v_mfma_f32_16x16x4_f32.  Values are split on their way from registers to LDS, once a
 // block, in the shadow of the MFMAs: 8 waves, two LDS buffers of three planes (72 KiB
 // each) of 16-byte chunks, swizzled like the bf16 tiles; the loads run two steps ahead.
-// 1000 x 8191 x 768 (12.6 GFLOP, one tile a CU): scores 65 us, G 72, dH and dW 71 to 79;
+// 1000 x 8191 x 768 (12.6 GFLOP, one tile a CU): scores 65 us, G^T 68, dH 73, dW 81 (192
+// blocks); with W, H and G^T transposed in memory for dH and dW 27 us more in all;
 // the MFMAs run 48 % of the time, the rest is the first loads, the step's barrier and the
 // epilogue.  The fp32 MFMAs took 172 us, parts made in front of the products 80.
 // Rows past the end of an operand re-read its last row.  Infinite operands give NaN.
 namespace split {
 constexpr int TM = 256, TN = 128, TT = 512;
-constexpr int PT = TN + 16;  // pitch of a [32][128] tile of B
-// bf16 elements of a plane: A's rows, then B's (BT: B's tile as it stands in memory)
-template <bool BT> constexpr int plane() { return TM * BK + (BT ? BK * PT : TN * BK); }
+constexpr int PA = TM + 16, PB = TN + 16;  // pitches of tiles [32][256] of A, [32][128] of B
+// bf16 elements of a plane: A's tile, then B's (AT, BT: as they stand in memory, [K][M], [K][N])
+template <bool AT> constexpr int a_tile() { return AT ? BK * PA : TM * BK; }
+template <bool AT, bool BT> constexpr int plane() { return a_tile<AT>() + (BT ? BK * PB : TN * BK); }
 using U16 = unsigned short;
 
 struct Raw {
@@ -552,16 +554,16 @@ struct Raw {
 };
 
 __device__ __forceinline__ int swz(int row, int c) { return c ^ ((row >> 1) & 3); }
-// place of a row of a [32][PT] tile: bits 2 and 3 swapped, so that the 32-byte pieces that
+// place of a row of a [32][..] tile: bits 2 and 3 swapped, so that the 32-byte pieces that
 // half a wave reads (rows 0 .. 3 and 8 .. 11, or four or sixteen behind them) share no bank
 __device__ __forceinline__ int place(int row) { return (row & 19) | (row & 4) << 1 | (row & 8) >> 1; }
 
-template <bool BT> __device__ __forceinline__ void store(uint4 raw, U16 *lds) {
+template <int PLANE> __device__ __forceinline__ void store(uint4 raw, U16 *lds) {
     float v[4] = {__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w)};
 #pragma unroll
     for (int part = 0; part < 3; ++part) {
         const uint2 q = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-        *reinterpret_cast<uint2 *>(lds + part * plane<BT>()) = q;
+        *reinterpret_cast<uint2 *>(lds + part * PLANE) = q;
         v[0] -= __uint_as_float(q.x << 16);
         v[1] -= __uint_as_float(q.x & 0xFFFF0000u);
         v[2] -= __uint_as_float(q.y << 16);
@@ -573,10 +575,12 @@ template <bool BT> __device__ __forceinline__ void store(uint4 raw, U16 *lds) {
 // Row strides below 2^22 (32-bit byte offsets in a tile).
 // BT: B is [K][N] as it stands in memory, b_rows of its K rows there (past them A is zero)
 // and b_cols columns (a multiple of four).  Its tile stays [32][128] in LDS, and the
-// fragments come out by transpose reads.
-template <bool BT>
+// fragments come out by transpose reads.  AT: A alike, with every row and column of a tile
+// in memory.
+template <bool AT, bool BT>
 __device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, const float *B, int64_t ldb, int b_rows, int b_cols,
                                      int K, floatx4 (&acc)[4][4], U16 *s0, U16 *s1) {
+    constexpr int PLANE = plane<AT, BT>(), A_TILE = a_tile<AT>();
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int arow0 = 64 * (w >> 1), brow0 = TM + 64 * (w & 1);
 #pragma unroll
@@ -591,34 +595,36 @@ __device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, co
 #pragma unroll
     for (int i = 0; i < 2; ++i) bo[i] = 4u * ((unsigned)min(r8 + 64 * i, b_rows - 1) * (unsigned)ldb + 4 * c8);
     const int to = r8 * BK + 8 * swz(r8, c8 >> 1) + 4 * (c8 & 1);  // the swizzle repeats every eight rows
-    // BT: thread -> B's row tid / 16, columns 4 (tid % 16) + 64 i
-    const int r16 = tid >> 4, c16 = tid & 15, bt_to = TM * BK + place(r16) * PT + 4 * c16;
+    // AT, BT: thread -> the tile's row tid / 16, columns 4 (tid % 16) + 64 i
+    const int r16 = tid >> 4, c16 = tid & 15, at_to = place(r16) * PA + 4 * c16, bt_to = A_TILE + place(r16) * PB + 4 * c16;
+    const unsigned at = 4u * ((unsigned)r16 * (unsigned)lda + 4 * c16);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
         if (BT) bo[i] = 4u * min(64 * i + 4 * c16, b_cols - 4);
     auto gload = [&](Raw &x, int step) {
-        const char *a = reinterpret_cast<const char *>(A + (int64_t)step * BK);
+        const char *a = reinterpret_cast<const char *>(AT ? A + (int64_t)step * BK * lda : A + (int64_t)step * BK);
         const int row0 = BT ? min(step * BK, b_rows - 1) : 0;
         const char *b = reinterpret_cast<const char *>(BT ? B + row0 * ldb : B + (int64_t)step * BK);
         const unsigned row = BT ? 4u * (unsigned)min(r16, b_rows - 1 - row0) * (unsigned)ldb : 0u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x.a[i] = *reinterpret_cast<const uint4 *>(a + ao[i]);
+        for (int i = 0; i < 4; ++i) x.a[i] = *reinterpret_cast<const uint4 *>(AT ? a + at + 256 * i : a + ao[i]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) x.b[i] = *reinterpret_cast<const uint4 *>(b + (row + bo[i]));
     };
     auto put = [&](const Raw &x, U16 *s, int i) {  // the i-th of the six pieces
-        if (BT && i >= 4) store<BT>(x.b[i < 4 ? 0 : i - 4], s + bt_to + 64 * (i - 4));
-        else store<BT>(i < 4 ? x.a[i < 4 ? i : 0] : x.b[i < 4 ? 0 : i - 4], s + to + 64 * (i < 4 ? i : TM / 64 + i - 4) * BK);
+        const uint4 v = i < 4 ? x.a[i < 4 ? i : 0] : x.b[i < 4 ? 0 : i - 4];
+        if (i < 4) store<PLANE>(v, s + (AT ? at_to + 64 * i : to + 64 * i * BK));
+        else store<PLANE>(v, s + (BT ? bt_to + 64 * (i - 4) : A_TILE + to + 64 * (i - 4) * BK));
     };
-    // BT: the lane's column l16 of a 16-column chunk, k = 8 g ..: rows 8 g + l16 / 4 and four behind it
-    const int bt_at = TM * BK + place(8 * g + (l16 >> 2)) * PT + 64 * (w & 1) + 4 * (l16 & 3);
-    auto fragment_t = [&](const U16 *s, int ni, int part) {
-        const U16 *at = s + part * plane<BT>() + bt_at + 16 * ni;
-        const shortx4 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * PT);
+    // AT, BT: the lane's column l16 of a 16-column chunk, k = 8 g ..: rows 8 g + l16 / 4 and four behind it
+    const int row_t = place(8 * g + (l16 >> 2)), col_t = 4 * (l16 & 3);
+    const int at_from = row_t * PA + arow0 + col_t, bt_from = A_TILE + row_t * PB + 64 * (w & 1) + col_t;
+    auto fragment_t = [&](const U16 *at, int pitch) {
+        const shortx4 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * pitch);
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     auto fragment = [&](const U16 *s, int row, int part) {
-        return *reinterpret_cast<const bf16x8 *>(s + part * plane<BT>() + (row + l16) * BK + 8 * swz(l16, g));
+        return *reinterpret_cast<const bf16x8 *>(s + part * PLANE + (row + l16) * BK + 8 * swz(l16, g));
     };
     // the products of the step in `cur`; the next step's values go from x to `next`
     auto step = [&](const U16 *cur, U16 *next, const Raw &x) {
@@ -626,13 +632,14 @@ __device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, co
 #pragma unroll
         for (int mi = 0; mi < 4; ++mi)
 #pragma unroll
-            for (int part = 0; part < 3; ++part) a[mi][part] = fragment(cur, arow0 + 16 * mi, part);
+            for (int part = 0; part < 3; ++part)
+                a[mi][part] = AT ? fragment_t(cur + part * PLANE + at_from + 16 * mi, PA) : fragment(cur, arow0 + 16 * mi, part);
 #pragma unroll
         for (int ni = 0; ni < 4; ++ni) {
             bf16x8 b[3];
 #pragma unroll
             for (int part = 0; part < 3; ++part)
-                b[part] = BT ? fragment_t(cur, ni, part) : fragment(cur, brow0 + 16 * ni, part);
+                b[part] = BT ? fragment_t(cur + part * PLANE + bt_from + 16 * ni, PB) : fragment(cur, brow0 + 16 * ni, part);
             constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};  // small products first
 #pragma unroll
             for (int j = 0; j < 6; ++j)
@@ -664,12 +671,12 @@ __device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, co
 }
 
 __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
-    __shared__ __align__(16) U16 s0[3 * plane<false>()], s1[3 * plane<false>()];
+    __shared__ __align__(16) U16 s0[3 * plane<false, false>()], s1[3 * plane<false, false>()];
     __shared__ float sB[2][TM], sS[2][TM], sT[2][TM];
     const qpam_ce_fwd_args &a = p.a;
     const int vt = blockIdx.x, r0 = blockIdx.y * TM, v0 = vt * TN;
     floatx4 acc[4][4];
-    tile<false>((const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0), (const float *)a.w + (int64_t)v0 * a.ldw,
+    tile<false, false>((const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0), (const float *)a.w + (int64_t)v0 * a.ldw,
                 a.ldw, min(TN, a.V - v0), 0, a.D, acc, s0, s1);
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1, vl = v0 + 64 * wn + l16;
@@ -710,10 +717,10 @@ __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
     }
 }
 
-// G [rows][Vp] and G^T [Vp][Rp] (each if there is a buffer for it) without the tokens'
-// one-hot terms; zero past the vocabulary and past the rows (Rp: a multiple of 256)
+// G^T [Vp][Rp] without the tokens' one-hot terms; zero past the vocabulary and past the rows
+// (Rp: a multiple of 256)
 __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
-    __shared__ __align__(16) U16 s0[3 * plane<false>()], s1[3 * plane<false>()];
+    __shared__ __align__(16) U16 s0[3 * plane<false, false>()], s1[3 * plane<false, false>()];
     __shared__ __align__(16) float sRow[3][TM];
     const qpam_ce_bwd_args &a = p.a;
     const int lr0 = blockIdx.y * TM, v0 = blockIdx.x * TN, tid = threadIdx.x;
@@ -724,11 +731,11 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
         sRow[2][tid] = q.slope;
     }
     floatx4 acc[4][4];
-    tile<false>((const float *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(TM, p.rows - lr0),
+    tile<false, false>((const float *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(TM, p.rows - lr0),
                 (const float *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(TN, a.V - v0), 0, a.D, acc, s0, s1);
     const int w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
-    float *G = (float *)p.gbuf, *GT = (float *)p.gtbuf;
+    float *GT = (float *)p.gtbuf;
 #pragma unroll
     for (int mi = 0; mi < 4; ++mi) {
         const int rl = 64 * wm + 16 * mi + 4 * g;
@@ -744,23 +751,23 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
                 const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -hb[r]);
                 const bool in = v < a.V && lr0 + rl + r < p.rows;
                 x[r] = in ? __builtin_amdgcn_exp2f(u) * __builtin_fmaf(h1[r], u, h0[r]) : 0.f;
-                if (G && lr0 + rl + r < p.rows) G[(int64_t)(lr0 + rl + r) * p.Vp + v] = x[r];
             }
-            if (GT) *reinterpret_cast<floatx4 *>(GT + (int64_t)v * p.Rp + lr0 + rl) = x;
+            *reinterpret_cast<floatx4 *>(GT + (int64_t)v * p.Rp + lr0 + rl) = x;
         }
     }
 }
 
-// C = A B (dH and dW), A [M][K], B [b_rows][N] with b_rows <= K and zeros in A past them, the
-// K axis in gridDim.z ranges of kper: one range writes C (or adds to it), several write
-// C + z split_stride, summed by sum_kernel in their order.
+// C = A B, B [b_rows][N] with b_rows <= K and zeros in A past them, A [M][K] (dW: G^T) or
+// with AT [K][M] (dH: G^T again).  The K axis in gridDim.z ranges of kper: one range writes
+// C (or adds to it), several write C + z split_stride, summed by sum_kernel in their order.
+template <bool AT>
 __global__ void __launch_bounds__(TT) gemm_kernel(const float *A, int64_t lda, int M, const float *B, int64_t ldb, int b_rows,
                                                   int N, int K, int kper, float *C, int64_t ldc, int64_t split_stride, int accumulate) {
-    __shared__ __align__(16) U16 s0[3 * plane<true>()], s1[3 * plane<true>()];
+    __shared__ __align__(16) U16 s0[3 * plane<AT, true>()], s1[3 * plane<AT, true>()];
     const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN, k0 = blockIdx.z * kper;
     floatx4 acc[4][4];
     const int kb = min(k0, b_rows - 1);  // a range past B's rows: A is zero there
-    tile<true>(A + (int64_t)m0 * lda + k0, lda, min(TM, M - m0), B + (int64_t)kb * ldb + n0, ldb, b_rows - kb, min(TN, N - n0),
+    tile<AT, true>(AT ? A + (int64_t)k0 * lda + m0 : A + (int64_t)m0 * lda + k0, lda, min(TM, M - m0), B + (int64_t)kb * ldb + n0, ldb, b_rows - kb, min(TN, N - n0),
                min(kper, K - k0), acc, s0, s1);
     C += blockIdx.z * split_stride;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
@@ -2382,12 +2389,16 @@ int dh_splits(int rows, int D, int Vp) {
     return std::max(1, std::min({256 / std::max(tiles, 1), Vp / 512, 16}));
 }
 
-// G, G^T (the rows padded to 256) and dH's partial sums: splits * rows <= 16 rows, and <=
+// Rows of one fp32 pass of the token scores: their 4-byte G^T fits the 8 bytes a row and
+// vocabulary entry that `chunk` stands for twice.
+int scores_f32_rows(const qpam_ce_bwd_args &a) { return (int)std::min<int64_t>(2 * (int64_t)a.chunk, a.N); }
+
+// G^T (the rows padded to 256) and dH's partial sums: splits * rows <= 16 rows, and <=
 // 256 TM as splits * tiles <= 256
 size_t scores_f32_ws(const qpam_ce_bwd_args &a) {
-    const int64_t Vp = round_up(a.V, split::TN), chunk = pass_rows(a), Rp = round_up((int)chunk, split::TM);
+    const int64_t Vp = round_up(a.V, split::TN), chunk = scores_f32_rows(a), Rp = round_up((int)chunk, split::TM);
     const int64_t part = std::min<int64_t>(16 * chunk, 256ll * split::TM) * a.D;
-    return (size_t)(chunk * Vp + Vp * Rp + part) * sizeof(float) + 256;
+    return (size_t)(Vp * Rp + part) * sizeof(float) + 256;
 }
 
 // Token scores in fp32: G tiles, then dH and dW (those that are asked for), all in bf16
@@ -2395,15 +2406,15 @@ size_t scores_f32_ws(const qpam_ce_bwd_args &a) {
 int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams &scores) {
     BwdParams p = scores;
     p.a = a;
-    p.write_g = a.dh != nullptr;
+    p.write_g = 0;
     p.Vp = round_up(a.V, split::TN);
-    const int chunk = pass_rows(a);
-    float *gb = (float *)a.workspace, *gt = gb + (int64_t)chunk * p.Vp, *part = gt + (int64_t)p.Vp * round_up(chunk, split::TM);
-    p.gbuf = a.dh ? gb : nullptr;
-    p.gtbuf = a.dw ? gt : nullptr;
-    auto gemm = [&](const char *what, const float *A, int64_t lda, int M, const float *B, int64_t ldb, int b_rows, int K, int kper,
+    const int chunk = scores_f32_rows(a);
+    float *gt = (float *)a.workspace, *part = gt + (int64_t)p.Vp * round_up(chunk, split::TM);
+    p.gbuf = nullptr;
+    p.gtbuf = gt;
+    auto gemm = [&](auto kernel, const char *what, const float *A, int64_t lda, int M, const float *B, int64_t ldb, int b_rows, int K, int kper,
                     float *C, int64_t ldc, int64_t stride, int accumulate) {
-        hipLaunchKernelGGL(split::gemm_kernel,
+        hipLaunchKernelGGL(kernel,
                            dim3((a.D + split::TN - 1) / split::TN, (M + split::TM - 1) / split::TM, (K + kper - 1) / kper),
                            dim3(split::TT), 0, stream, A, lda, M, B, ldb, b_rows, a.D, K, kper, C, ldc, stride, accumulate);
         return launch_status(what);
@@ -2417,11 +2428,11 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
         if ((st = launch_status("split scores_grad_kernel"))) return st;
         hipLaunchKernelGGL(scores_token_kernel<float>, dim3((p.rows + THREADS - 1) / THREADS), dim3(THREADS), 0, stream, p);
         if ((st = launch_status("scores_token_kernel"))) return st;
-        // dH[r0 .. r0 + rows] = G [rows][Vp] W
+        // dH[r0 .. r0 + rows] = (G^T [Vp][Rp])^T W
         const int splits = dh_splits(p.rows, a.D, p.Vp), kper = round_up((p.Vp + splits - 1) / splits, BK);
         float *dh = (float *)a.dh + (int64_t)r0 * a.lddh;
         if (a.dh) {
-            st = gemm("split gemm_kernel(dH)", gb, p.Vp, p.rows, (const float *)a.w, a.ldw, a.V, p.Vp, kper, splits > 1 ? part : dh,
+            st = gemm(split::gemm_kernel<true>, "split gemm_kernel(dH)", gt, p.Rp, p.rows, (const float *)a.w, a.ldw, a.V, p.Vp, kper, splits > 1 ? part : dh,
                       splits > 1 ? a.D : a.lddh, (int64_t)p.rows * a.D, 0);
             if (st) return st;
         }
@@ -2434,7 +2445,7 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
         }
         if (!a.dw) continue;
         // dW [V][D] (+)= G^T [Vp][Rp] H
-        st = gemm("split gemm_kernel(dW)", gt, p.Rp, a.V, (const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, p.rows, p.Rp, p.Rp, (float *)a.dw, a.lddw, 0, r0 > 0 ? 1 : 0);
+        st = gemm(split::gemm_kernel<false>, "split gemm_kernel(dW)", gt, p.Rp, a.V, (const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, p.rows, p.Rp, p.Rp, (float *)a.dw, a.lddw, 0, r0 > 0 ? 1 : 0);
         if (st) return st;
     }
     return QPAM_OK;
@@ -2594,8 +2605,8 @@ extern "C" int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void
     QPAM_REQUIRE(a->chunk >= 1, "qpam_linear_logprobs_bwd: chunk must be >= 1");
     QPAM_REQUIRE((!a->dh || a->lddh >= a->D) && (!a->dw || a->lddw >= a->D), "qpam_linear_logprobs_bwd: output leading dims must be >= D");
     QPAM_REQUIRE(a->dw_out == 1 || a->dw_out == 2, "qpam_linear_logprobs_bwd: dw_out must be 1 or 2");
-    QPAM_REQUIRE(a->dtype == QPAM_BF16 || (a->V < (1 << 22) - 256 && std::min(a->chunk, a->N) < (1 << 22) - 256),
-                 "qpam_linear_logprobs_bwd: fp32 takes V and chunk below 2^22 - 256");
+    QPAM_REQUIRE(a->dtype == QPAM_BF16 || (a->V < (1 << 22) - 256 && scores_f32_rows(bwd_args(*a)) < (1 << 22) - 256),
+                 "qpam_linear_logprobs_bwd: fp32 takes V and passes of 2 chunk rows below 2^22 - 256");
     const size_t need = qpam_linear_logprobs_bwd_workspace_size(a);
     QPAM_REQUIRE(a->workspace && a->workspace_bytes >= need && ((uintptr_t)a->workspace % 16) == 0,
                  "qpam_linear_logprobs_bwd: workspace needs %zu bytes (got %zu)", need, a->workspace_bytes);
