@@ -640,12 +640,12 @@ __device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, co
 #pragma unroll
             for (int part = 0; part < 3; ++part)
                 b[part] = BT ? fragment_t(cur + part * PLANE + bt_from + 16 * ni, PB) : fragment(cur, brow0 + 16 * ni, part);
-            constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};  // small products first
+            constexpr int QA[6] = {2, 0, 1, 1, 0, 0}, QB[6] = {0, 2, 1, 0, 1, 0};  // small products first
 #pragma unroll
             for (int j = 0; j < 6; ++j)
 #pragma unroll
                 for (int mi = 0; mi < 4; ++mi)
-                    acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mi][PA[j]], b[PB[j]], acc[mi][ni], 0, 0, 0);
+                    acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mi][QA[j]], b[QB[j]], acc[mi][ni], 0, 0, 0);
             if (ni < 3) {
                 put(x, next, 2 * ni);
                 put(x, next, 2 * ni + 1);
@@ -786,13 +786,18 @@ __global__ void __launch_bounds__(TT) gemm_kernel(const float *A, int64_t lda, i
             }
 }
 
-__global__ void __launch_bounds__(THREADS) sum_kernel(const float *part, int splits, int64_t rows, int cols, float *out, int64_t ldo) {
-    const int64_t n = rows * cols;
-    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * THREADS) {
-        float x = 0.f;
-        for (int z = 0; z < splits; ++z) x += part[z * n + i];
-        const int64_t r = i / cols;
-        out[r * ldo + (i - r * cols)] = x;
+// rows * cols is below 2^24 where there are several ranges; cols % 4 == 0
+__global__ void __launch_bounds__(THREADS) sum_kernel(const float *part, int ranges, int rows, int cols, float *out, int64_t ldo,
+                                                      int accumulate) {
+    const unsigned n4 = (unsigned)rows * (unsigned)cols / 4, per_row = cols / 4;
+    for (unsigned i = blockIdx.x * THREADS + threadIdx.x; i < n4; i += gridDim.x * THREADS) {
+        floatx4 x = reinterpret_cast<const floatx4 *>(part)[i];
+#pragma unroll 4
+        for (int z = 1; z < ranges; ++z) x += reinterpret_cast<const floatx4 *>(part)[(int64_t)z * n4 + i];
+        const unsigned r = i / per_row;
+        float *to = out + r * ldo + 4 * (i - r * per_row);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[j] = accumulate ? to[j] + x[j] : x[j];
     }
 }
 }  // namespace split
@@ -2382,22 +2387,23 @@ int validate_common(int N, int V, int D, int dtype, const void *h, int64_t ldh, 
     return QPAM_OK;
 }
 
-// Ranges of the vocabulary that share the token scores' fp32 dH of `rows` rows: a block for
-// each of the 256 CUs, at most 16 ranges and none below 512 entries.
-int dh_splits(int rows, int D, int Vp) {
-    const int tiles = ((rows + split::TM - 1) / split::TM) * ((D + split::TN - 1) / split::TN);
-    return std::max(1, std::min({256 / std::max(tiles, 1), Vp / 512, 16}));
+// Ranges of the K axis that share an [M][D] product of the token scores' fp32 backward: a
+// block for each of the 256 CUs, at most 16 ranges and none below 256 (eight steps).
+int k_ranges(int M, int D, int K) {
+    const int64_t tiles = (int64_t)((M + split::TM - 1) / split::TM) * ((D + split::TN - 1) / split::TN);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({256 / tiles, K / 256, 16}));
 }
+// ... and what their partial sums take at most: 16 ranges of M rows, or 256 tiles
+int64_t k_ranges_part(int64_t M, int D) { return std::min<int64_t>(16 * M * D, 256ll * split::TM * split::TN); }
 
 // Rows of one fp32 pass of the token scores: their 4-byte G^T fits the 8 bytes a row and
 // vocabulary entry that `chunk` stands for twice.
 int scores_f32_rows(const qpam_ce_bwd_args &a) { return (int)std::min<int64_t>(2 * (int64_t)a.chunk, a.N); }
 
-// G^T (the rows padded to 256) and dH's partial sums: splits * rows <= 16 rows, and <=
-// 256 TM as splits * tiles <= 256
+// G^T (the rows padded to 256) and a product's partial sums
 size_t scores_f32_ws(const qpam_ce_bwd_args &a) {
     const int64_t Vp = round_up(a.V, split::TN), chunk = scores_f32_rows(a), Rp = round_up((int)chunk, split::TM);
-    const int64_t part = std::min<int64_t>(16 * chunk, 256ll * split::TM) * a.D;
+    const int64_t part = std::max(k_ranges_part(chunk, a.D), k_ranges_part(a.V, a.D));
     return (size_t)(Vp * Rp + part) * sizeof(float) + 256;
 }
 
@@ -2412,12 +2418,18 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
     float *gt = (float *)a.workspace, *part = gt + (int64_t)p.Vp * round_up(chunk, split::TM);
     p.gbuf = nullptr;
     p.gtbuf = gt;
-    auto gemm = [&](auto kernel, const char *what, const float *A, int64_t lda, int M, const float *B, int64_t ldb, int b_rows, int K, int kper,
-                    float *C, int64_t ldc, int64_t stride, int accumulate) {
-        hipLaunchKernelGGL(kernel,
-                           dim3((a.D + split::TN - 1) / split::TN, (M + split::TM - 1) / split::TM, (K + kper - 1) / kper),
-                           dim3(split::TT), 0, stream, A, lda, M, B, ldb, b_rows, a.D, K, kper, C, ldc, stride, accumulate);
-        return launch_status(what);
+    // C [M][D] (+)= A B, in ranges of K where the tiles alone leave CUs idle
+    auto gemm = [&](auto kernel, const char *what, int M, const float *B, int64_t ldb, int b_rows, int K, float *C, int64_t ldc,
+                    int accumulate) {
+        const int ranges = k_ranges(M, a.D, K), kper = round_up((K + ranges - 1) / ranges, BK), n_k = (K + kper - 1) / kper;
+        hipLaunchKernelGGL(kernel, dim3((a.D + split::TN - 1) / split::TN, (M + split::TM - 1) / split::TM, n_k), dim3(split::TT), 0,
+                           stream, (const float *)gt, (int64_t)p.Rp, M, B, ldb, b_rows, a.D, K, kper, n_k > 1 ? part : C,
+                           n_k > 1 ? a.D : ldc, (int64_t)M * a.D, n_k > 1 ? 0 : accumulate);
+        const int st = launch_status(what);
+        if (st || n_k == 1) return st;
+        hipLaunchKernelGGL(split::sum_kernel, dim3((unsigned)(((int64_t)M * a.D / 4 + THREADS - 1) / THREADS)), dim3(THREADS), 0, stream,
+                           (const float *)part, n_k, M, a.D, C, ldc, accumulate);
+        return launch_status("split sum_kernel");
     };
     int st = QPAM_OK;
     for (int r0 = 0; r0 < a.N; r0 += chunk) {
@@ -2428,24 +2440,14 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
         if ((st = launch_status("split scores_grad_kernel"))) return st;
         hipLaunchKernelGGL(scores_token_kernel<float>, dim3((p.rows + THREADS - 1) / THREADS), dim3(THREADS), 0, stream, p);
         if ((st = launch_status("scores_token_kernel"))) return st;
-        // dH[r0 .. r0 + rows] = (G^T [Vp][Rp])^T W
-        const int splits = dh_splits(p.rows, a.D, p.Vp), kper = round_up((p.Vp + splits - 1) / splits, BK);
-        float *dh = (float *)a.dh + (int64_t)r0 * a.lddh;
-        if (a.dh) {
-            st = gemm(split::gemm_kernel<true>, "split gemm_kernel(dH)", gt, p.Rp, p.rows, (const float *)a.w, a.ldw, a.V, p.Vp, kper, splits > 1 ? part : dh,
-                      splits > 1 ? a.D : a.lddh, (int64_t)p.rows * a.D, 0);
-            if (st) return st;
-        }
-        if (a.dh && splits > 1) {
-            const int64_t n = (int64_t)p.rows * a.D;
-            hipLaunchKernelGGL(split::sum_kernel, dim3((unsigned)std::min<int64_t>((n + THREADS - 1) / THREADS, 4096)),
-                               dim3(THREADS), 0, stream, (const float *)part, (p.Vp + kper - 1) / kper, (int64_t)p.rows, a.D,
-                               dh, a.lddh);
-            if ((st = launch_status("split sum_kernel"))) return st;
-        }
-        if (!a.dw) continue;
-        // dW [V][D] (+)= G^T [Vp][Rp] H
-        st = gemm(split::gemm_kernel<false>, "split gemm_kernel(dW)", gt, p.Rp, a.V, (const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, p.rows, p.Rp, p.Rp, (float *)a.dw, a.lddw, 0, r0 > 0 ? 1 : 0);
+        // dH [rows][D] = (G^T [Vp][Rp])^T W, dW [V][D] (+)= G^T H
+        if (a.dh)
+            st = gemm(split::gemm_kernel<true>, "split gemm_kernel(dH)", p.rows, (const float *)a.w, a.ldw, a.V, p.Vp,
+                      (float *)a.dh + (int64_t)r0 * a.lddh, a.lddh, 0);
+        if (st) return st;
+        if (a.dw)
+            st = gemm(split::gemm_kernel<false>, "split gemm_kernel(dW)", a.V, (const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, p.rows,
+                      round_up(p.rows, BK), (float *)a.dw, a.lddw, r0 > 0 ? 1 : 0);
         if (st) return st;
     }
     return QPAM_OK;

@@ -281,3 +281,19 @@ def test_tiles_that_do_not_fill_their_last_round(gpu_lib, n, V, D):
     want = _reference(h, w, ids, 0.9, None, 0.0)
     _close(r.logprobs, want["lp"].cpu(), want["t_lp"].cpu())
     _close(r.entropy, want["H"].cpu(), want["t_H"].cpu())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V,D,chunk", [(1300, 300, 64, 300), (520, 150, 160, 4096), (66, 1500, 256, 4096), (200, 900, 64, 33)])
+def test_gradients_of_small_tables_and_several_passes(gpu_lib, n, V, D, chunk, dtype):
+    """Products with few tiles and long sums: shared K ranges, their partial sums added over the passes."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, gs = _data(n, V, D, dtype, dtype, n)
+    R = _reference(h, w, ids, 1.3, [g.double() for g in gs], 2.0 ** -8 if dtype == BF16 else 0.0)
+    hc, wc = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    r = linear_token_logprobs(hc, wc, ids.cuda(), temperature=1.3, chunk=chunk)
+    _close(r.logprobs, R["lp"], R["t_lp"])
+    _close(r.entropy, R["H"], R["t_H"])
+    dh, dw = torch.autograd.grad([r.logprobs, r.entropy], [hc, wc], [g.cuda() for g in gs])
+    _close(dh, R["dh"], R["t_dh"], torch.finfo(dtype).eps)
+    _close(dw, R["dw"], R["t_dw"], torch.finfo(dtype).eps)
