@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(THREADS) ce_gemm_kernel(const T *A, int64_t ld
             }
 }
 
-// Token scores in fp32, 256 x 128 tiles on the bf16 matrix units: every value is split into
+// Token scores in fp32, 256 x 128 tiles (or 128 x 64) on the bf16 matrix units: every value is split into
 // three bf16 parts, x = hi + mid + lo with |mid| <= 2^-9 |x|, |lo| <= 2^-18 |x| and nothing
 // left above 2^-27 |x|, and a product is the six part products down to 2^-18; the three
 // left out are below 2^-26 of it, less than one fp32 rounding.  A k-step of 32 takes a
@@ -542,15 +542,18 @@ __global__ void __launch_bounds__(THREADS) ce_gemm_kernel(const T *A, int64_t ld
 // epilogue.  The fp32 MFMAs took 172 us, parts made in front of the products 80.
 // Rows past the end of an operand re-read its last row.  Infinite operands give NaN.
 namespace split {
-constexpr int TM = 256, TN = 128, TT = 512;
-constexpr int PA = TM + 16, PB = TN + 16;  // pitches of tiles [32][256] of A, [32][128] of B
-// bf16 elements of a plane: A's tile, then B's (AT, BT: as they stand in memory, [K][M], [K][N])
-template <bool AT> constexpr int a_tile() { return AT ? BK * PA : TM * BK; }
-template <bool AT, bool BT> constexpr int plane() { return a_tile<AT>() + (BT ? BK * PB : TN * BK); }
+// S: a wave's 16 x 16 tiles along both axes; 4, or 2 for 128 x 64 tiles
+template <int S> constexpr int tm() { return 64 * S; }
+template <int S> constexpr int tn() { return 32 * S; }
+constexpr int TM = tm<4>(), TN = tn<4>(), TT = 512;
+// bf16 elements of a plane: A's tile, then B's (AT, BT: as they stand in memory, [K][M], [K][N],
+// rows 16 elements apart from the next)
+template <int S, bool AT> constexpr int a_tile() { return AT ? BK * (tm<S>() + 16) : tm<S>() * BK; }
+template <int S, bool AT, bool BT> constexpr int plane() { return a_tile<S, AT>() + BK * (tn<S>() + (BT ? 16 : 0)); }
 using U16 = unsigned short;
 
-struct Raw {
-    uint4 a[TM * BK / 4 / TT], b[TN * BK / 4 / TT];  // 4 and 2 loads a thread and step
+template <int S> struct Raw {
+    uint4 a[S], b[S / 2];  // a thread's loads of a step
 };
 
 __device__ __forceinline__ int swz(int row, int c) { return c ^ ((row >> 1) & 3); }
@@ -571,54 +574,55 @@ template <int PLANE> __device__ __forceinline__ void store(uint4 raw, U16 *lds) 
     }
 }
 
-// acc[mi][ni] lane holds C[64*(w>>1) + 16mi + 4g + r][64*(w&1) + 16ni + l16]; K % 32 == 0.
+// acc[mi][ni] lane holds C[16*S*(w>>1) + 16mi + 4g + r][16*S*(w&1) + 16ni + l16]; K % 32 == 0.
 // Row strides below 2^22 (32-bit byte offsets in a tile).
 // BT: B is [K][N] as it stands in memory, b_rows of its K rows there (past them A is zero)
-// and b_cols columns (a multiple of four).  Its tile stays [32][128] in LDS, and the
+// and b_cols columns (a multiple of four).  Its tile stays [32][N] in LDS, and the
 // fragments come out by transpose reads.  AT: A alike, with every row and column of a tile
 // in memory.
-template <bool AT, bool BT>
+template <int S, bool AT, bool BT>
 __device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, const float *B, int64_t ldb, int b_rows, int b_cols,
-                                     int K, floatx4 (&acc)[4][4], U16 *s0, U16 *s1) {
-    constexpr int PLANE = plane<AT, BT>(), A_TILE = a_tile<AT>();
+                                     int K, floatx4 (&acc)[S][S], U16 *s0, U16 *s1) {
+    constexpr int PLANE = plane<S, AT, BT>(), A_TILE = a_tile<S, AT>(), PA = tm<S>() + 16, PB = tn<S>() + 16;
+    constexpr int PIECES = S + S / 2;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
-    const int arow0 = 64 * (w >> 1), brow0 = TM + 64 * (w & 1);
+    const int arow0 = 16 * S * (w >> 1), bcol0 = 16 * S * (w & 1);
 #pragma unroll
-    for (int mi = 0; mi < 4; ++mi)
+    for (int mi = 0; mi < S; ++mi)
 #pragma unroll
-        for (int ni = 0; ni < 4; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int ni = 0; ni < S; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
     // thread -> rows tid / 8 + 64 i, values 4 (tid % 8) ..: half a chunk of eight
     const int r8 = tid >> 3, c8 = tid & 7;
-    unsigned ao[4], bo[2];
+    unsigned ao[S], bo[S / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ao[i] = 4u * ((unsigned)min(r8 + 64 * i, a_rows - 1) * (unsigned)lda + 4 * c8);
+    for (int i = 0; i < S; ++i) ao[i] = 4u * ((unsigned)min(r8 + 64 * i, a_rows - 1) * (unsigned)lda + 4 * c8);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) bo[i] = 4u * ((unsigned)min(r8 + 64 * i, b_rows - 1) * (unsigned)ldb + 4 * c8);
+    for (int i = 0; i < S / 2; ++i) bo[i] = 4u * ((unsigned)min(r8 + 64 * i, b_rows - 1) * (unsigned)ldb + 4 * c8);
     const int to = r8 * BK + 8 * swz(r8, c8 >> 1) + 4 * (c8 & 1);  // the swizzle repeats every eight rows
     // AT, BT: thread -> the tile's row tid / 16, columns 4 (tid % 16) + 64 i
     const int r16 = tid >> 4, c16 = tid & 15, at_to = place(r16) * PA + 4 * c16, bt_to = A_TILE + place(r16) * PB + 4 * c16;
     const unsigned at = 4u * ((unsigned)r16 * (unsigned)lda + 4 * c16);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < S / 2; ++i)
         if (BT) bo[i] = 4u * min(64 * i + 4 * c16, b_cols - 4);
-    auto gload = [&](Raw &x, int step) {
+    auto gload = [&](Raw<S> &x, int step) {
         const char *a = reinterpret_cast<const char *>(AT ? A + (int64_t)step * BK * lda : A + (int64_t)step * BK);
         const int row0 = BT ? min(step * BK, b_rows - 1) : 0;
         const char *b = reinterpret_cast<const char *>(BT ? B + row0 * ldb : B + (int64_t)step * BK);
         const unsigned row = BT ? 4u * (unsigned)min(r16, b_rows - 1 - row0) * (unsigned)ldb : 0u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x.a[i] = *reinterpret_cast<const uint4 *>(AT ? a + at + 256 * i : a + ao[i]);
+        for (int i = 0; i < S; ++i) x.a[i] = *reinterpret_cast<const uint4 *>(AT ? a + at + 256 * i : a + ao[i]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) x.b[i] = *reinterpret_cast<const uint4 *>(b + (row + bo[i]));
+        for (int i = 0; i < S / 2; ++i) x.b[i] = *reinterpret_cast<const uint4 *>(b + (row + bo[i]));
     };
-    auto put = [&](const Raw &x, U16 *s, int i) {  // the i-th of the six pieces
-        const uint4 v = i < 4 ? x.a[i < 4 ? i : 0] : x.b[i < 4 ? 0 : i - 4];
-        if (i < 4) store<PLANE>(v, s + (AT ? at_to + 64 * i : to + 64 * i * BK));
-        else store<PLANE>(v, s + (BT ? bt_to + 64 * (i - 4) : A_TILE + to + 64 * (i - 4) * BK));
+    auto put = [&](const Raw<S> &x, U16 *s, int i) {
+        const uint4 v = i < S ? x.a[i < S ? i : 0] : x.b[i < S ? 0 : i - S];
+        if (i < S) store<PLANE>(v, s + (AT ? at_to + 64 * i : to + 64 * i * BK));
+        else store<PLANE>(v, s + (BT ? bt_to + 64 * (i - S) : A_TILE + to + 64 * (i - S) * BK));
     };
     // AT, BT: the lane's column l16 of a 16-column chunk, k = 8 g ..: rows 8 g + l16 / 4 and four behind it
     const int row_t = place(8 * g + (l16 >> 2)), col_t = 4 * (l16 & 3);
-    const int at_from = row_t * PA + arow0 + col_t, bt_from = A_TILE + row_t * PB + 64 * (w & 1) + col_t;
+    const int at_from = row_t * PA + arow0 + col_t, bt_from = A_TILE + row_t * PB + bcol0 + col_t;
     auto fragment_t = [&](const U16 *at, int pitch) {
         const shortx4 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * pitch);
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -627,37 +631,36 @@ __device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, co
         return *reinterpret_cast<const bf16x8 *>(s + part * PLANE + (row + l16) * BK + 8 * swz(l16, g));
     };
     // the products of the step in `cur`; the next step's values go from x to `next`
-    auto step = [&](const U16 *cur, U16 *next, const Raw &x) {
-        bf16x8 a[4][3];
+    auto step = [&](const U16 *cur, U16 *next, const Raw<S> &x) {
+        bf16x8 a[S][3];
 #pragma unroll
-        for (int mi = 0; mi < 4; ++mi)
+        for (int mi = 0; mi < S; ++mi)
 #pragma unroll
             for (int part = 0; part < 3; ++part)
                 a[mi][part] = AT ? fragment_t(cur + part * PLANE + at_from + 16 * mi, PA) : fragment(cur, arow0 + 16 * mi, part);
 #pragma unroll
-        for (int ni = 0; ni < 4; ++ni) {
+        for (int ni = 0; ni < S; ++ni) {
             bf16x8 b[3];
 #pragma unroll
             for (int part = 0; part < 3; ++part)
-                b[part] = BT ? fragment_t(cur + part * PLANE + bt_from + 16 * ni, PB) : fragment(cur, brow0 + 16 * ni, part);
+                b[part] = BT ? fragment_t(cur + part * PLANE + bt_from + 16 * ni, PB) : fragment(cur + A_TILE, bcol0 + 16 * ni, part);
             constexpr int QA[6] = {2, 0, 1, 1, 0, 0}, QB[6] = {0, 2, 1, 0, 1, 0};  // small products first
 #pragma unroll
             for (int j = 0; j < 6; ++j)
 #pragma unroll
-                for (int mi = 0; mi < 4; ++mi)
+                for (int mi = 0; mi < S; ++mi)
                     acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mi][QA[j]], b[QB[j]], acc[mi][ni], 0, 0, 0);
-            if (ni < 3) {
-                put(x, next, 2 * ni);
-                put(x, next, 2 * ni + 1);
-            }
+            if (ni < S - 1)
+#pragma unroll
+                for (int i = ni * PIECES / (S - 1); i < (ni + 1) * PIECES / (S - 1); ++i) put(x, next, i);
         }
     };
     const int KT = K / BK;
-    Raw x0, x1;
+    Raw<S> x0, x1;
     gload(x0, 0);
     gload(x1, min(1, KT - 1));
 #pragma unroll
-    for (int i = 0; i < 6; ++i) put(x0, s0, i);
+    for (int i = 0; i < PIECES; ++i) put(x0, s0, i);
     __syncthreads();
     for (int kt = 0; kt < KT; kt += 2) {
         gload(x0, min(kt + 2, KT - 1));
@@ -670,28 +673,30 @@ __device__ __forceinline__ void tile(const float *A, int64_t lda, int a_rows, co
     }
 }
 
+template <int S>
 __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
-    __shared__ __align__(16) U16 s0[3 * plane<false, false>()], s1[3 * plane<false, false>()];
+    constexpr int TM = tm<S>(), TN = tn<S>();
+    __shared__ __align__(16) U16 s0[3 * plane<S, false, false>()], s1[3 * plane<S, false, false>()];
     __shared__ float sB[2][TM], sS[2][TM], sT[2][TM];
     const qpam_ce_fwd_args &a = p.a;
     const int vt = blockIdx.x, r0 = blockIdx.y * TM, v0 = vt * TN;
-    floatx4 acc[4][4];
-    tile<false, false>((const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0), (const float *)a.w + (int64_t)v0 * a.ldw,
-                a.ldw, min(TN, a.V - v0), 0, a.D, acc, s0, s1);
+    floatx4 acc[S][S];
+    tile<S, false, false>((const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0),
+                          (const float *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(TN, a.V - v0), 0, a.D, acc, s0, s1);
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
-    const int wm = w >> 1, wn = w & 1, vl = v0 + 64 * wn + l16;
+    const int wm = w >> 1, wn = w & 1, vl = v0 + 16 * S * wn + l16;
 #pragma unroll
-    for (int mi = 0; mi < 4; ++mi)
+    for (int mi = 0; mi < S; ++mi)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             float mx = -INFINITY;
 #pragma unroll
-            for (int ni = 0; ni < 4; ++ni)
+            for (int ni = 0; ni < S; ++ni)
                 if (vl + 16 * ni < a.V) mx = fmaxf(mx, acc[mi][ni][r]);
             const float b = row16_max(mx) * p.c;
             float s = 0.f, t = 0.f;
 #pragma unroll
-            for (int ni = 0; ni < 4; ++ni)
+            for (int ni = 0; ni < S; ++ni)
                 if (vl + 16 * ni < a.V) {
                     const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
                     s += e;
@@ -700,7 +705,7 @@ __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
             s = row16_sum(s);
             t = row16_sum(t);
             if (l16 == 0) {
-                const int row = 64 * wm + 16 * mi + 4 * g + r;
+                const int row = 16 * S * wm + 16 * mi + 4 * g + r;
                 sB[wn][row] = b;
                 sS[wn][row] = s;
                 sT[wn][row] = t;
@@ -719,8 +724,10 @@ __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
 
 // G^T [Vp][Rp] without the tokens' one-hot terms; zero past the vocabulary and past the rows
 // (Rp: a multiple of 256)
+template <int S>
 __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
-    __shared__ __align__(16) U16 s0[3 * plane<false, false>()], s1[3 * plane<false, false>()];
+    constexpr int TM = tm<S>(), TN = tn<S>();
+    __shared__ __align__(16) U16 s0[3 * plane<S, false, false>()], s1[3 * plane<S, false, false>()];
     __shared__ __align__(16) float sRow[3][TM];
     const qpam_ce_bwd_args &a = p.a;
     const int lr0 = blockIdx.y * TM, v0 = blockIdx.x * TN, tid = threadIdx.x;
@@ -730,21 +737,23 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
         sRow[1][tid] = q.base;
         sRow[2][tid] = q.slope;
     }
-    floatx4 acc[4][4];
-    tile<false, false>((const float *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(TM, p.rows - lr0),
-                (const float *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(TN, a.V - v0), 0, a.D, acc, s0, s1);
+    floatx4 acc[S][S];
+    // a tile of padding alone (the small ones) reads the last row
+    const int lr = min(lr0, p.rows - 1), vr = min(v0, a.V - 1);
+    tile<S, false, false>((const float *)a.h + (int64_t)(p.row0 + lr) * a.ldh, a.ldh, min(TM, p.rows - lr),
+                          (const float *)a.w + (int64_t)vr * a.ldw, a.ldw, min(TN, a.V - vr), 0, a.D, acc, s0, s1);
     const int w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
     float *GT = (float *)p.gtbuf;
 #pragma unroll
-    for (int mi = 0; mi < 4; ++mi) {
-        const int rl = 64 * wm + 16 * mi + 4 * g;
+    for (int mi = 0; mi < S; ++mi) {
+        const int rl = 16 * S * wm + 16 * mi + 4 * g;
         const floatx4 hb = *reinterpret_cast<const floatx4 *>(&sRow[0][rl]);
         const floatx4 h0 = *reinterpret_cast<const floatx4 *>(&sRow[1][rl]);
         const floatx4 h1 = *reinterpret_cast<const floatx4 *>(&sRow[2][rl]);
 #pragma unroll
-        for (int ni = 0; ni < 4; ++ni) {
-            const int v = v0 + 64 * wn + 16 * ni + l16;
+        for (int ni = 0; ni < S; ++ni) {
+            const int v = v0 + 16 * S * wn + 16 * ni + l16;
             floatx4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -763,11 +772,11 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
 template <bool AT>
 __global__ void __launch_bounds__(TT) gemm_kernel(const float *A, int64_t lda, int M, const float *B, int64_t ldb, int b_rows,
                                                   int N, int K, int kper, float *C, int64_t ldc, int64_t split_stride, int accumulate) {
-    __shared__ __align__(16) U16 s0[3 * plane<AT, true>()], s1[3 * plane<AT, true>()];
+    __shared__ __align__(16) U16 s0[3 * plane<4, AT, true>()], s1[3 * plane<4, AT, true>()];
     const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN, k0 = blockIdx.z * kper;
     floatx4 acc[4][4];
     const int kb = min(k0, b_rows - 1);  // a range past B's rows: A is zero there
-    tile<AT, true>(AT ? A + (int64_t)k0 * lda + m0 : A + (int64_t)m0 * lda + k0, lda, min(TM, M - m0), B + (int64_t)kb * ldb + n0, ldb, b_rows - kb, min(TN, N - n0),
+    tile<4, AT, true>(AT ? A + (int64_t)k0 * lda + m0 : A + (int64_t)m0 * lda + k0, lda, min(TM, M - m0), B + (int64_t)kb * ldb + n0, ldb, b_rows - kb, min(TN, N - n0),
                min(kper, K - k0), acc, s0, s1);
     C += blockIdx.z * split_stride;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
@@ -800,6 +809,11 @@ __global__ void __launch_bounds__(THREADS) sum_kernel(const float *part, int ran
         for (int j = 0; j < 4; ++j) to[j] = accumulate ? to[j] + x[j] : x[j];
     }
 }
+
+// 128 x 64 tiles (two blocks a CU) up to 128 tiles of 256 x 128, which leave half the CUs
+// idle.  Scores at D = 768, small against large: 12 tiles 24 and 52 us, 64 tiles 28 and 53,
+// 126 tiles 45 and 57, 160 tiles 61 and 58, 256 tiles 82 and 66.
+inline bool small_tiles(int64_t M, int64_t N) { return ((M + TM - 1) / TM) * ((N + TN - 1) / TN) <= 128; }
 }  // namespace split
 
 // ------------------------------------------------------ bf16 big tiles ----
@@ -2144,8 +2158,9 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     const bool wide_tiles = is_bf<T>() && (scores || use_wide(a.D));  // the direct-load loop takes any multiple of 32
     const tiles::Columns cols = tiles::columns(a.N, a.V);
     const bool score_tiles = scores && is_bf<T>() && !few;
+    const bool small = scores && !is_bf<T>() && !few && split::small_tiles(a.N, a.V);
     p.full_vt = cols.full;
-    p.n_vt = few ? thin::blocks(a.V) : score_tiles ? cols.n_vt : wide_tiles ? (a.V + wide::TN - 1) / wide::TN : (a.V + vocab_tile<T>() - 1) / vocab_tile<T>();
+    p.n_vt = few ? thin::blocks(a.V) : score_tiles ? cols.n_vt : small ? (a.V + split::tn<2>() - 1) / split::tn<2>() : wide_tiles ? (a.V + wide::TN - 1) / wide::TN : (a.V + vocab_tile<T>() - 1) / vocab_tile<T>();
     char *ws = (char *)a.workspace;
     const int64_t cnt = (int64_t)a.N * p.n_vt;
     p.part_m = (float *)ws;
@@ -2157,7 +2172,12 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     if (few) {
         st = thin::waves(a.V) == 16 ? thin::launch<T, 16>(p, stream) : thin::launch<T, 4>(p, stream);
     } else if (scores && !is_bf<T>()) {
-        hipLaunchKernelGGL(split::scores_tile_kernel, dim3(p.n_vt, (a.N + split::TM - 1) / split::TM), dim3(split::TT), 0, stream, p);
+        if (small)
+            hipLaunchKernelGGL(split::scores_tile_kernel<2>, dim3(p.n_vt, (a.N + split::tm<2>() - 1) / split::tm<2>()),
+                               dim3(split::TT), 0, stream, p);
+        else
+            hipLaunchKernelGGL(split::scores_tile_kernel<4>, dim3(p.n_vt, (a.N + split::TM - 1) / split::TM), dim3(split::TT), 0,
+                               stream, p);
         st = launch_status("split scores_tile_kernel");
     } else if (score_tiles) {
         const dim3 grid(tiles::grid(p.n_vt * ((a.N + tiles::TM - 1) / tiles::TM)));
@@ -2436,7 +2456,11 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
         p.row0 = r0;
         p.rows = std::min(chunk, a.N - r0);
         p.Rp = round_up(p.rows, split::TM);
-        hipLaunchKernelGGL(split::scores_grad_kernel, dim3(p.Vp / split::TN, p.Rp / split::TM), dim3(split::TT), 0, stream, p);
+        if (split::small_tiles(p.rows, p.Vp))
+            hipLaunchKernelGGL(split::scores_grad_kernel<2>, dim3(p.Vp / split::tn<2>(), p.Rp / split::tm<2>()), dim3(split::TT), 0,
+                               stream, p);
+        else
+            hipLaunchKernelGGL(split::scores_grad_kernel<4>, dim3(p.Vp / split::TN, p.Rp / split::TM), dim3(split::TT), 0, stream, p);
         if ((st = launch_status("split scores_grad_kernel"))) return st;
         hipLaunchKernelGGL(scores_token_kernel<float>, dim3((p.rows + THREADS - 1) / THREADS), dim3(THREADS), 0, stream, p);
         if ((st = launch_status("scores_token_kernel"))) return st;
@@ -2568,6 +2592,7 @@ extern "C" size_t qpam_linear_logprobs_fwd_workspace_size(const qpam_linear_logp
     const qpam_ce_fwd_args f = fwd_args(*a);
     if (a->N <= thin::ROWS) return (size_t)a->N * thin::blocks(a->V) * 12 + 256;
     if (a->dtype == QPAM_BF16) return (size_t)a->N * tiles::columns(a->N, a->V).n_vt * 12 + 256;
+    if (split::small_tiles(a->N, a->V)) return (size_t)a->N * ((a->V + split::tn<2>() - 1) / split::tn<2>()) * 12 + 256;
     return qpam_ce_fwd_workspace_size(&f);
 }
 
