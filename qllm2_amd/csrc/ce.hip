@@ -373,6 +373,7 @@ struct BwdParams {
     void *ht;        // [D][Rp]
     int write_g;     // bf16 path: also write G (only the hand-written dH GEMM reads it)
     // token scores
+    int full_vt;     // vocab tiles of 256 columns in front of the narrow ones (tiles::Columns)
     float inv_t, c;  // 1 / T, log2(e) / T
     const float *stats, *logprobs, *entropy, *g_logprobs, *g_entropy;
 };
@@ -1814,9 +1815,8 @@ __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
 }
 
 // G^T [Vp][Rp] (and G [rows][Vp] with WRITE_G) without the tokens' one-hot terms; zero past
-// the vocabulary and past the rows.  A 16-wide vocab slab of a wave goes through LDS and
-// leaves as 128-byte runs of G^T.
-template <bool WRITE_G>
+// the vocabulary and past the rows.  Tiles as in the scores' kernel.
+template <bool WRITE_G, int NARROW>
 __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
     constexpr int LD = 72;  // bf16 per staged vocab row: 64 tile rows + padding against bank conflicts
     __shared__ __align__(16) Stage s0, s1, s2, s3;
@@ -1824,23 +1824,12 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
     __shared__ __align__(16) float sRow[2][3][TM];  // the rows' scores, of this tile and the next
     const qpam_ce_bwd_args &a = p.a;
     const Stages stages{s0, s1, s2, s3};
-    const int KT = a.D / DK;
+    const int KT = a.D / DK, n_rt = p.Rp / TM;
     const int tid = threadIdx.x, w = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
-    Walk at(p.Rp / TM, p.Vp / TN);
-    if (!at.more()) return;
-    auto operands = [&]() {
-        const int lr0 = at.rt * TM, v0 = at.vt * TN;
-        return loads((const U16 *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(TM, p.rows - lr0),
-                     (const U16 *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(TN, a.V - v0));
-    };
-    auto keep_rows = [&](const RowScore &q, int buf) {
-        if (tid < TM) {
-            sRow[buf][0][tid] = q.b;
-            sRow[buf][1][tid] = q.base;
-            sRow[buf][2][tid] = q.slope;
-        }
-    };
+    Walk at(n_rt, p.full_vt);
+    const bool last = (int)blockIdx.x < n_rt * ((p.Vp - p.full_vt * TN) / (32 * NARROW));
+    const int last_rt = blockIdx.x % n_rt, last_v0 = p.full_vt * TN + 32 * NARROW * (blockIdx.x / n_rt);
     U16 *G = (U16 *)p.gbuf;
     U16 *GT = (U16 *)p.gtbuf;
     U16 *slab = sSlab + w * 16 * LD;
@@ -1848,26 +1837,31 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
     // lane / 8 + 8, 16 bytes a lane
     const U16 *from = slab + (lane >> 3) * LD + 8 * (lane & 7);
     const unsigned to = 2u * ((lane >> 3) * (unsigned)p.Rp + 8 * (lane & 7));
-    keep_rows(row_score(p, at.rt * TM + (tid & (TM - 1))), 0);
-    Loads q = operands();
-    start(stages, q, KT);
-    for (int buf = 0;; buf ^= 1) {
-        floatx4 acc[4][8];
-        product(stages, q, KT, acc);
-        const int lr0 = at.rt * TM, v0 = at.vt * TN;
-        at.next();
-        if (at.more()) {
-            keep_rows(row_score(p, at.rt * TM + (tid & (TM - 1))), buf ^ 1);
-            q = operands();
-            start(stages, q, KT);
+    Loads q;
+    auto load_next = [&](int buf) {
+        if (!at.more() && !last) return;
+        const int rt = at.more() ? at.rt : last_rt, v0 = at.more() ? at.vt * TN : last_v0, lr0 = rt * TM;
+        const RowScore x = row_score(p, lr0 + (tid & (TM - 1)));
+        if (tid < TM) {
+            sRow[buf][0][tid] = x.b;
+            sRow[buf][1][tid] = x.base;
+            sRow[buf][2][tid] = x.slope;
         }
+        const int vr = min(v0, a.V - 1);  // a narrow tile of padding alone reads the last row
+        q = loads((const U16 *)a.h + (int64_t)(p.row0 + lr0) * a.ldh, a.ldh, min(TM, p.rows - lr0), (const U16 *)a.w + (int64_t)vr * a.ldw,
+                  a.ldw, min(at.more() ? TN : 32 * NARROW, a.V - vr));
+        start(stages, q, KT);
+    };
+    // A 16-wide vocab slab of a wave goes through LDS and leaves as 128-byte runs of G^T.
+    auto write = [&](const auto &acc, auto ni_count, int lr0, int v0, int buf) {
+        constexpr int NI = decltype(ni_count)::value;
         // this lane's rows are 64 wm + 16 mi + 4 g + r; their scores are read again for every
         // slab, as 48 registers of them beside the accumulators spill
         const float *mine = &sRow[buf][0][64 * wm + 4 * g];
         auto slabs = [&](auto whole) {  // whole: every column is a vocabulary entry, every row a row
 #pragma unroll
-            for (int ni = 0; ni < 8; ++ni) {
-                const int vb = v0 + 128 * wn + 16 * ni, v = vb + l16;
+            for (int ni = 0; ni < NI; ++ni) {
+                const int vb = v0 + 16 * NI * wn + 16 * ni, v = vb + l16;
 #pragma unroll
                 for (int mi = 0; mi < 4; ++mi) {
                     const int rl0 = 64 * wm + 16 * mi + 4 * g;
@@ -1898,10 +1892,23 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
                 wave_lds_order();
             }
         };
-        if (v0 + TN <= a.V && lr0 + TM <= p.rows) slabs(std::true_type{});
+        if (v0 + 32 * NI <= a.V && lr0 + TM <= p.rows) slabs(std::true_type{});
         else slabs(std::false_type{});
-        if (!at.more()) return;
+    };
+    load_next(0);
+    int buf = 0;
+    for (; at.more(); buf ^= 1) {
+        floatx4 acc[4][8];
+        product(stages, q, KT, acc);
+        const int lr0 = at.rt * TM, v0 = at.vt * TN;
+        at.next();
+        load_next(buf ^ 1);
+        write(acc, std::integral_constant<int, 8>{}, lr0, v0, buf);
     }
+    if (!last) return;
+    floatx4 acc[4][NARROW];
+    product(stages, q, KT, acc);
+    write(acc, std::integral_constant<int, NARROW>{}, last_rt * TM, last_v0, buf);
 }
 }  // namespace tiles
 
@@ -2243,11 +2250,11 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
     const size_t gsmem = wide_tiles ? wide::KSMEM : big::SMEM;
     auto launch_grad = [&]() {
         if (scores) {
-            const dim3 grid(tiles::grid((p.Vp / tiles::TN) * (p.Rp / tiles::TM)));
-            if (p.write_g)
-                hipLaunchKernelGGL(tiles::scores_grad_kernel<true>, grid, dim3(tiles::TT), 0, stream, p);
-            else
-                hipLaunchKernelGGL(tiles::scores_grad_kernel<false>, grid, dim3(tiles::TT), 0, stream, p);
+            const tiles::Columns cols = tiles::columns(p.rows, p.Vp);
+            p.full_vt = cols.full;
+            auto kernel = p.write_g ? (cols.narrow == 2 ? tiles::scores_grad_kernel<true, 2> : tiles::scores_grad_kernel<true, 4>)
+                                    : (cols.narrow == 2 ? tiles::scores_grad_kernel<false, 2> : tiles::scores_grad_kernel<false, 4>);
+            hipLaunchKernelGGL(kernel, dim3(tiles::grid(cols.n_vt * (p.Rp / tiles::TM))), dim3(tiles::TT), 0, stream, p);
             const int st = launch_status("scores_grad_kernel");
             if (st) return st;
             hipLaunchKernelGGL(scores_token_kernel<U>, dim3((p.rows + THREADS - 1) / THREADS), dim3(THREADS), 0, stream, p);

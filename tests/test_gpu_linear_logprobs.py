@@ -297,3 +297,35 @@ def test_gradients_of_small_tables_and_several_passes(gpu_lib, n, V, D, chunk, d
     dh, dw = torch.autograd.grad([r.logprobs, r.entropy], [hc, wc], [g.cuda() for g in gs])
     _close(dh, R["dh"], R["t_dh"], torch.finfo(dtype).eps)
     _close(dw, R["dw"], R["t_dw"], torch.finfo(dtype).eps)
+
+
+@pytest.mark.parametrize("n,V,D", [(2047, 50261, 32), (4096, 50261, 64), (300, 10000, 96), (129, 700, 64)])
+def test_gradients_of_tiles_that_do_not_fill_their_last_round(gpu_lib, n, V, D):
+    """The gradient's tiles of the same kind, bf16, every row and column: dx rounded to bf16 (2^-8 each)
+    between the products, dh and dw rounded once more."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, gs = (x if isinstance(x, list) else x.cuda() for x in _data(n, V, D, BF16, BF16, 12))
+    gs = [g.cuda() for g in gs]
+    h.requires_grad_(), w.requires_grad_()
+    r = linear_token_logprobs(h, w, ids)
+    dh, dw = torch.autograd.grad([r.logprobs, r.entropy], [h, w], gs)
+    R = _reference(h.detach(), w.detach(), ids, 1.0, [g.double() for g in gs], 2.0 ** -8)
+    for got, k in ((dh, "dh"), (dw, "dw")):
+        _close(got, R[k].cpu(), R["t_" + k].cpu(), torch.finfo(BF16).eps)
+
+
+@pytest.mark.parametrize("n,V,D,chunk", [(300, 700, 64, 4096), (900, 500, 96, 70), (2, 300, 32, 1)])
+def test_hand_written_products(gpu_lib, monkeypatch, n, V, D, chunk):
+    """QPAM_CE_GEMM=hip: G beside G^T, dH and dW by the library's own kernels; a frozen operand's left out."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    monkeypatch.setenv("QPAM_CE_GEMM", "hip")
+    h, w, ids, gs = _data(n, V, D, BF16, BF16, 13)
+    R = _reference(h, w, ids, 1.0, [g.double() for g in gs], 2.0 ** -8)
+    hc, wc = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    for ops in ([hc, wc], [hc, wc.detach()], [hc.detach(), wc]):
+        r = linear_token_logprobs(*ops, ids.cuda(), chunk=chunk)
+        live = [o for o in ops if o.requires_grad]
+        got = torch.autograd.grad([r.logprobs, r.entropy], live, [g.cuda() for g in gs])
+        for o, g in zip(live, got):
+            k = "dh" if o is hc else "dw"
+            _close(g, R[k], R["t_" + k], torch.finfo(BF16).eps)
