@@ -797,7 +797,8 @@ __global__ void __launch_bounds__(TT) gemm_kernel(const float *A, int64_t lda, i
 }
 
 // rows * cols is below 2^24 where there are several ranges; cols % 4 == 0
-__global__ void __launch_bounds__(THREADS) sum_kernel(const float *part, int ranges, int rows, int cols, float *out, int64_t ldo,
+template <typename T>
+__global__ void __launch_bounds__(THREADS) sum_kernel(const float *part, int ranges, int rows, int cols, T *out, int64_t ldo,
                                                       int accumulate) {
     const unsigned n4 = (unsigned)rows * (unsigned)cols / 4, per_row = cols / 4;
     for (unsigned i = blockIdx.x * THREADS + threadIdx.x; i < n4; i += gridDim.x * THREADS) {
@@ -805,9 +806,13 @@ __global__ void __launch_bounds__(THREADS) sum_kernel(const float *part, int ran
 #pragma unroll 4
         for (int z = 1; z < ranges; ++z) x += reinterpret_cast<const floatx4 *>(part)[(int64_t)z * n4 + i];
         const unsigned r = i / per_row;
-        float *to = out + r * ldo + 4 * (i - r * per_row);
+        T *to = out + r * ldo + 4 * (i - r * per_row);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) to[j] = accumulate ? to[j] + x[j] : x[j];
+        for (int j = 0; j < 4; ++j) {
+            const float y = accumulate ? Elem<T>::load(to + j) + x[j] : x[j];
+            if constexpr (sizeof(T) == 2) to[j] = __builtin_bit_cast(unsigned short, (__bf16)y);
+            else to[j] = y;
+        }
     }
 }
 
@@ -1910,6 +1915,115 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
     product(stages, q, KT, acc);
     write(acc, std::integral_constant<int, NARROW>{}, last_rt * TM, last_v0, buf);
 }
+// dH = (G^T)^T W with both operands as they stand, [K][rows] and [K][D]: a stage holds 32 of
+// their rows by 256 columns, its 32-byte pieces swizzled by h(row) so that the eight rows
+// that half a wave's transpose read takes are in distinct banks.  The vocabulary is cut in
+// ranges that fill the CUs (gridDim.z); a range's sums leave in fp32, one range's as bf16.
+// Against 50261 x 768 with the sum: 16 rows 33 us, 200 rows 42, bound by reading W and the
+// partial sums (hipBLASLt, with 20 and 51 blocks: 107 and 197); 16384 rows x 1024 1.45 ms
+// (1.51).
+__device__ __forceinline__ int h_of(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
+
+__global__ void __launch_bounds__(TT) dh_kernel(const U16 *A, int64_t lda, int M, const U16 *B, int64_t ldb, int b_rows, int N, int K,
+                                                int kper, float *part, U16 *out, int64_t ldo) {
+    __shared__ __align__(16) Stage s0, s1, s2, s3;
+    const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN, k0 = blockIdx.z * kper, KT = min(kper, K - k0) / DK;
+    const int w = wave_id(), lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    // a wave's load j: rows 4 w + 2 j and the next, a 16-byte chunk a lane
+    int row[2];
+    unsigned ao[2], bo[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        row[j] = 4 * w + 2 * j + (lane >> 5);
+        const int col = 16 * (((lane >> 1) & 15) ^ h_of(row[j])) + 8 * (lane & 1);
+        ao[j] = 2u * ((unsigned)row[j] * (unsigned)lda + col);
+        bo[j] = 2u * min(col, N - n0 - 8);
+    }
+    const U16 *a0 = A + (int64_t)k0 * lda + m0;
+    auto load = [&](Stage &s, int step) {
+        const int k = k0 + step * DK, b0 = min(k, b_rows - 1);  // past B's rows A is zero: its last row again
+        const char *a = reinterpret_cast<const char *>(a0 + (int64_t)step * DK * lda);
+        const char *b = reinterpret_cast<const char *>(B + (int64_t)b0 * ldb + n0);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            to_lds(a + ao[j], &s.a[(4 * w + 2 * j) * TM]);
+            to_lds(b + (2u * (unsigned)min(row[j], b_rows - 1 - b0) * (unsigned)ldb + bo[j]), &s.b[(4 * w + 2 * j) * TN]);
+        }
+    };
+    // column l16 of a 16-column chunk, k = 8 g ..: rows 8 g + l16 / 4 and four behind it
+    const int frow = 8 * g + (l16 >> 2), at0 = frow * TM + 16 * h_of(frow) + 4 * (l16 & 3);
+    auto fragment = [&](const U16 *s, int base, int c) {  // chunk c, swizzled: c ^ h(row)
+        const U16 *at = s + (base ^ (16 * c));
+        const shortx4 lo = lds_read_tr(at), hi = lds_read_tr(at + 4 * TM);
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    floatx4 acc[4][8];
+#pragma unroll
+    for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 8; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
+    // the stage after this one is in LDS, and every wave is done reading this one
+    auto landed = [&]() {
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(8) & ~0xF00);
+        __builtin_amdgcn_s_barrier();
+        wave_lds_order();
+    };
+    load(s0, 0);
+    load(s1, min(1, KT - 1));
+    load(s2, min(2, KT - 1));
+    landed();
+    auto step = [&](int kt, const Stage &s, Stage &free) {  // stage kt; kt + 3 into the stage that kt - 1 left
+        load(free, min(kt + 3, KT - 1));
+        int base = at0;
+        asm volatile("" : "+v"(base));  // the fragments' addresses are made here: kept over the steps they spill
+        bf16x8 a[4], b[4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (half == 0) a[i] = fragment(s.a, base, 4 * (w >> 1) + i);
+                b[i] = fragment(s.b, base, 8 * (w & 1) + 4 * half + i);
+            }
+#pragma unroll
+            for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+                for (int mi = 0; mi < 4; ++mi)
+                    acc[mi][4 * half + ni] =
+                        __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[mi], b[ni], acc[mi][4 * half + ni], 0, 0, 0);
+        }
+        landed();
+    };
+    int kt = 0;
+    for (; kt + 3 < KT; kt += 4) {
+        step(kt, s0, s3);
+        step(kt + 1, s1, s0);
+        step(kt + 2, s2, s1);
+        step(kt + 3, s3, s2);
+    }
+    if (kt < KT) step(kt, s0, s3);
+    if (kt + 1 < KT) step(kt + 1, s1, s0);
+    if (kt + 2 < KT) step(kt + 2, s2, s1);
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // no direct load outlives the wave
+    const int m1 = m0 + 64 * (w >> 1) + 4 * g, n1 = n0 + 128 * (w & 1) + l16;
+    auto store = [&](auto *to, int64_t ld) {  // to: the lane's first element
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (m1 + 16 * mi + r < M) {
+#pragma unroll
+                    for (int ni = 0; ni < 8; ++ni)
+                        if (n1 + 16 * ni < N) {
+                            if constexpr (sizeof(*to) == 2) to[16 * ni] = __builtin_bit_cast(U16, (__bf16)acc[mi][ni][r]);
+                            else to[16 * ni] = acc[mi][ni][r];
+                        }
+                }
+                to += r < 3 ? ld : 13 * ld;
+            }
+    };
+    if (part) store(part + ((int64_t)blockIdx.z * M + m1) * N + n1, N);
+    else store(out + (int64_t)m1 * ldo + n1, ldo);
+}
 }  // namespace tiles
 
 // Token scores of few rows (a decode step's), bound by reading the table once.  A wave
@@ -2232,6 +2346,25 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     return st;
 }
 
+// The token scores' bf16 dH of a pass: ranges of the vocabulary (at least eight steps, as
+// many as `part` holds sums of) give every CU a block.
+int run_dh(const qpam_ce_bwd_args &a, const BwdParams &p, int r0, float *part, size_t part_bytes, hipStream_t stream) {
+    using U = unsigned short;
+    const int64_t tiles = (int64_t)((p.rows + tiles::TM - 1) / tiles::TM) * ((a.D + tiles::TN - 1) / tiles::TN);
+    const int64_t fit = (int64_t)(part_bytes / ((size_t)p.rows * a.D * sizeof(float)));
+    const int ranges = (int)std::max<int64_t>(1, std::min<int64_t>({256 / tiles, p.Vp / 256, fit}));
+    const int kper = round_up((p.Vp + ranges - 1) / ranges, BK), n_k = (p.Vp + kper - 1) / kper;
+    U *out = (U *)a.dh + (int64_t)r0 * a.lddh;
+    hipLaunchKernelGGL(tiles::dh_kernel, dim3((a.D + tiles::TN - 1) / tiles::TN, (p.rows + tiles::TM - 1) / tiles::TM, n_k),
+                       dim3(tiles::TT), 0, stream, (const U *)p.gtbuf, (int64_t)p.Rp, p.rows, (const U *)a.w, a.ldw, a.V, a.D, p.Vp, kper,
+                       n_k > 1 ? part : nullptr, out, a.lddh);
+    const int st = launch_status("dh_kernel");
+    if (st || n_k == 1) return st;
+    hipLaunchKernelGGL(split::sum_kernel<U>, dim3((unsigned)(((int64_t)p.rows * a.D / 4 + THREADS - 1) / THREADS)), dim3(THREADS), 0,
+                       stream, (const float *)part, n_k, p.rows, a.D, out, a.lddh, 0);
+    return launch_status("sum_kernel");
+}
+
 // dw_write: dW written (beta 0; one pass over the rows) by the library GEMM, in
 // bf16 (dw_out 1) or fp32 (dw_out 2); otherwise added into the fp32 dW
 int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams *scores, bool dw_write = false) {
@@ -2291,6 +2424,11 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
                                      q.dh_part, blas_ws, stream);
             if (st) return st;
             if (!a.dh) continue;
+            if (scores) {
+                st = run_dh(a, p, r0, q.dh_part, blas_ws, stream);
+                if (st) return st;
+                continue;
+            }
             st = blas::gemm_bf16(false, true, a.D, p.rows, a.V, a.w, a.ldw, p.gtbuf, p.Rp, 0.f,
                                  (U *)a.dh + (int64_t)r0 * a.lddh, a.lddh, false, q.dh_part, blas_ws, stream);
             if (st) return st;
@@ -2454,7 +2592,7 @@ int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParam
                            n_k > 1 ? a.D : ldc, (int64_t)M * a.D, n_k > 1 ? 0 : accumulate);
         const int st = launch_status(what);
         if (st || n_k == 1) return st;
-        hipLaunchKernelGGL(split::sum_kernel, dim3((unsigned)(((int64_t)M * a.D / 4 + THREADS - 1) / THREADS)), dim3(THREADS), 0, stream,
+        hipLaunchKernelGGL(split::sum_kernel<float>, dim3((unsigned)(((int64_t)M * a.D / 4 + THREADS - 1) / THREADS)), dim3(THREADS), 0, stream,
                            (const float *)part, n_k, M, a.D, C, ldc, accumulate);
         return launch_status("split sum_kernel");
     };
