@@ -1915,19 +1915,29 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
     product(stages, q, KT, acc);
     write(acc, std::integral_constant<int, NARROW>{}, last_rt * TM, last_v0, buf);
 }
-// dH = (G^T)^T W with both operands as they stand, [K][rows] and [K][D]: a stage holds 32 of
-// their rows by 256 columns, its 32-byte pieces swizzled by h(row) so that the eight rows
-// that half a wave's transpose read takes are in distinct banks.  The vocabulary is cut in
-// ranges that fill the CUs (gridDim.z); a range's sums leave in fp32, one range's as bf16.
-// Against 50261 x 768 with the sum: 16 rows 33 us, 200 rows 42, bound by reading W and the
-// partial sums (hipBLASLt, with 20 and 51 blocks: 107 and 197); 16384 rows x 1024 1.45 ms
-// (1.51).
+// dH = (G^T)^T W (AT) and dW = G^T H, [M][N] = A B with A [K][M] or [M][K] and B [b_rows][N] as
+// they stand (b_rows <= K, A is zero past them).  A stage of an operand whose rows are k
+// holds 32 of them by 256 columns, its 32-byte pieces swizzled by h(row) so that the eight
+// rows that half a wave's transpose read takes are in distinct banks.  K in `ranges` ranges
+// of kper where tiles are few; tiles in the order range, M, N over the XCDs' block ranges, so
+// that those which share operands share an L2.  A range's sums leave in fp32, each in its
+// place of `out`.
+// Against 50261 x 768, dH with the sum: 16 rows 33 us, 200 rows 42, bound by reading W and
+// the partial sums (hipBLASLt, with 20 and 51 blocks: 107 and 197).  16384 rows, 50261 x
+// 1024: both 2.70 ms, 1.25 PFLOP/s (hipBLASLt 3.08).
 __device__ __forceinline__ int h_of(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
 
-__global__ void __launch_bounds__(TT) dh_kernel(const U16 *A, int64_t lda, int M, const U16 *B, int64_t ldb, int b_rows, int N, int K,
-                                                int kper, float *part, U16 *out, int64_t ldo) {
+enum { OUT_BF16, OUT_F32, OUT_ADD };
+
+template <bool AT>
+__global__ void __launch_bounds__(TT) gemm_kernel(const U16 *A, int64_t lda, int M, const U16 *B, int64_t ldb, int b_rows, int N, int K,
+                                                  int kper, int ranges, void *out, int64_t ldo, int64_t range_stride, int mode) {
     __shared__ __align__(16) Stage s0, s1, s2, s3;
-    const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN, k0 = blockIdx.z * kper, KT = min(kper, K - k0) / DK;
+    const int n_ct = (N + TN - 1) / TN, tiles = (M + TM - 1) / TM * n_ct;
+    const int item = big::xcd_item(blockIdx.x, tiles * ranges);
+    if (item >= tiles * ranges) return;
+    const int z = item / tiles, rt = (item - z * tiles) / n_ct, ct = item - z * tiles - rt * n_ct;
+    const int m0 = rt * TM, n0 = ct * TN, k0 = z * kper, KT = min(kper, K - k0) / DK;
     const int w = wave_id(), lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
     // a wave's load j: rows 4 w + 2 j and the next, a 16-byte chunk a lane
     int row[2];
@@ -1936,23 +1946,25 @@ __global__ void __launch_bounds__(TT) dh_kernel(const U16 *A, int64_t lda, int M
     for (int j = 0; j < 2; ++j) {
         row[j] = 4 * w + 2 * j + (lane >> 5);
         const int col = 16 * (((lane >> 1) & 15) ^ h_of(row[j])) + 8 * (lane & 1);
-        ao[j] = 2u * ((unsigned)row[j] * (unsigned)lda + col);
         bo[j] = 2u * min(col, N - n0 - 8);
+        const int arow = 32 * w + 16 * j + (lane >> 2);  // A [M][K]: 16 rows of 64 bytes, every row of a tile in memory
+        ao[j] = AT ? 2u * ((unsigned)row[j] * (unsigned)lda + col) : 2u * (unsigned)arow * (unsigned)lda + 16 * wide::swz(arow, lane & 3);
     }
-    const U16 *a0 = A + (int64_t)k0 * lda + m0;
+    const U16 *a0 = AT ? A + (int64_t)k0 * lda + m0 : A + (int64_t)m0 * lda + k0;
     auto load = [&](Stage &s, int step) {
         const int k = k0 + step * DK, b0 = min(k, b_rows - 1);  // past B's rows A is zero: its last row again
-        const char *a = reinterpret_cast<const char *>(a0 + (int64_t)step * DK * lda);
+        const char *a = reinterpret_cast<const char *>(a0 + (AT ? (int64_t)step * DK * lda : (int64_t)step * DK));
         const char *b = reinterpret_cast<const char *>(B + (int64_t)b0 * ldb + n0);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            to_lds(a + ao[j], &s.a[(4 * w + 2 * j) * TM]);
+            to_lds(a + ao[j], &s.a[AT ? (4 * w + 2 * j) * TM : (32 * w + 16 * j) * DK]);
             to_lds(b + (2u * (unsigned)min(row[j], b_rows - 1 - b0) * (unsigned)ldb + bo[j]), &s.b[(4 * w + 2 * j) * TN]);
         }
     };
     // column l16 of a 16-column chunk, k = 8 g ..: rows 8 g + l16 / 4 and four behind it
     const int frow = 8 * g + (l16 >> 2), at0 = frow * TM + 16 * h_of(frow) + 4 * (l16 & 3);
-    auto fragment = [&](const U16 *s, int base, int c) {  // chunk c, swizzled: c ^ h(row)
+    const int a_at = (64 * (w >> 1) + l16) * DK + 8 * wide::swz(l16, g);
+    auto fragment_t = [&](const U16 *s, int base, int c) {  // chunk c, swizzled: c ^ h(row)
         const U16 *at = s + (base ^ (16 * c));
         const shortx4 lo = lds_read_tr(at), hi = lds_read_tr(at + 4 * TM);
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -1981,8 +1993,8 @@ __global__ void __launch_bounds__(TT) dh_kernel(const U16 *A, int64_t lda, int M
         for (int half = 0; half < 2; ++half) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (half == 0) a[i] = fragment(s.a, base, 4 * (w >> 1) + i);
-                b[i] = fragment(s.b, base, 8 * (w & 1) + 4 * half + i);
+                if (half == 0) a[i] = AT ? fragment_t(s.a, base, 4 * (w >> 1) + i) : fragment(s.a + a_at, i);
+                b[i] = fragment_t(s.b, base, 8 * (w & 1) + 4 * half + i);
             }
 #pragma unroll
             for (int ni = 0; ni < 4; ++ni)
@@ -2005,7 +2017,8 @@ __global__ void __launch_bounds__(TT) dh_kernel(const U16 *A, int64_t lda, int M
     if (kt + 2 < KT) step(kt + 2, s2, s1);
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // no direct load outlives the wave
     const int m1 = m0 + 64 * (w >> 1) + 4 * g, n1 = n0 + 128 * (w & 1) + l16;
-    auto store = [&](auto *to, int64_t ld) {  // to: the lane's first element
+    const int64_t first = z * range_stride + (int64_t)m1 * ldo + n1;
+    auto store = [&](auto *to, auto add) {  // to: the lane's first element
 #pragma unroll
         for (int mi = 0; mi < 4; ++mi)
 #pragma unroll
@@ -2015,14 +2028,15 @@ __global__ void __launch_bounds__(TT) dh_kernel(const U16 *A, int64_t lda, int M
                     for (int ni = 0; ni < 8; ++ni)
                         if (n1 + 16 * ni < N) {
                             if constexpr (sizeof(*to) == 2) to[16 * ni] = __builtin_bit_cast(U16, (__bf16)acc[mi][ni][r]);
-                            else to[16 * ni] = acc[mi][ni][r];
+                            else to[16 * ni] = add ? to[16 * ni] + acc[mi][ni][r] : acc[mi][ni][r];
                         }
                 }
-                to += r < 3 ? ld : 13 * ld;
+                to += r < 3 ? ldo : 13 * ldo;
             }
     };
-    if (part) store(part + ((int64_t)blockIdx.z * M + m1) * N + n1, N);
-    else store(out + (int64_t)m1 * ldo + n1, ldo);
+    if (mode == OUT_BF16) store(static_cast<U16 *>(out) + first, std::false_type{});
+    else if (mode == OUT_F32) store(static_cast<float *>(out) + first, std::false_type{});
+    else store(static_cast<float *>(out) + first, std::true_type{});
 }
 }  // namespace tiles
 
@@ -2346,22 +2360,57 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     return st;
 }
 
-// The token scores' bf16 dH of a pass: ranges of the vocabulary (at least eight steps, as
-// many as `part` holds sums of) give every CU a block.
-int run_dh(const qpam_ce_bwd_args &a, const BwdParams &p, int r0, float *part, size_t part_bytes, hipStream_t stream) {
+// Ranges of K (up to `most`, at least eight steps each) for a product whose tiles leave CUs
+// idle: a step takes `step_us`; the ranges' fp32 sums of `outputs` values are written and read
+// again at 5 MB a us, by a launch more (4 us).
+int best_ranges(int64_t most, int K, double step_us, int64_t outputs) {
+    most = std::min<int64_t>(most, K / 256);
+    int best = 1;
+    double least = K / BK * step_us;
+    for (int r = 2; r <= most; ++r) {
+        const double us = (double)K / BK / r * step_us + 4 + 8e-6 / 5 * outputs * r;
+        if (us < least) {
+            best = r;
+            least = us;
+        }
+    }
+    return best;
+}
+
+// [M][N] = A B of tiles::gemm_kernel.  Row tiles that fill whole rounds of the 256 CUs in one
+// launch; the rest, if they leave half the CUs idle, with K in ranges (as many as `part` holds
+// sums of).
+template <bool AT>
+int scores_gemm(const unsigned short *A, int64_t lda, int M, const unsigned short *B, int64_t ldb, int b_rows, int N, int K, void *out,
+                int64_t ldo, int mode, float *part, size_t part_bytes, hipStream_t stream) {
     using U = unsigned short;
-    const int64_t tiles = (int64_t)((p.rows + tiles::TM - 1) / tiles::TM) * ((a.D + tiles::TN - 1) / tiles::TN);
-    const int64_t fit = (int64_t)(part_bytes / ((size_t)p.rows * a.D * sizeof(float)));
-    const int ranges = (int)std::max<int64_t>(1, std::min<int64_t>({256 / tiles, p.Vp / 256, fit}));
-    const int kper = round_up((p.Vp + ranges - 1) / ranges, BK), n_k = (p.Vp + kper - 1) / kper;
-    U *out = (U *)a.dh + (int64_t)r0 * a.lddh;
-    hipLaunchKernelGGL(tiles::dh_kernel, dim3((a.D + tiles::TN - 1) / tiles::TN, (p.rows + tiles::TM - 1) / tiles::TM, n_k),
-                       dim3(tiles::TT), 0, stream, (const U *)p.gtbuf, (int64_t)p.Rp, p.rows, (const U *)a.w, a.ldw, a.V, a.D, p.Vp, kper,
-                       n_k > 1 ? part : nullptr, out, a.lddh);
-    const int st = launch_status("dh_kernel");
-    if (st || n_k == 1) return st;
-    hipLaunchKernelGGL(split::sum_kernel<U>, dim3((unsigned)(((int64_t)p.rows * a.D / 4 + THREADS - 1) / THREADS)), dim3(THREADS), 0,
-                       stream, (const float *)part, n_k, p.rows, a.D, out, a.lddh, 0);
+    auto launch = [&](int m0, int m, int ranges, int kper, void *to, int64_t ld, int how) {
+        const int tiles = ((m + tiles::TM - 1) / tiles::TM) * ((N + tiles::TN - 1) / tiles::TN);
+        hipLaunchKernelGGL(tiles::gemm_kernel<AT>, dim3(big::xcd_grid(tiles * ranges)), dim3(tiles::TT), 0, stream,
+                           AT ? A + m0 : A + (int64_t)m0 * lda, lda, m, B, ldb, b_rows, N, K, kper, ranges, to, ld,
+                           ranges > 1 ? (int64_t)m * ld : 0, how);
+        return launch_status("tiles gemm_kernel");
+    };
+    auto at = [&](int m) { return static_cast<char *>(out) + (int64_t)m * ldo * (mode == tiles::OUT_BF16 ? 2 : 4); };
+    const int64_t n_rt = (M + tiles::TM - 1) / tiles::TM, n_ct = (N + tiles::TN - 1) / tiles::TN;
+    const int full = (int)(n_rt * n_ct / 256 * 256 / n_ct), m0 = full * tiles::TM, rest = M - m0;
+    int ranges = 1;
+    if (rest > 0) {
+        const int64_t fit = (int64_t)(part_bytes / ((size_t)rest * N * sizeof(float)));
+        ranges = best_ranges(std::min(256 / ((n_rt - full) * n_ct), fit), K, 0.95, (int64_t)rest * N);
+    }
+    if (ranges == 1) return launch(0, M, 1, K, out, ldo, mode);
+    int st = full > 0 ? launch(0, m0, 1, K, out, ldo, mode) : QPAM_OK;
+    if (st) return st;
+    const int kper = round_up((K + ranges - 1) / ranges, BK), n_k = (K + kper - 1) / kper;
+    if (n_k == 1) return launch(m0, rest, 1, K, at(m0), ldo, mode);
+    if ((st = launch(m0, rest, n_k, kper, part, N, tiles::OUT_F32))) return st;
+    const dim3 grid((unsigned)(((int64_t)rest * N / 4 + THREADS - 1) / THREADS));
+    if (mode == tiles::OUT_BF16)
+        hipLaunchKernelGGL(split::sum_kernel<U>, grid, dim3(THREADS), 0, stream, (const float *)part, n_k, rest, N, (U *)at(m0), ldo, 0);
+    else
+        hipLaunchKernelGGL(split::sum_kernel<float>, grid, dim3(THREADS), 0, stream, (const float *)part, n_k, rest, N, (float *)at(m0),
+                           ldo, mode == tiles::OUT_ADD ? 1 : 0);
     return launch_status("sum_kernel");
 }
 
@@ -2418,17 +2467,25 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
             p.Rp = round_up(p.rows, big::BTM);
             int st = launch_grad();
             if (st) return st;
+            if (scores) {
+                const U *h = (const U *)a.h + (int64_t)r0 * a.ldh, *gt = (const U *)p.gtbuf;
+                const int how = !dw_write ? tiles::OUT_ADD : a.dw_out == 1 ? tiles::OUT_BF16 : tiles::OUT_F32;
+                if (a.dw)
+                    st = scores_gemm<false>(gt, p.Rp, a.V, h, a.ldh, p.rows, a.D, round_up(p.rows, BK), a.dw, a.lddw, how, q.dh_part,
+                                            blas_ws, stream);
+                if (st) return st;
+                if (a.dh)
+                    st = scores_gemm<true>(gt, p.Rp, p.rows, (const U *)a.w, a.ldw, a.V, a.D, p.Vp, (U *)a.dh + (int64_t)r0 * a.lddh,
+                                           a.lddh, tiles::OUT_BF16, q.dh_part, blas_ws, stream);
+                if (st) return st;
+                continue;
+            }
             if (a.dw)
                 st = blas::gemm_bf16(false, false, a.D, a.V, p.rows, (const U *)a.h + (int64_t)r0 * a.ldh, a.ldh,
                                      p.gtbuf, p.Rp, dw_write ? 0.f : 1.f, a.dw, a.lddw, !(dw_write && a.dw_out == 1),
                                      q.dh_part, blas_ws, stream);
             if (st) return st;
             if (!a.dh) continue;
-            if (scores) {
-                st = run_dh(a, p, r0, q.dh_part, blas_ws, stream);
-                if (st) return st;
-                continue;
-            }
             st = blas::gemm_bf16(false, true, a.D, p.rows, a.V, a.w, a.ldw, p.gtbuf, p.Rp, 0.f,
                                  (U *)a.dh + (int64_t)r0 * a.lddh, a.lddh, false, q.dh_part, blas_ws, stream);
             if (st) return st;
@@ -2552,11 +2609,10 @@ int validate_common(int N, int V, int D, int dtype, const void *h, int64_t ldh, 
     return QPAM_OK;
 }
 
-// Ranges of the K axis that share an [M][D] product of the token scores' fp32 backward: a
-// block for each of the 256 CUs, at most 16 ranges and none below 256 (eight steps).
+// Ranges of the K axis that share an [M][D] product of the token scores' fp32 backward
 int k_ranges(int M, int D, int K) {
     const int64_t tiles = (int64_t)((M + split::TM - 1) / split::TM) * ((D + split::TN - 1) / split::TN);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({256 / tiles, K / 256, 16}));
+    return best_ranges(std::min<int64_t>(256 / tiles, 16), K, 1.9, (int64_t)M * D);
 }
 // ... and what their partial sums take at most: 16 ranges of M rows, or 256 tiles
 int64_t k_ranges_part(int64_t M, int D) { return std::min<int64_t>(16 * M * D, 256ll * split::TM * split::TN); }
