@@ -1924,7 +1924,7 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
 // place of `out`.
 // Against 50261 x 768, dH with the sum: 16 rows 33 us, 200 rows 42, bound by reading W and
 // the partial sums (hipBLASLt, with 20 and 51 blocks: 107 and 197).  16384 rows, 50261 x
-// 1024: both 2.70 ms, 1.25 PFLOP/s (hipBLASLt 3.08).
+// 1024: 1.40 ms each, 1.20 PFLOP/s (hipBLASLt 1.51 and 1.60).
 __device__ __forceinline__ int h_of(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
 
 enum { OUT_BF16, OUT_F32, OUT_ADD };
