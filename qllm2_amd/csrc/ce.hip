@@ -394,7 +394,7 @@ __device__ __forceinline__ RowScore row_score(const BwdParams &p, int lr) {
     return {p.stats[2 * row], k * (g_lp + g_ent * (p.entropy[row] - LN2 * log2f(s))), k * g_ent * LN2};
 }
 
-// G at the rows' tokens, where the tiles left out the one-hot term: with p = e^logprob
+// G^T at the rows' tokens, where the tiles left out the one-hot term: with p = e^logprob
 //   G = (g_lp (1 - p) - g_ent p (logprob + entropy)) / T.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) scores_token_kernel(BwdParams p) {
@@ -410,7 +410,6 @@ __global__ void __launch_bounds__(THREADS) scores_token_kernel(BwdParams p) {
     if constexpr (sizeof(T) == 2) v = __builtin_bit_cast(unsigned short, (__bf16)x);
     else v = x;
     static_cast<T *>(p.gtbuf)[id * p.Rp + lr] = v;
-    if (p.write_g) static_cast<T *>(p.gbuf)[(int64_t)lr * p.Vp + id] = v;
 }
 
 // out[c][r] = in[r][c] for an R x Cc tile grid (64 x 64 LDS tiles); rows >= R
@@ -1819,9 +1818,9 @@ __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
     reduce_rows(p, acc, last_rt * TM, last_v0, p.full_vt + last_ct, sB, sS, sT);
 }
 
-// G^T [Vp][Rp] (and G [rows][Vp] with WRITE_G) without the tokens' one-hot terms; zero past
-// the vocabulary and past the rows.  Tiles as in the scores' kernel.
-template <bool WRITE_G, int NARROW>
+// G^T [Vp][Rp] without the tokens' one-hot terms; zero past the vocabulary and past the rows.
+// Tiles as in the scores' kernel.
+template <int NARROW>
 __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
     constexpr int LD = 72;  // bf16 per staged vocab row: 64 tile rows + padding against bank conflicts
     __shared__ __align__(16) Stage s0, s1, s2, s3;
@@ -1835,7 +1834,6 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
     Walk at(n_rt, p.full_vt);
     const bool last = (int)blockIdx.x < n_rt * ((p.Vp - p.full_vt * TN) / (32 * NARROW));
     const int last_rt = blockIdx.x % n_rt, last_v0 = p.full_vt * TN + 32 * NARROW * (blockIdx.x / n_rt);
-    U16 *G = (U16 *)p.gbuf;
     U16 *GT = (U16 *)p.gtbuf;
     U16 *slab = sSlab + w * 16 * LD;
     // a slab's way out in two stores of eight whole 128-byte lines: vocab rows lane / 8 and
@@ -1881,12 +1879,6 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
                         if (!whole && (v >= a.V || lr0 + rl0 + r >= p.rows)) x[r] = 0.f;
                     }
                     const unsigned lo = pack_bf16x2(x[0], x[1]), hi = pack_bf16x2(x[2], x[3]);
-                    if constexpr (WRITE_G) {
-                        const U16 gb[4] = {(U16)(lo & 0xFFFFu), (U16)(lo >> 16), (U16)(hi & 0xFFFFu), (U16)(hi >> 16)};
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (lr0 + rl0 + r < p.rows) G[(int64_t)(lr0 + rl0 + r) * p.Vp + v] = gb[r];
-                    }
                     *reinterpret_cast<uint2 *>(slab + l16 * LD + 16 * mi + 4 * g) = make_uint2(lo, hi);
                 }
                 wave_lds_order();  // the slab is this wave's own, and a wave's LDS accesses stay in order
@@ -2229,7 +2221,7 @@ size_t fwd_ws(const qpam_ce_fwd_args &a) {
 
 // Rows of one backward pass.  The reference keeps the fp32 logits and softmax of
 // `chunk` rows alive (8 bytes per row and vocabulary entry); a pass here covers
-// as many rows as fit those bytes: bf16 G^T alone (library GEMMs) takes 2 bytes,
+// as many rows as fit those bytes: bf16 G^T alone (library GEMMs, scores) takes 2 bytes,
 // bf16 G and G^T (hand-written GEMMs) 4 bytes, fp32 G and G^T 8 bytes.
 int pass_rows(const qpam_ce_bwd_args &a) {
     const int64_t factor = a.dtype == QPAM_BF16 ? (blas::enabled() ? 4 : 2) : 1;
@@ -2290,12 +2282,16 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     if (scores) p = *scores;
     p.a = a;
     const bool few = scores && a.N <= thin::ROWS;
-    const bool wide_tiles = is_bf<T>() && (scores || use_wide(a.D));  // the direct-load loop takes any multiple of 32
+    const bool wide_tiles = is_bf<T>() && use_wide(a.D);
     const tiles::Columns cols = tiles::columns(a.N, a.V);
     const bool score_tiles = scores && is_bf<T>() && !few;
     const bool small = scores && !is_bf<T>() && !few && split::small_tiles(a.N, a.V);
     p.full_vt = cols.full;
-    p.n_vt = few ? thin::blocks(a.V) : score_tiles ? cols.n_vt : small ? (a.V + split::tn<2>() - 1) / split::tn<2>() : wide_tiles ? (a.V + wide::TN - 1) / wide::TN : (a.V + vocab_tile<T>() - 1) / vocab_tile<T>();
+    auto tiles_of = [&](int width) { return (a.V + width - 1) / width; };
+    if (few) p.n_vt = thin::blocks(a.V);
+    else if (score_tiles) p.n_vt = cols.n_vt;
+    else if (small) p.n_vt = tiles_of(split::tn<2>());
+    else p.n_vt = tiles_of(wide_tiles ? wide::TN : vocab_tile<T>());
     char *ws = (char *)a.workspace;
     const int64_t cnt = (int64_t)a.N * p.n_vt;
     p.part_m = (float *)ws;
@@ -2425,7 +2421,7 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
     p.Vp = round_up(a.V, vocab_pad<U>());
     const int chunk = pass_rows(a);
     const int Rmax = round_up(chunk, big::BTM);
-    const bool wide_tiles = scores || use_wide(a.D);
+    const bool wide_tiles = use_wide(a.D);
     // the G-tile kernel: 256 x 256 tiles, or 256 x 128 for hidden sizes that are not
     // a multiple of 64 (Vp and Rp are multiples of both)
     const void *gkern = wide_tiles ? (const void *)wide::grad_tile_kernel : (const void *)big::grad_tile_kernel;
@@ -2434,8 +2430,7 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
         if (scores) {
             const tiles::Columns cols = tiles::columns(p.rows, p.Vp);
             p.full_vt = cols.full;
-            auto kernel = p.write_g ? (cols.narrow == 2 ? tiles::scores_grad_kernel<true, 2> : tiles::scores_grad_kernel<true, 4>)
-                                    : (cols.narrow == 2 ? tiles::scores_grad_kernel<false, 2> : tiles::scores_grad_kernel<false, 4>);
+            auto kernel = cols.narrow == 2 ? tiles::scores_grad_kernel<2> : tiles::scores_grad_kernel<4>;
             hipLaunchKernelGGL(kernel, dim3(tiles::grid(cols.n_vt * (p.Rp / tiles::TM))), dim3(tiles::TT), 0, stream, p);
             const int st = launch_status("scores_grad_kernel");
             if (st) return st;
@@ -2451,11 +2446,11 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
     };
     U *ws = (U *)a.workspace;
     const size_t smem = big::SMEM;
-    if (blas::enabled()) {
+    if (scores || blas::enabled()) {
         p.wt = p.gbuf = p.ht = nullptr;
         p.gtbuf = ws;
         q.dh_part = (float *)(((uintptr_t)(ws + (int64_t)p.Vp * Rmax) + 255) & ~(uintptr_t)255);
-        // G^T [Vp][Rp] from the fused grad tiles, then two library GEMMs (column-major views):
+        // G^T [Vp][Rp] from the fused grad tiles, then (the loss) two library GEMMs (column-major views):
         //   dW^T[D][V] += H^T G^T-view   (m = D, n = V, k = rows)
         //   dH^T[D][rows] = W^T G-view   (m = D, n = rows, k = V)
         p.write_g = 0;
@@ -2480,12 +2475,10 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
                 if (st) return st;
                 continue;
             }
-            if (a.dw)
-                st = blas::gemm_bf16(false, false, a.D, a.V, p.rows, (const U *)a.h + (int64_t)r0 * a.ldh, a.ldh,
-                                     p.gtbuf, p.Rp, dw_write ? 0.f : 1.f, a.dw, a.lddw, !(dw_write && a.dw_out == 1),
-                                     q.dh_part, blas_ws, stream);
+            st = blas::gemm_bf16(false, false, a.D, a.V, p.rows, (const U *)a.h + (int64_t)r0 * a.ldh, a.ldh,
+                                 p.gtbuf, p.Rp, dw_write ? 0.f : 1.f, a.dw, a.lddw, !(dw_write && a.dw_out == 1),
+                                 q.dh_part, blas_ws, stream);
             if (st) return st;
-            if (!a.dh) continue;
             st = blas::gemm_bf16(false, true, a.D, p.rows, a.V, a.w, a.ldw, p.gtbuf, p.Rp, 0.f,
                                  (U *)a.dh + (int64_t)r0 * a.lddh, a.lddh, false, q.dh_part, blas_ws, stream);
             if (st) return st;
@@ -2524,12 +2517,9 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
         st = launch_grad();
         if (st) return st;
         q.dh_ntiles_m = (p.rows + big::BTM - 1) / big::BTM;
-        if (a.dw) {
-            hipLaunchKernelGGL(big::dw_gemm_kernel, dim3(big::xcd_grid(q.n_dw)), dim3(THREADS), smem, stream, q);
-            st = launch_status("ce dw_gemm_kernel (bf16)");
-            if (st) return st;
-        }
-        if (!a.dh) continue;
+        hipLaunchKernelGGL(big::dw_gemm_kernel, dim3(big::xcd_grid(q.n_dw)), dim3(THREADS), smem, stream, q);
+        st = launch_status("ce dw_gemm_kernel (bf16)");
+        if (st) return st;
         hipLaunchKernelGGL(big::dh_gemm_kernel, dim3(big::xcd_grid(q.splits * q.dh_ntiles_m * q.dh_ntiles_n)),
                            dim3(THREADS), smem, stream, q);
         st = launch_status("ce dh_gemm_kernel (bf16)");
@@ -2633,11 +2623,9 @@ size_t scores_f32_ws(const qpam_ce_bwd_args &a) {
 int run_scores_f32(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams &scores) {
     BwdParams p = scores;
     p.a = a;
-    p.write_g = 0;
     p.Vp = round_up(a.V, split::TN);
     const int chunk = scores_f32_rows(a);
     float *gt = (float *)a.workspace, *part = gt + (int64_t)p.Vp * round_up(chunk, split::TM);
-    p.gbuf = nullptr;
     p.gtbuf = gt;
     // C [M][D] (+)= A B, in ranges of K where the tiles alone leave CUs idle
     auto gemm = [&](auto kernel, const char *what, int M, const float *B, int64_t ldb, int b_rows, int K, float *C, int64_t ldc,

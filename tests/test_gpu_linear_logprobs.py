@@ -316,7 +316,7 @@ def test_gradients_of_tiles_that_do_not_fill_their_last_round(gpu_lib, n, V, D):
 
 @pytest.mark.parametrize("n,V,D,chunk", [(300, 700, 64, 4096), (900, 500, 96, 70), (2, 300, 32, 1)])
 def test_hand_written_products(gpu_lib, monkeypatch, n, V, D, chunk):
-    """QPAM_CE_GEMM=hip: G beside G^T, dH and dW by the library's own kernels; a frozen operand's left out."""
+    """QPAM_CE_GEMM=hip changes the passes and their workspace; a frozen operand's product is left out."""
     from qllm2_amd.token_logprobs import linear_token_logprobs
     monkeypatch.setenv("QPAM_CE_GEMM", "hip")
     h, w, ids, gs = _data(n, V, D, BF16, BF16, 13)
