@@ -20,12 +20,13 @@
 // rows, the reference's own memory bound (it keeps chunk x V fp32 logits and
 // softmax alive).
 //
-// Token scores (SCORES variants of the same kernels; qpam_linear_logprobs_*): the
-// log probability of each row's token and the entropy of the row.  With c = log2(e) / T,
+// Token scores (qpam_linear_logprobs_*; namespaces split for fp32, tiles for bf16, thin
+// for few rows, with products of their own): the log probability of each row's token and
+// the entropy of the row.  With c = log2(e) / T,
 // b = c max x rounded and u = c x - b (one fma, so b's rounding shifts every u alike and
 // cancels), the tiles reduce s = sum 2^u and t = sum 2^u u, so that
 //   log prob = ln2 (u_token - log2 s),   entropy = ln2 (log2 s - t / s),
-// and the gradient tiles write
+// and the gradient tiles write (as G^T alone)
 //   G_v = -p_v / T (g_lp + g_ent (ln p_v + entropy)) + [v = token] g_lp / T.
 // Logits with |c x| past fp32's range give NaN.
 #include <algorithm>
