@@ -26,6 +26,7 @@
 // b = c max x rounded and u = c x - b (one fma, so b's rounding shifts every u alike and
 // cancels), the tiles reduce s = sum 2^u and t = sum 2^u u, so that
 //   log prob = ln2 (u_token - log2 s),   entropy = ln2 (log2 s - t / s),
+// with the token's logit from the same accumulators (the tile that holds its column keeps it),
 // and the gradient tiles write (as G^T alone)
 //   G_v = -p_v / T (g_lp + g_ent (ln p_v + entropy)) + [v = token] g_lp / T.
 // Logits with |c x| past fp32's range give NaN.
@@ -161,8 +162,27 @@ struct FwdParams {
     float *part_t;           // [N][n_vt] sum of 2^u u, in part_i's place
     int full_vt;             // vocab tiles of 256 columns in front of the narrow ones (tiles::Columns)
     float c;                 // log2(e) / T
+    float *token_x;          // [N] the logit of the row's token, as the tiles' sums have it
     float *logprobs, *entropy, *stats;
 };
+
+// the row's token, or -1: none, or no such row
+__device__ __forceinline__ int token_of(const FwdParams &p, int64_t id) {
+    return id != p.a.ignore_index && id >= 0 && id < p.a.V ? (int)id : -1;
+}
+__device__ __forceinline__ int row_token(const FwdParams &p, int row) { return row < p.a.N ? token_of(p, p.a.targets[row]) : -1; }
+
+// A lane's logits of one row, in columns v, v + 16, ..: the token's, if it is one of them, is
+// what the row's maximum and sums hold, so its log probability is at most 0.
+template <int NI> __device__ __forceinline__ void keep_token(const FwdParams &p, const floatx4 (&x)[NI], int r, int row, int token, int v) {
+    const unsigned at = (unsigned)(token - v);  // past 2^31 where there is none
+    if (at < 16u * NI && at % 16 == 0) {
+        float y = x[0][r];
+#pragma unroll
+        for (int ni = 1; ni < NI; ++ni) y = at == 16u * ni ? x[ni][r] : y;
+        p.token_x[row] = y;
+    }
+}
 
 // (b, s, t) of two parts of a row's logits as one (b = -inf: a part of nothing)
 __device__ __forceinline__ void join_scores(float &b, float &s, float &t, float ob, float os, float ot) {
@@ -286,15 +306,13 @@ __global__ void __launch_bounds__(THREADS) ce_fwd_finalize_kernel(FwdParams p) {
     }
 }
 
-// one wave per row: merge the vocab tiles into (b, s, t), add the token's logit
-template <typename T>
+// one wave per row: merge the vocab tiles into (b, s, t), add the token's logit.  Neither
+// a log probability above 0 nor an entropy below it is left by the last roundings.
 __global__ void __launch_bounds__(THREADS) scores_finalize_kernel(FwdParams p) {
     const qpam_ce_fwd_args &a = p.a;
     const int lane = threadIdx.x & 63;
     const int row = blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6);
     if (row >= a.N) return;
-    const int64_t id = a.targets[row];
-    const bool valid = id != a.ignore_index && id >= 0 && id < a.V;
     float b = -INFINITY, s = 0.f, t = 0.f;
     for (int vt = lane; vt < p.n_vt; vt += 64) {
         const int64_t o = (int64_t)row * p.n_vt + vt;
@@ -303,24 +321,12 @@ __global__ void __launch_bounds__(THREADS) scores_finalize_kernel(FwdParams p) {
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1)
         join_scores(b, s, t, __shfl_xor(b, off), __shfl_xor(s, off), __shfl_xor(t, off));
-    float dot = 0.f;
-    if (valid) {
-        constexpr int E = 16 / sizeof(T);  // rows are 16-byte aligned and whole vectors long
-        const uintx4 *hr = reinterpret_cast<const uintx4 *>((const T *)a.h + (int64_t)row * a.ldh);
-        const uintx4 *wr = reinterpret_cast<const uintx4 *>((const T *)a.w + id * a.ldw);
-        for (int k = lane; k < a.D / E; k += 64) {
-            const uintx4 hv = hr[k], wv = wr[k];
-            const T *he = reinterpret_cast<const T *>(&hv), *we = reinterpret_cast<const T *>(&wv);
-#pragma unroll
-            for (int i = 0; i < E; ++i) dot += Elem<T>::load(he + i) * Elem<T>::load(we + i);
-        }
-    }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) dot += __shfl_xor(dot, off);
     if (lane == 0) {
-        const float log_s = log2f(s);
-        p.logprobs[row] = valid ? LN2 * (__builtin_fmaf(dot, p.c, -b) - log_s) : 0.f;
-        p.entropy[row] = LN2 * (log_s - t / s);
+        const float log_s = log2f(s), ent = LN2 * (log_s - t / s);
+        float lp = 0.f;
+        if (row_token(p, row) >= 0) lp = LN2 * (__builtin_fmaf(p.token_x[row], p.c, -b) - log_s);
+        p.logprobs[row] = lp > 0.f ? 0.f : lp;
+        p.entropy[row] = ent < 0.f ? 0.f : ent;
         p.stats[2 * row] = b;
         p.stats[2 * row + 1] = s;
     }
@@ -679,17 +685,21 @@ __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
     constexpr int TM = tm<S>(), TN = tn<S>();
     __shared__ __align__(16) U16 s0[3 * plane<S, false, false>()], s1[3 * plane<S, false, false>()];
     __shared__ float sB[2][TM], sS[2][TM], sT[2][TM];
+    __shared__ __align__(16) int sToken[TM];
     const qpam_ce_fwd_args &a = p.a;
     const int vt = blockIdx.x, r0 = blockIdx.y * TM, v0 = vt * TN;
+    if (threadIdx.x < TM) sToken[threadIdx.x] = row_token(p, r0 + threadIdx.x);
     floatx4 acc[S][S];
     tile<S, false, false>((const float *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0),
                           (const float *)a.w + (int64_t)v0 * a.ldw, a.ldw, min(TN, a.V - v0), 0, a.D, acc, s0, s1);
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1, vl = v0 + 16 * S * wn + l16;
 #pragma unroll
-    for (int mi = 0; mi < S; ++mi)
+    for (int mi = 0; mi < S; ++mi) {
+        const intx4 token = *reinterpret_cast<const intx4 *>(&sToken[16 * S * wm + 16 * mi + 4 * g]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
+            keep_token(p, acc[mi], r, r0 + 16 * S * wm + 16 * mi + 4 * g + r, token[r], vl);
             float mx = -INFINITY;
 #pragma unroll
             for (int ni = 0; ni < S; ++ni)
@@ -712,6 +722,7 @@ __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
                 sT[wn][row] = t;
             }
         }
+    }
     __syncthreads();
     if (tid < TM && r0 + tid < a.N) {
         float b = sB[0][tid], s = sS[0][tid], t = sT[0][tid];
@@ -1714,17 +1725,33 @@ __device__ __forceinline__ void block_lds_sync() {
     wave_lds_order();
 }
 
+// The tokens of a tile's rows, and the rows (a bit each, 64 a word) whose token is one of its
+// columns: about one row of the 256 where tokens are spread, so most groups of 16 rows skip
+// the search for it (searched for in every group the scores take 2 % longer).
+struct Tokens {
+    int of[TM];
+    uint64_t here[TM / 64];
+};
+
 // A tile's (b, s, t) per row: over each wave's columns from v0 on, then the two waves of a row.
 template <int NI>
 __device__ __forceinline__ void reduce_rows(const FwdParams &p, const floatx4 (&acc)[4][NI], int r0, int v0, int vt,
-                                            float (&sB)[2][TM], float (&sS)[2][TM], float (&sT)[2][TM]) {
+                                            float (&sB)[2][TM], float (&sS)[2][TM], float (&sT)[2][TM], const Tokens &tokens) {
     const qpam_ce_fwd_args &a = p.a;
     const int tid = threadIdx.x, w = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
     const int vl = v0 + 16 * NI * wn + l16;  // this lane's column in tile ni: vl + 16 ni
+    wave_lds_order();                        // the tokens, written in front of the product's barriers
+    const uint64_t here = tokens.here[wm];
+    const uint32_t here_lo = __builtin_amdgcn_readfirstlane((int)here), here_hi = __builtin_amdgcn_readfirstlane((int)(here >> 32));
     auto rows = [&](auto whole) {            // whole: no column past the vocabulary
 #pragma unroll
         for (int mi = 0; mi < 4; ++mi) {
+            if (((mi < 2 ? here_lo : here_hi) >> (16 * (mi & 1))) & 0xFFFF) {
+                const intx4 token = *reinterpret_cast<const intx4 *>(&tokens.of[64 * wm + 16 * mi + 4 * g]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) keep_token(p, acc[mi], r, r0 + 64 * wm + 16 * mi + 4 * g + r, token[r], vl);
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 float mx = -INFINITY;
@@ -1785,38 +1812,54 @@ template <int NARROW>
 __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
     __shared__ __align__(16) Stage s0, s1, s2, s3;
     __shared__ float sB[2][TM], sS[2][TM], sT[2][TM];
+    __shared__ __align__(16) Tokens sTokens[2];  // of this tile and the next
     const qpam_ce_fwd_args &a = p.a;
     const Stages stages{s0, s1, s2, s3};
-    const int KT = a.D / DK, n_rt = (a.N + TM - 1) / TM;
+    const int KT = a.D / DK, n_rt = (a.N + TM - 1) / TM, tid = threadIdx.x;
     Walk at(n_rt, p.full_vt);
     const bool last = (int)blockIdx.x < n_rt * (p.n_vt - p.full_vt);
     const int last_rt = blockIdx.x % n_rt, last_ct = blockIdx.x / n_rt;
     const int last_v0 = p.full_vt * TN + 32 * NARROW * last_ct;
-    auto operands = [&](int rt, int v0, int cols) {
-        const int r0 = rt * TM;
-        return loads((const U16 *)a.h + (int64_t)r0 * a.ldh, a.ldh, min(TM, a.N - r0), (const U16 *)a.w + (int64_t)v0 * a.ldw,
-                     a.ldw, min(cols, a.V - v0));
-    };
     Loads q;
+    struct Place {
+        int r0, v0, cols;
+    };
+    auto place = [&]() { return at.more() ? Place{at.rt * TM, at.vt * TN, TN} : Place{last_rt * TM, last_v0, 32 * NARROW}; };
     auto load_next = [&]() {
-        if (at.more()) q = operands(at.rt, at.vt * TN, TN);
-        else if (last) q = operands(last_rt, last_v0, 32 * NARROW);
-        else return;
+        if (!at.more() && !last) return;
+        const Place t = place();
+        q = loads((const U16 *)a.h + (int64_t)t.r0 * a.ldh, a.ldh, min(TM, a.N - t.r0), (const U16 *)a.w + (int64_t)t.v0 * a.ldw,
+                  a.ldw, min(t.cols, a.V - t.v0));
         start(stages, q, KT);
     };
+    // the id of this thread's row in the tile at place(), loaded in front of the product before it
+    auto load_id = [&]() { return a.targets[min(place().r0 + (tid & (TM - 1)), a.N - 1)]; };
+    auto put_tokens = [&](int64_t id, int buf) {
+        if (tid >= TM) return;
+        const Place t = place();
+        const int token = t.r0 + tid < a.N ? token_of(p, id) : -1;
+        const uint64_t here = __ballot(token >= t.v0 && token - t.v0 < t.cols);
+        sTokens[buf].of[tid] = token;
+        if ((tid & 63) == 0) sTokens[buf].here[wave_id()] = here;
+    };
+    put_tokens(load_id(), 0);
     load_next();
+    int buf = 0;
     while (at.more()) {
-        floatx4 acc[4][8];
-        product(stages, q, KT, acc);
         const int rt = at.rt, vt = at.vt;
         at.next();
+        const int64_t id = load_id();
+        floatx4 acc[4][8];
+        product(stages, q, KT, acc);
+        put_tokens(id, buf ^ 1);
         load_next();
-        reduce_rows(p, acc, rt * TM, vt * TN, vt, sB, sS, sT);
+        reduce_rows(p, acc, rt * TM, vt * TN, vt, sB, sS, sT, sTokens[buf]);
+        buf ^= 1;
     }
     if (!last) return;
     floatx4 acc[4][NARROW];
     product(stages, q, KT, acc);
-    reduce_rows(p, acc, last_rt * TM, last_v0, p.full_vt + last_ct, sB, sS, sT);
+    reduce_rows(p, acc, last_rt * TM, last_v0, p.full_vt + last_ct, sB, sS, sT, sTokens[buf]);
 }
 
 // G^T [Vp][Rp] without the tokens' one-hot terms; zero past the vocabulary and past the rows.
@@ -2073,6 +2116,9 @@ __global__ void __launch_bounds__(64 * NW) scores_kernel(FwdParams p) {
     const qpam_ce_fwd_args &a = p.a;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int v0 = (blockIdx.x * NW + w) * 16;
+    int token[MI];  // of the lane's hidden rows
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) token[mi] = row_token(p, 16 * mi + l16);
     const int bytes = a.D * (int)sizeof(T), steps = bytes / 64, chunks = (bytes + HB - 1) / HB;
     // Rows past the end of an operand re-read its last row, chunks past a row's end its last
     // chunk.  A table load covers 8 rows, a hidden load 4; lane -> (row, chunk ^ row).
@@ -2153,6 +2199,9 @@ __global__ void __launch_bounds__(64 * NW) scores_kernel(FwdParams p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (v0 + 4 * g + r < a.V) m = fmaxf(m, acc[mi][r]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (token[mi] >= 0 && token[mi] == v0 + 4 * g + r) p.token_x[16 * mi + l16] = acc[mi][r];  // as keep_token
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
         const float b = m * p.c;
@@ -2299,6 +2348,7 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     p.part_s = p.part_m + cnt;
     p.part_i = (int *)(p.part_s + cnt);
     p.part_t = (float *)p.part_i;
+    p.token_x = p.part_t + cnt;
     p.red = nullptr;
     int st;
     if (few) {
@@ -2344,7 +2394,7 @@ int run_fwd(const qpam_ce_fwd_args &a, hipStream_t stream, const FwdParams *scor
     }
     if (st) return st;
     if (scores) {
-        hipLaunchKernelGGL(scores_finalize_kernel<T>, dim3((a.N + 3) / 4), dim3(THREADS), 0, stream, p);
+        hipLaunchKernelGGL(scores_finalize_kernel, dim3((a.N + 3) / 4), dim3(THREADS), 0, stream, p);
         return launch_status("scores_finalize_kernel");
     }
     hipLaunchKernelGGL(ce_fwd_finalize_kernel<T>, dim3((a.N + 3) / 4), dim3(THREADS), 0, stream, p);
@@ -2779,11 +2829,12 @@ extern "C" int qpam_ce_bwd(const qpam_ce_bwd_args *a, void *stream) {
 extern "C" size_t qpam_linear_logprobs_fwd_workspace_size(const qpam_linear_logprobs_args *a) {
     using namespace qpam::ce;
     if (!a || a->N < 1 || a->V < 1) return 0;
-    const qpam_ce_fwd_args f = fwd_args(*a);
-    if (a->N <= thin::ROWS) return (size_t)a->N * thin::blocks(a->V) * 12 + 256;
-    if (a->dtype == QPAM_BF16) return (size_t)a->N * tiles::columns(a->N, a->V).n_vt * 12 + 256;
-    if (split::small_tiles(a->N, a->V)) return (size_t)a->N * ((a->V + split::tn<2>() - 1) / split::tn<2>()) * 12 + 256;
-    return qpam_ce_fwd_workspace_size(&f);
+    // a row's (b, s, t) of every vocab tile, and its token's logit
+    auto bytes = [&](int n_vt) { return (size_t)a->N * n_vt * 12 + (size_t)a->N * 4 + 256; };
+    if (a->N <= thin::ROWS) return bytes(thin::blocks(a->V));
+    if (a->dtype == QPAM_BF16) return bytes(tiles::columns(a->N, a->V).n_vt);
+    if (split::small_tiles(a->N, a->V)) return bytes((a->V + split::tn<2>() - 1) / split::tn<2>());
+    return bytes((a->V + split::TN - 1) / split::TN);
 }
 
 extern "C" int qpam_linear_logprobs_fwd(const qpam_linear_logprobs_args *a, void *stream) {

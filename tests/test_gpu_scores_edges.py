@@ -1,0 +1,75 @@
+"""Token scores where rounding decides (qpam_linear_logprobs_fwd / _bwd): rows that are certain or
+all but certain of their token.  Tolerances beside each test, u = 2^-24."""
+
+import pytest
+import torch
+
+from test_gpu_linear_logprobs import BF16, F32, U, _close
+
+pytestmark = pytest.mark.gpu
+
+
+def _toward(w, first, second, a, b):
+    """Rows h with h . w[first] = a and h . w[second] = b, of least norm."""
+    f, s = w[first].double(), w[second].double()
+    ff, fs, ss = (f * f).sum(-1), (f * s).sum(-1), (s * s).sum(-1)
+    det = ff * ss - fs * fs
+    return ((a * ss - b * fs) / det)[:, None] * f + ((b * ff - a * fs) / det)[:, None] * s
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V,D", [(1, 700, 1536), (16, 1000, 512), (40, 33000, 512), (64, 300, 640), (65, 1000, 512),
+                                   (300, 1023, 512), (600, 9000, 256)])
+def test_certain_rows(gpu_lib, n, V, D, dtype):
+    """The token leads by 60 or more: 1 - p, the entropy and the row of dx are 0 to within V e^-60
+    (10^-22).  The token's logit is the row's maximum, so its own term is 2^0 and the sum is 1:
+    what is left is a rounding or two of numbers near 1, 4 u, and of one below 0 nothing."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    g = torch.Generator().manual_seed(n + V)
+    w = (torch.randn(V, D, generator=g) * 2.5 / D ** 0.5).to(dtype)
+    ids = torch.randint(0, V, (n,), generator=g)
+    h = (300 * w[ids].double() / (w[ids].double() ** 2).sum(-1, keepdim=True)).to(dtype)
+    x = h.double() @ w.double().T
+    lead = x.gather(1, ids[:, None])[:, 0] - x.scatter(1, ids[:, None], float("-inf")).max(-1).values
+    assert lead.min() >= 60
+    gs = [torch.randn(n, generator=g), torch.randn(n, generator=g)]
+    hc, wc = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    r = linear_token_logprobs(hc, wc, ids.cuda())
+    dh, dw = torch.autograd.grad([r.logprobs, r.entropy], [hc, wc], [t.cuda() for t in gs])
+    assert (r.logprobs <= 0).all() and (r.logprobs >= -4 * U).all(), r.logprobs.abs().max()
+    assert (r.entropy >= 0).all() and (r.entropy <= 4 * U).all(), r.entropy.abs().max()
+    dx = (8 * U * (gs[0].abs() + gs[1].abs())).double()
+    _close(dh, torch.zeros(n, D).double(), dx[:, None] * w[ids].double().abs() + 1e-20)
+    _close(dw, torch.zeros(V, D).double(),
+           torch.zeros(V, D).double().index_add_(0, ids, dx[:, None] * h.double().abs()) + 1e-18)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V,D", [(1, 300, 512), (24, 700, 768), (64, 40000, 512), (65, 1000, 512), (300, 1023, 512)])
+def test_nearly_certain_rows(gpu_lib, n, V, D, dtype):
+    """One other token eight below the row's own: 1 - p = e^-8 (3e-4).  A logit is off by the roundings
+    of its fp32 sum, at most E = (D + 4) u sum |h w| and in earnest about sqrt(D) of the D, so d ln p
+    = (1 - p) times that of the lead: relative to dx 2 E sqrt(D) / D at three times its deviation (6 E /
+    sqrt(D)), 4 u / (1 - p) for 1 - e^lp, and dx's rounding to bf16 (2^-8), as of the outputs."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    g = torch.Generator().manual_seed(n + V)
+    w = (torch.randn(V, D, generator=g) * 2.5 / D ** 0.5).to(dtype)
+    ids = torch.randperm(V, generator=g)[:n]
+    other = (ids + 1 + torch.randint(0, V - 1, (n,), generator=g)) % V
+    h = _toward(w, ids, other, 100.0, 92.0).to(dtype)
+    hd, wd = h.double(), w.double()
+    logp = torch.log_softmax(hd @ wd.T, -1)
+    p, g_lp = logp.exp(), torch.rand(n, generator=g) + 0.5
+    lp = logp.gather(1, ids[:, None])
+    assert ((lp > -0.01) & (lp < -1e-5)).all()
+    dx = -p * g_lp.double()[:, None]
+    dx.scatter_(1, ids[:, None], -torch.expm1(lp) * g_lp.double()[:, None])
+    hc, wc = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    r = linear_token_logprobs(hc, wc, ids.cuda())
+    dh, = torch.autograd.grad(r.logprobs, hc, g_lp.cuda())
+    assert (r.logprobs < 0).all() and (r.entropy > 0).all()
+    E = (D + 4) * U * (hd.abs() * wd[ids].abs()).sum(-1)
+    rel = 6 * E / D ** 0.5 + 4 * U / 1e-5 + (2.0 ** -7 if dtype == BF16 else 0.0)
+    want = dx @ wd
+    err = (dh.cpu().double() - want).norm(dim=-1) / want.norm(dim=-1)
+    assert (err <= rel).all(), (err / rel).max()
