@@ -22,14 +22,14 @@
 //
 // Token scores (qpam_linear_logprobs_*; namespaces split for fp32, tiles for bf16, thin
 // for few rows, with products of their own): the log probability of each row's token and
-// the entropy of the row.  With c = log2(e) / T,
-// b = c max x rounded and u = c x - b (one fma, so b's rounding shifts every u alike and
-// cancels), the tiles reduce s = sum 2^u and t = sum 2^u u, so that
+// the entropy of the row.  With c = log2(e) / T, m = max x and u = c (x - m), the tiles
+// reduce s = sum 2^u and t = sum 2^u u, so that
 //   log prob = ln2 (u_token - log2 s),   entropy = ln2 (log2 s - t / s),
 // with the token's logit from the same accumulators (the tile that holds its column keeps it),
 // and the gradient tiles write (as G^T alone)
 //   G_v = -p_v / T (g_lp + g_ent (ln p_v + entropy)) + [v = token] g_lp / T.
-// Logits with |c x| past fp32's range give NaN.
+// The maximum is taken off in front of c: a reference of c m in fp32 is off by 2^-25 of
+// itself, which is past the exponent's range from |c m| = 2^32 on (T = 1e-9).
 #include <algorithm>
 #include <type_traits>
 
@@ -184,14 +184,14 @@ template <int NI> __device__ __forceinline__ void keep_token(const FwdParams &p,
     }
 }
 
-// (b, s, t) of two parts of a row's logits as one (b = -inf: a part of nothing)
-__device__ __forceinline__ void join_scores(float &b, float &s, float &t, float ob, float os, float ot) {
-    const float nb = fmaxf(b, ob), lo = fmaxf(nb, -3.402823466e38f);
-    const float g = fmaxf(b - lo, U_FLOOR), og = fmaxf(ob - lo, U_FLOOR);
+// (m, s, t) of two parts of a row's logits as one (m = -inf: a part of nothing)
+__device__ __forceinline__ void join_scores(float c, float &m, float &s, float &t, float om, float os, float ot) {
+    const float nm = fmaxf(m, om), lo = fmaxf(nm, -3.402823466e38f);
+    const float g = fmaxf((m - lo) * c, U_FLOOR), og = fmaxf((om - lo) * c, U_FLOOR);
     const float f = __builtin_amdgcn_exp2f(g), of = __builtin_amdgcn_exp2f(og);
     t = f * (t + s * g) + of * (ot + os * og);
     s = f * s + of * os;
-    b = nb;
+    m = nm;
 }
 
 template <typename T>
@@ -306,28 +306,28 @@ __global__ void __launch_bounds__(THREADS) ce_fwd_finalize_kernel(FwdParams p) {
     }
 }
 
-// one wave per row: merge the vocab tiles into (b, s, t), add the token's logit.  Neither
+// one wave per row: merge the vocab tiles into (m, s, t), add the token's logit.  Neither
 // a log probability above 0 nor an entropy below it is left by the last roundings.
 __global__ void __launch_bounds__(THREADS) scores_finalize_kernel(FwdParams p) {
     const qpam_ce_fwd_args &a = p.a;
     const int lane = threadIdx.x & 63;
     const int row = blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6);
     if (row >= a.N) return;
-    float b = -INFINITY, s = 0.f, t = 0.f;
+    float m = -INFINITY, s = 0.f, t = 0.f;
     for (int vt = lane; vt < p.n_vt; vt += 64) {
         const int64_t o = (int64_t)row * p.n_vt + vt;
-        join_scores(b, s, t, p.part_m[o], p.part_s[o], p.part_t[o]);
+        join_scores(p.c, m, s, t, p.part_m[o], p.part_s[o], p.part_t[o]);
     }
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1)
-        join_scores(b, s, t, __shfl_xor(b, off), __shfl_xor(s, off), __shfl_xor(t, off));
+        join_scores(p.c, m, s, t, __shfl_xor(m, off), __shfl_xor(s, off), __shfl_xor(t, off));
     if (lane == 0) {
         const float log_s = log2f(s), ent = LN2 * (log_s - t / s);
         float lp = 0.f;
-        if (row_token(p, row) >= 0) lp = LN2 * (__builtin_fmaf(p.token_x[row], p.c, -b) - log_s);
+        if (row_token(p, row) >= 0) lp = LN2 * ((p.token_x[row] - m) * p.c - log_s);
         p.logprobs[row] = lp > 0.f ? 0.f : lp;
         p.entropy[row] = ent < 0.f ? 0.f : ent;
-        p.stats[2 * row] = b;
+        p.stats[2 * row] = m;
         p.stats[2 * row + 1] = s;
     }
 }
@@ -385,9 +385,9 @@ struct BwdParams {
     const float *stats, *logprobs, *entropy, *g_logprobs, *g_entropy;
 };
 
-// A row's part of G_v = 2^u (base + slope u), u = c x - b.  Zero for a row past the end.
+// A row's part of G_v = 2^u (base + slope u), u = c (x - m).  Zero for a row past the end.
 struct RowScore {
-    float b, base, slope;
+    float m, base, slope;
 };
 
 __device__ __forceinline__ RowScore row_score(const BwdParams &p, int lr) {
@@ -684,7 +684,7 @@ template <int S>
 __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
     constexpr int TM = tm<S>(), TN = tn<S>();
     __shared__ __align__(16) U16 s0[3 * plane<S, false, false>()], s1[3 * plane<S, false, false>()];
-    __shared__ float sB[2][TM], sS[2][TM], sT[2][TM];
+    __shared__ float sM[2][TM], sS[2][TM], sT[2][TM];
     __shared__ __align__(16) int sToken[TM];
     const qpam_ce_fwd_args &a = p.a;
     const int vt = blockIdx.x, r0 = blockIdx.y * TM, v0 = vt * TN;
@@ -704,31 +704,31 @@ __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
 #pragma unroll
             for (int ni = 0; ni < S; ++ni)
                 if (vl + 16 * ni < a.V) mx = fmaxf(mx, acc[mi][ni][r]);
-            const float b = row16_max(mx) * p.c;
+            const float m = row16_max(mx);
             float s = 0.f, t = 0.f;
 #pragma unroll
             for (int ni = 0; ni < S; ++ni)
                 if (vl + 16 * ni < a.V) {
-                    const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
+                    const float d = acc[mi][ni][r] - m, e = __builtin_amdgcn_exp2f(d * p.c);
                     s += e;
-                    t = __builtin_fmaf(e, u, t);
+                    t = __builtin_fmaf(e, d, t);
                 }
             s = row16_sum(s);
             t = row16_sum(t);
             if (l16 == 0) {
                 const int row = 16 * S * wm + 16 * mi + 4 * g + r;
-                sB[wn][row] = b;
+                sM[wn][row] = m;
                 sS[wn][row] = s;
-                sT[wn][row] = t;
+                sT[wn][row] = t * p.c;
             }
         }
     }
     __syncthreads();
     if (tid < TM && r0 + tid < a.N) {
-        float b = sB[0][tid], s = sS[0][tid], t = sT[0][tid];
-        join_scores(b, s, t, sB[1][tid], sS[1][tid], sT[1][tid]);
+        float m = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
+        join_scores(p.c, m, s, t, sM[1][tid], sS[1][tid], sT[1][tid]);
         const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
-        p.part_m[o] = b;
+        p.part_m[o] = m;
         p.part_s[o] = s;
         p.part_t[o] = t;
     }
@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
     const int lr0 = blockIdx.y * TM, v0 = blockIdx.x * TN, tid = threadIdx.x;
     if (tid < TM) {
         const RowScore q = row_score(p, lr0 + tid);
-        sRow[0][tid] = q.b;
+        sRow[0][tid] = q.m;
         sRow[1][tid] = q.base;
         sRow[2][tid] = q.slope;
     }
@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
 #pragma unroll
     for (int mi = 0; mi < S; ++mi) {
         const int rl = 16 * S * wm + 16 * mi + 4 * g;
-        const floatx4 hb = *reinterpret_cast<const floatx4 *>(&sRow[0][rl]);
+        const floatx4 hm = *reinterpret_cast<const floatx4 *>(&sRow[0][rl]);
         const floatx4 h0 = *reinterpret_cast<const floatx4 *>(&sRow[1][rl]);
         const floatx4 h1 = *reinterpret_cast<const floatx4 *>(&sRow[2][rl]);
 #pragma unroll
@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
             floatx4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -hb[r]);
+                const float u = (acc[mi][ni][r] - hm[r]) * p.c;
                 const bool in = v < a.V && lr0 + rl + r < p.rows;
                 x[r] = in ? __builtin_amdgcn_exp2f(u) * __builtin_fmaf(h1[r], u, h0[r]) : 0.f;
             }
@@ -1733,10 +1733,10 @@ struct Tokens {
     uint64_t here[TM / 64];
 };
 
-// A tile's (b, s, t) per row: over each wave's columns from v0 on, then the two waves of a row.
+// A tile's (m, s, t) per row: over each wave's columns from v0 on, then the two waves of a row.
 template <int NI>
 __device__ __forceinline__ void reduce_rows(const FwdParams &p, const floatx4 (&acc)[4][NI], int r0, int v0, int vt,
-                                            float (&sB)[2][TM], float (&sS)[2][TM], float (&sT)[2][TM], const Tokens &tokens) {
+                                            float (&sM)[2][TM], float (&sS)[2][TM], float (&sT)[2][TM], const Tokens &tokens) {
     const qpam_ce_fwd_args &a = p.a;
     const int tid = threadIdx.x, w = wave_id(), lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wm = w >> 1, wn = w & 1;
@@ -1758,22 +1758,22 @@ __device__ __forceinline__ void reduce_rows(const FwdParams &p, const floatx4 (&
 #pragma unroll
                 for (int ni = 0; ni < NI; ++ni)
                     if (whole || vl + 16 * ni < a.V) mx = fmaxf(mx, acc[mi][ni][r]);
-                const float b = row16_max(mx) * p.c;
+                const float m = row16_max(mx);
                 float s = 0.f, t = 0.f;
 #pragma unroll
                 for (int ni = 0; ni < NI; ++ni)
                     if (whole || vl + 16 * ni < a.V) {
-                        const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
+                        const float d = acc[mi][ni][r] - m, e = __builtin_amdgcn_exp2f(d * p.c);
                         s += e;
-                        t = __builtin_fmaf(e, u, t);
+                        t = __builtin_fmaf(e, d, t);
                     }
                 s = row16_sum(s);
                 t = row16_sum(t);
                 if (l16 == 0) {
                     const int row = 64 * wm + 16 * mi + 4 * g + r;
-                    sB[wn][row] = b;
+                    sM[wn][row] = m;
                     sS[wn][row] = s;
-                    sT[wn][row] = t;
+                    sT[wn][row] = t * p.c;
                 }
             }
         }
@@ -1782,10 +1782,10 @@ __device__ __forceinline__ void reduce_rows(const FwdParams &p, const floatx4 (&
     else rows(std::false_type{});
     block_lds_sync();
     if (tid < TM && r0 + tid < a.N) {
-        float b = sB[0][tid], s = sS[0][tid], t = sT[0][tid];
-        join_scores(b, s, t, sB[1][tid], sS[1][tid], sT[1][tid]);
+        float m = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
+        join_scores(p.c, m, s, t, sM[1][tid], sS[1][tid], sT[1][tid]);
         const int64_t o = (int64_t)(r0 + tid) * p.n_vt + vt;
-        p.part_m[o] = b;
+        p.part_m[o] = m;
         p.part_s[o] = s;
         p.part_t[o] = t;
     }
@@ -1811,7 +1811,7 @@ inline Columns columns(int N, int V) {
 template <int NARROW>
 __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
     __shared__ __align__(16) Stage s0, s1, s2, s3;
-    __shared__ float sB[2][TM], sS[2][TM], sT[2][TM];
+    __shared__ float sM[2][TM], sS[2][TM], sT[2][TM];
     __shared__ __align__(16) Tokens sTokens[2];  // of this tile and the next
     const qpam_ce_fwd_args &a = p.a;
     const Stages stages{s0, s1, s2, s3};
@@ -1853,13 +1853,13 @@ __global__ void __launch_bounds__(TT) scores_tile_kernel(FwdParams p) {
         product(stages, q, KT, acc);
         put_tokens(id, buf ^ 1);
         load_next();
-        reduce_rows(p, acc, rt * TM, vt * TN, vt, sB, sS, sT, sTokens[buf]);
+        reduce_rows(p, acc, rt * TM, vt * TN, vt, sM, sS, sT, sTokens[buf]);
         buf ^= 1;
     }
     if (!last) return;
     floatx4 acc[4][NARROW];
     product(stages, q, KT, acc);
-    reduce_rows(p, acc, last_rt * TM, last_v0, p.full_vt + last_ct, sB, sS, sT, sTokens[buf]);
+    reduce_rows(p, acc, last_rt * TM, last_v0, p.full_vt + last_ct, sM, sS, sT, sTokens[buf]);
 }
 
 // G^T [Vp][Rp] without the tokens' one-hot terms; zero past the vocabulary and past the rows.
@@ -1890,7 +1890,7 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
         const int rt = at.more() ? at.rt : last_rt, v0 = at.more() ? at.vt * TN : last_v0, lr0 = rt * TM;
         const RowScore x = row_score(p, lr0 + (tid & (TM - 1)));
         if (tid < TM) {
-            sRow[buf][0][tid] = x.b;
+            sRow[buf][0][tid] = x.m;
             sRow[buf][1][tid] = x.base;
             sRow[buf][2][tid] = x.slope;
         }
@@ -1912,13 +1912,13 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
 #pragma unroll
                 for (int mi = 0; mi < 4; ++mi) {
                     const int rl0 = 64 * wm + 16 * mi + 4 * g;
-                    const floatx4 hb = *reinterpret_cast<const floatx4 *>(mine + 16 * mi);
+                    const floatx4 hm = *reinterpret_cast<const floatx4 *>(mine + 16 * mi);
                     const floatx4 h0 = *reinterpret_cast<const floatx4 *>(mine + TM + 16 * mi);
                     const floatx4 h1 = *reinterpret_cast<const floatx4 *>(mine + 2 * TM + 16 * mi);
                     float x[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float u = __builtin_fmaf(acc[mi][ni][r], p.c, -hb[r]);
+                        const float u = (acc[mi][ni][r] - hm[r]) * p.c;
                         x[r] = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(h1[r], u, h0[r]);
                         if (!whole && (v >= a.V || lr0 + rl0 + r >= p.rows)) x[r] = 0.f;
                     }
@@ -2204,31 +2204,30 @@ __global__ void __launch_bounds__(64 * NW) scores_kernel(FwdParams p) {
             if (token[mi] >= 0 && token[mi] == v0 + 4 * g + r) p.token_x[16 * mi + l16] = acc[mi][r];  // as keep_token
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
-        const float b = m * p.c;
         float s = 0.f, t = 0.f;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (v0 + 4 * g + r < a.V) {
-                const float u = __builtin_fmaf(acc[mi][r], p.c, -b), e = __builtin_amdgcn_exp2f(u);
+                const float d = acc[mi][r] - m, e = __builtin_amdgcn_exp2f(d * p.c);
                 s += e;
-                t += e * u;
+                t += e * d;
             }
         s += __shfl_xor(s, 16);
         t += __shfl_xor(t, 16);
         s += __shfl_xor(s, 32);
         t += __shfl_xor(t, 32);
         if (g == 0) {
-            sM[w][16 * mi + l16] = b;
+            sM[w][16 * mi + l16] = m;
             sS[w][16 * mi + l16] = s;
-            sT[w][16 * mi + l16] = t;
+            sT[w][16 * mi + l16] = t * p.c;
         }
     }
     __syncthreads();
     if (tid < 16 * MI && tid < a.N) {
-        float b = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
-        for (int v = 1; v < NW; ++v) join_scores(b, s, t, sM[v][tid], sS[v][tid], sT[v][tid]);
+        float m = sM[0][tid], s = sS[0][tid], t = sT[0][tid];
+        for (int v = 1; v < NW; ++v) join_scores(p.c, m, s, t, sM[v][tid], sS[v][tid], sT[v][tid]);
         const int64_t o = (int64_t)tid * p.n_vt + blockIdx.x;
-        p.part_m[o] = b;
+        p.part_m[o] = m;
         p.part_s[o] = s;
         p.part_t[o] = t;
     }
@@ -2829,7 +2828,7 @@ extern "C" int qpam_ce_bwd(const qpam_ce_bwd_args *a, void *stream) {
 extern "C" size_t qpam_linear_logprobs_fwd_workspace_size(const qpam_linear_logprobs_args *a) {
     using namespace qpam::ce;
     if (!a || a->N < 1 || a->V < 1) return 0;
-    // a row's (b, s, t) of every vocab tile, and its token's logit
+    // a row's (m, s, t) of every vocab tile, and its token's logit
     auto bytes = [&](int n_vt) { return (size_t)a->N * n_vt * 12 + (size_t)a->N * 4 + 256; };
     if (a->N <= thin::ROWS) return bytes(thin::blocks(a->V));
     if (a->dtype == QPAM_BF16) return bytes(tiles::columns(a->N, a->V).n_vt);

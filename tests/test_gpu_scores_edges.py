@@ -1,10 +1,10 @@
 """Token scores where rounding decides (qpam_linear_logprobs_fwd / _bwd): rows that are certain or
-all but certain of their token.  Tolerances beside each test, u = 2^-24."""
+all but certain of their token, and low temperatures.  Tolerances beside each test, u = 2^-24."""
 
 import pytest
 import torch
 
-from test_gpu_linear_logprobs import BF16, F32, U, _close
+from test_gpu_linear_logprobs import BF16, F32, U, _close, _data
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,45 @@ def test_nearly_certain_rows(gpu_lib, n, V, D, dtype):
     want = dx @ wd
     err = (dh.cpu().double() - want).norm(dim=-1) / want.norm(dim=-1)
     assert (err <= rel).all(), (err / rel).max()
+
+
+def _whole(n, V, D, dtype, T):
+    """Operands whose logits are whole numbers, exact in every sum, with what they give at a low temperature T:
+    each row's k largest entries have p = 1 / k, the others 0 (e^-1000 and less).  The sum counts k exactly
+    up to L = V / 16 + 60 roundings, so ln k is off by 2 u (L + ln k + 1)."""
+    g = torch.Generator().manual_seed(n)
+    h, w = torch.randint(-2, 3, (n, D), generator=g).to(dtype), torch.randint(-1, 2, (V, D), generator=g).to(dtype)
+    ids = torch.randint(0, V, (n,), generator=g)
+    x = h.double() @ w.double().T
+    ids[::3] = x.argmax(-1)[::3]
+    ids[4::5] = -100
+    d = x.max(-1, keepdim=True).values - x
+    p = (d == 0).double()
+    ln_k = p.sum(-1).log()
+    t_ln = 2 * U * (V / 16 + 60 + ln_k + 1)
+    lp = torch.where(ids >= 0, -d.gather(1, ids.clamp(min=0)[:, None])[:, 0] / T - ln_k, 0.0)
+    return h, w, ids, p / p.sum(-1, keepdim=True), lp, ln_k, t_ln
+
+
+@pytest.mark.parametrize("T", [1e-3, 1e-9, 1e-12, 1e-25])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [5, 300, 2000])
+def test_low_temperatures(gpu_lib, n, dtype, T):
+    """A log probability -d / T is the product of three rounded factors: 8 u of it with the last sum."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, _, lp, ln_k, t_ln = _whole(n, 4200, 64, dtype, T)
+    r = linear_token_logprobs(h.cuda(), w.cuda(), ids.cuda(), temperature=T)
+    _close(r.logprobs, lp, 8 * U * lp.abs() + t_ln)
+    _close(r.entropy, ln_k, 2 * t_ln)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [20, 300])
+def test_low_temperature_of_rounded_logits(gpu_lib, n, dtype):
+    """At T = 1e-9 a logit's last bits are hundreds of units of u, so which entry leads is a matter of the
+    sums' order; each row's values stay a distribution's: lp <= 0, entropy of [0, ln V]."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, _ = _data(n, 700, 96, dtype, dtype, 21)
+    r = linear_token_logprobs(h.cuda(), w.cuda(), ids.cuda(), temperature=1e-9)
+    assert (r.logprobs <= 0).all() and r.logprobs.isfinite().all()
+    assert (r.entropy >= 0).all() and (r.entropy <= 6.5511).all()    # ln 700
