@@ -390,6 +390,11 @@ struct RowScore {
     float m, base, slope;
 };
 
+// u of one logit, kept where 2^u (base + slope u) is finite: above U_FLOOR, past which 2^u is 0
+// but slope u can be infinite (low temperatures), and at most 0, as the maximum is the
+// forward's and this sum may be off from it in its last bits.  A row with NaN has a NaN base.
+__device__ __forceinline__ float score_u(float x, float m, float c) { return __builtin_amdgcn_fmed3f((x - m) * c, U_FLOOR, 0.f); }
+
 __device__ __forceinline__ RowScore row_score(const BwdParams &p, int lr) {
     if (lr >= p.rows) return {0.f, 0.f, 0.f};
     const qpam_ce_bwd_args &a = p.a;
@@ -412,7 +417,7 @@ __global__ void __launch_bounds__(THREADS) scores_token_kernel(BwdParams p) {
     if (id == a.ignore_index || id < 0 || id >= a.V) return;
     const float g_lp = p.g_logprobs ? p.g_logprobs[row] : 0.f, g_ent = p.g_entropy ? p.g_entropy[row] : 0.f;
     const float lp = p.logprobs[row], q = expf(lp);
-    const float x = p.inv_t * (g_lp * (1.f - q) - g_ent * q * (lp + p.entropy[row]));
+    const float x = p.inv_t * (g_lp * (1.f - q) - g_ent * q * (fmaxf(lp, U_FLOOR) + p.entropy[row]));
     T v;
     if constexpr (sizeof(T) == 2) v = __builtin_bit_cast(unsigned short, (__bf16)x);
     else v = x;
@@ -769,7 +774,7 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
             floatx4 x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float u = (acc[mi][ni][r] - hm[r]) * p.c;
+                const float u = score_u(acc[mi][ni][r], hm[r], p.c);
                 const bool in = v < a.V && lr0 + rl + r < p.rows;
                 x[r] = in ? __builtin_amdgcn_exp2f(u) * __builtin_fmaf(h1[r], u, h0[r]) : 0.f;
             }
@@ -1918,7 +1923,7 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
                     float x[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float u = (acc[mi][ni][r] - hm[r]) * p.c;
+                        const float u = score_u(acc[mi][ni][r], hm[r], p.c);
                         x[r] = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(h1[r], u, h0[r]);
                         if (!whole && (v >= a.V || lr0 + rl0 + r >= p.rows)) x[r] = 0.f;
                     }

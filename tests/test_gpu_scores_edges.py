@@ -115,3 +115,41 @@ def test_low_temperature_of_rounded_logits(gpu_lib, n, dtype):
     r = linear_token_logprobs(h.cuda(), w.cuda(), ids.cuda(), temperature=1e-9)
     assert (r.logprobs <= 0).all() and r.logprobs.isfinite().all()
     assert (r.entropy >= 0).all() and (r.entropy <= 6.5511).all()    # ln 700
+
+
+@pytest.mark.parametrize("T", [1e-3, 1e-9, 1e-12, 1e-25])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V", [(5, 600), (300, 600), (1200, 4200)])
+def test_gradients_at_low_temperatures(gpu_lib, n, V, dtype, T):
+    """dx = ([v = token] - p) g_lp / T: the entropy's term is p (ln p + entropy) = 0 at the largest entries, off by
+    the errors of both logarithms, and 0 at the others however large their u."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, p, _, _, t_ln = _whole(n, V, 64, dtype, T)
+    g = torch.Generator().manual_seed(1)
+    gs = [torch.randn(n, generator=g) / n, torch.randn(n, generator=g) / n]
+    g_lp, g_ent = torch.where(ids >= 0, gs[0].double(), 0.0), gs[1].double()
+    one = torch.zeros_like(p).scatter_add_(1, ids.clamp(min=0)[:, None], g_lp[:, None])
+    dx = (one - p * g_lp[:, None]) / T
+    tol = p / T * (g_lp.abs() * (2 * t_ln + 8 * U) + g_ent.abs() * (4 * t_ln + 8 * U))[:, None] + 16 * U * one.abs() / T
+    tol += (2.0 ** -8 if dtype == BF16 else 4 * U) * (dx.abs() + tol)
+    hc, wc = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    r = linear_token_logprobs(hc, wc, ids.cuda(), temperature=T)
+    dh, dw = torch.autograd.grad([r.logprobs, r.entropy], [hc, wc], [t.cuda() for t in gs])
+    hd, wd = h.double(), w.double()
+    _close(dh, dx @ wd, tol @ wd.abs() + V * U * (dx.abs() @ wd.abs()), torch.finfo(dtype).eps)
+    _close(dw, dx.T @ hd, tol.T @ hd.abs() + n * U * (dx.abs().T @ hd.abs()), torch.finfo(dtype).eps)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [20, 300])
+def test_gradients_at_a_low_temperature_of_rounded_logits(gpu_lib, n, dtype):
+    """Where the forward's product and the backward's own differ in a logit's last bits (few fp32 rows), p =
+    2^u / s is of [0, 1] all the same: |dx| sums to at most 2 |g_lp| + 2 |g_ent| (1 + ln V) over a row, times
+    1 / T, and 4 for more than one entry at u = 0."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, gs = _data(n, 700, 96, dtype, dtype, 21)
+    hc, T = h.cuda().requires_grad_(), 1e-9
+    r = linear_token_logprobs(hc, w.cuda(), ids.cuda(), temperature=T)
+    dh, = torch.autograd.grad([r.logprobs, r.entropy], [hc], [t.cuda() for t in gs])
+    bound = 8 * (gs[0].abs() + gs[1].abs() * 7.56) / T * w.float().abs().max()
+    assert (dh.float().abs().cpu() <= bound[:, None]).all()
