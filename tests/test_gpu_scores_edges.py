@@ -1,10 +1,11 @@
 """Token scores where rounding decides (qpam_linear_logprobs_fwd / _bwd): rows that are certain or
-all but certain of their token, and low temperatures.  Tolerances beside each test, u = 2^-24."""
+all but certain of their token, low temperatures, and the kernel of few rows at its own widths.
+Tolerances beside each test, u = 2^-24."""
 
 import pytest
 import torch
 
-from test_gpu_linear_logprobs import BF16, F32, U, _close, _data
+from test_gpu_linear_logprobs import BF16, F32, U, _close, _data, _reference
 
 pytestmark = pytest.mark.gpu
 
@@ -153,3 +154,17 @@ def test_gradients_at_a_low_temperature_of_rounded_logits(gpu_lib, n, dtype):
     dh, = torch.autograd.grad([r.logprobs, r.entropy], [hc], [t.cuda() for t in gs])
     bound = 8 * (gs[0].abs() + gs[1].abs() * 7.56) / T * w.float().abs().max()
     assert (dh.float().abs().cpu() <= bound[:, None]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V,D", [(16, 1000, 1536), (9, 33000, 640), (20, 1000, 896), (30, 33000, 672), (33, 1000, 640),
+                                   (64, 33000, 1568), (1, 33000, 896), (64, 300, 1184)])
+def test_few_rows_of_real_widths(gpu_lib, n, V, D, dtype):
+    """Up to 64 rows over 5 to 25 stages of 256 bytes a row: every body of the unrolled loop and its return
+    to the first, with 16, 32 and 64 rows in blocks of 4 and of 16 waves.  Tolerances as for all sizes."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, _ = _data(n, V, D, dtype, dtype, n + D)
+    r = linear_token_logprobs(h.cuda(), w.cuda(), ids.cuda(), temperature=0.8)
+    R = _reference(h, w, ids, 0.8, None, 0.0)
+    _close(r.logprobs, R["lp"], R["t_lp"])
+    _close(r.entropy, R["H"], R["t_H"])
