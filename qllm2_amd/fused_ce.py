@@ -27,7 +27,18 @@ from ._ops import op
 __all__ = ["fused_linear_cross_entropy", "linear_ce_per_token", "linear_ce_stats"]
 
 
-def _operands(hidden_rows, weight_matrix):
+def _rows(x, max_stride):
+    """x [n, D] as the kernels read rows: unit column stride, at least D and at most max_stride elements
+    apart (rows of an expanded tensor share their memory), each a multiple of 16 bytes into memory; a
+    copy where it is not."""
+    vec = 16 // x.element_size()
+    if x.stride(1) == 1 and x.shape[1] <= x.stride(0) <= max_stride and not x.stride(0) % vec and not x.data_ptr() % 16:
+        return x
+    # contiguous() gives back a contiguous tensor whose storage starts off 16 bytes
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _operands(hidden_rows, weight_matrix, max_stride=2 ** 62):
     if not (hidden_rows.is_cuda and weight_matrix.is_cuda):
         raise ValueError("qpam fused CE: tensors must be on the GPU (no CPU path in this library)")
     if hidden_rows.dim() != 2 or weight_matrix.dim() != 2 or hidden_rows.shape[1] != weight_matrix.shape[1]:
@@ -38,12 +49,7 @@ def _operands(hidden_rows, weight_matrix):
     work = torch.bfloat16 if torch.bfloat16 in (hidden_rows.dtype, weight_matrix.dtype) else torch.float32
     h = hidden_rows.to(work)
     w = weight_matrix.to(work)
-    vec = 8 if work == torch.bfloat16 else 4
-    if h.stride(1) != 1 or h.stride(0) % vec or h.data_ptr() % 16:
-        h = h.contiguous()
-    if w.stride(1) != 1 or w.stride(0) % vec or w.data_ptr() % 16:
-        w = w.contiguous()
-    return h, w, (_lib.QPAM_BF16 if work == torch.bfloat16 else _lib.QPAM_F32)
+    return _rows(h, max_stride), _rows(w, max_stride), (_lib.QPAM_BF16 if work == torch.bfloat16 else _lib.QPAM_F32)
 
 
 def _fwd_args(h, w, dtype, targets, mask, ignore_index):

@@ -26,6 +26,8 @@ __all__ = ["TokenLogprobs", "token_logprobs", "linear_token_logprobs"]
 MAX_TOP_K = 64
 MAX_VOCAB = 2 ** 30  # 32-bit sizes below
 MAX_ROWS = 65535 * 128  # hidden rows: a launch's second axis
+MAX_STRIDE = 2 ** 22 - 1  # elements between hidden rows and between table rows: 32-bit offsets in a tile
+MAX_D = 2 ** 22 - 32     # ... and columns, padded to whole 32
 
 _CODE = {torch.float32: _lib.QPAM_F32, torch.bfloat16: _lib.QPAM_BF16}
 
@@ -179,8 +181,8 @@ def _check_linear(hidden_rows, weight_matrix, ids, temperature, chunk):
             or hidden_rows.shape[:-1] != ids.shape or not weight_matrix.numel()):
         raise ValueError(f"qpam {name}: hidden_rows [..., D], weight_matrix [V, D] and ids [...] expected, got "
                          f"{tuple(hidden_rows.shape)}, {tuple(weight_matrix.shape)} and {tuple(ids.shape)}")
-    if weight_matrix.shape[0] > MAX_VOCAB or weight_matrix.shape[1] >= 2 ** 22 or ids.numel() > MAX_ROWS:
-        raise ValueError(f"qpam {name}: at most 2^30 table rows, {MAX_ROWS} hidden rows, below 2^22 columns, got "
+    if weight_matrix.shape[0] > MAX_VOCAB or weight_matrix.shape[1] > MAX_D or ids.numel() > MAX_ROWS:
+        raise ValueError(f"qpam {name}: at most 2^30 table rows, {MAX_ROWS} hidden rows, {MAX_D} columns, got "
                          f"{tuple(weight_matrix.shape)} and {ids.numel()}")
     if chunk < 1:
         raise ValueError(f"qpam {name}: chunk {chunk} must be at least 1")
@@ -206,7 +208,7 @@ def _linear_forward(hidden_rows: Tensor, weight_matrix: Tensor, weight_copy: Opt
                     temperature: float, chunk: int, ignore_index: int) -> List[Tensor]:
     """hidden_rows [n, D], ids [n] int64 -> [logprobs, entropy, stats [n, 2]]; weight_copy:
     an fp32 weight_matrix in the rows' bf16."""
-    h, w, dtype = _operands(hidden_rows, weight_matrix if weight_copy is None else weight_copy)
+    h, w, dtype = _operands(hidden_rows, weight_matrix if weight_copy is None else weight_copy, MAX_STRIDE)
     n, dev = h.shape[0], h.device
     lp, ent, stats = (torch.empty(s, device=dev, dtype=torch.float32) for s in ((n,), (n,), (n, 2)))
     if n:
@@ -234,7 +236,7 @@ def _linear_gradient(hidden_rows: Tensor, weight_matrix: Tensor, ids: Tensor, lo
                      ignore_index: int, dw_fp32: bool, need_dh: bool = True, need_dw: bool = True) -> List[Tensor]:
     """[d hidden_rows, d weight_matrix] in the inputs' dtypes (d weight_matrix in fp32
     with dw_fp32); one that is not needed is an empty tensor."""
-    h, w, dtype = _operands(hidden_rows, weight_matrix)
+    h, w, dtype = _operands(hidden_rows, weight_matrix, MAX_STRIDE)
     n, dev = h.shape[0], h.device
     dw_fp32 = dw_fp32 or weight_matrix.dtype != w.dtype
     dh = torch.empty(h.shape if need_dh else 0, device=dev, dtype=h.dtype)
@@ -301,7 +303,8 @@ def linear_token_logprobs(hidden_rows: Tensor, weight_matrix: Tensor, ids: Tenso
     the operands' gradients.  The gradients have the operands' dtypes; that of an fp32
     weight_matrix with bf16 rows (a master table) leaves from the fp32 sums.  chunk
     bounds the backward's memory as in fused_ce.fused_linear_cross_entropy.  D off the
-    multiples of 32 pads both operands by copies.  Alternatives need the logits:
+    multiples of 32 pads both operands by copies; rows that are not apart by their
+    length or more and by less than 2^22 elements, each at a multiple of 16 bytes, are copied.  Alternatives need the logits:
     token_logprobs gives them."""
     _check_linear(hidden_rows, weight_matrix, ids, temperature, chunk)
     D = hidden_rows.shape[-1]

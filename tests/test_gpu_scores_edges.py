@@ -1,6 +1,6 @@
 """Token scores where rounding decides (qpam_linear_logprobs_fwd / _bwd): rows that are certain or
-all but certain of their token, low temperatures, and the kernel of few rows at its own widths.
-Tolerances beside each test, u = 2^-24."""
+all but certain of their token, low temperatures; the kernel of few rows at its own widths; the
+layouts that rows and tables arrive in.  Tolerances beside each test, u = 2^-24."""
 
 import pytest
 import torch
@@ -168,3 +168,61 @@ def test_few_rows_of_real_widths(gpu_lib, n, V, D, dtype):
     R = _reference(h, w, ids, 0.8, None, 0.0)
     _close(r.logprobs, R["lp"], R["t_lp"])
     _close(r.entropy, R["H"], R["t_H"])
+
+
+def _off_16(t):
+    """t in contiguous storage that starts one element off 16 bytes, as a slice of a flat parameter buffer does."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    flat[1:].copy_(t.reshape(-1))
+    return flat[1:].view(t.shape)
+
+
+def _far_apart(t):
+    """t's rows 2^22 elements apart, as one position's rows of a long batch are."""
+    return torch.zeros(t.shape[0], 2 ** 22 // t.shape[1], t.shape[1], dtype=t.dtype, device=t.device).index_copy_(
+        1, torch.tensor([3], device=t.device), t[:, None])[:, 3]
+
+
+LAYOUTS = {
+    "one row for all": (lambda h: h[:1].expand(h.shape[0], -1), lambda w: w[:1].expand(w.shape[0], -1)),
+    "a column as one row": (lambda h: h[:1].T.contiguous().T, lambda w: w),
+    "storage off 16 bytes": (_off_16, _off_16),
+    "rows 2^22 apart": (_far_apart, _far_apart),
+}
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("name", list(LAYOUTS))
+def test_layouts_of_rows_and_table(gpu_lib, name, dtype):
+    """Every layout gives the bits of the same values laid out row after row, with both gradients."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, gs = _data(7, 20, 64, dtype, dtype, 31)
+    f, k = LAYOUTS[name]
+    for a, b in ((f(h.cuda()), w.cuda()), (h.cuda(), k(w.cuda()))):
+        res = []
+        for x, y in ((a, b), (a.clone(memory_format=torch.contiguous_format), b.clone(memory_format=torch.contiguous_format))):
+            x, y = x.detach().requires_grad_(), y.detach().requires_grad_()
+            n = x.shape[0]
+            r = linear_token_logprobs(x, y, ids[:n].cuda())
+            res.append([r.logprobs, r.entropy, *torch.autograd.grad([r.logprobs, r.entropy], [x, y], [t[:n].cuda() for t in gs])])
+        for s, t in zip(*res):
+            assert torch.equal(s, t)
+
+
+@pytest.mark.parametrize("name", ["one row for all", "a column as one row", "storage off 16 bytes"])
+def test_layouts_of_the_loss(gpu_lib, name):
+    """fused_linear_cross_entropy takes its operands the same way."""
+    from qllm2_amd.fused_ce import fused_linear_cross_entropy, linear_ce_per_token
+    for dtype in (F32, BF16):
+        h, w, ids, _ = _data(7, 20, 64, dtype, dtype, 32)
+        ids = ids.clamp(max=19)
+        f, k = LAYOUTS[name]
+        for a, b in ((f(h.cuda()), w.cuda()), (h.cuda(), k(w.cuda()))):
+            res = []
+            for x, y in ((a, b), (a.clone(memory_format=torch.contiguous_format), b.clone(memory_format=torch.contiguous_format))):
+                x, y = x.detach().requires_grad_(), y.detach().requires_grad_()
+                t = ids[:x.shape[0]].cuda()
+                loss = fused_linear_cross_entropy(x, y, t)
+                res.append([loss, linear_ce_per_token(x, y, t), *torch.autograd.grad(loss, [x, y])])
+            for s, t in zip(*res):
+                assert torch.equal(s, t)

@@ -283,3 +283,15 @@ def test_direct_operators_equal_the_dispatched_ones():
         d = torch.autograd.forward_ad.make_dual(a.clone().requires_grad_(), a)
         direct(d, a, 2.0)
     assert torch.equal(torch.compile(lambda x: direct(x, x, 2.0)[0], backend="eager", fullgraph=True)(a), a * 3)
+
+
+def test_linear_token_logprobs_columns_that_pad_to_the_limit():
+    """Columns are padded to whole 32, and the padded rows stay below 2^22 apart."""
+    from qllm2_amd.token_logprobs import MAX_D, MAX_STRIDE, _check_linear
+    assert MAX_D % 32 == 0 and MAX_D <= MAX_STRIDE < MAX_D + 32
+    with FakeTensorMode():
+        h, w = (torch.empty(n, MAX_D + 1, device="cuda") for n in (4, 9))
+        ids = torch.empty(4, device="cuda", dtype=torch.long)
+        with pytest.raises(ValueError, match="columns"):
+            _check_linear(h, w, ids, 1.0, 1)
+        _check_linear(h[:, :-1], w[:, :-1], ids, 1.0, 1)
