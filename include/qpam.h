@@ -814,7 +814,7 @@ int qpam_ce_bwd(const qpam_ce_bwd_args *a, void *stream);
  *
  * qpam_embed_fwd: out[i][j] = scale * (re[ids[i]][j], im[ids[i]][j]), out
  * [n][dim][2] contiguous, in dtype; an id outside [0, V) reads nothing and gives
- * a row of zeros.  Tables of row strides ld_re, ld_im (elements), unit column
+ * a row of `outside`.  Tables of row strides ld_re, ld_im (elements), unit column
  * stride, any alignment.
  * qpam_embed_bwd: d_re[v][j] = scale * sum of dz[i][j][0] over ids[i] == v, d_im
  * from dz[i][j][1]: fp32 sums in the order of i, rounded once to dtype.  Writes
@@ -829,6 +829,7 @@ typedef struct {
     const void *ids;
     int64_t padding_idx;           /* backward; negative: none */
     float scale;
+    float outside;                 /* forward: the value of rows whose id is outside [0, V) */
     const void *re; int64_t ld_re; /* forward */
     const void *im; int64_t ld_im;
     void *out;

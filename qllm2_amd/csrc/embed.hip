@@ -1,7 +1,8 @@
 // The complex embedding lookup with scaling, and its gradient by sorted tokens.
 //
 // Forward (ComplexEmbed.forward, v11/complex_ops.py:223-235):
-//   out[n][j] = scale (re[id_n][j], im[id_n][j]),  interleaved [n][dim][2].
+//   out[n][j] = scale (re[id_n][j], im[id_n][j]),  interleaved [n][dim][2];
+// a row of a given value (`outside`) where id_n is no row of the table.
 // Backward:
 //   d re[v][j] = scale sum_{n: id_n = v} dz[n][j][0],  d im from dz[n][j][1],
 // dense [V][dim] tables: tokens that do not occur get zeros.
@@ -58,8 +59,8 @@ __global__ void __launch_bounds__(THREADS) lookup_kernel(qpam_embed_args a, int 
         alignas(16) T o[2 * W];
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            o[2 * i] = ok ? to_elem<T>(Elem<T>::load(r + i) * a.scale) : T(0);
-            o[2 * i + 1] = ok ? to_elem<T>(Elem<T>::load(m + i) * a.scale) : T(0);
+            o[2 * i] = to_elem<T>(ok ? Elem<T>::load(r + i) * a.scale : a.outside);
+            o[2 * i + 1] = to_elem<T>(ok ? Elem<T>::load(m + i) * a.scale : a.outside);
         }
         if constexpr (W > 1) {
             uintx4 *dst = reinterpret_cast<uintx4 *>(out + 2 * j);

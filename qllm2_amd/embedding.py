@@ -39,7 +39,7 @@ def _check(ids, weight_real, weight_imag):
 
 
 def _args(ids, V, dim, dtype, padding_idx, scale, *more):
-    """EmbedArgs, `more` being the fields from `re` on."""
+    """EmbedArgs, `more` being the fields from `outside` on."""
     return _lib.EmbedArgs(ids.numel(), V, dim, _CODE[dtype], ids.dtype == torch.int64, ids.data_ptr(), padding_idx, scale,
                           *more)
 
@@ -48,14 +48,15 @@ def _rows(w):
     return w if w.stride(1) == 1 and w.stride(0) >= w.shape[1] else w.contiguous()
 
 
-def _lookup(ids: Tensor, weight_real: Tensor, weight_imag: Tensor, scale: float, padding_idx: int) -> Tensor:
+def _lookup(ids: Tensor, weight_real: Tensor, weight_imag: Tensor, scale: float, padding_idx: int,
+            outside: float = 0.0) -> Tensor:
     """[*ids.shape, dim, 2] in the tables' dtype."""
     _check(ids, weight_real, weight_imag)
     V, dim = weight_real.shape
     ids, re, im = ids.contiguous(), _rows(weight_real), _rows(weight_imag)
     dev = re.device
     out = torch.empty(*ids.shape, dim, 2, device=dev, dtype=re.dtype)
-    a = _args(ids, V, dim, re.dtype, padding_idx, scale, re.data_ptr(), re.stride(0), im.data_ptr(), im.stride(0),
+    a = _args(ids, V, dim, re.dtype, padding_idx, scale, outside, re.data_ptr(), re.stride(0), im.data_ptr(), im.stride(0),
               out.data_ptr())
     with _lib.device(dev):
         _lib.check(_lib.lib().qpam_embed_fwd(ctypes.byref(a), _lib.stream_ptr(dev)), "qpam_embed_fwd")
@@ -66,7 +67,7 @@ embed_fwd_op = _ops.op("qpam::embed_fwd", direct=True)(_lookup)
 
 
 @embed_fwd_op.register_fake
-def _(ids, weight_real, weight_imag, scale, padding_idx):
+def _(ids, weight_real, weight_imag, scale, padding_idx, outside=0.0):
     return weight_real.new_empty(*ids.shape, weight_real.shape[1], 2)
 
 
@@ -77,7 +78,7 @@ def _gradient(ids: Tensor, dz: Tensor, num_embeddings: int, scale: float, paddin
     if dz.data_ptr() % 16:
         dz = dz.clone()
     grads = [torch.empty(num_embeddings, dim, device=dz.device, dtype=dz.dtype) for _ in range(2)]
-    a = _args(ids, num_embeddings, dim, dz.dtype, padding_idx, scale, None, 0, None, 0, None, dz.data_ptr(),
+    a = _args(ids, num_embeddings, dim, dz.dtype, padding_idx, scale, 0.0, None, 0, None, 0, None, dz.data_ptr(),
               grads[0].data_ptr(), grads[1].data_ptr())
     L = _lib.lib()
     nbytes = L.qpam_embed_bwd_workspace_size(ctypes.byref(a))
@@ -97,29 +98,30 @@ def _(ids, dz, num_embeddings, scale, padding_idx):
 
 
 def _setup(ctx, inputs, output):
-    ids, weight_real, _, ctx.scale, ctx.padding_idx = inputs
+    ids, weight_real, _, ctx.scale, ctx.padding_idx, _ = inputs
     ctx.save_for_backward(ids)
     ctx.num_embeddings, ctx.dtype = weight_real.shape[0], weight_real.dtype
 
 
 def _backward(ctx, dz):
     if dz is None:
-        return None, None, None, None, None
+        return None, None, None, None, None, None
     ids, = ctx.saved_tensors
     d_re, d_im = embed_bwd_op(ids, dz.to(ctx.dtype), ctx.num_embeddings, ctx.scale, ctx.padding_idx)
-    return None, d_re, d_im, None, None
+    return None, d_re, d_im, None, None, None
 
 
 embed_fwd_op.register_autograd(_backward, setup_context=_setup)
 
 
 def complex_embedding(ids: Tensor, weight_real: Tensor, weight_imag: Tensor, scale: float = 1.0,
-                      padding_idx: Optional[int] = None) -> Tensor:
+                      padding_idx: Optional[int] = None, outside: float = 0.0) -> Tensor:
     """scale * (weight_real[ids], weight_imag[ids]) as [*ids.shape, dim, 2] in the
     tables' dtype (float32 or bfloat16; products in fp32, rounded once).
 
     ids int64 or int32, any shape; tables [V, dim], rows of any stride.  An id
-    outside [0, V) gives a row of zeros and no gradient.  padding_idx (of [-V, V),
+    outside [0, V) gives a row of `outside` (zeros; NaN where it must not pass for a
+    token) and no gradient.  padding_idx (of [-V, V),
     as nn.Embedding's) is looked up like any id and gets no gradient.
     Differentiable in both tables (dense gradients, once: a second derivative
     raises)."""
@@ -129,4 +131,4 @@ def complex_embedding(ids: Tensor, weight_real: Tensor, weight_imag: Tensor, sca
         if not -V <= padding_idx < V:
             raise ValueError(f"qpam complex_embedding: padding_idx {padding_idx} outside [-{V}, {V})")
         pad = padding_idx + V if padding_idx < 0 else padding_idx
-    return embed_fwd_op(ids, weight_real, weight_imag, float(scale), pad)
+    return embed_fwd_op(ids, weight_real, weight_imag, float(scale), pad, float(outside))

@@ -221,8 +221,9 @@ class ModelDecoder:
         return F.linear(g.view(n, -1), blk["w_down"]).view(n, self.dim, 2)
 
     def _embedded(self, ids):
-        """Normed embedding rows [n, dim, 2] of ids [n]: the fp32 residual stream."""
-        return self._norm(complex_embedding(ids, *self._embed), self._norm_e)
+        """Normed embedding rows [n, dim, 2] of ids [n]: the fp32 residual stream (NaN for an
+        id outside the vocabulary)."""
+        return self._norm(complex_embedding(ids, *self._embed, outside=float("nan")), self._norm_e)
 
     def _lm_rows(self, h):
         """The LM head's rows [n, 2 dim] (GEMM dtype) from output-normed rows h [n, dim, 2]."""
@@ -266,13 +267,21 @@ class ModelDecoder:
                            y_scale=blk["pam_scale"], out_dtype=dt)
         return h, states
 
+    def _device_ids(self, ids):
+        """ids on the decoder's device.  Those that come from the host are checked there; reading
+        back those on the device would wait for it, so a wrong one decodes to NaN instead."""
+        if not ids.is_cuda and ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < self.vocab:
+            raise ValueError(f"ModelDecoder: token ids outside the vocabulary [0, {self.vocab})")
+        return ids.to(self._embed[0].device)
+
     def _prompt_ids(self, prompt_ids):
-        return prompt_ids.to(self._embed[0].device).long().view(-1)
+        return self._device_ids(prompt_ids).long().view(-1)
 
     @torch.no_grad()
     def prefill(self, prompt_ids):
         """The model over one prompt (ids [T]) with the fused PAM prefill:
-        (logits of its last token [V], the per-layer states)."""
+        (logits of its last token [V], the per-layer states).  Ids outside the vocabulary:
+        ValueError for a host tensor, NaN logits and states for one on the device."""
         h, states = self._prompt_rows(self._prompt_ids(prompt_ids))
         return self._head(h[-1:])[0], states
 
@@ -280,12 +289,16 @@ class ModelDecoder:
     def score(self, ids, temperature=1.0):
         """Of one sequence ids [T], T >= 2: for each token after the first, the log
         probability the model gives it after those before it, and the entropy of that
-        choice, fp32 [T - 1] each; no logits in memory."""
-        ids = self._prompt_ids(ids)
+        choice, fp32 [T - 1] each; no logits in memory.  Ids outside the vocabulary:
+        ValueError for a host tensor; in one on the device they and what follows score NaN."""
+        ids, on_device = self._prompt_ids(ids), ids.is_cuda
         if ids.numel() < 2:
             raise ValueError("ModelDecoder.score: at least two tokens")
         h, _ = self._prompt_rows(ids)
-        return linear_token_logprobs(self._lm_rows(h[:-1]), self._embed_w, ids[1:], temperature=temperature)
+        r = linear_token_logprobs(self._lm_rows(h[:-1]), self._embed_w, ids[1:], temperature=temperature)
+        if on_device:  # a row without a token would have log probability 0
+            r = r._replace(logprobs=r.logprobs.masked_fill((ids[1:] < 0) | (ids[1:] >= self.vocab), float("nan")))
+        return r
 
     def admit(self, prompt_ids):
         """A sequence with this prompt joins: its prefill's states enter a
@@ -304,10 +317,11 @@ class ModelDecoder:
     def step(self, ids, slots, host_slots=None):
         """One token of each listed sequence through the whole model: ids [n]
         (the tokens, device int64), slots [n] (int32 device, distinct live
-        slots).  Returns the next-token logits [n, V] (fp32; with graphs a
+        slots).  An id outside the vocabulary gives its own sequence NaN logits and
+        states from there on (ids of a host tensor: ValueError).  Returns the next-token logits [n, V] (fp32; with graphs a
         view of the graph's output buffer, valid until the bucket's next step)
         and advances the positions."""
-        n = ids.shape[0]
+        ids, n = self._device_ids(ids), ids.shape[0]
         if not self.graph_bucket:
             out = self._tokens(ids, slots)
             self.pool.advance(slots, host_slots)

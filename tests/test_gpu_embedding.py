@@ -249,3 +249,23 @@ def test_more_rows_than_one_launch_holds(gpu_lib):
     for rows in (slice(0, 3), slice(2 ** 25 - 4, n)):
         t = ids[rows].long()
         assert torch.equal(z[rows], torch.stack([re[t], im[t]], -1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("outside", [0.0, -2.5, float("inf"), float("nan")])
+@pytest.mark.parametrize("dim", [32, 7])
+def test_rows_of_ids_outside_the_table(gpu_lib, dim, outside, dtype):
+    """`outside` as it is, in whole rows; the table's rows and both gradients as without it."""
+    from qllm2_amd.embedding import complex_embedding
+    g = torch.Generator().manual_seed(dim)
+    re, im = (torch.randn(20, dim, generator=g).to(dtype).cuda().requires_grad_() for _ in range(2))
+    ids = torch.tensor([3, 20, -1, 0, 19, 2 ** 40, -2 ** 40, 3], device="cuda")
+    bad = (ids < 0) | (ids >= 20)
+    z = complex_embedding(ids, re, im, scale=1.5, outside=outside)
+    want = torch.full((4, dim, 2), outside, dtype=dtype, device="cuda")
+    assert torch.allclose(z[bad], want, rtol=0, atol=0, equal_nan=True)
+    plain = complex_embedding(ids, re, im, scale=1.5)
+    assert torch.equal(z[~bad], plain[~bad])
+    dz = torch.randn(8, dim, 2, generator=g).to(dtype).cuda()
+    for a, b in zip(torch.autograd.grad(z, [re, im], dz), torch.autograd.grad(plain, [re, im], dz)):
+        assert torch.equal(a, b)

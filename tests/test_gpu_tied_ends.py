@@ -179,3 +179,44 @@ def test_compiled_program_traces_the_operators(gpu_lib):
 
     for got, want in zip(torch.compile(f, backend="eager", fullgraph=True)(ids, re, im, w), f(ids, re, im, w)):
         assert torch.equal(got, want)
+
+
+def _decoder(dtype, graphs):
+    from qllm2_amd.model_decode import ModelDecoder
+    cfg = dict(dim=128, n_heads=2, head_dim=64, n_states=1, chunk_size=64)
+    p = VM.make_model_params(cfg, 2, 300, 78)
+    gpu = VM.V11LM(cfg, 2, {k: v.float() for k, v in p.items()}, dtype=torch.float32).cuda().eval()
+    return ModelDecoder(gpu, n_slots=4, max_len=64, dtype=dtype, graphs=graphs, graph_bucket=2)
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_model_decoder_ids_outside_the_vocabulary(gpu_lib, graphs):
+    """Host ids are refused; ids on the device, which the host does not read, give NaN logits, states and
+    scores from there on, in their own sequence alone (within a prompt the prefill's products of a chunk
+    may spread them to the tokens before)."""
+    dec = _decoder(torch.float32, graphs)
+    ok = torch.randint(0, 300, (9,), generator=torch.Generator().manual_seed(6))
+    for wrong in (300, -1, -100, 2 ** 40):
+        bad = ok.clone()
+        bad[4] = wrong
+        for call in (dec.prefill, dec.admit, dec.score):
+            with pytest.raises(ValueError, match="vocabulary"):
+                call(bad)
+        assert dec.prefill(bad.cuda())[0].isnan().all()
+        s = dec.score(bad.cuda())
+        assert s.logprobs[3:].isnan().all() and s.entropy[4:].isnan().all()
+        bad = ok.clone()
+        bad[-1] = wrong
+        assert dec.score(bad.cuda()).logprobs[-1].isnan()
+    assert torch.equal(dec.score(ok).logprobs, dec.score(ok.cuda()).logprobs)
+    first, _ = dec.admit(ok)
+    second, _ = dec.admit(ok.cuda())
+    slots, host = torch.tensor([first, second], dtype=torch.int32, device="cuda"), [first, second]
+    with pytest.raises(ValueError, match="vocabulary"):
+        dec.step(torch.tensor([5, 300]), slots, host)
+    a = dec.step(torch.tensor([5, 5], device="cuda"), slots, host).clone()
+    assert torch.equal(a[0], a[1])
+    b = dec.step(torch.tensor([7, 300], device="cuda"), slots, host).clone()
+    assert not b[0].isnan().any() and b[1].isnan().all()
+    c = dec.step(torch.tensor([8, 8]), slots, host).clone()    # host ids, as device ids
+    assert not c[0].isnan().any() and c[1].isnan().all()

@@ -295,3 +295,16 @@ def test_linear_token_logprobs_columns_that_pad_to_the_limit():
         with pytest.raises(ValueError, match="columns"):
             _check_linear(h, w, ids, 1.0, 1)
         _check_linear(h[:, :-1], w[:, :-1], ids, 1.0, 1)
+
+
+def test_model_decoder_refuses_host_ids_outside_the_vocabulary():
+    """Before anything moves to the device."""
+    from qllm2_amd.model_decode import ModelDecoder
+    dec = object.__new__(ModelDecoder)
+    dec.vocab, dec._embed = 300, [torch.empty(0)]
+    assert dec._device_ids(torch.tensor([0, 299])).tolist() == [0, 299]
+    assert dec._device_ids(torch.empty(0, dtype=torch.long)).numel() == 0
+    for wrong in ([5, 300], [-1], [0, 2 ** 40]):
+        for call in (dec.prefill, dec.admit, dec.score, lambda ids: dec.step(ids, None)):
+            with pytest.raises(ValueError, match="vocabulary"):
+                call(torch.tensor(wrong))
