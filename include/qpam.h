@@ -814,8 +814,9 @@ int qpam_ce_bwd(const qpam_ce_bwd_args *a, void *stream);
  *
  * qpam_embed_fwd: out[i][j] = scale * (re[ids[i]][j], im[ids[i]][j]), out
  * [n][dim][2] contiguous, in dtype; an id outside [0, V) reads nothing and gives
- * a row of `outside`.  Tables of row strides ld_re, ld_im (elements), unit column
- * stride, any alignment.
+ * a row of `outside`.  Tables of row strides ld_re, ld_im and column strides cs_re,
+ * cs_im (elements; rows apart by their length or more), any alignment: one
+ * interleaved table [V][dim][2] is im = re + 1 with column strides of 2.
  * qpam_embed_bwd: d_re[v][j] = scale * sum of dz[i][j][0] over ids[i] == v, d_im
  * from dz[i][j][1]: fp32 sums in the order of i, rounded once to dtype.  Writes
  * both contiguous [V][dim] tables (zeros for tokens that do not occur); ids
@@ -830,8 +831,8 @@ typedef struct {
     int64_t padding_idx;           /* backward; negative: none */
     float scale;
     float outside;                 /* forward: the value of rows whose id is outside [0, V) */
-    const void *re; int64_t ld_re; /* forward */
-    const void *im; int64_t ld_im;
+    const void *re; int64_t ld_re, cs_re; /* forward */
+    const void *im; int64_t ld_im, cs_im;
     void *out;
     const void *dz;                /* backward */
     void *d_re, *d_im;

@@ -12,7 +12,7 @@ import os
 import torch  # noqa: F401  (must be loaded before the HIP library)
 
 LIB_NAME = "libqpam.so"
-ABI_VERSION = 17
+ABI_VERSION = 18
 _HERE = os.path.dirname(os.path.abspath(__file__))
 
 QPAM_F32 = 0
@@ -258,8 +258,8 @@ class PlanesArgs(ctypes.Structure):
 class EmbedArgs(ctypes.Structure):
     _fields_ = [
         ("n", c_i64), ("V", c_i32), ("dim", c_i32), ("dtype", c_i32), ("ids_i64", c_i32), ("ids", c_ptr),
-        ("padding_idx", c_i64), ("scale", c_f32), ("outside", c_f32), ("re", c_ptr), ("ld_re", c_i64), ("im", c_ptr), ("ld_im", c_i64),
-        ("out", c_ptr), ("dz", c_ptr), ("d_re", c_ptr), ("d_im", c_ptr), ("workspace", c_ptr),
+        ("padding_idx", c_i64), ("scale", c_f32), ("outside", c_f32), ("re", c_ptr), ("ld_re", c_i64),
+        ("cs_re", c_i64), ("im", c_ptr), ("ld_im", c_i64), ("cs_im", c_i64), ("out", c_ptr), ("dz", c_ptr), ("d_re", c_ptr), ("d_im", c_ptr), ("workspace", c_ptr),
         ("workspace_bytes", ctypes.c_size_t),
     ]
 

@@ -38,9 +38,10 @@ __device__ __forceinline__ int64_t load_id(const void *ids, int is64, int64_t i)
 // ---------------------------------------------------------------- lookup ---
 // W complex values of one table row per lane and step: 16 bytes of each table in, two
 // 16-byte stores out.  Lanes to a row: the least power of two that covers it, at most a
-// wave, so that short rows share waves.  Bound by the launch (192 rows of 768 fp32: 3.3
+// wave, so that short rows share waves.  PAIRS: one interleaved table [V][dim][2] (im = re + 1,
+// columns two apart), whose rows are the output's form already.  W = 1: any column strides.  Bound by the launch (192 rows of 768 fp32: 3.3
 // us) or by HBM (16384 rows of 512 bf16, 33 MB written and as much read: 12.9 us).
-template <typename T, int W>
+template <typename T, int W, bool PAIRS>
 __global__ void __launch_bounds__(THREADS) lookup_kernel(qpam_embed_args a, int lanes_log2) {
     typedef T VecT __attribute__((ext_vector_type(W)));
     const int lanes = 1 << lanes_log2;  // lanes that share a row
@@ -53,15 +54,19 @@ __global__ void __launch_bounds__(THREADS) lookup_kernel(qpam_embed_args a, int 
     const T *im = static_cast<const T *>(a.im) + (ok ? id : 0) * a.ld_im;
     T *out = static_cast<T *>(a.out) + row * 2 * a.dim;
     for (int j = W * (int)(gid & (lanes - 1)); j < a.dim; j += W * lanes) {
-        T r[W], m[W];
-        *reinterpret_cast<VecT *>(r) = *reinterpret_cast<const VecT *>(re + j);
-        *reinterpret_cast<VecT *>(m) = *reinterpret_cast<const VecT *>(im + j);
-        alignas(16) T o[2 * W];
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            o[2 * i] = to_elem<T>(ok ? Elem<T>::load(r + i) * a.scale : a.outside);
-            o[2 * i + 1] = to_elem<T>(ok ? Elem<T>::load(m + i) * a.scale : a.outside);
+        alignas(16) T x[2 * W], o[2 * W];  // PAIRS: as they stand; otherwise the reals, then the imaginaries
+        if constexpr (PAIRS) {
+            *reinterpret_cast<VecT *>(x) = *reinterpret_cast<const VecT *>(re + 2 * j);
+            *reinterpret_cast<VecT *>(x + W) = *reinterpret_cast<const VecT *>(re + 2 * j + W);
+        } else if constexpr (W > 1) {
+            *reinterpret_cast<VecT *>(x) = *reinterpret_cast<const VecT *>(re + j);
+            *reinterpret_cast<VecT *>(x + W) = *reinterpret_cast<const VecT *>(im + j);
+        } else {
+            x[0] = re[j * a.cs_re];
+            x[1] = im[j * a.cs_im];
         }
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) o[i] = to_elem<T>(ok ? Elem<T>::load(x + (PAIRS ? i : i / 2 + i % 2 * W)) * a.scale : a.outside);
         if constexpr (W > 1) {
             uintx4 *dst = reinterpret_cast<uintx4 *>(out + 2 * j);
             dst[0] = reinterpret_cast<const uintx4 *>(o)[0];
@@ -487,8 +492,10 @@ int check(const qpam_embed_args &a, const char *who) {
 template <typename T>
 int run_lookup(const qpam_embed_args &a, hipStream_t stream) {
     constexpr int W = 16 / sizeof(T);
-    const bool wide = a.dim % W == 0 && a.ld_re % W == 0 && a.ld_im % W == 0 && ((uintptr_t)a.re % 16) == 0 &&
-                      ((uintptr_t)a.im % 16) == 0 && ((uintptr_t)a.out % 16) == 0;
+    const bool rows = a.dim % W == 0 && a.ld_re % W == 0 && ((uintptr_t)a.re % 16) == 0 && ((uintptr_t)a.out % 16) == 0;
+    const bool planes = rows && a.cs_re == 1 && a.cs_im == 1 && a.ld_im % W == 0 && ((uintptr_t)a.im % 16) == 0;
+    const bool pairs = rows && a.cs_re == 2 && a.cs_im == 2 && a.ld_im == a.ld_re && a.im == static_cast<const T *>(a.re) + 1;
+    const bool wide = planes || pairs;
     const int steps = wide ? a.dim / W : a.dim;
     int lg = 0;
     while (lg < 6 && (1 << lg) < steps) ++lg;
@@ -499,10 +506,12 @@ int run_lookup(const qpam_embed_args &a, hipStream_t stream) {
         s.ids = static_cast<const char *>(a.ids) + n0 * (a.ids_i64 ? 8 : 4);
         s.out = static_cast<T *>(a.out) + n0 * 2 * a.dim;
         const unsigned blocks = (unsigned)(((s.n << lg) + THREADS - 1) / THREADS);
-        if (wide)
-            hipLaunchKernelGGL((lookup_kernel<T, W>), dim3(blocks), dim3(THREADS), 0, stream, s, lg);
+        if (pairs)
+            hipLaunchKernelGGL((lookup_kernel<T, W, true>), dim3(blocks), dim3(THREADS), 0, stream, s, lg);
+        else if (planes)
+            hipLaunchKernelGGL((lookup_kernel<T, W, false>), dim3(blocks), dim3(THREADS), 0, stream, s, lg);
         else
-            hipLaunchKernelGGL((lookup_kernel<T, 1>), dim3(blocks), dim3(THREADS), 0, stream, s, lg);
+            hipLaunchKernelGGL((lookup_kernel<T, 1, false>), dim3(blocks), dim3(THREADS), 0, stream, s, lg);
         const int st = launch_status("embed lookup_kernel");
         if (st) return st;
     }
@@ -591,7 +600,9 @@ extern "C" int qpam_embed_fwd(const qpam_embed_args *a, void *stream) {
     int st = check(*a, "qpam_embed_fwd");
     if (st || a->n == 0) return st;
     QPAM_REQUIRE(a->re && a->im && a->out, "qpam_embed_fwd: null table or output");
-    QPAM_REQUIRE(a->ld_re >= a->dim && a->ld_im >= a->dim, "qpam_embed_fwd: table row strides below dim");
+    auto fits = [&](int64_t ld, int64_t cs) { return cs >= 1 && cs <= ((int64_t)1 << 40) && ld > (a->dim - 1) * cs; };
+    QPAM_REQUIRE(fits(a->ld_re, a->cs_re) && fits(a->ld_im, a->cs_im),
+                 "qpam_embed_fwd: table column strides below 1, or row strides below a row");
     return a->dtype == QPAM_BF16 ? run_lookup<unsigned short>(*a, (hipStream_t)stream)
                                  : run_lookup<float>(*a, (hipStream_t)stream);
 }

@@ -44,8 +44,14 @@ def _args(ids, V, dim, dtype, padding_idx, scale, *more):
                           *more)
 
 
-def _rows(w):
-    return w if w.stride(1) == 1 and w.stride(0) >= w.shape[1] else w.contiguous()
+def _table(w):
+    """w [V, dim] with its strides as the kernel reads them: columns apart, rows apart by their length; a copy
+    where it is not (a transposed or expanded table)."""
+    dim = w.shape[1]
+    cs = w.stride(1) if dim > 1 else 1
+    if cs < 1 or w.stride(0) <= (dim - 1) * cs:
+        w, cs = w.contiguous(), 1
+    return w, max(w.stride(0), dim), cs
 
 
 def _lookup(ids: Tensor, weight_real: Tensor, weight_imag: Tensor, scale: float, padding_idx: int,
@@ -53,10 +59,10 @@ def _lookup(ids: Tensor, weight_real: Tensor, weight_imag: Tensor, scale: float,
     """[*ids.shape, dim, 2] in the tables' dtype."""
     _check(ids, weight_real, weight_imag)
     V, dim = weight_real.shape
-    ids, re, im = ids.contiguous(), _rows(weight_real), _rows(weight_imag)
+    ids, (re, ld_re, cs_re), (im, ld_im, cs_im) = ids.contiguous(), _table(weight_real), _table(weight_imag)
     dev = re.device
     out = torch.empty(*ids.shape, dim, 2, device=dev, dtype=re.dtype)
-    a = _args(ids, V, dim, re.dtype, padding_idx, scale, outside, re.data_ptr(), re.stride(0), im.data_ptr(), im.stride(0),
+    a = _args(ids, V, dim, re.dtype, padding_idx, scale, outside, re.data_ptr(), ld_re, cs_re, im.data_ptr(), ld_im, cs_im,
               out.data_ptr())
     with _lib.device(dev):
         _lib.check(_lib.lib().qpam_embed_fwd(ctypes.byref(a), _lib.stream_ptr(dev)), "qpam_embed_fwd")
@@ -78,7 +84,7 @@ def _gradient(ids: Tensor, dz: Tensor, num_embeddings: int, scale: float, paddin
     if dz.data_ptr() % 16:
         dz = dz.clone()
     grads = [torch.empty(num_embeddings, dim, device=dz.device, dtype=dz.dtype) for _ in range(2)]
-    a = _args(ids, num_embeddings, dim, dz.dtype, padding_idx, scale, 0.0, None, 0, None, 0, None, dz.data_ptr(),
+    a = _args(ids, num_embeddings, dim, dz.dtype, padding_idx, scale, 0.0, None, 0, 0, None, 0, 0, None, dz.data_ptr(),
               grads[0].data_ptr(), grads[1].data_ptr())
     L = _lib.lib()
     nbytes = L.qpam_embed_bwd_workspace_size(ctypes.byref(a))
@@ -119,7 +125,8 @@ def complex_embedding(ids: Tensor, weight_real: Tensor, weight_imag: Tensor, sca
     """scale * (weight_real[ids], weight_imag[ids]) as [*ids.shape, dim, 2] in the
     tables' dtype (float32 or bfloat16; products in fp32, rounded once).
 
-    ids int64 or int32, any shape; tables [V, dim], rows of any stride.  An id
+    ids int64 or int32, any shape; tables [V, dim], rows and columns of any
+    stride: those of one interleaved [V, dim, 2] are read where they stand.  An id
     outside [0, V) gives a row of `outside` (zeros; NaN where it must not pass for a
     token) and no gradient.  padding_idx (of [-V, V),
     as nn.Embedding's) is looked up like any id and gets no gradient.

@@ -7,7 +7,7 @@ batch that shares one step_offset; here sequences join (admit: their prompt's
 prefill) and leave (release) between steps, each keeps its own position, and a
 step runs only the live rows:
 
-  embedding rows of the tokens, both tables' in one launch (qpam_embed_fwd)
+  embedding rows of the tokens (the tied table, interleaved [V, dim, 2]; qpam_embed_fwd)
   -> ComplexNorm                                     (qpam_cplx_fwd)
   -> per block (v11/model.py:1038-1049), h = norm1(x) from the step before:
        x += cgu_scale * down(cgu_gate(gate(h), act(up(h))))
@@ -167,11 +167,10 @@ class ModelDecoder:
         self._wver += 1
         self.engine.refresh_weights()
         with torch.no_grad():
-            tables = (m.embed.embed_real.weight, m.embed.embed_imag.weight)
-            e = torch.stack(tables, -1).float()                                                  # [V, dim, 2]
+            e = torch.stack([m.embed.embed_real.weight, m.embed.embed_imag.weight], -1).float()  # [V, dim, 2]
             self.vocab, self.dim = e.shape[0], e.shape[1]
-            self._embed = [t.detach().float().contiguous().clone() for t in tables]              # fp32, lookups
-            self._embed_w = e.reshape(self.vocab, 2 * self.dim).to(dt).contiguous()           # logits GEMM
+            self._embed = e.contiguous().unbind(-1)                                               # fp32, lookups
+            self._embed_w = e.reshape(self.vocab, 2 * self.dim).to(dt).contiguous()           # logits GEMM, fp32: the same memory
             self._blk = []
             if self.dim % 4 or self.dim > MAX_DIM:
                 raise NotImplementedError(f"ModelDecoder: dim {self.dim} (a multiple of 4 up to {MAX_DIM})")

@@ -269,3 +269,39 @@ def test_rows_of_ids_outside_the_table(gpu_lib, dim, outside, dtype):
     dz = torch.randn(8, dim, 2, generator=g).to(dtype).cuda()
     for a, b in zip(torch.autograd.grad(z, [re, im], dz), torch.autograd.grad(plain, [re, im], dz)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [1, 7, 64, 100])
+def test_tables_of_any_column_stride(gpu_lib, dim, dtype):
+    """Views of one interleaved table (16-byte aligned and not), columns two and five apart, a transposed and an
+    expanded table: the bits of contiguous ones, with both gradients."""
+    from qllm2_amd.embedding import complex_embedding
+    g = torch.Generator().manual_seed(dim)
+    rn = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()  # noqa: E731
+    ids, dz = torch.randint(-1, 31, (2, 40), generator=g).cuda(), rn(2, 40, dim, 2)
+    flat = rn(30 * dim * 2 + 1)[1:].view(30, dim, 2)
+    tables = [rn(30, dim, 2).unbind(-1), rn(30, dim, 2).unbind(-1)[::-1], flat.unbind(-1), rn(30, dim + 3, 2)[:, 2:2 + dim].unbind(-1),
+              (rn(30, dim * 5)[:, ::5], rn(30, dim * 2)[:, 1::2]), (rn(dim, 30).T, rn(30, dim)), (rn(1, dim).expand(30, dim), rn(30, dim)),
+              (rn(30, 1).expand(30, dim), rn(30, 2 * dim).view(30, dim, 2)[..., 0])]
+    for re, im in tables:
+        res = []
+        for a, b in ((re, im), (re.clone(memory_format=torch.contiguous_format), im.clone(memory_format=torch.contiguous_format))):
+            a, b = a.detach().requires_grad_(), b.detach().requires_grad_()
+            z = complex_embedding(ids, a, b, scale=1.5, padding_idx=3)
+            res.append([z, *torch.autograd.grad(z, [a, b], dz)])
+        for s, t in zip(*res):
+            assert torch.equal(s, t)
+
+
+def test_interleaved_tables_are_not_copied(gpu_lib):
+    from qllm2_amd.embedding import complex_embedding
+    for dtype in (torch.float32, torch.bfloat16):
+        table = torch.randn(20000, 64, 2, device="cuda").to(dtype)
+        ids = torch.arange(50, device="cuda")
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        z = complex_embedding(ids, *table.unbind(-1))
+        assert torch.equal(z, table[:50])
+        assert torch.cuda.max_memory_allocated() - before < table.numel() * table.element_size() // 4

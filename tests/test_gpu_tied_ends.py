@@ -220,3 +220,9 @@ def test_model_decoder_ids_outside_the_vocabulary(gpu_lib, graphs):
     assert not b[0].isnan().any() and b[1].isnan().all()
     c = dec.step(torch.tensor([8, 8]), slots, host).clone()    # host ids, as device ids
     assert not c[0].isnan().any() and c[1].isnan().all()
+
+
+def test_model_decoder_keeps_one_fp32_table(gpu_lib):
+    """The lookups read the LM head's own table where that is fp32."""
+    dec = _decoder(torch.float32, False)
+    assert {t.untyped_storage().data_ptr() for t in dec._embed} == {dec._embed_w.untyped_storage().data_ptr()}
