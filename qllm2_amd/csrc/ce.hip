@@ -1331,9 +1331,6 @@ __device__ __forceinline__ void dma_mma(const U16 *sA, const U16 *sB, floatx4 (&
     }
 }
 
-// s_waitcnt with vmcnt <= 8 and the other counters unconstrained
-constexpr int WAIT_VM8 = 8 | 0x70 | 0xF00;
-
 __device__ __forceinline__ void wgemm_tile_dma(const U16 *A, int64_t lda, int a_rows, const U16 *B, int64_t ldb,
                                                int b_rows, int K, floatx4 (&acc)[4][8]) {
     __shared__ __align__(16) U16 sA0[TM * DK], sA1[TM * DK], sA2[TM * DK], sA3[TM * DK];
@@ -1348,14 +1345,12 @@ __device__ __forceinline__ void wgemm_tile_dma(const U16 *A, int64_t lda, int a_
     dma_stage<0>(sA0, sB0, A, lda, a_rows, B, ldb, b_rows, 0);
     dma_stage<1>(sA1, sB1, A, lda, a_rows, B, ldb, b_rows, min(1, KT - 1) * DK);
     dma_stage<2>(sA2, sB2, A, lda, a_rows, B, ldb, b_rows, min(2, KT - 1) * DK);
-    __builtin_amdgcn_s_waitcnt(WAIT_VM8);
-    __builtin_amdgcn_s_barrier();
+    stage_barrier<8>();
 #define QPAM_DMA_STEP(KT_, CUR_A, CUR_B, NXT_A, NXT_B, NS)                                                    \
     dma_stage<NS>(NXT_A, NXT_B, A, lda, a_rows, B, ldb, b_rows, min((KT_) + 3, KT - 1) * DK);                 \
     __builtin_amdgcn_sched_barrier(0);                                                                         \
     dma_mma(CUR_A, CUR_B, acc, arow0, brow0, l16, g);                                                          \
-    __builtin_amdgcn_s_waitcnt(WAIT_VM8);                                                                      \
-    __builtin_amdgcn_s_barrier();
+    stage_barrier<8>();
     int kt = 0;
     for (; kt + 3 < KT; kt += 4) {
         QPAM_DMA_STEP(kt, sA0, sB0, sA3, sB3, 3)
@@ -1695,8 +1690,7 @@ __device__ __forceinline__ void product(const Stages &st, const Loads &q, int KT
     // fragment (row, chunk g); the swizzle repeats every eight rows
     const int aat = (64 * (w >> 1) + l16) * DK + 8 * wide::swz(l16, g);
     const int bat = (16 * NI * (w & 1) + l16) * DK + 8 * wide::swz(l16, g);
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(4));
-    __builtin_amdgcn_s_barrier();
+    stage_barrier<4>();
     Frags<NI> f0, f1;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1706,8 +1700,7 @@ __device__ __forceinline__ void product(const Stages &st, const Loads &q, int KT
 #define QPAM_STEP(KT_, CUR, STAGE, NEXT, NEXT_STAGE, FREE)                                     \
     load(FREE, q, min((KT_) + 3, KT - 1));                                                     \
     step(CUR, STAGE, NEXT, NEXT_STAGE, acc, aat, bat);                                         \
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(4));                                                 \
-    __builtin_amdgcn_s_barrier();
+    stage_barrier<4>();
     int kt = 0;
     for (; kt + 3 < KT; kt += 4) {
         QPAM_STEP(kt, f0, s0, f1, s1, s3)
@@ -1719,8 +1712,7 @@ __device__ __forceinline__ void product(const Stages &st, const Loads &q, int KT
     if (kt + 1 < KT) { QPAM_STEP(kt + 1, f1, s1, f0, s2, s0) }
     if (kt + 2 < KT) { QPAM_STEP(kt + 2, f0, s2, f1, s3, s1) }
 #undef QPAM_STEP
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-    __builtin_amdgcn_s_barrier();
+    stage_barrier<0>();
 }
 
 // The block's LDS writes before it are read after it; loads and stores stay in flight.
@@ -2017,8 +2009,7 @@ __global__ void __launch_bounds__(TT) gemm_kernel(const U16 *A, int64_t lda, int
         for (int ni = 0; ni < 8; ++ni) acc[mi][ni] = floatx4{0.f, 0.f, 0.f, 0.f};
     // the stage after this one is in LDS, and every wave is done reading this one
     auto landed = [&]() {
-        __builtin_amdgcn_s_waitcnt(waitcnt_vm(8) & ~0xF00);
-        __builtin_amdgcn_s_barrier();
+        stage_barrier<8>();
         wave_lds_order();
     };
     load(s0, 0);
@@ -2106,9 +2097,9 @@ __device__ __forceinline__ void mma(uintx4 w, uintx4 h, floatx4 &acc, float) {
 __device__ __forceinline__ void to_lds(const char *from, char *lds) {
     __builtin_amdgcn_global_load_lds(reinterpret_cast<const unsigned *>(from), reinterpret_cast<unsigned *>(lds), 16, 0, 0);
 }
-// direct loads still in flight at most `n`, and LDS reads stay behind the wait
+// direct loads still in flight at most `n`, the wave's LDS reads are done and later ones stay behind the wait
 template <int N> __device__ __forceinline__ void landed() {
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(N));
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(N) & ~0xF00);
     wave_lds_order();
 }
 
@@ -2176,7 +2167,7 @@ __global__ void __launch_bounds__(64 * NW) scores_kernel(FwdParams p) {
     load_w(WC, 2 * (J) + 2);                                                                    \
     landed<4 + HI>();                                                                           \
     multiply(WA, H, 2 * (J));                                                                   \
-    wave_lds_order();                                                                           \
+    wide::wave_lds_sync();                                                                      \
     load_w(WA, 2 * (J) + 3);                                                                    \
     landed<4 + HI>();                                                                           \
     multiply(WB_, H, 2 * (J) + 1);                                                              \

@@ -49,6 +49,15 @@ std::mutex &side_stream_mutex();
 // vmcnt is split over bits [3:0] and [15:14], expcnt is bits [6:4], lgkmcnt [11:8]
 constexpr int waitcnt_vm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x70 | 0xF00; }
 
+// The barrier between the stages of a pipeline of direct global -> LDS loads: at most VM of
+// the wave's vector memory operations are in flight, and its LDS reads are done, so that
+// the loads behind the barrier can overwrite what was read in front of it.  (The products
+// that use the values may move past the barrier, and the compiler's own wait with them.)
+template <int VM> __device__ __forceinline__ void stage_barrier() {
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(VM) & ~0xF00);
+    __builtin_amdgcn_s_barrier();
+}
+
 inline int launch_status(const char *what) {
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return fail(QPAM_ERR_HIP, "%s launch failed: %s", what, hipGetErrorString(err));

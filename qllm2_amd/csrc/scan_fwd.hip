@@ -485,7 +485,6 @@ __device__ __forceinline__ void pass32_dma(float *st, const qpam_scan_args &a, c
 // loads complete in order among themselves, so an older load still in flight
 // would keep all of this step's loads in flight too.
 constexpr int PASS32_LOADS = 8;
-constexpr int PASS32_WAIT = waitcnt_vm(PASS32_LOADS);
 
 // Decay weights of every (chain, chunk) for the state pass, all chunks at once
 // (a wave per chunk): D[C-1, s] = exp(min(L_last - L_s, 0)) (0 beyond the
@@ -538,8 +537,7 @@ __device__ __forceinline__ void state_pass_f32_body(const FwdParams &p) {
     pass32_dma(st0, a, kre, kim, vre, vim, drow, tot, 0, i0, wv, lane);
     pass32_dma(st1, a, kre, kim, vre, vim, drow, tot, min(1, n - 1), i0, wv, lane);
     // chunk 0's loads are the oldest: wait for them (chunk 1's eight may still run)
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(8));
-    __builtin_amdgcn_s_barrier();
+    stage_barrier<PASS32_LOADS>();
 
     // one chunk: store S_in(c), stream chunk c+2 into NXT, dS from CUR, S <- total S + dS
     // (the stages rotate through three unrolled steps)
@@ -570,8 +568,7 @@ __device__ __forceinline__ void state_pass_f32_body(const FwdParams &p) {
         }                                                                                              \
         sr = tc * sr + (u1 + u2);                                                                      \
         si = tc * si + (u3 - u1 + u2);                                                                 \
-        __builtin_amdgcn_s_waitcnt(PASS32_WAIT);                                                       \
-        __builtin_amdgcn_s_barrier();                                                                  \
+        stage_barrier<PASS32_LOADS>();                                                                 \
         ++c;                                                                                           \
     }
     int c = 0;
