@@ -884,7 +884,8 @@ int qpam_logprobs_bwd(const qpam_logprobs_args *a, void *stream);
  * (h [N][D], w [V][D] as qpam_ce_fwd's) without logits in memory, and the gradient:
  * the tied LM head's token scores (logits of V11LM.ce_from_lm, v11/model.py:1175-1190).
  * bf16 operands: fp32 sums of exact products; the gradient's dx is rounded to bf16
- * between the tiles and the two products dh = dx w, dw = dx^T h.  fp32
+ * between the tiles and the two products dh = dx w, dw = dx^T h, but for its entries at
+ * the rows' ids, which join them in fp32.  fp32
  * operands: each value as the sum of three bf16 parts, products to about 2^-24.  D a
  * multiple of 32; h and w as qpam_ce_fwd takes them, with row strides below 2^22.  V at
  * most 2^30 (backward in fp32: V, and 2 chunk or N, below 2^22 - 256).  Temperature 1e-30 to 1e30.

@@ -383,6 +383,9 @@ struct BwdParams {
     int full_vt;     // vocab tiles of 256 columns in front of the narrow ones (tiles::Columns)
     float inv_t, c;  // 1 / T, log2(e) / T
     const float *stats, *logprobs, *entropy, *g_logprobs, *g_entropy;
+    // bf16: G at the rows' tokens, in fp32 and not in G^T (scores_token_kernel); room for Rp rows
+    float *token_g;
+    int *token_id;  // -1: no token
 };
 
 // A row's part of G_v = 2^u (base + slope u), u = c (x - m).  Zero for a row past the end.
@@ -406,22 +409,28 @@ __device__ __forceinline__ RowScore row_score(const BwdParams &p, int lr) {
     return {p.stats[2 * row], k * (g_lp + g_ent * (p.entropy[row] - LN2 * log2f(s))), k * g_ent * LN2};
 }
 
-// G^T at the rows' tokens, where the tiles left out the one-hot term: with p = e^logprob
-//   G = (g_lp (1 - p) - g_ent p (logprob + entropy)) / T.
+// G at the rows' tokens, where the tiles left out the one-hot term: with p = e^logprob
+//   G = (g_lp (1 - p) - g_ent p (logprob + entropy)) / T,
+// in fp32 to G^T.  In bf16 it stays out of G^T (0 there) and joins the products' sums in fp32
+// (tiles::gemm_kernel): it is the largest entry of most rows, and its rounding to bf16 was nearly
+// all of the gradients' error beyond that of their own rounding (16384 x 50261 x 1024: 2.4e-3
+// with it, 1.7e-3 without, as products of an fp32 G).  The other entries are rounded to bf16,
+// 2^-8 of each at most and so little of the row where p is spread; G in two bf16 parts would
+// double the work of both products (2.7 of 6.1 ms).
 template <typename T>
 __global__ void __launch_bounds__(THREADS) scores_token_kernel(BwdParams p) {
     const qpam_ce_bwd_args &a = p.a;
     const int lr = blockIdx.x * THREADS + threadIdx.x, row = p.row0 + lr;
     if (lr >= p.rows) return;
     const int64_t id = a.targets[row];
-    if (id == a.ignore_index || id < 0 || id >= a.V) return;
+    const bool valid = id != a.ignore_index && id >= 0 && id < a.V;
+    if (sizeof(T) == 2) p.token_id[lr] = valid ? (int)id : -1;
+    if (!valid) return;
     const float g_lp = p.g_logprobs ? p.g_logprobs[row] : 0.f, g_ent = p.g_entropy ? p.g_entropy[row] : 0.f;
     const float lp = p.logprobs[row], q = expf(lp);
     const float x = p.inv_t * (g_lp * (1.f - q) - g_ent * q * (fmaxf(lp, U_FLOOR) + p.entropy[row]));
-    T v;
-    if constexpr (sizeof(T) == 2) v = __builtin_bit_cast(unsigned short, (__bf16)x);
-    else v = x;
-    static_cast<T *>(p.gtbuf)[id * p.Rp + lr] = v;
+    if (sizeof(T) == 2) p.token_g[lr] = x;
+    static_cast<T *>(p.gtbuf)[id * p.Rp + lr] = sizeof(T) == 2 ? T(0) : T(x);
 }
 
 // out[c][r] = in[r][c] for an R x Cc tile grid (64 x 64 LDS tiles); rows >= R
@@ -1955,6 +1964,10 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
 // of kper where tiles are few; tiles in the order range, M, N over the XCDs' block ranges, so
 // that those which share operands share an L2.  A range's sums leave in fp32, each in its
 // place of `out`.
+// The entries of G at the rows' tokens come in fp32 beside it (TokenTerms): dH's tiles add
+// g W[id] to their rows at the end; dW's tiles look for their own tokens among the rows' ids
+// and multiply them as further steps of 32 rows, g in three bf16 parts.  A range of K has the
+// entries that lie in it.
 // Against 50261 x 768, dH with the sum: 16 rows 33 us, 200 rows 42, bound by reading W and
 // the partial sums (hipBLASLt, with 20 and 51 blocks: 107 and 197).  16384 rows, 50261 x
 // 1024: 1.40 ms each, 1.20 PFLOP/s (hipBLASLt 1.51 and 1.60).
@@ -1962,9 +1975,19 @@ __device__ __forceinline__ int h_of(int row) { return (row & 3) | ((row >> 3) & 
 
 enum { OUT_BF16, OUT_F32, OUT_ADD };
 
+// dH: of rows 0 .. M - 1; dW: of rows 0 .. b_rows - 1, with row 0 of the product vocabulary entry v0.
+// Both arrays 16-byte aligned and a multiple of four long.
+struct TokenTerms {
+    const float *g;
+    const int *id;  // -1: none
+    int v0;
+};
+constexpr int SCAN = 16 * TT;  // rows whose ids a block looks through at once
+
 template <bool AT>
 __global__ void __launch_bounds__(TT) gemm_kernel(const U16 *A, int64_t lda, int M, const U16 *B, int64_t ldb, int b_rows, int N, int K,
-                                                  int kper, int ranges, void *out, int64_t ldo, int64_t range_stride, int mode) {
+                                                  int kper, int ranges, void *out, int64_t ldo, int64_t range_stride, int mode,
+                                                  TokenTerms t) {
     __shared__ __align__(16) Stage s0, s1, s2, s3;
     const int n_ct = (N + TN - 1) / TN, tiles = (M + TM - 1) / TM * n_ct;
     const int item = big::xcd_item(blockIdx.x, tiles * ranges);
@@ -2049,6 +2072,109 @@ __global__ void __launch_bounds__(TT) gemm_kernel(const U16 *A, int64_t lda, int
     if (kt + 2 < KT) step(kt + 2, s2, s1);
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // no direct load outlives the wave
     const int m1 = m0 + 64 * (w >> 1) + 4 * g, n1 = n0 + 128 * (w & 1) + l16;
+    if constexpr (AT) {  // g W[id], the columns of four rows in flight
+#pragma unroll
+        for (int mi = 0; mi < 4; ++mi) {
+            const int m = m1 + 16 * mi;
+            const intx4 id = m < M ? *reinterpret_cast<const intx4 *>(t.id + m) : intx4{-1, -1, -1, -1};
+            const floatx4 gt = m < M ? *reinterpret_cast<const floatx4 *>(t.g + m) : floatx4{0.f, 0.f, 0.f, 0.f};
+            bool on[4], any = false;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                on[r] = m + r < M && id[r] >= k0 && id[r] < k0 + kper;
+                any |= on[r];
+            }
+            if (__ballot(any) == 0) continue;
+            U16 x[4][8];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int ni = 0; ni < 8; ++ni) x[r][ni] = B[(int64_t)(on[r] ? id[r] : 0) * ldb + min(n1 + 16 * ni, N - 1)];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int ni = 0; ni < 8; ++ni)
+                    acc[mi][ni][r] = on[r] ? __builtin_fmaf(gt[r], bf16_to_f32(x[r][ni]), acc[mi][ni][r]) : acc[mi][ni][r];
+        }
+    } else {
+        // the stages' memory: g's parts as A tiles in s0.a, s1.a and s3.a, H's rows in s0.b, the list of
+        // matches (row in the scan << 8 | vocabulary entry in the tile) over s2, the waves' counts in s1.b
+        U16 *const part[3] = {s3.a, s1.a, s0.a};  // smallest first
+        int *list = reinterpret_cast<int *>(&s2), *counts = reinterpret_cast<int *>(s1.b);
+        const int tid = threadIdx.x, v0 = t.v0 + m0, k1 = min(k0 + kper, b_rows);
+        for (int c0 = k0; c0 < k1; c0 += SCAN) {
+            uint32_t hits = 0;
+            int v[16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = c0 + 16 * tid + 4 * q;
+                const intx4 id = row < k1 ? *reinterpret_cast<const intx4 *>(t.id + row) : intx4{-1, -1, -1, -1};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[4 * q + i] = id[i] - v0;
+                    if (row + i < k1 && id[i] >= v0 && v[4 * q + i] < TM) hits |= 1u << (4 * q + i);
+                }
+            }
+            int before = __popc(hits);  // inclusive over the wave's lanes
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int o = __shfl_up(before, off);
+                if (lane >= off) before += o;
+            }
+            __syncthreads();  // the products and the list of the scan before are done with
+            if (lane == 63) counts[w] = before;
+            __syncthreads();
+            int total = 0, at = before - __popc(hits);
+            for (int x = 0; x < TT / 64; ++x) {
+                if (x < w) at += counts[x];
+                total += counts[x];
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (hits >> i & 1) list[at++] = (16 * tid + i) << 8 | v[i];
+            for (int e0 = 0; e0 < total; e0 += DK) {
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+#pragma unroll
+                    for (int j = 0; j < TM * DK / 8 / TT; ++j)
+                        reinterpret_cast<uint4 *>(part[i])[tid + j * TT] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int from = c0 + (list[min(e0 + row[j], total - 1)] >> 8);
+                    to_lds(reinterpret_cast<const char *>(B + (int64_t)from * ldb + n0) + bo[j], &s0.b[(4 * w + 2 * j) * TN]);
+                }
+                __syncthreads();
+                if (tid < DK && e0 + tid < total) {
+                    const int e = list[e0 + tid], vl = e & 255;
+                    float x = t.g[c0 + (e >> 8)];
+#pragma unroll
+                    for (int i = 2; i >= 0; --i) {
+                        const U16 b = __builtin_bit_cast(U16, (__bf16)x);
+                        part[i][vl * DK + 8 * wide::swz(vl, tid >> 3) + (tid & 7)] = b;
+                        x -= bf16_to_f32(b);
+                    }
+                }
+                __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+                __syncthreads();
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    bf16x8 b[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) b[i] = fragment_t(s0.b, at0, 8 * (w & 1) + 4 * half + i);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+#pragma unroll
+                        for (int mi = 0; mi < 4; ++mi) {
+                            const bf16x8 a = fragment(part[i] + a_at, mi);
+#pragma unroll
+                            for (int ni = 0; ni < 4; ++ni)
+                                acc[mi][4 * half + ni] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[ni], acc[mi][4 * half + ni], 0, 0, 0);
+                        }
+                }
+            }
+        }
+    }
     const int64_t first = z * range_stride + (int64_t)m1 * ldo + n1;
     auto store = [&](auto *to, auto add) {  // to: the lane's first element
 #pragma unroll
@@ -2424,13 +2550,14 @@ int best_ranges(int64_t most, int K, double step_us, int64_t outputs) {
 // sums of).
 template <bool AT>
 int scores_gemm(const unsigned short *A, int64_t lda, int M, const unsigned short *B, int64_t ldb, int b_rows, int N, int K, void *out,
-                int64_t ldo, int mode, float *part, size_t part_bytes, hipStream_t stream) {
+                int64_t ldo, int mode, float *part, size_t part_bytes, tiles::TokenTerms terms, hipStream_t stream) {
     using U = unsigned short;
     auto launch = [&](int m0, int m, int ranges, int kper, void *to, int64_t ld, int how) {
         const int tiles = ((m + tiles::TM - 1) / tiles::TM) * ((N + tiles::TN - 1) / tiles::TN);
+        const tiles::TokenTerms t = AT ? tiles::TokenTerms{terms.g + m0, terms.id + m0, 0} : tiles::TokenTerms{terms.g, terms.id, m0};
         hipLaunchKernelGGL(tiles::gemm_kernel<AT>, dim3(big::xcd_grid(tiles * ranges)), dim3(tiles::TT), 0, stream,
                            AT ? A + m0 : A + (int64_t)m0 * lda, lda, m, B, ldb, b_rows, N, K, kper, ranges, to, ld,
-                           ranges > 1 ? (int64_t)m * ld : 0, how);
+                           ranges > 1 ? (int64_t)m * ld : 0, how, t);
         return launch_status("tiles gemm_kernel");
     };
     auto at = [&](int m) { return static_cast<char *>(out) + (int64_t)m * ldo * (mode == tiles::OUT_BF16 ? 2 : 4); };
@@ -2511,13 +2638,14 @@ int run_bwd_bf16(const qpam_ce_bwd_args &a, hipStream_t stream, const BwdParams 
             if (scores) {
                 const U *h = (const U *)a.h + (int64_t)r0 * a.ldh, *gt = (const U *)p.gtbuf;
                 const int how = !dw_write ? tiles::OUT_ADD : a.dw_out == 1 ? tiles::OUT_BF16 : tiles::OUT_F32;
+                const tiles::TokenTerms terms = {p.token_g, p.token_id, 0};
                 if (a.dw)
                     st = scores_gemm<false>(gt, p.Rp, a.V, h, a.ldh, p.rows, a.D, round_up(p.rows, BK), a.dw, a.lddw, how, q.dh_part,
-                                            blas_ws, stream);
+                                            blas_ws, terms, stream);
                 if (st) return st;
                 if (a.dh)
                     st = scores_gemm<true>(gt, p.Rp, p.rows, (const U *)a.w, a.ldw, a.V, a.D, p.Vp, (U *)a.dh + (int64_t)r0 * a.lddh,
-                                           a.lddh, tiles::OUT_BF16, q.dh_part, blas_ws, stream);
+                                           a.lddh, tiles::OUT_BF16, q.dh_part, blas_ws, terms, stream);
                 if (st) return st;
                 continue;
             }
@@ -2762,6 +2890,16 @@ qpam_ce_bwd_args bwd_args(const qpam_linear_logprobs_args &a) {
     return b;
 }
 
+// The bf16 token scores' workspace: the loss's, then the tokens of a pass's rows (p: their places).
+size_t token_ws(const qpam_ce_bwd_args &a, BwdParams *p) {
+    const size_t at = (qpam_ce_bwd_workspace_size(&a) + 255) & ~(size_t)255, rows = round_up(pass_rows(a), big::BTM);
+    if (p) {
+        p->token_g = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + at);
+        p->token_id = reinterpret_cast<int *>(p->token_g + rows);
+    }
+    return at + rows * (sizeof(float) + sizeof(int));
+}
+
 int validate_scores(const qpam_linear_logprobs_args &a, const char *who) {
     int st = validate_common(a.N, a.V, a.D, a.dtype, a.h, a.ldh, a.w, a.ldw, a.ids, who);
     if (st) return st;
@@ -2855,7 +2993,7 @@ extern "C" size_t qpam_linear_logprobs_bwd_workspace_size(const qpam_linear_logp
     using namespace qpam::ce;
     if (!a || a->N < 1 || a->V < 1 || a->chunk < 1) return 0;
     const qpam_ce_bwd_args b = bwd_args(*a);
-    return a->dtype == QPAM_F32 ? scores_f32_ws(b) : qpam_ce_bwd_workspace_size(&b);
+    return a->dtype == QPAM_F32 ? scores_f32_ws(b) : token_ws(b, nullptr);
 }
 
 extern "C" int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void *stream) {
@@ -2881,5 +3019,6 @@ extern "C" int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void
     p.entropy = a->entropy;
     p.g_logprobs = a->g_logprobs;
     p.g_entropy = a->g_entropy;
+    if (a->dtype == QPAM_BF16) token_ws(bwd_args(*a), &p);
     return run_backward(bwd_args(*a), (hipStream_t)stream, &p);
 }

@@ -300,7 +300,8 @@ def linear_token_logprobs(hidden_rows: Tensor, weight_matrix: Tensor, ids: Tenso
     Differentiable in hidden_rows and weight_matrix (once: a second derivative
     raises).  If either operand is bf16, both enter the products as bf16, with fp32
     sums; the logits' gradient is rounded to bf16 before the two products that give
-    the operands' gradients.  The gradients have the operands' dtypes; that of an fp32
+    the operands' gradients, but for its entries at the given ids, most rows' largest,
+    which join them in fp32.  The gradients have the operands' dtypes; that of an fp32
     weight_matrix with bf16 rows (a master table) leaves from the fp32 sums.  chunk
     bounds the backward's memory as in fused_ce.fused_linear_cross_entropy.  D off the
     multiples of 32 pads both operands by copies; rows that are not apart by their

@@ -226,3 +226,32 @@ def test_layouts_of_the_loss(gpu_lib, name):
                 res.append([loss, linear_ce_per_token(x, y, t), *torch.autograd.grad(loss, [x, y])])
             for s, t in zip(*res):
                 assert torch.equal(s, t)
+
+
+@pytest.mark.parametrize("wdtype", [BF16, F32])
+@pytest.mark.parametrize("n,V,D,chunk,same", [(300, 700, 64, 4096, False), (1, 300, 96, 4096, False), (40, 5000, 96, 4096, False),
+                                              (1100, 700, 96, 64, False), (2500, 9000, 64, 4096, False), (700, 600, 32, 4096, True),
+                                              (20000, 1000, 32, 8192, False)])
+def test_token_terms_are_not_rounded_between_the_products(gpu_lib, n, V, D, chunk, same, wdtype):
+    """bf16 rows: dx is rounded to bf16 (2^-8 of each entry) in front of the products but for the entries at the
+    rows' tokens, which join them in fp32.  All else as for fp32; an fp32 table's dw shows it undimmed."""
+    from qllm2_amd.token_logprobs import linear_token_logprobs
+    h, w, ids, gs = _data(n, V, D, BF16, wdtype, n + V)
+    if same:
+        ids = torch.where(ids == V + 1, ids, V // 2)
+    wr = w.to(BF16)
+    R = _reference(h, wr, ids, 0.9, [g.double() for g in gs], 0.0)
+    hd, wd = h.double(), wr.double()
+    logp = torch.log_softmax(hd @ wd.T / 0.9, -1)
+    p = logp.exp()
+    valid = (ids >= 0) & (ids < V)
+    dx = p * (torch.where(valid, gs[0].double(), 0.0)[:, None] + gs[1].double()[:, None] * (logp - (p * logp).sum(-1, keepdim=True))) / 0.9
+    dx[valid, ids[valid]] = 0
+    hc, wc = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    r = linear_token_logprobs(hc, wc, ids.cuda(), temperature=0.9, chunk=chunk)
+    for needs in ((hc, wc), (hc,), (wc,)):
+        for o, got in zip(needs, torch.autograd.grad([r.logprobs, r.entropy], needs, [g.cuda() for g in gs], retain_graph=True)):
+            if o is hc:
+                _close(got, R["dh"], R["t_dh"] + 2.0 ** -8 * (dx.abs() @ wd.abs()), torch.finfo(BF16).eps)
+            else:
+                _close(got, R["dw"], R["t_dw"] + 2.0 ** -8 * (dx.abs().T @ hd.abs()), torch.finfo(wdtype).eps)
