@@ -900,7 +900,7 @@ typedef struct {
     int64_t ignore_index;
     float temperature;
     float *logprobs, *entropy;     /* written by the forward, read by the backward, */
-    float *stats;                  /* [N][2]: as are max h w^T and sum exp(x - max x) */
+    float *stats;                  /* [N][2]: as are the row's max h w^T, sum exp(x - max x) */
     const float *g_logprobs, *g_entropy; /* each optional */
     void *dh; int64_t lddh;
     void *dw; int64_t lddw;

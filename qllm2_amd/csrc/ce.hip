@@ -1564,9 +1564,9 @@ __global__ void __launch_bounds__(WTHREADS) grad_tile_kernel(BwdParams p) {
 
 // Token scores' bf16 tiles, 256 x 256: loads, swizzle and wave layout as in `wide`, with a
 // k-step's first fragments read from LDS between the MFMAs of the step before, so that no
-// wave waits for LDS at the head of a step.  16384 x 50261 x 1024: scores 1.48 ms (1.14
-// PFLOP/s, the MFMA pipes 57 % busy at the 1.9 GHz that the card holds under this load, LDS
-// 23 %), G^T 1.80 ms with 1.65 GB of stores; two blocks of 128 x 256 a CU took 1.85 and 2.11.
+// wave waits for LDS at the head of a step.  16384 x 50261 x 1024: scores 1.55 ms (1.09
+// PFLOP/s, the MFMA pipes about 55 % busy at the 1.9 GHz that the card holds under this load, LDS
+// 23 %), G^T 1.78 ms with 1.65 GB of stores; two blocks of 128 x 256 a CU took 1.85 and 2.11.
 namespace tiles {
 constexpr int TM = wide::TM, TN = wide::TN, DK = wide::DK, TT = wide::WTHREADS;
 using U16 = unsigned short;
@@ -1968,9 +1968,10 @@ __global__ void __launch_bounds__(TT) scores_grad_kernel(BwdParams p) {
 // g W[id] to their rows at the end; dW's tiles look for their own tokens among the rows' ids
 // and multiply them as further steps of 32 rows, g in three bf16 parts.  A range of K has the
 // entries that lie in it.
-// Against 50261 x 768, dH with the sum: 16 rows 33 us, 200 rows 42, bound by reading W and
+// Against 50261 x 768, dH with the sum: 16 rows 29 us, 200 rows 39, bound by reading W and
 // the partial sums (hipBLASLt, with 20 and 51 blocks: 107 and 197).  16384 rows, 50261 x
-// 1024: 1.40 ms each, 1.20 PFLOP/s (hipBLASLt 1.51 and 1.60).
+// 1024: dW 1.40 ms, dH 1.43, 1.19 PFLOP/s (hipBLASLt 1.60 and 1.51); the tokens' entries take 5 us of
+// a call of few rows, 0.4 % of this one.
 __device__ __forceinline__ int h_of(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
 
 enum { OUT_BF16, OUT_F32, OUT_ADD };

@@ -40,7 +40,8 @@ __device__ __forceinline__ int64_t load_id(const void *ids, int is64, int64_t i)
 // 16-byte stores out.  Lanes to a row: the least power of two that covers it, at most a
 // wave, so that short rows share waves.  PAIRS: one interleaved table [V][dim][2] (im = re + 1,
 // columns two apart), whose rows are the output's form already.  W = 1: any column strides.  Bound by the launch (192 rows of 768 fp32: 3.3
-// us) or by HBM (16384 rows of 512 bf16, 33 MB written and as much read: 12.9 us).
+// us) or by gathering and storing: 16384 rows of 512 bf16 12.4 us, 33 MB written and 12 MB of
+// distinct rows read (3.7 TB/s; a frequent token's row comes from the caches).
 template <typename T, int W, bool PAIRS>
 __global__ void __launch_bounds__(THREADS) lookup_kernel(qpam_embed_args a, int lanes_log2) {
     typedef T VecT __attribute__((ext_vector_type(W)));
@@ -129,8 +130,8 @@ __device__ __forceinline__ void zero_tables(const SortParams &p) {
 // each wave ranks a contiguous part of it (stable: rounds of 64 in order, lanes of
 // a round in order), and the counts of [wave][digit] give every wave its places.
 // One launch instead of the six of the longer lists' two passes, and the other blocks
-// zero the tables beside it: 27 us for 16384 ids and 103 MB (the sort's own time; the
-// fill alone takes 15), 37 us for 3001 ids and 197 MB (the fill's).
+// zero the tables beside it: 37 us for 16384 ids and 103 MB (the sort's own time; the
+// fill alone takes 15), 27 us for 3001 ids and 197 MB (the fill's).
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
 constexpr int ROUNDS = 16, SMALL = SORT_THREADS * ROUNDS;
 constexpr size_t SORT_SMEM = SMALL * 6 + SORT_WAVES * RADIX * 4;

@@ -135,7 +135,8 @@ __device__ __forceinline__ void top_by_passes(const Row<T> &row, int k, uint64_t
 
 // Bound by HBM and, in bf16, nearly as much by the VALU (an exp, a maximum and five more
 // operations an entry: 50 us of the 75).  4000 rows of 50261 bf16 (402 MB): 75 us without
-// alternatives (5.3 TB/s), 82 with five, 86 with 32; 2048 rows fp32 (412 MB): 72 us.  One
+// alternatives (5.3 TB/s), 82 with five, 86 with 32; 2048 rows fp32 (412 MB): 72 us (5.8 TB/s),
+// 108 in a training pass, behind the 412 MB that the gradient before it has stored.  One
 // row of 50261 fp32 with five alternatives: 10.5 us, the block's own latency.
 template <typename T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS) row_kernel(Args a) {
