@@ -820,7 +820,8 @@ int qpam_ce_bwd(const qpam_ce_bwd_args *a, void *stream);
  * qpam_embed_bwd: d_re[v][j] = scale * sum of dz[i][j][0] over ids[i] == v, d_im
  * from dz[i][j][1]: fp32 sums in the order of i, rounded once to dtype.  Writes
  * both contiguous [V][dim] tables (zeros for tokens that do not occur); ids
- * outside [0, V) or equal to padding_idx give nothing.  dz [n][dim][2]
+ * outside [0, V) or equal to padding_idx give nothing.  n times the 512-byte pieces of a
+ * row (256 or 128 bytes at an odd dim) at most 2^27.  dz [n][dim][2]
  * contiguous.  dz, d_re, d_im and workspace 16-byte aligned. */
 typedef struct {
     int64_t n;

@@ -131,7 +131,7 @@ def complex_embedding(ids: Tensor, weight_real: Tensor, weight_imag: Tensor, sca
     token) and no gradient.  padding_idx (of [-V, V),
     as nn.Embedding's) is looked up like any id and gets no gradient.
     Differentiable in both tables (dense gradients, once: a second derivative
-    raises)."""
+    raises), up to 2^27 ids, fewer by the 512-byte pieces of a table's row."""
     pad = -1
     if padding_idx is not None:
         V = weight_real.shape[0]

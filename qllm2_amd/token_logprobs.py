@@ -304,9 +304,9 @@ def linear_token_logprobs(hidden_rows: Tensor, weight_matrix: Tensor, ids: Tenso
     which join them in fp32.  The gradients have the operands' dtypes; that of an fp32
     weight_matrix with bf16 rows (a master table) leaves from the fp32 sums.  chunk
     bounds the backward's memory as in fused_ce.fused_linear_cross_entropy.  D off the
-    multiples of 32 pads both operands by copies; rows that are not apart by their
-    length or more and by less than 2^22 elements, each at a multiple of 16 bytes, are copied.  Alternatives need the logits:
-    token_logprobs gives them."""
+    multiples of 32 pads both operands by copies; operands whose rows share memory, start
+    off 16 bytes or lie 2^22 elements apart are copied, too.  Log probabilities are at
+    most 0.  Alternatives need the logits: token_logprobs gives them."""
     _check_linear(hidden_rows, weight_matrix, ids, temperature, chunk)
     D = hidden_rows.shape[-1]
     h, w = hidden_rows.reshape(-1, D), weight_matrix
