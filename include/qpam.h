@@ -76,6 +76,11 @@
  *                       v11/flash_pam.py:56-152, v11/model.py:378-417, 491-576)
  *   qpam_pc_fwd/_bwd    v11/model.py:421-489 V11PAMLayer._forward_chunked_perchannel
  *                       and its autograd backward
+ *   qpam_linear4        ComplexLinear (v11/complex_ops.py:146-172) and the tied
+ *                       logits of one decode step (v11/model.py:1207-1245) from
+ *                       weights of 4 bits
+ *   qpam_copy_slots     the per-sequence state lists of V11LM.generate
+ *                       (v11/model.py:1207-1245) copied between sequences
  *   qpam_cgu_mix        the CGU's activation and gate between its projections,
  *                       ComplexGatedUnit.forward (v11/complex_ops.py:216-220;
  *                       activations :102-143)
@@ -914,6 +919,57 @@ size_t qpam_linear_logprobs_fwd_workspace_size(const qpam_linear_logprobs_args *
 int qpam_linear_logprobs_fwd(const qpam_linear_logprobs_args *a, void *stream);
 size_t qpam_linear_logprobs_bwd_workspace_size(const qpam_linear_logprobs_args *a);
 int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void *stream);
+
+/* Products of rows with 4-bit weights (ABI 19; inference only):
+ *   y[i][j] = sum_k x[i][k] w[j][k] (+ bias[j]),  w[j][k] = s[j][k / group] e[j][k]
+ * e: 4-bit floats (bit 3 the sign; 0, 0.5, 1, 1.5, 2, 3, 4, 6 by bits 0 to 2), s bf16, group
+ * 32, 64 or 128.  x [rows][k] and y [rows][n] in dtype (row strides ldx, ldy elements, any
+ * alignment of the type).  fp32 sums of exact products (fp32 rows: of three bf16 parts, exact),
+ * rounded once.
+ * is_complex: x [rows][k][2], y [rows][n][2], weights and bias complex; the codes and scales
+ * are those of rows of 2k real values, (re, im) side by side (v11/complex_ops.py:165-172:
+ * re = Wr xr - Wi xi, im = Wi xr + Wr xi).  planes 1: y's row is the n real parts, the n
+ * imaginary parts and then tail_n further real outputs x . tail[t] (tail [tail_n][2k] in
+ * dtype, row stride ld_tail: outputs whose weights stay whole).
+ * codes: blocks of 16 outputs x 128 inputs, [ceil(n/16)][ceil(K/128)][1024 bytes] with K = k
+ * (2k complex); in a block, byte 16 l + 4 s + b of lane l = 16 q + r holds the codes of output r and
+ * inputs 32 s + 8 q + 2 b (low half) and the next (high half).  scales: [ceil(n/16)]
+ * [ceil(K/128)][16][128/group] bf16.  Codes and scales outside n and K are zero.  codes
+ * 16-byte, scales 8-byte aligned.  n and k at most 2^24. */
+typedef struct {
+    int64_t rows;
+    int32_t n, k;
+    int32_t group;
+    int32_t is_complex;
+    int32_t dtype;
+    int32_t planes;
+    const void *x; int64_t ldx;
+    const void *codes;
+    const void *scales;
+    const float *bias;             /* optional; [n], [n][2] complex */
+    void *y; int64_t ldy;
+    int32_t tail_n;
+    const void *tail; int64_t ld_tail;
+} qpam_linear4_args;
+
+int qpam_linear4(const qpam_linear4_args *a, void *stream);
+
+/* state[dst[i]] = state[src[i]] for all i at once, the sources as they were before the call
+ * (ABI 19): pages of page_bytes, slot_bytes apart (both multiples of 4), in n_slots slots.  A src
+ * of -1 clears the page.  pos (optional, [n_slots]): moved and cleared with the pages.  The
+ * lists are on the host (host_lists 1: read before the call returns, at most 448) or on the
+ * device (at most 4096).  dst distinct; an entry with a dst outside [0, n_slots) or a src
+ * outside [-1, n_slots) does nothing. */
+typedef struct {
+    void *state;
+    int64_t slot_bytes, page_bytes;
+    int32_t n_slots, count;
+    const int32_t *src, *dst;
+    int32_t host_lists;
+    int32_t *pos;
+} qpam_slots_args;
+
+int qpam_copy_slots(const qpam_slots_args *a, void *stream);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ import os
 import torch  # noqa: F401  (must be loaded before the HIP library)
 
 LIB_NAME = "libqpam.so"
-ABI_VERSION = 18
+ABI_VERSION = 19
 _HERE = os.path.dirname(os.path.abspath(__file__))
 
 QPAM_F32 = 0
@@ -283,6 +283,21 @@ class LinearLogprobsArgs(ctypes.Structure):
     ]
 
 
+class Linear4Args(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64), ("n", c_i32), ("k", c_i32), ("group", c_i32), ("is_complex", c_i32), ("dtype", c_i32),
+        ("planes", c_i32), ("x", c_ptr), ("ldx", c_i64), ("codes", c_ptr), ("scales", c_ptr), ("bias", c_ptr),
+        ("y", c_ptr), ("ldy", c_i64), ("tail_n", c_i32), ("tail", c_ptr), ("ld_tail", c_i64),
+    ]
+
+
+class SlotsArgs(ctypes.Structure):
+    _fields_ = [
+        ("state", c_ptr), ("slot_bytes", c_i64), ("page_bytes", c_i64), ("n_slots", c_i32), ("count", c_i32),
+        ("src", c_ptr), ("dst", c_ptr), ("host_lists", c_i32), ("pos", c_ptr),
+    ]
+
+
 SIGNATURES = {
     "qpam_version": (ctypes.c_int, []),
     "qpam_last_error": (ctypes.c_char_p, []),
@@ -334,6 +349,8 @@ SIGNATURES = {
     "qpam_cweight_unpack": (ctypes.c_int, [ctypes.POINTER(CWeightArgs), c_ptr]),
     "qpam_cabs_bwd_acc": (ctypes.c_int, [c_i32, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
     "qpam_planes": (ctypes.c_int, [ctypes.POINTER(PlanesArgs), c_ptr]),
+    "qpam_linear4": (ctypes.c_int, [ctypes.POINTER(Linear4Args), c_ptr]),
+    "qpam_copy_slots": (ctypes.c_int, [ctypes.POINTER(SlotsArgs), c_ptr]),
     "qpam_slice_sum": (ctypes.c_int, [c_i32, c_i32, c_i32, c_i64, c_i64, c_ptr, c_ptr, c_ptr]),
 }
 

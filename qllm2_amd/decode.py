@@ -15,6 +15,8 @@ padding (the padded rows and columns of the state stay zero, since the padded
 entries of v and k are zero, and the padded columns of q add nothing to y).
 """
 
+import ctypes
+
 import torch
 import torch.nn.functional as F
 
@@ -304,6 +306,78 @@ def recur_step_additive(memory_state, decay_gamma, value_t, key_t, query_t):
             new_state.reshape(*lead, d, d, 2).to(memory_state.dtype))
 
 
+MAX_HOST_MOVES, MAX_MOVES = 448, 4096  # qpam_copy_slots: of one call, lists on the host and on the device
+
+
+def _list(v, name):
+    """A list of slot ids: (host list, None), or (None, int32 device tensor)."""
+    if torch.is_tensor(v) and v.is_cuda:
+        if v.dim() != 1 or v.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"qpam copy_slots: {name} must be one list of int32 or int64, got {v.dtype} {tuple(v.shape)}")
+        return None, v.to(torch.int32).contiguous()
+    return [int(i) for i in (v.tolist() if torch.is_tensor(v) else v)], None
+
+
+def copy_slots(state, src, dst, pos=None):
+    """state[dst[i]] = state[src[i]] for all i at once, in place and in one launch: every
+    source is read as it was before the call, so dst and src may share slots in any way (beams
+    that continue from each other).  A src of -1 clears the page.
+
+    state  [S, ...] fp32, the pages contiguous (a pool's, or one layer's view of it)
+    src, dst  slot ids, both host lists (or CPU tensors), or both device tensors, which are
+           not read back; dst distinct.  Host lists are checked: ids outside the pool or a
+           dst given twice raise.  On the device an entry outside the pool does nothing, and a
+           dst given twice gets one of its sources' values in each place.
+    pos    optional int32 [S], moved and cleared with the pages
+    Up to 4096 moves; host lists of more in several launches where no dst is also a src."""
+    _check_cuda(state, pos)
+    n_slots = state.shape[0] if state.dim() else 0
+    if state.dtype != torch.float32 or state.dim() < 2 or not state.numel() or not state[0].is_contiguous() \
+            or (n_slots > 1 and state.stride(0) < state[0].numel()):
+        raise ValueError(f"qpam copy_slots: state must be fp32 [S, ...] with contiguous pages, got {state.dtype} "
+                         f"{tuple(state.shape)} of strides {state.stride()}")
+    if pos is not None and (pos.dtype != torch.int32 or tuple(pos.shape) != (n_slots,) or not pos.is_contiguous()
+                            or pos.device != state.device):
+        raise ValueError(f"qpam copy_slots: pos must be contiguous int32 [{n_slots}] on {state.device}")
+    (src, src_t), (dst, dst_t) = _list(src, "src"), _list(dst, "dst")
+    if (src is None) != (dst is None):
+        raise ValueError("qpam copy_slots: src and dst must be both host lists or both device tensors")
+    count = len(src) if src is not None else src_t.numel()
+    if count != (len(dst) if dst is not None else dst_t.numel()):
+        raise ValueError("qpam copy_slots: src and dst of different lengths")
+    if src is None:
+        if src_t.device != state.device or dst_t.device != state.device:
+            raise ValueError(f"qpam copy_slots: lists must be on the host or on {state.device}")
+        if count > MAX_MOVES:
+            raise ValueError(f"qpam copy_slots: {count} moves (at most {MAX_MOVES} in device lists)")
+        pieces = [(src_t, dst_t)]
+    else:
+        if any(not -1 <= s < n_slots for s in src) or any(not 0 <= d < n_slots for d in dst):
+            raise ValueError(f"qpam copy_slots: slots outside the pool of {n_slots}")
+        if len(set(dst)) < count:
+            raise ValueError("qpam copy_slots: a dst given twice")
+        size = MAX_HOST_MOVES
+        if count > size and not set(dst).isdisjoint(src):
+            if count > MAX_MOVES:
+                raise ValueError(f"qpam copy_slots: {count} moves between slots that are both src and dst (at most {MAX_MOVES})")
+            src, dst = (torch.tensor(v, dtype=torch.int32).to(state.device) for v in (src, dst))
+            size = count
+        pieces = [(src[i:i + size], dst[i:i + size]) for i in range(0, count, size)]
+    a = _lib.SlotsArgs()
+    a.state, a.n_slots = state.data_ptr(), n_slots
+    a.slot_bytes, a.page_bytes = 4 * max(state.stride(0), state[0].numel()), 4 * state[0].numel()
+    a.pos = None if pos is None else pos.data_ptr()
+    with _lib.device(state.device):
+        for s, d in pieces:
+            if torch.is_tensor(s):
+                a.host_lists, a.count, a.src, a.dst = 0, s.numel(), s.data_ptr(), d.data_ptr()
+            else:
+                ints = _lib.c_i32 * len(s)
+                s, d = ints(*s), ints(*d)
+                a.host_lists, a.count, a.src, a.dst = 1, len(s), ctypes.addressof(s), ctypes.addressof(d)
+            _lib.check(_lib.lib().qpam_copy_slots(a, _lib.stream_ptr(state.device)), "qpam_copy_slots")
+
+
 def build_rope_cache(max_len, head_dim, device=None):
     """Complex RoPE table e^{i m theta_j} [max_len, head_dim, 2] fp32, the
     reference's build_rope_cache (v11/complex_ops.py:261-266):
@@ -324,7 +398,9 @@ class SlotPool:
     join (acquire, optionally with the states a prefill produced) and leave
     (release) between steps, and one `step` per layer updates every listed slot
     with one kernel launch (qpam_decode_step with per-slot RoPE); `advance`
-    moves the listed slots' positions by one token.
+    moves the listed slots' positions by one token.  Sequences continue from each
+    other's states by copies within the pool, one launch for any number of slots
+    (qpam_copy_slots): `fork`, `reorder`, `compact`, `clear`.
     """
 
     def __init__(self, n_slots, n_layers, n_heads, head_dim, n_states=1, device="cuda", max_len=4096):
@@ -373,8 +449,67 @@ class SlotPool:
         return slot
 
     def release(self, slot):
-        self.live.discard(slot)
-        self._free.append(slot)
+        if slot in self.live:  # a slot released twice must not be handed out twice
+            self.live.discard(slot)
+            self._free.append(slot)
+
+    def _live(self, slots, what):
+        if not self.live.issuperset(slots):
+            raise ValueError(f"SlotPool.{what}: slots {sorted(set(slots) - self.live)} hold no sequence")
+
+    def fork(self, slot, count=1):
+        """`count` more sequences that continue from where `slot` is (samples of one
+        prompt, the first beams of a search): its states and position are copied to free
+        slots in one launch.  Returns their ids."""
+        self._live([slot], "fork")
+        if not 0 <= count <= len(self._free):
+            raise RuntimeError(f"SlotPool: {len(self._free)} free slots, {count} asked for")
+        ids = self._free[len(self._free) - count:][::-1]
+        copy_slots(self.state, [slot] * count, ids, pos=self.pos)
+        del self._free[len(self._free) - count:]
+        self.live.update(ids)
+        for i in ids:
+            self._host_pos[i] = self._host_pos[slot]
+        return ids
+
+    def reorder(self, slots, parents):
+        """Each live slot slots[i] continues from where parents[i] was (beam search, in
+        place; a slot may be its own parent and several slots' parent).  Host lists, or
+        device tensors, which are not read back (then ids outside the pool do nothing)."""
+        host = not (torch.is_tensor(slots) and slots.is_cuda)
+        if host and not (torch.is_tensor(parents) and parents.is_cuda):
+            slots, parents = ([int(i) for i in v] for v in (slots, parents))
+            self._live(slots + parents, "reorder")
+        copy_slots(self.state, parents, slots, pos=self.pos)
+        if host:
+            for s, p in zip(slots, [self._host_pos[p] for p in parents]):
+                self._host_pos[s] = p
+        else:  # whose position moved where is not known here: no live slot is further than the furthest
+            furthest = max((self._host_pos[s] for s in self.live), default=0)
+            for s in self.live:
+                self._host_pos[s] = furthest
+
+    def compact(self):
+        """The live sequences moved to the pool's lowest slots, those that are there already
+        kept.  Returns {old slot: new slot} of the moved ones."""
+        usable = sorted([*self._free, *self.live])
+        front = set(usable[:len(self.live)])
+        old, new = sorted(self.live - front), sorted(front - self.live)
+        copy_slots(self.state, old, new, pos=self.pos)
+        for s, d in zip(old, new):
+            self._host_pos[d] = self._host_pos[s]
+        self.live = front
+        self._free = usable[len(front):][::-1]
+        return dict(zip(old, new))
+
+    def clear(self, slots):
+        """The listed live slots' states emptied and their positions set to 0, in one launch
+        (host ids)."""
+        slots = [int(s) for s in slots]
+        self._live(slots, "clear")
+        copy_slots(self.state, [-1] * len(slots), slots, pos=self.pos)
+        for s in slots:
+            self._host_pos[s] = 0
 
     def layer_state(self, layer):
         """View [n_slots, n_heads, n_states, d, d, 2] of one layer (no copy)."""
