@@ -38,13 +38,18 @@ the prologue kernel before the decode kernel); the engine reads their
 parameters by the reference's names.  The states, the prologue and the
 decode kernel run in fp32; the projection and o_proj GEMMs run in fp32 or,
 with dtype=torch.bfloat16, on bf16 copies of the weights and inputs with fp32
-accumulation (the gates' small GEMMs stay fp32).
+accumulation (the gates' small GEMMs stay fp32).  With weight_bits=4 the two are
+products with 4-bit weights (linear4): q, k, v and o_proj from codes with group
+scales, the decay logits from their own weights in the same launch.
 """
+
+import copy
 
 import torch
 import torch.nn.functional as F
 
 from .decode import SlotPool
+from .linear4 import GROUPS, Weight4, complex_linear4
 from .pam_layer import _in_weight
 from .pam_prologue import HEAD_DIM, HEAD_DIMS, cabs, mag_linear, prologue_decode, proj_columns
 
@@ -53,16 +58,72 @@ def _cat_planes(x):
     return torch.cat([x[..., 0], x[..., 1]], dim=-1)
 
 
+def check_weight_bits(who, bits, group):
+    if bits not in (None, 4):
+        raise ValueError(f"{who}: 4-bit weights, or None for the GEMM dtype's, got {bits}")
+    if group not in GROUPS:
+        raise ValueError(f"{who}: weight_group {group} (one of {GROUPS})")
+
+
+def complex_product(x, w, b):
+    """ComplexLinear of rows x [n, in, 2] -> [n, out, 2]: w a Weight4, or the real matrix on interleaved rows."""
+    if isinstance(w, Weight4):
+        return complex_linear4(x, w, b)
+    n = x.shape[0]
+    return F.linear(x.reshape(n, -1), w, b).view(n, -1, 2)
+
+
+def complex_weight4(mods, group):
+    """Weight4 and bias [out, 2] (or None) of ComplexLinear modules stacked along their outputs."""
+    cat = lambda name: torch.cat([getattr(m, name) for m in mods], 0)  # noqa: E731
+    w = Weight4.quantize(cat("weight_real"), cat("weight_imag"), group)
+    if all(getattr(m, "bias_real", None) is None for m in mods):
+        return w, None
+    zero = lambda m: m.weight_real.new_zeros(m.weight_real.shape[0])  # noqa: E731
+    b = [torch.cat([zero(m) if getattr(m, "bias_real", None) is None else getattr(m, name) for m in mods])
+         for name in ("bias_real", "bias_imag")]
+    return w, torch.stack(b, -1).float().contiguous()
+
+
+def _replaced(obj, **values):
+    """A shallow copy of a module (or plain object) with some attributes of its own."""
+    new = copy.copy(obj)
+    if isinstance(new, torch.nn.Module):
+        for part in ("_parameters", "_buffers", "_modules"):
+            new.__dict__[part] = {k: v for k, v in obj.__dict__[part].items() if k not in values}
+        new.__dict__.update(values)
+    else:
+        for k, v in values.items():
+            setattr(new, k, v)
+    return new
+
+
+def quantized_layer(layer, group):
+    """`layer` (a PAM layer) with the values of its 4-bit q, k, v and o_proj weights in
+    their place: what a prompt runs on where the tokens after it run on the codes."""
+    def projection(m):
+        w = Weight4.quantize(m.weight_real, m.weight_imag, group).dequantize().to(m.weight_real.dtype)
+        return _replaced(m, weight_real=w[..., 0].contiguous(), weight_imag=w[..., 1].contiguous())
+
+    names = (["qkv_proj"] if layer.fused_qkv else ["q_proj", "k_proj", "v_proj"]) + ["o_proj"]
+    return _replaced(layer, **{name: projection(getattr(layer, name)) for name in names})
+
+
 class DecodeEngine:
     """Decode state and per-step work of `layers` (V11PAMLayer modules, or any
-    module with their attributes) for up to `n_slots` concurrent sequences."""
+    module with their attributes) for up to `n_slots` concurrent sequences.
+    weight_bits=4: the ComplexLinear weights as 4-bit codes, a scale for
+    weight_group of them (32, 64 or 128)."""
 
     MAX_GRAPHS = 64  # captured graphs kept at once (each holds its own buffers)
 
-    def __init__(self, layers, n_slots, *, max_len=4096, graphs=False, graph_bucket=16, dtype=torch.float32):
+    def __init__(self, layers, n_slots, *, max_len=4096, graphs=False, graph_bucket=16, dtype=torch.float32,
+                 weight_bits=None, weight_group=32):
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("DecodeEngine: dtype must be float32 or bfloat16")
+        check_weight_bits("DecodeEngine", weight_bits, weight_group)
         self.dtype = dtype
+        self.weight_bits, self.weight_group = weight_bits, weight_group
         self.layers = list(layers)
         l0 = self.layers[0]
         self.n_heads, self.head_dim, self.n_states = l0.num_heads, l0.head_dim, l0.n_states
@@ -102,15 +163,21 @@ class DecodeEngine:
                 w_in, b_in = _in_weight(layer, h, d, cols)
                 wr, wi = layer.o_proj.weight_real, layer.o_proj.weight_imag
                 dim = wr.shape[0]
-                # y interleaved [n, H d, 2] -> out interleaved [n, dim, 2]
-                w_out = torch.stack([torch.stack([wr, -wi], -1), torch.stack([wi, wr], -1)], 1).reshape(2 * dim, -1)
-                b_out = None
-                if getattr(layer.o_proj, "bias_real", None) is not None:
-                    b_out = torch.stack([layer.o_proj.bias_real, layer.o_proj.bias_imag], 1).reshape(2 * dim)
                 dt = self.dtype  # the projection and o_proj GEMMs' dtype
-                entry = dict(w_in=w_in.to(dt).contiguous(), b_in=None if b_in is None else b_in.to(dt),
-                             w_out=w_out.to(dt).contiguous(), b_out=None if b_out is None else b_out.to(dt),
-                             dim=dim, w_mag=None,
+                if self.weight_bits == 4:  # q, k, v in codes, the decay logits' rows (and padding) whole
+                    mods = [layer.qkv_proj] if layer.fused_qkv else [layer.q_proj, layer.k_proj, layer.v_proj]
+                    tail = w_in[6 * h * d:].to(dt).contiguous()
+                    w_in, b_in = complex_weight4(mods, self.weight_group)
+                    w_out, b_out = complex_weight4([layer.o_proj], self.weight_group)
+                else:
+                    # y interleaved [n, H d, 2] -> out interleaved [n, dim, 2]
+                    w_out = torch.stack([torch.stack([wr, -wi], -1), torch.stack([wi, wr], -1)], 1).reshape(2 * dim, -1)
+                    b_out = None
+                    if getattr(layer.o_proj, "bias_real", None) is not None:
+                        b_out = torch.stack([layer.o_proj.bias_real, layer.o_proj.bias_imag], 1).reshape(2 * dim)
+                    tail, w_in, w_out = None, w_in.to(dt).contiguous(), w_out.to(dt).contiguous()
+                    b_in, b_out = (None if b is None else b.to(dt) for b in (b_in, b_out))
+                entry = dict(w_in=w_in, b_in=b_in, tail=tail, w_out=w_out, b_out=b_out, dim=dim, w_mag=None,
                              dt_bias=(layer.dt_bias if layer.dt_proj.bias is None
                                       else layer.dt_bias + layer.dt_proj.bias).float().contiguous(),
                              state_offset=(layer.state_dt_offset.float().contiguous() if self.n_states > 1
@@ -147,6 +214,18 @@ class DecodeEngine:
 
     def release(self, slot):
         self.pool.release(slot)
+
+    def fork(self, slot, count=1):
+        """`count` more sequences from where `slot` is: their slot ids (SlotPool.fork)."""
+        return self.pool.fork(slot, count)
+
+    def reorder(self, slots, parents):
+        """slots[i] continues from where parents[i] was (SlotPool.reorder)."""
+        self.pool.reorder(slots, parents)
+
+    def compact(self):
+        """The live sequences in the lowest slots: {old slot: new slot} (SlotPool.compact)."""
+        return self.pool.compact()
 
     def layer_state(self, layer_idx, slot):
         """State of one sequence in one layer as the reference holds it:
@@ -196,7 +275,10 @@ class DecodeEngine:
         if n == 0:
             return x.new_zeros(0, dim, 2)
         x = x.contiguous() if x.dtype in (torch.float32, torch.bfloat16) else x.float().contiguous()
-        proj = F.linear(x.view(n, 2 * dim).to(self.dtype), w["w_in"], w["b_in"]).view(n, 1, -1)
+        if w["tail"] is not None:
+            proj = complex_linear4(x.to(self.dtype), w["w_in"], w["b_in"], planes=True, tail=w["tail"]).view(n, 1, -1)
+        else:
+            proj = F.linear(x.view(n, 2 * dim).to(self.dtype), w["w_in"], w["b_in"]).view(n, 1, -1)
         if not layer.use_rope:
             raise NotImplementedError("DecodeEngine applies RoPE per slot; layers without RoPE are not supported")
         out = torch.empty(n, h, d, 2, device=x.device, dtype=self.dtype)
@@ -208,7 +290,7 @@ class DecodeEngine:
                                     phase_col=(h if layer.use_gsp else 0) if m > 1 else -1,
                                     state_offset=w["state_offset"], qk_norm=layer.qk_norm,
                                     gamma_floor=layer.gamma_floor or 0.0)
-            return F.linear(y.view(n, 2 * h * d), w["w_out"], w["b_out"]).view(n, dim, 2)
+            return complex_product(y.view(n, h * d, 2), w["w_out"], w["b_out"])
         protect, phase, routing = self._gates(layer, x, w)
         # the prologue writes fp32 planes (what the decode kernel reads) from a bf16 or fp32 projection
         (qr, qi), (kr, ki), (vr, vi), gamma, rot = prologue_decode(
@@ -224,7 +306,7 @@ class DecodeEngine:
         # every listed slot is live, so the kernel writes every row of y: no zero fill
         # y in the GEMM dtype straight from the decode kernel (no conversion pass before o_proj)
         y = self.pool.step(layer_idx, q, k, v, g, slots, rot=r, q_scale=d ** -0.5, compact=True, out=out)
-        return F.linear(y.view(n, 2 * h * d), w["w_out"], w["b_out"]).view(n, dim, 2)
+        return complex_product(y.view(n, h * d, 2), w["w_out"], w["b_out"])
 
     def _layers(self, x, slots, between):
         for li in range(len(self.layers)):

@@ -28,6 +28,13 @@ accumulation; the residual stream, the norms' statistics and the PAM states
 stay fp32).  With graphs=True a whole step (every layer and the head) is
 captured once per live-count bucket and replayed.
 
+With weight_bits=4 every ComplexLinear is a product with 4-bit weights (linear4), with
+table_bits=4 the logits' table too; prompts and scores run on the values that the codes
+stand for, so a sequence meets one model throughout.
+
+fork gives a sequence's slot to further samples of it, reorder lets the beams of a search
+continue from each other, compact moves the live sequences together.
+
 What the answers are worth: logprobs gives the log probabilities of chosen tokens,
 entropies and top alternatives of a step's logits, score the log probabilities of
 a whole given sequence without its logits.
@@ -49,7 +56,8 @@ from . import _lib
 from . import pam_layer
 from . import triton_kernels as tk
 from .embedding import complex_embedding
-from .engine import DecodeEngine
+from .engine import DecodeEngine, check_weight_bits, complex_product, complex_weight4, quantized_layer
+from .linear4 import Weight4, linear4
 from .token_logprobs import linear_token_logprobs, token_logprobs
 
 MAX_DIM = 2048  # qpam_resid_norm: a thread per four complex columns, 512 per row
@@ -138,20 +146,28 @@ def _bias(lin):
 
 
 class ModelDecoder:
-    """Decode of `model` (V11LM-shaped) for up to `n_slots` concurrent sequences."""
+    """Decode of `model` (V11LM-shaped) for up to `n_slots` concurrent sequences.
+    weight_bits=4: every ComplexLinear's weights as 4-bit codes with a scale for
+    weight_group of them; table_bits=4: the tied table in the logits, too (the
+    embedding lookup keeps its values)."""
 
     MAX_GRAPHS = 64
 
-    def __init__(self, model, n_slots, *, max_len=4096, dtype=torch.float32, graphs=False, graph_bucket=16):
+    def __init__(self, model, n_slots, *, max_len=4096, dtype=torch.float32, graphs=False, graph_bucket=16,
+                 weight_bits=None, weight_group=32, table_bits=None):
         if getattr(model, "pos_embed", None) is not None:
             raise NotImplementedError("ModelDecoder: learned position embeddings (use_learned_pos) are not supported")
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("ModelDecoder: dtype must be float32 or bfloat16")
+        check_weight_bits("ModelDecoder", weight_bits, weight_group)
+        check_weight_bits("ModelDecoder", table_bits, weight_group)
+        self.weight_bits, self.weight_group, self.table_bits = weight_bits, weight_group, table_bits
         self.model = model
         self.blocks = list(model.blocks)
         self.dtype = dtype
         self.engine = DecodeEngine([b.pam for b in self.blocks], n_slots, max_len=max_len, graphs=graphs,
-                                   graph_bucket=graph_bucket, dtype=dtype)
+                                   graph_bucket=graph_bucket, dtype=dtype, weight_bits=weight_bits,
+                                   weight_group=weight_group)
         self.pool = self.engine.pool
         self.graph_bucket = self.engine.graph_bucket
         self._graphs = {}
@@ -170,7 +186,14 @@ class ModelDecoder:
             e = torch.stack([m.embed.embed_real.weight, m.embed.embed_imag.weight], -1).float()  # [V, dim, 2]
             self.vocab, self.dim = e.shape[0], e.shape[1]
             self._embed = e.contiguous().unbind(-1)                                               # fp32, lookups
-            self._embed_w = e.reshape(self.vocab, 2 * self.dim).to(dt).contiguous()           # logits GEMM, fp32: the same memory
+            table, self._table4 = e.reshape(self.vocab, 2 * self.dim), None
+            if self.table_bits == 4:
+                self._table4 = Weight4.quantize(table, group=self.weight_group)
+                table = self._table4.dequantize()                                             # score's products
+            self._embed_w = table.to(dt).contiguous()                                         # logits GEMM, fp32: the same memory
+            # prompts on the values that the codes stand for
+            self._prompt_layers = [quantized_layer(b.pam, self.weight_group) if self.weight_bits == 4 else b.pam
+                                   for b in self.blocks]
             self._blk = []
             if self.dim % 4 or self.dim > MAX_DIM:
                 raise NotImplementedError(f"ModelDecoder: dim {self.dim} (a multiple of 4 up to {MAX_DIM})")
@@ -181,17 +204,14 @@ class ModelDecoder:
                 hid = cgu.gate_proj.weight_real.shape[0]
                 if hid % 4:
                     raise NotImplementedError(f"ModelDecoder: CGU width {hid} (a multiple of 4)")
-                w_gu = torch.cat([interleaved_weight(cgu.gate_proj.weight_real, cgu.gate_proj.weight_imag),
-                                  interleaved_weight(cgu.up_proj.weight_real, cgu.up_proj.weight_imag)], 0)
+                w_gu, w_down = self._weight(cgu.gate_proj, cgu.up_proj), self._weight(cgu.down_proj)
                 # the activation by its parameters (v11/complex_ops.py:102-143): ModReLU has a
                 # bias, ModSwish a bias and beta, the phase-modulated one also phase_alpha / _beta
                 phase = hasattr(act, "phase_alpha")
                 self._blk.append(dict(
                     norm1=(b.norm1.scale.float().contiguous(), float(b.norm1.eps)),
                     norm2=(b.norm2.scale.float().contiguous(), float(b.norm2.eps)),
-                    w_gu=w_gu.to(dt).contiguous(), hid=hid,
-                    w_down=interleaved_weight(cgu.down_proj.weight_real, cgu.down_proj.weight_imag).to(dt)
-                    .contiguous(),
+                    w_gu=w_gu, hid=hid, w_down=w_down,
                     act_bias=prm(act.bias),
                     act_beta=prm(act.beta) if hasattr(act, "beta") else None,
                     act_pa=prm(act.phase_alpha) if phase else None,
@@ -201,9 +221,17 @@ class ModelDecoder:
             self._norm_o = (m.output_norm.scale.float().contiguous(), float(m.output_norm.eps))
             self._norm_h = (m.lm_head_norm.scale.float().contiguous(), float(m.lm_head_norm.eps))
             lp = m.lm_head_proj
-            self._w_head = interleaved_weight(lp.weight_real, lp.weight_imag).to(dt).contiguous()
+            self._w_head = self._weight(lp)
             bh = _bias(lp)
             self._b_head = None if bh is None else bh.to(dt).contiguous()
+            if self.weight_bits == 4 and bh is not None:
+                self._b_head = bh.float().view(-1, 2).contiguous()
+
+    def _weight(self, *mods):
+        """ComplexLinear modules stacked along their outputs, as complex_product takes them (without biases)."""
+        if self.weight_bits == 4:
+            return complex_weight4(mods, self.weight_group)[0]
+        return torch.cat([interleaved_weight(m.weight_real, m.weight_imag) for m in mods], 0).to(self.dtype).contiguous()
 
     # ------------------------------------------------------------ pieces
     @staticmethod
@@ -215,9 +243,9 @@ class ModelDecoder:
         [n, dim, 2] in the GEMM dtype: gate and up in one GEMM, the activation
         and the gate in one launch, the down GEMM."""
         n = h.shape[0]
-        gu = F.linear(h.reshape(n, -1), blk["w_gu"])                          # [n, 4 hid]: gate, up interleaved
+        gu = complex_product(h, blk["w_gu"], None).view(n, -1)                # [n, 4 hid]: gate, up interleaved
         g = cgu_mix(gu, blk["hid"], blk["act_bias"], blk["act_beta"], blk["act_pa"], blk["act_pb"])
-        return F.linear(g.view(n, -1), blk["w_down"]).view(n, self.dim, 2)
+        return complex_product(g, blk["w_down"], None)
 
     def _embedded(self, ids):
         """Normed embedding rows [n, dim, 2] of ids [n]: the fp32 residual stream (NaN for an
@@ -227,12 +255,13 @@ class ModelDecoder:
     def _lm_rows(self, h):
         """The LM head's rows [n, 2 dim] (GEMM dtype) from output-normed rows h [n, dim, 2]."""
         n = h.shape[0]
-        lm = F.linear(h.reshape(n, -1), self._w_head, self._b_head).view(n, self.dim, 2)
+        lm = complex_product(h, self._w_head, self._b_head)
         return self._norm(lm, self._norm_h).reshape(n, -1)
 
     def _head(self, h):
         """Logits [n, V] (fp32) from output-normed rows h [n, dim, 2] (GEMM dtype)."""
-        logits = F.linear(self._lm_rows(h), self._embed_w)                      # [n, V]
+        lm = self._lm_rows(h)
+        logits = F.linear(lm, self._embed_w) if self._table4 is None else linear4(lm, self._table4)   # [n, V]
         return logits if logits.dtype == torch.float32 else logits.float()
 
     def _next_norm(self, li):
@@ -258,9 +287,9 @@ class ModelDecoder:
         x = self._embedded(ids)                                                 # [t, dim, 2] fp32
         h = resid_norm(x, *self._next_norm(-1), out_dtype=dt)
         states = []
-        for li, (blk, b) in enumerate(zip(self._blk, self.blocks)):
+        for li, (blk, pam) in enumerate(zip(self._blk, self._prompt_layers)):
             h2 = resid_norm(x, *blk["norm2"], y=self._cgu(h, blk), y_scale=blk["cgu_scale"])
-            y, s = pam_layer.forward(b.pam, h2.view(1, t, self.dim, 2), None, 0)
+            y, s = pam_layer.forward(pam, h2.view(1, t, self.dim, 2), None, 0)
             states.append(s)
             h = resid_norm(x, *self._next_norm(li), y=y.reshape(t, self.dim, 2).contiguous(),
                            y_scale=blk["pam_scale"], out_dtype=dt)
@@ -307,6 +336,19 @@ class ModelDecoder:
 
     def release(self, slot):
         self.engine.release(slot)
+
+    def fork(self, slot, count=1):
+        """`count` more sequences from where `slot` is (samples of one prompt): their slot ids."""
+        return self.engine.fork(slot, count)
+
+    def reorder(self, slots, parents):
+        """slots[i] continues from where parents[i] was: a beam search's step, in place, with
+        host lists or device tensors."""
+        self.engine.reorder(slots, parents)
+
+    def compact(self):
+        """The live sequences in the lowest slots: {old slot: new slot} of the moved ones."""
+        return self.engine.compact()
 
     def layer_state(self, layer_idx, slot):
         return self.engine.layer_state(layer_idx, slot)
