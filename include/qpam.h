@@ -950,8 +950,11 @@ typedef struct {
     void *y; int64_t ldy;
     int32_t tail_n;
     const void *tail; int64_t ld_tail;
+    void *workspace;               /* qpam_linear4_workspace_size bytes, 16-byte aligned: rows in the */
+    size_t workspace_bytes;        /* kernels' layout, where more than a few are in another */
 } qpam_linear4_args;
 
+size_t qpam_linear4_workspace_size(const qpam_linear4_args *a);
 int qpam_linear4(const qpam_linear4_args *a, void *stream);
 
 /* state[dst[i]] = state[src[i]] for all i at once, the sources as they were before the call

@@ -288,6 +288,7 @@ class Linear4Args(ctypes.Structure):
         ("rows", c_i64), ("n", c_i32), ("k", c_i32), ("group", c_i32), ("is_complex", c_i32), ("dtype", c_i32),
         ("planes", c_i32), ("x", c_ptr), ("ldx", c_i64), ("codes", c_ptr), ("scales", c_ptr), ("bias", c_ptr),
         ("y", c_ptr), ("ldy", c_i64), ("tail_n", c_i32), ("tail", c_ptr), ("ld_tail", c_i64),
+        ("workspace", c_ptr), ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -349,6 +350,7 @@ SIGNATURES = {
     "qpam_cweight_unpack": (ctypes.c_int, [ctypes.POINTER(CWeightArgs), c_ptr]),
     "qpam_cabs_bwd_acc": (ctypes.c_int, [c_i32, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
     "qpam_planes": (ctypes.c_int, [ctypes.POINTER(PlanesArgs), c_ptr]),
+    "qpam_linear4_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(Linear4Args)]),
     "qpam_linear4": (ctypes.c_int, [ctypes.POINTER(Linear4Args), c_ptr]),
     "qpam_copy_slots": (ctypes.c_int, [ctypes.POINTER(SlotsArgs), c_ptr]),
     "qpam_slice_sum": (ctypes.c_int, [c_i32, c_i32, c_i32, c_i64, c_i64, c_ptr, c_ptr, c_ptr]),

@@ -263,8 +263,261 @@ __global__ __launch_bounds__(1024) void rows_kernel(Par p) {
     }
 }
 
+// ---------------------------------------------------------------- more rows --
+// From here on rows are bf16 planes [parts][rows][ldx], 16-byte aligned, whole blocks of 128 inputs: the
+// caller's where they are that, else laid out by lay_rows_kernel (fp32 rows: their three parts).  Rows are
+// the MFMA's rows as they stand; of a complex weight's codes come two operands, (wr, -wi) and (wi, wr),
+// whose sums are the real and the imaginary outputs in the same lane.
+
+struct Rows {
+    const unsigned short *x;
+    long ldx, plane;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void lay_rows_kernel(const T *x, long ldx, long rows, int kr, int kp, unsigned short *out) {
+    const long per = kp / 8;
+    for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < rows * per; at += (long)gridDim.x * 256) {
+        const long row = at / per;
+        const int k = (int)(at - row * per) * 8;
+        Eight<T> v;
+        v.load(x + row * ldx, k, kr, 0);
+        bf16x8 part[Eight<T>::PARTS];
+        v.split(part);
+#pragma unroll
+        for (int h = 0; h < Eight<T>::PARTS; ++h)
+            *reinterpret_cast<bf16x8 *>(out + ((long)h * rows + row) * kp + k) = part[h];
+    }
+}
+
+template <bool CPLX, int NT> constexpr int columns() { return CPLX ? 2 * NT : NT; }
+
+// The MFMA operands of one step's codes.
+template <bool CPLX, int NT>
+__device__ __forceinline__ void operands(const unsigned (&w)[NT], bf16x8 (&f)[columns<CPLX, NT>()]) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const bf16x8 e = widen(w[t]);
+        if constexpr (CPLX) {
+            uintx4 a = __builtin_bit_cast(uintx4, e), b;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                b[j] = __builtin_amdgcn_alignbit(a[j], a[j], 16);
+                a[j] ^= 0x80000000u;
+            }
+            f[2 * t] = frag(a), f[2 * t + 1] = frag(b);
+        } else {
+            f[t] = e;
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void put_pair(const Par &p, long row, int col, float re, float im) {
+    T *y = static_cast<T *>(p.y) + row * p.ldy;
+    if (p.bias) re += p.bias[2 * (long)col], im += p.bias[2 * (long)col + 1];
+    if (p.planes) {
+        put(y, col, re);
+        put(y, (long)p.n + col, im);
+    } else if constexpr (sizeof(T) == 2) {
+        const unsigned v = pack_bf16x2(re, im);
+        __builtin_memcpy(y + 2 * (long)col, &v, 4);
+    } else {
+        const floatx2 v = {re, im};
+        __builtin_memcpy(y + 2 * (long)col, &v, 8);
+    }
+}
+
+// Sums of four neighbouring rows and one output (complex: its two parts).
+template <typename T, bool CPLX>
+__device__ __forceinline__ void finish(const Par &p, long row, int col, floatx4 a, floatx4 b) {
+    if (col >= p.n) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (row + i >= p.rows) return;
+        if constexpr (CPLX) put_pair<T>(p, row + i, col, a[i], b[i]);
+        else put(static_cast<T *>(p.y), (row + i) * p.ldy + col, a[i] + (p.bias ? p.bias[col] : 0.f));
+    }
+}
+
+// A weight block of the wave: its codes and, per output, its scales.
+template <int NT, int G> struct Block {
+    uintx4 w[NT];
+    float s[NT][G];
+    __device__ __forceinline__ void load(const Par &p, int tile0, int c, int lane) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const long blk = (long)min(tile0 + t, p.tiles - 1) * p.chunks + c;
+            w[t] = reinterpret_cast<const uintx4 *>(p.codes)[blk * 64 + lane];
+            const unsigned short *at = p.scales + (blk * TR + (lane & 15)) * G;
+            if constexpr (G == 4) {
+                const ushortx4 v = *reinterpret_cast<const ushortx4 *>(at);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) s[t][g] = bf16_to_f32(v[g]);
+            } else if constexpr (G == 2) {
+                const unsigned v = *reinterpret_cast<const unsigned *>(at);
+                s[t][0] = __uint_as_float(v << 16), s[t][1] = __uint_as_float(v & 0xffff0000u);
+            } else {
+                s[t][0] = bf16_to_f32(*at);
+            }
+        }
+    }
+};
+
+// One weight block times the wave's rows: MFMAs into a group's sums, those times the scale into acc.
+// x(m, step, h) gives the operand of 16 rows.
+template <int PARTS, bool CPLX, int MT, int NT, int G, typename X>
+__device__ __forceinline__ void multiply(const Block<NT, G> &b, floatx4 (&acc)[MT][columns<CPLX, NT>()], X &&x) {
+    constexpr int NF = columns<CPLX, NT>(), STEPS = 4 / G;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        floatx4 sum[MT][NF];
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+            const int ks = g * STEPS + st;
+            unsigned w[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) w[t] = b.w[t][ks];
+            bf16x8 f[NF];
+            operands<CPLX, NT>(w, f);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < PARTS; ++h) {
+                    const bf16x8 xf = x(m, ks, h);
+#pragma unroll
+                    for (int n = 0; n < NF; ++n)
+                        sum[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, f[n], st || h ? sum[m][n] : floatx4{0, 0, 0, 0}, 0, 0, 0);
+                }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NF; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[m][n][i] = fmaf(b.s[n * NT / NF][g], sum[m][n][i], acc[m][n][i]);
+    }
+}
+
+// Block b's place: outputs ct (units of a block's), rows rb.  The row blocks of the same weights come one after
+// another on one XCD, so they find them in its L2.
+__device__ __forceinline__ bool place(const Par &p, long b, int &ct, int &rb) {
+    const long per = 8L * p.row_blocks;
+    ct = (int)(b / per) * 8 + (int)(b & 7), rb = (int)((b / 8) % p.row_blocks);
+    return true;
+}
+
+// Some rows (a decode step's): a block of MT x 16 rows by NT x 16 outputs whose waves take the weight blocks
+// along the inputs in turn, rows from the caches.
+template <typename T, int PARTS, bool CPLX, int MT, int NT, int G>
+__global__ __launch_bounds__(512) void step_kernel(Par p, Rows r) {
+    constexpr int NF = columns<CPLX, NT>();
+    extern __shared__ floatx4 join[];
+    const int waves = blockDim.x >> 6, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long all = (long)p.col_blocks * p.row_blocks;
+    if (blockIdx.x >= all) {
+        tail_dots<T>(p, blockIdx.x - all, waves);
+        return;
+    }
+    int ct, rb;
+    place(p, blockIdx.x, ct, rb);
+    if (ct * NT >= p.tiles) return;
+    const int l16 = lane & 15, q = lane >> 4;
+    const long row0 = (long)rb * MT * 16;
+    const unsigned short *xr[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) xr[m] = r.x + min(row0 + m * 16 + l16, p.rows - 1) * r.ldx + 8 * q;
+    floatx4 acc[MT][NF];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NF; ++n) acc[m][n] = floatx4{0, 0, 0, 0};
+    for (int c = wave; c < p.chunks; c += waves) {
+        Block<NT, G> b;
+        b.load(p, ct * NT, c, lane);
+        multiply<PARTS, CPLX, MT, NT, G>(b, acc, [&](int m, int ks, int h) {
+            return *reinterpret_cast<const bf16x8 *>(xr[m] + h * r.plane + c * TK + 32 * ks);
+        });
+    }
+    // the waves' sums, 16 rows at a time
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        if (m) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NF; ++n) join[(wave * NF + n) * 64 + lane] = acc[m][n];
+        __syncthreads();
+        for (int slot = threadIdx.x; slot < NT * 64; slot += blockDim.x) {
+            const int t = slot >> 6, ln = slot & 63;
+            floatx4 v[NF / NT];
+#pragma unroll
+            for (int z = 0; z < NF / NT; ++z) {
+                v[z] = join[(t * (NF / NT) + z) * 64 + ln];
+                for (int o = 1; o < waves; ++o) v[z] += join[(o * NF + t * (NF / NT) + z) * 64 + ln];
+            }
+            finish<T, CPLX>(p, row0 + m * 16 + 4 * (ln >> 4), (ct * NT + t) * 16 + (ln & 15), v[0], v[NF / NT - 1]);
+        }
+    }
+}
+
+// Many rows (a prompt's): WM x WN waves of MT x 16 rows by NT x 16 outputs; the rows of a weight block of 128
+// inputs through LDS in the MFMA's order (direct loads, two buffers), the weights through registers.
+template <typename T, int PARTS, bool CPLX, int WM, int WN, int MT, int NT, int G>
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Par p, Rows r) {
+    constexpr int NF = columns<CPLX, NT>(), WAVES = WM * WN, MB = WM * MT, PIECES = PARTS * MB * 4;
+    static_assert(PIECES % WAVES == 0, "the waves load alike");
+    __shared__ uintx4 stage[2 * PIECES * 64];   // [2][PARTS][MB][4][64]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wn = wave / WM;
+    const long all = (long)p.col_blocks * p.row_blocks;
+    if (blockIdx.x >= all) {
+        tail_dots<T>(p, blockIdx.x - all, WAVES);
+        return;
+    }
+    int ct, rb;
+    place(p, blockIdx.x, ct, rb);
+    if (ct * WN * NT >= p.tiles) return;
+    const int l16 = lane & 15, q = lane >> 4, tile0 = (ct * WN + wn) * NT;
+    const long row0 = (long)rb * MB * 16;
+    auto fetch = [&](int c) {
+        uintx4 *to = stage + (c & 1) * PIECES * 64;
+#pragma unroll
+        for (int i = 0; i < PIECES / WAVES; ++i) {
+            const int piece = i * WAVES + wave, ks = piece & 3, m = (piece >> 2) % MB, h = (piece >> 2) / MB;
+            const unsigned short *from = r.x + h * r.plane + min(row0 + m * 16 + l16, p.rows - 1) * r.ldx + c * TK + 32 * ks + 8 * q;
+            __builtin_amdgcn_global_load_lds(reinterpret_cast<const unsigned *>(from), reinterpret_cast<unsigned *>(to + piece * 64), 16, 0, 0);
+        }
+    };
+    floatx4 acc[MT][NF];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NF; ++n) acc[m][n] = floatx4{0, 0, 0, 0};
+    Block<NT, G> b, next;
+    fetch(0);
+    b.load(p, tile0, 0, lane);
+    stage_barrier<0>();
+    for (int c = 0; c < p.chunks; ++c) {
+        if (c + 1 < p.chunks) {
+            fetch(c + 1);
+            next.load(p, tile0, c + 1, lane);
+        }
+        const uintx4 *from = stage + (c & 1) * PIECES * 64;
+        multiply<PARTS, CPLX, MT, NT, G>(b, acc, [&](int m, int ks, int h) {
+            return frag(from[((h * MB + wm * MT + m) * 4 + ks) * 64 + lane]);
+        });
+        b = next;
+        stage_barrier<0>();
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            finish<T, CPLX>(p, row0 + (wm * MT + m) * 16 + 4 * q, (tile0 + t) * 16 + l16, acc[m][t * (NF / NT)], acc[m][t * (NF / NT) + NF / NT - 1]);
+}
+
+// ---------------------------------------------------------------- launches --
+
 template <typename T, bool CPLX, int MT, int NT, int G>
-int launch(Par p, int waves, hipStream_t stream) {
+int launch_rows(Par p, int waves, hipStream_t stream) {
     p.col_blocks = ((p.tiles + NT - 1) / NT + 7) / 8 * 8;
     const long vrows = CPLX ? 2 * p.rows : p.rows;
     p.row_blocks = (int)((vrows + MT * TR - 1) / (MT * TR));
@@ -275,28 +528,74 @@ int launch(Par p, int waves, hipStream_t stream) {
     return launch_status("qpam_linear4");
 }
 
+template <typename T, bool CPLX, int MT, int NT, int G>
+int launch_step(Par p, const Rows &r, hipStream_t stream) {
+    constexpr int PARTS = Eight<T>::PARTS, NF = columns<CPLX, NT>();
+    p.col_blocks = ((p.tiles + NT - 1) / NT + 7) / 8 * 8;
+    p.row_blocks = (int)((p.rows + MT * 16 - 1) / (MT * 16));
+    // as few rounds over the inputs as 8 waves need, by as few waves as make that many
+    const int rounds = (p.chunks + 7) / 8, waves = (p.chunks + rounds - 1) / rounds;
+    const long tail_blocks = p.tail_n ? (p.rows * p.tail_n + waves - 1) / waves : 0;
+    const long blocks = (long)p.col_blocks * p.row_blocks + tail_blocks;
+    step_kernel<T, PARTS, CPLX, MT, NT, G><<<dim3((unsigned)blocks), dim3(64 * waves), (size_t)waves * NF * 1024, stream>>>(p, r);
+    return launch_status("qpam_linear4");
+}
+
+template <typename T, bool CPLX, int WM, int WN, int MT, int NT, int G>
+int launch_tile(Par p, const Rows &r, hipStream_t stream) {
+    constexpr int PARTS = Eight<T>::PARTS;
+    p.col_blocks = ((p.tiles + NT * WN - 1) / (NT * WN) + 7) / 8 * 8;
+    p.row_blocks = (int)((p.rows + WM * MT * 16 - 1) / (WM * MT * 16));
+    const long tail_blocks = p.tail_n ? (p.rows * p.tail_n + WM * WN - 1) / (WM * WN) : 0;
+    const long blocks = (long)p.col_blocks * p.row_blocks + tail_blocks;
+    tile_kernel<T, PARTS, CPLX, WM, WN, MT, NT, G><<<dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream>>>(p, r);
+    return launch_status("qpam_linear4");
+}
+
+constexpr int few_rows(bool cplx) { return cplx ? 8 : 16; }
+int padded(int kr) { return (kr + TK - 1) / TK * TK; }
+
+// Rows that the kernels for more rows read as they stand.
+bool stand(const qpam_linear4_args *a, int kr) {
+    return a->dtype == QPAM_BF16 && kr % TK == 0 && (uintptr_t)a->x % 16 == 0 && a->ldx % 8 == 0;
+}
+
+size_t lay_bytes(const qpam_linear4_args *a) {
+    const int kr = a->is_complex ? 2 * a->k : a->k;
+    if (a->rows <= few_rows(a->is_complex) || stand(a, kr)) return 0;
+    return (size_t)a->rows * padded(kr) * 2 * (a->dtype == QPAM_BF16 ? 1 : 3);
+}
+
 template <typename T, bool CPLX, int G>
-int choose(const Par &p, hipStream_t stream) {
-    const long v = CPLX ? 2 * p.rows : p.rows;
-    if (v <= 16) return launch<T, CPLX, 1, 1, G>(p, 16, stream);
-    if (v <= 32) return launch<T, CPLX, 2, 2, G>(p, 16, stream);
-    return launch<T, CPLX, 4, 2, G>(p, 8, stream);
+int choose(const Par &p, const Rows &r, hipStream_t stream) {
+    if (p.rows <= few_rows(CPLX)) return launch_rows<T, CPLX, 1, 1, G>(p, 16, stream);
+    if (p.rows <= 16) return launch_step<T, CPLX, 1, 2, G>(p, r, stream);
+    if (p.rows <= 32) return launch_step<T, CPLX, 2, 2, G>(p, r, stream);
+    if (p.rows <= 400) return launch_step<T, CPLX, 4, 2, G>(p, r, stream);
+    constexpr int WM = sizeof(T) == 2 ? 2 : 1;
+    return launch_tile<T, CPLX, WM, 4 / WM, 4, CPLX ? 2 : 4, G>(p, r, stream);
 }
 
 template <typename T>
-int by_group(const Par &p, int cplx, int group, hipStream_t stream) {
+int by_group(const Par &p, const Rows &r, int cplx, int group, hipStream_t stream) {
     if (cplx) {
-        if (group == 32) return choose<T, true, 4>(p, stream);
-        if (group == 64) return choose<T, true, 2>(p, stream);
-        return choose<T, true, 1>(p, stream);
+        if (group == 32) return choose<T, true, 4>(p, r, stream);
+        if (group == 64) return choose<T, true, 2>(p, r, stream);
+        return choose<T, true, 1>(p, r, stream);
     }
-    if (group == 32) return choose<T, false, 4>(p, stream);
-    if (group == 64) return choose<T, false, 2>(p, stream);
-    return choose<T, false, 1>(p, stream);
+    if (group == 32) return choose<T, false, 4>(p, r, stream);
+    if (group == 64) return choose<T, false, 2>(p, r, stream);
+    return choose<T, false, 1>(p, r, stream);
 }
 
 }  // namespace w4
 }  // namespace qpam
+
+extern "C" size_t qpam_linear4_workspace_size(const qpam_linear4_args *a) {
+    const int64_t k = a->is_complex ? 2 * (int64_t)a->k : a->k;
+    if (a->rows < 1 || a->rows > (1L << 40) || k < 1 || k > (1 << 25)) return 0;
+    return qpam::w4::lay_bytes(a);
+}
 
 extern "C" int qpam_linear4(const qpam_linear4_args *a, void *stream) {
     using namespace qpam;
@@ -325,16 +624,32 @@ extern "C" int qpam_linear4(const qpam_linear4_args *a, void *stream) {
     p.codes = static_cast<const unsigned char *>(a->codes), p.scales = static_cast<const unsigned short *>(a->scales);
     p.bias = a->bias, p.planes = a->planes, p.tail_n = a->tail_n, p.tail = a->tail;
     p.vec = kr % 8 == 0 && (uintptr_t)a->x % 16 == 0 && a->ldx * elem % 16 == 0;
+    const size_t bytes = w4::lay_bytes(a);
+    if (bytes && (!a->workspace || a->workspace_bytes < bytes || (uintptr_t)a->workspace % 16))
+        return fail(QPAM_ERR_WORKSPACE, "qpam_linear4: workspace of %zu bytes (16-byte aligned) needed", bytes);
+    hipStream_t st = (hipStream_t)stream;
     // a launch has fewer than 2^32 threads: rows in pieces
     const long per_block = (long)(p.tiles + 8) * 1024;
     const long step = std::max<long>(64, ((1L << 31) / per_block) * 8 / (1 + a->tail_n));
-    for (long r = 0; r < a->rows; r += step) {
-        p.rows = std::min<long>(step, a->rows - r);
-        p.x = static_cast<const char *>(a->x) + r * a->ldx * elem;
-        p.y = static_cast<char *>(a->y) + r * a->ldy * elem;
-        const int st = a->dtype == QPAM_BF16 ? w4::by_group<unsigned short>(p, a->is_complex, a->group, (hipStream_t)stream)
-                                             : w4::by_group<float>(p, a->is_complex, a->group, (hipStream_t)stream);
-        if (st) return st;
+    for (long at = 0; at < a->rows; at += step) {
+        p.rows = std::min<long>(step, a->rows - at);
+        p.x = static_cast<const char *>(a->x) + at * a->ldx * elem;
+        p.y = static_cast<char *>(a->y) + at * a->ldy * elem;
+        w4::Rows r{static_cast<const unsigned short *>(p.x), a->ldx, 0};
+        if (bytes) {  // each piece in turn through the same memory
+            const int kp = w4::padded(kr);
+            unsigned short *ws = static_cast<unsigned short *>(a->workspace);
+            const long blocks = std::min<long>((p.rows * (kp / 8) + 255) / 256, 1 << 20);
+            if (a->dtype == QPAM_BF16)
+                w4::lay_rows_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(static_cast<const unsigned short *>(p.x), a->ldx, p.rows, kr, kp, ws);
+            else
+                w4::lay_rows_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(static_cast<const float *>(p.x), a->ldx, p.rows, kr, kp, ws);
+            if (const int e = launch_status("qpam_linear4")) return e;
+            r = w4::Rows{ws, kp, p.rows * kp};
+        }
+        const int e = a->dtype == QPAM_BF16 ? w4::by_group<unsigned short>(p, r, a->is_complex, a->group, st)
+                                            : w4::by_group<float>(p, r, a->is_complex, a->group, st);
+        if (e) return e;
     }
     return QPAM_OK;
 }

@@ -174,8 +174,13 @@ def _product(x: Tensor, codes: Tensor, scales: Tensor, n: int, k: int, group: in
     a = _lib.Linear4Args(rows.shape[0], n, k, group, is_complex, _CODE[x.dtype], planes, rows.data_ptr(), ldx, codes.data_ptr(),
                          scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), z * n + extra, extra,
                          None if tail is None else tail.data_ptr(), 0 if tail is None else tail.stride(0))
+    L = _lib.lib()
+    nbytes = L.qpam_linear4_workspace_size(ctypes.byref(a))
+    if nbytes:
+        ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
     with _lib.device(x.device):
-        _lib.check(_lib.lib().qpam_linear4(ctypes.byref(a), _lib.stream_ptr(x.device)), "qpam_linear4")
+        _lib.check(L.qpam_linear4(ctypes.byref(a), _lib.stream_ptr(x.device)), "qpam_linear4")
     return out
 
 
