@@ -931,11 +931,13 @@ int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void *stream);
  * re = Wr xr - Wi xi, im = Wi xr + Wr xi).  planes 1: y's row is the n real parts, the n
  * imaginary parts and then tail_n further real outputs x . tail[t] (tail [tail_n][2k] in
  * dtype, row stride ld_tail: outputs whose weights stay whole).
- * codes: blocks of 16 outputs x 128 inputs, [ceil(n/16)][ceil(K/128)][1024 bytes] with K = k
- * (2k complex); in a block, byte 16 l + 4 s + b of lane l = 16 q + r holds the codes of output r and
- * inputs 32 s + 8 q + 2 b (low half) and the next (high half).  scales: [ceil(n/16)]
- * [ceil(K/128)][16][128/group] bf16.  Codes and scales outside n and K are zero.  codes
- * 16-byte, scales 8-byte aligned.  n and k at most 2^24. */
+ * codes: blocks of 16 outputs x 64 inputs, [ceil(n/16)][ceil(K/64)][512 bytes] with K = k (2k
+ * complex); in a block, byte 8 l + 4 s + b of lane l = 16 q + r holds the codes of output r and
+ * inputs 32 s + 8 q + 2 b (low half) and the next (high half).  scales, bf16: group 32
+ * [ceil(n/16)][ceil(K/64)][16][2], group 64 [ceil(n/16)][ceil(K/64)][16], group 128
+ * [ceil(n/16)][ceil(K/128)][16].  Codes and scales outside n and K are zero.  codes 16-byte,
+ * scales 4-byte aligned.  n at most 2^22, k
+ * 2^24. */
 typedef struct {
     int64_t rows;
     int32_t n, k;

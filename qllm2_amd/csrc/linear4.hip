@@ -14,8 +14,8 @@
 // (xi, xr) made from a row x, the real and the imaginary output are two rows of one real product.  (The
 // same product as a real matrix [wr, -wi; wi, wr] has every weight twice.)
 //
-// Layout (qpam_linear4 in the header): 1 KB blocks of 16 outputs x 128 inputs in the order of the MFMA's
-// B operand, so a wave reads its weights as whole consecutive 16-byte lanes.
+// Layout (qpam_linear4 in the header): 512-byte blocks of 16 outputs x 64 inputs in the order of the MFMA's
+// B operand, so a wave reads its weights as whole consecutive 8-byte lanes.
 #include <algorithm>
 
 #include "common.h"
@@ -24,22 +24,23 @@ namespace qpam {
 namespace w4 {
 
 constexpr int TR = 16;    // outputs of a weight block
-constexpr int TK = 128;   // inputs of a weight block
+constexpr int TK = 64;    // inputs of a weight block: two MFMA steps
 
 struct Par {
     long rows;                 // x rows of this launch
-    int n, kr;                 // outputs (complex ones), real inputs
-    int chunks, tiles;         // weight blocks along the inputs, along the outputs
+    int n, kr;                 // outputs (complex ones), real inputs of the rows that the kernel reads
+    int units, tiles;          // weight blocks along the inputs, along the outputs
+    int scale_step;            // weight blocks that share a scale (2 of group 128)
     const void *x; long ldx;
     const unsigned char *codes;
     const unsigned short *scales;
     const float *bias;
     void *y; long ldy;
     int planes;
-    int row_blocks;            // blocks along the rows
-    int col_blocks;            // blocks along the outputs, rounded up to the XCDs
-    int vec;                   // 16-byte loads of x are aligned and whole
-    int tail_n;
+    int slices;                // grid slices of 8 blocks along the outputs; behind them (times splits) those of the tail
+    int splits, share;         // ranges of `share` weight blocks along the inputs whose sums are joined by join_kernel
+    floatx4 *sums;
+    int tail_n, tail_k;        // of the caller's rows x
     const void *tail; long ld_tail;
 };
 
@@ -55,220 +56,78 @@ __device__ __forceinline__ bf16x8 widen(unsigned w) {
     return frag(r);
 }
 
-// 8 values of a row from input k on, zeros behind the last input
-template <typename T> struct Eight;
-template <> struct Eight<unsigned short> {
-    uintx4 v;
-    __device__ __forceinline__ void load(const unsigned short *row, int k, int kr, int vec) {
-        v = uintx4{0, 0, 0, 0};
-        if (vec) {
-            if (k < kr) v = *reinterpret_cast<const uintx4 *>(row + k);
-        } else {
+// fp32 values as sums of three bf16 values, the largest last: each the leading 8 bits of what is left, so the
+// sum is exact.  Infinities and NaN stay in the last alone (inf - inf would make NaN of them).
+__device__ __forceinline__ void split(const float (&v)[8], bf16x8 (&p)[3]) {
+    uintx4 hi, mid, lo;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (k + j < kr) v[j >> 1] |= (unsigned)row[k + j] << (16 * (j & 1));
+    for (int j = 0; j < 4; ++j) {
+        unsigned h[2], m[2], l[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float f = v[2 * j + e];
+            h[e] = __float_as_uint(f) & 0xffff0000u;
+            const float r = (h[e] & 0x7f800000u) == 0x7f800000u ? 0.f : f - __uint_as_float(h[e]);
+            m[e] = __float_as_uint(r) & 0xffff0000u;
+            l[e] = __float_as_uint(r - __uint_as_float(m[e]));
+            // a NaN whose payload is in the low bits alone stays a NaN
+            if (f != f) h[e] |= 0x400000u;
         }
+        hi[j] = h[0] >> 16 | (h[1] & 0xffff0000u);
+        mid[j] = m[0] >> 16 | (m[1] & 0xffff0000u);
+        lo[j] = l[0] >> 16 | (l[1] & 0xffff0000u);
     }
-    // the row (xr, -xi) of a complex row where im is 0, (xi, xr) where it is 1
-    __device__ __forceinline__ void turn(int im) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = im ? (v[j] >> 16 | v[j] << 16) : v[j] ^ 0x80000000u;
-    }
-    static constexpr int PARTS = 1;
-    __device__ __forceinline__ void split(bf16x8 (&p)[1]) const { p[0] = frag(v); }
-};
-template <> struct Eight<float> {
-    float v[8];
-    __device__ __forceinline__ void load(const float *row, int k, int kr, int vec) {
-        if (vec) {
-            floatx4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-            if (k < kr) {
-                a = *reinterpret_cast<const floatx4 *>(row + k);
-                b = *reinterpret_cast<const floatx4 *>(row + k + 4);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = k + j < kr ? row[k + j] : 0.f;
-        }
-    }
-    __device__ __forceinline__ void turn(int im) {
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const float a = v[j], b = v[j + 1];
-            v[j] = im ? b : a;
-            v[j + 1] = im ? a : -b;
-        }
-    }
-    static constexpr int PARTS = 3;
-    // v as a sum of three bf16 values, the largest last: each the leading 8 bits of what is left, so the
-    // sum is exact.  Infinities and NaN stay in the first alone (inf - inf would make NaN of them).
-    __device__ __forceinline__ void split(bf16x8 (&p)[3]) const {
-        uintx4 hi, mid, lo;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            unsigned h[2], m[2], l[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float f = v[2 * j + e];
-                h[e] = __float_as_uint(f) & 0xffff0000u;
-                const float r = (h[e] & 0x7f800000u) == 0x7f800000u ? 0.f : f - __uint_as_float(h[e]);
-                m[e] = __float_as_uint(r) & 0xffff0000u;
-                l[e] = __float_as_uint(r - __uint_as_float(m[e]));
-                // a NaN whose payload is in the low bits alone stays a NaN
-                if (f != f) h[e] |= 0x400000u;
-            }
-            hi[j] = h[0] >> 16 | (h[1] & 0xffff0000u);
-            mid[j] = m[0] >> 16 | (m[1] & 0xffff0000u);
-            lo[j] = l[0] >> 16 | (l[1] & 0xffff0000u);
-        }
-        p[0] = frag(lo), p[1] = frag(mid), p[2] = frag(hi);
-    }
-};
+    p[0] = frag(lo), p[1] = frag(mid), p[2] = frag(hi);
+}
 
 __device__ __forceinline__ void put(float *y, long at, float v) { y[at] = v; }
 __device__ __forceinline__ void put(unsigned short *y, long at, float v) { y[at] = (unsigned short)pack_bf16x2(v, v); }
 __device__ __forceinline__ float wide(float v) { return v; }
 __device__ __forceinline__ float wide(unsigned short v) { return bf16_to_f32(v); }
 
-// Four neighbouring (virtual) rows of output col, finished sums.
-template <typename T, bool CPLX>
-__device__ __forceinline__ void store4(const Par &p, long vrow, int col, floatx4 v) {
-    T *y = static_cast<T *>(p.y);
-    if (col >= p.n) return;
-    if constexpr (CPLX) {
-        float br = 0.f, bi = 0.f;
-        if (p.bias) br = p.bias[2 * (long)col], bi = p.bias[2 * (long)col + 1];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const long row = (vrow >> 1) + i;
-            if (row >= p.rows) return;
-            const long at = row * p.ldy;
-            put(y, at + (p.planes ? col : 2 * (long)col), v[2 * i] + br);
-            put(y, at + (p.planes ? (long)p.n + col : 2 * (long)col + 1), v[2 * i + 1] + bi);
-        }
-    } else {
-        const float b = p.bias ? p.bias[col] : 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (vrow + i < p.rows) put(y, (vrow + i) * p.ldy + col, v[i] + b);
-    }
-}
-
-// Outputs whose weights stay whole (the decay logits of a projection): a wave per row and output, the
-// inputs over its lanes.
+// Outputs whose weights stay whole (the decay logits of a projection): a wave per row and TAIL outputs, the
+// inputs over its lanes, 8 at a time where they are aligned.
+constexpr int TAIL = 4;
 template <typename T>
-__device__ void tail_dots(const Par &p, long block, int waves) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long pair = block * waves + wave;
-    const long row = pair / p.tail_n;
-    const int t = (int)(pair - row * p.tail_n);
+__device__ void tail_dots(const Par &p, int waves) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), groups = (p.tail_n + TAIL - 1) / TAIL;
+    const long block = ((long)((int)blockIdx.z - p.slices * p.splits) * gridDim.y + blockIdx.y) * 8 + blockIdx.x, pair = block * waves + wave;
+    const long row = pair / groups;
+    const int t0 = (int)(pair - row * groups) * TAIL;
     if (row >= p.rows) return;
-    const T *x = static_cast<const T *>(p.x) + row * p.ldx, *w = static_cast<const T *>(p.tail) + t * p.ld_tail;
-    float s = 0.f;
-    for (int k = lane; k < p.kr; k += 64) s = fmaf(wide(x[k]), wide(w[k]), s);
-    s = row16_sum(s);
-    s += __shfl_xor(s, 16);
-    s += __shfl_xor(s, 32);
-    if (lane == 0) put(static_cast<T *>(p.y), row * p.ldy + 2 * (long)p.n + t, s);
-}
-
-// A block: MT x 16 (virtual) rows by NT x 16 outputs, its waves the weight blocks along the inputs in
-// turn, their sums joined through LDS in the waves' order.
-template <typename T, bool CPLX, int MT, int NT, int G>
-__global__ __launch_bounds__(1024) void rows_kernel(Par p) {
-    extern __shared__ floatx4 join[];
-    const int waves = blockDim.x >> 6, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long b = blockIdx.x, all = (long)p.col_blocks * p.row_blocks;
-    if (b >= all) {
-        tail_dots<T>(p, b - all, waves);
-        return;
-    }
-    // the row blocks of one weight tile on one XCD, next to each other, so they find it in its L2
-    const long per = 8L * p.row_blocks;
-    const int ct = (int)(b / per) * 8 + (int)(b & 7), rb = (int)((b / 8) % p.row_blocks);
-    if (ct * NT >= p.tiles) return;
-    const int l16 = lane & 15, q = lane >> 4;
-    const long vrow0 = (long)rb * MT * TR;
-    const T *xr[MT];
+    const T *x = static_cast<const T *>(p.x) + row * p.ldx, *w[TAIL];
+    float s[TAIL];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {  // rows behind the last read the last one, and are not written
-        const long v = vrow0 + m * TR + l16, row = CPLX ? v >> 1 : v;
-        xr[m] = static_cast<const T *>(p.x) + (row < p.rows ? row : p.rows - 1) * p.ldx;
-    }
-    floatx4 acc[MT][NT];
+    for (int t = 0; t < TAIL; ++t) w[t] = static_cast<const T *>(p.tail) + min(t0 + t, p.tail_n - 1) * p.ld_tail, s[t] = 0.f;
+    constexpr int V = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(V)));
+    const bool whole = !(((uintptr_t)x | (uintptr_t)w[0] | (uintptr_t)(p.ld_tail * sizeof(T))) & 15);
+    for (int k = V * lane; k < p.tail_k; k += 64 * V) {   // (the same order of the sums in either form)
+        if (whole && k + V <= p.tail_k) {
+            const vec a = *reinterpret_cast<const vec *>(x + k);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+            for (int t = 0; t < TAIL; ++t) {
+                const vec b = *reinterpret_cast<const vec *>(w[t] + k);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[m][t] = floatx4{0, 0, 0, 0};
-
-    for (int c = wave; c < p.chunks; c += waves) {
-        uintx4 w[NT];
-        float s[NT][G];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int tile = min(ct * NT + t, p.tiles - 1);
-            const long blk = (long)tile * p.chunks + c;
-            w[t] = reinterpret_cast<const uintx4 *>(p.codes)[blk * 64 + lane];
-#pragma unroll
-            for (int g = 0; g < G; ++g) s[t][g] = bf16_to_f32(p.scales[(blk * TR + l16) * G + g]);
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            constexpr int STEPS = 4 / G;
-            floatx4 sum[MT][NT];
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) sum[m][t] = floatx4{0, 0, 0, 0};
-#pragma unroll
-            for (int st = 0; st < STEPS; ++st) {
-                const int ks = g * STEPS + st;
-                bf16x8 wf[NT];
-#pragma unroll
-                for (int t = 0; t < NT; ++t) wf[t] = widen(w[t][ks]);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    Eight<T> x;
-                    x.load(xr[m], c * TK + 32 * ks + 8 * q, p.kr, p.vec);
-                    if (CPLX) x.turn(lane & 1);
-                    bf16x8 part[Eight<T>::PARTS];
-                    x.split(part);
-#pragma unroll
-                    for (int h = 0; h < Eight<T>::PARTS; ++h)
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-                            sum[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(part[h], wf[t], sum[m][t], 0, 0, 0);
-                }
+                for (int j = 0; j < V; ++j) s[t] = fmaf(wide(a[j]), wide(b[j]), s[t]);
             }
+        } else {
+            for (int j = k; j < min(k + V, p.tail_k); ++j)
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[m][t][i] = fmaf(s[t][g], sum[m][t][i], acc[m][t][i]);
+                for (int t = 0; t < TAIL; ++t) s[t] = fmaf(wide(x[j]), wide(w[t][j]), s[t]);
         }
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) join[(wave * MT * NT + m * NT + t) * 64 + lane] = acc[m][t];
-    __syncthreads();
-    for (int slot = threadIdx.x; slot < MT * NT * 64; slot += blockDim.x) {
-        floatx4 v = join[slot];
-        for (int o = 1; o < waves; ++o) v += join[o * MT * NT * 64 + slot];
-        const int t = (slot >> 6) % NT, m = (slot >> 6) / NT, ln = slot & 63;
-        store4<T, CPLX>(p, vrow0 + m * TR + 4 * (ln >> 4), (ct * NT + t) * TR + (ln & 15), v);
+    for (int t = 0; t < TAIL; ++t) {
+        float v = row16_sum(s[t]);
+        v += __shfl_xor(v, 16);
+        v += __shfl_xor(v, 32);
+        if (lane == 0 && t0 + t < p.tail_n) put(static_cast<T *>(p.y), row * p.ldy + 2 * (long)p.n + t0 + t, v);
     }
 }
 
-// ---------------------------------------------------------------- more rows --
-// From here on rows are bf16 planes [parts][rows][ldx], 16-byte aligned, whole blocks of 128 inputs: the
-// caller's where they are that, else laid out by lay_rows_kernel (fp32 rows: their three parts).  Rows are
-// the MFMA's rows as they stand; of a complex weight's codes come two operands, (wr, -wi) and (wi, wr),
-// whose sums are the real and the imaginary outputs in the same lane.
-
+// Where a kernel reads rows as bf16 planes [parts][rows][ldx], 16-byte aligned, whole blocks of inputs: the
+// caller's where they are that, else laid out by lay_rows_kernel (fp32 rows: their three parts).
 struct Rows {
     const unsigned short *x;
     long ldx, plane;
@@ -280,16 +139,22 @@ __global__ __launch_bounds__(256) void lay_rows_kernel(const T *x, long ldx, lon
     for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < rows * per; at += (long)gridDim.x * 256) {
         const long row = at / per;
         const int k = (int)(at - row * per) * 8;
-        Eight<T> v;
-        v.load(x + row * ldx, k, kr, 0);
-        bf16x8 part[Eight<T>::PARTS];
-        v.split(part);
+        T v[8];
 #pragma unroll
-        for (int h = 0; h < Eight<T>::PARTS; ++h)
-            *reinterpret_cast<bf16x8 *>(out + ((long)h * rows + row) * kp + k) = part[h];
+        for (int j = 0; j < 8; ++j) v[j] = k + j < kr ? x[row * ldx + k + j] : T(0);
+        unsigned short *to = out + row * kp + k;
+        if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<uintx4 *>(to) = __builtin_bit_cast(uintx4, v);
+        } else {
+            bf16x8 part[3];
+            split(v, part);
+#pragma unroll
+            for (int h = 0; h < 3; ++h) *reinterpret_cast<bf16x8 *>(to + (long)h * rows * kp) = part[h];
+        }
     }
 }
 
+template <typename T> constexpr int parts() { return sizeof(T) == 2 ? 1 : 3; }
 template <bool CPLX, int NT> constexpr int columns() { return CPLX ? 2 * NT : NT; }
 
 // The MFMA operands of one step's codes.
@@ -340,37 +205,77 @@ __device__ __forceinline__ void finish(const Par &p, long row, int col, floatx4 
     }
 }
 
-// A weight block of the wave: its codes and, per output, its scales.
-template <int NT, int G> struct Block {
-    uintx4 w[NT];
-    float s[NT][G];
-    __device__ __forceinline__ void load(const Par &p, int tile0, int c, int lane) {
+// The finished sums of 16 rows by a weight tile, to y; of a range of the inputs, to where join_kernel adds them.
+template <typename T, bool CPLX>
+__device__ __forceinline__ void deliver(const Par &p, int split, int tile, long m, int lane, floatx4 a, floatx4 b) {
+    if (p.splits == 1) {
+        finish<T, CPLX>(p, m * 16 + 4 * (lane >> 4), tile * TR + (lane & 15), a, b);
+    } else {
+        const long ms = (p.rows + 15) / 16;
+        if (tile >= p.tiles || m >= ms) return;
+        floatx4 *to = p.sums + (((long)split * p.tiles + tile) * ms + m) * (CPLX ? 128 : 64) + lane;
+        to[0] = a;
+        if (CPLX) to[64] = b;
+    }
+}
+
+template <typename T, bool CPLX>
+__global__ __launch_bounds__(256) void join_kernel(Par p) {
+    const long ms = (p.rows + 15) / 16, unit = (long)blockIdx.x * 4 + (threadIdx.x >> 6);   // a wave per tile and 16 rows
+    if (unit >= p.tiles * ms) return;
+    const int lane = threadIdx.x & 63;
+    const floatx4 *from = p.sums + unit * (CPLX ? 128 : 64) + lane;
+    floatx4 a = from[0], b = CPLX ? from[64] : a;
+    for (int o = 1; o < p.splits; ++o) {
+        from += p.tiles * ms * (CPLX ? 128 : 64);
+        a += from[0];
+        if (CPLX) b += from[64];
+    }
+    const int tile = (int)(unit / ms);
+    finish<T, CPLX>(p, (unit - tile * ms) * 16 + 4 * (lane >> 4), tile * TR + (lane & 15), a, b);
+}
+
+// The wave's weights: where its tiles' blocks and scales begin (the same for all lanes), and what a lane adds.
+template <int NT, int GU> struct Tiles {
+    const unsigned char *codes[NT];
+    const unsigned short *scales[NT];
+    __device__ __forceinline__ Tiles(const Par &p, int tile0) {
+        const int per = GU == 2 ? 2 * p.units : p.scale_step == 1 ? p.units : (p.units + 1) / 2;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {   // tiles behind the last read the last one, and are not written
+            const long tile = min(tile0 + t, p.tiles - 1);
+            codes[t] = p.codes + tile * p.units * 512;
+            scales[t] = p.scales + tile * per * TR;
+        }
+    }
+};
+
+// A weight block of the wave: its codes and, per output, its scales (GU groups of a block).
+template <int NT, int GU> struct Block {
+    uintx2 w[NT];
+    unsigned s[NT];
+    __device__ __forceinline__ void load(const Par &p, const Tiles<NT, GU> &from, int u, int lane) {
+        const int at = GU == 2 ? 2 * u : p.scale_step == 1 ? u : u >> 1;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const long blk = (long)min(tile0 + t, p.tiles - 1) * p.chunks + c;
-            w[t] = reinterpret_cast<const uintx4 *>(p.codes)[blk * 64 + lane];
-            const unsigned short *at = p.scales + (blk * TR + (lane & 15)) * G;
-            if constexpr (G == 4) {
-                const ushortx4 v = *reinterpret_cast<const ushortx4 *>(at);
-#pragma unroll
-                for (int g = 0; g < 4; ++g) s[t][g] = bf16_to_f32(v[g]);
-            } else if constexpr (G == 2) {
-                const unsigned v = *reinterpret_cast<const unsigned *>(at);
-                s[t][0] = __uint_as_float(v << 16), s[t][1] = __uint_as_float(v & 0xffff0000u);
-            } else {
-                s[t][0] = bf16_to_f32(*at);
-            }
+            w[t] = reinterpret_cast<const uintx2 *>(from.codes[t] + (long)u * 512)[(unsigned)lane];
+            const unsigned short *sc = from.scales[t] + (long)at * TR;
+            if constexpr (GU == 2) s[t] = reinterpret_cast<const unsigned *>(sc)[(unsigned)lane & 15];
+            else s[t] = sc[(unsigned)lane & 15];
         }
+    }
+    __device__ __forceinline__ float scale(int t, int g) const {
+        return __uint_as_float(GU == 2 && g ? s[t] & 0xffff0000u : s[t] << 16);
     }
 };
 
 // One weight block times the wave's rows: MFMAs into a group's sums, those times the scale into acc.
 // x(m, step, h) gives the operand of 16 rows.
-template <int PARTS, bool CPLX, int MT, int NT, int G, typename X>
-__device__ __forceinline__ void multiply(const Block<NT, G> &b, floatx4 (&acc)[MT][columns<CPLX, NT>()], X &&x) {
-    constexpr int NF = columns<CPLX, NT>(), STEPS = 4 / G;
+template <int PARTS, bool CPLX, int MT, int NT, int GU, typename X>
+__device__ __forceinline__ void multiply(const Block<NT, GU> &b, floatx4 (&acc)[MT][columns<CPLX, NT>()], X &&x) {
+    constexpr int NF = columns<CPLX, NT>(), STEPS = 2 / GU;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
+    for (int g = 0; g < GU; ++g) {
         floatx4 sum[MT][NF];
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) {
@@ -395,197 +300,309 @@ __device__ __forceinline__ void multiply(const Block<NT, G> &b, floatx4 (&acc)[M
 #pragma unroll
             for (int n = 0; n < NF; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[m][n][i] = fmaf(b.s[n * NT / NF][g], sum[m][n][i], acc[m][n][i]);
+                for (int i = 0; i < 4; ++i) acc[m][n][i] = fmaf(b.scale(n * NT / NF, g), sum[m][n][i], acc[m][n][i]);
     }
 }
 
-// Block b's place: outputs ct (units of a block's), rows rb.  The row blocks of the same weights come one after
-// another on one XCD, so they find them in its L2.
-__device__ __forceinline__ bool place(const Par &p, long b, int &ct, int &rb) {
-    const long per = 8L * p.row_blocks;
-    ct = (int)(b / per) * 8 + (int)(b & 7), rb = (int)((b / 8) % p.row_blocks);
+// Grid [8][row blocks][splits * slices]: block x takes outputs 8 z + x, rows y.  The row blocks of the same weights are
+// on one XCD (the first axis), one after another, so they find them in its L2.  False: a block of the tail, done.
+template <typename T>
+__device__ __forceinline__ bool place(const Par &p, int waves, int &ct, int &split, int &first, int &end) {
+    int z = blockIdx.z;
+    if (z >= p.slices * p.splits) {
+        tail_dots<T>(p, waves);
+        return false;
+    }
+    split = 0, first = 0, end = p.units;
+    if (p.splits > 1) {
+        split = z / p.slices, z -= split * p.slices;
+        first = split * p.share, end = min(first + p.share, p.units);
+    }
+    ct = z * 8 + blockIdx.x;
     return true;
 }
 
-// Some rows (a decode step's): a block of MT x 16 rows by NT x 16 outputs whose waves take the weight blocks
-// along the inputs in turn, rows from the caches.
-template <typename T, int PARTS, bool CPLX, int MT, int NT, int G>
-__global__ __launch_bounds__(512) void step_kernel(Par p, Rows r) {
-    constexpr int NF = columns<CPLX, NT>();
-    extern __shared__ floatx4 join[];
-    const int waves = blockDim.x >> 6, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long all = (long)p.col_blocks * p.row_blocks;
-    if (blockIdx.x >= all) {
-        tail_dots<T>(p, blockIdx.x - all, waves);
-        return;
+template <typename V> __device__ __forceinline__ V at(const void *base, unsigned bytes) {
+    return *reinterpret_cast<const V *>(static_cast<const char *>(base) + bytes);
+}
+
+// The rows' part of a weight block, in registers: bf16 planes, or fp32 rows cut into their parts where they are used.
+// `row`: what a lane adds to the first row's start, in bytes (below 2^32).
+template <typename XT, int PARTS, int MT> struct Part {
+    uintx4 v[MT][2][PARTS];
+    __device__ __forceinline__ void load(const XT *x, const unsigned (&row)[MT], long plane, int k, int kr) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int h = 0; h < PARTS; ++h) {
+                    // behind the last input: the codes there are zero, but what is read must be, too
+                    const bool in = k + 32 * ks < kr;
+                    const uintx4 a = at<uintx4>(x + h * plane, row[m] + (in ? k + 32 * ks : 0) * 2u);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[m][ks][h][j] = in ? a[j] : 0;
+                }
     }
-    int ct, rb;
-    place(p, blockIdx.x, ct, rb);
-    if (ct * NT >= p.tiles) return;
-    const int l16 = lane & 15, q = lane >> 4;
-    const long row0 = (long)rb * MT * 16;
-    const unsigned short *xr[MT];
+    __device__ __forceinline__ void get(int m, int ks, bf16x8 (&p)[PARTS]) const {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) xr[m] = r.x + min(row0 + m * 16 + l16, p.rows - 1) * r.ldx + 8 * q;
-    floatx4 acc[MT][NF];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < NF; ++n) acc[m][n] = floatx4{0, 0, 0, 0};
-    for (int c = wave; c < p.chunks; c += waves) {
-        Block<NT, G> b;
-        b.load(p, ct * NT, c, lane);
-        multiply<PARTS, CPLX, MT, NT, G>(b, acc, [&](int m, int ks, int h) {
-            return *reinterpret_cast<const bf16x8 *>(xr[m] + h * r.plane + c * TK + 32 * ks);
-        });
+        for (int h = 0; h < PARTS; ++h) p[h] = frag(v[m][ks][h]);
     }
-    // the waves' sums, 16 rows at a time
+};
+template <int MT> struct Part<float, 1, MT> {
+    floatx4 v[MT][2][2];
+    __device__ __forceinline__ void load(const float *x, const unsigned (&row)[MT], long, int k, int kr) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        if (m) __syncthreads();
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < NF; ++n) join[(wave * NF + n) * 64 + lane] = acc[m][n];
-        __syncthreads();
-        for (int slot = threadIdx.x; slot < NT * 64; slot += blockDim.x) {
-            const int t = slot >> 6, ln = slot & 63;
-            floatx4 v[NF / NT];
+            for (int ks = 0; ks < 2; ++ks) {
+                const bool in = k + 32 * ks < kr;
+                const unsigned from = row[m] + (in ? k + 32 * ks : 0) * 4u;
 #pragma unroll
-            for (int z = 0; z < NF / NT; ++z) {
-                v[z] = join[(t * (NF / NT) + z) * 64 + ln];
-                for (int o = 1; o < waves; ++o) v[z] += join[(o * NF + t * (NF / NT) + z) * 64 + ln];
+                for (int e = 0; e < 2; ++e) {
+                    const floatx4 a = at<floatx4>(x, from + 16 * e);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[m][ks][e][j] = in ? a[j] : 0.f;
+                }
             }
-            finish<T, CPLX>(p, row0 + m * 16 + 4 * (ln >> 4), (ct * NT + t) * 16 + (ln & 15), v[0], v[NF / NT - 1]);
+    }
+    __device__ __forceinline__ void get(int m, int ks, bf16x8 (&p)[3]) const {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = v[m][ks][j / 4][j % 4];
+        split(f, p);
+    }
+};
+
+// A few rows (a decode step's): a block of 16 rows by NT x 16 outputs whose waves take the weight blocks along the
+// inputs in turn, each wave's next AHEAD ones in flight while it multiplies; their sums joined through LDS in the
+// waves' order.  XT: bf16 planes, or float rows as they stand.
+template <typename T, typename XT, bool CPLX, int NT, int GU, int WAVES, int AHEAD>
+__global__ __launch_bounds__(64 * WAVES) void step_kernel(Par p, Rows r) {
+    constexpr int PARTS = parts<T>(), NF = columns<CPLX, NT>(), Z = NF / NT, XP = sizeof(XT) == 4 ? 1 : PARTS;
+    __shared__ floatx4 join[WAVES * NF * 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int ct, split, first, end;
+    if (!place<T>(p, WAVES, ct, split, first, end) || ct * NT >= p.tiles) return;
+    const int q = lane >> 4;
+    const long row0 = (long)blockIdx.y * 16;
+    const XT *x0 = reinterpret_cast<const XT *>(r.x) + row0 * r.ldx;
+    // rows behind the last read the last one, and are not written
+    const unsigned row[1] = {(unsigned)min(lane & 15, (int)min(p.rows - row0, 16L) - 1) * (unsigned)r.ldx * (unsigned)sizeof(XT)};
+    floatx4 acc[1][NF];
+#pragma unroll
+    for (int n = 0; n < NF; ++n) acc[0][n] = floatx4{0, 0, 0, 0};
+    const Tiles<NT, GU> tiles(p, ct * NT);
+    Block<NT, GU> b[AHEAD];
+    Part<XT, XP, 1> x[AHEAD];
+    auto fetch = [&](int i, int u) {  // (behind the last block: that again, not used)
+        u = min(u, p.units - 1);
+        b[i].load(p, tiles, u, lane);
+        x[i].load(x0, row, r.plane, u * TK + 8 * q, p.kr);
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) fetch(i, first + wave + i * WAVES);
+    for (int u = first + wave; u < end; u += AHEAD * WAVES) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (u + i * WAVES >= end) break;
+            bf16x8 part[PARTS];
+            multiply<PARTS, CPLX, 1, NT, GU>(b[i], acc, [&](int m, int ks, int h) {
+                if (h == 0) x[i].get(m, ks, part);
+                return part[h];
+            });
+            if (u + (i + AHEAD) * WAVES < end) fetch(i, u + (i + AHEAD) * WAVES);
         }
+    }
+#pragma unroll
+    for (int n = 0; n < NF; ++n) join[(wave * NF + n) * 64 + lane] = acc[0][n];
+    __syncthreads();
+    for (int slot = threadIdx.x; slot < NT * 64; slot += 64 * WAVES) {
+        const int ln = slot & 63, t = slot >> 6;
+        floatx4 v[Z];
+#pragma unroll
+        for (int z = 0; z < Z; ++z) {
+            const floatx4 *from = join + (t * Z + z) * 64 + ln;
+            v[z] = from[0];
+#pragma unroll
+            for (int o = 1; o < WAVES; ++o) v[z] += from[o * NF * 64];
+        }
+        deliver<T, CPLX>(p, split, ct * NT + t, blockIdx.y, ln, v[0], v[Z - 1]);
     }
 }
 
-// Many rows (a prompt's): WM x WN waves of MT x 16 rows by NT x 16 outputs; the rows of a weight block of 128
-// inputs through LDS in the MFMA's order (direct loads, two buffers), the weights through registers.
-template <typename T, int PARTS, bool CPLX, int WM, int WN, int MT, int NT, int G>
-__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Par p, Rows r) {
-    constexpr int NF = columns<CPLX, NT>(), WAVES = WM * WN, MB = WM * MT, PIECES = PARTS * MB * 4;
-    static_assert(PIECES % WAVES == 0, "the waves load alike");
-    __shared__ uintx4 stage[2 * PIECES * 64];   // [2][PARTS][MB][4][64]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wn = wave / WM;
-    const long all = (long)p.col_blocks * p.row_blocks;
-    if (blockIdx.x >= all) {
-        tail_dots<T>(p, blockIdx.x - all, WAVES);
-        return;
-    }
-    int ct, rb;
-    place(p, blockIdx.x, ct, rb);
-    if (ct * WN * NT >= p.tiles) return;
+// More rows: WN waves side by side of MT x 16 rows by NT x 16 outputs, WK times along the inputs; the rows of the
+// weight blocks at hand through LDS in the MFMA's order (direct loads, AHEAD buffers), the weights through
+// registers.  With WK > 1 (a decode step's rows, where there are few blocks) the sums are joined through LDS.
+template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD>
+__global__ __launch_bounds__(64 * WN * WK) void tile_kernel(Par p, Rows r) {
+    constexpr int PARTS = parts<T>(), NF = columns<CPLX, NT>(), Z = NF / NT, WAVES = WN * WK, PIECES = PARTS * MT * 2,
+                  EACH = (PIECES + WN - 1) / WN;
+    static_assert(PIECES % WN == 0 || WN % PIECES == 0, "the waves load alike");   // (with fewer pieces than waves, some twice)
+    constexpr int STAGE = AHEAD * WK * PIECES * 64, JOIN = WK > 1 ? WAVES * MT * NF * 64 : 0;
+    __shared__ uintx4 stage[STAGE > JOIN ? STAGE : JOIN];   // [AHEAD][WK][PARTS][MT][2][64]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wk = wave / WN;
+    int ct, split, first, end;
+    if (!place<T>(p, WAVES, ct, split, first, end) || ct * WN * NT >= p.tiles) return;
     const int l16 = lane & 15, q = lane >> 4, tile0 = (ct * WN + wn) * NT;
-    const long row0 = (long)rb * MB * 16;
-    auto fetch = [&](int c) {
-        uintx4 *to = stage + (c & 1) * PIECES * 64;
+    const long row0 = (long)blockIdx.y * MT * 16;
+    const int last = (int)min(p.rows - row0, (long)MT * 16) - 1;
+    const unsigned short *x0[EACH];   // a piece's place in the first row, and what a lane adds (bytes, below 2^32)
+    unsigned row[EACH];
 #pragma unroll
-        for (int i = 0; i < PIECES / WAVES; ++i) {
-            const int piece = i * WAVES + wave, ks = piece & 3, m = (piece >> 2) % MB, h = (piece >> 2) / MB;
-            const unsigned short *from = r.x + h * r.plane + min(row0 + m * 16 + l16, p.rows - 1) * r.ldx + c * TK + 32 * ks + 8 * q;
-            __builtin_amdgcn_global_load_lds(reinterpret_cast<const unsigned *>(from), reinterpret_cast<unsigned *>(to + piece * 64), 16, 0, 0);
-        }
+    for (int i = 0; i < EACH; ++i) {
+        const int piece = (i * WN + wn) % PIECES, ks = piece & 1, m = (piece >> 1) % MT, h = (piece >> 1) / MT;
+        x0[i] = r.x + row0 * r.ldx + h * r.plane + 32 * ks;
+        row[i] = ((unsigned)min(m * 16 + l16, last) * (unsigned)r.ldx + 8 * q) * 2;
+    }
+    const Tiles<NT, GU> tiles(p, tile0);
+    Block<NT, GU> b[AHEAD];
+    // Block u into buffer i (behind the last: that again, so that the loads in flight can be counted).
+    auto fetch = [&](int i, int u) {
+        u = min(u, p.units - 1);
+        uintx4 *to = stage + (i * WK + wk) * PIECES * 64;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j)
+            __builtin_amdgcn_global_load_lds(reinterpret_cast<const unsigned *>(reinterpret_cast<const char *>(x0[j] + (long)u * TK) + row[j]),
+                                             reinterpret_cast<unsigned *>(to + (j * WN + wn) % PIECES * 64), 16, 0, 0);
+        b[i].load(p, tiles, u, lane);
     };
     floatx4 acc[MT][NF];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NF; ++n) acc[m][n] = floatx4{0, 0, 0, 0};
-    Block<NT, G> b, next;
-    fetch(0);
-    b.load(p, tile0, 0, lane);
-    stage_barrier<0>();
-    for (int c = 0; c < p.chunks; ++c) {
-        if (c + 1 < p.chunks) {
-            fetch(c + 1);
-            next.load(p, tile0, c + 1, lane);
+#pragma unroll
+    for (int i = 0; i < AHEAD - 1; ++i) fetch(i, first + wk + i * WK);
+    const int rounds = (end - first + WK - 1) / WK;
+    for (int v = 0; v < rounds; v += AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (v + i >= rounds) break;
+            // round v + i has arrived, for every wave; the buffer of the one before is free
+            stage_barrier<(AHEAD - 2) * (EACH + 2 * NT)>();
+            const int u = first + wk + (v + i) * WK;
+            fetch((i + AHEAD - 1) % AHEAD, u + (AHEAD - 1) * WK);
+            if (WK > 1 && u >= end) continue;
+            const uintx4 *from = stage + (i * WK + wk) * PIECES * 64 + lane;
+            multiply<PARTS, CPLX, MT, NT, GU>(b[i], acc, [&](int m, int ks, int h) { return frag(from[((h * MT + m) * 2 + ks) * 64]); });
         }
-        const uintx4 *from = stage + (c & 1) * PIECES * 64;
-        multiply<PARTS, CPLX, MT, NT, G>(b, acc, [&](int m, int ks, int h) {
-            return frag(from[((h * MB + wm * MT + m) * 4 + ks) * 64 + lane]);
-        });
-        b = next;
-        stage_barrier<0>();
     }
+    if constexpr (WK == 1) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-            finish<T, CPLX>(p, row0 + (wm * MT + m) * 16 + 4 * q, (tile0 + t) * 16 + l16, acc[m][t * (NF / NT)], acc[m][t * (NF / NT) + NF / NT - 1]);
+            for (int t = 0; t < NT; ++t)
+                deliver<T, CPLX>(p, split, tile0 + t, (long)blockIdx.y * MT + m, lane, acc[m][t * Z], acc[m][t * Z + Z - 1]);
+    } else {
+        stage_barrier<0>();
+        floatx4 *join = reinterpret_cast<floatx4 *>(stage);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NF; ++n) join[(wave * MT * NF + m * NF + n) * 64 + lane] = acc[m][n];
+        __syncthreads();
+        for (int slot = threadIdx.x; slot < WN * MT * NT * 64; slot += 64 * WAVES) {
+            const int ln = slot & 63, t = (slot >> 6) % NT, m = (slot >> 6) / NT % MT, w = (slot >> 6) / (NT * MT);
+            floatx4 v[Z];
+#pragma unroll
+            for (int z = 0; z < Z; ++z) {
+                const floatx4 *from = join + (w * MT * NF + m * NF + t * Z + z) * 64 + ln;
+                v[z] = from[0];
+#pragma unroll
+                for (int o = 1; o < WK; ++o) v[z] += from[o * WN * MT * NF * 64];
+            }
+            deliver<T, CPLX>(p, split, (ct * WN + w) * NT + t, (long)blockIdx.y * MT + m, ln, v[0], v[Z - 1]);
+        }
+    }
 }
 
 // ---------------------------------------------------------------- launches --
 
-template <typename T, bool CPLX, int MT, int NT, int G>
-int launch_rows(Par p, int waves, hipStream_t stream) {
-    p.col_blocks = ((p.tiles + NT - 1) / NT + 7) / 8 * 8;
-    const long vrows = CPLX ? 2 * p.rows : p.rows;
-    p.row_blocks = (int)((vrows + MT * TR - 1) / (MT * TR));
-    if (waves > p.chunks) waves = p.chunks;
-    const long tail_blocks = p.tail_n ? (p.rows * p.tail_n + waves - 1) / waves : 0;
-    const long blocks = (long)p.col_blocks * p.row_blocks + tail_blocks;
-    rows_kernel<T, CPLX, MT, NT, G><<<dim3((unsigned)blocks), dim3(64 * waves), (size_t)waves * MT * NT * 1024, stream>>>(p);
+// The grid of blocks of `rows` rows by `tiles` weight tiles, with the tail's dots behind them.
+dim3 grid_of(Par &p, int rows, int tiles, int waves) {
+    const int row_blocks = (int)((p.rows + rows - 1) / rows);
+    p.slices = ((p.tiles + tiles - 1) / tiles + 7) / 8;
+    const long per = 8L * row_blocks * waves, dots = p.rows * ((p.tail_n + TAIL - 1) / TAIL);
+    return dim3(8, row_blocks, p.slices * p.splits + (int)((dots + per - 1) / per));
+}
+
+template <typename T, bool CPLX>
+int join_splits(const Par &p, hipStream_t stream) {
+    if (int e = launch_status("qpam_linear4")) return e;
+    if (p.splits == 1) return QPAM_OK;
+    const long units = p.tiles * ((p.rows + 15) / 16);
+    join_kernel<T, CPLX><<<dim3((unsigned)((units + 3) / 4)), dim3(256), 0, stream>>>(p);
     return launch_status("qpam_linear4");
 }
 
-template <typename T, bool CPLX, int MT, int NT, int G>
+template <typename T, typename XT, bool CPLX, int NT, int GU, int WAVES, int AHEAD>
 int launch_step(Par p, const Rows &r, hipStream_t stream) {
-    constexpr int PARTS = Eight<T>::PARTS, NF = columns<CPLX, NT>();
-    p.col_blocks = ((p.tiles + NT - 1) / NT + 7) / 8 * 8;
-    p.row_blocks = (int)((p.rows + MT * 16 - 1) / (MT * 16));
-    // as few rounds over the inputs as 8 waves need, by as few waves as make that many
-    const int rounds = (p.chunks + 7) / 8, waves = (p.chunks + rounds - 1) / rounds;
-    const long tail_blocks = p.tail_n ? (p.rows * p.tail_n + waves - 1) / waves : 0;
-    const long blocks = (long)p.col_blocks * p.row_blocks + tail_blocks;
-    step_kernel<T, PARTS, CPLX, MT, NT, G><<<dim3((unsigned)blocks), dim3(64 * waves), (size_t)waves * NF * 1024, stream>>>(p, r);
-    return launch_status("qpam_linear4");
+    const dim3 grid = grid_of(p, 16, NT, WAVES);
+    step_kernel<T, XT, CPLX, NT, GU, WAVES, AHEAD><<<grid, dim3(64 * WAVES), 0, stream>>>(p, r);
+    return join_splits<T, CPLX>(p, stream);
 }
 
-template <typename T, bool CPLX, int WM, int WN, int MT, int NT, int G>
+template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD>
 int launch_tile(Par p, const Rows &r, hipStream_t stream) {
-    constexpr int PARTS = Eight<T>::PARTS;
-    p.col_blocks = ((p.tiles + NT * WN - 1) / (NT * WN) + 7) / 8 * 8;
-    p.row_blocks = (int)((p.rows + WM * MT * 16 - 1) / (WM * MT * 16));
-    const long tail_blocks = p.tail_n ? (p.rows * p.tail_n + WM * WN - 1) / (WM * WN) : 0;
-    const long blocks = (long)p.col_blocks * p.row_blocks + tail_blocks;
-    tile_kernel<T, PARTS, CPLX, WM, WN, MT, NT, G><<<dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream>>>(p, r);
-    return launch_status("qpam_linear4");
+    const dim3 grid = grid_of(p, MT * 16, WN * NT, WN * WK);
+    tile_kernel<T, CPLX, WN, WK, MT, NT, GU, AHEAD><<<grid, dim3(64 * WN * WK), 0, stream>>>(p, r);
+    return join_splits<T, CPLX>(p, stream);
 }
 
-constexpr int few_rows(bool cplx) { return cplx ? 8 : 16; }
 int padded(int kr) { return (kr + TK - 1) / TK * TK; }
 
-// Rows that the kernels for more rows read as they stand.
+// Rows that the kernels read as they stand: aligned 16-byte pieces (of few rows any number of them, fp32 too), lanes'
+// offsets below 2^32.
 bool stand(const qpam_linear4_args *a, int kr) {
-    return a->dtype == QPAM_BF16 && kr % TK == 0 && (uintptr_t)a->x % 16 == 0 && a->ldx % 8 == 0;
+    const int elem = a->dtype == QPAM_BF16 ? 2 : 4;
+    if ((uintptr_t)a->x % 16 || (a->rows > 1 && (a->ldx * elem % 16 || a->ldx > (1 << 24))) || kr % 8) return false;
+    return a->rows <= 16 || (a->dtype == QPAM_BF16 && kr % TK == 0);
 }
 
-size_t lay_bytes(const qpam_linear4_args *a) {
-    const int kr = a->is_complex ? 2 * a->k : a->k;
-    if (a->rows <= few_rows(a->is_complex) || stand(a, kr)) return 0;
-    return (size_t)a->rows * padded(kr) * 2 * (a->dtype == QPAM_BF16 ? 1 : 3);
+// What a call runs: a shape of blocks, ranges along the inputs, and the workspace.
+struct Plan {
+    int shape, splits, share;
+    size_t lay, sums;
+};
+constexpr int STEP = 0;
+struct Shape { int wn, wk, mt; };
+constexpr Shape SHAPES[] = {{1, 8, 1}, {2, 4, 1}, {2, 4, 2}, {4, 2, 2}, {4, 2, 4}, {8, 1, 4}};
+constexpr int SHAPE_COUNT = sizeof(SHAPES) / sizeof(SHAPES[0]);
+
+Plan plan(const qpam_linear4_args *a) {
+    const int kr = a->is_complex ? 2 * a->k : a->k, units = padded(kr) / TK, tiles = (a->n + TR - 1) / TR;
+    Plan l{STEP, 1, units, 0, 0};
+    if (!stand(a, kr)) l.lay = ((size_t)a->rows * padded(kr) * 2 * (a->dtype == QPAM_BF16 ? 1 : 3) + 255) / 256 * 256;
+    auto blocks = [&](int i) {
+        const int nt = !a->is_complex && i == SHAPE_COUNT - 1 ? 2 : 1;
+        return (long)((tiles + SHAPES[i].wn * nt - 1) / (SHAPES[i].wn * nt)) * ((a->rows + 16 * SHAPES[i].mt - 1) / (16 * SHAPES[i].mt));
+    };
+    if (a->rows > 16)
+        for (l.shape = SHAPE_COUNT - 1; l.shape > 1 && blocks(l.shape) < 200; --l.shape) {}
+    return l;
 }
 
-template <typename T, bool CPLX, int G>
-int choose(const Par &p, const Rows &r, hipStream_t stream) {
-    if (p.rows <= few_rows(CPLX)) return launch_rows<T, CPLX, 1, 1, G>(p, 16, stream);
-    if (p.rows <= 16) return launch_step<T, CPLX, 1, 2, G>(p, r, stream);
-    if (p.rows <= 32) return launch_step<T, CPLX, 2, 2, G>(p, r, stream);
-    if (p.rows <= 400) return launch_step<T, CPLX, 4, 2, G>(p, r, stream);
-    constexpr int WM = sizeof(T) == 2 ? 2 : 1;
-    return launch_tile<T, CPLX, WM, 4 / WM, 4, CPLX ? 2 : 4, G>(p, r, stream);
+template <typename T, bool CPLX, int GU>
+int run(const Plan &l, const Par &p, const Rows &r, hipStream_t stream) {
+    typedef unsigned short B;
+    switch (l.shape) {
+    case STEP:
+        if constexpr (sizeof(T) == 4)
+            if (!l.lay) return launch_step<T, float, CPLX, 1, GU, 8, 3>(p, r, stream);
+        return launch_step<T, B, CPLX, 1, GU, 8, 3>(p, r, stream);
+    case 1: return launch_tile<T, CPLX, 2, 4, 1, 1, GU, 3>(p, r, stream);
+    case 2: return launch_tile<T, CPLX, 2, 4, 2, 1, GU, 3>(p, r, stream);
+    case 3: return launch_tile<T, CPLX, 4, 2, 2, 1, GU, 3>(p, r, stream);
+    case 4: return launch_tile<T, CPLX, 4, 2, 4, 1, GU, 3>(p, r, stream);
+    default: return launch_tile<T, CPLX, 8, 1, 4, CPLX ? 1 : 2, GU, 3>(p, r, stream);
+    }
 }
 
 template <typename T>
-int by_group(const Par &p, const Rows &r, int cplx, int group, hipStream_t stream) {
-    if (cplx) {
-        if (group == 32) return choose<T, true, 4>(p, r, stream);
-        if (group == 64) return choose<T, true, 2>(p, r, stream);
-        return choose<T, true, 1>(p, r, stream);
-    }
-    if (group == 32) return choose<T, false, 4>(p, r, stream);
-    if (group == 64) return choose<T, false, 2>(p, r, stream);
-    return choose<T, false, 1>(p, r, stream);
+int by_group(const Plan &l, const Par &p, const Rows &r, int cplx, int group, hipStream_t stream) {
+    if (cplx) return group == 32 ? run<T, true, 2>(l, p, r, stream) : run<T, true, 1>(l, p, r, stream);
+    return group == 32 ? run<T, false, 2>(l, p, r, stream) : run<T, false, 1>(l, p, r, stream);
 }
 
 }  // namespace w4
@@ -593,8 +610,9 @@ int by_group(const Par &p, const Rows &r, int cplx, int group, hipStream_t strea
 
 extern "C" size_t qpam_linear4_workspace_size(const qpam_linear4_args *a) {
     const int64_t k = a->is_complex ? 2 * (int64_t)a->k : a->k;
-    if (a->rows < 1 || a->rows > (1L << 40) || k < 1 || k > (1 << 25)) return 0;
-    return qpam::w4::lay_bytes(a);
+    if (a->rows < 1 || a->rows > (1L << 40) || k < 1 || k > (1 << 25) || a->n < 1 || a->n > (1 << 22)) return 0;
+    const qpam::w4::Plan l = qpam::w4::plan(a);
+    return l.lay + l.sums;
 }
 
 extern "C" int qpam_linear4(const qpam_linear4_args *a, void *stream) {
@@ -602,7 +620,7 @@ extern "C" int qpam_linear4(const qpam_linear4_args *a, void *stream) {
     QPAM_REQUIRE(a, "qpam_linear4: null arguments");
     QPAM_REQUIRE(a->dtype == QPAM_F32 || a->dtype == QPAM_BF16, "qpam_linear4: unknown dtype %d", a->dtype);
     QPAM_REQUIRE(a->rows >= 0 && a->rows <= (1L << 40), "qpam_linear4: %ld rows", (long)a->rows);
-    QPAM_REQUIRE(a->n >= 1 && a->n <= (1 << 24) && a->k >= 1 && a->k <= (1 << 24), "qpam_linear4: sizes n = %d, k = %d (1 to 2^24)",
+    QPAM_REQUIRE(a->n >= 1 && a->n <= (1 << 22) && a->k >= 1 && a->k <= (1 << 24), "qpam_linear4: sizes n = %d (1 to 2^22), k = %d (1 to 2^24)",
                  a->n, a->k);
     QPAM_REQUIRE(a->group == 32 || a->group == 64 || a->group == 128, "qpam_linear4: group %d (32, 64 or 128)", a->group);
     QPAM_REQUIRE(a->tail_n >= 0 && a->tail_n <= 4096, "qpam_linear4: tail of %d outputs", a->tail_n);
@@ -612,31 +630,31 @@ extern "C" int qpam_linear4(const qpam_linear4_args *a, void *stream) {
     const int kr = a->is_complex ? 2 * a->k : a->k, wide_y = (a->is_complex ? 2 : 1) * a->n + a->tail_n;
     const int elem = a->dtype == QPAM_BF16 ? 2 : 4;
     QPAM_REQUIRE(a->x && a->codes && a->scales && a->y && (!a->tail_n || a->tail), "qpam_linear4: null pointer");
-    QPAM_REQUIRE((uintptr_t)a->codes % 16 == 0 && (uintptr_t)a->scales % 8 == 0, "qpam_linear4: codes or scales not aligned");
+    QPAM_REQUIRE((uintptr_t)a->codes % 16 == 0 && (uintptr_t)a->scales % 4 == 0, "qpam_linear4: codes or scales not aligned");
     QPAM_REQUIRE((uintptr_t)a->x % elem == 0 && (uintptr_t)a->y % elem == 0 && (uintptr_t)a->tail % elem == 0 &&
                  (uintptr_t)a->bias % 4 == 0, "qpam_linear4: pointer not aligned to its type");
     QPAM_REQUIRE((a->ldx >= kr || a->rows == 1) && (a->ldy >= wide_y || a->rows == 1) && (!a->tail_n || a->ld_tail >= kr || a->tail_n == 1),
                  "qpam_linear4: row strides shorter than the rows");
     w4::Par p{};
     p.n = a->n, p.kr = kr;
-    p.chunks = (kr + w4::TK - 1) / w4::TK, p.tiles = (a->n + w4::TR - 1) / w4::TR;
+    p.units = (kr + w4::TK - 1) / w4::TK, p.scale_step = a->group == 128 ? 2 : 1, p.tiles = (a->n + w4::TR - 1) / w4::TR;
     p.ldx = a->ldx, p.ldy = a->ldy, p.ld_tail = a->ld_tail;
     p.codes = static_cast<const unsigned char *>(a->codes), p.scales = static_cast<const unsigned short *>(a->scales);
-    p.bias = a->bias, p.planes = a->planes, p.tail_n = a->tail_n, p.tail = a->tail;
-    p.vec = kr % 8 == 0 && (uintptr_t)a->x % 16 == 0 && a->ldx * elem % 16 == 0;
-    const size_t bytes = w4::lay_bytes(a);
-    if (bytes && (!a->workspace || a->workspace_bytes < bytes || (uintptr_t)a->workspace % 16))
-        return fail(QPAM_ERR_WORKSPACE, "qpam_linear4: workspace of %zu bytes (16-byte aligned) needed", bytes);
+    p.bias = a->bias, p.planes = a->planes, p.tail_n = a->tail_n, p.tail_k = kr, p.tail = a->tail;
+    const w4::Plan l = w4::plan(a);
+    if (l.lay + l.sums && (!a->workspace || a->workspace_bytes < l.lay + l.sums || (uintptr_t)a->workspace % 16))
+        return fail(QPAM_ERR_WORKSPACE, "qpam_linear4: workspace of %zu bytes (16-byte aligned) needed", l.lay + l.sums);
+    p.splits = l.splits, p.share = l.share;
+    p.sums = reinterpret_cast<floatx4 *>(static_cast<char *>(a->workspace) + l.lay);
     hipStream_t st = (hipStream_t)stream;
-    // a launch has fewer than 2^32 threads: rows in pieces
-    const long per_block = (long)(p.tiles + 8) * 1024;
-    const long step = std::max<long>(64, ((1L << 31) / per_block) * 8 / (1 + a->tail_n));
+    // a launch has fewer than 2^32 threads, a grid's second axis 2^16 blocks: rows in pieces
+    const long step = std::min<long>(1 << 19, std::max<long>(16, (1L << 31) / ((p.tiles + 8L) * 1024 / 16 + 64L * a->tail_n) / 16 * 16));
     for (long at = 0; at < a->rows; at += step) {
         p.rows = std::min<long>(step, a->rows - at);
         p.x = static_cast<const char *>(a->x) + at * a->ldx * elem;
         p.y = static_cast<char *>(a->y) + at * a->ldy * elem;
         w4::Rows r{static_cast<const unsigned short *>(p.x), a->ldx, 0};
-        if (bytes) {  // each piece in turn through the same memory
+        if (l.lay) {  // each piece in turn through the same memory
             const int kp = w4::padded(kr);
             unsigned short *ws = static_cast<unsigned short *>(a->workspace);
             const long blocks = std::min<long>((p.rows * (kp / 8) + 255) / 256, 1 << 20);
@@ -646,9 +664,10 @@ extern "C" int qpam_linear4(const qpam_linear4_args *a, void *stream) {
                 w4::lay_rows_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(static_cast<const float *>(p.x), a->ldx, p.rows, kr, kp, ws);
             if (const int e = launch_status("qpam_linear4")) return e;
             r = w4::Rows{ws, kp, p.rows * kp};
+            p.kr = kp;
         }
-        const int e = a->dtype == QPAM_BF16 ? w4::by_group<unsigned short>(p, r, a->is_complex, a->group, st)
-                                            : w4::by_group<float>(p, r, a->is_complex, a->group, st);
+        const int e = a->dtype == QPAM_BF16 ? w4::by_group<unsigned short>(l, p, r, a->is_complex, a->group, st)
+                                            : w4::by_group<float>(l, p, r, a->is_complex, a->group, st);
         if (e) return e;
     }
     return QPAM_OK;

@@ -22,7 +22,7 @@ __all__ = ["Weight4", "complex_linear4", "dequantize4", "linear4", "quantize4"]
 
 GROUPS = (32, 64, 128)
 MAGNITUDES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
-_ROWS, _COLS = 16, 128   # outputs and inputs of a block of the kernel's layout
+_ROWS, _COLS = 16, 64    # outputs and inputs of a block of the kernel's layout
 _CODE = {torch.float32: _lib.QPAM_F32, torch.bfloat16: _lib.QPAM_BF16}
 
 
@@ -90,6 +90,11 @@ def dequantize4(codes: Tensor, scales: Tensor, columns: int, group: int = 32) ->
     return values[idx.int()] * scales.float().repeat_interleave(group, 1)[:, :columns]
 
 
+def _scales_of(columns, group):
+    """Steps along a row that have scales of their own in the layout, and how many each."""
+    return -(-columns // max(group, _COLS)), max(1, _COLS // group)
+
+
 class Weight4:
     """A weight [out_features, in_features] of 4-bit codes and group scales (quantize4's),
     laid out once for the kernel on the codes' device.  With `complex` the columns are
@@ -99,18 +104,19 @@ class Weight4:
         columns = 2 * in_features if complex else in_features
         _check_codes(codes, scales, columns, group)
         n = codes.shape[0]
-        if n > 1 << 24 or in_features > 1 << 24:
-            raise ValueError(f"qpam linear4: weight [{n}, {in_features}] too large (2^24 each)")
+        if n > 1 << 22 or in_features > 1 << 24:
+            raise ValueError(f"qpam linear4: weight [{n}, {in_features}] too large (2^22, 2^24)")
         self.out_features, self.in_features, self.group, self.complex = n, int(in_features), int(group), bool(complex)
-        tiles, chunks, g = -(-n // _ROWS), -(-columns // _COLS), _COLS // group
+        tiles, blocks = -(-n // _ROWS), -(-columns // _COLS)
         pad = torch.nn.functional.pad
         if columns % 2:  # the half of a byte behind the last column
             codes = torch.cat([codes[:, :-1], codes[:, -1:] & 15], 1)
-        c = pad(codes, (0, chunks * _COLS // 2 - codes.shape[1], 0, tiles * _ROWS - n))
-        # [tile, output, chunk, step, quarter, byte] -> [tile, chunk, quarter, output, step, byte]
-        self.codes = c.view(tiles, _ROWS, chunks, 4, 4, 4).permute(0, 2, 4, 1, 3, 5).contiguous().view(-1)
-        s = pad(scales, (0, chunks * g - scales.shape[1], 0, tiles * _ROWS - n))
-        self.scales = s.view(tiles, _ROWS, chunks, g).permute(0, 2, 1, 3).contiguous().view(-1)
+        c = pad(codes, (0, blocks * _COLS // 2 - codes.shape[1], 0, tiles * _ROWS - n))
+        # [tile, output, block, step, quarter, byte] -> [tile, block, quarter, output, step, byte]
+        self.codes = c.view(tiles, _ROWS, blocks, 2, 4, 4).permute(0, 2, 4, 1, 3, 5).contiguous().view(-1)
+        per, g = _scales_of(columns, group)
+        s = pad(scales, (0, per * g - scales.shape[1], 0, tiles * _ROWS - n))
+        self.scales = s.view(tiles, _ROWS, per, g).permute(0, 2, 1, 3).contiguous().view(-1)
 
     @classmethod
     def quantize(cls, weight: Tensor, weight_imag: Optional[Tensor] = None, group: int = 32) -> "Weight4":
@@ -121,9 +127,10 @@ class Weight4:
     def dequantize(self) -> Tensor:
         """The fp32 values: [out, in], complex [out, in, 2]."""
         n, columns = self.out_features, self.in_features * (2 if self.complex else 1)
-        tiles, chunks, g = -(-n // _ROWS), -(-columns // _COLS), _COLS // self.group
-        c = self.codes.view(tiles, chunks, 4, _ROWS, 4, 4).permute(0, 3, 1, 4, 2, 5).reshape(tiles * _ROWS, -1)
-        s = self.scales.view(tiles, chunks, _ROWS, g).permute(0, 2, 1, 3).reshape(tiles * _ROWS, -1)
+        tiles, blocks = -(-n // _ROWS), -(-columns // _COLS)
+        per, g = _scales_of(columns, self.group)
+        c = self.codes.view(tiles, blocks, 4, _ROWS, 2, 4).permute(0, 3, 1, 4, 2, 5).reshape(tiles * _ROWS, -1)
+        s = self.scales.view(tiles, per, _ROWS, g).permute(0, 2, 1, 3).reshape(tiles * _ROWS, -1)
         w = dequantize4(c[:n, :-(-columns // 2)], s[:n, :-(-columns // self.group)], columns, self.group)
         return w.view(n, self.in_features, 2) if self.complex else w
 

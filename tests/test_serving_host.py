@@ -65,14 +65,19 @@ def test_layout_and_back(n, k, group):
         codes = torch.randint(0, 256, (n, -(-k * z // 2)), generator=g, dtype=torch.uint8)
         scales = torch.randn(n, -(-k * z // group), generator=g).to(torch.bfloat16)
         w = Weight4(codes, scales, k, group, complex=z == 2)
-        tiles, chunks = -(-n // 16), -(-k * z // 128)
-        assert w.codes.numel() == tiles * chunks * 1024 and w.scales.numel() == tiles * chunks * 16 * 128 // group
+        tiles, blocks = -(-n // 16), -(-k * z // 64)
+        assert w.codes.numel() == tiles * blocks * 512
+        assert w.scales.numel() == tiles * 16 * (-(-k * z // 128) if group == 128 else blocks * 64 // group)
         assert torch.equal(w.dequantize().reshape(n, -1), dequantize4(codes, scales, k * z, group))
-        # the place that the header names: output r, input 32 s + 8 q + 2 b of a block
+        # the places that the header names: output r, input 32 s + 8 q + 2 b of a block
         r, c = n - 1, k * z - 1
-        at = ((r // 16) * chunks + c // 128) * 1024 + 16 * (16 * (c % 32 // 8) + r % 16) + 4 * (c % 128 // 32) + c % 8 // 2
+        at = ((r // 16) * blocks + c // 64) * 512 + 8 * (16 * (c % 32 // 8) + r % 16) + 4 * (c % 64 // 32) + c % 8 // 2
         assert int(w.codes[at] >> 4 * (c % 2)) & 15 == int(codes[r, c // 2] >> 4 * (c % 2)) & 15
+        per, each = (-(-k * z // 128), 1) if group == 128 else (blocks, 64 // group)
+        at = (((r // 16) * per + c // (group * each)) * 16 + r % 16) * each + c // group % each
+        assert w.scales[at] == scales[r, c // group]
         if c % 2 == 0:
+            at = ((r // 16) * blocks + c // 64) * 512 + 8 * (16 * (c % 32 // 8) + r % 16) + 4 * (c % 64 // 32) + c % 8 // 2
             assert int(w.codes[at]) >> 4 == 0
 
 
