@@ -269,38 +269,45 @@ template <int NT, int GU> struct Block {
     }
 };
 
-// One weight block times the wave's rows: MFMAs into a group's sums, those times the scale into acc.
+// One weight block times the wave's rows: MFMAs into a group's sums of 16 rows, those times the scale into acc while
+// the next 16 rows' MFMAs run (two sets of sums instead of one for every row: 2000 x 768 -> 4608 complex 97 -> 67 us
+// with two weight tiles a wave, whose sums alone had filled the registers).
 // x(m, step, h) gives the operand of 16 rows.
 template <int PARTS, bool CPLX, int MT, int NT, int GU, typename X>
 __device__ __forceinline__ void multiply(const Block<NT, GU> &b, floatx4 (&acc)[MT][columns<CPLX, NT>()], X &&x) {
     constexpr int NF = columns<CPLX, NT>(), STEPS = 2 / GU;
+    floatx4 sum[2][NF];
+    bf16x8 f[STEPS][NF];
 #pragma unroll
-    for (int g = 0; g < GU; ++g) {
-        floatx4 sum[MT][NF];
+    for (int i = 0; i <= GU * MT; ++i) {
+        const int g = i / MT, m = i % MT;
+        if (i < GU * MT) {
+            if (m == 0) {
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-            const int ks = g * STEPS + st;
-            unsigned w[NT];
+                for (int st = 0; st < STEPS; ++st) {
+                    unsigned w[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) w[t] = b.w[t][ks];
-            bf16x8 f[NF];
-            operands<CPLX, NT>(w, f);
+                    for (int t = 0; t < NT; ++t) w[t] = b.w[t][g * STEPS + st];
+                    operands<CPLX, NT>(w, f[st]);
+                }
+            }
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int st = 0; st < STEPS; ++st)
 #pragma unroll
                 for (int h = 0; h < PARTS; ++h) {
-                    const bf16x8 xf = x(m, ks, h);
+                    const bf16x8 xf = x(m, g * STEPS + st, h);
 #pragma unroll
                     for (int n = 0; n < NF; ++n)
-                        sum[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, f[n], st || h ? sum[m][n] : floatx4{0, 0, 0, 0}, 0, 0, 0);
+                        sum[i & 1][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf, f[st][n], st || h ? sum[i & 1][n] : floatx4{0, 0, 0, 0}, 0, 0, 0);
                 }
         }
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
+        if (i) {
+            const int pg = (i - 1) / MT, pm = (i - 1) % MT;
 #pragma unroll
             for (int n = 0; n < NF; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[m][n][i] = fmaf(b.scale(n * NT / NF, g), sum[m][n][i], acc[m][n][i]);
+                for (int j = 0; j < 4; ++j) acc[pm][n][j] = fmaf(b.scale(n * NT / NF, pg), sum[(i - 1) & 1][n][j], acc[pm][n][j]);
+        }
     }
 }
 
@@ -434,11 +441,11 @@ __global__ __launch_bounds__(64 * WAVES) void step_kernel(Par p, Rows r) {
 // More rows: WN waves side by side of MT x 16 rows by NT x 16 outputs, WK times along the inputs; the rows of the
 // weight blocks at hand through LDS in the MFMA's order (direct loads, AHEAD buffers), the weights through
 // registers.  With WK > 1 (a decode step's rows, where there are few blocks) the sums are joined through LDS.
-template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD>
-__global__ __launch_bounds__(64 * WN * WK) void tile_kernel(Par p, Rows r) {
+template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD, int OCC>
+__global__ __launch_bounds__(64 * WN * WK, OCC) void tile_kernel(Par p, Rows r) {
     constexpr int PARTS = parts<T>(), NF = columns<CPLX, NT>(), Z = NF / NT, WAVES = WN * WK, PIECES = PARTS * MT * 2,
                   EACH = (PIECES + WN - 1) / WN;
-    static_assert(PIECES % WN == 0 || WN % PIECES == 0, "the waves load alike");   // (with fewer pieces than waves, some twice)
+    // (the waves load alike, so that the loads in flight can be counted: where PIECES is no multiple of WN some twice)
     constexpr int STAGE = AHEAD * WK * PIECES * 64, JOIN = WK > 1 ? WAVES * MT * NF * 64 : 0;
     __shared__ uintx4 stage[STAGE > JOIN ? STAGE : JOIN];   // [AHEAD][WK][PARTS][MT][2][64]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wk = wave / WN;
@@ -543,10 +550,10 @@ int launch_step(Par p, const Rows &r, hipStream_t stream) {
     return join_splits<T, CPLX>(p, stream);
 }
 
-template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD>
+template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD, int OCC = 1>
 int launch_tile(Par p, const Rows &r, hipStream_t stream) {
     const dim3 grid = grid_of(p, MT * 16, WN * NT, WN * WK);
-    tile_kernel<T, CPLX, WN, WK, MT, NT, GU, AHEAD><<<grid, dim3(64 * WN * WK), 0, stream>>>(p, r);
+    tile_kernel<T, CPLX, WN, WK, MT, NT, GU, AHEAD, OCC><<<grid, dim3(64 * WN * WK), 0, stream>>>(p, r);
     return join_splits<T, CPLX>(p, stream);
 }
 
@@ -560,42 +567,67 @@ bool stand(const qpam_linear4_args *a, int kr) {
     return a->rows <= 16 || (a->dtype == QPAM_BF16 && kr % TK == 0);
 }
 
-// What a call runs: a shape of blocks, ranges along the inputs, and the workspace.
+// What a call runs: a shape of blocks (run), ranges along the inputs, and the workspace.
 struct Plan {
     int shape, splits, share;
     size_t lay, sums;
 };
-constexpr int STEP = 0;
-struct Shape { int wn, wk, mt; };
-constexpr Shape SHAPES[] = {{1, 8, 1}, {2, 4, 1}, {2, 4, 2}, {4, 2, 2}, {4, 2, 4}, {8, 1, 4}};
-constexpr int SHAPE_COUNT = sizeof(SHAPES) / sizeof(SHAPES[0]);
 
+// The shape by the number of 16 x 16 pieces of the result: as long as the GPU's 256 CUs have no more than about one
+// block each, a block of fewer pieces with more waves along the inputs is done earlier; then larger ones, which
+// read less.  Measured (us, K = 1536 real inputs; complex, group 32 bf16 | group 64 fp32 with its layout):
+//   pieces   144: step 4.5 | 7.3, 2 x 1 pieces 5.2 | 7.9      288: 6.0 | 11.2, 2 x 1 5.3 | 8.0
+//   576: 2 x 1 7.3 | 12.6, 2 x 2 (fp32 4 x 1) 6.9 | 10.1      1728: 2 x 2 11.1, 4 x 2 9.0 | 14.5, 6 x 2 21.0
+//   9216: 4 x 2 26.3 | 60.7, 4 x 4 of 2 tiles 29 | 58.6, 4 x 2 of 2 tiles | 44.8
+//   36000: 4 x 2 (8 x 4 of one tile 72), 4 x 4 of 2 tiles 66 | 4 x 2 of 2 tiles 137
 Plan plan(const qpam_linear4_args *a) {
     const int kr = a->is_complex ? 2 * a->k : a->k, units = padded(kr) / TK, tiles = (a->n + TR - 1) / TR;
-    Plan l{STEP, 1, units, 0, 0};
-    if (!stand(a, kr)) l.lay = ((size_t)a->rows * padded(kr) * 2 * (a->dtype == QPAM_BF16 ? 1 : 3) + 255) / 256 * 256;
-    auto blocks = [&](int i) {
-        const int nt = !a->is_complex && i == SHAPE_COUNT - 1 ? 2 : 1;
-        return (long)((tiles + SHAPES[i].wn * nt - 1) / (SHAPES[i].wn * nt)) * ((a->rows + 16 * SHAPES[i].mt - 1) / (16 * SHAPES[i].mt));
-    };
-    if (a->rows > 16)
-        for (l.shape = SHAPE_COUNT - 1; l.shape > 1 && blocks(l.shape) < 200; --l.shape) {}
+    const bool f32 = a->dtype == QPAM_F32;
+    Plan l{0, 1, units, 0, 0};
+    if (!stand(a, kr)) l.lay = ((size_t)a->rows * padded(kr) * 2 * (f32 ? 3 : 1) + 255) / 256 * 256;
+    const long pieces = (a->rows + 15) / 16 * tiles;
+    if (a->rows <= 16 && tiles >= 1024) {
+        l.shape = 1;
+    } else if (a->rows > 16 && pieces > 256) {
+        l.shape = pieces <= 512 ? 2 : pieces <= 1024 ? 3 : pieces <= (f32 ? 2048 : a->is_complex ? 12288 : 4096) ? 4 : 5;
+        if (f32 && l.shape == 5 && pieces > 8192) l.shape = 6;
+    }
+    // few tiles of long fp32 rows: more blocks by ranges of the inputs, joined in a launch of their own (16 rows x 4608
+    // inputs, 48 tiles: 14.8 -> 9.2 us; bf16 7.5 -> 7.0, not worth the memory)
+    if (f32 && l.shape == 0 && pieces <= 64 && units >= 48) {
+        l.splits = 4, l.share = (units + 3) / 4;
+        l.sums = (size_t)l.splits * pieces * (a->is_complex ? 2048 : 1024);
+    }
     return l;
 }
 
 template <typename T, bool CPLX, int GU>
 int run(const Plan &l, const Par &p, const Rows &r, hipStream_t stream) {
     typedef unsigned short B;
+    constexpr bool F32 = sizeof(T) == 4;
     switch (l.shape) {
-    case STEP:
-        if constexpr (sizeof(T) == 4)
+    case 0:
+        if constexpr (F32)
             if (!l.lay) return launch_step<T, float, CPLX, 1, GU, 8, 3>(p, r, stream);
-        return launch_step<T, B, CPLX, 1, GU, 8, 3>(p, r, stream);
-    case 1: return launch_tile<T, CPLX, 2, 4, 1, 1, GU, 3>(p, r, stream);
-    case 2: return launch_tile<T, CPLX, 2, 4, 2, 1, GU, 3>(p, r, stream);
-    case 3: return launch_tile<T, CPLX, 4, 2, 2, 1, GU, 3>(p, r, stream);
-    case 4: return launch_tile<T, CPLX, 4, 2, 4, 1, GU, 3>(p, r, stream);
-    default: return launch_tile<T, CPLX, 8, 1, 4, CPLX ? 1 : 2, GU, 3>(p, r, stream);
+        return launch_step<T, B, CPLX, 1, GU, 8, F32 ? 2 : 3>(p, r, stream);
+    case 1:  // a table's many outputs: fewer reads of the rows (50261 x 1536 bf16, 16 rows: 24 us with one tile, 14.5 with four)
+        if constexpr (F32)
+            if (!l.lay) return launch_step<T, float, CPLX, CPLX ? 2 : 4, GU, 8, 1>(p, r, stream);
+        return launch_step<T, B, CPLX, CPLX ? 2 : 4, GU, 8, F32 ? 1 : 2>(p, r, stream);
+    case 2: return launch_tile<T, CPLX, 2, 4, 1, 1, GU, F32 ? 2 : 3>(p, r, stream);
+    case 3:
+        if constexpr (F32) return launch_tile<T, CPLX, 4, 2, 1, 1, GU, 2>(p, r, stream);
+        else return launch_tile<T, CPLX, 2, 4, 2, 1, GU, 3>(p, r, stream);
+    case 4: return launch_tile<T, CPLX, 4, 2, 2, 1, GU, F32 ? 2 : 3>(p, r, stream);
+    default:
+        if constexpr (F32) {
+            if (l.shape == 5) return launch_tile<T, CPLX, 6, 1, 2, 1, GU, 2>(p, r, stream);
+            return launch_tile<T, CPLX, 4, 1, 2, CPLX ? 2 : 4, GU, 2, 3>(p, r, stream);
+        } else if constexpr (CPLX) {
+            return launch_tile<T, CPLX, 4, 1, 4, 2, GU, 3, 3>(p, r, stream);
+        } else {
+            return launch_tile<T, CPLX, 8, 1, 4, 2, GU, 3>(p, r, stream);
+        }
     }
 }
 
