@@ -46,7 +46,8 @@ __device__ __forceinline__ bool move_of(const Par &p, const Lists &h, int i, int
 template <typename V, bool HOST, int LANES, int E, int THREADS>
 __global__ __launch_bounds__(THREADS) void copy_kernel(Par p, Lists h) {
     constexpr int AT_ONCE = THREADS / LANES;
-    const int first = threadIdx.x / LANES;
+    // (a wave's own moves, where it has them: their slots are the same for its lanes)
+    const int first = LANES >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / LANES) : threadIdx.x / LANES;
     if (blockIdx.x == p.columns) {  // the positions, one block's
         int v[MOST / THREADS];
 #pragma unroll
@@ -83,7 +84,7 @@ __global__ __launch_bounds__(THREADS) void copy_kernel(Par p, Lists h) {
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < E; ++e)
-        if (to[e] >= 0) *reinterpret_cast<V *>(p.state + to[e] * p.slot_bytes + at) = v[e];
+        if (to[e] >= 0) __builtin_nontemporal_store(v[e], reinterpret_cast<V *>(p.state + to[e] * p.slot_bytes + at));
 }
 
 template <typename V, bool HOST, int LANES, int E, int THREADS>
@@ -98,9 +99,12 @@ int launch(Par p, const Lists &h, hipStream_t stream) {
 
 template <typename V, bool HOST>
 int choose(const Par &p, const Lists &h, hipStream_t stream) {
-    if (p.count <= 16) return launch<V, HOST, 64, 4, 256>(p, h, stream);
-    if (p.count <= 64) return launch<V, HOST, 64, 16, 256>(p, h, stream);
-    if (p.count <= 256) return launch<V, HOST, 16, 16, 256>(p, h, stream);
+    // 1 KB of a page side by side as long as the block has room for the moves: shorter pieces cost bandwidth (128 moves
+    // of 6.3 MB pages: 235 us, with 512 bytes 256, with 256 bytes 274), fewer waves a block, too (64 moves of 18.9 MB:
+    // 16 waves 327, 8 waves 338, 4 waves 356)
+    if (p.count <= 32) return launch<V, HOST, 64, 8, 256>(p, h, stream);
+    if (p.count <= 128) return launch<V, HOST, 64, 8, 1024>(p, h, stream);
+    if (p.count <= 256) return launch<V, HOST, 64, 16, 1024>(p, h, stream);
     if (p.count <= 1024) return launch<V, HOST, 16, 16, 1024>(p, h, stream);
     return launch<V, HOST, 4, 16, 1024>(p, h, stream);
 }

@@ -331,11 +331,13 @@ def copy_slots(state, src, dst, pos=None):
     pos    optional int32 [S], moved and cleared with the pages
     Up to 4096 moves; host lists of more in several launches where no dst is also a src."""
     _check_cuda(state, pos)
-    n_slots = state.shape[0] if state.dim() else 0
-    if state.dtype != torch.float32 or state.dim() < 2 or not state.numel() or not state[0].is_contiguous() \
-            or (n_slots > 1 and state.stride(0) < state[0].numel()):
+    shape, stride = state.shape, state.stride()
+    n_slots = shape[0] if shape else 0
+    page = state.numel() // n_slots if n_slots else 0
+    if state.dtype != torch.float32 or len(shape) < 2 or not page \
+            or not (state.is_contiguous() or (state[0].is_contiguous() and (n_slots == 1 or stride[0] >= page))):
         raise ValueError(f"qpam copy_slots: state must be fp32 [S, ...] with contiguous pages, got {state.dtype} "
-                         f"{tuple(state.shape)} of strides {state.stride()}")
+                         f"{tuple(shape)} of strides {stride}")
     if pos is not None and (pos.dtype != torch.int32 or tuple(pos.shape) != (n_slots,) or not pos.is_contiguous()
                             or pos.device != state.device):
         raise ValueError(f"qpam copy_slots: pos must be contiguous int32 [{n_slots}] on {state.device}")
@@ -365,7 +367,7 @@ def copy_slots(state, src, dst, pos=None):
         pieces = [(src[i:i + size], dst[i:i + size]) for i in range(0, count, size)]
     a = _lib.SlotsArgs()
     a.state, a.n_slots = state.data_ptr(), n_slots
-    a.slot_bytes, a.page_bytes = 4 * max(state.stride(0), state[0].numel()), 4 * state[0].numel()
+    a.slot_bytes, a.page_bytes = 4 * max(stride[0], page), 4 * page
     a.pos = None if pos is None else pos.data_ptr()
     with _lib.device(state.device):
         for s, d in pieces:

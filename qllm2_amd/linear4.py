@@ -10,7 +10,6 @@ neighbouring codes of an output's row share a bf16 scale.  The products are exac
 summed in fp32; nothing but the result is rounded to the rows' dtype.
 """
 
-import ctypes
 from typing import Optional
 
 import torch
@@ -138,13 +137,15 @@ class Weight4:
 def _check_rows(x, codes, scales, n, k, is_complex, bias, planes, tail):
     if not (x.is_cuda and codes.is_cuda):
         raise ValueError("qpam linear4: tensors must be on the GPU (no CPU path in this library)")
-    if any(t is not None and t.device != x.device for t in (codes, scales, bias, tail)):
+    dev = x.device
+    if codes.device != dev or scales.device != dev or (bias is not None and bias.device != dev) \
+            or (tail is not None and tail.device != dev):
         raise ValueError("qpam linear4: rows, weight, bias and tail must be on one device")
     if x.dtype not in _CODE:
         raise ValueError(f"qpam linear4: rows must be float32 or bfloat16, got {x.dtype}")
-    last = (k, 2) if is_complex else (k,)
-    if tuple(x.shape[-len(last):]) != last or x.dim() < len(last):
-        raise ValueError(f"qpam linear4: rows of {list(last)} expected, got {tuple(x.shape)}")
+    shape = x.shape
+    if not (len(shape) > 1 and shape[-1] == 2 and shape[-2] == k if is_complex else len(shape) and shape[-1] == k):
+        raise ValueError(f"qpam linear4: rows of {[k, 2] if is_complex else [k]} expected, got {tuple(shape)}")
     if bias is not None and tuple(bias.shape) != ((n, 2) if is_complex else (n,)):
         raise ValueError(f"qpam linear4: bias must be {[n, 2] if is_complex else [n]}, got {tuple(bias.shape)}")
     if tail is not None and (not planes or tail.dim() != 2 or tail.shape[1] != 2 * k or tail.dtype != x.dtype
@@ -153,10 +154,12 @@ def _check_rows(x, codes, scales, n, k, is_complex, bias, planes, tail):
                          f"{tuple(tail.shape)}")
 
 
-def _rows(x, last):
-    """x as [rows, columns] with unit column stride, and its row stride; a copy where its strides do not give that."""
-    x = x.flatten(-2) if last == 2 and x.stride(-1) == 1 and x.stride(-2) == 2 else x.contiguous().flatten(-2) if last == 2 else x
-    columns = x.shape[-1]
+def _rows(x, columns, is_complex):
+    """x as rows of unit column stride that do not overlap, and their stride; a copy where its strides do not give that."""
+    if x.is_contiguous():
+        return x, columns
+    if is_complex:
+        x = x.flatten(-2) if x.stride(-1) == 1 and x.stride(-2) == 2 else x.contiguous().flatten(-2)
     x = x.reshape(-1, columns)
     if (columns > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < columns):
         x = x.contiguous()
@@ -168,26 +171,27 @@ def _product(x: Tensor, codes: Tensor, scales: Tensor, n: int, k: int, group: in
     """[*, n] (complex [*, n, 2]; with planes [*, 2 n + tail rows]) in x's dtype."""
     _check_rows(x, codes, scales, n, k, is_complex, bias, planes, tail)
     z = 2 if is_complex else 1
-    lead = x.shape[:-z]
     extra = 0 if tail is None else tail.shape[0]
-    out = torch.empty(*lead, *((n, 2) if is_complex and not planes else (z * n + extra,)), device=x.device, dtype=x.dtype)
-    if not out.numel():
+    wide = z * n + extra
+    out = torch.empty((*x.shape[:-z], n, 2) if is_complex and not planes else (*x.shape[:-z], wide), device=x.device, dtype=x.dtype)
+    count = out.numel() // wide
+    if not count:
         return out
-    rows, ldx = _rows(x, z)
+    rows, ldx = _rows(x, z * k, is_complex)
     if bias is not None:
         bias = bias.detach().float().contiguous()
     if tail is not None and (tail.stride(1) != 1 or tail.stride(0) < 2 * k):
         tail = tail.contiguous()
-    a = _lib.Linear4Args(rows.shape[0], n, k, group, is_complex, _CODE[x.dtype], planes, rows.data_ptr(), ldx, codes.data_ptr(),
-                         scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), z * n + extra, extra,
+    a = _lib.Linear4Args(count, n, k, group, is_complex, _CODE[x.dtype], planes, rows.data_ptr(), ldx, codes.data_ptr(),
+                         scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), wide, extra,
                          None if tail is None else tail.data_ptr(), 0 if tail is None else tail.stride(0))
-    L = _lib.lib()
-    nbytes = L.qpam_linear4_workspace_size(ctypes.byref(a))
+    L, dev = _lib.lib(), x.device
+    nbytes = L.qpam_linear4_workspace_size(a)
     if nbytes:
-        ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    with _lib.device(x.device):
-        _lib.check(L.qpam_linear4(ctypes.byref(a), _lib.stream_ptr(x.device)), "qpam_linear4")
+    with _lib.device(dev):
+        _lib.check(L.qpam_linear4(a, _lib.stream_ptr(dev)), "qpam_linear4")
     return out
 
 
