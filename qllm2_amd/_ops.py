@@ -26,7 +26,7 @@ import threading
 import torch
 
 _LIB = torch.library.Library("qpam", "FRAGMENT")
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_USUAL = {torch.Tensor, torch.nn.Parameter, type(None), bool, int, float}
 _CALL = threading.local()  # the dispatch keys of the call that is entering its autograd function
 
 
@@ -56,7 +56,10 @@ def _nothing_listens(args):
         return False
     if torch.autograd.forward_ad._current_level >= 0:
         return False
-    return all(type(a) in _PLAIN or not isinstance(a, torch.Tensor) for a in args)
+    for a in args:  # (most arguments by a look at their type alone: a third of this check's time)
+        if type(a) not in _USUAL and isinstance(a, torch.Tensor):
+            return False
+    return True
 
 
 class Op:

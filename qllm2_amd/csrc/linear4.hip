@@ -586,8 +586,10 @@ Plan plan(const qpam_linear4_args *a) {
     Plan l{0, 1, units, 0, 0};
     if (!stand(a, kr)) l.lay = ((size_t)a->rows * padded(kr) * 2 * (f32 ? 3 : 1) + 255) / 256 * 256;
     const long pieces = (a->rows + 15) / 16 * tiles;
-    if (a->rows <= 16 && tiles >= 1024) {
-        l.shape = 1;
+    // of few rows a block takes 16, 32 or 64 outputs: up to 256 blocks each has a CU, and fewer blocks read the rows less
+    // often (fp32, 288 tiles: 16 outputs 8.0 us, 32 6.0; 576: 32 outputs 10.3, 64 7.9; bf16, 576 tiles and 16 rows: 7.7, 6.7)
+    if (a->rows <= 16 && tiles > 256) {
+        l.shape = tiles > (f32 ? 512 : 1024) ? 7 : 1;
     } else if (a->rows > 16 && pieces > 256) {
         l.shape = pieces <= 512 ? 2 : pieces <= 1024 ? 3 : pieces <= (f32 ? 2048 : a->is_complex ? 12288 : 4096) ? 4 : 5;
         if (f32 && l.shape == 5 && pieces > 8192) l.shape = 6;
@@ -608,12 +610,16 @@ int run(const Plan &l, const Par &p, const Rows &r, hipStream_t stream) {
     switch (l.shape) {
     case 0:
         if constexpr (F32)
-            if (!l.lay) return launch_step<T, float, CPLX, 1, GU, 8, 3>(p, r, stream);
+            if (!l.lay) return launch_step<T, float, CPLX, 1, GU, 16, 1>(p, r, stream);
         return launch_step<T, B, CPLX, 1, GU, 8, F32 ? 2 : 3>(p, r, stream);
-    case 1:  // a table's many outputs: fewer reads of the rows (50261 x 1536 bf16, 16 rows: 24 us with one tile, 14.5 with four)
+    case 1:
         if constexpr (F32)
-            if (!l.lay) return launch_step<T, float, CPLX, CPLX ? 2 : 4, GU, 8, 1>(p, r, stream);
-        return launch_step<T, B, CPLX, CPLX ? 2 : 4, GU, 8, F32 ? 1 : 2>(p, r, stream);
+            if (!l.lay) return launch_step<T, float, CPLX, 2, GU, 16, 1>(p, r, stream);
+        return launch_step<T, B, CPLX, 2, GU, 8, F32 ? 1 : 2>(p, r, stream);
+    case 7:
+        if constexpr (F32)
+            if (!l.lay) return launch_step<T, float, CPLX, 4, GU, 8, 1>(p, r, stream);
+        return launch_step<T, B, CPLX, 4, GU, 8, F32 ? 1 : 2>(p, r, stream);
     case 2: return launch_tile<T, CPLX, 2, 4, 1, 1, GU, F32 ? 2 : 3>(p, r, stream);
     case 3:
         if constexpr (F32) return launch_tile<T, CPLX, 4, 2, 1, 1, GU, 2>(p, r, stream);

@@ -178,7 +178,7 @@ def _product(x: Tensor, codes: Tensor, scales: Tensor, n: int, k: int, group: in
     if not count:
         return out
     rows, ldx = _rows(x, z * k, is_complex)
-    if bias is not None:
+    if bias is not None and not (bias.dtype == torch.float32 and bias.is_contiguous()):
         bias = bias.detach().float().contiguous()
     if tail is not None and (tail.stride(1) != 1 or tail.stride(0) < 2 * k):
         tail = tail.contiguous()

@@ -95,6 +95,26 @@ def test_complex_products(gpu_lib, n, K, N, group, dtype):
     _check(complex_linear4(x, w, planes=True, tail=tail), x, w, tail=tail, planes=True)
 
 
+SHAPES = [  # sizes on either side of where the blocks' shape changes, few inputs; long rows of few outputs
+    (16, 64, 4100), (16, 72, 8300), (3, 100, 16500), (20, 130, 1500), (40, 96, 2000), (100, 96, 1700), (200, 130, 2000),
+    (300, 64, 3300), (600, 96, 4000), (1000, 72, 4000), (10, 3100, 40), (16, 6200, 1000), (60, 3100, 17),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,K,N", SHAPES)
+@pytest.mark.parametrize("group", [32, 128])
+def test_every_shape_of_blocks(gpu_lib, n, K, N, group, dtype):
+    w = Weight4(*_codes(N, K, group, 50), K, group)
+    x, b = _rows((n, K), dtype, 51), _rows((N,), F32, 52)
+    _check(linear4(x, w, b), x, w, b)
+    K = K // 2
+    w = Weight4(*_codes(N, 2 * K, group, 53), K, group, complex=True)
+    x, tail = _rows((n, K, 2), dtype, 54), _rows((3, 2 * K), dtype, 55)
+    _check(complex_linear4(x, w), x, w)
+    _check(complex_linear4(x, w, planes=True, tail=tail), x, w, tail=tail, planes=True)
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_every_weight_in_its_place(gpu_lib, group):
     """Unit rows give the weights back bit for bit: the layout, the codes, their scales."""
