@@ -25,7 +25,8 @@ struct Par {
     int n_slots, count;
     const int *src, *dst;
     int *pos;
-    long columns;                 // blocks along a page
+    long start;                   // where in a page this launch begins
+    unsigned columns;             // blocks along the page
 };
 struct Lists {
     int src[HOST_MOVES], dst[HOST_MOVES];
@@ -66,7 +67,7 @@ __global__ __launch_bounds__(THREADS) void copy_kernel(Par p, Lists h) {
         }
         return;
     }
-    const long at = ((long)blockIdx.x * LANES + threadIdx.x % LANES) * (long)sizeof(V);
+    const long at = p.start + ((long)blockIdx.x * LANES + threadIdx.x % LANES) * (long)sizeof(V);
     const bool in = at < p.page_bytes;
     V v[E];
     int to[E];
@@ -90,11 +91,17 @@ __global__ __launch_bounds__(THREADS) void copy_kernel(Par p, Lists h) {
 template <typename V, bool HOST, int LANES, int E, int THREADS>
 int launch(Par p, const Lists &h, hipStream_t stream) {
     static_assert(THREADS / LANES * E <= MOST, "more moves than a call has");
-    const long per = LANES * (long)sizeof(V);
-    p.columns = (p.page_bytes + per - 1) / per;
-    QPAM_REQUIRE(p.columns < (1L << 32) / THREADS - 1, "qpam_copy_slots: page of %ld bytes", p.page_bytes);
-    copy_kernel<V, HOST, LANES, E, THREADS><<<dim3((unsigned)(p.columns + (p.pos ? 1 : 0))), dim3(THREADS), 0, stream>>>(p, h);
-    return launch_status("qpam_copy_slots");
+    // a launch has fewer than 2^32 threads: long pages in pieces, the positions with the last
+    const long per = LANES * (long)sizeof(V), most = (1L << 31) / THREADS;
+    int *const pos = p.pos;
+    for (p.start = 0; p.start < p.page_bytes; p.start += most * per) {
+        const long columns = (p.page_bytes - p.start + per - 1) / per;
+        p.columns = (unsigned)std::min(columns, most);
+        p.pos = columns <= most ? pos : nullptr;
+        copy_kernel<V, HOST, LANES, E, THREADS><<<dim3(p.columns + (p.pos ? 1 : 0)), dim3(THREADS), 0, stream>>>(p, h);
+        if (const int e = launch_status("qpam_copy_slots")) return e;
+    }
+    return QPAM_OK;
 }
 
 template <typename V, bool HOST>

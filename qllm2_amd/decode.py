@@ -314,6 +314,8 @@ def _list(v, name):
     if torch.is_tensor(v) and v.is_cuda:
         if v.dim() != 1 or v.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"qpam copy_slots: {name} must be one list of int32 or int64, got {v.dtype} {tuple(v.shape)}")
+        if v.dtype == torch.int64:  # (what 32 bits would wrap stays outside any pool)
+            v = v.clamp(-2, 2 ** 31 - 1)
         return None, v.to(torch.int32).contiguous()
     return [int(i) for i in (v.tolist() if torch.is_tensor(v) else v)], None
 

@@ -191,7 +191,9 @@ def _product(x: Tensor, codes: Tensor, scales: Tensor, n: int, k: int, group: in
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
     with _lib.device(dev):
-        _lib.check(L.qpam_linear4(a, _lib.stream_ptr(dev)), "qpam_linear4")
+        status = L.qpam_linear4(a, _lib.stream_ptr(dev))
+    if status:
+        _lib.check(status, "qpam_linear4")
     return out
 
 
@@ -205,8 +207,9 @@ def _(x, codes, scales, n, k, group, is_complex, bias, planes, tail):
     return x.new_empty(*x.shape[:-z], *((n, 2) if is_complex and not planes else (z * n + extra,)))
 
 
-def _refuse_gradients(*ts):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+def _refuse_gradients(x, bias, tail):
+    if (x.requires_grad or (bias is not None and bias.requires_grad) or (tail is not None and tail.requires_grad)) \
+            and torch.is_grad_enabled():
         raise ValueError("qpam linear4: products with 4-bit weights have no gradient (call under torch.no_grad())")
 
 
@@ -215,7 +218,7 @@ def linear4(x: Tensor, weight: Weight4, bias: Optional[Tensor] = None) -> Tensor
     strides; fp32 sums, one rounding).  bias [out].  No gradient."""
     if weight.complex:
         raise ValueError("qpam linear4: a complex weight (complex_linear4)")
-    _refuse_gradients(x, bias)
+    _refuse_gradients(x, bias, None)
     return linear4_op(x, weight.codes, weight.scales, weight.out_features, weight.in_features, weight.group, False, bias, False,
                       None)
 

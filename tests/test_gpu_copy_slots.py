@@ -102,6 +102,16 @@ def test_device_entries_outside_the_pool_do_nothing(gpu_lib):
     assert torch.equal(state, want) and torch.equal(pos, want_pos)
 
 
+def test_device_entries_of_64_bits_outside_the_pool(gpu_lib):
+    """Ids that 32 bits would wrap into the pool."""
+    state, pos = _pool(10, (500,), 5)
+    want = _want(state, [1], [2])
+    src = torch.tensor([1, 2 ** 32, -2 ** 32 + 4, -2 ** 32 - 1, 3, 4], device="cuda")
+    dst = torch.tensor([2, 0, 5, 6, 2 ** 32 + 7, -2 ** 32 + 8], device="cuda")
+    copy_slots(state, src, dst, pos=pos)
+    assert torch.equal(state, want)
+
+
 def test_offsets_past_32_bits(gpu_lib):
     state = torch.zeros(700, 1 << 22, device="cuda")   # 11.7 GB: slots from 512 on start past 2^31 elements
     state[690].normal_()
@@ -120,6 +130,19 @@ def test_large_pages(gpu_lib):
     copy_slots(state, [0, 1], [1, 0])
     assert not state[0].any() and torch.equal(state[1, -50:], torch.full((50,), 3.0, device="cuda")) and float(state[1, 0]) == 2.0
     assert float(state[1].sum()) == 250.0 and not state[2].any()
+
+
+def test_long_pages_of_many_moves(gpu_lib):
+    """A page of more pieces than a launch has threads for, 1100 moves (two of them real)."""
+    state = torch.zeros(4, 40 << 20, device="cuda")   # 160 MB: 2.6 million 64-byte pieces, 1024 threads each
+    state[1, -3:] = 5.0
+    state[1, 0] = 7.0
+    pos = torch.arange(4, device="cuda", dtype=torch.int32)
+    src, dst = torch.full((1100,), 99, device="cuda", dtype=torch.int32), torch.full((1100,), 99, device="cuda", dtype=torch.int32)
+    src[3], dst[3], src[1090], dst[1090] = 1, 3, 0, 1
+    copy_slots(state, src, dst, pos=pos)
+    assert not state[:3].any() and float(state[3].sum()) == 22.0 and float(state[3, 0]) == 7.0 and float(state[3, -1]) == 5.0
+    assert pos.tolist() == [0, 0, 2, 1]
 
 
 def test_streams_and_graphs(gpu_lib):
