@@ -38,6 +38,7 @@ struct Par {
     void *y; long ldy;
     int planes;
     int slices;                // grid slices of 8 blocks along the outputs; behind them (times splits) those of the tail
+    int whole;                 // of the slices, those of the tile kernel's whole blocks; behind them blocks of half as many outputs
     int splits, share;         // ranges of `share` weight blocks along the inputs whose sums are joined by join_kernel
     floatx4 *sums;
     int tail_n, tail_k;        // of the caller's rows x
@@ -441,17 +442,15 @@ __global__ __launch_bounds__(64 * WAVES) void step_kernel(Par p, Rows r) {
 // More rows: WN waves side by side of MT x 16 rows by NT x 16 outputs, WK times along the inputs; the rows of the
 // weight blocks at hand through LDS in the MFMA's order (direct loads, AHEAD buffers), the weights through
 // registers.  With WK > 1 (a decode step's rows, where there are few blocks) the sums are joined through LDS.
-template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD, int OCC>
-__global__ __launch_bounds__(64 * WN * WK, OCC) void tile_kernel(Par p, Rows r) {
+// `tile`: the block's first weight tile.
+template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD>
+__device__ __forceinline__ void tile_block(const Par &p, const Rows &r, uintx4 *stage, int tile) {
     constexpr int PARTS = parts<T>(), NF = columns<CPLX, NT>(), Z = NF / NT, WAVES = WN * WK, PIECES = PARTS * MT * 2,
                   EACH = (PIECES + WN - 1) / WN;
     // (the waves load alike, so that the loads in flight can be counted: where PIECES is no multiple of WN some twice)
-    constexpr int STAGE = AHEAD * WK * PIECES * 64, JOIN = WK > 1 ? WAVES * MT * NF * 64 : 0;
-    __shared__ uintx4 stage[STAGE > JOIN ? STAGE : JOIN];   // [AHEAD][WK][PARTS][MT][2][64]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wk = wave / WN;
-    int ct, split, first, end;
-    if (!place<T>(p, WAVES, ct, split, first, end) || ct * WN * NT >= p.tiles) return;
-    const int l16 = lane & 15, q = lane >> 4, tile0 = (ct * WN + wn) * NT;
+    if (tile >= p.tiles) return;
+    const int l16 = lane & 15, q = lane >> 4, tile0 = tile + wn * NT;
     const long row0 = (long)blockIdx.y * MT * 16;
     const int last = (int)min(p.rows - row0, (long)MT * 16) - 1;
     const unsigned short *x0[EACH];   // a piece's place in the first row, and what a lane adds (bytes, below 2^32)
@@ -480,17 +479,17 @@ __global__ __launch_bounds__(64 * WN * WK, OCC) void tile_kernel(Par p, Rows r) 
 #pragma unroll
         for (int n = 0; n < NF; ++n) acc[m][n] = floatx4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < AHEAD - 1; ++i) fetch(i, first + wk + i * WK);
-    const int rounds = (end - first + WK - 1) / WK;
+    for (int i = 0; i < AHEAD - 1; ++i) fetch(i, wk + i * WK);
+    const int rounds = (p.units + WK - 1) / WK;
     for (int v = 0; v < rounds; v += AHEAD) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             if (v + i >= rounds) break;
             // round v + i has arrived, for every wave; the buffer of the one before is free
             stage_barrier<(AHEAD - 2) * (EACH + 2 * NT)>();
-            const int u = first + wk + (v + i) * WK;
+            const int u = wk + (v + i) * WK;
             fetch((i + AHEAD - 1) % AHEAD, u + (AHEAD - 1) * WK);
-            if (WK > 1 && u >= end) continue;
+            if (WK > 1 && u >= p.units) continue;
             const uintx4 *from = stage + (i * WK + wk) * PIECES * 64 + lane;
             multiply<PARTS, CPLX, MT, NT, GU>(b[i], acc, [&](int m, int ks, int h) { return frag(from[((h * MT + m) * 2 + ks) * 64]); });
         }
@@ -500,7 +499,7 @@ __global__ __launch_bounds__(64 * WN * WK, OCC) void tile_kernel(Par p, Rows r) 
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int t = 0; t < NT; ++t)
-                deliver<T, CPLX>(p, split, tile0 + t, (long)blockIdx.y * MT + m, lane, acc[m][t * Z], acc[m][t * Z + Z - 1]);
+                finish<T, CPLX>(p, row0 + m * 16 + 4 * q, (tile0 + t) * TR + l16, acc[m][t * Z], acc[m][t * Z + Z - 1]);
     } else {
         stage_barrier<0>();
         floatx4 *join = reinterpret_cast<floatx4 *>(stage);
@@ -519,20 +518,35 @@ __global__ __launch_bounds__(64 * WN * WK, OCC) void tile_kernel(Par p, Rows r) 
 #pragma unroll
                 for (int o = 1; o < WK; ++o) v[z] += from[o * WN * MT * NF * 64];
             }
-            deliver<T, CPLX>(p, split, (ct * WN + w) * NT + t, (long)blockIdx.y * MT + m, ln, v[0], v[Z - 1]);
+            finish<T, CPLX>(p, row0 + m * 16 + 4 * (ln >> 4), (tile + w * NT + t) * TR + (ln & 15), v[0], v[Z - 1]);
         }
+    }
+}
+
+template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD, int OCC>
+__global__ __launch_bounds__(64 * WN * WK, OCC) void tile_kernel(Par p, Rows r) {
+    constexpr int STAGE = AHEAD * WK * parts<T>() * MT * 128, JOIN = WK > 1 ? WN * WK * MT * columns<CPLX, NT>() * 64 : 0;
+    __shared__ uintx4 stage[STAGE > JOIN ? STAGE : JOIN];   // [AHEAD][WK][PARTS][MT][2][64]
+    const int z = blockIdx.z;
+    if (z >= p.slices) {
+        tail_dots<T>(p, WN * WK);
+    } else if (NT == 1 || z < p.whole) {
+        tile_block<T, CPLX, WN, WK, MT, NT, GU, AHEAD>(p, r, stage, (z * 8 + blockIdx.x) * WN * NT);
+    } else if constexpr (NT > 1) {
+        tile_block<T, CPLX, WN, WK, MT, NT / 2, GU, AHEAD>(p, r, stage, p.whole * 8 * WN * NT + ((z - p.whole) * 8 + blockIdx.x) * WN * (NT / 2));
     }
 }
 
 // ---------------------------------------------------------------- launches --
 
-// The grid of blocks of `rows` rows by `tiles` weight tiles, with the tail's dots behind them.
-dim3 grid_of(Par &p, int rows, int tiles, int waves) {
+// The grid of p.slices slices by blocks of `rows` rows, with the tail's dots behind them.
+dim3 grid_of(const Par &p, int rows, int waves) {
     const int row_blocks = (int)((p.rows + rows - 1) / rows);
-    p.slices = ((p.tiles + tiles - 1) / tiles + 7) / 8;
     const long per = 8L * row_blocks * waves, dots = p.rows * ((p.tail_n + TAIL - 1) / TAIL);
     return dim3(8, row_blocks, p.slices * p.splits + (int)((dots + per - 1) / per));
 }
+
+int slices_of(int tiles, int each) { return ((tiles + each - 1) / each + 7) / 8; }
 
 template <typename T, bool CPLX>
 int join_splits(const Par &p, hipStream_t stream) {
@@ -545,14 +559,23 @@ int join_splits(const Par &p, hipStream_t stream) {
 
 template <typename T, typename XT, bool CPLX, int NT, int GU, int WAVES, int AHEAD>
 int launch_step(Par p, const Rows &r, hipStream_t stream) {
-    const dim3 grid = grid_of(p, 16, NT, WAVES);
+    p.slices = slices_of(p.tiles, NT);
+    const dim3 grid = grid_of(p, 16, WAVES);
     step_kernel<T, XT, CPLX, NT, GU, WAVES, AHEAD><<<grid, dim3(64 * WAVES), 0, stream>>>(p, r);
     return join_splits<T, CPLX>(p, stream);
 }
 
 template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD, int OCC = 1>
 int launch_tile(Par p, const Rows &r, hipStream_t stream) {
-    const dim3 grid = grid_of(p, MT * 16, WN * NT, WN * WK);
+    p.slices = p.whole = slices_of(p.tiles, WN * NT);
+    if (NT > 1) {
+        // the blocks behind the last whole round of 256 (a CU each) in halves, where those are one round at most
+        const long slice = 8 * ((p.rows + MT * 16 - 1) / (MT * 16)), blocks = (p.tiles + WN * NT - 1) / (WN * NT) * slice / 8;
+        const int whole = (int)(blocks / 256 * 256 / slice);
+        const int halves = slices_of(p.tiles - whole * 8 * WN * NT, WN * NT / 2);
+        if (whole && blocks % 256 && halves * slice <= 256 + slice) p.whole = whole, p.slices = whole + halves;
+    }
+    const dim3 grid = grid_of(p, MT * 16, WN * WK);
     tile_kernel<T, CPLX, WN, WK, MT, NT, GU, AHEAD, OCC><<<grid, dim3(64 * WN * WK), 0, stream>>>(p, r);
     return join_splits<T, CPLX>(p, stream);
 }
