@@ -441,11 +441,13 @@ __global__ __launch_bounds__(64 * WAVES) void step_kernel(Par p, Rows r) {
 
 // More rows: WN waves side by side of MT x 16 rows by NT x 16 outputs, WK times along the inputs; the rows of the
 // weight blocks at hand through LDS in the MFMA's order (direct loads, AHEAD buffers), the weights through
-// registers.  With WK > 1 (a decode step's rows, where there are few blocks) the sums are joined through LDS.
+// registers.  A round is U weight blocks of the wave (two, where there are many: half the barriers, the LDS reads of
+// the second under the products of the first: 512 x 1536 -> 50261 real 98 -> 93 us).  With WK > 1 (a decode step's
+// rows, where there are few blocks) the sums are joined through LDS.
 // `tile`: the block's first weight tile.
-template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD>
+template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD, int U>
 __device__ __forceinline__ void tile_block(const Par &p, const Rows &r, uintx4 *stage, int tile) {
-    constexpr int PARTS = parts<T>(), NF = columns<CPLX, NT>(), Z = NF / NT, WAVES = WN * WK, PIECES = PARTS * MT * 2,
+    constexpr int PARTS = parts<T>(), NF = columns<CPLX, NT>(), Z = NF / NT, WAVES = WN * WK, PIECES = PARTS * MT * 2 * U,
                   EACH = (PIECES + WN - 1) / WN;
     // (the waves load alike, so that the loads in flight can be counted: where PIECES is no multiple of WN some twice)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wk = wave / WN;
@@ -455,23 +457,25 @@ __device__ __forceinline__ void tile_block(const Par &p, const Rows &r, uintx4 *
     const int last = (int)min(p.rows - row0, (long)MT * 16) - 1;
     const unsigned short *x0[EACH];   // a piece's place in the first row, and what a lane adds (bytes, below 2^32)
     unsigned row[EACH];
+    int block[EACH];                  // of the round's
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-        const int piece = (i * WN + wn) % PIECES, ks = piece & 1, m = (piece >> 1) % MT, h = (piece >> 1) / MT;
+        const int piece = (i * WN + wn) % PIECES, ks = piece & 1, m = (piece >> 1) % MT, h = (piece >> 1) / MT % PARTS, un = (piece >> 1) / (MT * PARTS);
+        block[i] = un;
         x0[i] = r.x + row0 * r.ldx + h * r.plane + 32 * ks;
         row[i] = ((unsigned)min(m * 16 + l16, last) * (unsigned)r.ldx + 8 * q) * 2;
     }
     const Tiles<NT, GU> tiles(p, tile0);
-    Block<NT, GU> b[AHEAD];
-    // Block u into buffer i (behind the last: that again, so that the loads in flight can be counted).
+    Block<NT, GU> b[AHEAD][U];
+    // The round from block u on into buffer i (behind the last block: that again, so that the loads in flight can be counted).
     auto fetch = [&](int i, int u) {
-        u = min(u, p.units - 1);
         uintx4 *to = stage + (i * WK + wk) * PIECES * 64;
 #pragma unroll
         for (int j = 0; j < EACH; ++j)
-            __builtin_amdgcn_global_load_lds(reinterpret_cast<const unsigned *>(reinterpret_cast<const char *>(x0[j] + (long)u * TK) + row[j]),
+            __builtin_amdgcn_global_load_lds(reinterpret_cast<const unsigned *>(reinterpret_cast<const char *>(x0[j] + (long)min(u + block[j], p.units - 1) * TK) + row[j]),
                                              reinterpret_cast<unsigned *>(to + (j * WN + wn) % PIECES * 64), 16, 0, 0);
-        b[i].load(p, tiles, u, lane);
+#pragma unroll
+        for (int e = 0; e < U; ++e) b[i][e].load(p, tiles, min(u + e, p.units - 1), lane);
     };
     floatx4 acc[MT][NF];
 #pragma unroll
@@ -479,19 +483,22 @@ __device__ __forceinline__ void tile_block(const Par &p, const Rows &r, uintx4 *
 #pragma unroll
         for (int n = 0; n < NF; ++n) acc[m][n] = floatx4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < AHEAD - 1; ++i) fetch(i, wk + i * WK);
-    const int rounds = (p.units + WK - 1) / WK;
+    for (int i = 0; i < AHEAD - 1; ++i) fetch(i, (wk + i * WK) * U);
+    const int rounds = (p.units + WK * U - 1) / (WK * U);
     for (int v = 0; v < rounds; v += AHEAD) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             if (v + i >= rounds) break;
             // round v + i has arrived, for every wave; the buffer of the one before is free
-            stage_barrier<(AHEAD - 2) * (EACH + 2 * NT)>();
-            const int u = wk + (v + i) * WK;
-            fetch((i + AHEAD - 1) % AHEAD, u + (AHEAD - 1) * WK);
-            if (WK > 1 && u >= p.units) continue;
-            const uintx4 *from = stage + (i * WK + wk) * PIECES * 64 + lane;
-            multiply<PARTS, CPLX, MT, NT, GU>(b[i], acc, [&](int m, int ks, int h) { return frag(from[((h * MT + m) * 2 + ks) * 64]); });
+            stage_barrier<(AHEAD - 2) * (EACH + 2 * NT * U)>();
+            const int u = (wk + (v + i) * WK) * U;
+            fetch((i + AHEAD - 1) % AHEAD, u + (AHEAD - 1) * WK * U);
+#pragma unroll
+            for (int e = 0; e < U; ++e) {
+                if ((WK > 1 || e) && u + e >= p.units) break;
+                const uintx4 *from = stage + (i * WK + wk) * PIECES * 64 + e * PARTS * MT * 128 + lane;
+                multiply<PARTS, CPLX, MT, NT, GU>(b[i][e], acc, [&](int m, int ks, int h) { return frag(from[((h * MT + m) * 2 + ks) * 64]); });
+            }
         }
     }
     if constexpr (WK == 1) {
@@ -523,17 +530,17 @@ __device__ __forceinline__ void tile_block(const Par &p, const Rows &r, uintx4 *
     }
 }
 
-template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD, int OCC>
+template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD, int OCC, int U>
 __global__ __launch_bounds__(64 * WN * WK, OCC) void tile_kernel(Par p, Rows r) {
-    constexpr int STAGE = AHEAD * WK * parts<T>() * MT * 128, JOIN = WK > 1 ? WN * WK * MT * columns<CPLX, NT>() * 64 : 0;
-    __shared__ uintx4 stage[STAGE > JOIN ? STAGE : JOIN];   // [AHEAD][WK][PARTS][MT][2][64]
+    constexpr int STAGE = AHEAD * WK * parts<T>() * MT * 128 * U, JOIN = WK > 1 ? WN * WK * MT * columns<CPLX, NT>() * 64 : 0;
+    __shared__ uintx4 stage[STAGE > JOIN ? STAGE : JOIN];   // [AHEAD][WK][U][PARTS][MT][2][64]
     const int z = blockIdx.z;
     if (z >= p.slices) {
         tail_dots<T>(p, WN * WK);
     } else if (NT == 1 || z < p.whole) {
-        tile_block<T, CPLX, WN, WK, MT, NT, GU, AHEAD>(p, r, stage, (z * 8 + blockIdx.x) * WN * NT);
+        tile_block<T, CPLX, WN, WK, MT, NT, GU, AHEAD, U>(p, r, stage, (z * 8 + blockIdx.x) * WN * NT);
     } else if constexpr (NT > 1) {
-        tile_block<T, CPLX, WN, WK, MT, NT / 2, GU, AHEAD>(p, r, stage, p.whole * 8 * WN * NT + ((z - p.whole) * 8 + blockIdx.x) * WN * (NT / 2));
+        tile_block<T, CPLX, WN, WK, MT, NT / 2, GU, AHEAD, U>(p, r, stage, p.whole * 8 * WN * NT + ((z - p.whole) * 8 + blockIdx.x) * WN * (NT / 2));
     }
 }
 
@@ -565,7 +572,7 @@ int launch_step(Par p, const Rows &r, hipStream_t stream) {
     return join_splits<T, CPLX>(p, stream);
 }
 
-template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD, int OCC = 1>
+template <typename T, bool CPLX, int WN, int WK, int MT, int NT, int GU, int AHEAD, int OCC = 1, int U = 1>
 int launch_tile(Par p, const Rows &r, hipStream_t stream) {
     p.slices = p.whole = slices_of(p.tiles, WN * NT);
     if (NT > 1) {
@@ -576,7 +583,7 @@ int launch_tile(Par p, const Rows &r, hipStream_t stream) {
         if (whole && blocks % 256 && halves * slice <= 256 + slice) p.whole = whole, p.slices = whole + halves;
     }
     const dim3 grid = grid_of(p, MT * 16, WN * WK);
-    tile_kernel<T, CPLX, WN, WK, MT, NT, GU, AHEAD, OCC><<<grid, dim3(64 * WN * WK), 0, stream>>>(p, r);
+    tile_kernel<T, CPLX, WN, WK, MT, NT, GU, AHEAD, OCC, U><<<grid, dim3(64 * WN * WK), 0, stream>>>(p, r);
     return join_splits<T, CPLX>(p, stream);
 }
 
@@ -601,8 +608,8 @@ struct Plan {
 // read less.  Measured (us, K = 1536 real inputs; complex, group 32 bf16 | group 64 fp32 with its layout):
 //   pieces   144: step 4.5 | 7.3, 2 x 1 pieces 5.2 | 7.9      288: 6.0 | 11.2, 2 x 1 5.3 | 8.0
 //   576: 2 x 1 7.3 | 12.6, 2 x 2 (fp32 4 x 1) 6.9 | 10.1      1728: 2 x 2 11.1, 4 x 2 9.0 | 14.5, 6 x 2 21.0
-//   9216: 4 x 2 26.3 | 60.7, 4 x 4 of 2 tiles 29 | 58.6, 4 x 2 of 2 tiles | 44.8
-//   36000: 4 x 2 (8 x 4 of one tile 72), 4 x 4 of 2 tiles 66 | 4 x 2 of 2 tiles 137
+//   2304, 3456: | 4 x 2 22.6, 23.0, 6 x 2 18.9, 27.1, 4 x 2 of two tiles 23.4, 23.4
+//   9216: 4 x 2 26.3 | 54.7, 4 x 4 of two tiles 29, 4 x 2 of two tiles | 39.6      36000: 4 x 4 of two tiles 66, 8 x 4 72
 Plan plan(const qpam_linear4_args *a) {
     const int kr = a->is_complex ? 2 * a->k : a->k, units = padded(kr) / TK, tiles = (a->n + TR - 1) / TR;
     const bool f32 = a->dtype == QPAM_F32;
@@ -615,7 +622,7 @@ Plan plan(const qpam_linear4_args *a) {
         l.shape = tiles > (f32 ? 512 : 1024) ? 7 : 1;
     } else if (a->rows > 16 && pieces > 256) {
         l.shape = pieces <= 512 ? 2 : pieces <= 1024 ? 3 : pieces <= (f32 ? 2048 : a->is_complex ? 12288 : 4096) ? 4 : 5;
-        if (f32 && l.shape == 5 && pieces > 8192) l.shape = 6;
+        if (f32 && l.shape == 5 && pieces > 3000) l.shape = 6;
     }
     // few tiles of long fp32 rows: more blocks by ranges of the inputs, joined in a launch of their own (16 rows x 4608
     // inputs, 48 tiles: 14.8 -> 9.2 us; bf16 7.5 -> 7.0, not worth the memory)
@@ -649,13 +656,15 @@ int run(const Plan &l, const Par &p, const Rows &r, hipStream_t stream) {
         else return launch_tile<T, CPLX, 2, 4, 2, 1, GU, 3>(p, r, stream);
     case 4: return launch_tile<T, CPLX, 4, 2, 2, 1, GU, F32 ? 2 : 3>(p, r, stream);
     default:
-        if constexpr (F32) {
-            if (l.shape == 5) return launch_tile<T, CPLX, 6, 1, 2, 1, GU, 2>(p, r, stream);
-            return launch_tile<T, CPLX, 4, 1, 2, CPLX ? 2 : 4, GU, 2, 3>(p, r, stream);
+        if constexpr (F32 && CPLX) {
+            if (l.shape == 5) return launch_tile<T, CPLX, 6, 1, 2, 1, GU, 2, 1, 2>(p, r, stream);
+            return launch_tile<T, CPLX, 4, 1, 2, 2, GU, 2, 3, 2>(p, r, stream);
+        } else if constexpr (F32) {
+            return launch_tile<T, CPLX, 8, 1, 2, 2, GU, 2, 1, 2>(p, r, stream);
         } else if constexpr (CPLX) {
-            return launch_tile<T, CPLX, 4, 1, 4, 2, GU, 3, 3>(p, r, stream);
+            return launch_tile<T, CPLX, 4, 1, 4, 2, GU, 3, 2>(p, r, stream);
         } else {
-            return launch_tile<T, CPLX, 8, 1, 4, 2, GU, 3>(p, r, stream);
+            return launch_tile<T, CPLX, 8, 1, 4, 2, GU, 2, 1, 2>(p, r, stream);
         }
     }
 }

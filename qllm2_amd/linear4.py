@@ -173,7 +173,7 @@ def _product(x: Tensor, codes: Tensor, scales: Tensor, n: int, k: int, group: in
     z = 2 if is_complex else 1
     extra = 0 if tail is None else tail.shape[0]
     wide = z * n + extra
-    out = torch.empty((*x.shape[:-z], n, 2) if is_complex and not planes else (*x.shape[:-z], wide), device=x.device, dtype=x.dtype)
+    out = x.new_empty((*x.shape[:-z], n, 2) if is_complex and not planes else (*x.shape[:-z], wide))
     count = out.numel() // wide
     if not count:
         return out
