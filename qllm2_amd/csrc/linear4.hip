@@ -330,54 +330,79 @@ __device__ __forceinline__ bool place(const Par &p, int waves, int &ct, int &spl
     return true;
 }
 
+// 16 bytes at any address of the type (the hardware's global loads take them off their alignment).
 template <typename V> __device__ __forceinline__ V at(const void *base, unsigned bytes) {
-    return *reinterpret_cast<const V *>(static_cast<const char *>(base) + bytes);
+    V v;
+    __builtin_memcpy(&v, static_cast<const char *>(base) + bytes, sizeof(V));
+    return v;
 }
 
 // The rows' part of a weight block, in registers: bf16 planes, or fp32 rows cut into their parts where they are used.
-// `row`: what a lane adds to the first row's start, in bytes (below 2^32).
-template <typename XT, int PARTS, int MT> struct Part {
-    uintx4 v[MT][2][PARTS];
-    __device__ __forceinline__ void load(const XT *x, const unsigned (&row)[MT], long plane, int k, int kr) {
+// `row`: what a lane adds to the first row's start, in bytes (below 2^32).  A block that ends behind the last input kr
+// is read by as many values as there are, zeros beyond (the codes there are zero, but a value of the next row may be a NaN).
+template <typename XT, int PARTS> struct Part {
+    uintx4 v[2][PARTS];
+    __device__ __forceinline__ void load(const XT *x, unsigned row, long plane, int u, int q, int kr) {
+        const int k = u * TK + 8 * q;
+        if ((u + 1) * TK <= kr) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int h = 0; h < PARTS; ++h) v[ks][h] = at<uintx4>(x + h * plane, row + (k + 32 * ks) * 2u);
+        } else {
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int h = 0; h < PARTS; ++h) {
-                    // behind the last input: the codes there are zero, but what is read must be, too
-                    const bool in = k + 32 * ks < kr;
-                    const uintx4 a = at<uintx4>(x + h * plane, row[m] + (in ? k + 32 * ks : 0) * 2u);
+                    const int f = k + 32 * ks;
+                    ushortx8 a = {0, 0, 0, 0, 0, 0, 0, 0};
+                    if (f + 8 <= kr) {
+                        a = at<ushortx8>(x + h * plane, row + f * 2u);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[m][ks][h][j] = in ? a[j] : 0;
+                        for (int j = 0; j < 7; ++j)
+                            if (f + j < kr) a[j] = at<unsigned short>(x + h * plane, row + (f + j) * 2u);
+                    }
+                    v[ks][h] = __builtin_bit_cast(uintx4, a);
                 }
+        }
     }
-    __device__ __forceinline__ void get(int m, int ks, bf16x8 (&p)[PARTS]) const {
+    __device__ __forceinline__ void get(int ks, bf16x8 (&p)[PARTS]) const {
 #pragma unroll
-        for (int h = 0; h < PARTS; ++h) p[h] = frag(v[m][ks][h]);
+        for (int h = 0; h < PARTS; ++h) p[h] = frag(v[ks][h]);
     }
 };
-template <int MT> struct Part<float, 1, MT> {
-    floatx4 v[MT][2][2];
-    __device__ __forceinline__ void load(const float *x, const unsigned (&row)[MT], long, int k, int kr) {
+template <> struct Part<float, 1> {
+    floatx4 v[2][2];
+    __device__ __forceinline__ void load(const float *x, unsigned row, long, int u, int q, int kr) {
+        const int k = u * TK + 8 * q;
+        if ((u + 1) * TK <= kr) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                const bool in = k + 32 * ks < kr;
-                const unsigned from = row[m] + (in ? k + 32 * ks : 0) * 4u;
+                for (int e = 0; e < 2; ++e) v[ks][e] = at<floatx4>(x, row + (k + 32 * ks + 4 * e) * 4u);
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const floatx4 a = at<floatx4>(x, from + 16 * e);
+                    const int f = k + 32 * ks + 4 * e;
+                    floatx4 a = {0, 0, 0, 0};
+                    if (f + 4 <= kr) {
+                        a = at<floatx4>(x, row + f * 4u);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[m][ks][e][j] = in ? a[j] : 0.f;
+                        for (int j = 0; j < 3; ++j)
+                            if (f + j < kr) a[j] = at<float>(x, row + (f + j) * 4u);
+                    }
+                    v[ks][e] = a;
                 }
-            }
+        }
     }
-    __device__ __forceinline__ void get(int m, int ks, bf16x8 (&p)[3]) const {
+    __device__ __forceinline__ void get(int ks, bf16x8 (&p)[3]) const {
         float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = v[m][ks][j / 4][j % 4];
+        for (int j = 0; j < 8; ++j) f[j] = v[ks][j / 4][j % 4];
         split(f, p);
     }
 };
@@ -396,17 +421,17 @@ __global__ __launch_bounds__(64 * WAVES) void step_kernel(Par p, Rows r) {
     const long row0 = (long)blockIdx.y * 16;
     const XT *x0 = reinterpret_cast<const XT *>(r.x) + row0 * r.ldx;
     // rows behind the last read the last one, and are not written
-    const unsigned row[1] = {(unsigned)min(lane & 15, (int)min(p.rows - row0, 16L) - 1) * (unsigned)r.ldx * (unsigned)sizeof(XT)};
+    const unsigned row = (unsigned)min(lane & 15, (int)min(p.rows - row0, 16L) - 1) * (unsigned)r.ldx * (unsigned)sizeof(XT);
     floatx4 acc[1][NF];
 #pragma unroll
     for (int n = 0; n < NF; ++n) acc[0][n] = floatx4{0, 0, 0, 0};
     const Tiles<NT, GU> tiles(p, ct * NT);
     Block<NT, GU> b[AHEAD];
-    Part<XT, XP, 1> x[AHEAD];
+    Part<XT, XP> x[AHEAD];
     auto fetch = [&](int i, int u) {  // (behind the last block: that again, not used)
         u = min(u, p.units - 1);
         b[i].load(p, tiles, u, lane);
-        x[i].load(x0, row, r.plane, u * TK + 8 * q, p.kr);
+        x[i].load(x0, row, r.plane, u, q, p.kr);
     };
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) fetch(i, first + wave + i * WAVES);
@@ -416,7 +441,7 @@ __global__ __launch_bounds__(64 * WAVES) void step_kernel(Par p, Rows r) {
             if (u + i * WAVES >= end) break;
             bf16x8 part[PARTS];
             multiply<PARTS, CPLX, 1, NT, GU>(b[i], acc, [&](int m, int ks, int h) {
-                if (h == 0) x[i].get(m, ks, part);
+                if (h == 0) x[i].get(ks, part);
                 return part[h];
             });
             if (u + (i + AHEAD) * WAVES < end) fetch(i, u + (i + AHEAD) * WAVES);
@@ -589,14 +614,6 @@ int launch_tile(Par p, const Rows &r, hipStream_t stream) {
 
 int padded(int kr) { return (kr + TK - 1) / TK * TK; }
 
-// Rows that the kernels read as they stand: aligned 16-byte pieces (of few rows any number of them, fp32 too), lanes'
-// offsets below 2^32.
-bool stand(const qpam_linear4_args *a, int kr) {
-    const int elem = a->dtype == QPAM_BF16 ? 2 : 4;
-    if ((uintptr_t)a->x % 16 || (a->rows > 1 && (a->ldx * elem % 16 || a->ldx > (1 << 24))) || kr % 8) return false;
-    return a->rows <= 16 || (a->dtype == QPAM_BF16 && kr % TK == 0);
-}
-
 // What a call runs: a shape of blocks (run), ranges along the inputs, and the workspace.
 struct Plan {
     int shape, splits, share;
@@ -605,29 +622,32 @@ struct Plan {
 
 // The shape by the number of 16 x 16 pieces of the result: as long as the GPU's 256 CUs have no more than about one
 // block each, a block of fewer pieces with more waves along the inputs is done earlier; then larger ones, which
-// read less.  Measured (us, K = 1536 real inputs; complex, group 32 bf16 | group 64 fp32 with its layout):
-//   pieces   144: step 4.5 | 7.3, 2 x 1 pieces 5.2 | 7.9      288: 6.0 | 11.2, 2 x 1 5.3 | 8.0
-//   576: 2 x 1 7.3 | 12.6, 2 x 2 (fp32 4 x 1) 6.9 | 10.1      1728: 2 x 2 11.1, 4 x 2 9.0 | 14.5, 6 x 2 21.0
-//   2304, 3456: | 4 x 2 22.6, 23.0, 6 x 2 18.9, 27.1, 4 x 2 of two tiles 23.4, 23.4
-//   9216: 4 x 2 26.3 | 54.7, 4 x 4 of two tiles 29, 4 x 2 of two tiles | 39.6      36000: 4 x 4 of two tiles 66, 8 x 4 72
+// read less.  Measured (us, K = 1536 real inputs, complex):
+//   bf16, group 32.  16 rows, 576 tiles: step kernel of one tile 7.7, of two 6.7.  More rows, pieces
+//     144: step 4.5, 2 x 1 pieces 5.2       288: 6.0, 5.3       576: 2 x 1 7.3, 2 x 2 6.9       1728: 2 x 2 11.1, 4 x 2 9.0
+//     9216: 4 x 2 26.3, 4 x 4 of two tiles 29       36000: 4 x 4 of two tiles 66, 8 x 4 of one 72
+//   fp32, group 64: the step kernel cuts the rows itself; the others read them laid out, 2 us and a launch more
+//     192: one tile 6.6, two 7.0       432: 10.0, 7.3       864: two 10.8, four 9.2       1152: four 16.3, 4 x 2 13.3 + 2
+//     2304, 3456 (laid out): 4 x 2 22.6, 23.0, 6 x 2 18.9, 27.1, 4 x 2 of two tiles 23.4, 23.4       9216: 54.7, -, 39.6
 Plan plan(const qpam_linear4_args *a) {
     const int kr = a->is_complex ? 2 * a->k : a->k, units = padded(kr) / TK, tiles = (a->n + TR - 1) / TR;
     const bool f32 = a->dtype == QPAM_F32;
+    // the step kernel reads rows as they stand where a lane's offset is below 2^32, the tile kernel aligned ones of bf16 in
+    // whole blocks of inputs
+    const bool near = a->rows == 1 || a->ldx <= (1 << 24);
+    const bool whole = !f32 && near && (uintptr_t)a->x % 16 == 0 && kr % TK == 0 && (a->rows == 1 || a->ldx % 8 == 0);
     Plan l{0, 1, units, 0, 0};
-    if (!stand(a, kr)) l.lay = ((size_t)a->rows * padded(kr) * 2 * (f32 ? 3 : 1) + 255) / 256 * 256;
     const long pieces = (a->rows + 15) / 16 * tiles;
-    // of few rows a block takes 16, 32 or 64 outputs: up to 256 blocks each has a CU, and fewer blocks read the rows less
-    // often (fp32, 288 tiles: 16 outputs 8.0 us, 32 6.0; 576: 32 outputs 10.3, 64 7.9; bf16, 576 tiles and 16 rows: 7.7, 6.7)
-    if (a->rows <= 16 && tiles > 256) {
-        l.shape = tiles > (f32 ? 512 : 1024) ? 7 : 1;
-    } else if (a->rows > 16 && pieces > 256) {
-        l.shape = pieces <= 512 ? 2 : pieces <= 1024 ? 3 : pieces <= (f32 ? 2048 : a->is_complex ? 12288 : 4096) ? 4 : 5;
-        if (f32 && l.shape == 5 && pieces > 3000) l.shape = 6;
-    }
-    // few tiles of long fp32 rows: more blocks by ranges of the inputs, joined in a launch of their own (16 rows x 4608
+    if (a->rows <= 16 || (f32 && near && pieces <= 2048))
+        l.shape = pieces <= 256 ? 0 : pieces <= (f32 ? 512 : 1024) ? 1 : 7;
+    else if (pieces > 256)  // (shape 3: 32 rows by two tiles)
+        l.shape = pieces <= 512 ? 2 : (a->rows + 31) / 32 * ((tiles + 1) / 2) <= 256 ? 3 : pieces <= (f32 ? 2048 : a->is_complex ? 12288 : 4096) ? 4 : f32 && pieces > 3000 ? 6 : 5;
+    const bool step = l.shape < 2 || l.shape == 7;
+    if (step ? !near : !whole) l.lay = ((size_t)a->rows * padded(kr) * 2 * (f32 ? 3 : 1) + 255) / 256 * 256;
+    // few pieces of long fp32 rows: more blocks by ranges of the inputs, joined in a launch of their own (16 rows x 4608
     // inputs, 48 tiles: 14.8 -> 9.2 us; bf16 7.5 -> 7.0, not worth the memory)
-    if (f32 && l.shape == 0 && pieces <= 64 && units >= 48) {
-        l.splits = 4, l.share = (units + 3) / 4;
+    if (f32 && l.shape == 0 && pieces <= 128 && units >= 48) {
+        l.splits = pieces <= 64 ? 4 : 2, l.share = (units + l.splits - 1) / l.splits;
         l.sums = (size_t)l.splits * pieces * (a->is_complex ? 2048 : 1024);
     }
     return l;

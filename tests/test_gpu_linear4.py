@@ -213,6 +213,18 @@ def test_offsets_past_32_bits(gpu_lib):
     _check(linear4(x, w), x, w)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [5, 40])
+def test_rows_far_apart(gpu_lib, n, dtype):
+    """A row stride above 2^24 elements; from there on rows are laid out for the kernels."""
+    K = 200
+    x = torch.empty(n, (1 << 24) + 8, device="cuda", dtype=dtype)[:, 3:3 + K]
+    x.copy_(_rows((n, K), dtype, 60))
+    for N in (50, 5000, 9000):
+        w = Weight4(*_codes(N, K, 64, 61), K, 64)
+        _check(linear4(x, w), x, w)
+
+
 def test_streams_and_graphs(gpu_lib):
     K, N = 256, 130
     w = Weight4(*_codes(N, 2 * K, 32, 27), K, 32, complex=True)
