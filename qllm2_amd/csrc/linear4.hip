@@ -257,12 +257,15 @@ template <int NT, int GU> struct Block {
     unsigned s[NT];
     __device__ __forceinline__ void load(const Par &p, const Tiles<NT, GU> &from, int u, int lane) {
         const int at = GU == 2 ? 2 * u : p.scale_step == 1 ? u : u >> 1;
+        // (scalar base, vector offset: left to itself the compiler adds both in vector registers at each load)
+        unsigned ow = lane * 8, os = (lane & 15) * 2 * GU;
+        asm("" : "+v"(ow), "+v"(os));
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            w[t] = reinterpret_cast<const uintx2 *>(from.codes[t] + (long)u * 512)[(unsigned)lane];
-            const unsigned short *sc = from.scales[t] + (long)at * TR;
-            if constexpr (GU == 2) s[t] = reinterpret_cast<const unsigned *>(sc)[(unsigned)lane & 15];
-            else s[t] = sc[(unsigned)lane & 15];
+            w[t] = *reinterpret_cast<const uintx2 *>(from.codes[t] + (long)u * 512 + ow);
+            const char *sc = reinterpret_cast<const char *>(from.scales[t] + (long)at * TR) + os;
+            if constexpr (GU == 2) s[t] = *reinterpret_cast<const unsigned *>(sc);
+            else s[t] = *reinterpret_cast<const unsigned short *>(sc);
         }
     }
     __device__ __forceinline__ float scale(int t, int g) const {
