@@ -10,9 +10,16 @@
 // the weight s e nor anything else is rounded to bf16 on the way.  fp32 rows are cut into three bf16 parts
 // (24 bits = 3 x 8, exact), three products each.
 //
-// A complex weight is two neighbouring codes (re, im) and is read once: with the rows (xr, -xi) and
-// (xi, xr) made from a row x, the real and the imaginary output are two rows of one real product.  (The
-// same product as a real matrix [wr, -wi; wi, wr] has every weight twice.)
+// A complex weight is two neighbouring codes (re, im) and is read once: of a widened pair come the operands
+// (wr, -wi) and (wi, wr) of the real and of the imaginary output, a sign and a rotation away, and both meet
+// the row as it stands.  (The same product as a real matrix [wr, -wi; wi, wr] reads every weight twice.)
+//
+// What bounds it: few rows, the launch and one trip to memory (768 -> 768 complex, one row: 3.0 us in a graph;
+// a graph's empty kernel 1.9), with a large table its bytes (50261 x 1536, one row: 10.9 us, 4.0 TB/s of 5.0).
+// Some hundred rows and prompts, the vector instructions beside the MFMAs: a multiply-add for every output and
+// group (one a group and MFMA lane: as long as the MFMAs themselves at group 32), the widening and turning of a
+// step's codes once per 64 rows (512 x 1536 -> 50261 real, group 64: 38 % of the SIMDs' cycles MFMA, 41 % other
+// vector work, LDS reads without conflicts; 2000 x 768 -> 4608 complex, group 32: 42 % and 67 %).
 //
 // Layout (qpam_linear4 in the header): 512-byte blocks of 16 outputs x 64 inputs in the order of the MFMA's
 // B operand, so a wave reads its weights as whole consecutive 8-byte lanes.
@@ -220,20 +227,25 @@ __device__ __forceinline__ void deliver(const Par &p, int split, int tile, long 
     }
 }
 
+// The sums of the ranges (at most SPLITS, all read before any is added), a wave per tile and 16 rows.
+constexpr int SPLITS = 4;
 template <typename T, bool CPLX>
-__global__ __launch_bounds__(256) void join_kernel(Par p) {
-    const long ms = (p.rows + 15) / 16, unit = (long)blockIdx.x * 4 + (threadIdx.x >> 6);   // a wave per tile and 16 rows
-    if (unit >= p.tiles * ms) return;
-    const int lane = threadIdx.x & 63;
-    const floatx4 *from = p.sums + unit * (CPLX ? 128 : 64) + lane;
-    floatx4 a = from[0], b = CPLX ? from[64] : a;
-    for (int o = 1; o < p.splits; ++o) {
-        from += p.tiles * ms * (CPLX ? 128 : 64);
-        a += from[0];
-        if (CPLX) b += from[64];
-    }
-    const int tile = (int)(unit / ms);
-    finish<T, CPLX>(p, (unit - tile * ms) * 16 + 4 * (lane >> 4), tile * TR + (lane & 15), a, b);
+__global__ __launch_bounds__(64) void join_kernel(Par p) {
+    constexpr int Z = CPLX ? 2 : 1;
+    const long ms = (p.rows + 15) / 16;
+    const int lane = threadIdx.x, tile = blockIdx.x;
+    const floatx4 *from = p.sums + (tile * ms + blockIdx.y) * Z * 64 + lane;
+    floatx4 v[SPLITS][Z];
+#pragma unroll
+    for (int o = 0; o < SPLITS; ++o)
+#pragma unroll
+        for (int z = 0; z < Z; ++z) v[o][z] = from[min(o, p.splits - 1) * p.tiles * ms * Z * 64 + z * 64];
+#pragma unroll
+    for (int o = 1; o < SPLITS; ++o)
+#pragma unroll
+        for (int z = 0; z < Z; ++z)
+            if (o < p.splits) v[0][z] += v[o][z];
+    finish<T, CPLX>(p, (long)blockIdx.y * 16 + 4 * (lane >> 4), tile * TR + (lane & 15), v[0][0], v[0][Z - 1]);
 }
 
 // The wave's weights: where its tiles' blocks and scales begin (the same for all lanes), and what a lane adds.
@@ -587,8 +599,7 @@ template <typename T, bool CPLX>
 int join_splits(const Par &p, hipStream_t stream) {
     if (int e = launch_status("qpam_linear4")) return e;
     if (p.splits == 1) return QPAM_OK;
-    const long units = p.tiles * ((p.rows + 15) / 16);
-    join_kernel<T, CPLX><<<dim3((unsigned)((units + 3) / 4)), dim3(256), 0, stream>>>(p);
+    join_kernel<T, CPLX><<<dim3(p.tiles, (unsigned)((p.rows + 15) / 16)), dim3(64), 0, stream>>>(p);
     return launch_status("qpam_linear4");
 }
 

@@ -8,7 +8,9 @@
 // any permutation runs in place with no order of the moves, no second copy of a page and no plan, also
 // where the lists are on the device; a page that several moves read comes from memory once (the block's
 // other reads of it hit its caches).  Bound: HBM, one read of each distinct source, one write of each
-// destination.
+// destination: 15 copies of a page of 18.9 MB 49 us (6.1 TB/s, a fill 6.8), 128 beams of 6.3 MB in place 225 us
+// (5.1 TB/s, a copy 5.0).  The stores pass the caches by (nontemporal): the next reader of a pool this large finds
+// them in memory either way (the 15 copies: 68 us without).
 #include <algorithm>
 
 #include "common.h"

@@ -198,6 +198,21 @@ def test_small_and_large_values(gpu_lib, scale):
     _check(linear4(mixed, w), mixed, w)
 
 
+def test_more_rows_than_a_grid_takes(gpu_lib):
+    """Rows in pieces of 2^19, the tail's with them."""
+    n = (1 << 19) + 100
+    w = Weight4(*_codes(5, 32, 32, 70), 16, 32, complex=True)
+    x, tail = _rows((n, 16, 2), BF16, 71), _rows((3, 32), BF16, 72)
+    y = complex_linear4(x, w, planes=True, tail=tail)
+    for at in (slice(0, 64), slice((1 << 19) - 32, (1 << 19) + 32), slice(n - 64, n)):
+        _check(y[at], x[at], w, tail=tail, planes=True)
+    w = Weight4(*_codes(40, 90, 64, 73), 90, 64)
+    x = _rows((n, 90), F32, 74)
+    y = linear4(x, w)
+    for at in (slice(0, 64), slice((1 << 19) - 32, (1 << 19) + 32), slice(n - 64, n)):
+        _check(y[at], x[at], w)
+
+
 def test_offsets_past_32_bits(gpu_lib):
     """Outputs, then rows, of more than 2^31 elements."""
     K, N, n = 32, 50000, 45000
