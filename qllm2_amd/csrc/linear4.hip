@@ -64,28 +64,39 @@ __device__ __forceinline__ bf16x8 widen(unsigned w) {
     return frag(r);
 }
 
-// fp32 values as sums of three bf16 values, the largest last: each the leading 8 bits of what is left, so the
-// sum is exact.  Infinities and NaN stay in the last alone (inf - inf would make NaN of them).
+// fp32 values as sums of three bf16 values, the largest last: each what is left rounded to bf16 (to nearest: 8 + 8 + 8
+// bits hold the 24 and the sum is exact).  For magnitudes below FAR; NaN stays NaN.
+constexpr float FAR = 3.3e38f;   // from near 2^128 on the first rounding may overflow
 __device__ __forceinline__ void split(const float (&v)[8], bf16x8 (&p)[3]) {
-    uintx4 hi, mid, lo;
+    uintx4 part[3];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        unsigned h[2], m[2], l[2];
+        float a = v[2 * j], b = v[2 * j + 1];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const float f = v[2 * j + e];
-            h[e] = __float_as_uint(f) & 0xffff0000u;
-            const float r = (h[e] & 0x7f800000u) == 0x7f800000u ? 0.f : f - __uint_as_float(h[e]);
-            m[e] = __float_as_uint(r) & 0xffff0000u;
-            l[e] = __float_as_uint(r - __uint_as_float(m[e]));
-            // a NaN whose payload is in the low bits alone stays a NaN
-            if (f != f) h[e] |= 0x400000u;
+        for (int h = 2; h >= 0; --h) {
+            const unsigned w = pack_bf16x2(a, b);
+            part[h][j] = w;
+            a -= __uint_as_float(w << 16);
+            b -= __uint_as_float(w & 0xffff0000u);
         }
-        hi[j] = h[0] >> 16 | (h[1] & 0xffff0000u);
-        mid[j] = m[0] >> 16 | (m[1] & 0xffff0000u);
-        lo[j] = l[0] >> 16 | (l[1] & 0xffff0000u);
     }
-    p[0] = frag(lo), p[1] = frag(mid), p[2] = frag(hi);
+#pragma unroll
+    for (int h = 0; h < 3; ++h) p[h] = frag(part[h]);
+}
+// The same of any value (the same parts of those below FAR, so that a row's bits do not hang on its neighbours'): the
+// others by cutting bits off, infinities in the last part alone (inf - inf would make NaN of them).
+__device__ __forceinline__ void split_any(const float (&v)[8], bf16x8 (&p)[3]) {
+    float near[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) near[j] = fabsf(v[j]) > FAR ? 0.f : v[j];
+    split(near, p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if (!(fabsf(v[j]) > FAR)) continue;
+        const float hi = __uint_as_float(__float_as_uint(v[j]) & 0xffff0000u);
+        const float r = fabsf(v[j]) == INFINITY ? 0.f : v[j] - hi, mid = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+        p[2][j] = (__bf16)hi, p[1][j] = (__bf16)mid, p[0][j] = (__bf16)(r - mid);
+    }
 }
 
 __device__ __forceinline__ void put(float *y, long at, float v) { y[at] = v; }
@@ -155,7 +166,7 @@ __global__ __launch_bounds__(256) void lay_rows_kernel(const T *x, long ldx, lon
             *reinterpret_cast<uintx4 *>(to) = __builtin_bit_cast(uintx4, v);
         } else {
             bf16x8 part[3];
-            split(v, part);
+            split_any(v, part);
 #pragma unroll
             for (int h = 0; h < 3; ++h) *reinterpret_cast<bf16x8 *>(to + (long)h * rows * kp) = part[h];
         }
@@ -382,7 +393,8 @@ template <typename XT, int PARTS> struct Part {
                 }
         }
     }
-    __device__ __forceinline__ void get(int ks, bf16x8 (&p)[PARTS]) const {
+    __device__ __forceinline__ bool far() const { return false; }
+    template <bool ANY> __device__ __forceinline__ void get(int ks, bf16x8 (&p)[PARTS]) const {
 #pragma unroll
         for (int h = 0; h < PARTS; ++h) p[h] = frag(v[ks][h]);
     }
@@ -414,11 +426,19 @@ template <> struct Part<float, 1> {
                 }
         }
     }
-    __device__ __forceinline__ void get(int ks, bf16x8 (&p)[3]) const {
+    // Whether any lane has a value that split does not take.
+    __device__ __forceinline__ bool far() const {
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) m = fmaxf(fmaxf(m, fabsf(v[j / 8][j / 4 % 2][j % 4])), fabsf(v[j / 8][j / 4 % 2][j % 4 + 1]));
+        return __any(m > FAR);
+    }
+    template <bool ANY> __device__ __forceinline__ void get(int ks, bf16x8 (&p)[3]) const {
         float f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = v[ks][j / 4][j % 4];
-        split(f, p);
+        if (ANY) split_any(f, p);
+        else split(f, p);
     }
 };
 
@@ -455,10 +475,16 @@ __global__ __launch_bounds__(64 * WAVES) void step_kernel(Par p, Rows r) {
         for (int i = 0; i < AHEAD; ++i) {
             if (u + i * WAVES >= end) break;
             bf16x8 part[PARTS];
-            multiply<PARTS, CPLX, 1, NT, GU>(b[i], acc, [&](int m, int ks, int h) {
-                if (h == 0) x[i].get(ks, part);
-                return part[h];
-            });
+            if (!x[i].far())
+                multiply<PARTS, CPLX, 1, NT, GU>(b[i], acc, [&](int m, int ks, int h) {
+                    if (h == 0) x[i].template get<false>(ks, part);
+                    return part[h];
+                });
+            else
+                multiply<PARTS, CPLX, 1, NT, GU>(b[i], acc, [&](int m, int ks, int h) {
+                    if (h == 0) x[i].template get<true>(ks, part);
+                    return part[h];
+                });
             if (u + (i + AHEAD) * WAVES < end) fetch(i, u + (i + AHEAD) * WAVES);
         }
     }
@@ -674,11 +700,11 @@ int run(const Plan &l, const Par &p, const Rows &r, hipStream_t stream) {
     switch (l.shape) {
     case 0:
         if constexpr (F32)
-            if (!l.lay) return launch_step<T, float, CPLX, 1, GU, 16, 1>(p, r, stream);
+            if (!l.lay) return launch_step<T, float, CPLX, 1, GU, 8, 2>(p, r, stream);
         return launch_step<T, B, CPLX, 1, GU, 8, F32 ? 2 : 3>(p, r, stream);
     case 1:
         if constexpr (F32)
-            if (!l.lay) return launch_step<T, float, CPLX, 2, GU, 16, 1>(p, r, stream);
+            if (!l.lay) return launch_step<T, float, CPLX, 2, GU, 8, 1>(p, r, stream);
         return launch_step<T, B, CPLX, 2, GU, 8, F32 ? 1 : 2>(p, r, stream);
     case 7:
         if constexpr (F32)
