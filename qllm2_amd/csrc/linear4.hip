@@ -663,12 +663,14 @@ struct Plan {
 // The shape by the number of 16 x 16 pieces of the result: as long as the GPU's 256 CUs have no more than about one
 // block each, a block of fewer pieces with more waves along the inputs is done earlier; then larger ones, which
 // read less.  Measured (us, K = 1536 real inputs, complex):
-//   bf16, group 32.  16 rows, 576 tiles: step kernel of one tile 7.7, of two 6.7.  More rows, pieces
-//     144: step 4.5, 2 x 1 pieces 5.2       288: 6.0, 5.3       576: 2 x 1 7.3, 2 x 2 6.9       1728: 2 x 2 11.1, 4 x 2 9.0
-//     9216: 4 x 2 26.3, 4 x 4 of two tiles 29       36000: 4 x 4 of two tiles 66, 8 x 4 of one 72
+//   bf16, group 32, step kernel of one, two, four tiles, and tiles of a x b pieces
+//     144 pieces: step 4.1, 4.8, 6.0; 2 x 1 5.1       288: 5.7, 4.9, 6.1; 2 x 1 5.2       576: 7.6, 6.7, 6.3; 2 x 2 6.7
+//     1152 (16 rows): 12.7, 9.6, 10.6; 4 x 2 11.4     1728 (192 rows): 16.0, 11.5, 10.7; 2 x 2 11.0, 4 x 2 8.4
+//     9216: 4 x 2 26.3, 4 x 4 of two tiles 29         36000: 4 x 4 of two tiles 66, 8 x 4 of one 72
 //   fp32, group 64: the step kernel cuts the rows itself; the others read them laid out, 2 us and a launch more
-//     192: one tile 6.6, two 7.0       432: 10.0, 7.3       864: two 10.8, four 9.2       1152: four 16.3, 4 x 2 13.3 + 2
-//     2304, 3456 (laid out): 4 x 2 22.6, 23.0, 6 x 2 18.9, 27.1, 4 x 2 of two tiles 23.4, 23.4       9216: 54.7, -, 39.6
+//     216: step 6.0, 6.3, 8.0      288: 8.9, 6.4, 8.1     576: 12.5, 10.1, 8.4     1152: 19.4, 13.7, 15.1; 4 x 2 13.4 + 2
+//     2016: 29.8, 17.8, 15.7; 6 x 2 17.5 + 2              2304: 35.1, 20.4, 21.5; 6 x 2 17.5 + 2, 4 x 2 of two tiles 21.6 + 2
+//     3456: 48.7, 27.2, 28.0; 26.5 + 2, 21.9 + 2          9216: 114, 61, 62; 48 + 2, 38 + 2
 Plan plan(const qpam_linear4_args *a) {
     const int kr = a->is_complex ? 2 * a->k : a->k, units = padded(kr) / TK, tiles = (a->n + TR - 1) / TR;
     const bool f32 = a->dtype == QPAM_F32;
@@ -685,7 +687,7 @@ Plan plan(const qpam_linear4_args *a) {
     const bool step = l.shape < 2 || l.shape == 7;
     if (step ? !near : !whole) l.lay = ((size_t)a->rows * padded(kr) * 2 * (f32 ? 3 : 1) + 255) / 256 * 256;
     // few pieces of long fp32 rows: more blocks by ranges of the inputs, joined in a launch of their own (16 rows x 4608
-    // inputs, 48 tiles: 14.8 -> 9.2 us; bf16 7.5 -> 7.0, not worth the memory)
+    // inputs, 48 tiles: 11.4 -> 7.4 us; bf16 7.5 -> 7.0, not worth the memory)
     if (f32 && l.shape == 0 && pieces <= 128 && units >= 48) {
         l.splits = pieces <= 64 ? 4 : 2, l.share = (units + l.splits - 1) / l.splits;
         l.sums = (size_t)l.splits * pieces * (a->is_complex ? 2048 : 1024);
