@@ -99,11 +99,14 @@ def _scales_of(columns, group):
 class Weight4:
     """A weight [out_features, in_features] of 4-bit codes and group scales (quantize4's),
     laid out once for the kernel on the codes' device.  With `complex` the columns are
-    2 * in_features, re and im side by side.  The codes and scales are copied."""
+    2 * in_features, re and im side by side.  The codes and scales are copied; scales
+    that are not finite: ValueError (a group of zeros times infinity would be zeros)."""
 
     def __init__(self, codes: Tensor, scales: Tensor, in_features: int, group: int = 32, complex: bool = False):
         columns = 2 * in_features if complex else in_features
         _check_codes(codes, scales, columns, group)
+        if not bool(torch.isfinite(scales).all()):
+            raise ValueError("qpam linear4: scales that are not finite")
         n = codes.shape[0]
         if n > 1 << 22 or in_features > 1 << 24:
             raise ValueError(f"qpam linear4: weight [{n}, {in_features}] too large (2^22, 2^24)")

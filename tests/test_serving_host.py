@@ -110,6 +110,14 @@ def test_weight_refusals():
         quantize4(torch.zeros(3, 4), group=16)
 
 
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_scales_that_are_not_finite_are_refused(value):
+    codes, scales = quantize4(torch.randn(4, 64))
+    scales[2, 1] = value
+    with pytest.raises(ValueError, match="finite"):
+        Weight4(codes, scales, 64)
+
+
 def test_product_refusals():
     w, c = Weight4.quantize(torch.randn(8, 32)), Weight4.quantize(torch.randn(8, 32), torch.randn(8, 32))
     with pytest.raises(ValueError, match="GPU"):
