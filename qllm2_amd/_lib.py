@@ -419,6 +419,16 @@ def stream_ptr(device=None):
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
 
 
+def launch(fn, args, dev):
+    """fn(args, the current stream of dev) with dev the current device: the two above for
+    calls of a few microseconds (0.3 us against 0.9)."""
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
+        return fn(args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(dev):
+        return fn(args, torch.cuda.current_stream(dev).cuda_stream)
+
+
 def ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
 

@@ -356,7 +356,7 @@ def copy_slots(state, src, dst, pos=None):
             raise ValueError(f"qpam copy_slots: {count} moves (at most {MAX_MOVES} in device lists)")
         pieces = [(src_t, dst_t)]
     else:
-        if any(not -1 <= s < n_slots for s in src) or any(not 0 <= d < n_slots for d in dst):
+        if count and (min(src) < -1 or max(src) >= n_slots or min(dst) < 0 or max(dst) >= n_slots):
             raise ValueError(f"qpam copy_slots: slots outside the pool of {n_slots}")
         if len(set(dst)) < count:
             raise ValueError("qpam copy_slots: a dst given twice")
@@ -367,19 +367,20 @@ def copy_slots(state, src, dst, pos=None):
             src, dst = (torch.tensor(v, dtype=torch.int32).to(state.device) for v in (src, dst))
             size = count
         pieces = [(src[i:i + size], dst[i:i + size]) for i in range(0, count, size)]
-    a = _lib.SlotsArgs()
-    a.state, a.n_slots = state.data_ptr(), n_slots
-    a.slot_bytes, a.page_bytes = 4 * max(stride[0], page), 4 * page
-    a.pos = None if pos is None else pos.data_ptr()
-    with _lib.device(state.device):
-        for s, d in pieces:
-            if torch.is_tensor(s):
-                a.host_lists, a.count, a.src, a.dst = 0, s.numel(), s.data_ptr(), d.data_ptr()
-            else:
-                ints = _lib.c_i32 * len(s)
-                s, d = ints(*s), ints(*d)
-                a.host_lists, a.count, a.src, a.dst = 1, len(s), ctypes.addressof(s), ctypes.addressof(d)
-            _lib.check(_lib.lib().qpam_copy_slots(a, _lib.stream_ptr(state.device)), "qpam_copy_slots")
+    L, dev = _lib.lib(), state.device
+    at, slot_bytes = state.data_ptr(), 4 * max(stride[0], page)
+    at_pos = None if pos is None else pos.data_ptr()
+    for s, d in pieces:
+        host = not torch.is_tensor(s)
+        if host:
+            ints = _lib.c_i32 * len(s)
+            s, d = ints(*s), ints(*d)
+            a, n = (ctypes.addressof(s), ctypes.addressof(d)), len(s)
+        else:
+            a, n = (s.data_ptr(), d.data_ptr()), s.numel()
+        status = _lib.launch(L.qpam_copy_slots, _lib.SlotsArgs(at, slot_bytes, 4 * page, n_slots, n, *a, host, at_pos), dev)
+        if status:
+            _lib.check(status, "qpam_copy_slots")
 
 
 def build_rope_cache(max_len, head_dim, device=None):

@@ -195,8 +195,7 @@ def _product(x: Tensor, codes: Tensor, scales: Tensor, n: int, k: int, group: in
     if nbytes:
         ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    with _lib.device(dev):
-        status = L.qpam_linear4(a, _lib.stream_ptr(dev))
+    status = _lib.launch(L.qpam_linear4, a, dev)
     if status:
         _lib.check(status, "qpam_linear4")
     return out
