@@ -936,9 +936,8 @@ int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void *stream);
  * complex); in a block, byte 8 l + 4 s + b of lane l = 16 q + r holds the codes of output r and
  * inputs 32 s + 8 q + 2 b (low half) and the next (high half).  scales, bf16: group 32
  * [ceil(n/16)][ceil(K/64)][16][2], group 64 [ceil(n/16)][ceil(K/64)][16], group 128
- * [ceil(n/16)][ceil(K/128)][16].  Codes and scales outside n and K are zero.  codes 16-byte,
- * scales 4-byte aligned.  n at most 2^22, k
- * 2^24. */
+ * [ceil(n/16)][ceil(K/128)][16].  Codes and scales outside n and K are zero, the scales finite;
+ * codes 16-byte, scales 4-byte aligned.  n at most 2^22, k 2^24. */
 typedef struct {
     int64_t rows;
     int32_t n, k;
