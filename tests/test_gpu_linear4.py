@@ -240,6 +240,20 @@ def test_rows_far_apart(gpu_lib, n, dtype):
         _check(linear4(x, w), x, w)
 
 
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_far_apart_in_every_shape(gpu_lib, dtype, group):
+    """The laid rows' shapes of blocks between the ones above, real and complex."""
+    K, n = 150, 40
+    x = torch.empty(n, (1 << 24) + 8, device="cuda", dtype=dtype)[:, 3:3 + K]
+    x.copy_(_rows((n, K), dtype, 62))
+    for N in (1700, 3200, 16000):
+        w = Weight4(*_codes(N, K, group, 63), K, group)
+        _check(linear4(x, w), x, w)
+        w = Weight4(*_codes(N, K, group, 64), K // 2, group, complex=True)
+        _check(complex_linear4(x.unflatten(1, (K // 2, 2)), w), x, w)
+
+
 def test_streams_and_graphs(gpu_lib):
     K, N = 256, 130
     w = Weight4(*_codes(N, 2 * K, 32, 27), K, 32, complex=True)
