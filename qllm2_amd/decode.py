@@ -418,6 +418,7 @@ class SlotPool:
                                  device=self.device, dtype=torch.float32)
         self.pos = torch.zeros(n_slots, device=self.device, dtype=torch.int32)
         self._host_pos = [0] * n_slots       # host copy of pos: the table is grown before a step needs it
+        self._exact = True                   # False: after a reorder with device lists, no less than pos
         self.rope = build_rope_cache(max_len, head_dim, device=self.device)
         self._free = list(range(n_slots - 1, -1, -1))
         self.live = set()
@@ -480,7 +481,9 @@ class SlotPool:
     def reorder(self, slots, parents):
         """Each live slot slots[i] continues from where parents[i] was (beam search, in
         place; a slot may be its own parent and several slots' parent).  Host lists, or
-        device tensors, which are not read back (then ids outside the pool do nothing)."""
+        device tensors, which are not read back (then ids outside the pool do nothing, and
+        that the others are of live slots is the caller's to see to).  The host keeps positions,
+        too: like `advance` not for a captured graph (copy_slots is)."""
         host = not (torch.is_tensor(slots) and slots.is_cuda)
         if host and not (torch.is_tensor(parents) and parents.is_cuda):
             slots, parents = ([int(i) for i in v] for v in (slots, parents))
@@ -493,6 +496,7 @@ class SlotPool:
             furthest = max((self._host_pos[s] for s in self.live), default=0)
             for s in self.live:
                 self._host_pos[s] = furthest
+            self._exact = False
 
     def compact(self):
         """The live sequences moved to the pool's lowest slots, those that are there already
@@ -525,6 +529,24 @@ class SlotPool:
         if max_pos >= self.rope.shape[0]:
             self.rope = build_rope_cache(2 * (max_pos + 1), self.head_dim, device=self.device)
 
+    def cover(self):
+        """Grow the rotary table where a live slot's position has passed its end.  After
+        reorders with device lists the host's positions may be ahead of the slots': when they
+        reach the end the slots' own are read back first (the host waits for the device).  From
+        three quarters of the table on it is grown then, as what starts there would soon be
+        read back again."""
+        if not self.live:
+            return
+        furthest = max(self._host_pos[s] for s in self.live)
+        if furthest < self.rope.shape[0]:
+            return
+        if not self._exact and not torch.cuda.is_current_stream_capturing():
+            self._host_pos, self._exact = self.pos.tolist(), True
+            furthest = max(self._host_pos[s] for s in self.live)
+            if 4 * furthest >= 3 * self.rope.shape[0]:
+                furthest = max(furthest, self.rope.shape[0])
+        self.ensure_len(furthest)
+
     def step(self, layer, q, k, v, gamma, active, rot=None, q_scale=None, out=None, compact=False):
         """One token for the listed slots on one layer: q, k, v [n_slots, heads, d, 2]
         (or planar (re, im) pairs of [n_slots, heads, d], as decode_step takes)
@@ -533,8 +555,7 @@ class SlotPool:
         the listed slots in order ([n_active, ...]).  RoPE at each slot's position; the
         table is grown first (doubling) when a live slot's position passes its end."""
         scale = self.head_dim ** -0.5 if q_scale is None else q_scale
-        if self.live:
-            self.ensure_len(max(self._host_pos[s] for s in self.live))
+        self.cover()
         return decode_step(self.layer_state(layer), q, k, v, gamma, active=active, rot=rot, q_scale=scale,
                            out=out, rope=self.rope, pos=self.pos, compact=compact)
 
@@ -544,8 +565,7 @@ class SlotPool:
         decode_step_proj takes them (gate, protect_col, phase_col,
         state_offset, qk_norm, gamma_floor)."""
         scale = self.head_dim ** -0.5 if q_scale is None else q_scale
-        if self.live:
-            self.ensure_len(max(self._host_pos[s] for s in self.live))
+        self.cover()
         return decode_step_proj(self.layer_state(layer), proj, dt_bias, active=active, q_scale=scale, out=out,
                                 rope=self.rope, pos=self.pos, compact=compact, **prologue)
 

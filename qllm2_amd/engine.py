@@ -338,8 +338,7 @@ class DecodeEngine:
             raise ValueError(f"DecodeEngine: {n} rows for {self.n_slots} slots")
         if host_slots is None:
             host_slots = slots.tolist()
-        if self.pool.live:  # grow the rotary table as SlotPool.step would, before any capture or replay
-            self.pool.ensure_len(max(self.pool._host_pos[s] for s in self.pool.live))
+        self.pool.cover()  # the rotary table as SlotPool.step would, before any capture or replay
         nb = -(-n // self.graph_bucket) * self.graph_bucket
         rope = self.pool.rope.data_ptr()
         if self._graphs and next(iter(self._graphs))[2] != rope:

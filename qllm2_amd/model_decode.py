@@ -371,8 +371,7 @@ class ModelDecoder:
             raise ValueError(f"ModelDecoder: {n} rows for {self.engine.n_slots} slots")
         if host_slots is None:
             host_slots = slots.tolist()
-        if self.pool.live:
-            self.pool.ensure_len(max(self.pool._host_pos[s] for s in self.pool.live))
+        self.pool.cover()
         nb = -(-n // self.graph_bucket) * self.graph_bucket
         rope = self.pool.rope.data_ptr()
         if self._graphs and next(iter(self._graphs))[1] != rope:
