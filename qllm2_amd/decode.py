@@ -455,6 +455,7 @@ class SlotPool:
         return slot
 
     def release(self, slot):
+        slot = int(slot)
         if slot in self.live:  # a slot released twice must not be handed out twice
             self.live.discard(slot)
             self._free.append(slot)
@@ -467,6 +468,7 @@ class SlotPool:
         """`count` more sequences that continue from where `slot` is (samples of one
         prompt, the first beams of a search): its states and position are copied to free
         slots in one launch.  Returns their ids."""
+        slot = int(slot)
         self._live([slot], "fork")
         if not 0 <= count <= len(self._free):
             raise RuntimeError(f"SlotPool: {len(self._free)} free slots, {count} asked for")

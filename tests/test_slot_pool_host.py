@@ -1,7 +1,9 @@
 """The slot pool's bookkeeping on the host (CPU): positions after reorders whose lists are on
-the device.  The copies themselves are tested on the GPU; here they are assignments, and a
-list "on the device" is one whose values the pool must not see."""
+the device, slot ids of any integer type.  The copies themselves are tested on the GPU; here
+they are assignments, and a list "on the device" is one whose values the pool must not see."""
 
+import numpy as np
+import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
@@ -96,3 +98,16 @@ def test_a_position_from_another_sequence_counts(monkeypatch):
     for _ in range(6):
         _step(pool, [near])
     assert int(pool.pos[near]) == 20 and pool.rope.shape[0] > 16
+
+
+@pytest.mark.parametrize("kind", [int, np.int64, torch.tensor])
+def test_slot_ids_of_any_integer_type(monkeypatch, kind):
+    pool = _pool(monkeypatch)
+    a = pool.acquire(5)
+    kids = pool.fork(kind(a), 2)
+    assert pool.live == {a, *kids} and [pool._host_pos[k] for k in kids] == [5, 5]
+    for s in (a, *kids):
+        pool.release(kind(s))
+    assert not pool.live and sorted(pool._free) == list(range(6)) and all(type(s) is int for s in pool._free)
+    pool.release(kind(a))   # twice: handed out once
+    assert sorted(pool._free) == list(range(6))
