@@ -16,6 +16,7 @@ entries of v and k are zero, and the padded columns of q add nothing to y).
 """
 
 import ctypes
+import operator
 
 import torch
 import torch.nn.functional as F
@@ -311,13 +312,20 @@ MAX_HOST_MOVES, MAX_MOVES = 448, 4096  # qpam_copy_slots: of one call, lists on 
 
 def _list(v, name):
     """A list of slot ids: (host list, None), or (None, int32 device tensor)."""
-    if torch.is_tensor(v) and v.is_cuda:
-        if v.dim() != 1 or v.dtype not in (torch.int32, torch.int64):
+    if torch.is_tensor(v):
+        whole = v.dtype in (torch.int32, torch.int64) if v.is_cuda else \
+            not v.numel() or not (v.is_floating_point() or v.is_complex() or v.dtype == torch.bool)
+        if v.dim() != 1 or not whole:
             raise ValueError(f"qpam copy_slots: {name} must be one list of int32 or int64, got {v.dtype} {tuple(v.shape)}")
-        if v.dtype == torch.int64:  # (what 32 bits would wrap stays outside any pool)
-            v = v.clamp(-2, 2 ** 31 - 1)
-        return None, v.to(torch.int32).contiguous()
-    return [int(i) for i in (v.tolist() if torch.is_tensor(v) else v)], None
+        if v.is_cuda:
+            if v.dtype == torch.int64:  # (what 32 bits would wrap stays outside any pool)
+                v = v.clamp(-2, 2 ** 31 - 1)
+            return None, v.to(torch.int32).contiguous()
+        v = v.tolist()
+    try:
+        return [operator.index(i) for i in v], None   # (int() would cut a 1.5 to slot 1)
+    except TypeError:
+        raise ValueError(f"qpam copy_slots: {name} must be one list of integers") from None
 
 
 def copy_slots(state, src, dst, pos=None):
@@ -488,7 +496,7 @@ class SlotPool:
         too: like `advance` not for a captured graph (copy_slots is)."""
         host = not (torch.is_tensor(slots) and slots.is_cuda)
         if host and not (torch.is_tensor(parents) and parents.is_cuda):
-            slots, parents = ([int(i) for i in v] for v in (slots, parents))
+            slots, parents = _list(slots, "slots")[0], _list(parents, "parents")[0]
             self._live(slots + parents, "reorder")
         copy_slots(self.state, parents, slots, pos=self.pos)
         if host:
@@ -516,7 +524,7 @@ class SlotPool:
     def clear(self, slots):
         """The listed live slots' states emptied and their positions set to 0, in one launch
         (host ids)."""
-        slots = [int(s) for s in slots]
+        slots = _list(slots, "slots")[0]
         self._live(slots, "clear")
         copy_slots(self.state, [-1] * len(slots), slots, pos=self.pos)
         for s in slots:

@@ -111,3 +111,34 @@ def test_slot_ids_of_any_integer_type(monkeypatch, kind):
     assert not pool.live and sorted(pool._free) == list(range(6)) and all(type(s) is int for s in pool._free)
     pool.release(kind(a))   # twice: handed out once
     assert sorted(pool._free) == list(range(6))
+
+
+@pytest.mark.parametrize("ids", [[1.5, 2], torch.tensor([1.0, 2.0]), torch.tensor([[1, 2]]), [[1], [2]], torch.tensor(1),
+                                 torch.tensor([True, False])])
+def test_lists_that_are_no_ids_are_refused(ids):
+    """Not cut to integers: a slot of 1.5 would be slot 1."""
+    with FakeTensorMode():
+        state = torch.empty(4, 8, device="cuda")
+    for src, dst in ((ids, [0, 3]), ([0, 3], ids)):
+        with pytest.raises(ValueError, match="must be one list"):
+            decode.copy_slots(state, src, dst)
+
+
+def test_pool_calls_refuse_lists_that_are_no_ids(monkeypatch):
+    pool = _pool(monkeypatch)
+    a, b = pool.acquire(), pool.acquire()
+    for call in (lambda: pool.reorder([a, b], [0.5, 1]), lambda: pool.reorder(torch.tensor([0.0, 1.0]), [a, b]),
+                 lambda: pool.clear([0.5])):
+        with pytest.raises(ValueError, match="must be one list"):
+            call()
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int16, torch.int32, torch.int64])
+def test_host_tensors_of_any_integer_type(monkeypatch, dtype):
+    pool = _pool(monkeypatch)
+    a, b = pool.acquire(3), pool.acquire(5)
+    pool.reorder(torch.tensor([a, b], dtype=dtype), torch.tensor([b, a], dtype=dtype))
+    assert pool._host_pos[a] == 5 and pool._host_pos[b] == 3
+    pool.reorder(torch.tensor([]), [])
+    pool.clear(torch.tensor([a], dtype=dtype))
+    assert pool.pos[[a, b]].tolist() == [0, 3]
