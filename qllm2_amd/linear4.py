@@ -16,6 +16,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib, _ops
 
@@ -215,11 +216,14 @@ def _refuse_gradients(x, bias, tail):
     if (x.requires_grad or (bias is not None and bias.requires_grad) or (tail is not None and tail.requires_grad)) \
             and torch.is_grad_enabled():
         raise ValueError("qpam linear4: products with 4-bit weights have no gradient (call under torch.no_grad())")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in (x, bias, tail)):
+        raise ValueError("qpam linear4: products with 4-bit weights have no gradient, in forward mode neither")
 
 
 def linear4(x: Tensor, weight: Weight4, bias: Optional[Tensor] = None) -> Tensor:
     """x [..., in] times a real Weight4: [..., out] in x's dtype (float32 or bfloat16, any
-    strides; fp32 sums, one rounding).  bias [out].  No gradient."""
+    strides; fp32 sums, one rounding).  bias [out].  No gradient, in either mode (ValueError)."""
     if weight.complex:
         raise ValueError("qpam linear4: a complex weight (complex_linear4)")
     _refuse_gradients(x, bias, None)
