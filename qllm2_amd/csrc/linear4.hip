@@ -741,6 +741,7 @@ int by_group(const Plan &l, const Par &p, const Rows &r, int cplx, int group, hi
 }  // namespace qpam
 
 extern "C" size_t qpam_linear4_workspace_size(const qpam_linear4_args *a) {
+    if (!a) return 0;
     const int64_t k = a->is_complex ? 2 * (int64_t)a->k : a->k;
     if (a->rows < 1 || a->rows > (1L << 40) || k < 1 || k > (1 << 25) || a->n < 1 || a->n > (1 << 22)) return 0;
     const qpam::w4::Plan l = qpam::w4::plan(a);

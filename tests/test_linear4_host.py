@@ -1,10 +1,14 @@
-"""CPU checks of the 4-bit products: gradients in either mode are refused."""
+"""CPU checks of the 4-bit products: gradients in either mode are refused; the entries' arguments."""
+
+import subprocess
+import sys
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from qllm2_amd.linear4 import Weight4, complex_linear4, linear4
+from tests.conftest import ROOT
 
 
 def _calls():
@@ -37,3 +41,11 @@ def test_reverse_mode_gradients_are_refused(call, shape):
         torch.func.grad(lambda t: call(t).sum())(torch.randn(shape))
     with pytest.raises(ValueError, match="no gradient"):
         torch.func.vmap(torch.func.grad(lambda t: call(t).sum()))(torch.randn(3, *shape))
+
+
+def test_entries_take_null_arguments():
+    """No bytes and an error (in a process of its own: reading them ended it)."""
+    code = ("from qllm2_amd import _lib; L = _lib.lib(); "
+            "assert L.qpam_linear4_workspace_size(None) == 0 and L.qpam_linear4(None, None) == _lib.QPAM_ERR_ARG; "
+            "assert L.qpam_copy_slots(None, None) == _lib.QPAM_ERR_ARG")
+    assert subprocess.run([sys.executable, "-c", code], cwd=ROOT, timeout=300).returncode == 0
