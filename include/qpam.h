@@ -925,8 +925,9 @@ int qpam_linear_logprobs_bwd(const qpam_linear_logprobs_args *a, void *stream);
  * e: 4-bit floats (bit 3 the sign; 0, 0.5, 1, 1.5, 2, 3, 4, 6 by bits 0 to 2), s bf16, group
  * 32, 64 or 128.  x [rows][k] and y [rows][n] in dtype (row strides ldx, ldy elements, any
  * alignment of the type).  fp32 sums of exact products (fp32 rows: of three bf16 parts, exact),
- * rounded once.  A group's sum of x e must be finite before its scale (|x| below 2^120); of an
- * fp32 value, what is below 2^-126 in its second and third part counts as zero.
+ * rounded once.  The sum of x e over a group (64 inputs of a group of 128) must be finite before its
+ * scale (|x| below 2^119: 64 x 6 of them); an fp32 value below 2^-110 counts as its nearest
+ * multiple of 2^-133 (bf16's smallest step).
  * is_complex: x [rows][k][2], y [rows][n][2], weights and bias complex; the codes and scales
  * are those of rows of 2k real values, (re, im) side by side (v11/complex_ops.py:165-172:
  * re = Wr xr - Wi xi, im = Wi xr + Wr xi).  planes 1: y's row is the n real parts, the n

@@ -8,8 +8,9 @@ here a complex weight is two neighbouring codes, read once.  A code is a 4-bit f
 (sign, 2 bits of exponent, 1 of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6), `group`
 neighbouring codes of an output's row share a bf16 scale.  The products are exact and
 summed in fp32; nothing but the result is rounded to the rows' dtype.  (A group's sum is
-formed before its scale: rows of magnitudes below 2^120.  fp32 rows are cut into three bf16
-parts; of values below 2^-108 the parts under 2^-126 count as zero.)
+formed before its scale, of up to 64 inputs at once: rows of magnitudes below 2^119.  fp32
+rows are cut into three bf16 parts: a value below 2^-110 counts as its nearest multiple of
+2^-133, bf16's smallest step.)
 """
 
 from typing import Optional

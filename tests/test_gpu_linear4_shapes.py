@@ -108,6 +108,38 @@ def test_the_largest_values(gpu_lib, n, N, lo, hi):
             assert torch.equal(_product(x, w), _one_product(x, at, w))
 
 
+@pytest.mark.parametrize("cplx", [False, True])
+@pytest.mark.parametrize("n,N", [(5, 200), (16, 4100), (16, 16500), (520, 1100), (700, 1900)])
+def test_the_smallest_values(gpu_lib, n, N, cplx):
+    """Exact from 2^-110 on, where the third part's last bit is bf16's smallest step of 2^-133; below it the nearest
+    multiple of that, subnormal parts among them."""
+    K = 200
+    w = _powers(N, K, 32, cplx, 40, 60)
+    x, at = _one_a_row(_bits(n, -110, -100, 21), K, F32)
+    assert torch.equal(_product(x, w), _one_product(x, at, w))
+    x, at = _one_a_row(_bits(n, -126, -110, 22), K, F32)
+    near = (torch.round(x.double() * 2.0 ** 133) * 2.0 ** -133).to(F32)   # (24 bits at most: exact)
+    assert torch.equal(_product(x, w), _one_product(near, at, w)) and (near != x).any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cplx", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,N", [(5, 40), (40, 1500), (520, 1100)])
+def test_whole_groups_of_the_largest_magnitude(gpu_lib, n, N, group, cplx, dtype):
+    """Rows just below 2^119 and weights of 6, all of one sign, under small scales: a group's sum is finite."""
+    K = 256
+    codes = torch.full((N, K // 2), 0xF7 if cplx else 0x77, device="cuda", dtype=torch.uint8)   # 6 and -6, or 6
+    scales = torch.full((N, K // group), 2.0 ** -60, device="cuda", dtype=BF16)
+    w = Weight4(codes, scales, K // 2 if cplx else K, group, complex=cplx)
+    largest = torch.tensor((2 - 2.0 ** -(23 if dtype == F32 else 7)) * 2.0 ** 118, device="cuda", dtype=dtype)
+    x = largest.expand(n, K).contiguous()
+    y = _product(x, w)
+    assert torch.isfinite(y).all()
+    z = x.unflatten(1, (-1, 2)) if cplx else x
+    _check(y.unflatten(1, (-1, 2)) if cplx else y, z, w)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("cplx", [False, True])
 @pytest.mark.parametrize("K", INPUTS)
