@@ -30,7 +30,8 @@ captured once per live-count bucket and replayed.
 
 With weight_bits=4 every ComplexLinear is a product with 4-bit weights (linear4), with
 table_bits=4 the logits' table too; prompts and scores run on the values that the codes
-stand for, so a sequence meets one model throughout.
+stand for (a prompt's PAM layers hold them in the model's dtype), so a sequence meets one
+model throughout.
 
 fork gives a sequence's slot to further samples of it, reorder lets the beams of a search
 continue from each other, compact moves the live sequences together.
@@ -58,9 +59,10 @@ from . import triton_kernels as tk
 from .embedding import complex_embedding
 from .engine import DecodeEngine, check_weight_bits, complex_product, complex_weight4, quantized_layer
 from .linear4 import Weight4, linear4
-from .token_logprobs import linear_token_logprobs, token_logprobs
+from .token_logprobs import TokenLogprobs, linear_token_logprobs, token_logprobs
 
 MAX_DIM = 2048  # qpam_resid_norm: a thread per four complex columns, 512 per row
+SCORE_LOGITS = 2 ** 26  # fp32 logits that score holds at once where the table is in 4 bits (256 MB)
 
 
 def _code(t):
@@ -186,11 +188,10 @@ class ModelDecoder:
             e = torch.stack([m.embed.embed_real.weight, m.embed.embed_imag.weight], -1).float()  # [V, dim, 2]
             self.vocab, self.dim = e.shape[0], e.shape[1]
             self._embed = e.contiguous().unbind(-1)                                               # fp32, lookups
-            table, self._table4 = e.reshape(self.vocab, 2 * self.dim), None
-            if self.table_bits == 4:
-                self._table4 = Weight4.quantize(table, group=self.weight_group)
-                table = self._table4.dequantize()                                             # score's products
-            self._embed_w = table.to(dt).contiguous()                                         # logits GEMM, fp32: the same memory
+            table = e.reshape(self.vocab, 2 * self.dim)
+            # the logits' table: codes, or the GEMM's (in fp32 the lookups' memory)
+            self._table4 = Weight4.quantize(table, group=self.weight_group) if self.table_bits == 4 else None
+            self._embed_w = table.to(dt).contiguous() if self._table4 is None else None
             # prompts on the values that the codes stand for
             self._prompt_layers = [quantized_layer(b.pam, self.weight_group) if self.weight_bits == 4 else b.pam
                                    for b in self.blocks]
@@ -264,6 +265,16 @@ class ModelDecoder:
         logits = F.linear(lm, self._embed_w) if self._table4 is None else linear4(lm, self._table4)   # [n, V]
         return logits if logits.dtype == torch.float32 else logits.float()
 
+    def _scores(self, lm, ids, temperature):
+        """TokenLogprobs of the LM head's rows lm [n, 2 dim] for the tokens ids [n]."""
+        if self._table4 is None:
+            return linear_token_logprobs(lm, self._embed_w, ids, temperature=temperature)
+        # fp32 logits of the codes' exact products (bf16 rows as fp32 ones), some rows' at a time
+        rows = max(1, SCORE_LOGITS // self.vocab)
+        parts = [token_logprobs(linear4(x.float(), self._table4), i, temperature=temperature)
+                 for x, i in zip(lm.split(rows), ids.split(rows))]
+        return TokenLogprobs(torch.cat([p.logprobs for p in parts]), torch.cat([p.entropy for p in parts]))
+
     def _next_norm(self, li):
         """The norm after block li's PAM residual (li = -1: after the embedding norm)."""
         return self._blk[li + 1]["norm1"] if li + 1 < len(self._blk) else self._norm_o
@@ -317,13 +328,15 @@ class ModelDecoder:
     def score(self, ids, temperature=1.0):
         """Of one sequence ids [T], T >= 2: for each token after the first, the log
         probability the model gives it after those before it, and the entropy of that
-        choice, fp32 [T - 1] each; no logits in memory.  Ids outside the vocabulary:
-        ValueError for a host tensor; in one on the device they and what follows score NaN."""
+        choice, fp32 [T - 1] each; no logits in memory (with table_bits=4 SCORE_LOGITS of them
+        at a time).  Ids outside the vocabulary:
+        ValueError for a host tensor; in one on the device they and what follows score NaN (and
+        up to 15 tokens before one, which share a tile of the prompt's scan with it)."""
         ids, on_device = self._prompt_ids(ids), ids.is_cuda
         if ids.numel() < 2:
             raise ValueError("ModelDecoder.score: at least two tokens")
         h, _ = self._prompt_rows(ids)
-        r = linear_token_logprobs(self._lm_rows(h[:-1]), self._embed_w, ids[1:], temperature=temperature)
+        r = self._scores(self._lm_rows(h[:-1]), ids[1:], temperature)
         if on_device:  # a row without a token would have log probability 0
             r = r._replace(logprobs=r.logprobs.masked_fill((ids[1:] < 0) | (ids[1:] >= self.vocab), float("nan")))
         return r
