@@ -662,15 +662,34 @@ struct Plan {
 
 // The shape by the number of 16 x 16 pieces of the result: as long as the GPU's 256 CUs have no more than about one
 // block each, a block of fewer pieces with more waves along the inputs is done earlier; then larger ones, which
-// read less.  Measured (us, K = 1536 real inputs, complex):
-//   bf16, group 32, step kernel of one, two, four tiles, and tiles of a x b pieces
-//     144 pieces: step 4.1, 4.8, 6.0; 2 x 1 5.1       288: 5.7, 4.9, 6.1; 2 x 1 5.2       576: 7.6, 6.7, 6.3; 2 x 2 6.7
-//     1152 (16 rows): 12.7, 9.6, 10.6; 4 x 2 11.4     1728 (192 rows): 16.0, 11.5, 10.7; 2 x 2 11.0, 4 x 2 8.4
-//     9216: 4 x 2 26.3, 4 x 4 of two tiles 29         36000: 4 x 4 of two tiles 66, 8 x 4 of one 72
-//   fp32, group 64: the step kernel cuts the rows itself; the others read them laid out, 2 us and a launch more
-//     216: step 6.0, 6.3, 8.0      288: 8.9, 6.4, 8.1     576: 12.5, 10.1, 8.4     1152: 19.4, 13.7, 15.1; 4 x 2 13.4 + 2
-//     2016: 29.8, 17.8, 15.7; 6 x 2 17.5 + 2              2304: 35.1, 20.4, 21.5; 6 x 2 17.5 + 2, 4 x 2 of two tiles 21.6 + 2
-//     3456: 48.7, 27.2, 28.0; 26.5 + 2, 21.9 + 2          9216: 114, 61, 62; 48 + 2, 38 + 2
+// read less.  Shapes 0, 1 and 7: the step kernel of one, two and four tiles; 2 to 6: tiles in LDS (run below).
+// Measured (us in a graph, 1536 real inputs, complex / real weights; in brackets the rule's):
+//   bf16, group 32           0            1            7            2          3            4            5
+//   1 row, 144 pieces    [3.3 / 3.0]   4.0 / 3.4    5.4 / 4.2
+//   1 row, 288            3.9 / 3.5   [4.1 / 3.5]   5.5 / 4.3
+//   1 row, 1152           7.2 / 6.0    7.6 / 5.8   [9.5 / 6.8]
+//   16 rows, 576          7.8 / 7.5   [6.9 / 6.5]   6.5 / 5.6
+//   16 rows, 1152        12.7 / 12.6   9.7 / 8.7  [10.8 / 8.2]
+//   192 rows, 288         5.9 / 5.8    5.1 / 4.7    6.4 / 5.4   [5.4 / 5.1]   6.9 / 6.8    8.2 / 7.3
+//   192 rows, 576         7.7 / 7.5    6.8 / 6.4    6.6 / 5.4    7.3 / 7.1   [7.0 / 6.8]   8.3 / 7.4
+//   192 rows, 1728       16.2 / 14.1  11.9 / 10.5  11.1 / 7.8   12.8 / 12.0  11.2 / 10.9  [8.6 / 7.6]  20.8 / 22.3
+//   512 rows, 4608         34 / 34    23.0 / 21.8  23.4 / 15.8  26.2 / 26.1  23.7 / 23.4 [17.0]/ 15.8  21.2 /[22.6]
+//   512 rows, 9216                                                                       [27.8]/ 26.0  25.1 /[23.5]
+//   2000 rows, 36000                                                                       99 / 84    [69 / 48]
+//   fp32, group 64: the step kernel cuts the rows itself; the others read them laid out by a launch more, counted here
+//                            0            1            7            5            6
+//   16 rows, 144 pieces  [5.8 / 5.7]   6.3 / 5.9    8.0 / 6.5
+//   16 rows, 288          9.0 / 8.7   [6.5 / 6.1]   8.3 / 6.7
+//   16 rows, 1152        19.5 / 21.8  14.4 / 12.9 [15.7 / 11.7]
+//   192 rows, 1728       26.2 / 28.6  17.8 / 16.1 [15.6 / 11.1] 22.7 / 26.6   26.4
+//   192 rows, 2304       33.8 / 35.0  20.4 / 19.2  21.7 / 14.4 [22.9 / 26.9]  26.4
+//   512 rows, 4608         58 / 61    33.7 / 32.4  35.3 / 22.4  34.9 /[31.3] [32.0]
+//   512 rows, 9216                                 61.6 / 37.5  56.9 /[36.5] [47.0]
+//   2000 rows, 36000                                248 / 149    186 /[112]  [162]
+// The limits were set on complex weights and are the same for 1 and 16 rows; what they cost elsewhere: up to a quarter
+// where a step shape is ahead (1152 pieces of a few rows, 288 and 576 of more, real bf16 ones up to some 5000), half the
+// time of real fp32 products from 2048 to some 6000 pieces.  fp32 shapes 2, 3 and 4 and the step kernels of laid fp32
+// rows are of rows more than 2^24 elements apart alone.
 Plan plan(const qpam_linear4_args *a) {
     const int kr = a->is_complex ? 2 * a->k : a->k, units = padded(kr) / TK, tiles = (a->n + TR - 1) / TR;
     const bool f32 = a->dtype == QPAM_F32;
